@@ -557,7 +557,7 @@ class DecodeEngine:
         n0 = self._lib.launch_count()
         self._gemm_events = gemm_events
         try:
-            with torch.cuda.graph(g):
+            with self._lib.graph_capture(g):
                 for t in range(n_steps):
                     self._decode_step(min(start_len + t + 1, self.S), out[t], events)
         finally:
