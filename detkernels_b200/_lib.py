@@ -6,7 +6,9 @@ device memory, the current stream and tensor metadata.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import gc
 import os
 import threading
 
@@ -27,6 +29,7 @@ DK_BF16 = 2
 
 MATMUL_K_SLICES = 8
 ATTN_KV_SPLIT = 256
+WORKSPACE_COUNTER_BYTES = 1 << 20
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -88,6 +91,20 @@ SIGNATURES = {
     "dk_attention_batch_variant": (_int, [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p,
                                           _i64, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _int, _c_void_p, _size,
                                           _c_void_p]),
+    "dk_paged_plan_workspace_size": (_size, [_i64]),
+    "dk_paged_plan": (_int, [_c_void_p, _i64, _i32, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i64, _c_void_p,
+                             _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i32,
+                             _i64, _c_void_p, _size, _c_void_p]),
+    "dk_qk_norm_rope": (_int, [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64,
+                               _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64,
+                               _c_void_p, _c_void_p, _int, _c_void_p, _c_void_p, _int, _c_void_p, _i64, _i64, _i32,
+                               _i32, _i32, _i32, _int, _f32, _int, _c_void_p]),
+    "dk_attention_prefix_state_size": (_size, [_i64, _i32, _i32, _i32, _i64]),
+    "dk_attention_shared_prefix": (_int, [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i32,
+                                          _c_void_p, _i64, _i32, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64,
+                                          _c_void_p, _i64, _i32, _i64, _i32, _c_void_p, _i64, _i64, _c_void_p,
+                                          _c_void_p, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _int, _c_void_p, _size,
+                                          _c_void_p, _size, _c_void_p]),
 }
 
 
@@ -262,6 +279,37 @@ def workspace(nbytes: int, device, stream: int):
             buf = torch.zeros(size, dtype=torch.uint8, device=dev)
             _workspaces[key] = buf
         return buf
+
+
+def call_workspace(nbytes: int, device, stream: int):
+    """``workspace`` for a call that may be captured: while the stream is being captured the scratch
+    belongs to the graph (allocated and its counters zeroed inside it), so that no two graphs share
+    one and none outlives the buffer it was captured with."""
+    import torch
+    if nbytes <= 0:
+        return None
+    if not torch.cuda.is_current_stream_capturing():
+        return workspace(nbytes, device, stream)
+    buf = torch.empty(int(nbytes), dtype=torch.uint8, device=device)
+    buf[:WORKSPACE_COUNTER_BYTES].zero_()
+    return buf
+
+
+@contextlib.contextmanager
+def graph_capture(graph):
+    """``torch.cuda.graph(graph)`` with Python's cyclic collector held off: a model and its engines refer
+    to each other, and a dead engine's graphs, destroyed by the collector in the middle of another
+    capture, would invalidate that capture."""
+    import torch
+    gc.collect()
+    held = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph):
+            yield
+    finally:
+        if held:
+            gc.enable()
 
 
 def reset_workspaces(device=None) -> None:

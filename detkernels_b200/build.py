@@ -2,8 +2,8 @@
 
     python -m detkernels_b200.build          # -> detkernels_b200/libdetkernels_b200.so
 
-The library is a single CUDA translation unit (csrc/dk_lib.cu) compiled with
-nvcc for `sm_100a` only.  It links the CUDA runtime statically and reaches the
+The library is three CUDA translation units (csrc/*.cu), compiled side by side
+with nvcc for `sm_100a` only.  It links the CUDA runtime statically and reaches the
 driver API (tensor-map encoding) through cudaGetDriverEntryPointByVersion, so
 the .so loads on a machine without a GPU driver (symbol checks, CPU tests).
 """
@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
@@ -25,7 +26,7 @@ STAMP_PATH = LIB_PATH + ".srchash"
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
     "--expt-relaxed-constexpr",
 ]
 
@@ -63,18 +64,29 @@ def is_up_to_date() -> bool:
         return f.read().strip() == source_hash()
 
 
+def _run(cmds, verbose):
+    """Run commands side by side; raises with their output if one fails."""
+    procs = []
+    for cmd in cmds:
+        if verbose:
+            print("[detkernels_b200] " + " ".join(cmd), flush=True)
+        procs.append(subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))
+    outs = [p.communicate()[0] for p in procs]
+    if any(p.returncode for p in procs):
+        sys.stderr.write("".join(o for p, o in zip(procs, outs) if p.returncode))
+        raise RuntimeError("nvcc failed building %s" % LIB_NAME)
+
+
 def build(force: bool = False, verbose: bool = True) -> str:
-    """Compile csrc/dk_lib.cu into LIB_PATH unless it is already current."""
+    """Compile csrc/*.cu into LIB_PATH unless it is already current."""
     if not force and is_up_to_date():
         return LIB_PATH
     tmp = LIB_PATH + ".tmp"
-    cmd = [nvcc_path(), *NVCC_FLAGS, "-I", INCLUDE, "-o", tmp, os.path.join(CSRC, "dk_lib.cu")]
-    if verbose:
-        print("[detkernels_b200] " + " ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError("nvcc failed building %s" % LIB_NAME)
+    units = [os.path.join(CSRC, name) for name in sorted(os.listdir(CSRC)) if name.endswith(".cu")]
+    with tempfile.TemporaryDirectory() as obj_dir:
+        objs = [os.path.join(obj_dir, os.path.basename(u) + ".o") for u in units]
+        _run([[nvcc_path(), *NVCC_FLAGS, "-I", INCLUDE, "-c", "-o", o, u] for u, o in zip(units, objs)], verbose)
+        _run([[nvcc_path(), *NVCC_FLAGS, "-shared", "-o", tmp, *objs]], verbose)
     os.replace(tmp, LIB_PATH)
     with open(STAMP_PATH, "w") as f:
         f.write(source_hash())

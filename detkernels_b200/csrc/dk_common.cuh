@@ -26,10 +26,11 @@
 namespace dk {
 
 // ---------------------------------------------------------------------------
-// Device status word (one per device, per loaded library image).
+// Device status word (one per device and translation unit of the library; dk_device_status reads
+// and clears them all).
 // ---------------------------------------------------------------------------
-__device__ int g_status_code;    // 0 = ok, else a DK_ERR_* code (first error wins)
-__device__ int g_status_detail;  // kernel-specific detail for the first error
+static __device__ int g_status_code;    // 0 = ok, else a DK_ERR_* code (first error wins)
+static __device__ int g_status_detail;  // kernel-specific detail for the first error
 
 // Wall-clock limit for any single wait inside a kernel.  A healthy wait on
 // this library's barriers completes in microseconds.
@@ -170,7 +171,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int de
 // returns normally; otherwise the wait completes and the status stays clean.
 constexpr int kSelfTestDetail = 0x7E57;
 
-__global__ void __launch_bounds__(64) bounded_wait_selftest_kernel(int skip_arrive, unsigned long long limit_ns) {
+static __global__ void __launch_bounds__(64) bounded_wait_selftest_kernel(int skip_arrive, unsigned long long limit_ns) {
   __shared__ __align__(8) uint64_t bar;
   if (threadIdx.x == 0) {
     mbar_init(&bar, 1);

@@ -1,0 +1,347 @@
+// Per-head RMSNorm of queries and keys with the position rotation in the same pass, K and V stored
+// into a KV cache.
+//
+//   y = x * rsqrt(mean(x^2) + eps) * w              (one head vector x of D elements, f32)
+//   (a, b) -> (a cos - b sin, a sin + b cos)        for each pair of the first rd elements of y
+//
+// with pairs (i, i + rd / 2), or (2i, 2i + 1) when interleaved, and cos/sin of the row's position
+// from an f32 table.  Everything stays in f32 until the one rounding of the store.  The sum of
+// squares of a vector has a fixed order (a lane's elements in order, then a butterfly), so a row's
+// bits do not depend on the other rows.
+//
+// Memory bound: every vector is read and written once.  A group of lanes owns a vector in 16-byte
+// chunks, lane l holding chunks l, l + L, l + 2L, ... with L = rd / 2 in chunks, so both elements of
+// a pair sit in one lane; the row's cos/sin stay in registers over the vectors a group walks.
+#pragma once
+
+#include "dk_common.cuh"
+
+namespace dk {
+namespace rope {
+
+constexpr int kThreads = 256;
+constexpr int kMaxDim = 512;
+
+enum : int {
+  kDetPos = 0x610,    // a position outside the table
+  kDetSlot = 0x611,   // a slot outside the cache
+};
+
+struct Params {
+  const void *q, *k, *v;                 // [T, H | Hkv, D]; v null: no cache
+  int64_t q_sr, q_sh, k_sr, k_sh, v_sr, v_sh;
+  void *qo, *ko;                         // ko null: K goes to the cache only
+  int64_t qo_sr, qo_sh, ko_sr, ko_sh;
+  void *kc, *vc;                         // cache [n_slabs, Hkv, cap, D]
+  int64_t c_sn, c_sh, c_st;
+  int64_t cap, n_slabs;
+  const int64_t* slots;
+  const void* pos;                       // int32 or int64 [T]
+  int pos64;
+  const void *qw, *kw;
+  int wdtype;
+  const float* table;                    // [max_pos, rd]: cos then sin
+  int64_t max_pos;
+  int64_t n_rows;
+  int H, Hkv, D, rd, interleaved;
+  float eps;
+  int nvec;                              // vectors a row: H + Hkv (+ Hkv with a cache)
+  int lanes;                             // vector path: lanes that hold chunks (L)
+  int glog;                              // log2 of the group's lane count
+  int vpu;                               // vectors a warp walks (a multiple of the groups in it)
+  int upr;                               // warps a row
+};
+
+template <typename T>
+struct Chunk {
+  static constexpr int N = 16 / sizeof(T);
+};
+
+__device__ __forceinline__ float load_w(const void* w, int dtype, int i) {
+  if (dtype == DK_F32) return static_cast<const float*>(w)[i];
+  if (dtype == DK_F16) return __half2float(static_cast<const __half*>(w)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
+}
+
+// A row's position and cache place; false when the position is outside the table.
+struct Row {
+  int64_t pos;
+  int64_t cache;      // element offset of the row's token in head 0 of the cache, -1: not stored
+};
+__device__ __forceinline__ bool describe_row(const Params& p, int64_t t, bool report, Row& r) {
+  r.pos = p.pos64 ? static_cast<const int64_t*>(p.pos)[t] : static_cast<const int32_t*>(p.pos)[t];
+  r.cache = -1;
+  if (r.pos < 0 || r.pos >= p.max_pos) {
+    if (report) report_error(DK_ERR_DEVICE_CHECK, kDetPos);
+    return false;
+  }
+  if (p.slots) {
+    const int64_t s = p.slots[t];
+    if (s >= 0) {
+      const bool narrow = s <= 0xffffffffLL && p.cap <= 0xffffffffLL;
+      const int64_t n = narrow ? static_cast<int64_t>(static_cast<uint32_t>(s) / static_cast<uint32_t>(p.cap)) : s / p.cap;
+      if (n >= p.n_slabs) {
+        if (report) report_error(DK_ERR_DEVICE_CHECK, kDetSlot);
+      } else {
+        r.cache = n * p.c_sn + (s - n * p.cap) * p.c_st;
+      }
+    }
+  }
+  return true;
+}
+
+// Where vector i of row t comes from and goes to (q heads, then k heads, then v heads).
+template <typename T>
+struct Place {
+  const T* src;
+  T* dst;       // null: nowhere
+  T* dst2;      // a key's second destination (k_out beside the cache)
+  int kind;     // 0 q, 1 k, 2 v
+};
+template <typename T>
+__device__ __forceinline__ Place<T> place(const Params& p, const Row& row, int64_t t, int i) {
+  Place<T> o;
+  o.dst2 = nullptr;
+  if (i < p.H) {
+    o.kind = 0;
+    o.src = static_cast<const T*>(p.q) + t * p.q_sr + i * p.q_sh;
+    o.dst = static_cast<T*>(p.qo) + t * p.qo_sr + i * p.qo_sh;
+  } else if (i < p.H + p.Hkv) {
+    const int h = i - p.H;
+    o.kind = 1;
+    o.src = static_cast<const T*>(p.k) + t * p.k_sr + h * p.k_sh;
+    o.dst = p.ko ? static_cast<T*>(p.ko) + t * p.ko_sr + h * p.ko_sh : nullptr;
+    if (row.cache >= 0) o.dst2 = static_cast<T*>(p.kc) + row.cache + h * p.c_sh;
+  } else {
+    const int h = i - p.H - p.Hkv;
+    o.kind = 2;
+    o.src = static_cast<const T*>(p.v) + t * p.v_sr + h * p.v_sh;
+    o.dst = row.cache >= 0 ? static_cast<T*>(p.vc) + row.cache + h * p.c_sh : nullptr;
+  }
+  return o;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& c, float* x);
+template <>
+__device__ __forceinline__ void unpack<float>(const uint4& c, float* x) {
+  x[0] = __uint_as_float(c.x);
+  x[1] = __uint_as_float(c.y);
+  x[2] = __uint_as_float(c.z);
+  x[3] = __uint_as_float(c.w);
+}
+template <>
+__device__ __forceinline__ void unpack<__nv_bfloat16>(const uint4& c, float* x) {
+  const uint32_t u[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(u[i] << 16);
+    x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+  }
+}
+template <>
+__device__ __forceinline__ void unpack<__half>(const uint4& c, float* x) {
+  const uint32_t u[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack(const float* x);
+template <>
+__device__ __forceinline__ uint4 pack<float>(const float* x) {
+  return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+}
+template <>
+__device__ __forceinline__ uint4 pack<__nv_bfloat16>(const float* x) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    u[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+template <>
+__device__ __forceinline__ uint4 pack<__half>(const float* x) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+    u[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+// Vector path.  NC: chunks a lane holds (chunk l + j L, j < NC).  Rotated chunks: 0 and 1 (pairs
+// between them) or, interleaved, those with index < rd / N (pairs inside a chunk).
+template <typename T, int NC, bool INTER>
+__global__ void __launch_bounds__(kThreads) vec_kernel(const Params p) {
+  constexpr int N = Chunk<T>::N;
+  constexpr int UB = NC <= 2 ? 4 : 2;   // vectors in flight per group
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int64_t t = unit / p.upr;
+  if (t >= p.n_rows) return;
+  const int part = static_cast<int>(unit - t * p.upr);
+  const int gl = 1 << p.glog, gpw = 32 >> p.glog;
+  const int l = lane & (gl - 1), gi = lane >> p.glog;
+  const bool on = l < p.lanes;
+  Row row;
+  if (!describe_row(p, t, lane == 0 && part == 0, row)) return;
+  // this lane's angles: pairs of chunk 0 with chunk 1 share index i in [l N, l N + N); interleaved,
+  // chunk j's pairs are i = (l + j L) N / 2 + [0, N / 2)
+  const float* cs = p.table + row.pos * p.rd;
+  const int half = p.rd >> 1;
+  float co[INTER ? NC * N / 2 : N], si[INTER ? NC * N / 2 : N];
+  if (on) {
+    if constexpr (INTER) {
+#pragma unroll
+      for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          const int pi = (l + j * p.lanes) * (N / 2) + i;
+          co[j * (N / 2) + i] = pi < half ? cs[pi] : 1.0f;
+          si[j * (N / 2) + i] = pi < half ? cs[half + pi] : 0.0f;
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        co[i] = cs[l * N + i];
+        si[i] = cs[half + l * N + i];
+      }
+    }
+  }
+  const int end = min(p.nvec, (part + 1) * p.vpu);
+  for (int i0 = part * p.vpu + gi; i0 - gi < end; i0 += UB * gpw) {
+    Place<T> pl[UB];
+    uint4 c[UB][NC];
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      const int i = i0 + u * gpw;
+      if (i < end) {
+        pl[u] = place<T>(p, row, t, i);
+        if (on) {
+#pragma unroll
+          for (int j = 0; j < NC; ++j)
+            c[u][j] = *reinterpret_cast<const uint4*>(pl[u].src + (l + j * p.lanes) * N);
+        }
+      } else {
+        pl[u].kind = 3;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      // every lane of the warp takes part in the shuffles
+      float x[NC][N];
+      float ss = 0.0f;
+      const bool live = on && pl[u].kind < 2;
+      if (live) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          unpack<T>(c[u][j], x[j]);
+#pragma unroll
+          for (int e = 0; e < N; ++e) ss = __fmaf_rn(x[j][e], x[j][e], ss);
+        }
+      }
+      for (int d = gl >> 1; d > 0; d >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, d));
+      if (live) {
+        const float rs = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(p.D)), p.eps));
+        const void* w = pl[u].kind ? p.kw : p.qw;
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+          for (int e = 0; e < N; ++e)
+            x[j][e] = __fmul_rn(__fmul_rn(x[j][e], rs), load_w(w, p.wdtype, (l + j * p.lanes) * N + e));
+        if constexpr (INTER) {
+#pragma unroll
+          for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int e = 0; e < N / 2; ++e) {
+              const float a = x[j][2 * e], b = x[j][2 * e + 1];
+              const float cc = co[j * (N / 2) + e], sn = si[j * (N / 2) + e];
+              x[j][2 * e] = __fmaf_rn(a, cc, -__fmul_rn(b, sn));
+              x[j][2 * e + 1] = __fmaf_rn(a, sn, __fmul_rn(b, cc));
+            }
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const float a = x[0][e], b = x[1][e];
+            x[0][e] = __fmaf_rn(a, co[e], -__fmul_rn(b, si[e]));
+            x[1][e] = __fmaf_rn(a, si[e], __fmul_rn(b, co[e]));
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NC; ++j) c[u][j] = pack<T>(x[j]);
+      }
+      if (on && pl[u].kind < 3) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          const int off = (l + j * p.lanes) * N;
+          if (pl[u].dst) *reinterpret_cast<uint4*>(pl[u].dst + off) = c[u][j];
+          if (pl[u].dst2) *reinterpret_cast<uint4*>(pl[u].dst2 + off) = c[u][j];
+        }
+      }
+    }
+  }
+}
+
+// Any D <= kMaxDim, rotary width, stride and alignment: a warp per vector, staged in shared memory.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) any_kernel(const Params p) {
+  __shared__ float s_x[kThreads / 32][kMaxDim];
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float* x = s_x[warp];
+  const int64_t n = p.n_rows * p.nvec;
+  for (int64_t w = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + warp; w < n;
+       w += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
+    const int64_t t = w / p.nvec;
+    const int i = static_cast<int>(w - t * p.nvec);
+    Row row;
+    if (!describe_row(p, t, lane == 0 && i == 0, row)) continue;
+    const Place<T> pl = place<T>(p, row, t, i);
+    float ss = 0.0f;
+    for (int e = lane; e < p.D; e += 32) {
+      const float f = to_f32<T>(pl.src[e]);
+      x[e] = f;
+      ss = __fmaf_rn(f, f, ss);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, d));
+    __syncwarp();
+    const float rs = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(p.D)), p.eps));
+    const float* cs = p.table + row.pos * p.rd;
+    const int half = p.rd >> 1;
+    const void* wt = pl.kind == 1 ? p.kw : p.qw;
+    for (int e = lane; e < p.D; e += 32) {
+      T out;
+      if (pl.kind == 2) {
+        out = pl.src[e];
+      } else {
+        float y = __fmul_rn(__fmul_rn(x[e], rs), load_w(wt, p.wdtype, e));
+        if (e < p.rd) {
+          const int pi = p.interleaved ? e >> 1 : (e < half ? e : e - half);
+          const bool first = p.interleaved ? !(e & 1) : e < half;
+          const int oe = p.interleaved ? e ^ 1 : (first ? e + half : e - half);
+          const float o = __fmul_rn(__fmul_rn(x[oe], rs), load_w(wt, p.wdtype, oe));
+          const float c = cs[pi], s = cs[half + pi];
+          y = first ? __fmaf_rn(y, c, -__fmul_rn(o, s)) : __fmaf_rn(o, s, __fmul_rn(y, c));
+        }
+        out = from_f32<T>(y);
+      }
+      if (pl.dst) pl.dst[e] = out;
+      if (pl.dst2) pl.dst2[e] = out;
+    }
+    __syncwarp();
+  }
+}
+
+}  // namespace rope
+}  // namespace dk

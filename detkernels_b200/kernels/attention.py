@@ -12,6 +12,10 @@ Drop-in for the reference's ``kernels/attention.py``:
   length.  ``block_s`` is accepted for signature compatibility.
 * ``attention_batch_variant`` (attention.py:301-348): the deliberately variant
   twin -- a fixed split COUNT with f32 atomics when B*H < split_bh_threshold.
+* ``attention_shared_prefix`` (no counterpart in the reference): decode
+  attention of rows that share a prefix, whose part is computed once for the
+  whole batch on the tensor cores; ``attention_shared_prefix_reference`` is its
+  plain form.
 
 Shapes: q [B, H, D]; k, v [B, H_kv, S, D]; out like q.
 """
@@ -192,4 +196,141 @@ def attention_batch_variant(q, k, v, scale: float | None = None, split_bh_thresh
         k.stride(2), out.data_ptr(), out.stride(0), out.stride(1), B, H, S, D, float(scale), int(split_s),
         _lib.dtype_code(q.dtype), ws.data_ptr(), ws.numel(), stream)
     _lib.check(rc, "attention_batch_variant")
+    return out
+
+
+def attention_shared_prefix_reference(q, k_prefix, v_prefix, k, v, kv_lens, scale: float | None = None):
+    """Plain PyTorch attention of rows behind a shared prefix, f32.
+
+    q: (R, H, D); k_prefix, v_prefix: (H_kv, P, D); k, v: (R, H_kv, S, D), row r's own tokens, of which
+    it reads the first kv_lens[r] after the prefix.  A row that reads nothing is zero."""
+    import torch
+
+    outs = []
+    for r in range(q.shape[0]):
+        n = int(kv_lens[r])
+        kr = torch.cat([k_prefix, k[r, :, :n].to(k_prefix.dtype)], dim=1)[None]
+        vr = torch.cat([v_prefix, v[r, :, :n].to(v_prefix.dtype)], dim=1)[None]
+        outs.append(attention_reference(q[r:r + 1], kr, vr, scale) if kr.shape[2] else torch.zeros_like(q[r:r + 1]))
+    return torch.cat(outs) if outs else torch.empty_like(q)
+
+
+def _tma_strides(t, name):
+    """Element strides of a 16-bit cache tensor as the kernels need them (unit along D, the others
+    multiples of 8 elements, 16-byte aligned base); a dimension of one element takes any stride."""
+    st = list(t.stride())
+    nat = 1
+    for i in range(t.dim() - 1, -1, -1):
+        if t.shape[i] <= 1:
+            st[i] = nat
+        nat = max(nat, st[i] * max(1, t.shape[i]))
+    if st[-1] != 1 or any(s % 8 for s in st[:-1]) or t.data_ptr() % 16:
+        raise ValueError("%s: unit stride along head_dim, strides that are multiples of 8 elements and a 16-byte "
+                         "aligned start required" % name)
+    return st
+
+
+def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *, prefix_len=None, prefix_blocks=None,
+                            block_table=None, row_tiles=None, max_kv_len=None, scale=None, out=None, workspace=None):
+    """Batch-invariant decode attention of rows that share a prefix.
+
+    q [R, H, D]; row r attends to the first ``prefix_len`` tokens of the prefix and then to the first
+    kv_lens[r] tokens of its own KV sequence (row r reads sequence r, or ``row_tiles`` as in
+    ``attention_decode``).  The prefix part is computed once for all rows.
+
+    k_prefix, v_prefix: [H_kv, P, D]; or, with ``prefix_blocks`` (int32 CUDA [ceil(prefix_len / page)]),
+    block pools [n_blocks, H_kv, page, D] (page a multiple of 64) whose block prefix_blocks[t // page]
+    holds prefix token t.  prefix_len defaults to all of it; 0 is plain ``attention_decode``.
+    k_cache, v_cache, kv_lens, block_table, max_kv_len: as in ``attention_decode`` (kv_lens and
+    max_kv_len count the rows' own tokens only).  bf16 or f16; head_dim 32, 64 or 128; at most 16 query
+    heads per KV head.
+
+    A row's bits depend on its q, the prefix, its own tokens and nothing else of the batch."""
+    import torch
+
+    for t in (q, k_prefix, v_prefix, k_cache, v_cache):
+        assert t.is_cuda and t.device == q.device, "attention_shared_prefix requires CUDA tensors on one device"
+    R, H, D = q.shape
+    for t in (k_prefix, v_prefix, k_cache, v_cache):
+        if t.dtype != q.dtype:
+            raise TypeError("attention_shared_prefix: q, the prefix and the caches must share a dtype")
+    assert v_prefix.shape == k_prefix.shape and v_cache.shape == k_cache.shape, "q/k/v shape mismatch"
+    n_seq, Hkv, cap, Dk = k_cache.shape
+    assert Dk == D and H % Hkv == 0, "q/k/v shape mismatch"
+    n_pool = page_p = 0
+    if prefix_blocks is None:
+        assert k_prefix.dim() == 3 and k_prefix.shape[0] == Hkv and k_prefix.shape[2] == D, "prefix shape mismatch"
+        p_cap = k_prefix.shape[1]
+    else:
+        assert prefix_blocks.dtype == torch.int32 and prefix_blocks.device == q.device and prefix_blocks.dim() == 1
+        assert prefix_blocks.numel() <= 1 or prefix_blocks.stride(0) == 1
+        assert k_prefix.dim() == 4 and k_prefix.shape[1] == Hkv and k_prefix.shape[3] == D, "prefix shape mismatch"
+        n_pool, page_p = k_prefix.shape[0], k_prefix.shape[2]
+        p_cap = prefix_blocks.numel() * page_p
+    P = p_cap if prefix_len is None else int(prefix_len)
+    if P < 0 or P > p_cap:
+        raise ValueError("attention_shared_prefix: prefix_len %d outside [0, %d]" % (P, p_cap))
+    uniform = isinstance(kv_lens, int)
+    if not uniform:
+        assert kv_lens.dtype == torch.int32 and kv_lens.device == q.device and kv_lens.numel() == R
+        kv_lens = kv_lens.contiguous()
+    n_blocks = page = width = bt_stride = 0
+    if block_table is not None:
+        assert block_table.dtype == torch.int32 and block_table.device == q.device and block_table.dim() == 2
+        assert block_table.shape[1] <= 1 or block_table.stride(1) == 1
+        n_blocks, page = n_seq, cap
+        n_seq, width = block_table.shape
+        cap, bt_stride = width * page, max(block_table.stride(0), width)
+    if max_kv_len is None:
+        max_kv_len = kv_lens if uniform else cap
+    max_kv_len = int(max_kv_len)
+    if max_kv_len < 0 or (max_kv_len and not cap):
+        raise ValueError("attention_shared_prefix: max_kv_len %d outside the cache" % max_kv_len)
+    if uniform and not 0 <= kv_lens <= max_kv_len:
+        raise ValueError("attention_shared_prefix: kv_lens %d outside [0, %d]" % (kv_lens, max_kv_len))
+    if scale is None:
+        scale = 1.0 / (D ** 0.5)
+    if out is None:
+        out = torch.empty((R, H, D), dtype=q.dtype, device=q.device)
+    assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and out.stride(2) == 1
+    if row_tiles is not None:
+        assert row_tiles.dtype == torch.int32 and row_tiles.device == q.device and row_tiles.is_contiguous()
+        assert row_tiles.dim() == 2 and row_tiles.shape[1] == 3
+    if R == 0:
+        return out
+    if q.data_ptr() % 16 or q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8:
+        q = q.clone(memory_format=torch.contiguous_format)
+    with torch.cuda.device(q.device):
+        if P == 0:
+            return attention_decode(q, k_cache, v_cache, kv_lens, scale=scale, row_tiles=row_tiles,
+                                    max_kv_len=max_kv_len, out=out, workspace=workspace, block_table=block_table)
+        ps, vps = _tma_strides(k_prefix, "k_prefix"), _tma_strides(v_prefix, "v_prefix")
+        assert ps == vps, "k and v prefixes must share strides"
+        cs = [0, 0, 0, 1]
+        n_tiles, rows_per_tile = (R, 1) if row_tiles is None else (row_tiles.shape[0], 2)
+        lib = _lib.load()
+        stream = _lib.stream_ptr(q.device)
+        if max_kv_len:
+            cs, cvs = _tma_strides(k_cache, "k_cache"), _tma_strides(v_cache, "v_cache")
+            assert cs == cvs, "k and v caches must share strides"
+            if uniform:
+                kv_lens = torch.full((R,), kv_lens, dtype=torch.int32, device=q.device)
+            if workspace is None:
+                workspace = _lib.call_workspace(
+                    lib.dk_attention_workspace_size(n_tiles, rows_per_tile, H, Hkv, D, max_kv_len), q.device, stream)
+        nbytes = lib.dk_attention_prefix_state_size(R, H, Hkv, D, P)
+        state = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+        rc = lib.dk_attention_shared_prefix(
+            q.data_ptr(), q.stride(0), q.stride(1), k_prefix.data_ptr(), v_prefix.data_ptr(),
+            ps[0] if prefix_blocks is not None else 0, ps[-3], ps[-2], P,
+            prefix_blocks.data_ptr() if prefix_blocks is not None else None, n_pool, page_p, k_cache.data_ptr(),
+            v_cache.data_ptr(), cs[0], cs[1], cs[2], n_seq, cap,
+            block_table.data_ptr() if block_table is not None else None, bt_stride, width, n_blocks, page,
+            out.data_ptr(), out.stride(0), out.stride(1), None if uniform and not max_kv_len else kv_lens.data_ptr(),
+            row_tiles.data_ptr() if row_tiles is not None else None, n_tiles, R, H, Hkv, D, max_kv_len, float(scale),
+            _lib.dtype_code(q.dtype), state.data_ptr(), state.numel(),
+            workspace.data_ptr() if workspace is not None else None,
+            workspace.numel() if workspace is not None else 0, stream)
+    _lib.check(rc, "attention_shared_prefix")
+    _lib.count_launch(3 if max_kv_len else 2)
     return out

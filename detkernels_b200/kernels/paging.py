@@ -1,0 +1,131 @@
+"""Page plan of a serving step, built on the GPU from the requests' lengths.
+
+The device counterpart of ``tiny_model.BlockAllocator`` and of the host side of
+``DecodeEngine.plan``: block-table growth from a free list, the slot of every
+new token in the paged cache, its sequence, position and attention length, and
+the attention kernels' row tiles, in two launches without a host round trip.
+No counterpart in the reference (its cache is one tensor grown by
+``torch.cat``, tiny_model.py:119-125).
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+from detkernels_b200 import _lib
+
+
+class PagedPlan(NamedTuple):
+    """One step's plan; the fields that were not asked for are None."""
+    block_table: object            # int32 [B, blocks_per_seq] (the caller's tensor, grown in place)
+    cursor: Optional[object]       # int32 [1]: free blocks handed out, this step's included
+    cu_rows: object                # int32 [B + 1]: first row of each sequence, and the total
+    row_seq: Optional[object]      # int32 [n_rows]
+    row_pos: Optional[object]      # int32 [n_rows]
+    slots: Optional[object]        # int64 [n_rows]: block * page_size + token in the block
+    q_lens: Optional[object]       # int32 [n_rows]: row_pos + 1
+    row_tiles: Optional[object]    # int32 [n_tiles, 3]: (first row, rows, sequence)
+
+
+def paged_plan_reference(block_table, kv_lens, new_lens, page_size, *, free_blocks=None, cursor=0, rows_per_tile=0):
+    """Plain Python plan of one step on host sequences; block_table is a list of lists.  Returns the
+    fields of PagedPlan as Python lists (block_table a grown copy)."""
+    table = [list(row) for row in block_table]
+    cu, seq, pos, slots, tiles = [0], [], [], [], []
+    for b, (kv, new) in enumerate(zip(kv_lens, new_lens)):
+        if free_blocks is not None:
+            for pg in range(-(-kv // page_size), -(-(kv + new) // page_size)):
+                table[b][pg] = free_blocks[cursor]
+                cursor += 1
+        for t in range(kv, kv + new):
+            seq.append(b)
+            pos.append(t)
+            slots.append(table[b][t // page_size] * page_size + t % page_size)
+        if rows_per_tile:
+            tiles += [(cu[-1] + i, min(rows_per_tile, new - i), b) for i in range(0, new, rows_per_tile)]
+        cu.append(cu[-1] + new)
+    return PagedPlan(table, cursor, cu, seq, pos, slots, [t + 1 for t in pos], tiles)
+
+
+def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=None, cursor=None,
+               n_rows: Optional[int] = None, rows_per_tile: int = 0, n_tiles: Optional[int] = None,
+               out: Optional[PagedPlan] = None) -> PagedPlan:
+    """Plan one step in which sequence b, holding kv_lens[b] tokens, gets new_lens[b] more.
+
+    block_table: int32 CUDA [>= B, blocks_per_seq]; kv_lens, new_lens: int32 CUDA [B].
+    free_blocks (int32 CUDA [F]) and cursor (int32 CUDA [1], how many of them are already handed out):
+    the table entries of the pages that the new tokens open become the next free blocks, in sequence
+    order; without them the table must already cover every sequence.  Other entries, and rows of the
+    table past B, stay as they are.
+    n_rows: how many new tokens there are (the sum of new_lens, or a bound on it): asks for row_seq,
+    row_pos, slots and q_lens.  rows_per_tile and n_tiles (the sum of ceil(new_lens / rows_per_tile), or
+    a bound) ask for row_tiles.  Entries past the step's own total stay as they are (uninitialised in new tensors).
+    out: a PagedPlan of an earlier call whose tensors take the results (its cursor may be ``cursor``).
+
+    A negative length, a sequence longer than its table row, an exhausted free list or more rows or tiles
+    than announced sets the device status (``_lib.raise_on_device_error``) and leaves the table and all
+    outputs but cu_rows as they were."""
+    import torch
+
+    dev = block_table.device
+    B = kv_lens.numel()
+    assert block_table.is_cuda and kv_lens.device == dev and new_lens.device == dev, \
+        "paged_plan requires CUDA tensors on one device"
+    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] >= B
+    assert block_table.shape[1] <= 1 or block_table.stride(1) == 1, "block_table: unit stride along a row"
+    for t in (kv_lens, new_lens):
+        assert t.dtype == torch.int32 and t.dim() == 1 and t.numel() == B, "lengths must be int32 [B]"
+    if page_size < 1:
+        raise ValueError("paged_plan: page_size must be positive")
+    if (free_blocks is None) != (cursor is None):
+        raise ValueError("paged_plan: free_blocks and cursor go together")
+    if free_blocks is not None:
+        assert free_blocks.dtype == torch.int32 and free_blocks.device == dev and free_blocks.is_contiguous()
+        assert cursor.dtype == torch.int32 and cursor.device == dev and cursor.numel() == 1
+    if rows_per_tile < 0 or (rows_per_tile > 0 and n_tiles is None) or (rows_per_tile == 0 and n_tiles):
+        raise ValueError("paged_plan: rows_per_tile and n_tiles go together")
+    for n in (n_rows, n_tiles):
+        if n is not None and n < 0:
+            raise ValueError("paged_plan: n_rows and n_tiles must not be negative")
+
+    def take(field, shape, dtype):
+        t = getattr(out, field) if out is not None else None
+        if t is None:
+            return torch.empty(shape, dtype=dtype, device=dev)
+        assert t.dtype == dtype and t.device == dev and tuple(t.shape) == tuple(shape) and t.is_contiguous(), \
+            "paged_plan: out.%s does not fit" % field
+        return t
+
+    with torch.cuda.device(dev):
+        kv_lens, new_lens = kv_lens.contiguous(), new_lens.contiguous()
+        cu = take("cu_rows", (B + 1,), torch.int32)
+        cur = take("cursor", (1,), torch.int32) if cursor is not None else None
+        row_seq = row_pos = slots = q_lens = tiles = None
+        if n_rows is not None:
+            row_seq = take("row_seq", (n_rows,), torch.int32)
+            row_pos = take("row_pos", (n_rows,), torch.int32)
+            slots = take("slots", (n_rows,), torch.int64)
+            q_lens = take("q_lens", (n_rows,), torch.int32)
+        if rows_per_tile > 0:
+            tiles = take("row_tiles", (n_tiles, 3), torch.int32)
+        plan = PagedPlan(block_table, cur, cu, row_seq, row_pos, slots, q_lens, tiles)
+        if B == 0:
+            cu.zero_()
+            if cur is not None and cur.data_ptr() != cursor.data_ptr():
+                cur.copy_(cursor.view(1))
+            return plan
+        lib = _lib.load()
+        ws = torch.empty(lib.dk_paged_plan_workspace_size(B), dtype=torch.uint8, device=dev)
+
+        def ptr(t):
+            # an output of no entries is still asked for: its pointer is never followed
+            return None if t is None else (t.data_ptr() or ws.data_ptr())
+
+        rc = lib.dk_paged_plan(
+            block_table.data_ptr(), max(block_table.stride(0), block_table.shape[1]), block_table.shape[1],
+            kv_lens.data_ptr(), new_lens.data_ptr(), B, int(page_size),
+            ptr(free_blocks), 0 if free_blocks is None else free_blocks.numel(), ptr(cursor), ptr(cur), cu.data_ptr(),
+            ptr(row_seq), ptr(row_pos), ptr(slots), ptr(q_lens), n_rows or 0, ptr(tiles), int(rows_per_tile),
+            n_tiles or 0, ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev))
+    _lib.check(rc, "paged_plan")
+    _lib.count_launch(2)
+    return plan

@@ -331,6 +331,82 @@ int dk_gdn_forward(const void* q, const void* k, const void* v, const void* g, c
                    int head_dim_k, int head_dim_v, int dtype, int gb_dtype, float scale, const void* initial_state,
                    int state_dtype, float* final_state, int chunk_size, void* stream);
 
+/* ---- Serving steps: page plan, head norm + rotation into the cache, shared-prefix attention ----
+ * No counterparts in the reference (its cache is one tensor grown by torch.cat, its decoder has no
+ * rotation, and every row reads its whole KV sequence: kernels/tiny_model.py:99-140). */
+
+/* Scratch bytes of dk_paged_plan (uninitialised memory will do). */
+size_t dk_paged_plan_workspace_size(int64_t n_seqs);
+/* Plans one step of n_seqs sequences on the device.  Sequence b holds kv_lens[b] tokens and gets
+ * new_lens[b] more (device int32[n_seqs], >= 0).
+ *  - free_blocks (device int32[n_free], may be NULL: the table is only read): the table entries
+ *    [ceil(kv / page_size), ceil((kv + new) / page_size)) of row b of block_table [n_seqs][blocks_per_seq]
+ *    become the next free blocks from position *cursor on, in sequence order; *cursor_out = *cursor + the
+ *    number taken (cursor_out may be cursor).  The other entries stay as they are.
+ *  - cu_rows: int32[n_seqs + 1], the exclusive sums of new_lens.
+ *  - row_seq, row_pos, slots, q_lens (all or none; n_rows entries each): row cu_rows[b] + i is token
+ *    pos = kv_lens[b] + i of sequence b, at slot table[b][pos / page_size] * page_size + pos % page_size,
+ *    and attends to q_lens = pos + 1 tokens.  Entries past cu_rows[n_seqs] stay as they are.
+ *  - row_tiles (may be NULL; int32[n_tiles][3]): (first row, rows, sequence) of up to rows_per_tile rows
+ *    of one sequence, the row_tiles of the attention entry points.  Tiles past the last stay as they are.
+ * A negative length or a sequence beyond blocks_per_seq pages (detail 0x600), too few free blocks (0x601)
+ * or more rows or tiles than the outputs hold (0x602) is recorded as DK_ERR_DEVICE_CHECK; then only cu_rows
+ * and the workspace are written and *cursor_out = *cursor. */
+int dk_paged_plan(int32_t* block_table, int64_t block_table_stride, int32_t blocks_per_seq, const int32_t* kv_lens,
+                  const int32_t* new_lens, int32_t n_seqs, int32_t page_size, const int32_t* free_blocks,
+                  int64_t n_free, const int32_t* cursor, int32_t* cursor_out, int32_t* cu_rows, int32_t* row_seq,
+                  int32_t* row_pos, int64_t* slots, int32_t* q_lens, int64_t n_rows, int32_t* row_tiles,
+                  int32_t rows_per_tile, int64_t n_tiles, void* workspace, size_t workspace_bytes, void* stream);
+
+/* RMSNorm of every query and key head followed by the rotation of its first rotary_dim elements, f32
+ * math, one rounding at the store.  q [n_rows, n_q_heads, head_dim], k and v [n_rows, n_kv_heads,
+ * head_dim]: element strides by row and head, unit stride along head_dim.  Pairs are (i, i +
+ * rotary_dim / 2), or (2i, 2i + 1) when interleaved; row r's angles are row positions[r] (device int32, or
+ * int64 when positions_64) of rope_table: f32 [max_pos, rotary_dim] = cos[rotary_dim / 2], sin[...].
+ * q_out may be q and k_out may be k (same strides).  With k_cache / v_cache [cache_slabs, n_kv_heads,
+ * cache_capacity, head_dim] (slab = sequence or block), slots (device int64[n_rows]) and v, the rotated
+ * key and the value of row r go to slab slots[r] / cache_capacity, token slots[r] % cache_capacity; a
+ * negative slot stores nothing, one beyond the cache is recorded (DK_ERR_DEVICE_CHECK, detail 0x611) and
+ * stores nothing.  k_out may be NULL with a cache.  A position outside the table is recorded (0x610) and
+ * its row not written.  head_dim <= 512; any dtype of the three for q/k/v/caches, and for the weights
+ * [head_dim].  16-byte aligned vectors take the vector path. */
+int dk_qk_norm_rope(const void* q, int64_t q_stride_row, int64_t q_stride_head, const void* k, int64_t k_stride_row,
+                    int64_t k_stride_head, const void* v, int64_t v_stride_row, int64_t v_stride_head, void* q_out,
+                    int64_t q_out_stride_row, int64_t q_out_stride_head, void* k_out, int64_t k_out_stride_row,
+                    int64_t k_out_stride_head, void* k_cache, void* v_cache, int64_t cache_stride_slab,
+                    int64_t cache_stride_head, int64_t cache_stride_tok, int64_t cache_slabs, int64_t cache_capacity,
+                    const int64_t* slots, const void* positions, int positions_64, const void* q_weight,
+                    const void* k_weight, int weight_dtype, const float* rope_table, int64_t max_pos, int64_t n_rows,
+                    int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t rotary_dim, int interleaved,
+                    float eps, int dtype, void* stream);
+
+/* Scratch bytes of the prefix states of dk_attention_shared_prefix (uninitialised memory will do). */
+size_t dk_attention_prefix_state_size(int64_t n_rows, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                      int64_t prefix_len);
+/* Decode attention of rows that share a prefix: row r attends to the prefix_len prefix tokens and then
+ * to tokens [0, kv_len_r) of its own KV sequence, the prefix part computed once for all rows.
+ * The prefix: k_prefix / v_prefix [n_kv_heads, prefix_len, head_dim] (prefix_stride_head / _tok), or,
+ * with prefix_blocks (device int32[ceil(prefix_len / prefix_page)]), block pools [prefix_pool_blocks,
+ * n_kv_heads, prefix_page, head_dim] whose block prefix_blocks[t / prefix_page] holds token t (a block id
+ * outside the pool: DK_ERR_DEVICE_CHECK, detail 0x62a).  prefix_page is a multiple of 64.
+ * The rows' own tokens: q, k, v, kv_lens, row_tiles, max_kv_len, scale, workspace as in
+ * dk_attention_batch_invariant, or with block_table as in dk_attention_paged_batch_invariant
+ * (kv_stride_seq is then the block stride); max_kv_len = 0: no row has any, and k, v and kv_lens are not
+ * read.  q must be 16-byte aligned with strides that are multiples of 8 elements.
+ * Batch invariant: a row's bits follow from its q, the prefix and its own tokens. */
+int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_stride_head, const void* k_prefix,
+                               const void* v_prefix, int64_t prefix_stride_block, int64_t prefix_stride_head,
+                               int64_t prefix_stride_tok, int32_t prefix_len, const int32_t* prefix_blocks,
+                               int64_t prefix_pool_blocks, int32_t prefix_page, const void* k, const void* v,
+                               int64_t kv_stride_seq, int64_t kv_stride_head, int64_t kv_stride_tok, int64_t kv_n_seq,
+                               int64_t kv_capacity, const int32_t* block_table, int64_t block_table_stride,
+                               int32_t blocks_per_seq, int64_t n_blocks, int32_t page_size, void* out,
+                               int64_t out_stride_row, int64_t out_stride_head, const int32_t* kv_lens,
+                               const int32_t* row_tiles, int32_t n_tiles, int32_t n_rows, int32_t n_q_heads,
+                               int32_t n_kv_heads, int32_t head_dim, int32_t max_kv_len, float scale, int dtype,
+                               void* state, size_t state_bytes, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif
