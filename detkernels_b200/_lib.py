@@ -29,7 +29,6 @@ DK_BF16 = 2
 
 MATMUL_K_SLICES = 8
 ATTN_KV_SPLIT = 256
-WORKSPACE_COUNTER_BYTES = 1 << 20
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -99,12 +98,12 @@ SIGNATURES = {
                                _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64,
                                _c_void_p, _c_void_p, _int, _c_void_p, _c_void_p, _int, _c_void_p, _i64, _i64, _i32,
                                _i32, _i32, _i32, _int, _f32, _int, _c_void_p]),
-    "dk_attention_prefix_state_size": (_size, [_i64, _i32, _i32, _i32, _i64]),
+    "dk_attention_shared_prefix_workspace_size": (_size, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "dk_attention_shared_prefix": (_int, [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i32,
                                           _c_void_p, _i64, _i32, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64,
                                           _c_void_p, _i64, _i32, _i64, _i32, _c_void_p, _i64, _i64, _c_void_p,
                                           _c_void_p, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _int, _c_void_p, _size,
-                                          _c_void_p, _size, _c_void_p]),
+                                          _c_void_p]),
 }
 
 
@@ -279,20 +278,6 @@ def workspace(nbytes: int, device, stream: int):
             buf = torch.zeros(size, dtype=torch.uint8, device=dev)
             _workspaces[key] = buf
         return buf
-
-
-def call_workspace(nbytes: int, device, stream: int):
-    """``workspace`` for a call that may be captured: while the stream is being captured the scratch
-    belongs to the graph (allocated and its counters zeroed inside it), so that no two graphs share
-    one and none outlives the buffer it was captured with."""
-    import torch
-    if nbytes <= 0:
-        return None
-    if not torch.cuda.is_current_stream_capturing():
-        return workspace(nbytes, device, stream)
-    buf = torch.empty(int(nbytes), dtype=torch.uint8, device=device)
-    buf[:WORKSPACE_COUNTER_BYTES].zero_()
-    return buf
 
 
 @contextlib.contextmanager

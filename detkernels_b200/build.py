@@ -2,7 +2,7 @@
 
     python -m detkernels_b200.build          # -> detkernels_b200/libdetkernels_b200.so
 
-The library is three CUDA translation units (csrc/*.cu), compiled side by side
+The library is two CUDA translation units (csrc/*.cu), compiled side by side
 with nvcc for `sm_100a` only.  It links the CUDA runtime statically and reaches the
 driver API (tensor-map encoding) through cudaGetDriverEntryPointByVersion, so
 the .so loads on a machine without a GPU driver (symbol checks, CPU tests).

@@ -99,9 +99,6 @@ struct Params {
   float* ws_o;        // [n_tiles][hkv][max_splits][rows_cap][D]
   float* ws_ml;       // [n_tiles][hkv][max_splits][rows_cap][2]
   int32_t* counters;  // [n_tiles][hkv]
-  // state instances (ST): each (row, query head)'s softmax state instead of its output
-  float* st_o;        // [n_rows][hq][D], sum of p v
-  float* st_ml;       // [n_rows][hq][2], running max (log2 units; -inf for an empty row) and sum
 };
 
 // K and V tensor maps: 64-token boxes for whole blocks and 16-token boxes for the tail of a
@@ -315,10 +312,7 @@ __device__ __forceinline__ int describe_item(const Params& p, int64_t w, Item& i
 // Occupancy: 3 CTAs per SM for d <= 64, except the wide multi-row (prefill) instances
 // (KM >= 8), which run 2 per SM without register spills, and the single-row instances,
 // 4 per SM (both measured faster).
-// ST: the launch writes (m, l, O) states for a later merge and follows another kernel of the same
-// call that has itself waited for everything this one reads, so it starts without waiting for that
-// kernel; it waits before it ends, so that a wait for this grid covers both.
-template <typename T, int D, int KM, bool T1, bool ST = false>
+template <typename T, int D, int KM, bool T1>
 __global__ void __launch_bounds__(kThreads, (D == 128 || (!T1 && KM >= 8)) ? 2 : (T1 ? 4 : 3))
     attn_kernel(const __grid_constant__ KvMaps maps, const Params p) {
   using C = Cfg<D, T1>;
@@ -361,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, (D == 128 || (!T1 && KM >= 8)) ? 2 :
     tma_prefetch_desc(&maps.k16);
     tma_prefetch_desc(&maps.v16);
   }
-  if constexpr (!ST) pdl_wait();   // lengths, tiles and q may come from the previous kernel
+  pdl_wait();   // lengths, tiles and q may come from the previous kernel
   if (threadIdx.x == 0) pdl_launch_dependents();
   __syncthreads();   // barrier initialisation visible to every warp
 
@@ -532,13 +526,7 @@ __global__ void __launch_bounds__(kThreads, (D == 128 || (!T1 && KM >= 8)) ? 2 :
         for (int e = ctid; e < valid_rows * D; e += kConsumerWarps * 32) {
           const int rho = e / D, d = e % D;
           const int i = rho / p.G, gh = rho % p.G;
-          if constexpr (ST) {
-            const int64_t m = (int64_t)(r0 + i) * p.hq + (kvh * p.G + gh);
-            p.st_o[m * D + d] = 0.0f;
-            if (d == 0) *reinterpret_cast<float2*>(p.st_ml + 2 * m) = make_float2(-INFINITY, 0.0f);
-          } else {
-            out[(int64_t)(r0 + i) * p.o_sr + (int64_t)(kvh * p.G + gh) * p.o_sh + d] = from_f32<T>(0.0f);
-          }
+          out[(int64_t)(r0 + i) * p.o_sr + (int64_t)(kvh * p.G + gh) * p.o_sh + d] = from_f32<T>(0.0f);
         }
       }
       break;
@@ -862,14 +850,8 @@ __global__ void __launch_bounds__(kThreads, (D == 128 || (!T1 && KM >= 8)) ? 2 :
       if (e < valid_rows * D) {
         const int rho = e / D, d = e % D;
         const int i = rho / p.G, gh = rho % p.G;
-        if constexpr (ST) {   // a row of length 0 merged nothing: (-inf, 0, 0)
-          const int64_t m = (int64_t)(r0 + i) * p.hq + (kvh * p.G + gh);
-          p.st_o[m * D + d] = run_o[k];
-          if (d == 0) *reinterpret_cast<float2*>(p.st_ml + 2 * m) = make_float2(run_m[k], run_l[k]);
-        } else {
-          const float r = (s_len[i] == 0) ? 0.0f : __fdiv_rn(run_o[k], run_l[k]);
-          out[(int64_t)(r0 + i) * p.o_sr + (int64_t)(kvh * p.G + gh) * p.o_sh + d] = from_f32<T>(r);
-        }
+        const float r = (s_len[i] == 0) ? 0.0f : __fdiv_rn(run_o[k], run_l[k]);
+        out[(int64_t)(r0 + i) * p.o_sr + (int64_t)(kvh * p.G + gh) * p.o_sh + d] = from_f32<T>(r);
       }
     }
     } while (0);
@@ -881,7 +863,6 @@ __global__ void __launch_bounds__(kThreads, (D == 128 || (!T1 && KM >= 8)) ? 2 :
       iph ^= 1u;
     }
   }
-  if constexpr (ST) pdl_wait();
 }
 
 }  // namespace attn

@@ -147,9 +147,8 @@ static inline cudaError_t unit_status(int clear, int* code, int* detail) {
   return e;
 }
 
-// Status words of the other translation units (same contract as unit_status).
+// Status word of dk_serving.cu (same contract as unit_status).
 cudaError_t serving_status(int clear, int* code, int* detail);
-cudaError_t attention_state_status(int clear, int* code, int* detail);
 
 }  // namespace host
 }  // namespace dk

@@ -2,44 +2,48 @@
 //
 // The query heads of all rows that read KV head h are the rows of one matrix Q_h [R * G, D]; with
 // S = Q_h K_h^T * scale, the prefix contributes to each row the softmax state (m, l, O) with
-// l = sum 2^(S log2e - m), O = sum 2^(S log2e - m) V, which joins the state of the row's own tokens
-// (the decode attention kernel's state instances) in combine_kernel: out = O / l.
+// l = sum 2^(S log2e - m), O = sum 2^(S log2e - m) V, which joins the states of the row's own tokens
+// (dk_own.cuh) in combine_kernel: out = O / l.
 //
 // Fixed reduction structure (the definition of a row's bits):
-//   * The prefix is cut into chunks of chunk_tokens(P) tokens: 512, or more for a prefix beyond
-//     16384 tokens so that there are at most 32.  The size follows the prefix length only.
+//   * The prefix is cut into chunks whose size follows the prefix length and head_dim only
+//     (chunk_tokens).
 //   * Inside a chunk, blocks of 128 tokens in order: S from tcgen05.mma (f32 accumulation over D in
 //     16-deep steps), a reference maximum m that is raised only when a block's maximum exceeds it
 //     by more than 8 (a factor 256, so the weights stay in range of either 16-bit type), weights
 //     2^(S c - m) rounded to the input type for P.V as the left operand of a second tcgen05.mma in
 //     TMEM, l summed in f32 from the unrounded weights in a fixed order.
-//   * The chunks' states are joined in order inside groups of kGroup chunks, the groups' states in
-//     order, and the row's own tokens last.
+//   * The chunks' states are joined in order inside groups of kGroup chunks (head_dim <= 64 only),
+//     the groups' states in order, and the states of the row's own tokens last.
 // No step looks at another row, so a row's bits do not depend on the batch.
 //
 // Work: an item is (up to two tiles of 128 rows, KV head, run of tokens), one persistent CTA per SM.
 // Warp 8 streams K and V blocks with TMA, warp 9 issues the MMAs, two warpgroups hold one row a
 // thread and do the softmax.  The two tiles of an item share K and V and alternate on the tensor
 // cores; an item of one tile alternates two score buffers instead.  A run is a whole group, whose
-// chunks are joined in registers, or, when that leaves SMs idle, one chunk, whose state
-// combine_kernel joins; both give the same bits.
+// chunks are joined in TMEM (which has room for that beside two 64-wide accumulators, not 128-wide
+// ones), or, when that leaves SMs idle, one chunk, whose state combine_kernel joins; both give the
+// same bits.
 #pragma once
 
 #include "dk_common.cuh"
+#include "dk_own.cuh"
 
 namespace dk {
 namespace prefix {
 
+using own::exp2_hw;
+using own::join;
+using own::join_weights;
+using own::pack2;
+
 constexpr int kBlock = 128;      // tokens a block
 constexpr int kRows = 128;       // rows a tile
-constexpr int kGroup = 8;        // chunks a group
-constexpr int kMinChunk = 512;
-constexpr int kMaxChunks = 32;
 constexpr int kSoftThreads = 256;
 constexpr int kThreads = 384;    // two softmax warpgroups; TMA, MMA and two idle warps
-constexpr int kLaunchRegs = 168; // registers a thread at launch; 384 * 168 = 256 * 224 + 128 * 56
-constexpr int kSoftRegs = 224;
-constexpr int kIoRegs = 56;
+constexpr int kLaunchRegs = 168; // registers a thread at launch; 384 * 168 = 256 * 208 + 128 * 88
+constexpr int kSoftRegs = 208;
+constexpr int kIoRegs = 88;
 constexpr float kLazy = 8.0f;
 
 enum : int {
@@ -55,10 +59,17 @@ enum : int {
   kDetPage = 0x62a,   // a prefix block id outside the pool
 };
 
-// Tokens a chunk: a function of the prefix length alone.
-__host__ __device__ inline int64_t chunk_tokens(int64_t prefix_len) {
-  const int64_t span = static_cast<int64_t>(kMinChunk) * kMaxChunks;
-  return kMinChunk * ((prefix_len + span - 1) / span);
+// Chunks a group.
+__host__ __device__ constexpr int group_chunks(int head_dim) { return head_dim <= 64 ? 8 : 1; }
+
+// Tokens a chunk: a function of the prefix length and head_dim alone.  Short chunks give a small
+// batch enough items to fill the SMs; every chunk of a 128-wide head costs each row a 512-byte state
+// through memory, so those are longer.
+__host__ __device__ inline int64_t chunk_tokens(int64_t prefix_len, int head_dim) {
+  if (head_dim <= 64) return 512 * ((prefix_len + 16383) / 16384);
+  if (prefix_len <= 4096) return 512;
+  if (prefix_len <= 16384) return 1024;
+  return ((prefix_len + 15) / 16 + kBlock - 1) / kBlock * kBlock;
 }
 
 struct Params {
@@ -76,6 +87,7 @@ struct Params {
   int32_t n_blocks;
   float c;                // |scale| * log2(e)
   uint32_t flip;          // sign mask for q (0x80008000 when scale < 0)
+  int zero;               // scale is 0: q is multiplied by it on the way in
   float* st_o;            // [n_runs][rows][hq][D]
   float* st_ml;           // [n_runs][rows][hq][2]
   int64_t st_rows;        // rows * hq
@@ -99,6 +111,8 @@ struct Cfg {
   static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * QTILE + 8 * TBUF + 512;
   static constexpr uint32_t S_COL = 0;            // two score buffers of 128 columns
   static constexpr uint32_t O_COL = 256;          // two accumulators of DP columns
+  static constexpr bool GROUPED = group_chunks(D) > 1;
+  static constexpr uint32_t R_COL = 384;          // grouped: the joined chunks of either tile, DP columns each
 };
 
 template <uint32_t N>
@@ -130,35 +144,45 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&v)[
       : "memory");
 }
 
-// 2^x by the single hardware instruction; 2^-inf = 0, 2^0 = 1.
-__device__ __forceinline__ float exp2_hw(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+}
+
+// Two f32 operations an instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
 }
 
 template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
+__device__ __forceinline__ uint4 times_zero(uint4 v) {
+  uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const T lo = *reinterpret_cast<const T*>(&u[i]), hi = *(reinterpret_cast<const T*>(&u[i]) + 1);
+    u[i] = pack2<T>(__fmul_rn(to_f32<T>(lo), 0.0f), __fmul_rn(to_f32<T>(hi), 0.0f));
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
 }
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-// Weights (a, b) that join state (m, ..) with (ms, ..): the joined value is v * a + vs * b.
-__device__ __forceinline__ float join_weights(float m, float ms, float& a, float& b) {
-  const float mn = fmaxf(m, ms);
-  const float ref = (mn == -INFINITY) ? 0.0f : mn;
-  a = exp2_hw(__fsub_rn(m, ref));
-  b = exp2_hw(__fsub_rn(ms, ref));
-  return mn;
-}
-__device__ __forceinline__ float join(float v, float a, float vs, float b) { return __fmaf_rn(v, a, __fmul_rn(vs, b)); }
 
 // Bounded wait by a whole warp, with one answer for all of its lanes.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int detail, bool& abort_flag) {
@@ -418,13 +442,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
             v.y ^= p.flip;
             v.z ^= p.flip;
             v.w ^= p.flip;
+            if (p.zero) v = times_zero<T>(v);
           }
           *reinterpret_cast<uint4*>(qt + (c >> 3) * C::HALF + (((c & 7) ^ (r & 7)) << 4)) = v;
         }
         fence_proxy_async_smem();
         mbar_arrive(&q_ready[t]);
       }
-      float run_o[D], run_m = -INFINITY, run_l = 0.0f;
+      float run_m = -INFINITY, run_l = 0.0f;
       float m = -INFINITY, l = 0.0f;
       for (int b = 0; b < it.n_blocks; ++b) {
         const int second = it.tiles == 1 ? (b & 1) : 0;   // a one-tile item's second buffer
@@ -436,20 +461,24 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
         tc_fence_after();
         if (warp_live) {
           const uint32_t s_t0 = tmem + lane_base + C::S_COL + (sb ? 128 : 0);
-          float mx = -INFINITY;
+          float s[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_t0 + c * 32, s[c]);
+          tmem_ld_wait();
+          if (valid < kBlock) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) s[c][i] = (c * 32 + i < valid) ? s[c][i] : -INFINITY;
+          }
+          float mx4[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            float s[32];
-            tmem_ld_32x32b_x32(s_t0 + c * 32, s);
-            tmem_ld_wait();
-            if (valid < kBlock) {
+            mx4[c] = fmaxf(s[c][0], s[c][1]);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) s[i] = (c * 32 + i < valid) ? s[i] : -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, s[i]);
+            for (int i = 2; i < 32; i += 2) mx4[c] = fmaxf(mx4[c], fmaxf(s[c][i], s[c][i + 1]));
           }
-          mx = __fmul_rn(mx, p.c);
+          const float mx = __fmul_rn(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), p.c);
           float alpha = 1.0f;
           if (first) {
             m = mx;
@@ -462,104 +491,103 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
             // rescale the accumulator once the previous block's P.V is done
             if (!warp_wait(&o_full[t], (ocnt - 1) & 1, kDetOut, abort_flag)) break;
             tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < C::DP / 32; ++c) {
-              float o[32];
-              tmem_ld_32x32b_x32(o_t + c * 32, o);
+#pragma unroll 1
+            for (int c = 0; c < C::DP / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld_x16(o_t + c * 16, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __fmul_rn(o[i], alpha);
-              tmem_st_32x32b_x32(o_t + c * 32, o);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__fmul_rn(__uint_as_float(o[i]), alpha));
+              tmem_st_x16(o_t + c * 16, o);
             }
-            tmem_st_wait();
             l = __fmul_rn(l, alpha);
           }
           const float neg = (m == -INFINITY) ? 0.0f : -m;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const float2 c2 = make_float2(p.c, p.c), n2 = make_float2(neg, neg);
+          float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            float s[32];
-            tmem_ld_32x32b_x32(s_t0 + c * 32, s);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) s[i] = __fmaf_rn(s[i], p.c, neg);
-            if (valid < kBlock) {   // after the scale, which may be 0
-#pragma unroll
-              for (int i = 0; i < 32; ++i) s[i] = (c * 32 + i < valid) ? s[i] : -INFINITY;
-            }
             uint32_t pk[16];
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              const float e0 = exp2_hw(s[i]), e1 = exp2_hw(s[i + 1]);
-              sum[(i >> 1) & 3] = __fadd_rn(sum[(i >> 1) & 3], __fadd_rn(e0, e1));
-              pk[i >> 1] = pack2<T>(e0, e1);
+              float2 e = fma2(make_float2(s[c][i], s[c][i + 1]), c2, n2);
+              e.x = exp2_hw(e.x);
+              e.y = exp2_hw(e.y);
+              sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
+              pk[i >> 1] = pack2<T>(e.x, e.y);
             }
             tmem_st_x16(s_t0 + c * 16, pk);
           }
-          l = __fadd_rn(l, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
+          const float2 ps = add2(sum[0], sum[1]);
+          l = __fadd_rn(l, __fadd_rn(ps.x, ps.y));
           tmem_st_wait();
         }
         tc_fence_before();
         mbar_arrive(&p_ready[sb]);
         ++ocnt;
-        if ((b + 1) % p.chunk_blocks == 0 || b + 1 == it.n_blocks) {
-          // the chunk's state joins the run's
+        const bool last = b + 1 == it.n_blocks;
+        if ((b + 1) % p.chunk_blocks == 0 || last) {
+          // the chunk's state joins the run's, which leaves with the last chunk
           if (!warp_wait(&o_full[t], (ocnt - 1) & 1, kDetOut, abort_flag)) break;
           tc_fence_after();
           if (warp_live) {
             const bool head = b < p.chunk_blocks;   // the run's first chunk
-            float a = 0.0f, bb = 1.0f;
+            float wa = 0.0f, wb = 1.0f;
             if (head) {
               run_m = m;
               run_l = l;
             } else {
-              run_m = join_weights(run_m, m, a, bb);
-              run_l = join(run_l, a, l, bb);
+              run_m = join_weights(run_m, m, wa, wb);
+              run_l = join(run_l, wa, l, wb);
             }
+            const int64_t st0 = static_cast<int64_t>(it.run) * p.st_rows;
+            int64_t dst[4];
+            if (last) {
+              if (valid_row) {
+                const int64_t row = mrow / p.G;
+                const int64_t idx = st0 + row * p.hq + it.kvh * p.G + (mrow - row * p.G);
+                *reinterpret_cast<float2*>(p.st_ml + 2 * idx) = make_float2(run_m, run_l);
+              }
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              float o[32];
-              tmem_ld_32x32b_x32(o_t + c * 32, o);
+              for (int j = 0; j < 4; ++j) {   // rows this lane writes, 16 bytes of each a piece
+                const int64_t mm = m0 + (warp & 3) * 32 + j * 8 + (lane >> 2);
+                const int64_t row = mm / p.G;
+                dst[j] = mm < p.rg ? (st0 + row * p.hq + it.kvh * p.G + (mm - row * p.G)) * D + (lane & 3) * 4 : -1;
+              }
+            }
+            const uint32_t r_t = tmem + lane_base + C::R_COL + t * C::DP;
+#pragma unroll 2
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16], r[16];
+              tmem_ld_x16(o_t + c * 16, o);
+              if (C::GROUPED && !head) tmem_ld_x16(r_t + c * 16, r);
               tmem_ld_wait();
+              if (C::GROUPED && !head) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) run_o[c * 32 + i] = head ? o[i] : join(run_o[c * 32 + i], a, o[i], bb);
+                for (int i = 0; i < 16; ++i)
+                  o[i] = __float_as_uint(join(__uint_as_float(r[i]), wa, __uint_as_float(o[i]), wb));
+              }
+              if (C::GROUPED && !last) {
+                tmem_st_x16(r_t + c * 16, o);
+              } else {
+                // transposed, so that a row's 64 bytes leave together
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  *reinterpret_cast<uint4*>(tb + lane * C::TPAD + i * 4) =
+                      make_uint4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const float4 v = *reinterpret_cast<const float4*>(tb + (j * 8 + (lane >> 2)) * C::TPAD + (lane & 3) * 4);
+                  if (dst[j] >= 0) *reinterpret_cast<float4*>(p.st_o + dst[j] + c * 16) = v;
+                }
+              }
             }
+            if (C::GROUPED && !last) tmem_st_wait();
           }
           tc_fence_before();
           mbar_arrive(&o_free[t]);
-        }
-      }
-      if (abort_flag) break;
-      if (warp_live) {
-        // the run's state, transposed 16 columns at a time so that a row's 64 bytes leave together
-        const int64_t st0 = static_cast<int64_t>(it.run) * p.st_rows;
-        const int64_t wm0 = m0 + (warp & 3) * 32;
-        if (valid_row) {
-          const int64_t row = mrow / p.G;
-          const int64_t idx = st0 + row * p.hq + it.kvh * p.G + (mrow - row * p.G);
-          *reinterpret_cast<float2*>(p.st_ml + 2 * idx) = make_float2(run_m, run_l);
-        }
-        int64_t dst[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int64_t mm = wm0 + j * 8 + (lane >> 2);
-          const int64_t row = mm / p.G;
-          dst[j] = mm < p.rg ? (st0 + row * p.hq + it.kvh * p.G + (mm - row * p.G)) * D + (lane & 3) * 4 : -1;
-        }
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<float4*>(tb + lane * C::TPAD + i * 4) =
-                make_float4(run_o[c * 16 + i * 4], run_o[c * 16 + i * 4 + 1], run_o[c * 16 + i * 4 + 2],
-                            run_o[c * 16 + i * 4 + 3]);
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 v = *reinterpret_cast<const float4*>(tb + (j * 8 + (lane >> 2)) * C::TPAD + (lane & 3) * 4);
-            if (dst[j] >= 0) *reinterpret_cast<float4*>(p.st_o + dst[j] + c * 16) = v;
-          }
         }
       }
     }
@@ -573,36 +601,49 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
   }
 }
 
-// out[row, head] = O / l of the joined states: the prefix's runs (kGroup chunks at a time when a run
-// is a chunk), then the row's own tokens.  One warp a (row, head).
+// out[row, head] = O / l of the joined states: the prefix's runs (per_group of them at a time), then
+// the row's own tokens (own_splits states, or one where a warp joined them all).  One warp a (row,
+// head), UN states in flight.
 constexpr int kCombineWarps = 4;
 
+struct CombineParams {
+  const float* st_o;
+  const float* st_ml;
+  int n_runs, per_group;
+  const int32_t* kv_lens;   // null: no row has tokens of its own
+  int own_max;              // states the own tokens may have: 1 (joined already) or the split limit
+  int64_t st_rows;
+  int hq;
+  void* out;
+  int64_t o_sr, o_sh;
+};
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const float* st_o, const float* st_ml,
-                                                                     int n_runs, int per_group, bool own,
-                                                                     int64_t st_rows, int hq, T* out, int64_t o_sr,
-                                                                     int64_t o_sh) {
+__global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const CombineParams p) {
   constexpr int V = D / 32;
   constexpr int UN = 8;
   pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int64_t m = static_cast<int64_t>(blockIdx.x) * kCombineWarps + (threadIdx.x >> 5);
-  if (m >= st_rows) return;
+  if (m >= p.st_rows) return;
+  const int64_t row = m / p.hq;
+  int n_own = 0;
+  if (p.kv_lens) n_own = min(max((p.kv_lens[row] + own::kSplit - 1) / own::kSplit, 0), p.own_max);
+  const int n = p.n_runs + n_own;
   float tm = -INFINITY, tl = 0.0f, to[V];   // the groups joined so far
   float gm = -INFINITY, gl = 0.0f, go[V];   // the open group
 #pragma unroll
   for (int i = 0; i < V; ++i) to[i] = go[i] = 0.0f;
-  const int n = n_runs + (own ? 1 : 0);
   for (int s0 = 0; s0 < n; s0 += UN) {
     float2 ml[UN];
     float o[UN][V];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       if (s0 + u < n) {
-        const int64_t idx = (s0 + u) * st_rows + m;
-        ml[u] = __ldcg(reinterpret_cast<const float2*>(st_ml + 2 * idx));
-        const float* src = st_o + idx * D + lane * V;
+        const int64_t idx = (s0 + u) * p.st_rows + m;
+        ml[u] = __ldcg(reinterpret_cast<const float2*>(p.st_ml + 2 * idx));
+        const float* src = p.st_o + idx * D + lane * V;
         if constexpr (V == 4) {
           const float4 f = __ldcg(reinterpret_cast<const float4*>(src));
           o[u][0] = f.x;
@@ -622,39 +663,34 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const float
     for (int u = 0; u < UN; ++u) {
       const int s = s0 + u;
       if (s < n) {
-        const bool mine = s == n_runs;               // the row's own tokens: a group of one
-        const int in_group = mine ? 0 : s % per_group;
-        if (in_group == 0) {
+        const bool head = s < p.n_runs ? s % p.per_group == 0 : s == p.n_runs;
+        const bool tail = s < p.n_runs ? (s + 1) % p.per_group == 0 || s + 1 == p.n_runs : s + 1 == n;
+        float a = 0.0f, b = 1.0f;
+        if (head) {
           gm = ml[u].x;
           gl = ml[u].y;
-#pragma unroll
-          for (int i = 0; i < V; ++i) go[i] = o[u][i];
         } else {
-          float a, b;
           gm = join_weights(gm, ml[u].x, a, b);
           gl = join(gl, a, ml[u].y, b);
-#pragma unroll
-          for (int i = 0; i < V; ++i) go[i] = join(go[i], a, o[u][i], b);
         }
-        if (mine || in_group == per_group - 1 || s == n_runs - 1) {
-          if (!mine && s < per_group) {   // the first group
+#pragma unroll
+        for (int i = 0; i < V; ++i) go[i] = head ? o[u][i] : join(go[i], a, o[u][i], b);
+        if (tail) {
+          const bool only = s < p.per_group && s < p.n_runs;   // the first group
+          if (only) {
             tm = gm;
             tl = gl;
-#pragma unroll
-            for (int i = 0; i < V; ++i) to[i] = go[i];
           } else {
-            float a, b;
             tm = join_weights(tm, gm, a, b);
             tl = join(tl, a, gl, b);
-#pragma unroll
-            for (int i = 0; i < V; ++i) to[i] = join(to[i], a, go[i], b);
           }
+#pragma unroll
+          for (int i = 0; i < V; ++i) to[i] = only ? go[i] : join(to[i], a, go[i], b);
         }
       }
     }
   }
-  const int64_t row = m / hq;
-  T* dst = out + row * o_sr + (m - row * hq) * o_sh + lane * V;
+  T* dst = static_cast<T*>(p.out) + row * p.o_sr + (m - row * p.hq) * p.o_sh + lane * V;
 #pragma unroll
   for (int i = 0; i < V; ++i) dst[i] = from_f32<T>(__fdiv_rn(to[i], tl));
 }

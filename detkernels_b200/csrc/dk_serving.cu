@@ -1,6 +1,5 @@
 // C ABI of the serving operators (see include/detkernels_b200.h): the page plan of a step, the
 // per-head norm with rotation into a KV cache, and attention over a shared prefix.
-#include "dk_attention_state.h"
 #include "dk_common.cuh"
 #include "dk_host.cuh"
 #include "dk_paging.cuh"
@@ -86,28 +85,48 @@ int rope_launch(dk::rope::Params& p, cudaStream_t st) {
 struct PrefixPlan {
   int64_t rg;           // rows * G
   int chunk_blocks, n_chunks, run_blocks, n_runs, n_pairs, per_group;
+  int max_splits, spu, upt, own_states;   // own tokens: splits a row, splits a unit, units a (tile, head), states a row
 };
 
-// Chunk or whole group a run (schedule only, the bits are the same): whole groups when they give
-// most SMs an item, else chunks, whose states then travel through the workspace.
-PrefixPlan plan_prefix(int64_t n_rows, int64_t hkv, int64_t G, int64_t prefix_len) {
+// Schedule (the bits are the same for every choice).  Prefix: a whole group of chunks a run when that
+// gives most SMs an item, else a chunk a run, whose states then travel through memory.  Own tokens: all
+// splits of a (tile, KV head) by one warp when there are three waves of those, else enough units for
+// three waves.
+PrefixPlan plan_prefix(int64_t n_rows, int64_t n_tiles, int64_t hkv, int64_t G, int64_t head_dim, int64_t prefix_len,
+                       int64_t max_kv_len) {
   PrefixPlan pl{};
+  const int sms = sm_count(current_device());
   pl.rg = n_rows * G;
-  pl.chunk_blocks = static_cast<int>(dk::prefix::chunk_tokens(prefix_len) / dk::prefix::kBlock);
+  pl.chunk_blocks = static_cast<int>(dk::prefix::chunk_tokens(prefix_len, static_cast<int>(head_dim)) /
+                                     dk::prefix::kBlock);
   const int64_t blocks = ceil_div(prefix_len, dk::prefix::kBlock);
   pl.n_chunks = static_cast<int>(ceil_div(blocks, pl.chunk_blocks));
   pl.n_pairs = static_cast<int>(ceil_div(pl.rg, 2 * dk::prefix::kRows));
-  const int64_t groups = ceil_div(pl.n_chunks, dk::prefix::kGroup);
-  const bool whole = 4 * groups * pl.n_pairs * hkv >= 3LL * sm_count(current_device());
-  pl.run_blocks = pl.chunk_blocks * (whole ? dk::prefix::kGroup : 1);
+  const int gc = dk::prefix::group_chunks(static_cast<int>(head_dim));
+  const int64_t groups = ceil_div(pl.n_chunks, gc);
+  const bool whole = gc == 1 || 4 * groups * pl.n_pairs * hkv >= 3LL * sms;
+  pl.run_blocks = pl.chunk_blocks * (whole ? gc : 1);
   pl.n_runs = static_cast<int>(whole ? groups : pl.n_chunks);
-  pl.per_group = whole ? 1 : dk::prefix::kGroup;
+  pl.per_group = whole ? 1 : gc;
+  pl.max_splits = static_cast<int>(ceil_div(max_kv_len, dk::own::kSplit));
+  if (pl.max_splits > 0) {
+    const int64_t units = n_tiles * hkv;
+    const int64_t target = 3LL * (head_dim == 128 ? 9 : 14) * sms;
+    int64_t upt = units >= target ? 1 : ceil_div(target, units);
+    if (upt > pl.max_splits) upt = pl.max_splits;
+    pl.spu = static_cast<int>(ceil_div(pl.max_splits, upt));
+    pl.upt = static_cast<int>(ceil_div(pl.max_splits, pl.spu));
+    pl.own_states = pl.upt == 1 ? 1 : pl.max_splits;
+  }
   return pl;
 }
 
+size_t state_o_bytes(const PrefixPlan& pl, int64_t st_rows, int64_t D) {
+  const size_t states = static_cast<size_t>(pl.n_runs + pl.own_states) * st_rows;
+  return (states * D * sizeof(float) + 255) / 256 * 256;
+}
 size_t prefix_state_bytes(const PrefixPlan& pl, int64_t st_rows, int64_t D) {
-  const size_t states = static_cast<size_t>(pl.n_runs + 1) * st_rows;   // + the rows' own tokens
-  return (states * D * sizeof(float) + 255) / 256 * 256 + states * 2 * sizeof(float);
+  return state_o_bytes(pl, st_rows, D) + static_cast<size_t>(pl.n_runs + pl.own_states) * st_rows * 2 * sizeof(float);
 }
 
 template <typename T, int D>
@@ -136,14 +155,30 @@ int prefix_launch(const dk::prefix::Maps& maps, const dk::prefix::Params& p, cud
   return DK_OK;
 }
 
+// Follows prefix_launch on the same stream and starts without waiting for it: prefix_kernel has itself
+// waited for whatever wrote the inputs before it lets the next kernel begin.
 template <typename T, int D>
-int combine_launch(const dk::prefix::Params& p, const PrefixPlan& pl, bool own, void* out, int64_t o_sr, int64_t o_sh,
-                   cudaStream_t st) {
+int own_launch(const dk::own::Params& p, cudaStream_t st) {
+  using C = dk::own::Cfg<D>;
+  auto fn = dk::own::own_kernel<T, D>;
+  static bool done[kMaxDevices] = {false};
+  const int dev = current_device();
+  if (dev < 0 || dev >= kMaxDevices || !done[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+    if (e != cudaSuccess) return fail(DK_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    if (dev >= 0 && dev < kMaxDevices) done[dev] = true;
+  }
+  const int64_t grid = static_cast<int64_t>(p.n_tiles) * p.upt * p.hkv;
+  cudaError_t e = launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(32), C::SMEM, st, p);
+  if (e != cudaSuccess) return fail(DK_ERR_CUDA, "attention_shared_prefix: launch failed: %s", cudaGetErrorString(e));
+  return DK_OK;
+}
+
+template <typename T, int D>
+int combine_launch(const dk::prefix::CombineParams& p, cudaStream_t st) {
   const int64_t grid = ceil_div(p.st_rows, dk::prefix::kCombineWarps);
   cudaError_t e = launch_pdl(dk::prefix::combine_kernel<T, D>, dim3(static_cast<unsigned>(grid)),
-                             dim3(dk::prefix::kCombineWarps * 32), 0, st, static_cast<const float*>(p.st_o),
-                             static_cast<const float*>(p.st_ml), pl.n_runs, pl.per_group, own, p.st_rows, p.hq,
-                             static_cast<T*>(out), o_sr, o_sh);
+                             dim3(dk::prefix::kCombineWarps * 32), 0, st, p);
   if (e != cudaSuccess) return fail(DK_ERR_CUDA, "attention_shared_prefix: launch failed: %s", cudaGetErrorString(e));
   return DK_OK;
 }
@@ -272,12 +307,14 @@ int dk_qk_norm_rope(const void* q, int64_t q_stride_row, int64_t q_stride_head, 
   return rope_launch<__nv_bfloat16>(p, st);
 }
 
-size_t dk_attention_prefix_state_size(int64_t n_rows, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
-                                      int64_t prefix_len) {
-  if (n_rows <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads || head_dim <= 0 || prefix_len <= 0)
+size_t dk_attention_shared_prefix_workspace_size(int32_t n_rows, int32_t n_tiles, int32_t n_q_heads, int32_t n_kv_heads,
+                                      int32_t head_dim, int32_t prefix_len, int32_t max_kv_len) {
+  if (n_rows <= 0 || n_tiles <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads || head_dim <= 0 ||
+      prefix_len <= 0 || max_kv_len < 0)
     return 0;
-  return prefix_state_bytes(plan_prefix(n_rows, n_kv_heads, n_q_heads / n_kv_heads, prefix_len), n_rows * n_q_heads,
-                            head_dim);
+  return prefix_state_bytes(plan_prefix(n_rows, n_tiles, n_kv_heads, n_q_heads / n_kv_heads, head_dim, prefix_len,
+                                        max_kv_len),
+                            static_cast<int64_t>(n_rows) * n_q_heads, head_dim);
 }
 
 int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_stride_head, const void* k_prefix,
@@ -290,8 +327,7 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
                                int64_t out_stride_row, int64_t out_stride_head, const int32_t* kv_lens,
                                const int32_t* row_tiles, int32_t n_tiles, int32_t n_rows, int32_t n_q_heads,
                                int32_t n_kv_heads, int32_t head_dim, int32_t max_kv_len, float scale, int dtype,
-                               void* state, size_t state_bytes, void* workspace, size_t workspace_bytes,
-                               void* stream) {
+                               void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "attention_shared_prefix";
   if (dtype != DK_BF16 && dtype != DK_F16) return fail(DK_ERR_UNSUPPORTED, "%s: dtype must be bf16 or f16", what);
   if (head_dim != 32 && head_dim != 64 && head_dim != 128)
@@ -299,7 +335,7 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
   if (n_rows < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || n_kv_heads > 65535)
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: bad head counts", what);
   const int G = n_q_heads / n_kv_heads;
-  if (G > 16) return fail(DK_ERR_UNSUPPORTED, "%s: more than 16 query heads per kv head", what);
+  if (G > dk::own::kRows) return fail(DK_ERR_UNSUPPORTED, "%s: more than 16 query heads per kv head", what);
   if (prefix_len <= 0) return fail(DK_ERR_INVALID_ARGUMENT, "%s: prefix_len must be positive", what);
   if (max_kv_len < 0) return fail(DK_ERR_INVALID_ARGUMENT, "%s: max_kv_len < 0", what);
   if (n_rows == 0) return DK_OK;
@@ -311,14 +347,36 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: the prefix needs 16-byte aligned rows", what);
   if (prefix_blocks && (prefix_page <= 0 || prefix_page % 64 || prefix_pool_blocks <= 0 || prefix_pool_blocks > kI32Max))
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: a paged prefix needs a page size that is a multiple of 64", what);
+  const bool own = max_kv_len > 0;
+  if (own) {
+    if (!k || !v || !kv_lens) return fail(DK_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+    if (!aligned16(k) || !aligned16(v) || kv_stride_seq % 8 || kv_stride_head % 8 || kv_stride_tok % 8)
+      return fail(DK_ERR_INVALID_ARGUMENT, "%s: the caches need 16-byte aligned rows", what);
+    if (block_table) {
+      if (page_size <= 0 || page_size % 64 || blocks_per_seq <= 0 || n_blocks <= 0 || n_blocks > kI32Max ||
+          block_table_stride < blocks_per_seq)
+        return fail(DK_ERR_INVALID_ARGUMENT,
+                    "%s: a paged cache needs page_size a multiple of 64, blocks_per_seq > 0, n_blocks > 0 and "
+                    "block_table_stride >= blocks_per_seq", what);
+      kv_capacity = static_cast<int64_t>(page_size) * blocks_per_seq;
+    }
+    if (kv_capacity <= 0 || kv_n_seq <= 0 || kv_capacity > kI32Max || kv_n_seq > kI32Max)
+      return fail(DK_ERR_INVALID_ARGUMENT, "%s: bad KV extents", what);
+    if (!row_tiles && kv_n_seq < n_rows) return fail(DK_ERR_INVALID_ARGUMENT, "%s: fewer KV sequences than rows", what);
+  }
+  if (!row_tiles) n_tiles = n_rows;
+  if (n_tiles <= 0) return fail(DK_ERR_INVALID_ARGUMENT, "%s: n_tiles must be positive with row_tiles", what);
   const int64_t st_rows = static_cast<int64_t>(n_rows) * n_q_heads;
-  const PrefixPlan pl = plan_prefix(n_rows, n_kv_heads, G, prefix_len);
-  if (ceil_div(st_rows, dk::prefix::kCombineWarps) > kI32Max)
+  const PrefixPlan pl = plan_prefix(n_rows, n_tiles, n_kv_heads, G, head_dim, prefix_len, max_kv_len);
+  if (ceil_div(st_rows, dk::prefix::kCombineWarps) > kI32Max ||
+      static_cast<int64_t>(n_tiles) * n_kv_heads * (pl.upt > 0 ? pl.upt : 1) > kI32Max)
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: too many rows", what);
   const size_t need = prefix_state_bytes(pl, st_rows, head_dim);
-  if (!state || state_bytes < need || !aligned16(state))
-    return fail(DK_ERR_WORKSPACE, "%s: state scratch of %zu bytes needed, %zu given", what, need, state_bytes);
+  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+    return fail(DK_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
 
+  float* st_o = static_cast<float*>(workspace);
+  float* st_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + state_o_bytes(pl, st_rows, head_dim));
   dk::prefix::Params p{};
   p.q = q;
   p.q_sr = q_stride_row;
@@ -335,13 +393,12 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
   p.blocks = prefix_blocks;
   p.page = prefix_blocks ? prefix_page : 0;
   p.n_blocks = prefix_blocks ? static_cast<int32_t>(prefix_pool_blocks) : 0;
-  p.c = fabsf(scale) * 1.4426950408889634f;
+  p.zero = scale == 0.0f ? 1 : 0;
+  p.c = (p.zero ? 1.0f : fabsf(scale)) * 1.4426950408889634f;
   p.flip = scale < 0.0f ? 0x80008000u : 0u;
   p.st_rows = st_rows;
-  p.st_o = static_cast<float*>(state);
-  p.st_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(state) +
-                                     (static_cast<size_t>(pl.n_runs + 1) * st_rows * head_dim * sizeof(float) + 255) /
-                                         256 * 256);
+  p.st_o = st_o;
+  p.st_ml = st_ml;
 
   // K/V prefix maps: (d, token, kv head, block); a contiguous prefix is one block of prefix_len tokens,
   // so that what lies behind it reads as zero
@@ -361,26 +418,61 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
   if (rc) return rc;
 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define DK_PREFIX_DISPATCH(FN, ...)                                                            \
+#define DK_DISPATCH_16(FN, ...)                                                                \
   (dtype == DK_BF16 ? (head_dim == 32   ? FN<__nv_bfloat16, 32>(__VA_ARGS__)                   \
                        : head_dim == 64 ? FN<__nv_bfloat16, 64>(__VA_ARGS__)                   \
                                         : FN<__nv_bfloat16, 128>(__VA_ARGS__))                 \
                     : (head_dim == 32   ? FN<__half, 32>(__VA_ARGS__)                          \
                        : head_dim == 64 ? FN<__half, 64>(__VA_ARGS__)                          \
                                         : FN<__half, 128>(__VA_ARGS__)))
-  rc = DK_PREFIX_DISPATCH(prefix_launch, maps, p, st);
+  rc = DK_DISPATCH_16(prefix_launch, maps, p, st);
   if (rc) return rc;
-  const bool own = max_kv_len > 0;
   if (own) {
-    const PagedKV pg{block_table, block_table_stride, page_size, blocks_per_seq, n_blocks};
-    const int64_t at = static_cast<int64_t>(pl.n_runs) * st_rows;
-    rc = attention_state(q, q_stride_row, q_stride_head, k, v, kv_stride_seq, kv_stride_head, kv_stride_tok, kv_n_seq,
-                         kv_capacity, kv_lens, row_tiles, n_tiles, n_rows, n_q_heads, n_kv_heads, head_dim, max_kv_len,
-                         scale, dtype, workspace, workspace_bytes, stream, block_table ? &pg : nullptr, what,
-                         p.st_o + at * head_dim, p.st_ml + at * 2);
+    dk::own::Params o{};
+    o.q = q;
+    o.q_sr = q_stride_row;
+    o.q_sh = q_stride_head;
+    o.k = k;
+    o.v = v;
+    o.c_sn = kv_stride_seq;
+    o.c_sh = kv_stride_head;
+    o.c_st = kv_stride_tok;
+    o.kv_lens = kv_lens;
+    o.tiles = row_tiles;
+    o.n_tiles = n_tiles;
+    o.n_rows = n_rows;
+    o.hq = n_q_heads;
+    o.hkv = n_kv_heads;
+    o.G = G;
+    o.n_seq = static_cast<int32_t>(kv_n_seq);
+    o.capacity = static_cast<int32_t>(kv_capacity < max_kv_len ? kv_capacity : max_kv_len);
+    o.block_table = block_table;
+    o.bt_stride = block_table_stride;
+    o.page = block_table ? page_size : 0;
+    o.n_blocks = static_cast<int32_t>(n_blocks);
+    o.max_splits = pl.max_splits;
+    o.spu = pl.spu;
+    o.upt = pl.upt;
+    o.scale_log2 = scale * 1.4426950408889634f;
+    o.st_rows = st_rows;
+    o.st_o = st_o + static_cast<int64_t>(pl.n_runs) * st_rows * head_dim;
+    o.st_ml = st_ml + static_cast<int64_t>(pl.n_runs) * st_rows * 2;
+    rc = DK_DISPATCH_16(own_launch, o, st);
     if (rc) return rc;
   }
-  return DK_PREFIX_DISPATCH(combine_launch, p, pl, own, out, out_stride_row, out_stride_head, st);
+  dk::prefix::CombineParams c{};
+  c.st_o = st_o;
+  c.st_ml = st_ml;
+  c.n_runs = pl.n_runs;
+  c.per_group = pl.per_group;
+  c.kv_lens = own ? kv_lens : nullptr;
+  c.own_max = pl.own_states;
+  c.st_rows = st_rows;
+  c.hq = n_q_heads;
+  c.out = out;
+  c.o_sr = out_stride_row;
+  c.o_sh = out_stride_head;
+  return DK_DISPATCH_16(combine_launch, c, st);
 }
 
 }  // extern "C"

@@ -243,7 +243,9 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
     holds prefix token t.  prefix_len defaults to all of it; 0 is plain ``attention_decode``.
     k_cache, v_cache, kv_lens, block_table, max_kv_len: as in ``attention_decode`` (kv_lens and
     max_kv_len count the rows' own tokens only).  bf16 or f16; head_dim 32, 64 or 128; at most 16 query
-    heads per KV head.
+    heads per KV head.  workspace: uint8 CUDA tensor of at least
+    ``dk_attention_shared_prefix_workspace_size`` bytes (a new one if not given; its contents do not
+    matter, and calls that may overlap need separate ones).
 
     A row's bits depend on its q, the prefix, its own tokens and nothing else of the batch."""
     import torch
@@ -303,23 +305,20 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
     with torch.cuda.device(q.device):
         if P == 0:
             return attention_decode(q, k_cache, v_cache, kv_lens, scale=scale, row_tiles=row_tiles,
-                                    max_kv_len=max_kv_len, out=out, workspace=workspace, block_table=block_table)
+                                    max_kv_len=max_kv_len, out=out, block_table=block_table)
         ps, vps = _tma_strides(k_prefix, "k_prefix"), _tma_strides(v_prefix, "v_prefix")
         assert ps == vps, "k and v prefixes must share strides"
         cs = [0, 0, 0, 1]
-        n_tiles, rows_per_tile = (R, 1) if row_tiles is None else (row_tiles.shape[0], 2)
-        lib = _lib.load()
-        stream = _lib.stream_ptr(q.device)
+        n_tiles = R if row_tiles is None else row_tiles.shape[0]
         if max_kv_len:
             cs, cvs = _tma_strides(k_cache, "k_cache"), _tma_strides(v_cache, "v_cache")
             assert cs == cvs, "k and v caches must share strides"
             if uniform:
                 kv_lens = torch.full((R,), kv_lens, dtype=torch.int32, device=q.device)
-            if workspace is None:
-                workspace = _lib.call_workspace(
-                    lib.dk_attention_workspace_size(n_tiles, rows_per_tile, H, Hkv, D, max_kv_len), q.device, stream)
-        nbytes = lib.dk_attention_prefix_state_size(R, H, Hkv, D, P)
-        state = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+        lib = _lib.load()
+        nbytes = lib.dk_attention_shared_prefix_workspace_size(R, n_tiles, H, Hkv, D, P, max_kv_len)
+        if workspace is None:
+            workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
         rc = lib.dk_attention_shared_prefix(
             q.data_ptr(), q.stride(0), q.stride(1), k_prefix.data_ptr(), v_prefix.data_ptr(),
             ps[0] if prefix_blocks is not None else 0, ps[-3], ps[-2], P,
@@ -328,9 +327,7 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
             block_table.data_ptr() if block_table is not None else None, bt_stride, width, n_blocks, page,
             out.data_ptr(), out.stride(0), out.stride(1), None if uniform and not max_kv_len else kv_lens.data_ptr(),
             row_tiles.data_ptr() if row_tiles is not None else None, n_tiles, R, H, Hkv, D, max_kv_len, float(scale),
-            _lib.dtype_code(q.dtype), state.data_ptr(), state.numel(),
-            workspace.data_ptr() if workspace is not None else None,
-            workspace.numel() if workspace is not None else 0, stream)
+            _lib.dtype_code(q.dtype), workspace.data_ptr(), workspace.numel(), _lib.stream_ptr(q.device))
     _lib.check(rc, "attention_shared_prefix")
     _lib.count_launch(3 if max_kv_len else 2)
     return out

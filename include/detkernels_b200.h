@@ -380,19 +380,22 @@ int dk_qk_norm_rope(const void* q, int64_t q_stride_row, int64_t q_stride_head, 
                     int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t rotary_dim, int interleaved,
                     float eps, int dtype, void* stream);
 
-/* Scratch bytes of the prefix states of dk_attention_shared_prefix (uninitialised memory will do). */
-size_t dk_attention_prefix_state_size(int64_t n_rows, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
-                                      int64_t prefix_len);
+/* Workspace bytes of dk_attention_shared_prefix (uninitialised memory will do; no counters).  n_tiles =
+ * n_rows without row_tiles. */
+size_t dk_attention_shared_prefix_workspace_size(int32_t n_rows, int32_t n_tiles, int32_t n_q_heads, int32_t n_kv_heads,
+                                      int32_t head_dim, int32_t prefix_len, int32_t max_kv_len);
 /* Decode attention of rows that share a prefix: row r attends to the prefix_len prefix tokens and then
  * to tokens [0, kv_len_r) of its own KV sequence, the prefix part computed once for all rows.
  * The prefix: k_prefix / v_prefix [n_kv_heads, prefix_len, head_dim] (prefix_stride_head / _tok), or,
  * with prefix_blocks (device int32[ceil(prefix_len / prefix_page)]), block pools [prefix_pool_blocks,
  * n_kv_heads, prefix_page, head_dim] whose block prefix_blocks[t / prefix_page] holds token t (a block id
  * outside the pool: DK_ERR_DEVICE_CHECK, detail 0x62a).  prefix_page is a multiple of 64.
- * The rows' own tokens: q, k, v, kv_lens, row_tiles, max_kv_len, scale, workspace as in
+ * The rows' own tokens: q, k, v, kv_lens, row_tiles, max_kv_len, scale as in
  * dk_attention_batch_invariant, or with block_table as in dk_attention_paged_batch_invariant
- * (kv_stride_seq is then the block stride); max_kv_len = 0: no row has any, and k, v and kv_lens are not
- * read.  q must be 16-byte aligned with strides that are multiples of 8 elements.
+ * (kv_stride_seq is then the block stride); max_kv_len = 0: no row has any, and k, v, kv_lens and
+ * row_tiles are not read.  A length beyond max_kv_len or the cache (detail 0x210), a malformed tile (0x211)
+ * or a block id outside the pool (0x212) is recorded as DK_ERR_DEVICE_CHECK.  Nothing beyond a row's own
+ * length reaches it, whatever the cache holds there.  q must be 16-byte aligned with strides that are multiples of 8 elements.
  * Batch invariant: a row's bits follow from its q, the prefix and its own tokens. */
 int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_stride_head, const void* k_prefix,
                                const void* v_prefix, int64_t prefix_stride_block, int64_t prefix_stride_head,
@@ -404,8 +407,7 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
                                int64_t out_stride_row, int64_t out_stride_head, const int32_t* kv_lens,
                                const int32_t* row_tiles, int32_t n_tiles, int32_t n_rows, int32_t n_q_heads,
                                int32_t n_kv_heads, int32_t head_dim, int32_t max_kv_len, float scale, int dtype,
-                               void* state, size_t state_bytes, void* workspace, size_t workspace_bytes,
-                               void* stream);
+                               void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -91,11 +91,11 @@ def test_refusals_on_the_host():
         attention_shared_prefix(z, z, z, z[None], z[None], 1)
     lib = _lib.load()
 
-    def call(dtype=_lib.DK_BF16, D=64, H=4, Hkv=2, P=10, pb=None, pool=0, pg=0, qs=512, q=16, state=16, state_bytes=0,
-             max_len=0, pst=64):
+    def call(dtype=_lib.DK_BF16, D=64, H=4, Hkv=2, P=10, pb=None, pool=0, pg=0, qs=512, q=16, max_len=0, pst=64,
+             cst=64, n_seq=3, table=None, page=0, width=1):
         return lib.dk_attention_shared_prefix(
-            q, qs, D, 16, 16, 0, 640, pst, P, pb, pool, pg, 16, 16, 0, 0, 0, 1, 64, None, 0, 0, 0, 0, 16, qs, D, None,
-            None, 0, 3, H, Hkv, D, max_len, 0.1, dtype, state, state_bytes, None, 0, None)
+            q, qs, D, 16, 16, 0, 640, pst, P, pb, pool, pg, 16, 16, 0, 0, cst, n_seq, 64, table, width, width, 4, page,
+            16, qs, D, 16, None, 0, 3, H, Hkv, D, max_len, 0.1, dtype, 16, 0, None)
     assert call(dtype=_lib.DK_F32) == _lib.DK_ERR_UNSUPPORTED
     assert call(D=96) == _lib.DK_ERR_UNSUPPORTED and call(H=34) == _lib.DK_ERR_UNSUPPORTED
     assert call(H=5) == _lib.DK_ERR_INVALID_ARGUMENT and call(P=0) == _lib.DK_ERR_INVALID_ARGUMENT
@@ -103,9 +103,12 @@ def test_refusals_on_the_host():
     assert call(q=8) == _lib.DK_ERR_INVALID_ARGUMENT and call(qs=260) == _lib.DK_ERR_INVALID_ARGUMENT
     assert call(pst=68) == _lib.DK_ERR_INVALID_ARGUMENT
     assert call(pb=16, pool=4, pg=96) == _lib.DK_ERR_INVALID_ARGUMENT
+    assert call(max_len=9, cst=4) == _lib.DK_ERR_INVALID_ARGUMENT
+    assert call(max_len=9, n_seq=2) == _lib.DK_ERR_INVALID_ARGUMENT and "fewer KV sequences" in _lib.last_error()
+    assert call(max_len=9, table=16, page=32) == _lib.DK_ERR_INVALID_ARGUMENT
     assert call() == _lib.DK_ERR_WORKSPACE and "bytes needed" in _lib.last_error()
     # room for the chunk states of every (row, head) and for the rows' own tokens
-    assert lib.dk_attention_prefix_state_size(3, 4, 2, 64, 1025) >= 4 * 3 * 4 * (64 + 2) * 4
+    assert lib.dk_attention_shared_prefix_workspace_size(3, 3, 4, 2, 64, 1025, 600) >= (3 + 3) * 3 * 4 * (64 + 2) * 4
 
 
 def test_reference_joins_prefix_and_own_tokens():
@@ -211,6 +214,53 @@ def test_a_row_does_not_depend_on_its_batch(dev, H, Hkv, D, P):
         assert torch.equal(_call(q[lo:hi], part, lens[lo:hi]), full[lo:hi])
     again = _call(q, kw, lens)
     assert torch.equal(again, full)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D,page", [("bf16", 64, 64), ("f16", 128, 0), ("bf16", 32, 128)])
+def test_values_behind_a_rows_end_never_reach_it(dev, dt, D, page):
+    """Prefill rows whose later tokens hold infinities and NaN, and cache rows with NaN behind the end: each
+    row's bits are those of a call that only has its own tokens."""
+    import torch
+    lens, H, Hkv = [37, 5], 4, 2
+    q0, kp, vp, own, kw = _make(dev, _dt(dt), 2, H, Hkv, D, 150, lens, page, seed=6)
+    rows = sum(lens)
+    q = torch.randn(rows, H, D, device=dev, generator=torch.Generator(device=dev).manual_seed(8)).to(_dt(dt))
+    q_lens = [i + 1 for n in lens for i in range(n)]
+    tiles = torch.from_numpy(_tiles(lens, 16 // (H // Hkv))).to(dev)
+    want = _call(q, kw, q_lens, row_tiles=tiles)
+    kc, vc = (x.clone() for x in kw["kv"])
+    for t, bad in ((20, float("inf")), (21, float("nan")), (30, -float("inf"))):
+        if page:
+            b = int(kw["kwargs"]["block_table"][0, t // page])
+            vc[b, :, t % page, 3], kc[b, :, t % page, 1] = bad, float("nan")
+        else:
+            vc[0, :, t, 3], kc[0, :, t, 1] = bad, float("nan")
+            vc[:, :, 37:], kc[:, :, 37:] = float("nan"), float("nan")
+    kw2 = dict(kw, kv=(kc, vc))
+    if page:
+        kw2["prefix"] = kw["prefix"]
+    got = _call(q, kw2, q_lens, row_tiles=tiles)
+    fine = [r for r in range(rows) if r < 20 or r >= 37]
+    assert torch.equal(got[fine], want[fine]) and torch.isfinite(got[fine].float()).all()
+    assert torch.isnan(got[21:37].float()).any(-1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,H,Hkv,D,page", [(2, 4, 1, 64, 64), (3, 2, 2, 128, 0), (1, 16, 1, 128, 256), (700, 2, 1, 32, 0)])
+def test_long_own_sequences(dev, R, H, Hkv, D, page):
+    """Own tokens over many splits, by one warp (many rows) or many (few rows): one definition, the same bits."""
+    import torch
+    rng = np.random.default_rng(R)
+    lens = [int(x) for x in rng.integers(0, 1300 if R > 100 else 5000, size=R)]
+    lens[0] = 1025
+    q, kp, vp, own, kw = _make(dev, torch.bfloat16, R, H, Hkv, D, 77, lens, page, seed=R)
+    out = _call(q, kw, lens)
+    some = list(range(min(R, 3)))
+    _tol_check(out[some], q[some], kp, vp, [own[i][0] for i in some], [own[i][1] for i in some], D ** -0.5)
+    if R > 100:
+        part = dict(kw, kv=tuple(x[:2] for x in kw["kv"]))
+        assert torch.equal(_call(q[:2], part, lens[:2]), out[:2])
 
 
 @pytest.mark.gpu
