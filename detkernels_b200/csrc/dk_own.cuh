@@ -1,16 +1,19 @@
 // A row's own tokens behind a shared prefix: split-KV decode attention that leaves softmax states.
 //
-// Fixed reduction structure: the row's tokens [0, len) in splits of kSplit = 256; inside a split
+// Fixed reduction structure: the row's tokens [0, len) in splits of kSplit = 64; inside a split
 // groups of 16 tokens in order with an online softmax (m, l, O), scores from mma.m16n8k16 (f32
 // accumulation), weights rounded to the input type for P.V and summed as rounded; split states
 // joined in order.  Nothing depends on the batch, the tile a row sits in or the schedule.
 //
 // Work: a unit is (row tile of at most 16 query rows of one sequence, KV head, run of splits), one
 // warp each, with no barrier wider than the warp: short sequences, which are what follows a shared
-// prefix, leave many small units whose loads overlap each other across the 14 (head_dim 64) or 9
-// (128) warps an SM holds.  K and V come through a ring of 16-token stages (cp.async, zero filled
-// past the sequence's end, so that whatever the cache holds there is never read).  A warp that owns
-// all splits joins them in registers; otherwise every split leaves its state for combine_kernel.
+// prefix, leave many small units whose loads overlap each other.  The products are formed transposed
+// (S^T = K q^T, O^T = V^T P^T: the tokens, then the head_dim, are the MMA's 16 rows and the query rows
+// its 8 columns), so up to 8 query rows a tile cost half the MMAs and registers of the upright form;
+// a column's bits do not depend on the others, so tiles of 16 rows (two column halves) give the same.
+// K and V come through a ring of 16-token stages (cp.async, zero filled past the sequence's end, so
+// that whatever the cache holds there is never read).  A warp that owns all splits joins them in
+// registers; otherwise every split leaves its state for combine_kernel.
 #pragma once
 
 #include <type_traits>
@@ -20,7 +23,7 @@
 namespace dk {
 namespace own {
 
-constexpr int kSplit = 256;
+constexpr int kSplit = 64;
 constexpr int kStep = 16;
 constexpr int kRows = 16;
 
@@ -73,9 +76,9 @@ struct Params {
   int32_t page, n_blocks;
   int32_t max_splits, spu, upt;   // splits a unit, units a (tile, head)
   float scale_log2;
-  float* st_o;                // [max_splits, or 1 when upt == 1][n_rows * hq][D]
-  float* st_ml;               // [..][n_rows * hq][2]
-  int64_t st_rows;
+  float* st_o;                // [max_splits, or 1 when upt == 1][D / 4][st_rows][4]
+  float* st_ml;               // [..][st_rows][2]
+  int64_t st_rows;            // hkv * rows * G: state row (kvh * rows + row) * G + head in the group
 };
 
 template <int D>
@@ -83,7 +86,7 @@ struct Cfg {
   static constexpr int ROWB = D * 2;
   static constexpr int TENSOR = kStep * ROWB;
   static constexpr int STAGE = 2 * TENSOR;
-  static constexpr int STAGES = D == 128 ? 3 : (D == 64 ? 4 : 6);
+  static constexpr int STAGES = D == 128 ? 3 : 4;
   static constexpr int SMEM = STAGES * STAGE;
 };
 
@@ -144,10 +147,17 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool l
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 
-template <typename T, int D>
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {   // an 8 x 8 matrix of 16-bit values
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// NB: column halves (8 query rows each).
+template <typename T, int D, int NB>
 __global__ void __launch_bounds__(32) own_kernel(const Params p) {
   using C = Cfg<D>;
-  constexpr int KC = D / 16, NT = D / 8, CPR = D / 8;
+  constexpr int KC = D / 16, CPR = D / 8;
   constexpr int PER = kStep * CPR / 32;   // 16-byte chunks a lane copies of each tensor a step
   extern __shared__ __align__(128) uint8_t ring[];
   pdl_launch_dependents();
@@ -164,7 +174,7 @@ __global__ void __launch_bounds__(32) own_kernel(const Params p) {
     seq = p.tiles[3 * tile + 2];
   }
   // every exit waits for the kernel before this one (see the launch)
-  if (nr < 1 || nr * p.G > kRows || r0 < 0 || r0 + nr > p.n_rows || seq < 0 || seq >= p.n_seq) {
+  if (nr < 1 || nr * p.G > 8 * NB || r0 < 0 || r0 + nr > p.n_rows || seq < 0 || seq >= p.n_seq) {
     if (lane == 0 && unit == 0 && kvh == 0) report_error(DK_ERR_DEVICE_CHECK, kDetTile);
     pdl_wait();
     return;
@@ -186,16 +196,25 @@ __global__ void __launch_bounds__(32) own_kernel(const Params p) {
   }
   const int g = lane >> 2, t4 = lane & 3;
   const int valid_rows = nr * p.G;
-  const int i0 = g / p.G, i1 = (g + 8) / p.G;      // tile rows of this lane's query rows
-  const int len0 = __shfl_sync(0xffffffffu, my_len, min(i0, 31)), len1 = __shfl_sync(0xffffffffu, my_len, min(i1, 31));
-  const bool v0 = g < valid_rows, v1 = g + 8 < valid_rows;
-  const int end0 = v0 ? len0 : 0, end1 = v1 ? len1 : 0;
+  // this lane's columns: query rows 8 h + 2 t4 + e of the tile, their tile rows and token ends
+  int col_row[NB][2], end[NB][2];
+#pragma unroll
+  for (int h = 0; h < NB; ++h)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int rho = 8 * h + 2 * t4 + e;
+      col_row[h][e] = rho / p.G;
+      const int len = __shfl_sync(0xffffffffu, my_len, min(col_row[h][e], 31));
+      end[h][e] = rho < valid_rows ? len : 0;
+    }
 
   // ---- loads: lane's chunks of a step, one page lookup a step (a page holds whole steps) ----
   const T* kb = static_cast<const T*>(p.k) + static_cast<int64_t>(kvh) * p.c_sh;
   const T* vb = static_cast<const T*>(p.v) + static_cast<int64_t>(kvh) * p.c_sh;
   const uint32_t ring_a = smem_u32(ring);
-  int pg_first = -64, pg_mine = 0;                 // 32 table entries, one a lane
+  constexpr int RPI = 32 / CPR > 0 ? 32 / CPR : 1;   // rows an instruction of the warp covers
+  const int ld_r = lane / CPR, ld_c = lane % CPR;    // D = 128: 2 rows of 16 chunks an instruction
+  int pg_first = -64, pg_mine = 0;                   // 32 table entries, one a lane
   const int n_steps = (t_end - t_begin + kStep - 1) / kStep;
   auto issue = [&](int st) {
     if (st < n_steps) {
@@ -217,16 +236,20 @@ __global__ void __launch_bounds__(32) own_kernel(const Params p) {
         slab = __shfl_sync(0xffffffffu, pg_mine, pg - pg_first);
         tok = t0 - pg * p.page;
       }
-      const int64_t base = slab * p.c_sn + static_cast<int64_t>(tok) * p.c_st;
+      const int64_t off0 = slab * p.c_sn + static_cast<int64_t>(tok + ld_r) * p.c_st + ld_c * 8;
+      const T* ks = kb + off0;
+      const T* vs = vb + off0;
+      const int64_t inc = RPI * p.c_st;
       const uint32_t dst = ring_a + (st % C::STAGES) * C::STAGE;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int e = lane + i * 32, r = e / CPR, c = e % CPR;
+        const int r = ld_r + i * RPI;
         const bool live = t0 + r < t_end;
-        const int64_t off = live ? base + static_cast<int64_t>(r) * p.c_st + c * 8 : 0;
-        const uint32_t d = dst + chunk_off<D>(r, c);
-        cp_async16(d, kb + off, live);
-        cp_async16(d + C::TENSOR, vb + off, live);
+        const uint32_t d = dst + chunk_off<D>(r, ld_c);
+        cp_async16(d, live ? ks : kb, live);
+        cp_async16(d + C::TENSOR, live ? vs : vb, live);
+        ks += inc;
+        vs += inc;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -234,42 +257,49 @@ __global__ void __launch_bounds__(32) own_kernel(const Params p) {
 #pragma unroll
   for (int st = 0; st < C::STAGES - 1; ++st) issue(st);
 
-  // ---- query fragments ----
-  uint32_t qa[KC][4];
-  {
-    const T* q = static_cast<const T*>(p.q);
-    const T* q0 = q + static_cast<int64_t>(r0 + i0) * p.q_sr + static_cast<int64_t>(kvh * p.G + g - i0 * p.G) * p.q_sh;
-    const T* q1 = q + static_cast<int64_t>(r0 + i1) * p.q_sr + static_cast<int64_t>(kvh * p.G + g + 8 - i1 * p.G) * p.q_sh;
+  // ---- query fragments: q^T, column g of each half ----
+  uint32_t qb[NB][KC][2];
+#pragma unroll
+  for (int h = 0; h < NB; ++h) {
+    const int rho = 8 * h + g, i = rho / p.G;
+    const T* q = static_cast<const T*>(p.q) + static_cast<int64_t>(r0 + i) * p.q_sr +
+                 static_cast<int64_t>(kvh * p.G + rho - i * p.G) * p.q_sh;
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
-      const int d = kc * 16 + 2 * t4;
-      qa[kc][0] = v0 ? *reinterpret_cast<const uint32_t*>(q0 + d) : 0u;
-      qa[kc][1] = v1 ? *reinterpret_cast<const uint32_t*>(q1 + d) : 0u;
-      qa[kc][2] = v0 ? *reinterpret_cast<const uint32_t*>(q0 + d + 8) : 0u;
-      qa[kc][3] = v1 ? *reinterpret_cast<const uint32_t*>(q1 + d + 8) : 0u;
+      qb[h][kc][0] = rho < valid_rows ? *reinterpret_cast<const uint32_t*>(q + kc * 16 + 2 * t4) : 0u;
+      qb[h][kc][1] = rho < valid_rows ? *reinterpret_cast<const uint32_t*>(q + kc * 16 + 2 * t4 + 8) : 0u;
     }
   }
   const int mi = lane >> 3, ri = lane & 7;
-  const int k_row = (mi >> 1) * 8 + ri, k_c = mi & 1;   // K: two 8-token tiles, k halves
-  const int v_row = (mi & 1) * 8 + ri, v_c = mi >> 1;   // V transposed: token halves, two 8-wide d tiles
+  const int k_row = (mi & 1) * 8 + ri, k_c = mi >> 1;   // K as stored: token halves, then k halves
+  const int v_row = (mi >> 1) * 8 + ri, v_c = mi & 1;   // V transposed: d halves, then token halves
 
-  float o[NT][4], m_r[2], l_r[2];
-  float run_o[NT][4], run_m[2], run_l[2];
+  float o[NB][KC][4], m_r[NB][2], l_r[NB][2];
+  float run_o[NB][KC][4], run_m[NB][2], run_l[NB][2];
   const bool direct = p.upt == 1;
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+  for (int h = 0; h < NB; ++h) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[j][e] = run_o[j][e] = 0.0f;
-  m_r[0] = m_r[1] = run_m[0] = run_m[1] = -INFINITY;
-  l_r[0] = l_r[1] = run_l[0] = run_l[1] = 0.0f;
+    for (int j = 0; j < KC; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[h][j][e] = run_o[h][j][e] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      m_r[h][e] = run_m[h][e] = -INFINITY;
+      l_r[h][e] = run_l[h][e] = 0.0f;
+    }
+  }
 
-  auto store = [&](int64_t s, int h, float m, float l, const float (&a)[NT][4]) {
-    const int rho = g + 8 * h, i = h ? i1 : i0;
-    const int64_t idx = s * p.st_rows + static_cast<int64_t>(r0 + i) * p.hq + kvh * p.G + (rho - i * p.G);
-    if (t4 == 0) *reinterpret_cast<float2*>(p.st_ml + 2 * idx) = make_float2(m, l);
-    float* dst = p.st_o + idx * D + 2 * t4;
+  const int64_t n0 = (static_cast<int64_t>(kvh) * p.n_rows + r0) * p.G + 2 * t4;   // state row of column 2 t4
+  auto store = [&](int64_t s, int h, int e, float m, float l, const float (&a)[KC][4]) {
+    const int64_t n = n0 + 8 * h + e;
+    if (g == 0) *reinterpret_cast<float2*>(p.st_ml + 2 * (s * p.st_rows + n)) = make_float2(m, l);
+    float* dst = p.st_o + ((s * (D / 4) + (g >> 2)) * p.st_rows + n) * 4 + (g & 3);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) *reinterpret_cast<float2*>(dst + j * 8) = make_float2(a[j][2 * h], a[j][2 * h + 1]);
+    for (int j = 0; j < KC; ++j) {
+      dst[static_cast<int64_t>(4 * j) * p.st_rows * 4] = a[j][e];
+      dst[static_cast<int64_t>(4 * j + 2) * p.st_rows * 4] = a[j][2 + e];
+    }
   };
 
   for (int st = 0; st < n_steps; ++st) {
@@ -278,70 +308,75 @@ __global__ void __launch_bounds__(32) own_kernel(const Params p) {
     issue(st + C::STAGES - 1);   // into the stage read in the previous step
     const uint32_t ka = ring_a + (st % C::STAGES) * C::STAGE, va = ka + C::TENSOR;
     const int t0 = t_begin + st * kStep;
-    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+    float sc[NB][4];
+#pragma unroll
+    for (int h = 0; h < NB; ++h) sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.0f;
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
-      uint32_t b[4];
-      ldsm_x4(ka + chunk_off<D>(k_row, 2 * kc + k_c), b);
-      mma<T>(s0, qa[kc], b[0], b[1]);
-      mma<T>(s1, qa[kc], b[2], b[3]);
+      uint32_t a[4];
+      ldsm_x4(ka + chunk_off<D>(k_row, 2 * kc + k_c), a);
+#pragma unroll
+      for (int h = 0; h < NB; ++h) mma<T>(sc[h], a, qb[h][kc][0], qb[h][kc][1]);
     }
-    const int tk = t0 + 2 * t4;
-    uint32_t pa[4];
-    float alpha[2];
+    // scores: sc[h][0..1] token t0 + g, sc[h][2..3] token t0 + g + 8, columns 2 t4 and 2 t4 + 1
+    uint32_t pb[NB][2];
+    bool same = true;
+    float alpha[NB][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float x[4] = {__fmul_rn(s0[2 * h], p.scale_log2), __fmul_rn(s0[2 * h + 1], p.scale_log2),
-                    __fmul_rn(s1[2 * h], p.scale_log2), __fmul_rn(s1[2 * h + 1], p.scale_log2)};
-      const int end = h ? end1 : end0;
-      if (tk + 0 >= end) x[0] = -INFINITY;
-      if (tk + 1 >= end) x[1] = -INFINITY;
-      if (tk + 8 >= end) x[2] = -INFINITY;
-      if (tk + 9 >= end) x[3] = -INFINITY;
-      float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(m_r[h], mx);
-      const float ref = (mn == -INFINITY) ? 0.0f : mn;
-      alpha[h] = exp2_hw(__fsub_rn(m_r[h], ref));
+    for (int h = 0; h < NB; ++h) {
+      float x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = exp2_hw(__fsub_rn(x[e], ref));
-      pa[h] = pack2<T>(x[0], x[1]);
-      pa[h + 2] = pack2<T>(x[2], x[3]);
-      const float2 a = unpack2<T>(pa[h]), b = unpack2<T>(pa[h + 2]);
-      l_r[h] = __fmaf_rn(l_r[h], alpha[h], __fadd_rn(__fadd_rn(a.x, a.y), __fadd_rn(b.x, b.y)));
-      m_r[h] = mn;
-    }
-    if (alpha[0] != 1.0f || alpha[1] != 1.0f) {   // a factor of exactly 1 changes nothing
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        o[j][0] = __fmul_rn(o[j][0], alpha[0]);
-        o[j][1] = __fmul_rn(o[j][1], alpha[0]);
-        o[j][2] = __fmul_rn(o[j][2], alpha[1]);
-        o[j][3] = __fmul_rn(o[j][3], alpha[1]);
+      for (int e = 0; e < 2; ++e) {
+        x[e] = (t0 + g < end[h][e]) ? __fmul_rn(sc[h][e], p.scale_log2) : -INFINITY;
+        x[2 + e] = (t0 + g + 8 < end[h][e]) ? __fmul_rn(sc[h][2 + e], p.scale_log2) : -INFINITY;
+        float mx = fmaxf(x[e], x[2 + e]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float mn = fmaxf(m_r[h][e], mx);
+        const float ref = (mn == -INFINITY) ? 0.0f : mn;
+        alpha[h][e] = exp2_hw(__fsub_rn(m_r[h][e], ref));
+        same = same && alpha[h][e] == 1.0f;
+        x[e] = exp2_hw(__fsub_rn(x[e], ref));
+        x[2 + e] = exp2_hw(__fsub_rn(x[2 + e], ref));
+        m_r[h][e] = mn;
       }
+      const uint32_t lo = pack2<T>(x[0], x[1]), hi = pack2<T>(x[2], x[3]);
+      const float2 a = unpack2<T>(lo), b = unpack2<T>(hi);
+      l_r[h][0] = __fmaf_rn(l_r[h][0], alpha[h][0], __fadd_rn(a.x, b.x));
+      l_r[h][1] = __fmaf_rn(l_r[h][1], alpha[h][1], __fadd_rn(a.y, b.y));
+      pb[h][0] = transpose8(lo);
+      pb[h][1] = transpose8(hi);
+    }
+    if (!same) {   // a factor of exactly 1 changes nothing
+#pragma unroll
+      for (int h = 0; h < NB; ++h)
+#pragma unroll
+        for (int j = 0; j < KC; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[h][j][e] = __fmul_rn(o[h][j][e], alpha[h][e & 1]);
     }
     // a row's weights beyond its end are 0, which a non-finite value there (a later row's token) must
     // not meet: then each row goes alone, longest first, over values cut at its own end
     bool alone = false;
     if (t0 + kStep > min_len && min_len < max_len) {
-      uint32_t wild = 0;
+      bool wild = false;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int e = lane + i * 32, r = e / CPR, c = e % CPR;
-        const uint4 x = *reinterpret_cast<const uint4*>(ring + (va - ring_a) + chunk_off<D>(r, c));
+        const int r = ld_r + i * RPI;
+        const uint4 x = *reinterpret_cast<const uint4*>(ring + (va - ring_a) + chunk_off<D>(r, ld_c));
         wild |= t0 + r >= min_len && (non_finite<T>(x.x) || non_finite<T>(x.y) || non_finite<T>(x.z) ||
                                       non_finite<T>(x.w));
       }
-      alone = __any_sync(0xffffffffu, wild != 0);
+      alone = __any_sync(0xffffffffu, wild);
     }
     if (!alone) {
 #pragma unroll
-      for (int pc = 0; pc < D / 16; ++pc) {
-        uint32_t b[4];
-        ldsm_x4_t(va + chunk_off<D>(v_row, 2 * pc + v_c), b);
-        mma<T>(o[2 * pc], pa, b[0], b[1]);
-        mma<T>(o[2 * pc + 1], pa, b[2], b[3]);
+      for (int j = 0; j < KC; ++j) {
+        uint32_t a[4];
+        ldsm_x4_t(va + chunk_off<D>(v_row, 2 * j + v_c), a);
+#pragma unroll
+        for (int h = 0; h < NB; ++h) mma<T>(o[h][j], a, pb[h][0], pb[h][1]);
       }
     } else {
       int left = lane < nr ? my_len : -1;
@@ -351,66 +386,76 @@ __global__ void __launch_bounds__(32) own_kernel(const Params p) {
         if (lane == row) left = -1;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const int e = lane + i * 32, r = e / CPR, c = e % CPR;
-          if (t0 + r >= cut) *reinterpret_cast<uint4*>(ring + (va - ring_a) + chunk_off<D>(r, c)) = make_uint4(0, 0, 0, 0);
+          const int r = ld_r + i * RPI;
+          if (t0 + r >= cut)
+            *reinterpret_cast<uint4*>(ring + (va - ring_a) + chunk_off<D>(r, ld_c)) = make_uint4(0, 0, 0, 0);
         }
         __syncwarp();
 #pragma unroll
-        for (int pc = 0; pc < D / 16; ++pc) {
-          uint32_t b[4];
-          ldsm_x4_t(va + chunk_off<D>(v_row, 2 * pc + v_c), b);
+        for (int j = 0; j < KC; ++j) {
+          uint32_t a[4];
+          ldsm_x4_t(va + chunk_off<D>(v_row, 2 * j + v_c), a);
 #pragma unroll
-          for (int j = 2 * pc; j < 2 * pc + 2; ++j) {
-            float one[4] = {o[j][0], o[j][1], o[j][2], o[j][3]};
-            mma<T>(one, pa, b[2 * (j & 1)], b[2 * (j & 1) + 1]);
+          for (int h = 0; h < NB; ++h) {
+            float one[4] = {o[h][j][0], o[h][j][1], o[h][j][2], o[h][j][3]};
+            mma<T>(one, a, pb[h][0], pb[h][1]);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if ((e < 2 ? i0 : i1) == row) o[j][e] = one[e];
+              if (col_row[h][e & 1] == row) o[h][j][e] = one[e];
           }
         }
         __syncwarp();
       }
     }
-    __syncwarp();
     if ((st + 1) % (kSplit / kStep) == 0 || st + 1 == n_steps) {
       const int sp_begin = t0 / kSplit * kSplit;   // first token of the split that ends here
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        l_r[h] = __fadd_rn(l_r[h], __shfl_xor_sync(0xffffffffu, l_r[h], 1));
-        l_r[h] = __fadd_rn(l_r[h], __shfl_xor_sync(0xffffffffu, l_r[h], 2));
-        if (sp_begin < (h ? end1 : end0)) {        // the row has tokens in this split
-          if (!direct) {
-            store(sp_begin / kSplit, h, m_r[h], l_r[h], o);
-          } else if (sp_begin == 0) {
-            run_m[h] = m_r[h];
-            run_l[h] = l_r[h];
+      for (int h = 0; h < NB; ++h) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              run_o[j][2 * h] = o[j][2 * h];
-              run_o[j][2 * h + 1] = o[j][2 * h + 1];
-            }
-          } else {
-            float a, b;
-            run_m[h] = join_weights(run_m[h], m_r[h], a, b);
-            run_l[h] = join(run_l[h], a, l_r[h], b);
+        for (int e = 0; e < 2; ++e) {
+          float l = l_r[h][e];
+          l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 4));
+          l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 8));
+          l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 16));
+          if (sp_begin < end[h][e]) {        // the row has tokens in this split
+            if (!direct) {
+              store(sp_begin / kSplit, h, e, m_r[h][e], l, o[h]);
+            } else if (sp_begin == 0) {
+              run_m[h][e] = m_r[h][e];
+              run_l[h][e] = l;
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              run_o[j][2 * h] = join(run_o[j][2 * h], a, o[j][2 * h], b);
-              run_o[j][2 * h + 1] = join(run_o[j][2 * h + 1], a, o[j][2 * h + 1], b);
+              for (int j = 0; j < KC; ++j) {
+                run_o[h][j][e] = o[h][j][e];
+                run_o[h][j][2 + e] = o[h][j][2 + e];
+              }
+            } else {
+              float a, b;
+              run_m[h][e] = join_weights(run_m[h][e], m_r[h][e], a, b);
+              run_l[h][e] = join(run_l[h][e], a, l, b);
+#pragma unroll
+              for (int j = 0; j < KC; ++j) {
+                run_o[h][j][e] = join(run_o[h][j][e], a, o[h][j][e], b);
+                run_o[h][j][2 + e] = join(run_o[h][j][2 + e], a, o[h][j][2 + e], b);
+              }
             }
           }
+          m_r[h][e] = -INFINITY;
+          l_r[h][e] = 0.0f;
         }
-        m_r[h] = -INFINITY;
-        l_r[h] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) o[j][2 * h] = o[j][2 * h + 1] = 0.0f;
+        for (int j = 0; j < KC; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[h][j][e] = 0.0f;
       }
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (direct) {
-    if (end0 > 0) store(0, 0, run_m[0], run_l[0], run_o);
-    if (end1 > 0) store(0, 1, run_m[1], run_l[1], run_o);
+#pragma unroll
+    for (int h = 0; h < NB; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (end[h][e] > 0) store(0, h, e, run_m[h][e], run_l[h][e], run_o[h]);
   }
   pdl_wait();
 }

@@ -88,9 +88,9 @@ struct Params {
   float c;                // |scale| * log2(e)
   uint32_t flip;          // sign mask for q (0x80008000 when scale < 0)
   int zero;               // scale is 0: q is multiplied by it on the way in
-  float* st_o;            // [n_runs][rows][hq][D]
-  float* st_ml;           // [n_runs][rows][hq][2]
-  int64_t st_rows;        // rows * hq
+  float* st_o;            // [n_runs][D / 4][st_rows][4]: a column of four for 32 rows is one store of a warp
+  float* st_ml;           // [n_runs][st_rows][2]
+  int64_t st_rows;        // hkv * rows * G: state row (kvh * rows + row) * G + head in the group
 };
 
 struct Maps {
@@ -104,16 +104,26 @@ struct Cfg {
   static constexpr int BOX = 64 * 128;            // bytes of a 64-token box
   static constexpr int HALF = 2 * BOX;            // 128 tokens x 64 elements
   static constexpr int STAGE = NH * HALF;         // a K or V block
-  static constexpr int STAGES = D == 128 ? 4 : 8;
+  static constexpr int STAGES = D == 128 ? 5 : 8;
   static constexpr int QTILE = NH * HALF;
-  static constexpr int TPAD = 20;                 // floats a row of a warp's transpose buffer (16 used)
-  static constexpr int TBUF = 32 * TPAD * 4;
-  static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * QTILE + 8 * TBUF + 512;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * QTILE + 512;
   static constexpr uint32_t S_COL = 0;            // two score buffers of 128 columns
   static constexpr uint32_t O_COL = 256;          // two accumulators of DP columns
+  static constexpr int FMA_OF_4 = 0;              // weights of every four whose 2^x takes the FMA pipe
   static constexpr bool GROUPED = group_chunks(D) > 1;
   static constexpr uint32_t R_COL = 384;          // grouped: the joined chunks of either tile, DP columns each
 };
+
+// True for one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
 
 template <uint32_t N>
 __device__ __forceinline__ void reg_dec() {
@@ -173,6 +183,41 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return r;
 }
 
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 2^x for x <= 2^20 on the FMA pipe, two at a time: x = n + f with n the nearest integer (by adding and
+// taking away 1.5 * 2^23), 2^f by the degree-4 polynomial of least relative error on [-1/2, 1/2] (Remez
+// exchange; 2^-18.5), times 2^n.  Below -127 the factor and so the result is 0; NaN stays NaN.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  const float2 magic = make_float2(12582912.0f, 12582912.0f), nmagic = make_float2(-12582912.0f, -12582912.0f);
+  x.x = max_nan(x.x, -127.0f);
+  x.y = max_nan(x.y, -127.0f);
+  const float2 t = add2(x, magic);
+  const float2 n = add2(t, nmagic);
+  const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+  float2 p = make_float2(0.009570102207362652f, 0.009570102207362652f);
+  p = fma2(p, f, make_float2(0.05591785907745361f, 0.05591785907745361f));
+  p = fma2(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
+  p = fma2(p, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+  const float2 s = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                               __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
+  return mul2(p, s);
+}
+
 template <typename T>
 __device__ __forceinline__ uint4 times_zero(uint4 v) {
   uint32_t u[4] = {v.x, v.y, v.z, v.w};
@@ -195,12 +240,12 @@ struct Item {
   int pair, kvh, run, tiles;
   int t_begin, n_blocks, tokens;   // first token, blocks, tokens
 };
-__device__ __forceinline__ Item item_at(const Params& p, int64_t w) {
+__device__ __forceinline__ Item item_at(const Params& p, uint32_t w) {
   Item it;
-  it.pair = static_cast<int>(w % p.n_pairs);
-  const int64_t r = w / p.n_pairs;
-  it.kvh = static_cast<int>(r % p.hkv);
-  it.run = static_cast<int>(r / p.hkv);
+  const uint32_t r = w / static_cast<uint32_t>(p.n_pairs);
+  it.pair = static_cast<int>(w - r * p.n_pairs);
+  it.run = static_cast<int>(r / static_cast<uint32_t>(p.hkv));
+  it.kvh = static_cast<int>(r - it.run * static_cast<uint32_t>(p.hkv));
   it.tiles = (static_cast<int64_t>(it.pair) * 2 + 1) * kRows < p.rg ? 2 : 1;
   it.t_begin = it.run * p.run_blocks * kBlock;
   it.tokens = min(p.prefix_len - it.t_begin, p.run_blocks * kBlock);
@@ -216,20 +261,22 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = base;
   uint8_t* s_q = ring + C::STAGES * C::STAGE;
-  float* s_t = reinterpret_cast<float*>(s_q + 2 * C::QTILE);
-  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(s_t) + 8 * C::TBUF);
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_q + 2 * C::QTILE);
   uint64_t* empty = full + C::STAGES;
   // score barriers: 0 and 1 by tile, 2 the second buffer of a one-tile item (tile 1's columns); each
   // has one warpgroup that waits for every phase of it in order
   uint64_t* s_full = empty + C::STAGES;   // [3]
   uint64_t* p_ready = s_full + 3;         // [3]
-  uint64_t* o_full = p_ready + 3;         // [2] by tile: P.V of a block done
+  uint64_t* p_half = p_ready + 3;         // [3] the first 64 tokens' weights are in TMEM
+  uint64_t* o_full = p_half + 3;         // [2] by tile: P.V of a block done
   uint64_t* o_free = o_full + 2;          // [2] by tile: the accumulator has been read
   uint64_t* q_ready = o_free + 2;         // [2] by tile
   uint64_t* done = q_ready + 2;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(done + 1);
 
-  const int warp = threadIdx.x >> 5;
+  // one value for the whole warp as the compiler sees it: the MMA issuer's operands then stay in
+  // uniform registers (from per-thread ones each tcgen05.mma took ~140 cycles to issue)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -239,6 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
     for (int i = 0; i < 3; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_ready[i], 128);
+      mbar_init(&p_half[i], 128);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&o_full[t], 1);
@@ -263,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
   pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
 
-  const int64_t n_items = static_cast<int64_t>(p.n_pairs) * p.hkv * p.n_runs;
+  const uint32_t n_items = static_cast<uint32_t>(p.n_pairs) * p.hkv * p.n_runs;   // < 2^31 (the host checks)
   bool abort_flag = false;
 
   if (warp >= 8) {
@@ -273,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
       int stage = 0;
       uint32_t phase = 0;
       int64_t fills = 0;
-      for (int64_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
+      for (uint32_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
         const Item it = item_at(p, w);
         for (int b = 0; b < it.n_blocks && !abort_flag; ++b) {
           const int t0 = it.t_begin + b * kBlock;
@@ -317,96 +365,120 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
       // ---------------- MMA issuer ----------------
       constexpr uint32_t idesc_s = umma_idesc_f16(FMT, 0, 0, kRows, kBlock);
       constexpr uint32_t idesc_o = umma_idesc_f16(FMT, 0, 1, kRows, C::DP);
-      const uint32_t ring_a = smem_u32(ring), q_a = smem_u32(s_q);
-      int64_t used = 0;                      // stages taken so far (K, V, K, V, ...)
-      uint32_t pc[3] = {0, 0, 0};            // p_ready phases seen
-      uint32_t qc[2] = {0, 0}, oc[2] = {0, 0};
-      auto wait_stage = [&](int64_t f) {
-        return warp_wait(&full[f % C::STAGES], static_cast<uint32_t>((f / C::STAGES) & 1), kDetFull, abort_flag);
-      };
-      // scores of tile t, block with K in stage f, by score barrier sb
-      auto issue_qk = [&](int t, int sb, int64_t f) {
-        if (lane == 0) {
-          const uint32_t kb = ring_a + static_cast<uint32_t>(f % C::STAGES) * C::STAGE;
-          const uint32_t qb = q_a + t * C::QTILE;
+      // descriptors of stage 0 / tile 0; an offset of n bytes adds n / 16
+      const uint64_t k_desc = umma_sdesc(smem_u32(ring), 16, 1024, 2);
+      const uint64_t v_desc = umma_sdesc(smem_u32(ring), C::HALF, 1024, 2);
+      const uint64_t q_desc = umma_sdesc(smem_u32(s_q), 16, 1024, 2);
+      const bool leader = elect_one();
+      int stage = 0;                         // next stage to take: K, V, K, V, ... in the order of the loads
+      uint32_t phase = 0;
+      uint32_t pph = 0;                      // p_ready parities by bit
+      uint32_t qph = 0, oph = 3;             // q_ready, o_free parities by bit (the first o_free wait passes)
+      // scores of tile t, K block in stage st, by score barrier sb
+      auto issue_qk = [&](int t, int sb, int st) {
+        if (leader) {
+          const uint64_t kd = k_desc + static_cast<uint64_t>(st * (C::STAGE / 16));
+          const uint64_t qd = q_desc + static_cast<uint64_t>(t * (C::QTILE / 16));
+          const uint32_t d = tmem + C::S_COL + (sb ? 128 : 0);
 #pragma unroll
           for (int j = 0; j < C::DP / 16; ++j) {
-            const uint32_t off = (j >> 2) * C::HALF + (j & 3) * 32;
-            tc_mma_f16(tmem + C::S_COL + (sb ? 128 : 0), umma_sdesc(qb + off, 16, 1024, 2), umma_sdesc(kb + off, 16, 1024, 2),
-                       idesc_s, j > 0 ? 1u : 0u);
+            const uint64_t off = ((j >> 2) * C::HALF + (j & 3) * 32) / 16;
+            tc_mma_f16(d, qd + off, kd + off, idesc_s, j > 0 ? 1u : 0u);
           }
           tc_commit(&s_full[sb]);
         }
         __syncwarp();
       };
-      for (int64_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
+      auto take = [&](int& st) {   // the next stage in order, once it is full
+        st = stage;
+        if (!warp_wait(&full[st], phase, kDetFull, abort_flag)) return false;
+        if (++stage == C::STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+        return true;
+      };
+      for (uint32_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
         const Item it = item_at(p, w);
         const int nb = it.n_blocks;
         for (int t = 0; t < it.tiles; ++t) {
-          if (!warp_wait(&q_ready[t], qc[t] & 1, kDetQ, abort_flag)) break;
-          ++qc[t];
+          if (!warp_wait(&q_ready[t], (qph >> t) & 1, kDetQ, abort_flag)) break;
+          qph ^= 1u << t;
         }
         if (abort_flag) break;
-        const int64_t f0 = used;   // block b: K in fill f0 + 2b, V in f0 + 2b + 1
-        used += 2 * static_cast<int64_t>(nb);
         tc_fence_after();
-        if (!wait_stage(f0)) break;
-        for (int t = 0; t < it.tiles; ++t) issue_qk(t, t, f0);
-        if (lane == 0) tc_commit(&empty[f0 % C::STAGES]);
+        int ks, vs;
+        if (!take(ks)) break;
+        for (int t = 0; t < it.tiles; ++t) issue_qk(t, t, ks);
+        if (leader) tc_commit(&empty[ks]);
+        // a block's V and the next block's K are waited for ahead of their use, while MMAs run
+        if (!take(vs) || (nb > 1 && !take(ks))) break;
+        int in_chunk = 0;
         for (int b = 0; b < nb && !abort_flag; ++b) {
           const bool more = b + 1 < nb;
-          const int64_t fk = f0 + 2 * (b + 1), fv = f0 + 2 * b + 1;
-          if (it.tiles == 1 && more) {   // the next block's scores go to the other buffer
-            if (!wait_stage(fk)) break;
-            issue_qk(0, (b + 1) & 1 ? 2 : 0, fk);
-            if (lane == 0) tc_commit(&empty[fk % C::STAGES]);
-          }
+          const bool fresh = in_chunk == 0;      // a new chunk overwrites the accumulator
+          if (++in_chunk == p.chunk_blocks) in_chunk = 0;
           const int valid = min(kBlock, it.tokens - b * kBlock);
           const int steps = (valid + 15) >> 4;   // 16-token steps of P.V that hold a token
+          if (valid & 15) {
+            // tokens past the prefix inside the last step: zero rows of V (whatever the cache holds
+            // there must not meet their zero weights)
+            uint8_t* vb = ring + vs * C::STAGE;
+            const int rows = steps * 16 - valid;
+            for (int e = lane; e < rows * C::NH * 8; e += 32) {
+              const int r = valid + e / (C::NH * 8), c = e % (C::NH * 8);
+              *reinterpret_cast<uint4*>(vb + (c >> 3) * C::HALF + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (it.tiles == 1 && more) {   // the next block's scores go to the other buffer
+            issue_qk(0, (b + 1) & 1 ? 2 : 0, ks);
+            if (leader) tc_commit(&empty[ks]);
+          }
+          int vs_next = 0, ks_next = 0;
           for (int t = 0; t < it.tiles; ++t) {
             const int sb = it.tiles == 2 ? t : (b & 1 ? 2 : 0);
-            if (!warp_wait(&p_ready[sb], pc[sb] & 1, kDetProbs, abort_flag)) break;
-            ++pc[sb];
-            if (b % p.chunk_blocks == 0) {   // a new chunk overwrites the accumulator
-              if (!warp_wait(&o_free[t], (oc[t] & 1) ^ 1u, kDetOutFree, abort_flag)) break;
-              ++oc[t];
+            if (fresh) {
+              if (!warp_wait(&o_free[t], (oph >> t) & 1, kDetOutFree, abort_flag)) break;
+              oph ^= 1u << t;
             }
-            if (t == 0) {
-              if (!wait_stage(fv)) break;
-              if (valid & 15) {
-                // tokens past the prefix inside the last step: zero rows of V (whatever the cache
-                // holds there must not meet their zero weights)
-                uint8_t* vb = ring + (fv % C::STAGES) * C::STAGE;
-                const int rows = steps * 16 - valid;
-                for (int e = lane; e < rows * C::NH * 8; e += 32) {
-                  const int r = valid + e / (C::NH * 8), c = e % (C::NH * 8);
-                  *reinterpret_cast<uint4*>(vb + (c >> 3) * C::HALF + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-              }
-            }
+            const uint64_t vd = v_desc + static_cast<uint64_t>(vs * (C::STAGE / 16));
+            const uint32_t o = tmem + C::O_COL + t * C::DP, pt = tmem + C::S_COL + (sb ? 128 : 0);
+            // the first half of the weights, then the second
+            if (!warp_wait(&p_half[sb], (pph >> sb) & 1, kDetProbs, abort_flag)) break;
             tc_fence_after();
-            if (lane == 0) {
-              const uint32_t vb = ring_a + static_cast<uint32_t>(fv % C::STAGES) * C::STAGE;
-              for (int j = 0; j < steps; ++j)
-                mma_ts(tmem + C::O_COL + t * C::DP, tmem + C::S_COL + (sb ? 128 : 0) + j * 8,
-                       umma_sdesc(vb + j * 2048, C::HALF, 1024, 2), idesc_o,
-                       (b % p.chunk_blocks != 0 || j > 0) ? 1u : 0u);
+            if (leader) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (j < steps)
+                  mma_ts(o, pt + j * 8, vd + static_cast<uint64_t>(j * (2048 / 16)), idesc_o, (fresh && j == 0) ? 0u : 1u);
+            }
+            __syncwarp();
+            if (!warp_wait(&p_ready[sb], (pph >> sb) & 1, kDetProbs, abort_flag)) break;
+            pph ^= 1u << sb;
+            tc_fence_after();
+            if (leader) {
+#pragma unroll
+              for (int j = 4; j < 8; ++j)
+                if (j < steps)
+                  mma_ts(o, pt + j * 8, vd + static_cast<uint64_t>(j * (2048 / 16)), idesc_o, 1u);
               tc_commit(&o_full[t]);
-              if (t + 1 == it.tiles) tc_commit(&empty[fv % C::STAGES]);
+              if (t + 1 == it.tiles) tc_commit(&empty[vs]);
             }
             __syncwarp();
             if (it.tiles == 2 && more) {
-              if (t == 0 && !wait_stage(fk)) break;
-              issue_qk(t, t, fk);
-              if (t == 1 && lane == 0) tc_commit(&empty[fk % C::STAGES]);
+              issue_qk(t, t, ks);
+              if (t == 1 && leader) tc_commit(&empty[ks]);
             }
+            if (t == 0 && more && (!take(vs_next) || (b + 2 < nb && !take(ks_next)))) break;
           }
+          vs = vs_next;
+          ks = ks_next;
         }
       }
       // all issued MMAs are complete before TMEM is freed
-      if (lane == 0) tc_commit(done);
+      if (leader) tc_commit(done);
       __syncwarp();
       bool fin = false;
       warp_wait(done, 0, kDetDone, fin);
@@ -418,47 +490,70 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
     const int r = threadIdx.x & 127;            // row of the tile
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t o_t = tmem + lane_base + C::O_COL + t * C::DP;
-    float* tb = s_t + warp * (C::TBUF / 4);
     uint32_t sc[2] = {0, 0};                    // score phases consumed: own barrier, second buffer
     uint32_t ocnt = 0;                          // P.V completions of this tile so far
-    for (int64_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
+    // This row's query vector of an item into the swizzled K-major operand tile, asynchronously ...
+    uint8_t* const q_row = s_q + t * C::QTILE + r * 128;
+    auto fetch_q = [&](const Item& it) {
+      const int64_t mrow = (static_cast<int64_t>(it.pair) * 2 + t) * kRows + r;
+      const bool valid = mrow < p.rg;
+      const int64_t row = valid ? mrow / p.G : 0;
+      const T* src = static_cast<const T*>(p.q) + row * p.q_sr +
+                     (it.kvh * p.G + (valid ? mrow - row * p.G : 0)) * p.q_sh;
+#pragma unroll
+      for (int c = 0; c < C::DP / 8; ++c)
+        own::cp_async16(smem_u32(q_row + (c >> 3) * C::HALF + (((c & 7) ^ (r & 7)) << 4)), src + (c < D / 8 ? c * 8 : 0),
+                        valid && c < D / 8);
+    };
+    // ... and, once there, handed to the tensor cores.
+    auto q_here = [&]() {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if (p.flip | p.zero) {
+#pragma unroll 1
+        for (int c = 0; c < D / 8; ++c) {
+          uint4* at = reinterpret_cast<uint4*>(q_row + (c >> 3) * C::HALF + (((c & 7) ^ (r & 7)) << 4));
+          uint4 v = *at;
+          v.x ^= p.flip;
+          v.y ^= p.flip;
+          v.z ^= p.flip;
+          v.w ^= p.flip;
+          *at = p.zero ? times_zero<T>(v) : v;
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&q_ready[t]);
+    };
+    bool q_loaded = false;
+    for (uint32_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
       const Item it = item_at(p, w);
       if (t >= it.tiles) continue;
+      Item next{};                                // the next item that has this tile
+      uint32_t wn = w;
+      do {
+        wn += gridDim.x;
+        if (wn < n_items) next = item_at(p, wn);
+      } while (wn < n_items && t >= next.tiles);
       const int64_t m0 = (static_cast<int64_t>(it.pair) * 2 + t) * kRows;   // first row of the tile
-      const int64_t mrow = m0 + r;
-      const bool valid_row = mrow < p.rg;
       const bool warp_live = m0 + (warp & 3) * 32 < p.rg;
-      {
-        // this row's query vector into the swizzled K-major operand tile
-        uint8_t* qt = s_q + t * C::QTILE + r * 128;
-        const int64_t row = mrow / p.G;
-        const T* src = static_cast<const T*>(p.q) + row * p.q_sr + (it.kvh * p.G + (mrow - row * p.G)) * p.q_sh;
-#pragma unroll
-        for (int c = 0; c < C::DP / 8; ++c) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (valid_row && c < D / 8) {
-            v = *reinterpret_cast<const uint4*>(src + c * 8);
-            v.x ^= p.flip;
-            v.y ^= p.flip;
-            v.z ^= p.flip;
-            v.w ^= p.flip;
-            if (p.zero) v = times_zero<T>(v);
-          }
-          *reinterpret_cast<uint4*>(qt + (c >> 3) * C::HALF + (((c & 7) ^ (r & 7)) << 4)) = v;
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(&q_ready[t]);
+      if (!q_loaded) {   // the CTA's first item with this tile; later ones are fetched ahead
+        fetch_q(it);
+        q_here();
       }
+      q_loaded = false;
       float run_m = -INFINITY, run_l = 0.0f;
       float m = -INFINITY, l = 0.0f;
+      int in_chunk = 0;
       for (int b = 0; b < it.n_blocks; ++b) {
         const int second = it.tiles == 1 ? (b & 1) : 0;   // a one-tile item's second buffer
         const int sb = second ? 2 : t;
-        const bool first = b % p.chunk_blocks == 0;
+        const bool first = in_chunk == 0;
+        if (++in_chunk == p.chunk_blocks) in_chunk = 0;
         const int valid = min(kBlock, it.tokens - b * kBlock);
         if (!warp_wait(&s_full[sb], sc[second] & 1, kDetScores, abort_flag)) break;
         ++sc[second];
         tc_fence_after();
+        const bool last = b + 1 == it.n_blocks;
+        if (last && wn < n_items) fetch_q(next);   // all scores of this item are formed: q's place is free
         if (warp_live) {
           const uint32_t s_t0 = tmem + lane_base + C::S_COL + (sb ? 128 : 0);
           float s[4][32];
@@ -511,22 +606,36 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               float2 e = fma2(make_float2(s[c][i], s[c][i + 1]), c2, n2);
-              e.x = exp2_hw(e.x);
-              e.y = exp2_hw(e.y);
+              if (((i >> 1) & 3) >= 4 - C::FMA_OF_4) {   // by column alone, so by token
+                e = exp2_fma(e);
+              } else {
+                e.x = exp2_hw(e.x);
+                e.y = exp2_hw(e.y);
+              }
               sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
               pk[i >> 1] = pack2<T>(e.x, e.y);
             }
             tmem_st_x16(s_t0 + c * 16, pk);
+            if (c == 1) {
+              tmem_st_wait();
+              tc_fence_before();
+              mbar_arrive(&p_half[sb]);
+            }
           }
+          tmem_st_wait();
           const float2 ps = add2(sum[0], sum[1]);
           l = __fadd_rn(l, __fadd_rn(ps.x, ps.y));
-          tmem_st_wait();
+        } else {
+          mbar_arrive(&p_half[sb]);
         }
         tc_fence_before();
         mbar_arrive(&p_ready[sb]);
         ++ocnt;
-        const bool last = b + 1 == it.n_blocks;
-        if ((b + 1) % p.chunk_blocks == 0 || last) {
+        if (last && wn < n_items) {
+          q_here();
+          q_loaded = true;
+        }
+        if (in_chunk == 0 || last) {
           // the chunk's state joins the run's, which leaves with the last chunk
           if (!warp_wait(&o_full[t], (ocnt - 1) & 1, kDetOut, abort_flag)) break;
           tc_fence_after();
@@ -540,21 +649,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
               run_m = join_weights(run_m, m, wa, wb);
               run_l = join(run_l, wa, l, wb);
             }
-            const int64_t st0 = static_cast<int64_t>(it.run) * p.st_rows;
-            int64_t dst[4];
-            if (last) {
-              if (valid_row) {
-                const int64_t row = mrow / p.G;
-                const int64_t idx = st0 + row * p.hq + it.kvh * p.G + (mrow - row * p.G);
-                *reinterpret_cast<float2*>(p.st_ml + 2 * idx) = make_float2(run_m, run_l);
-              }
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {   // rows this lane writes, 16 bytes of each a piece
-                const int64_t mm = m0 + (warp & 3) * 32 + j * 8 + (lane >> 2);
-                const int64_t row = mm / p.G;
-                dst[j] = mm < p.rg ? (st0 + row * p.hq + it.kvh * p.G + (mm - row * p.G)) * D + (lane & 3) * 4 : -1;
-              }
-            }
+            const int64_t mrow = m0 + r;
+            const bool valid_row = mrow < p.rg;
+            const int64_t n = it.kvh * p.rg + mrow;   // state row
+            if (last && valid_row)
+              *reinterpret_cast<float2*>(p.st_ml + 2 * (it.run * p.st_rows + n)) = make_float2(run_m, run_l);
+            float* dst = p.st_o + (static_cast<int64_t>(it.run) * (D / 4) * p.st_rows + n) * 4;
             const uint32_t r_t = tmem + lane_base + C::R_COL + t * C::DP;
 #pragma unroll 2
             for (int c = 0; c < D / 16; ++c) {
@@ -570,17 +670,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
               if (C::GROUPED && !last) {
                 tmem_st_x16(r_t + c * 16, o);
               } else {
-                // transposed, so that a row's 64 bytes leave together
-                __syncwarp();
+                if (valid_row) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  *reinterpret_cast<uint4*>(tb + lane * C::TPAD + i * 4) =
-                      make_uint4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
-                __syncwarp();
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const float4 v = *reinterpret_cast<const float4*>(tb + (j * 8 + (lane >> 2)) * C::TPAD + (lane & 3) * 4);
-                  if (dst[j] >= 0) *reinterpret_cast<float4*>(p.st_o + dst[j] + c * 16) = v;
+                  for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<uint4*>(dst + (c * 4 + i) * p.st_rows * 4) =
+                        make_uint4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
                 }
               }
             }
@@ -602,69 +696,69 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
 }
 
 // out[row, head] = O / l of the joined states: the prefix's runs (per_group of them at a time), then
-// the row's own tokens (own_splits states, or one where a warp joined them all).  One warp a (row,
-// head), UN states in flight.
-constexpr int kCombineWarps = 4;
-
+// the row's own tokens.  A CTA takes 32 state rows, a lane each; its warps split the columns in fours
+// (one coalesced load a state), and the outputs go through shared memory so that a head's row leaves
+// whole.
 struct CombineParams {
-  const float* st_o;
-  const float* st_ml;
+  const float* st_o;        // [states][D / 4][st_rows][4]
+  const float* st_ml;       // [states][st_rows][2]
   int n_runs, per_group;
   const int32_t* kv_lens;   // null: no row has tokens of its own
   int own_max;              // states the own tokens may have: 1 (joined already) or the split limit
-  int64_t st_rows;
-  int hq;
+  int64_t st_rows, rg;      // hkv * rows * G, rows * G
+  int G;
   void* out;
   int64_t o_sr, o_sh;
 };
 
+template <int D>
+struct CombineCfg {
+  static constexpr int WARPS = D / 16;        // 4 column quads a warp
+  static constexpr int PAD = D + 2;           // 16-bit elements a row of the output buffer
+};
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const CombineParams p) {
-  constexpr int V = D / 32;
-  constexpr int UN = 8;
+__global__ void __launch_bounds__(CombineCfg<D>::WARPS * 32) combine_kernel(const CombineParams p) {
+  using C = CombineCfg<D>;
+  constexpr int Q = 4;      // column quads a thread
+  constexpr int UN = 4;     // states in flight
+  __shared__ __align__(16) T s_out[32][C::PAD];
   pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int64_t m = static_cast<int64_t>(blockIdx.x) * kCombineWarps + (threadIdx.x >> 5);
-  if (m >= p.st_rows) return;
-  const int64_t row = m / p.hq;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  const bool live = n < p.st_rows;
+  const int64_t kvh = live ? n / p.rg : 0, mrow = live ? n - kvh * p.rg : 0, row = mrow / p.G;
   int n_own = 0;
-  if (p.kv_lens) n_own = min(max((p.kv_lens[row] + own::kSplit - 1) / own::kSplit, 0), p.own_max);
-  const int n = p.n_runs + n_own;
-  float tm = -INFINITY, tl = 0.0f, to[V];   // the groups joined so far
-  float gm = -INFINITY, gl = 0.0f, go[V];   // the open group
+  if (live && p.kv_lens) n_own = min(max((p.kv_lens[row] + own::kSplit - 1) / own::kSplit, 0), p.own_max);
+  const int total = live ? p.n_runs + n_own : 0;
+  const float* src = p.st_o + (static_cast<int64_t>(warp) * Q * p.st_rows + n) * 4;
+  const int64_t quad = p.st_rows * 4, state = quad * (D / 4);
+  float tm = -INFINITY, tl = 0.0f;          // the groups joined so far
+  float gm = -INFINITY, gl = 0.0f;          // the open group
+  float4 to[Q], go[Q];
 #pragma unroll
-  for (int i = 0; i < V; ++i) to[i] = go[i] = 0.0f;
-  for (int s0 = 0; s0 < n; s0 += UN) {
+  for (int i = 0; i < Q; ++i) to[i] = go[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto join4 = [](float4 v, float a, float4 vs, float b) {
+    return make_float4(join(v.x, a, vs.x, b), join(v.y, a, vs.y, b), join(v.z, a, vs.z, b), join(v.w, a, vs.w, b));
+  };
+  for (int s0 = 0; s0 < total; s0 += UN) {
     float2 ml[UN];
-    float o[UN][V];
+    float4 o[UN][Q];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      if (s0 + u < n) {
-        const int64_t idx = (s0 + u) * p.st_rows + m;
-        ml[u] = __ldcg(reinterpret_cast<const float2*>(p.st_ml + 2 * idx));
-        const float* src = p.st_o + idx * D + lane * V;
-        if constexpr (V == 4) {
-          const float4 f = __ldcg(reinterpret_cast<const float4*>(src));
-          o[u][0] = f.x;
-          o[u][1] = f.y;
-          o[u][2] = f.z;
-          o[u][3] = f.w;
-        } else if constexpr (V == 2) {
-          const float2 f = __ldcg(reinterpret_cast<const float2*>(src));
-          o[u][0] = f.x;
-          o[u][1] = f.y;
-        } else {
-          o[u][0] = __ldcg(src);
-        }
+      if (s0 + u < total) {
+        ml[u] = __ldcg(reinterpret_cast<const float2*>(p.st_ml + 2 * ((s0 + u) * p.st_rows + n)));
+#pragma unroll
+        for (int i = 0; i < Q; ++i) o[u][i] = __ldcg(reinterpret_cast<const float4*>(src + (s0 + u) * state + i * quad));
       }
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       const int s = s0 + u;
-      if (s < n) {
+      if (s < total) {
         const bool head = s < p.n_runs ? s % p.per_group == 0 : s == p.n_runs;
-        const bool tail = s < p.n_runs ? (s + 1) % p.per_group == 0 || s + 1 == p.n_runs : s + 1 == n;
+        const bool tail = s < p.n_runs ? (s + 1) % p.per_group == 0 || s + 1 == p.n_runs : s + 1 == total;
         float a = 0.0f, b = 1.0f;
         if (head) {
           gm = ml[u].x;
@@ -674,7 +768,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const Combi
           gl = join(gl, a, ml[u].y, b);
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) go[i] = head ? o[u][i] : join(go[i], a, o[u][i], b);
+        for (int i = 0; i < Q; ++i) go[i] = head ? o[u][i] : join4(go[i], a, o[u][i], b);
         if (tail) {
           const bool only = s < p.per_group && s < p.n_runs;   // the first group
           if (only) {
@@ -685,14 +779,27 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const Combi
             tl = join(tl, a, gl, b);
           }
 #pragma unroll
-          for (int i = 0; i < V; ++i) to[i] = only ? go[i] : join(to[i], a, go[i], b);
+          for (int i = 0; i < Q; ++i) to[i] = only ? go[i] : join4(to[i], a, go[i], b);
         }
       }
     }
   }
-  T* dst = static_cast<T*>(p.out) + row * p.o_sr + (m - row * p.hq) * p.o_sh + lane * V;
 #pragma unroll
-  for (int i = 0; i < V; ++i) dst[i] = from_f32<T>(__fdiv_rn(to[i], tl));
+  for (int i = 0; i < Q; ++i) {
+    T* d = &s_out[lane][(warp * Q + i) * 4];
+    *reinterpret_cast<uint32_t*>(d) = pack2<T>(__fdiv_rn(to[i].x, tl), __fdiv_rn(to[i].y, tl));
+    *reinterpret_cast<uint32_t*>(d + 2) = pack2<T>(__fdiv_rn(to[i].z, tl), __fdiv_rn(to[i].w, tl));
+  }
+  __syncthreads();
+  T* out = static_cast<T*>(p.out);
+#pragma unroll 4
+  for (int k = warp; k < 32; k += C::WARPS) {
+    const int64_t nk = static_cast<int64_t>(blockIdx.x) * 32 + k;
+    if (nk >= p.st_rows) break;
+    const int64_t kh = nk / p.rg, mk = nk - kh * p.rg, rk = mk / p.G;
+    T* dst = out + rk * p.o_sr + (kh * p.G + mk - rk * p.G) * p.o_sh;
+    for (int d = lane; d < D; d += 32) dst[d] = s_out[k][d];
+  }
 }
 
 }  // namespace prefix

@@ -157,10 +157,10 @@ int prefix_launch(const dk::prefix::Maps& maps, const dk::prefix::Params& p, cud
 
 // Follows prefix_launch on the same stream and starts without waiting for it: prefix_kernel has itself
 // waited for whatever wrote the inputs before it lets the next kernel begin.
-template <typename T, int D>
-int own_launch(const dk::own::Params& p, cudaStream_t st) {
+template <typename T, int D, int NB>
+int own_launch_nb(const dk::own::Params& p, cudaStream_t st) {
   using C = dk::own::Cfg<D>;
-  auto fn = dk::own::own_kernel<T, D>;
+  auto fn = dk::own::own_kernel<T, D, NB>;
   static bool done[kMaxDevices] = {false};
   const int dev = current_device();
   if (dev < 0 || dev >= kMaxDevices || !done[dev]) {
@@ -174,11 +174,19 @@ int own_launch(const dk::own::Params& p, cudaStream_t st) {
   return DK_OK;
 }
 
+// Tiles of at most 8 query rows (a row without row_tiles and up to 8 heads a group) take the form of one
+// column half; a query row's bits are the same in either.
+template <typename T, int D>
+int own_launch(const dk::own::Params& p, cudaStream_t st) {
+  if (!p.tiles && p.G <= 8) return own_launch_nb<T, D, 1>(p, st);
+  return own_launch_nb<T, D, 2>(p, st);
+}
+
 template <typename T, int D>
 int combine_launch(const dk::prefix::CombineParams& p, cudaStream_t st) {
-  const int64_t grid = ceil_div(p.st_rows, dk::prefix::kCombineWarps);
+  const int64_t grid = ceil_div(p.st_rows, 32);
   cudaError_t e = launch_pdl(dk::prefix::combine_kernel<T, D>, dim3(static_cast<unsigned>(grid)),
-                             dim3(dk::prefix::kCombineWarps * 32), 0, st, p);
+                             dim3(dk::prefix::CombineCfg<D>::WARPS * 32), 0, st, p);
   if (e != cudaSuccess) return fail(DK_ERR_CUDA, "attention_shared_prefix: launch failed: %s", cudaGetErrorString(e));
   return DK_OK;
 }
@@ -368,8 +376,8 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
   if (n_tiles <= 0) return fail(DK_ERR_INVALID_ARGUMENT, "%s: n_tiles must be positive with row_tiles", what);
   const int64_t st_rows = static_cast<int64_t>(n_rows) * n_q_heads;
   const PrefixPlan pl = plan_prefix(n_rows, n_tiles, n_kv_heads, G, head_dim, prefix_len, max_kv_len);
-  if (ceil_div(st_rows, dk::prefix::kCombineWarps) > kI32Max ||
-      static_cast<int64_t>(n_tiles) * n_kv_heads * (pl.upt > 0 ? pl.upt : 1) > kI32Max)
+  if (st_rows > kI32Max || static_cast<int64_t>(n_tiles) * n_kv_heads * (pl.upt > 0 ? pl.upt : 1) > kI32Max ||
+      static_cast<int64_t>(pl.n_pairs) * n_kv_heads * pl.n_runs > kI32Max - 2 * sm_count(current_device()))
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: too many rows", what);
   const size_t need = prefix_state_bytes(pl, st_rows, head_dim);
   if (!workspace || workspace_bytes < need || !aligned16(workspace))
@@ -468,7 +476,8 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
   c.kv_lens = own ? kv_lens : nullptr;
   c.own_max = pl.own_states;
   c.st_rows = st_rows;
-  c.hq = n_q_heads;
+  c.rg = pl.rg;
+  c.G = G;
   c.out = out;
   c.o_sr = out_stride_row;
   c.o_sh = out_stride_head;
