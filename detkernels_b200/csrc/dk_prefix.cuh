@@ -18,9 +18,9 @@
 // No step looks at another row, so a row's bits do not depend on the batch.
 //
 // Work: an item is (up to two tiles of 128 rows, KV head, run of tokens), one persistent CTA per SM.
-// Warp 8 streams K and V blocks with TMA, warp 9 issues the MMAs, two warpgroups hold one row a
-// thread and do the softmax.  The two tiles of an item share K and V and alternate on the tensor
-// cores; an item of one tile alternates two score buffers instead.  A run is a whole group, whose
+// One warp streams K and V blocks with TMA, one warp a tile issues its MMAs, and a warpgroup a tile does
+// the softmax, a row a thread.  The two tiles of an item share K and V and alternate on the tensor
+// cores; when there is one tile only, it alternates between two score buffers instead.  A run is a whole group, whose
 // chunks are joined in TMEM (which has room for that beside two 64-wide accumulators, not 128-wide
 // ones), or, when that leaves SMs idle, one chunk, whose state combine_kernel joins; both give the
 // same bits.
@@ -39,8 +39,8 @@ using own::pack2;
 
 constexpr int kBlock = 128;      // tokens a block
 constexpr int kRows = 128;       // rows a tile
-constexpr int kSoftThreads = 256;
-constexpr int kThreads = 384;    // two softmax warpgroups; TMA, MMA and two idle warps
+constexpr int kSoftWarps = 8;    // a warpgroup a tile
+constexpr int kThreads = 384;    // softmax warps, then one for TMA, two for MMA and an idle one
 constexpr int kLaunchRegs = 168; // registers a thread at launch; 384 * 168 = 256 * 208 + 128 * 88
 constexpr int kSoftRegs = 208;
 constexpr int kIoRegs = 88;
@@ -56,6 +56,7 @@ enum : int {
   kDetOutFree = 0x626,
   kDetDrain = 0x627,
   kDetDone = 0x628,
+  kDetTurn = 0x629,
   kDetPage = 0x62a,   // a prefix block id outside the pool
 };
 
@@ -76,7 +77,7 @@ struct Params {
   const void* q;
   int64_t q_sr, q_sh;
   int32_t hq, hkv, G;
-  int64_t rg;             // rows * G
+  int32_t rg;             // rows * G
   int32_t prefix_len;
   int32_t chunk_blocks;   // blocks a chunk
   int32_t run_blocks;     // blocks a run: a chunk or a group
@@ -104,7 +105,7 @@ struct Cfg {
   static constexpr int BOX = 64 * 128;            // bytes of a 64-token box
   static constexpr int HALF = 2 * BOX;            // 128 tokens x 64 elements
   static constexpr int STAGE = NH * HALF;         // a K or V block
-  static constexpr int STAGES = D == 128 ? 5 : 8;
+  static constexpr int STAGES = D == 128 ? 4 : 8;
   static constexpr int QTILE = NH * HALF;
   static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * QTILE + 512;
   static constexpr uint32_t S_COL = 0;            // two score buffers of 128 columns
@@ -246,7 +247,7 @@ __device__ __forceinline__ Item item_at(const Params& p, uint32_t w) {
   it.pair = static_cast<int>(w - r * p.n_pairs);
   it.run = static_cast<int>(r / static_cast<uint32_t>(p.hkv));
   it.kvh = static_cast<int>(r - it.run * static_cast<uint32_t>(p.hkv));
-  it.tiles = (static_cast<int64_t>(it.pair) * 2 + 1) * kRows < p.rg ? 2 : 1;
+  it.tiles = (it.pair * 2 + 1) * kRows < p.rg ? 2 : 1;
   it.t_begin = it.run * p.run_blocks * kBlock;
   it.tokens = min(p.prefix_len - it.t_begin, p.run_blocks * kBlock);
   it.n_blocks = (it.tokens + kBlock - 1) / kBlock;
@@ -263,16 +264,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
   uint8_t* s_q = ring + C::STAGES * C::STAGE;
   uint64_t* full = reinterpret_cast<uint64_t*>(s_q + 2 * C::QTILE);
   uint64_t* empty = full + C::STAGES;
-  // score barriers: 0 and 1 by tile, 2 the second buffer of a one-tile item (tile 1's columns); each
+  // score barriers: 0 and 1 by tile, 2 the second buffer of a lone tile (tile 1's columns); each
   // has one warpgroup that waits for every phase of it in order
   uint64_t* s_full = empty + C::STAGES;   // [3]
   uint64_t* p_ready = s_full + 3;         // [3]
-  uint64_t* p_half = p_ready + 3;         // [3] the first 64 tokens' weights are in TMEM
+  uint64_t* p_half = p_ready + 3;         // [3] the first 64 tokens' weights are in TMEM (p_ready: the others')
   uint64_t* o_full = p_half + 3;         // [2] by tile: P.V of a block done
   uint64_t* o_free = o_full + 2;          // [2] by tile: the accumulator has been read
   uint64_t* q_ready = o_free + 2;         // [2] by tile
-  uint64_t* done = q_ready + 2;
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* turn = q_ready + 2;           // [2] by tile: the other tile's issuer has issued its group
+  uint64_t* done = turn + 2;              // [2]
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(done + 2);
 
   // one value for the whole warp as the compiler sees it: the MMA issuer's operands then stay in
   // uniform registers (from per-thread ones each tcgen05.mma took ~140 cycles to issue)
@@ -281,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], 2);   // both MMA issuers
     }
     for (int i = 0; i < 3; ++i) {
       mbar_init(&s_full[i], 1);
@@ -292,15 +294,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
       mbar_init(&o_full[t], 1);
       mbar_init(&o_free[t], 128);
       mbar_init(&q_ready[t], 128);
+      mbar_init(&turn[t], 1);
     }
-    mbar_init(done, 1);
+    mbar_init(&done[0], 1);
+    mbar_init(&done[1], 1);
     fence_mbar_init();
   }
-  if (warp == 8 && lane == 0) {
+  if (warp == kSoftWarps && lane == 0) {
     tma_prefetch_desc(&maps.k);
     tma_prefetch_desc(&maps.v);
   }
-  if (warp == 9) {
+  if (warp == kSoftWarps + 1) {
     tmem_alloc(s_tmem, 512);
     tmem_relinquish();
   }
@@ -312,15 +316,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
   if (threadIdx.x == 0) pdl_launch_dependents();
 
   const uint32_t n_items = static_cast<uint32_t>(p.n_pairs) * p.hkv * p.n_runs;   // < 2^31 (the host checks)
+  // At most 128 rows: tile 0 alone alternates between both score buffers.  (Not in an item whose second
+  // tile is empty while others have two: the buffer is then the other issuer's.)
+  const bool dbl = p.rg <= kRows;
   bool abort_flag = false;
 
-  if (warp >= 8) {
+  if (warp >= kSoftWarps) {
     reg_dec<kIoRegs>();
-    if (warp == 8 && lane == 0) {
+    if (warp == kSoftWarps && lane == 0) {
       // ---------------- TMA producer: K block, V block, K block, ... ----------------
       int stage = 0;
       uint32_t phase = 0;
-      int64_t fills = 0;
+      uint32_t fills = 0;
       for (uint32_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
         const Item it = item_at(p, w);
         for (int b = 0; b < it.n_blocks && !abort_flag; ++b) {
@@ -359,71 +366,73 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
       }
       // every copy has landed before the CTA may end
       bool drain = false;
-      for (int64_t f = (fills > C::STAGES ? fills - C::STAGES : 0); f < fills; ++f)
+      for (uint32_t f = (fills > C::STAGES ? fills - C::STAGES : 0); f < fills; ++f)
         mbar_wait(&full[f % C::STAGES], static_cast<uint32_t>((f / C::STAGES) & 1), kDetDrain, drain);
-    } else if (warp == 9) {
-      // ---------------- MMA issuer ----------------
+    } else if (warp == kSoftWarps + 1 || warp == kSoftWarps + 2) {
+      // ---------------- MMA issuers, one a tile ----------------
+      const int t = warp - (kSoftWarps + 1);
       constexpr uint32_t idesc_s = umma_idesc_f16(FMT, 0, 0, kRows, kBlock);
       constexpr uint32_t idesc_o = umma_idesc_f16(FMT, 0, 1, kRows, C::DP);
-      // descriptors of stage 0 / tile 0; an offset of n bytes adds n / 16
+      // descriptors of stage 0; an offset of n bytes adds n / 16
       const uint64_t k_desc = umma_sdesc(smem_u32(ring), 16, 1024, 2);
       const uint64_t v_desc = umma_sdesc(smem_u32(ring), C::HALF, 1024, 2);
-      const uint64_t q_desc = umma_sdesc(smem_u32(s_q), 16, 1024, 2);
+      const uint64_t q_desc = umma_sdesc(smem_u32(s_q) + t * C::QTILE, 16, 1024, 2);
+      const uint32_t o_col = tmem + C::O_COL + t * C::DP;
       const bool leader = elect_one();
-      int stage = 0;                         // next stage to take: K, V, K, V, ... in the order of the loads
-      uint32_t phase = 0;
-      uint32_t pph = 0;                      // p_ready parities by bit
-      uint32_t qph = 0, oph = 3;             // q_ready, o_free parities by bit (the first o_free wait passes)
-      // scores of tile t, K block in stage st, by score barrier sb
-      auto issue_qk = [&](int t, int sb, int st) {
+      uint32_t fill = 0;                     // stages taken: K, V, K, V, ... in the order of the loads
+      uint32_t pph = 0;                      // weights parities by score barrier
+      uint32_t qph = 0, oph = 1;             // q_ready, o_free parities (the first o_free wait passes)
+      uint32_t tph = t ^ 1;                  // turn parity (tile 0 goes first)
+      auto wait_fill = [&](uint32_t f) {
+        return warp_wait(&full[f % C::STAGES], (f / C::STAGES) & 1, kDetFull, abort_flag);
+      };
+      // scores from the K block of fill f, by score barrier sb
+      auto issue_qk = [&](int sb, uint32_t f) {
         if (leader) {
-          const uint64_t kd = k_desc + static_cast<uint64_t>(st * (C::STAGE / 16));
-          const uint64_t qd = q_desc + static_cast<uint64_t>(t * (C::QTILE / 16));
+          const uint64_t kd = k_desc + static_cast<uint64_t>((f % C::STAGES) * (C::STAGE / 16));
           const uint32_t d = tmem + C::S_COL + (sb ? 128 : 0);
 #pragma unroll
           for (int j = 0; j < C::DP / 16; ++j) {
             const uint64_t off = ((j >> 2) * C::HALF + (j & 3) * 32) / 16;
-            tc_mma_f16(d, qd + off, kd + off, idesc_s, j > 0 ? 1u : 0u);
+            tc_mma_f16(d, q_desc + off, kd + off, idesc_s, j > 0 ? 1u : 0u);
           }
           tc_commit(&s_full[sb]);
+          tc_commit(&empty[f % C::STAGES]);
         }
         __syncwarp();
-      };
-      auto take = [&](int& st) {   // the next stage in order, once it is full
-        st = stage;
-        if (!warp_wait(&full[st], phase, kDetFull, abort_flag)) return false;
-        if (++stage == C::STAGES) {
-          stage = 0;
-          phase ^= 1u;
-        }
-        return true;
       };
       for (uint32_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
         const Item it = item_at(p, w);
         const int nb = it.n_blocks;
-        for (int t = 0; t < it.tiles; ++t) {
-          if (!warp_wait(&q_ready[t], (qph >> t) & 1, kDetQ, abort_flag)) break;
-          qph ^= 1u << t;
+        const uint32_t f0 = fill;            // block b: K in fill f0 + 2 b, V in f0 + 2 b + 1
+        fill += 2 * nb;
+        if (t >= it.tiles) {
+          // not this tile's item: its stages still need this warp's release, in order
+          for (uint32_t f = f0; f != fill; ++f) {
+            if (!wait_fill(f)) break;
+            if (leader) mbar_arrive(&empty[f % C::STAGES]);
+          }
+          continue;
         }
-        if (abort_flag) break;
+        if (!warp_wait(&q_ready[t], qph, kDetQ, abort_flag)) break;
+        qph ^= 1u;
+        if (!wait_fill(f0)) break;
         tc_fence_after();
-        int ks, vs;
-        if (!take(ks)) break;
-        for (int t = 0; t < it.tiles; ++t) issue_qk(t, t, ks);
-        if (leader) tc_commit(&empty[ks]);
-        // a block's V and the next block's K are waited for ahead of their use, while MMAs run
-        if (!take(vs) || (nb > 1 && !take(ks))) break;
+        issue_qk(t, f0);
         int in_chunk = 0;
-        for (int b = 0; b < nb && !abort_flag; ++b) {
+        for (int b = 0; b < nb; ++b) {
           const bool more = b + 1 < nb;
           const bool fresh = in_chunk == 0;      // a new chunk overwrites the accumulator
           if (++in_chunk == p.chunk_blocks) in_chunk = 0;
+          const uint32_t fv = f0 + 2 * b + 1;
+          if (!wait_fill(fv) || (more && !wait_fill(fv + 1))) break;
+          if (dbl && more) issue_qk((b + 1) & 1 ? 2 : 0, fv + 1);   // into the other buffer
           const int valid = min(kBlock, it.tokens - b * kBlock);
           const int steps = (valid + 15) >> 4;   // 16-token steps of P.V that hold a token
           if (valid & 15) {
             // tokens past the prefix inside the last step: zero rows of V (whatever the cache holds
-            // there must not meet their zero weights)
-            uint8_t* vb = ring + vs * C::STAGE;
+            // there must not meet their zero weights); both issuers write the same zeros
+            uint8_t* vb = ring + (fv % C::STAGES) * C::STAGE;
             const int rows = steps * 16 - valid;
             for (int e = lane; e < rows * C::NH * 8; e += 32) {
               const int r = valid + e / (C::NH * 8), c = e % (C::NH * 8);
@@ -432,56 +441,49 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
             fence_proxy_async_smem();
             __syncwarp();
           }
-          if (it.tiles == 1 && more) {   // the next block's scores go to the other buffer
-            issue_qk(0, (b + 1) & 1 ? 2 : 0, ks);
-            if (leader) tc_commit(&empty[ks]);
+          if (fresh) {
+            if (!warp_wait(&o_free[t], oph, kDetOutFree, abort_flag)) break;
+            oph ^= 1u;
           }
-          int vs_next = 0, ks_next = 0;
-          for (int t = 0; t < it.tiles; ++t) {
-            const int sb = it.tiles == 2 ? t : (b & 1 ? 2 : 0);
-            if (fresh) {
-              if (!warp_wait(&o_free[t], (oph >> t) & 1, kDetOutFree, abort_flag)) break;
-              oph ^= 1u << t;
-            }
-            const uint64_t vd = v_desc + static_cast<uint64_t>(vs * (C::STAGE / 16));
-            const uint32_t o = tmem + C::O_COL + t * C::DP, pt = tmem + C::S_COL + (sb ? 128 : 0);
-            // the first half of the weights, then the second
-            if (!warp_wait(&p_half[sb], (pph >> sb) & 1, kDetProbs, abort_flag)) break;
-            tc_fence_after();
-            if (leader) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (j < steps)
-                  mma_ts(o, pt + j * 8, vd + static_cast<uint64_t>(j * (2048 / 16)), idesc_o, (fresh && j == 0) ? 0u : 1u);
-            }
-            __syncwarp();
-            if (!warp_wait(&p_ready[sb], (pph >> sb) & 1, kDetProbs, abort_flag)) break;
-            pph ^= 1u << sb;
-            tc_fence_after();
-            if (leader) {
-#pragma unroll
-              for (int j = 4; j < 8; ++j)
-                if (j < steps)
-                  mma_ts(o, pt + j * 8, vd + static_cast<uint64_t>(j * (2048 / 16)), idesc_o, 1u);
-              tc_commit(&o_full[t]);
-              if (t + 1 == it.tiles) tc_commit(&empty[vs]);
-            }
-            __syncwarp();
-            if (it.tiles == 2 && more) {
-              issue_qk(t, t, ks);
-              if (t == 1 && leader) tc_commit(&empty[ks]);
-            }
-            if (t == 0 && more && (!take(vs_next) || (b + 2 < nb && !take(ks_next)))) break;
+          const int sb = dbl && (b & 1) ? 2 : t;
+          const uint64_t vd = v_desc + static_cast<uint64_t>((fv % C::STAGES) * (C::STAGE / 16));
+          const uint32_t pt = tmem + C::S_COL + (sb ? 128 : 0);
+          // the first half of the weights, then the second
+          if (!warp_wait(&p_half[sb], (pph >> sb) & 1, kDetProbs, abort_flag)) break;
+          if (it.tiles == 2) {
+            // the two issuers take turns, so that one tile's products run under the other's softmax
+            // (left alone they fall into step, and both wait for each)
+            if (!warp_wait(&turn[t], tph, kDetTurn, abort_flag)) break;
+            tph ^= 1u;
           }
-          vs = vs_next;
-          ks = ks_next;
+          tc_fence_after();
+          if (leader) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j < steps)
+                mma_ts(o_col, pt + j * 8, vd + static_cast<uint64_t>(j * (2048 / 16)), idesc_o, (fresh && j == 0) ? 0u : 1u);
+          }
+          __syncwarp();
+          if (!warp_wait(&p_ready[sb], (pph >> sb) & 1, kDetProbs, abort_flag)) break;
+          pph ^= 1u << sb;
+          tc_fence_after();
+          if (leader) {
+#pragma unroll
+            for (int j = 4; j < 8; ++j)
+              if (j < steps) mma_ts(o_col, pt + j * 8, vd + static_cast<uint64_t>(j * (2048 / 16)), idesc_o, 1u);
+            tc_commit(&o_full[t]);
+            tc_commit(&empty[fv % C::STAGES]);
+          }
+          __syncwarp();
+          if (!dbl && more) issue_qk(t, fv + 1);
+          if (it.tiles == 2 && leader) mbar_arrive(&turn[t ^ 1]);
         }
       }
       // all issued MMAs are complete before TMEM is freed
-      if (leader) tc_commit(done);
+      if (leader) tc_commit(&done[t]);
       __syncwarp();
       bool fin = false;
-      warp_wait(done, 0, kDetDone, fin);
+      warp_wait(&done[t], 0, kDetDone, fin);
     }
   } else {
     // ---------------- softmax: one row a thread ----------------
@@ -492,26 +494,33 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
     const uint32_t o_t = tmem + lane_base + C::O_COL + t * C::DP;
     uint32_t sc[2] = {0, 0};                    // score phases consumed: own barrier, second buffer
     uint32_t ocnt = 0;                          // P.V completions of this tile so far
-    // This row's query vector of an item into the swizzled K-major operand tile, asynchronously ...
-    uint8_t* const q_row = s_q + t * C::QTILE + r * 128;
+    // The tile's query rows into the swizzled K-major operand tile, asynchronously: neighbouring threads
+    // take neighbouring chunks of a row ...
+    const int tt = threadIdx.x & 127;
+    constexpr int CPR = C::DP / 8;              // 16-byte chunks a row
+    constexpr int QN = kRows * CPR / 128;       // chunks a thread
+    auto q_at = [&](int i) {
+      const int e = i * 128 + tt, row = e / CPR, c = e % CPR;
+      return s_q + t * C::QTILE + (c >> 3) * C::HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+    };
     auto fetch_q = [&](const Item& it) {
-      const int64_t mrow = (static_cast<int64_t>(it.pair) * 2 + t) * kRows + r;
-      const bool valid = mrow < p.rg;
-      const int64_t row = valid ? mrow / p.G : 0;
-      const T* src = static_cast<const T*>(p.q) + row * p.q_sr +
-                     (it.kvh * p.G + (valid ? mrow - row * p.G : 0)) * p.q_sh;
-#pragma unroll
-      for (int c = 0; c < C::DP / 8; ++c)
-        own::cp_async16(smem_u32(q_row + (c >> 3) * C::HALF + (((c & 7) ^ (r & 7)) << 4)), src + (c < D / 8 ? c * 8 : 0),
-                        valid && c < D / 8);
+#pragma unroll 4
+      for (int i = 0; i < QN; ++i) {
+        const int e = i * 128 + tt, c = e % CPR;
+        const uint32_t mrow = (it.pair * 2 + t) * kRows + e / CPR;
+        const bool valid = mrow < static_cast<uint32_t>(p.rg) && c < D / 8;
+        const uint32_t row = valid ? mrow / static_cast<uint32_t>(p.G) : 0, gh = valid ? mrow - row * p.G : 0;
+        own::cp_async16(smem_u32(q_at(i)), static_cast<const T*>(p.q) + row * p.q_sr + (it.kvh * p.G + gh) * p.q_sh +
+                                               (valid ? c * 8 : 0), valid);
+      }
     };
     // ... and, once there, handed to the tensor cores.
     auto q_here = [&]() {
       asm volatile("cp.async.wait_all;" ::: "memory");
       if (p.flip | p.zero) {
 #pragma unroll 1
-        for (int c = 0; c < D / 8; ++c) {
-          uint4* at = reinterpret_cast<uint4*>(q_row + (c >> 3) * C::HALF + (((c & 7) ^ (r & 7)) << 4));
+        for (int i = 0; i < QN; ++i) {
+          uint4* at = reinterpret_cast<uint4*>(q_at(i));
           uint4 v = *at;
           v.x ^= p.flip;
           v.y ^= p.flip;
@@ -527,13 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
     for (uint32_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
       const Item it = item_at(p, w);
       if (t >= it.tiles) continue;
-      Item next{};                                // the next item that has this tile
-      uint32_t wn = w;
-      do {
-        wn += gridDim.x;
-        if (wn < n_items) next = item_at(p, wn);
-      } while (wn < n_items && t >= next.tiles);
-      const int64_t m0 = (static_cast<int64_t>(it.pair) * 2 + t) * kRows;   // first row of the tile
+      const int m0 = (it.pair * 2 + t) * kRows;   // first row of the tile
       const bool warp_live = m0 + (warp & 3) * 32 < p.rg;
       if (!q_loaded) {   // the CTA's first item with this tile; later ones are fetched ahead
         fetch_q(it);
@@ -544,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
       float m = -INFINITY, l = 0.0f;
       int in_chunk = 0;
       for (int b = 0; b < it.n_blocks; ++b) {
-        const int second = it.tiles == 1 ? (b & 1) : 0;   // a one-tile item's second buffer
+        const int second = dbl ? (b & 1) : 0;
         const int sb = second ? 2 : t;
         const bool first = in_chunk == 0;
         if (++in_chunk == p.chunk_blocks) in_chunk = 0;
@@ -553,7 +556,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
         ++sc[second];
         tc_fence_after();
         const bool last = b + 1 == it.n_blocks;
-        if (last && wn < n_items) fetch_q(next);   // all scores of this item are formed: q's place is free
+        if (last) {   // all scores of this item are formed: q's place is free for the next one with this tile
+          for (uint32_t wn = w + gridDim.x; wn < n_items && !q_loaded; wn += gridDim.x) {
+            const Item next = item_at(p, wn);
+            if (t < next.tiles) {
+              fetch_q(next);
+              q_loaded = true;
+            }
+          }
+        }
         if (warp_live) {
           const uint32_t s_t0 = tmem + lane_base + C::S_COL + (sb ? 128 : 0);
           float s[4][32];
@@ -631,10 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
         tc_fence_before();
         mbar_arrive(&p_ready[sb]);
         ++ocnt;
-        if (last && wn < n_items) {
-          q_here();
-          q_loaded = true;
-        }
+        if (q_loaded) q_here();
         if (in_chunk == 0 || last) {
           // the chunk's state joins the run's, which leaves with the last chunk
           if (!warp_wait(&o_full[t], (ocnt - 1) & 1, kDetOut, abort_flag)) break;
@@ -649,9 +657,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
               run_m = join_weights(run_m, m, wa, wb);
               run_l = join(run_l, wa, l, wb);
             }
-            const int64_t mrow = m0 + r;
-            const bool valid_row = mrow < p.rg;
-            const int64_t n = it.kvh * p.rg + mrow;   // state row
+            const bool valid_row = m0 + r < p.rg;
+            const int n = it.kvh * p.rg + m0 + r;   // state row
             if (last && valid_row)
               *reinterpret_cast<float2*>(p.st_ml + 2 * (it.run * p.st_rows + n)) = make_float2(run_m, run_l);
             float* dst = p.st_o + (static_cast<int64_t>(it.run) * (D / 4) * p.st_rows + n) * 4;
@@ -689,14 +696,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kSoftWarps + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
 }
 
 // out[row, head] = O / l of the joined states: the prefix's runs (per_group of them at a time), then
-// the row's own tokens.  A CTA takes 32 state rows, a lane each; its warps split the columns in fours
+// the row's own tokens.  A CTA takes 32 state rows, a lane each; its warps take four columns each
 // (one coalesced load a state), and the outputs go through shared memory so that a head's row leaves
 // whole.
 struct CombineParams {
@@ -711,94 +718,83 @@ struct CombineParams {
   int64_t o_sr, o_sh;
 };
 
-template <int D>
-struct CombineCfg {
-  static constexpr int WARPS = D / 16;        // 4 column quads a warp
-  static constexpr int PAD = D + 2;           // 16-bit elements a row of the output buffer
-};
+constexpr int kCombineCols = 32;   // columns a CTA takes of its 32 state rows, four a warp
 
 template <typename T, int D>
-__global__ void __launch_bounds__(CombineCfg<D>::WARPS * 32) combine_kernel(const CombineParams p) {
-  using C = CombineCfg<D>;
-  constexpr int Q = 4;      // column quads a thread
-  constexpr int UN = 4;     // states in flight
-  __shared__ __align__(16) T s_out[32][C::PAD];
+__global__ void __launch_bounds__(kCombineCols * 8) combine_kernel(const CombineParams p) {
+  constexpr int UN = 8;     // states in flight
+  __shared__ __align__(16) T s_out[32][kCombineCols + 2];
   pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t n = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   const bool live = n < p.st_rows;
-  const int64_t kvh = live ? n / p.rg : 0, mrow = live ? n - kvh * p.rg : 0, row = mrow / p.G;
+  const int quad = static_cast<int>(blockIdx.y) * (kCombineCols / 4) + warp;
+  const uint32_t rg = static_cast<uint32_t>(p.rg), G = static_cast<uint32_t>(p.G);
+  const uint32_t mrow = live ? static_cast<uint32_t>(n) % rg : 0;
   int n_own = 0;
-  if (live && p.kv_lens) n_own = min(max((p.kv_lens[row] + own::kSplit - 1) / own::kSplit, 0), p.own_max);
+  if (live && p.kv_lens) n_own = min(max((p.kv_lens[mrow / G] + own::kSplit - 1) / own::kSplit, 0), p.own_max);
   const int total = live ? p.n_runs + n_own : 0;
-  const float* src = p.st_o + (static_cast<int64_t>(warp) * Q * p.st_rows + n) * 4;
-  const int64_t quad = p.st_rows * 4, state = quad * (D / 4);
+  const float* src = p.st_o + (static_cast<int64_t>(quad) * p.st_rows + n) * 4;
+  const int64_t state = p.st_rows * D;
   float tm = -INFINITY, tl = 0.0f;          // the groups joined so far
   float gm = -INFINITY, gl = 0.0f;          // the open group
-  float4 to[Q], go[Q];
-#pragma unroll
-  for (int i = 0; i < Q; ++i) to[i] = go[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float4 to = make_float4(0.0f, 0.0f, 0.0f, 0.0f), go = to;
   auto join4 = [](float4 v, float a, float4 vs, float b) {
     return make_float4(join(v.x, a, vs.x, b), join(v.y, a, vs.y, b), join(v.z, a, vs.z, b), join(v.w, a, vs.w, b));
   };
+  int in_group = 0;
   for (int s0 = 0; s0 < total; s0 += UN) {
     float2 ml[UN];
-    float4 o[UN][Q];
+    float4 o[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       if (s0 + u < total) {
         ml[u] = __ldcg(reinterpret_cast<const float2*>(p.st_ml + 2 * ((s0 + u) * p.st_rows + n)));
-#pragma unroll
-        for (int i = 0; i < Q; ++i) o[u][i] = __ldcg(reinterpret_cast<const float4*>(src + (s0 + u) * state + i * quad));
+        o[u] = __ldcg(reinterpret_cast<const float4*>(src + (s0 + u) * state));
       }
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       const int s = s0 + u;
       if (s < total) {
-        const bool head = s < p.n_runs ? s % p.per_group == 0 : s == p.n_runs;
-        const bool tail = s < p.n_runs ? (s + 1) % p.per_group == 0 || s + 1 == p.n_runs : s + 1 == total;
-        float a = 0.0f, b = 1.0f;
-        if (head) {
+        float a, b;
+        if (in_group == 0) {
           gm = ml[u].x;
           gl = ml[u].y;
+          go = o[u];
         } else {
           gm = join_weights(gm, ml[u].x, a, b);
           gl = join(gl, a, ml[u].y, b);
+          go = join4(go, a, o[u], b);
         }
-#pragma unroll
-        for (int i = 0; i < Q; ++i) go[i] = head ? o[u][i] : join4(go[i], a, o[u][i], b);
-        if (tail) {
-          const bool only = s < p.per_group && s < p.n_runs;   // the first group
-          if (only) {
+        ++in_group;
+        if (s < p.n_runs ? in_group == p.per_group || s + 1 == p.n_runs : s + 1 == total) {
+          in_group = 0;
+          if (s < p.per_group && s < p.n_runs) {   // the first group
             tm = gm;
             tl = gl;
+            to = go;
           } else {
             tm = join_weights(tm, gm, a, b);
             tl = join(tl, a, gl, b);
+            to = join4(to, a, go, b);
           }
-#pragma unroll
-          for (int i = 0; i < Q; ++i) to[i] = only ? go[i] : join4(to[i], a, go[i], b);
         }
       }
     }
   }
-#pragma unroll
-  for (int i = 0; i < Q; ++i) {
-    T* d = &s_out[lane][(warp * Q + i) * 4];
-    *reinterpret_cast<uint32_t*>(d) = pack2<T>(__fdiv_rn(to[i].x, tl), __fdiv_rn(to[i].y, tl));
-    *reinterpret_cast<uint32_t*>(d + 2) = pack2<T>(__fdiv_rn(to[i].z, tl), __fdiv_rn(to[i].w, tl));
-  }
+  *reinterpret_cast<uint32_t*>(&s_out[lane][warp * 4]) = pack2<T>(__fdiv_rn(to.x, tl), __fdiv_rn(to.y, tl));
+  *reinterpret_cast<uint32_t*>(&s_out[lane][warp * 4 + 2]) = pack2<T>(__fdiv_rn(to.z, tl), __fdiv_rn(to.w, tl));
   __syncthreads();
-  T* out = static_cast<T*>(p.out);
-#pragma unroll 4
-  for (int k = warp; k < 32; k += C::WARPS) {
+  T* out = static_cast<T*>(p.out) + blockIdx.y * kCombineCols + lane;
+#pragma unroll
+  for (int k = warp; k < 32; k += kCombineCols / 4) {
     const int64_t nk = static_cast<int64_t>(blockIdx.x) * 32 + k;
-    if (nk >= p.st_rows) break;
-    const int64_t kh = nk / p.rg, mk = nk - kh * p.rg, rk = mk / p.G;
-    T* dst = out + rk * p.o_sr + (kh * p.G + mk - rk * p.G) * p.o_sh;
-    for (int d = lane; d < D; d += 32) dst[d] = s_out[k][d];
+    if (nk < p.st_rows) {
+      const uint32_t kh = static_cast<uint32_t>(nk) / rg, mk = static_cast<uint32_t>(nk) - kh * rg, rk = mk / G;
+      out[rk * p.o_sr + (kh * G + mk - rk * G) * p.o_sh] = s_out[k][lane];
+    }
   }
 }
 

@@ -185,8 +185,8 @@ int own_launch(const dk::own::Params& p, cudaStream_t st) {
 template <typename T, int D>
 int combine_launch(const dk::prefix::CombineParams& p, cudaStream_t st) {
   const int64_t grid = ceil_div(p.st_rows, 32);
-  cudaError_t e = launch_pdl(dk::prefix::combine_kernel<T, D>, dim3(static_cast<unsigned>(grid)),
-                             dim3(dk::prefix::CombineCfg<D>::WARPS * 32), 0, st, p);
+  cudaError_t e = launch_pdl(dk::prefix::combine_kernel<T, D>, dim3(static_cast<unsigned>(grid), D / 32),
+                             dim3(dk::prefix::kCombineCols * 8), 0, st, p);
   if (e != cudaSuccess) return fail(DK_ERR_CUDA, "attention_shared_prefix: launch failed: %s", cudaGetErrorString(e));
   return DK_OK;
 }
@@ -392,7 +392,7 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
   p.hq = n_q_heads;
   p.hkv = n_kv_heads;
   p.G = G;
-  p.rg = pl.rg;
+  p.rg = static_cast<int32_t>(pl.rg);
   p.prefix_len = prefix_len;
   p.chunk_blocks = pl.chunk_blocks;
   p.run_blocks = pl.run_blocks;
