@@ -97,9 +97,9 @@ PrefixPlan plan_prefix(int64_t n_rows, int64_t n_tiles, int64_t hkv, int64_t G, 
   PrefixPlan pl{};
   const int sms = sm_count(current_device());
   pl.rg = n_rows * G;
-  pl.chunk_blocks = static_cast<int>(dk::prefix::chunk_tokens(prefix_len, static_cast<int>(head_dim)) /
-                                     dk::prefix::kBlock);
-  const int64_t blocks = ceil_div(prefix_len, dk::prefix::kBlock);
+  const int block = dk::prefix::block_tokens(static_cast<int>(head_dim));
+  pl.chunk_blocks = static_cast<int>(dk::prefix::chunk_tokens(prefix_len, static_cast<int>(head_dim)) / block);
+  const int64_t blocks = ceil_div(prefix_len, block);
   pl.n_chunks = static_cast<int>(ceil_div(blocks, pl.chunk_blocks));
   pl.n_pairs = static_cast<int>(ceil_div(pl.rg, 2 * dk::prefix::kRows));
   const int gc = dk::prefix::group_chunks(static_cast<int>(head_dim));
@@ -185,8 +185,9 @@ int own_launch(const dk::own::Params& p, cudaStream_t st) {
 template <typename T, int D>
 int combine_launch(const dk::prefix::CombineParams& p, cudaStream_t st) {
   const int64_t grid = ceil_div(p.st_rows, 32);
-  cudaError_t e = launch_pdl(dk::prefix::combine_kernel<T, D>, dim3(static_cast<unsigned>(grid), D / 32),
-                             dim3(dk::prefix::kCombineCols * 8), 0, st, p);
+  cudaError_t e = launch_pdl(dk::prefix::combine_kernel<T, D>, 
+                             dim3(static_cast<unsigned>(grid), D / dk::prefix::CombineCfg<D>::COLS),
+                             dim3(dk::prefix::kCombineThreads), 0, st, p);
   if (e != cudaSuccess) return fail(DK_ERR_CUDA, "attention_shared_prefix: launch failed: %s", cudaGetErrorString(e));
   return DK_OK;
 }
@@ -392,6 +393,7 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
   p.hq = n_q_heads;
   p.hkv = n_kv_heads;
   p.G = G;
+  p.g_magic = ((1ull << 36) + G - 1) / G;
   p.rg = static_cast<int32_t>(pl.rg);
   p.prefix_len = prefix_len;
   p.chunk_blocks = pl.chunk_blocks;
@@ -478,6 +480,7 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
   c.st_rows = st_rows;
   c.rg = pl.rg;
   c.G = G;
+  c.g_magic = p.g_magic;
   c.out = out;
   c.o_sr = out_stride_row;
   c.o_sh = out_stride_head;
