@@ -71,8 +71,8 @@ __host__ __device__ constexpr int group_chunks(int head_dim) { return head_dim <
 // batch enough items to fill the SMs; every chunk of a 128-wide head costs each row a 512-byte state
 // through memory, so those are longer.
 __host__ __device__ inline int64_t chunk_tokens(int64_t prefix_len, int head_dim) {
-  if (head_dim <= 64) return 512 * ((prefix_len + 16383) / 16384);
-  if (prefix_len <= 4096) return 512;
+  if (prefix_len <= 2048) return 512;
+  if (head_dim <= 64) return 1024 * ((prefix_len + 32767) / 32768);
   if (prefix_len <= 16384) return 1024;
   return ((prefix_len + 15) / 16 + 127) / 128 * 128;
 }

@@ -15,7 +15,7 @@ def _tol_check(got, q, kp, vp, ks, vs, scale):
     """Row by row against f64.  With A = sum p |v| / sum p and half a step h = eps / 2 of the type: the
     rounded weights move the result by at most 2 h A (h in the sums of products, and h in the own tokens'
     sum of weights), a score's f32 dot product of D terms is off by at most D 2^-24 sum |q k| scale =: E,
-    which moves weights and their sum by E each, the f32 sums of a chunk by 2 (512 + 64) 2^-24 A, and the
+    which moves weights and their sum by E each, the f32 sums of a chunk by 2 (1024 or a sixteenth of the prefix, + 64) 2^-24 A, and the
     store rounds once.  (ks, vs: a row's own tokens [H_kv, n, D], n may be 0.)"""
     import torch
     R, H, D = got.shape
@@ -29,7 +29,7 @@ def _tol_check(got, q, kp, vp, ks, vs, scale):
         p = torch.softmax(s, -1)
         want = (p[:, None] @ v)[:, 0]
         A = (p[:, None] @ v.abs())[:, 0]
-        chunk = 512 * max(1, -(-kp.shape[1] // 16384))
+        chunk = max(1024, kp.shape[1] // 16 + 128)
         tol = eps / 2 * want.abs() + A * (eps + 2 * E + 2 * (chunk + 64) * 2.0 ** -24)
         if got.dtype == torch.float16:
             tol = tol + 2.0 ** -25 + v.abs().amax() * 2.0 ** -24    # subnormal weights and results
