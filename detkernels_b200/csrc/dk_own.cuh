@@ -12,8 +12,8 @@
 // its 8 columns), so up to 8 query rows a tile cost half the MMAs and registers of the upright form;
 // a column's bits do not depend on the others, so tiles of 16 rows (two column halves) give the same.
 // K and V come through a ring of 16-token stages (cp.async, zero filled past the sequence's end, so
-// that whatever the cache holds there is never read).  A warp that owns all splits joins them in
-// registers; otherwise every split leaves its state for combine_kernel.
+// that whatever the cache holds there is never read).  A warp that owns all splits joins them in its
+// shared memory; otherwise every split leaves its state for combine_kernel.
 #pragma once
 
 #include <type_traits>
@@ -87,7 +87,9 @@ struct Cfg {
   static constexpr int TENSOR = kStep * ROWB;
   static constexpr int STAGE = 2 * TENSOR;
   static constexpr int STAGES = D == 128 ? 3 : 4;
-  static constexpr int SMEM = STAGES * STAGE;
+  // the ring, then (joined splits, when a warp owns all of them) 8 NB rows of D floats, a lane's own apart
+  static constexpr int RING = STAGES * STAGE;
+  static constexpr int smem(int nb, bool direct) { return RING + (direct ? 8 * nb * D * 4 : 0); }
 };
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
@@ -155,7 +157,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {   // an 8 x 8 matri
 
 // NB: column halves (8 query rows each).
 template <typename T, int D, int NB>
-__global__ void __launch_bounds__(32) own_kernel(const Params p) {
+__global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 14) : (D == 128 ? 12 : 16)) own_kernel(const Params p) {
   using C = Cfg<D>;
   constexpr int KC = D / 16, CPR = D / 8;
   constexpr int PER = kStep * CPR / 32;   // 16-byte chunks a lane copies of each tensor a step
@@ -167,13 +169,13 @@ __global__ void __launch_bounds__(32) own_kernel(const Params p) {
   w /= p.hkv;
   const int unit = static_cast<int>(w % p.upt);
   const int tile = static_cast<int>(w / p.upt);
+  // every exit waits for the kernel before this one (see the launch)
   int r0 = tile, nr = 1, seq = tile;
   if (p.tiles) {
     r0 = p.tiles[3 * tile];
     nr = p.tiles[3 * tile + 1];
     seq = p.tiles[3 * tile + 2];
   }
-  // every exit waits for the kernel before this one (see the launch)
   if (nr < 1 || nr * p.G > 8 * NB || r0 < 0 || r0 + nr > p.n_rows || seq < 0 || seq >= p.n_seq) {
     if (lane == 0 && unit == 0 && kvh == 0) report_error(DK_ERR_DEVICE_CHECK, kDetTile);
     pdl_wait();
@@ -275,14 +277,15 @@ __global__ void __launch_bounds__(32) own_kernel(const Params p) {
   const int v_row = (mi >> 1) * 8 + ri, v_c = mi & 1;   // V transposed: d halves, then token halves
 
   float o[NB][KC][4], m_r[NB][2], l_r[NB][2];
-  float run_o[NB][KC][4], run_m[NB][2], run_l[NB][2];
+  float run_m[NB][2], run_l[NB][2];
   const bool direct = p.upt == 1;
+  float* const run_o = reinterpret_cast<float*>(ring + C::RING) + lane;   // [h][j][e] 32 apart
 #pragma unroll
   for (int h = 0; h < NB; ++h) {
 #pragma unroll
     for (int j = 0; j < KC; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[h][j][e] = run_o[h][j][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) o[h][j][e] = 0.0f;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       m_r[h][e] = run_m[h][e] = -INFINITY;
@@ -291,14 +294,14 @@ __global__ void __launch_bounds__(32) own_kernel(const Params p) {
   }
 
   const int64_t n0 = (static_cast<int64_t>(kvh) * p.n_rows + r0) * p.G + 2 * t4;   // state row of column 2 t4
-  auto store = [&](int64_t s, int h, int e, float m, float l, const float (&a)[KC][4]) {
+  auto store = [&](int64_t s, int h, int e, float m, float l, auto&& a) {
     const int64_t n = n0 + 8 * h + e;
     if (g == 0) *reinterpret_cast<float2*>(p.st_ml + 2 * (s * p.st_rows + n)) = make_float2(m, l);
     float* dst = p.st_o + ((s * (D / 4) + (g >> 2)) * p.st_rows + n) * 4 + (g & 3);
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
-      dst[static_cast<int64_t>(4 * j) * p.st_rows * 4] = a[j][e];
-      dst[static_cast<int64_t>(4 * j + 2) * p.st_rows * 4] = a[j][2 + e];
+      dst[static_cast<int64_t>(4 * j) * p.st_rows * 4] = a(j, e);
+      dst[static_cast<int64_t>(4 * j + 2) * p.st_rows * 4] = a(j, 2 + e);
     }
   };
 
@@ -419,14 +422,14 @@ __global__ void __launch_bounds__(32) own_kernel(const Params p) {
           l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 16));
           if (sp_begin < end[h][e]) {        // the row has tokens in this split
             if (!direct) {
-              store(sp_begin / kSplit, h, e, m_r[h][e], l, o[h]);
+              store(sp_begin / kSplit, h, e, m_r[h][e], l, [&](int j, int i) { return o[h][j][i]; });
             } else if (sp_begin == 0) {
               run_m[h][e] = m_r[h][e];
               run_l[h][e] = l;
 #pragma unroll
               for (int j = 0; j < KC; ++j) {
-                run_o[h][j][e] = o[h][j][e];
-                run_o[h][j][2 + e] = o[h][j][2 + e];
+                run_o[((h * KC + j) * 4 + e) * 32] = o[h][j][e];
+                run_o[((h * KC + j) * 4 + 2 + e) * 32] = o[h][j][2 + e];
               }
             } else {
               float a, b;
@@ -434,8 +437,10 @@ __global__ void __launch_bounds__(32) own_kernel(const Params p) {
               run_l[h][e] = join(run_l[h][e], a, l, b);
 #pragma unroll
               for (int j = 0; j < KC; ++j) {
-                run_o[h][j][e] = join(run_o[h][j][e], a, o[h][j][e], b);
-                run_o[h][j][2 + e] = join(run_o[h][j][2 + e], a, o[h][j][2 + e], b);
+                float& r0 = run_o[((h * KC + j) * 4 + e) * 32];
+                float& r1 = run_o[((h * KC + j) * 4 + 2 + e) * 32];
+                r0 = join(r0, a, o[h][j][e], b);
+                r1 = join(r1, a, o[h][j][2 + e], b);
               }
             }
           }
@@ -455,7 +460,8 @@ __global__ void __launch_bounds__(32) own_kernel(const Params p) {
     for (int h = 0; h < NB; ++h)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        if (end[h][e] > 0) store(0, h, e, run_m[h][e], run_l[h][e], run_o[h]);
+        if (end[h][e] > 0)
+          store(0, h, e, run_m[h][e], run_l[h][e], [&](int j, int i) { return run_o[((h * KC + j) * 4 + i) * 32]; });
   }
   pdl_wait();
 }

@@ -701,17 +701,17 @@ struct CombineParams {
   int64_t o_sr, o_sh;
 };
 
-constexpr int kCombineThreads = 256;
-template <int D>
+// Q: column quads a thread; UN: states a batch (the next batch is in flight while one is joined).  Many CTAs
+// keep memory busy with wide threads (4, 2), few with deep ones (1, 8).
+template <int D, int Q>
 struct CombineCfg {
-  static constexpr int COLS = D < 64 ? D : 64;   // columns a CTA takes of its 32 state rows
-  static constexpr int Q = COLS / 32;            // column quads a thread
+  static constexpr int WARPS = Q == 1 ? 8 : D / 4 / Q;
+  static constexpr int COLS = WARPS * Q * 4;   // columns a CTA takes of its 32 state rows
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kCombineThreads, 3) combine_kernel(const CombineParams p) {
-  using C = CombineCfg<D>;
-  constexpr int UN = 4, Q = C::Q;     // states in flight
+template <typename T, int D, int Q, int UN>
+__global__ void __launch_bounds__(CombineCfg<D, Q>::WARPS * 32) combine_kernel(const CombineParams p) {
+  using C = CombineCfg<D, Q>;
   __shared__ __align__(16) T s_out[32][C::COLS + 2];
   pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
@@ -720,14 +720,30 @@ __global__ void __launch_bounds__(kCombineThreads, 3) combine_kernel(const Combi
   const bool live = n < p.st_rows;
   const int quad = static_cast<int>(blockIdx.y) * (C::COLS / 4) + warp * Q;
   const uint32_t rg = static_cast<uint32_t>(p.rg);
-  const uint32_t kvh0 = live ? static_cast<uint32_t>(n) / rg : 0, mrow = live ? static_cast<uint32_t>(n) - kvh0 * rg : 0;
-  int n_own = 0;
-  if (live && p.kv_lens)
-    n_own = min(max((p.kv_lens[div_g(mrow, p.g_magic)] + own::kSplit - 1) / own::kSplit, 0), p.own_max);
-  const int total = live ? p.n_runs + n_own : 0;
   const float4* src = reinterpret_cast<const float4*>(p.st_o) + static_cast<int64_t>(quad) * p.st_rows + n;
   const float2* mls = reinterpret_cast<const float2*>(p.st_ml) + n;
   const int64_t state = p.st_rows * (D / 4);
+  float2 ml[2][UN];
+  float4 o[2][UN][Q];
+  auto fetch = [&](int buf, int s0, int begin, int end) {   // states s0 .. s0 + UN - 1 that lie in [begin, end)
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      if (s0 + u >= begin && s0 + u < end) {
+        ml[buf][u] = __ldcg(mls + (s0 + u) * p.st_rows);
+#pragma unroll
+        for (int i = 0; i < Q; ++i) o[buf][u][i] = __ldcg(src + (s0 + u) * state + i * p.st_rows);
+      }
+    }
+  };
+  const int runs = live ? p.n_runs : 0;
+  fetch(0, 0, 0, runs);        // the prefix's states do not wait for the row's length
+  int n_own = 0;
+  if (live && p.kv_lens) {
+    const uint32_t mrow = static_cast<uint32_t>(n) % rg;
+    n_own = min(max((p.kv_lens[div_g(mrow, p.g_magic)] + own::kSplit - 1) / own::kSplit, 0), p.own_max);
+  }
+  const int total = runs + n_own;
+  fetch(0, 0, runs, total);
   float tm = -INFINITY, tl = 0.0f;          // the groups joined so far
   float gm = -INFINITY, gl = 0.0f;          // the open group
   float4 to[Q], go[Q];
@@ -737,46 +753,38 @@ __global__ void __launch_bounds__(kCombineThreads, 3) combine_kernel(const Combi
     return make_float4(join(v.x, a, vs.x, b), join(v.y, a, vs.y, b), join(v.z, a, vs.z, b), join(v.w, a, vs.w, b));
   };
   int in_group = 0;
-  for (int s0 = 0; s0 < total; s0 += UN) {
-    float2 ml[UN];
-    float4 o[UN][Q];
+  for (int s0 = 0; s0 < total; s0 += 2 * UN) {
 #pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      if (s0 + u < total) {
-        ml[u] = __ldcg(mls + (s0 + u) * p.st_rows);
+    for (int buf = 0; buf < 2; ++buf) {
+      fetch(buf ^ 1, s0 + (buf + 1) * UN, 0, total);
 #pragma unroll
-        for (int i = 0; i < Q; ++i) o[u][i] = __ldcg(src + (s0 + u) * state + i * p.st_rows);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      const int s = s0 + u;
-      if (s < total) {
-        float a, b;
-        if (in_group == 0) {
-          gm = ml[u].x;
-          gl = ml[u].y;
-#pragma unroll
-          for (int i = 0; i < Q; ++i) go[i] = o[u][i];
-        } else {
-          gm = join_weights(gm, ml[u].x, a, b);
-          gl = join(gl, a, ml[u].y, b);
-#pragma unroll
-          for (int i = 0; i < Q; ++i) go[i] = join4(go[i], a, o[u][i], b);
-        }
-        ++in_group;
-        if (s < p.n_runs ? in_group == p.per_group || s + 1 == p.n_runs : s + 1 == total) {
-          in_group = 0;
-          if (s < p.per_group && s < p.n_runs) {   // the first group
-            tm = gm;
-            tl = gl;
-#pragma unroll
-            for (int i = 0; i < Q; ++i) to[i] = go[i];
+      for (int u = 0; u < UN; ++u) {
+        const int s = s0 + buf * UN + u;
+        if (s < total) {
+          float a = 0.0f, b = 1.0f;
+          const bool head = in_group == 0;
+          if (head) {
+            gm = ml[buf][u].x;
+            gl = ml[buf][u].y;
           } else {
-            tm = join_weights(tm, gm, a, b);
-            tl = join(tl, a, gl, b);
+            gm = join_weights(gm, ml[buf][u].x, a, b);
+            gl = join(gl, a, ml[buf][u].y, b);
+          }
 #pragma unroll
-            for (int i = 0; i < Q; ++i) to[i] = join4(to[i], a, go[i], b);
+          for (int i = 0; i < Q; ++i) go[i] = head ? o[buf][u][i] : join4(go[i], a, o[buf][u][i], b);
+          ++in_group;
+          if (s < p.n_runs ? in_group == p.per_group || s + 1 == p.n_runs : s + 1 == total) {
+            in_group = 0;
+            const bool only = s < p.per_group && s < p.n_runs;   // the first group
+            if (only) {
+              tm = gm;
+              tl = gl;
+            } else {
+              tm = join_weights(tm, gm, a, b);
+              tl = join(tl, a, gl, b);
+            }
+#pragma unroll
+            for (int i = 0; i < Q; ++i) to[i] = only ? go[i] : join4(to[i], a, go[i], b);
           }
         }
       }
@@ -789,15 +797,15 @@ __global__ void __launch_bounds__(kCombineThreads, 3) combine_kernel(const Combi
     *reinterpret_cast<uint32_t*>(d + 2) = pack2<T>(__fdiv_rn(to[i].z, tl), __fdiv_rn(to[i].w, tl));
   }
   __syncthreads();
-  T* out = static_cast<T*>(p.out) + blockIdx.y * C::COLS;
+  T* out = static_cast<T*>(p.out) + blockIdx.y * C::COLS + lane;
 #pragma unroll
-  for (int k = warp; k < 32; k += kCombineThreads / 32) {
+  for (int k = warp; k < 32; k += C::WARPS) {
     const uint32_t nk = blockIdx.x * 32u + k;
     if (nk < p.st_rows) {
       const uint32_t kh = nk / rg, mk = nk - kh * rg, rk = div_g(mk, p.g_magic);
       T* dst = out + rk * p.o_sr + (kh * p.G + mk - rk * p.G) * p.o_sh;
 #pragma unroll
-      for (int d = 0; d < C::COLS; d += 32) dst[d + lane] = s_out[k][d + lane];
+      for (int d = 0; d < C::COLS; d += 32) dst[d] = s_out[k][lane + d];
     }
   }
 }

@@ -161,6 +161,7 @@ template <typename T, int D, int NB>
 int own_launch_nb(const dk::own::Params& p, cudaStream_t st) {
   using C = dk::own::Cfg<D>;
   auto fn = dk::own::own_kernel<T, D, NB>;
+  const int smem = C::smem(NB, p.upt == 1);
   static bool done[kMaxDevices] = {false};
   const int dev = current_device();
   if (dev < 0 || dev >= kMaxDevices || !done[dev]) {
@@ -169,7 +170,7 @@ int own_launch_nb(const dk::own::Params& p, cudaStream_t st) {
     if (dev >= 0 && dev < kMaxDevices) done[dev] = true;
   }
   const int64_t grid = static_cast<int64_t>(p.n_tiles) * p.upt * p.hkv;
-  cudaError_t e = launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(32), C::SMEM, st, p);
+  cudaError_t e = launch_pdl(fn, dim3(static_cast<unsigned>(grid)), dim3(32), smem, st, p);
   if (e != cudaSuccess) return fail(DK_ERR_CUDA, "attention_shared_prefix: launch failed: %s", cudaGetErrorString(e));
   return DK_OK;
 }
@@ -182,14 +183,21 @@ int own_launch(const dk::own::Params& p, cudaStream_t st) {
   return own_launch_nb<T, D, 2>(p, st);
 }
 
-template <typename T, int D>
-int combine_launch(const dk::prefix::CombineParams& p, cudaStream_t st) {
-  const int64_t grid = ceil_div(p.st_rows, 32);
-  cudaError_t e = launch_pdl(dk::prefix::combine_kernel<T, D>, 
-                             dim3(static_cast<unsigned>(grid), D / dk::prefix::CombineCfg<D>::COLS),
-                             dim3(dk::prefix::kCombineThreads), 0, st, p);
+template <typename T, int D, int Q, int UN>
+int combine_launch_q(const dk::prefix::CombineParams& p, cudaStream_t st) {
+  using C = dk::prefix::CombineCfg<D, Q>;
+  cudaError_t e = launch_pdl(dk::prefix::combine_kernel<T, D, Q, UN>,
+                             dim3(static_cast<unsigned>(ceil_div(p.st_rows, 32)), D / C::COLS), dim3(C::WARPS * 32), 0,
+                             st, p);
   if (e != cudaSuccess) return fail(DK_ERR_CUDA, "attention_shared_prefix: launch failed: %s", cudaGetErrorString(e));
   return DK_OK;
+}
+
+// Few CTAs (two an SM at most): one quad a thread and deep batches, since nothing else covers a batch's latency.
+template <typename T, int D>
+int combine_launch(const dk::prefix::CombineParams& p, cudaStream_t st) {
+  if (ceil_div(p.st_rows, 32) * (D / 32) <= 2LL * sm_count(current_device())) return combine_launch_q<T, D, 1, 8>(p, st);
+  return combine_launch_q<T, D, 4, 2>(p, st);
 }
 
 }  // namespace
