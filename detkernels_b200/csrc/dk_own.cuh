@@ -13,7 +13,8 @@
 // a column's bits do not depend on the others, so tiles of 16 rows (two column halves) give the same.
 // K and V come through a ring of 16-token stages (cp.async, zero filled past the sequence's end, so
 // that whatever the cache holds there is never read).  A warp that owns all splits joins them in its
-// shared memory; otherwise every split leaves its state for combine_kernel.
+// shared memory, then with the prefix's states, and writes the output; otherwise every split leaves its
+// state for combine_kernel.
 #pragma once
 
 #include <type_traits>
@@ -62,6 +63,9 @@ __device__ __forceinline__ float join_weights(float m, float ms, float& a, float
   return mn;
 }
 __device__ __forceinline__ float join(float v, float a, float vs, float b) { return __fmaf_rn(v, a, __fmul_rn(vs, b)); }
+__device__ __forceinline__ float4 join4(float4 v, float a, float4 vs, float b) {
+  return make_float4(join(v.x, a, vs.x, b), join(v.y, a, vs.y, b), join(v.z, a, vs.z, b), join(v.w, a, vs.w, b));
+}
 
 struct Params {
   const void *q, *k, *v;
@@ -76,9 +80,15 @@ struct Params {
   int32_t page, n_blocks;
   int32_t max_splits, spu, upt;   // splits a unit, units a (tile, head)
   float scale_log2;
-  float* st_o;                // [max_splits, or 1 when upt == 1][D / 4][st_rows][4]
-  float* st_ml;               // [..][st_rows][2]
+  float* st_o;                // [max_splits][D / 4][st_rows][4], when out is null
+  float* st_ml;               // [max_splits][st_rows][2]
   int64_t st_rows;            // hkv * rows * G: state row (kvh * rows + row) * G + head in the group
+  // upt == 1: a unit owns all of its rows' splits, joins them with the prefix's states and writes the output
+  void* out;
+  int64_t o_sr, o_sh;
+  const float* px_o;          // [n_runs][D / 4][st_rows][4]
+  const float* px_ml;         // [n_runs][st_rows][2]
+  int32_t n_runs, per_group;
 };
 
 template <int D>
@@ -87,9 +97,10 @@ struct Cfg {
   static constexpr int TENSOR = kStep * ROWB;
   static constexpr int STAGE = 2 * TENSOR;
   static constexpr int STAGES = D == 128 ? 3 : 4;
-  // the ring, then (joined splits, when a warp owns all of them) 8 NB rows of D floats, a lane's own apart
   static constexpr int RING = STAGES * STAGE;
-  static constexpr int smem(int nb, bool direct) { return RING + (direct ? 8 * nb * D * 4 : 0); }
+  static constexpr int ROWF = D + 4;   // floats of a joined row in shared memory (conflict free either way)
+  // the ring, then, for a warp that owns all splits, its 8 NB rows and their (m, l)
+  static constexpr int smem(int nb, bool all) { return RING + (all ? 8 * nb * (ROWF + 2) * 4 : 0); }
 };
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
@@ -190,9 +201,10 @@ __global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 14) : (D == 128 
   }
   const int max_len = __reduce_max_sync(0xffffffffu, my_len);
   const int min_len = __reduce_min_sync(0xffffffffu, lane < nr ? my_len : max_len);
+  const bool all = p.upt == 1;
   const int t_begin = unit * p.spu * kSplit;
   const int t_end = min(max_len, t_begin + p.spu * kSplit);
-  if (t_begin >= t_end) {
+  if (t_begin >= t_end && !all) {
     pdl_wait();
     return;
   }
@@ -278,8 +290,8 @@ __global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 14) : (D == 128 
 
   float o[NB][KC][4], m_r[NB][2], l_r[NB][2];
   float run_m[NB][2], run_l[NB][2];
-  const bool direct = p.upt == 1;
-  float* const run_o = reinterpret_cast<float*>(ring + C::RING) + lane;   // [h][j][e] 32 apart
+  float* const run_o = reinterpret_cast<float*>(ring + C::RING);   // [8 NB][ROWF]
+  float* const run_ml = run_o + 8 * NB * C::ROWF;                  // [8 NB][2]
 #pragma unroll
   for (int h = 0; h < NB; ++h) {
 #pragma unroll
@@ -294,14 +306,14 @@ __global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 14) : (D == 128 
   }
 
   const int64_t n0 = (static_cast<int64_t>(kvh) * p.n_rows + r0) * p.G + 2 * t4;   // state row of column 2 t4
-  auto store = [&](int64_t s, int h, int e, float m, float l, auto&& a) {
+  auto store = [&](int64_t s, int h, int e, float m, float l) {
     const int64_t n = n0 + 8 * h + e;
     if (g == 0) *reinterpret_cast<float2*>(p.st_ml + 2 * (s * p.st_rows + n)) = make_float2(m, l);
     float* dst = p.st_o + ((s * (D / 4) + (g >> 2)) * p.st_rows + n) * 4 + (g & 3);
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
-      dst[static_cast<int64_t>(4 * j) * p.st_rows * 4] = a(j, e);
-      dst[static_cast<int64_t>(4 * j + 2) * p.st_rows * 4] = a(j, 2 + e);
+      dst[static_cast<int64_t>(4 * j) * p.st_rows * 4] = o[h][j][e];
+      dst[static_cast<int64_t>(4 * j + 2) * p.st_rows * 4] = o[h][j][2 + e];
     }
   };
 
@@ -421,15 +433,16 @@ __global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 14) : (D == 128 
           l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 8));
           l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 16));
           if (sp_begin < end[h][e]) {        // the row has tokens in this split
-            if (!direct) {
-              store(sp_begin / kSplit, h, e, m_r[h][e], l, [&](int j, int i) { return o[h][j][i]; });
+            float* const row = run_o + (8 * h + 2 * t4 + e) * C::ROWF + g;
+            if (!all) {
+              store(sp_begin / kSplit, h, e, m_r[h][e], l);
             } else if (sp_begin == 0) {
               run_m[h][e] = m_r[h][e];
               run_l[h][e] = l;
 #pragma unroll
               for (int j = 0; j < KC; ++j) {
-                run_o[((h * KC + j) * 4 + e) * 32] = o[h][j][e];
-                run_o[((h * KC + j) * 4 + 2 + e) * 32] = o[h][j][2 + e];
+                row[16 * j] = o[h][j][e];
+                row[16 * j + 8] = o[h][j][2 + e];
               }
             } else {
               float a, b;
@@ -437,10 +450,8 @@ __global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 14) : (D == 128 
               run_l[h][e] = join(run_l[h][e], a, l, b);
 #pragma unroll
               for (int j = 0; j < KC; ++j) {
-                float& r0 = run_o[((h * KC + j) * 4 + e) * 32];
-                float& r1 = run_o[((h * KC + j) * 4 + 2 + e) * 32];
-                r0 = join(r0, a, o[h][j][e], b);
-                r1 = join(r1, a, o[h][j][2 + e], b);
+                row[16 * j] = join(row[16 * j], a, o[h][j][e], b);
+                row[16 * j + 8] = join(row[16 * j + 8], a, o[h][j][2 + e], b);
               }
             }
           }
@@ -455,15 +466,88 @@ __global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 14) : (D == 128 
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
-  if (direct) {
+  pdl_wait();
+  if (!all) return;
+  // ---- join with the prefix's states and write the output: a lane takes row lane / 4 of a half and every
+  // fourth column quad ----
+  if (g == 0) {
 #pragma unroll
     for (int h = 0; h < NB; ++h)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        if (end[h][e] > 0)
-          store(0, h, e, run_m[h][e], run_l[h][e], [&](int j, int i) { return run_o[((h * KC + j) * 4 + i) * 32]; });
+        *reinterpret_cast<float2*>(run_ml + 2 * (8 * h + 2 * t4 + e)) = make_float2(run_m[h][e], run_l[h][e]);
   }
-  pdl_wait();
+  __syncwarp();
+  constexpr int QL = D / 16;   // quads a lane
+#pragma unroll 1
+  for (int h = 0; h < NB; ++h) {
+    const int rho = 8 * h + g, i = rho / p.G;
+    const int len = __shfl_sync(0xffffffffu, my_len, min(i, 31));
+    if (rho >= valid_rows) continue;
+    const int64_t n = (static_cast<int64_t>(kvh) * p.n_rows + r0) * p.G + rho;
+    const float2* mls = reinterpret_cast<const float2*>(p.px_ml) + n;
+    const float4* src = reinterpret_cast<const float4*>(p.px_o) + static_cast<int64_t>(t4) * p.st_rows + n;
+    float tm = -INFINITY, tl = 0.0f, gm = -INFINITY, gl = 0.0f;
+    float4 to[QL], go[QL];
+    int in_group = 0;
+    for (int s = 0; s < p.n_runs; ++s) {
+      const float2 ml = __ldcg(mls + s * p.st_rows);
+      float4 v[QL];
+#pragma unroll
+      for (int k = 0; k < QL; ++k) v[k] = __ldcg(src + (static_cast<int64_t>(s) * (D / 4) + 4 * k) * p.st_rows);
+      float a = 0.0f, b = 1.0f;
+      const bool head = in_group == 0;
+      if (head) {
+        gm = ml.x;
+        gl = ml.y;
+      } else {
+        gm = join_weights(gm, ml.x, a, b);
+        gl = join(gl, a, ml.y, b);
+      }
+#pragma unroll
+      for (int k = 0; k < QL; ++k) go[k] = head ? v[k] : join4(go[k], a, v[k], b);
+      if (++in_group == p.per_group || s + 1 == p.n_runs) {
+        in_group = 0;
+        const bool only = s < p.per_group;
+        if (only) {
+          tm = gm;
+          tl = gl;
+        } else {
+          tm = join_weights(tm, gm, a, b);
+          tl = join(tl, a, gl, b);
+        }
+#pragma unroll
+        for (int k = 0; k < QL; ++k) to[k] = only ? go[k] : join4(to[k], a, go[k], b);
+      }
+    }
+    float a = 1.0f, b = 0.0f;
+    if (len > 0) {
+      const float2 ml = *reinterpret_cast<const float2*>(run_ml + 2 * rho);
+      join_weights(tm, ml.x, a, b);
+      tl = join(tl, a, ml.y, b);
+    }
+    T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(r0 + i) * p.o_sr +
+             static_cast<int64_t>(kvh * p.G + rho - i * p.G) * p.o_sh;
+    const bool vec = (reinterpret_cast<uintptr_t>(dst) & 7u) == 0;
+#pragma unroll
+    for (int k = 0; k < QL; ++k) {
+      const int d = 4 * (t4 + 4 * k);
+      float4 v = to[k];
+      if (len > 0) v = join4(v, a, *reinterpret_cast<const float4*>(run_o + rho * C::ROWF + d), b);
+      const uint32_t lo = pack2<T>(__fdiv_rn(v.x, tl), __fdiv_rn(v.y, tl));
+      const uint32_t hi = pack2<T>(__fdiv_rn(v.z, tl), __fdiv_rn(v.w, tl));
+      if (vec) {
+        *reinterpret_cast<uint2*>(dst + d) = make_uint2(lo, hi);
+      } else {
+        const T* e = reinterpret_cast<const T*>(&lo);
+        dst[d] = e[0];
+        dst[d + 1] = e[1];
+        e = reinterpret_cast<const T*>(&hi);
+        dst[d + 2] = e[0];
+        dst[d + 3] = e[1];
+      }
+    }
+  }
 }
 
 }  // namespace own

@@ -35,6 +35,7 @@ namespace prefix {
 
 using own::exp2_hw;
 using own::join;
+using own::join4;
 using own::join_weights;
 using own::pack2;
 
@@ -693,7 +694,7 @@ struct CombineParams {
   const float* st_ml;       // [states][st_rows][2]
   int n_runs, per_group;
   const int32_t* kv_lens;   // null: no row has tokens of its own
-  int own_max;              // states the own tokens may have: 1 (joined already) or the split limit
+  int own_max;              // the most states a row's own tokens have
   int64_t st_rows, rg;      // hkv * rows * G, rows * G
   int G;
   uint64_t g_magic;         // ceil(2^36 / G)
@@ -749,9 +750,6 @@ __global__ void __launch_bounds__(CombineCfg<D, Q>::WARPS * 32) combine_kernel(c
   float4 to[Q], go[Q];
 #pragma unroll
   for (int i = 0; i < Q; ++i) to[i] = go[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  auto join4 = [](float4 v, float a, float4 vs, float b) {
-    return make_float4(join(v.x, a, vs.x, b), join(v.y, a, vs.y, b), join(v.z, a, vs.z, b), join(v.w, a, vs.w, b));
-  };
   int in_group = 0;
   for (int s0 = 0; s0 < total; s0 += 2 * UN) {
 #pragma unroll

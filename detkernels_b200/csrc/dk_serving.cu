@@ -90,8 +90,9 @@ struct PrefixPlan {
 
 // Schedule (the bits are the same for every choice).  Prefix: a whole group of chunks a run when that
 // gives most SMs an item, else a chunk a run, whose states then travel through memory.  Own tokens: all
-// splits of a (tile, KV head) by one warp when there are three waves of those, else enough units for
-// three waves.
+// splits of a (tile, KV head) by one warp, which then also joins the prefix's states and writes the output,
+// when there are 12 such warps an SM (512 rows of 4 KV heads, 1 to 127 tokens: 125 us against 144 split up);
+// else enough units for three waves, and combine_kernel.
 PrefixPlan plan_prefix(int64_t n_rows, int64_t n_tiles, int64_t hkv, int64_t G, int64_t head_dim, int64_t prefix_len,
                        int64_t max_kv_len) {
   PrefixPlan pl{};
@@ -112,11 +113,11 @@ PrefixPlan plan_prefix(int64_t n_rows, int64_t n_tiles, int64_t hkv, int64_t G, 
   if (pl.max_splits > 0) {
     const int64_t units = n_tiles * hkv;
     const int64_t target = 3LL * (head_dim == 128 ? 9 : 14) * sms;
-    int64_t upt = units >= target ? 1 : ceil_div(target, units);
+    int64_t upt = units >= 12LL * sms ? 1 : ceil_div(target, units);
     if (upt > pl.max_splits) upt = pl.max_splits;
     pl.spu = static_cast<int>(ceil_div(pl.max_splits, upt));
     pl.upt = static_cast<int>(ceil_div(pl.max_splits, pl.spu));
-    pl.own_states = pl.upt == 1 ? 1 : pl.max_splits;
+    pl.own_states = pl.upt == 1 ? 0 : pl.max_splits;
   }
   return pl;
 }
@@ -475,8 +476,17 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
     o.st_rows = st_rows;
     o.st_o = st_o + static_cast<int64_t>(pl.n_runs) * st_rows * head_dim;
     o.st_ml = st_ml + static_cast<int64_t>(pl.n_runs) * st_rows * 2;
+    if (pl.upt == 1) {
+      o.out = out;
+      o.o_sr = out_stride_row;
+      o.o_sh = out_stride_head;
+      o.px_o = st_o;
+      o.px_ml = st_ml;
+      o.n_runs = pl.n_runs;
+      o.per_group = pl.per_group;
+    }
     rc = DK_DISPATCH_16(own_launch, o, st);
-    if (rc) return rc;
+    if (rc || pl.upt == 1) return rc;
   }
   dk::prefix::CombineParams c{};
   c.st_o = st_o;
