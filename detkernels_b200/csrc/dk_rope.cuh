@@ -44,7 +44,7 @@ struct Params {
   int64_t max_pos;
   int64_t n_rows;
   int H, Hkv, D, rd, interleaved;
-  float eps;
+  float eps, inv_d;                      // inv_d: 1 / D
   int nvec;                              // vectors a row: H + Hkv (+ Hkv with a cache)
   int lanes;                             // vector path: lanes that hold chunks (L)
   int glog;                              // log2 of the group's lane count
@@ -178,113 +178,159 @@ __device__ __forceinline__ uint4 pack<__half>(const float* x) {
 
 // Vector path.  NC: chunks a lane holds (chunk l + j L, j < NC).  Rotated chunks: 0 and 1 (pairs
 // between them) or, interleaved, those with index < rd / N (pairs inside a chunk).
+//
+// Warps walk units (a row, or part of one when rows are few) grid-stride, the next unit's position and
+// slot in flight while one is rotated.  The weights stay in shared memory as f32 and the angles are read
+// back from the cache a batch at a time, as 16-byte vectors: the loop is bound by the instructions it
+// issues before the bytes it moves, so that the 62,794-row prefill of 32 heads of 64 (floor 86 us) took
+// 161 us with both in registers through a type switch, 123 us with four vectors a lane in flight and
+// the spills of that, and takes 113 us with two.  One resident set of 3 CTAs an SM walks all units;
+// one CTA per 8 units took 15 % more.
 template <typename T, int NC, bool INTER>
-__global__ void __launch_bounds__(kThreads) vec_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 3) vec_kernel(const Params p) {
   constexpr int N = Chunk<T>::N;
-  constexpr int UB = NC <= 2 ? 4 : 2;   // vectors in flight per group
+  constexpr int UB = NC <= 2 ? 2 : 1;   // vectors in flight per group
+  constexpr int NA = INTER ? NC * N / 2 : N;   // angles a lane holds
+  __shared__ __align__(16) float s_w[2][kMaxDim];
   pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
+  for (int i = threadIdx.x; i < 2 * p.D; i += kThreads) {
+    const int k = i >= p.D;
+    if (k ? p.Hkv > 0 : p.H > 0) s_w[k][i - k * p.D] = load_w(k ? p.kw : p.qw, p.wdtype, i - k * p.D);
+  }
+  __syncthreads();
   const int lane = threadIdx.x & 31;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  const int64_t t = unit / p.upr;
-  if (t >= p.n_rows) return;
-  const int part = static_cast<int>(unit - t * p.upr);
   const int gl = 1 << p.glog, gpw = 32 >> p.glog;
   const int l = lane & (gl - 1), gi = lane >> p.glog;
   const bool on = l < p.lanes;
-  Row row;
-  if (!describe_row(p, t, lane == 0 && part == 0, row)) return;
-  // this lane's angles: pairs of chunk 0 with chunk 1 share index i in [l N, l N + N); interleaved,
-  // chunk j's pairs are i = (l + j L) N / 2 + [0, N / 2)
-  const float* cs = p.table + row.pos * p.rd;
-  const int half = p.rd >> 1;
-  float co[INTER ? NC * N / 2 : N], si[INTER ? NC * N / 2 : N];
-  if (on) {
-    if constexpr (INTER) {
-#pragma unroll
-      for (int j = 0; j < NC; ++j)
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-          const int pi = (l + j * p.lanes) * (N / 2) + i;
-          co[j * (N / 2) + i] = pi < half ? cs[pi] : 1.0f;
-          si[j * (N / 2) + i] = pi < half ? cs[half + pi] : 0.0f;
-        }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        co[i] = cs[l * N + i];
-        si[i] = cs[half + l * N + i];
-      }
-    }
-  }
-  const int end = min(p.nvec, (part + 1) * p.vpu);
-  for (int i0 = part * p.vpu + gi; i0 - gi < end; i0 += UB * gpw) {
-    Place<T> pl[UB];
+  const int half = p.rd >> 1, cstep = p.lanes * N;   // elements between a lane's chunks
+  const uint32_t units = static_cast<uint32_t>(p.n_rows) * p.upr;   // < 2^31 (the host checks)
+  const uint32_t step = gridDim.x * (kThreads / 32);
+  uint32_t unit = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  Row row{0, -1};
+  bool good = unit < units && describe_row(p, unit / p.upr, lane == 0 && unit % p.upr == 0, row);
+  for (; unit < units; unit += step) {
+    const uint32_t t = unit / p.upr, part = unit - t * p.upr;
+    const Row now = row;
+    const bool go = good;
+    const uint32_t next = unit + step;
+    if (next < units) good = describe_row(p, next / p.upr, lane == 0 && next % p.upr == 0, row);
+    if (!go) continue;   // (the whole warp: one row a unit)
+    const int begin = static_cast<int>(part) * p.vpu;
+    const int end = min(p.nvec, begin + p.vpu);
+    // the row's tensors at this lane's first chunk
+    const T* const qs = static_cast<const T*>(p.q) + t * p.q_sr + l * N;
+    const T* const ks = static_cast<const T*>(p.k) + t * p.k_sr + l * N;
+    const T* const vs = static_cast<const T*>(p.v) + t * p.v_sr + l * N;
+    T* const qd = static_cast<T*>(p.qo) + t * p.qo_sr + l * N;
+    T* const kd = static_cast<T*>(p.ko) + t * p.ko_sr + l * N;
+    T* const kc = static_cast<T*>(p.kc) + now.cache + l * N;
+    T* const vc = static_cast<T*>(p.vc) + now.cache + l * N;
     uint4 c[UB][NC];
+    for (int i0 = begin; i0 < end; i0 += UB * gpw) {
+      if (on) {
 #pragma unroll
-    for (int u = 0; u < UB; ++u) {
-      const int i = i0 + u * gpw;
-      if (i < end) {
-        pl[u] = place<T>(p, row, t, i);
-        if (on) {
+        for (int u = 0; u < UB; ++u) {
+          const int i = i0 + gi + u * gpw;
+          if (i < end) {
+            const T* src = i < p.H ? qs + i * p.q_sh
+                                   : (i < p.H + p.Hkv ? ks + (i - p.H) * p.k_sh : vs + (i - p.H - p.Hkv) * p.v_sh);
 #pragma unroll
-          for (int j = 0; j < NC; ++j)
-            c[u][j] = *reinterpret_cast<const uint4*>(pl[u].src + (l + j * p.lanes) * N);
-        }
-      } else {
-        pl[u].kind = 3;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < UB; ++u) {
-      // every lane of the warp takes part in the shuffles
-      float x[NC][N];
-      float ss = 0.0f;
-      const bool live = on && pl[u].kind < 2;
-      if (live) {
-#pragma unroll
-        for (int j = 0; j < NC; ++j) {
-          unpack<T>(c[u][j], x[j]);
-#pragma unroll
-          for (int e = 0; e < N; ++e) ss = __fmaf_rn(x[j][e], x[j][e], ss);
-        }
-      }
-      for (int d = gl >> 1; d > 0; d >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, d));
-      if (live) {
-        const float rs = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(p.D)), p.eps));
-        const void* w = pl[u].kind ? p.kw : p.qw;
-#pragma unroll
-        for (int j = 0; j < NC; ++j)
-#pragma unroll
-          for (int e = 0; e < N; ++e)
-            x[j][e] = __fmul_rn(__fmul_rn(x[j][e], rs), load_w(w, p.wdtype, (l + j * p.lanes) * N + e));
-        if constexpr (INTER) {
-#pragma unroll
-          for (int j = 0; j < NC; ++j)
-#pragma unroll
-            for (int e = 0; e < N / 2; ++e) {
-              const float a = x[j][2 * e], b = x[j][2 * e + 1];
-              const float cc = co[j * (N / 2) + e], sn = si[j * (N / 2) + e];
-              x[j][2 * e] = __fmaf_rn(a, cc, -__fmul_rn(b, sn));
-              x[j][2 * e + 1] = __fmaf_rn(a, sn, __fmul_rn(b, cc));
-            }
-        } else {
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const float a = x[0][e], b = x[1][e];
-            x[0][e] = __fmaf_rn(a, co[e], -__fmul_rn(b, si[e]));
-            x[1][e] = __fmaf_rn(a, si[e], __fmul_rn(b, co[e]));
+            for (int j = 0; j < NC; ++j) c[u][j] = __ldcs(reinterpret_cast<const uint4*>(src + j * cstep));
           }
         }
-#pragma unroll
-        for (int j = 0; j < NC; ++j) c[u][j] = pack<T>(x[j]);
       }
-      if (on && pl[u].kind < 3) {
+      // this lane's angles: pairs of chunk 0 with chunk 1 share index i in [l N, l N + N); interleaved,
+      // chunk j's pairs are i = (l + j L) N / 2 + [0, N / 2)  (re-read a batch from the cache: no registers held)
+      float co[NA], si[NA];
+      if (on) {
+        const float* cs = p.table + now.pos * p.rd;
+        if constexpr (INTER) {
 #pragma unroll
-        for (int j = 0; j < NC; ++j) {
-          const int off = (l + j * p.lanes) * N;
-          if (pl[u].dst) *reinterpret_cast<uint4*>(pl[u].dst + off) = c[u][j];
-          if (pl[u].dst2) *reinterpret_cast<uint4*>(pl[u].dst2 + off) = c[u][j];
+          for (int j = 0; j < NC; ++j) {
+            const int at = (l + j * p.lanes) * (N / 2);
+            const bool rot = at < half;   // a chunk is rotated as a whole
+#pragma unroll
+            for (int i = 0; i < N / 2; i += 2) {
+              const float2 a = rot ? __ldg(reinterpret_cast<const float2*>(cs + at + i)) : make_float2(1.0f, 1.0f);
+              const float2 b = rot ? __ldg(reinterpret_cast<const float2*>(cs + half + at + i)) : make_float2(0.0f, 0.0f);
+              co[j * (N / 2) + i] = a.x;
+              co[j * (N / 2) + i + 1] = a.y;
+              si[j * (N / 2) + i] = b.x;
+              si[j * (N / 2) + i + 1] = b.y;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; i += 4) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(cs + l * N + i));
+            const float4 b = __ldg(reinterpret_cast<const float4*>(cs + half + l * N + i));
+            co[i] = a.x, co[i + 1] = a.y, co[i + 2] = a.z, co[i + 3] = a.w;
+            si[i] = b.x, si[i + 1] = b.y, si[i + 2] = b.z, si[i + 3] = b.w;
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UB; ++u) {
+        // every lane of the warp takes part in the shuffles
+        const int i = i0 + gi + u * gpw;
+        const bool live = on && i < end && i < p.H + p.Hkv;
+        float x[NC][N];
+        float ss = 0.0f;
+        if (live) {
+#pragma unroll
+          for (int j = 0; j < NC; ++j) {
+            unpack<T>(c[u][j], x[j]);
+#pragma unroll
+            for (int e = 0; e < N; ++e) ss = __fmaf_rn(x[j][e], x[j][e], ss);
+          }
+        }
+        for (int d = gl >> 1; d > 0; d >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, d));
+        if (live) {
+          const float rs = rsqrtf(__fmaf_rn(ss, p.inv_d, p.eps));
+          const float* w = s_w[i >= p.H] + l * N;
+#pragma unroll
+          for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int e = 0; e < N; e += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(w + j * cstep + e);
+              x[j][e] = __fmul_rn(__fmul_rn(x[j][e], rs), f.x);
+              x[j][e + 1] = __fmul_rn(__fmul_rn(x[j][e + 1], rs), f.y);
+              x[j][e + 2] = __fmul_rn(__fmul_rn(x[j][e + 2], rs), f.z);
+              x[j][e + 3] = __fmul_rn(__fmul_rn(x[j][e + 3], rs), f.w);
+            }
+          if constexpr (INTER) {
+#pragma unroll
+            for (int j = 0; j < NC; ++j)
+#pragma unroll
+              for (int e = 0; e < N / 2; ++e) {
+                const float a = x[j][2 * e], b = x[j][2 * e + 1];
+                const float cc = co[j * (N / 2) + e], sn = si[j * (N / 2) + e];
+                x[j][2 * e] = __fmaf_rn(a, cc, -__fmul_rn(b, sn));
+                x[j][2 * e + 1] = __fmaf_rn(a, sn, __fmul_rn(b, cc));
+              }
+          } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+              const float a = x[0][e], b = x[1][e];
+              x[0][e] = __fmaf_rn(a, co[e], -__fmul_rn(b, si[e]));
+              x[1][e] = __fmaf_rn(a, si[e], __fmul_rn(b, co[e]));
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < NC; ++j) c[u][j] = pack<T>(x[j]);
+        }
+        if (on && i < end) {
+          const int h = i < p.H ? i : (i < p.H + p.Hkv ? i - p.H : i - p.H - p.Hkv);
+          T* dst = i < p.H ? qd + h * p.qo_sh : (now.cache >= 0 ? (i < p.H + p.Hkv ? kc : vc) + h * p.c_sh : nullptr);
+          if (dst) {
+#pragma unroll
+            for (int j = 0; j < NC; ++j) *reinterpret_cast<uint4*>(dst + j * cstep) = c[u][j];
+          }
+          if (p.ko && i >= p.H && i < p.H + p.Hkv) {
+#pragma unroll
+            for (int j = 0; j < NC; ++j) *reinterpret_cast<uint4*>(kd + h * p.ko_sh + j * cstep) = c[u][j];
+          }
         }
       }
     }
@@ -316,7 +362,7 @@ __global__ void __launch_bounds__(kThreads) any_kernel(const Params p) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, d));
     __syncwarp();
-    const float rs = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(p.D)), p.eps));
+    const float rs = rsqrtf(__fmaf_rn(ss, p.inv_d, p.eps));
     const float* cs = p.table + row.pos * p.rd;
     const int half = p.rd >> 1;
     const void* wt = pl.kind == 1 ? p.kw : p.qw;

@@ -24,8 +24,9 @@ size_t plan_ws_bytes(int64_t n_seqs) { return static_cast<size_t>(2 + 2 * (n_seq
 // ============================ head norm + rotation ============================
 template <typename T, int NC, bool INTER>
 cudaError_t rope_vec(const dk::rope::Params& p, cudaStream_t st) {
-  const int64_t units = p.n_rows * p.upr;
-  const int64_t grid = ceil_div(units, dk::rope::kThreads / 32);
+  const int64_t want = ceil_div(p.n_rows * p.upr, dk::rope::kThreads / 32);
+  const int64_t cap = 3LL * sm_count(current_device());   // resident CTAs; each walks units
+  const int64_t grid = want < cap ? want : cap;
   return launch_pdl(dk::rope::vec_kernel<T, NC, INTER>, dim3(static_cast<unsigned>(grid)), dim3(dk::rope::kThreads), 0,
                     st, p);
 }
@@ -36,12 +37,12 @@ int rope_launch(dk::rope::Params& p, cudaStream_t st) {
   auto ok16 = [](const void* ptr, int64_t a, int64_t b) { return !ptr || (aligned16(ptr) && a % N == 0 && b % N == 0); };
   bool vec = ok16(p.q, p.q_sr, p.q_sh) && ok16(p.k, p.k_sr, p.k_sh) && ok16(p.v, p.v_sr, p.v_sh) &&
              ok16(p.qo, p.qo_sr, p.qo_sh) && ok16(p.ko, p.ko_sr, p.ko_sh) && ok16(p.kc, p.c_sn, p.c_sh) &&
-             ok16(p.vc, p.c_st, 0) && p.D % N == 0;
+             ok16(p.vc, p.c_st, 0) && aligned16(p.table) && p.D % N == 0;
   int nc = 0;
   if (vec) {
     const int chunks = p.D / N;
     if (p.interleaved) {
-      vec = chunks % 2 == 0;
+      vec = chunks % 2 == 0 && p.rd % N == 0;   // whole chunks are rotated
       nc = 2;
       p.lanes = chunks / 2;
     } else {
@@ -66,8 +67,7 @@ int rope_launch(dk::rope::Params& p, cudaStream_t st) {
     const int per = (p.n_rows >= full) ? static_cast<int>(ceil_div(p.nvec, gpw)) : 1;
     p.vpu = per * gpw;
     p.upr = static_cast<int>(ceil_div(p.nvec, p.vpu));
-    if (ceil_div(p.n_rows * p.upr, dk::rope::kThreads / 32) > kI32Max)
-      return fail(DK_ERR_INVALID_ARGUMENT, "qk_norm_rope: too many rows");
+    if (p.n_rows * p.upr > kI32Max - (1 << 20)) return fail(DK_ERR_INVALID_ARGUMENT, "qk_norm_rope: too many rows");
     if (p.interleaved) e = rope_vec<T, 2, true>(p, st);
     else if (nc == 2) e = rope_vec<T, 2, false>(p, st);
     else e = rope_vec<T, 4, false>(p, st);
@@ -318,6 +318,7 @@ int dk_qk_norm_rope(const void* q, int64_t q_stride_row, int64_t q_stride_head, 
   p.n_rows = n_rows;
   p.H = n_q_heads; p.Hkv = n_kv_heads; p.D = head_dim; p.rd = rotary_dim; p.interleaved = interleaved ? 1 : 0;
   p.eps = eps;
+  p.inv_d = 1.0f / static_cast<float>(head_dim);
   p.nvec = n_q_heads + n_kv_heads * (cache ? 2 : 1);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == DK_F32) return rope_launch<float>(p, st);
