@@ -250,8 +250,21 @@ def dtype_code(dtype) -> int:
 
 
 def stream_ptr(device=None) -> int:
+    """The current stream of the device (the current one's by default) as a raw handle."""
     import torch
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device if isinstance(device, int) else getattr(device, "index", None)
+    if index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+_no_guard = contextlib.nullcontext()
+
+
+def on_device(device):
+    """``torch.cuda.device(device)`` for a tensor's device, which costs nothing when it is the current one."""
+    import torch
+    return _no_guard if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 _workspaces = {}

@@ -6,8 +6,12 @@
 // sequence b (r in [R[b], R[b + 1])) is token pos = kv[b] + r - R[b] of it, at slot
 // table[b, pos / page] * page + pos % page, and tile T[b] + i covers rows R[b] + i rpt on.
 //
-// Two launches: one CTA validates the lengths and scans them, then a grid writes rows, table
-// entries and tiles, each output element finding its sequence by binary search in the sums.
+// One CTA validates the lengths and scans them, then rows are written: a CTA takes a run of rows,
+// finds the sequences of its two ends by a 32-way search in the sums, and a thread finds the first of
+// its four consecutive rows between those.  The row that opens a new page also writes the table entry,
+// and the row that opens a tile the tile, so that one search serves all outputs.  Bound by the 20
+// bytes stored per row when rows are many, by the latency of the two kernels' loads when they are few.
+// MEASPLAN
 #pragma once
 
 #include "dk_common.cuh"
@@ -16,7 +20,9 @@ namespace dk {
 namespace paging {
 
 constexpr int kScanThreads = 1024;
+constexpr int kScanItems = 8;     // sequences a thread scans in one round, at most
 constexpr int kFillThreads = 256;
+constexpr int kRowVec = 4;        // consecutive rows of a thread
 
 enum : int {
   kDetLens = 0x600,   // a negative length, or a sequence past its row of the block table
@@ -45,11 +51,15 @@ struct Params {
   int32_t* tiles;           // null: no tiles
   int32_t rpt;
   int64_t n_tiles;
+  int vec;                  // the row outputs take 16-byte stores
   // scratch: [0] 1 when the plan stands, [1] cursor, then cu_blk [n_seqs + 1], cu_tile [n_seqs + 1]
   int32_t* ws;
 };
 
-__device__ __forceinline__ int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+__device__ __forceinline__ uint32_t ceil_div32(uint32_t a, uint32_t b) {
+  const uint32_t q = a / b;
+  return q + (a != q * b);
+}
 
 struct Sum3 {
   int64_t r, k, t;
@@ -70,54 +80,221 @@ __device__ __forceinline__ Sum3 warp_scan(Sum3 v, int lane) {
   return v;
 }
 
+// The last b with cu[b] <= x (cu ascending, cu[0] = 0 <= x < cu[n]): the sequence element x belongs to,
+// between lo and hi (cu[lo] <= x < cu[hi]).
+__device__ __forceinline__ int find_seq(const int32_t* cu, int lo, int hi, int32_t x) {
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+// The same by a whole warp, 32 ways a step.
+__device__ __forceinline__ int find_seq_warp(const int32_t* cu, int n, int32_t x, int lane) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) >> 5;
+    const int at = lo + (lane + 1) * step;
+    const int below = __popc(__ballot_sync(0xffffffffu, at < hi && cu[at] <= x));
+    lo += below * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
+// Rows, and with them the new table entries and the tiles (block-wide, CTA `cta` of `ctas`).
+__device__ void fill_rows(const Params& p, int64_t cursor, int cta, int ctas) {
+  __shared__ int s_end[2];
+  const int32_t* cu = p.cu_rows;
+  const int32_t* cu_blk = p.ws + 2;
+  const int32_t* cu_tile = cu_blk + p.n_seqs + 1;
+  const int64_t n = cu[p.n_seqs];
+  const int64_t run = static_cast<int64_t>(blockDim.x) * kRowVec;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t page = p.page, rpt = p.rpt;
+  for (int64_t r0 = cta * run; r0 < n; r0 += ctas * run) {
+    if (warp < 2) {
+      const int64_t x = warp == 0 ? r0 : (r0 + run < n ? r0 + run : n) - 1;
+      const int b = find_seq_warp(cu, p.n_seqs, static_cast<int32_t>(x), lane);
+      if (lane == 0) s_end[warp] = b;
+    }
+    __syncthreads();
+    const int64_t r = r0 + static_cast<int64_t>(threadIdx.x) * kRowVec;
+    if (r < n) {
+      const int first = static_cast<int>(r);
+      const int cnt = n - r < kRowVec ? static_cast<int>(n - r) : kRowVec;
+      const int last_seq = s_end[1];
+      int b = find_seq(cu, s_end[0], last_seq + 1, first);
+      int begin = 0, end = 0;          // rows of sequence b
+      uint32_t pg = 0, off = 0, have = 0;
+      int32_t kv = 0;
+      int64_t blk = 0;
+      bool fresh = true;               // the page's block is not known yet
+      int seq[kRowVec], pos[kRowVec];
+      int64_t slot[kRowVec];
+#pragma unroll
+      for (int i = 0; i < kRowVec; ++i) {
+        if (i < cnt) {
+          if (i == 0 || first + i >= end) {
+            if (i > 0) b = find_seq(cu, b + 1, last_seq + 1, first + i);
+            begin = cu[b];
+            end = cu[b + 1];
+            kv = p.kv[b];
+            have = ceil_div32(kv, page);
+            const uint32_t at = static_cast<uint32_t>(kv + (first + i - begin));
+            pg = at / page;
+            off = at - pg * page;
+            fresh = true;
+          } else if (++off == page) {
+            off = 0;
+            ++pg;
+            fresh = true;
+          }
+          if (fresh) {
+            if (p.free_list && pg >= have) {
+              const int32_t got = p.free_list[cursor + cu_blk[b] + (pg - have)];
+              // a new page's first token is one of the new rows
+              if (off == 0) p.table[b * p.table_stride + pg] = got;
+              blk = got;
+            } else {
+              blk = p.table[b * p.table_stride + pg];
+            }
+            fresh = false;
+          }
+          seq[i] = b;
+          pos[i] = kv + (first + i - begin);
+          slot[i] = blk * page + off;
+          if (p.tiles) {
+            const uint32_t in = first + i - begin;
+            const uint32_t tile = in / rpt;
+            if (tile * rpt == in) {
+              int32_t* t = p.tiles + 3 * (static_cast<int64_t>(cu_tile[b]) + tile);
+              t[0] = first + i;
+              t[1] = min(p.rpt, end - (first + i));
+              t[2] = b;
+            }
+          }
+        }
+      }
+      if (p.vec && cnt == kRowVec) {
+        *reinterpret_cast<int4*>(p.row_seq + r) = make_int4(seq[0], seq[1], seq[2], seq[3]);
+        *reinterpret_cast<int4*>(p.row_pos + r) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        *reinterpret_cast<int4*>(p.q_lens + r) = make_int4(pos[0] + 1, pos[1] + 1, pos[2] + 1, pos[3] + 1);
+        *reinterpret_cast<longlong2*>(p.slots + r) = make_longlong2(slot[0], slot[1]);
+        *reinterpret_cast<longlong2*>(p.slots + r + 2) = make_longlong2(slot[2], slot[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kRowVec; ++i)
+          if (i < cnt) {
+            p.row_seq[r + i] = seq[i];
+            p.row_pos[r + i] = pos[i];
+            p.q_lens[r + i] = pos[i] + 1;
+            p.slots[r + i] = slot[i];
+          }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// New table entries and tiles of a call that asks for no rows.
+__device__ void fill_without_rows(const Params& p, int64_t cursor, int64_t tid, int64_t step) {
+  const int32_t* cu_blk = p.ws + 2;
+  const int32_t* cu_tile = cu_blk + p.n_seqs + 1;
+  if (p.free_list) {
+    const int64_t n = cu_blk[p.n_seqs];
+    for (int64_t j = tid; j < n; j += step) {
+      const int b = find_seq(cu_blk, 0, p.n_seqs, static_cast<int32_t>(j));
+      const int64_t have = ceil_div32(p.kv[b], p.page);
+      p.table[b * p.table_stride + have + (j - cu_blk[b])] = p.free_list[cursor + j];
+    }
+  }
+  if (p.tiles) {
+    const int64_t n = cu_tile[p.n_seqs];
+    for (int64_t t = tid; t < n; t += step) {
+      const int b = find_seq(cu_tile, 0, p.n_seqs, static_cast<int32_t>(t));
+      const int32_t at = static_cast<int32_t>(t - cu_tile[b]) * p.rpt;
+      p.tiles[3 * t + 0] = p.cu_rows[b] + at;
+      p.tiles[3 * t + 1] = min(p.rpt, p.nw[b] - at);
+      p.tiles[3 * t + 2] = b;
+    }
+  }
+}
+
+// One CTA: checks and sums; ALONE: the rest of the plan as well (few outputs: a second launch costs
+// more than one CTA's stores).
+template <bool ALONE>
 __global__ void __launch_bounds__(kScanThreads) scan_kernel(const Params p) {
   __shared__ Sum3 s_warp[32];
-  __shared__ int s_bad;
+  __shared__ int s_bad, s_ok;
+  __shared__ int64_t s_cursor;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  if (threadIdx.x == 0) s_bad = 0;
+  if (warp == 0) s_warp[lane] = Sum3{0, 0, 0};   // a block of fewer warps leaves the rest at zero
   pdl_wait();
-  if (threadIdx.x == 0) {
-    pdl_launch_dependents();
-    s_bad = 0;
-  }
+  if (threadIdx.x == 0) pdl_launch_dependents();
   __syncthreads();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int32_t* cu_blk = p.ws + 2;
   int32_t* cu_tile = cu_blk + p.n_seqs + 1;
+  const int threads = blockDim.x;
+  const int items = min(kScanItems, (p.n_seqs + threads - 1) / threads);   // consecutive sequences of a thread
   Sum3 base{0, 0, 0};
-  for (int b0 = 0; b0 < p.n_seqs; b0 += kScanThreads) {
-    const int b = b0 + threadIdx.x;
+  for (int64_t b0 = 0; b0 < p.n_seqs; b0 += threads * items) {
+    const int64_t b = b0 + static_cast<int64_t>(threadIdx.x) * items;
+    int32_t kv[kScanItems], nw[kScanItems];
+#pragma unroll
+    for (int i = 0; i < kScanItems; ++i) {
+      const bool is = i < items && b + i < p.n_seqs;
+      kv[i] = is ? p.kv[b + i] : 0;
+      nw[i] = is ? p.nw[b + i] : 0;
+    }
     Sum3 v{0, 0, 0};
-    if (b < p.n_seqs) {
-      const int64_t kv = p.kv[b], n = p.nw[b];
-      const int64_t have = ceil_div64(kv, p.page), need = ceil_div64(kv + n, p.page);
-      if (kv < 0 || n < 0 || need > p.width) {
-        s_bad = 1;
-      } else {
-        v.r = n;
-        v.k = need - have;
-        v.t = p.rpt > 0 ? ceil_div64(n, p.rpt) : 0;
+    int32_t blk[kScanItems], til[kScanItems];
+#pragma unroll
+    for (int i = 0; i < kScanItems; ++i) {
+      blk[i] = til[i] = 0;
+      if (i < items) {
+        // both below 2^31, so their sum is below 2^32
+        const uint32_t have = ceil_div32(kv[i], p.page), need = ceil_div32(static_cast<uint32_t>(kv[i]) + nw[i], p.page);
+        if (kv[i] < 0 || nw[i] < 0 || need > static_cast<uint32_t>(p.width)) {
+          s_bad = 1;
+          nw[i] = 0;
+        } else {
+          blk[i] = need - have;
+          if (p.rpt > 0) til[i] = ceil_div32(nw[i], p.rpt);
+        }
+        v.r += nw[i];
+        v.k += blk[i];
+        v.t += til[i];
       }
     }
     const Sum3 incl = warp_scan(v, lane);
     if (lane == 31) s_warp[warp] = incl;
     __syncthreads();
     if (warp == 0) {
-      const Sum3 w = s_warp[lane];
-      const Sum3 wi = warp_scan(w, lane);
+      const Sum3 wi = warp_scan(s_warp[lane], lane);
+      __syncwarp();
       s_warp[lane] = wi;
     }
     __syncthreads();
-    Sum3 off = base;
+    Sum3 at{base.r + incl.r - v.r, base.k + incl.k - v.k, base.t + incl.t - v.t};
     if (warp > 0) {
-      off.r += s_warp[warp - 1].r;
-      off.k += s_warp[warp - 1].k;
-      off.t += s_warp[warp - 1].t;
+      at.r += s_warp[warp - 1].r;
+      at.k += s_warp[warp - 1].k;
+      at.t += s_warp[warp - 1].t;
     }
-    if (b < p.n_seqs) {
-      p.cu_rows[b] = static_cast<int32_t>(off.r + incl.r - v.r);
-      cu_blk[b] = static_cast<int32_t>(off.k + incl.k - v.k);
-      cu_tile[b] = static_cast<int32_t>(off.t + incl.t - v.t);
+#pragma unroll
+    for (int i = 0; i < kScanItems; ++i) {
+      if (i < items && b + i < p.n_seqs) {
+        p.cu_rows[b + i] = static_cast<int32_t>(at.r);
+        cu_blk[b + i] = static_cast<int32_t>(at.k);
+        cu_tile[b + i] = static_cast<int32_t>(at.t);
+      }
+      at.r += nw[i];
+      at.k += blk[i];
+      at.t += til[i];
     }
-    const Sum3 tot = s_warp[31];
+    const Sum3 tot = s_warp[warps - 1];
     base.r += tot.r;
     base.k += tot.k;
     base.t += tot.t;
@@ -140,17 +317,15 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(const Params p) {
     if (p.cursor_out) *p.cursor_out = static_cast<int32_t>(bad ? cur : cur + base.k);
     p.ws[1] = static_cast<int32_t>(cur);
     p.ws[0] = bad ? 0 : 1;
+    s_ok = !bad;
+    s_cursor = cur;
   }
-}
-
-// The last b with cu[b] <= x (cu ascending, cu[0] = 0 <= x < cu[n]): the sequence element x belongs to.
-__device__ __forceinline__ int find_seq(const int32_t* cu, int n, int32_t x) {
-  int lo = 0, hi = n;   // cu[lo] <= x < cu[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= x) lo = mid; else hi = mid;
+  if constexpr (ALONE) {
+    __syncthreads();
+    if (!s_ok) return;
+    if (p.row_seq) fill_rows(p, s_cursor, 0, 1);
+    else fill_without_rows(p, s_cursor, threadIdx.x, blockDim.x);
   }
-  return lo;
 }
 
 __global__ void __launch_bounds__(kFillThreads) fill_kernel(const Params p) {
@@ -158,44 +333,11 @@ __global__ void __launch_bounds__(kFillThreads) fill_kernel(const Params p) {
   if (threadIdx.x == 0) pdl_launch_dependents();
   if (p.ws[0] == 0) return;
   const int64_t cursor = p.ws[1];
-  const int32_t* cu_blk = p.ws + 2;
-  const int32_t* cu_tile = cu_blk + p.n_seqs + 1;
-  const int64_t tid = static_cast<int64_t>(blockIdx.x) * kFillThreads + threadIdx.x;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kFillThreads;
-  if (p.row_seq) {
-    const int64_t n = p.cu_rows[p.n_seqs];
-    for (int64_t r = tid; r < n; r += step) {
-      const int b = find_seq(p.cu_rows, p.n_seqs, static_cast<int32_t>(r));
-      const int32_t kv = p.kv[b];
-      const int32_t pos = kv + static_cast<int32_t>(r) - p.cu_rows[b];
-      const int32_t pg = pos / p.page;
-      const int32_t have = static_cast<int32_t>(ceil_div64(kv, p.page));
-      const int64_t blk = (p.free_list && pg >= have) ? p.free_list[cursor + cu_blk[b] + (pg - have)]
-                                                      : p.table[b * p.table_stride + pg];
-      p.row_seq[r] = b;
-      p.row_pos[r] = pos;
-      p.slots[r] = blk * p.page + (pos - pg * p.page);
-      p.q_lens[r] = pos + 1;
-    }
-  }
-  if (p.free_list) {
-    const int64_t n = cu_blk[p.n_seqs];
-    for (int64_t j = tid; j < n; j += step) {
-      const int b = find_seq(cu_blk, p.n_seqs, static_cast<int32_t>(j));
-      const int64_t have = ceil_div64(p.kv[b], p.page);
-      p.table[b * p.table_stride + have + (j - cu_blk[b])] = p.free_list[cursor + j];
-    }
-  }
-  if (p.tiles) {
-    const int64_t n = cu_tile[p.n_seqs];
-    for (int64_t t = tid; t < n; t += step) {
-      const int b = find_seq(cu_tile, p.n_seqs, static_cast<int32_t>(t));
-      const int32_t at = static_cast<int32_t>(t - cu_tile[b]) * p.rpt;
-      p.tiles[3 * t + 0] = p.cu_rows[b] + at;
-      p.tiles[3 * t + 1] = min(p.rpt, p.nw[b] - at);
-      p.tiles[3 * t + 2] = b;
-    }
-  }
+  if (p.row_seq)
+    fill_rows(p, cursor, blockIdx.x, gridDim.x);
+  else
+    fill_without_rows(p, cursor, static_cast<int64_t>(blockIdx.x) * kFillThreads + threadIdx.x,
+                      static_cast<int64_t>(gridDim.x) * kFillThreads);
 }
 
 }  // namespace paging

@@ -1,5 +1,7 @@
 // C ABI of the serving operators (see include/detkernels_b200.h): the page plan of a step, the
 // per-head norm with rotation into a KV cache, and attention over a shared prefix.
+#include <algorithm>
+
 #include "dk_common.cuh"
 #include "dk_host.cuh"
 #include "dk_paging.cuh"
@@ -255,21 +257,28 @@ int dk_paged_plan(int32_t* block_table, int64_t block_table_stride, int32_t bloc
   p.rpt = row_tiles ? rows_per_tile : 0;
   p.n_tiles = n_tiles;
   p.ws = static_cast<int32_t*>(workspace);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_pdl(dk::paging::scan_kernel, dim3(1), dim3(dk::paging::kScanThreads), 0, st, p);
-  if (e != cudaSuccess) return fail(DK_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
-  if (!rows && !row_tiles && !free_blocks) return DK_OK;
-  int64_t most = rows ? n_rows : 0;
-  if (row_tiles && n_tiles > most) most = n_tiles;
-  if (free_blocks) {
-    const int64_t grow = n_free < static_cast<int64_t>(n_seqs) * blocks_per_seq ? n_free
-                                                                                : static_cast<int64_t>(n_seqs) * blocks_per_seq;
-    if (!rows && grow > most) most = grow;
+  p.vec = aligned16(row_seq) && aligned16(row_pos) && aligned16(slots) && aligned16(q_lens);
+  // at most so many outputs of each kind (the growth is known on the device only)
+  int64_t most = rows ? n_rows : n_tiles;
+  if (free_blocks && !rows) {
+    const int64_t grow = static_cast<int64_t>(n_seqs) * blocks_per_seq;
+    most = std::max(most, std::min(grow, n_free));
   }
-  const int64_t want = ceil_div(most > 0 ? most : 1, dk::paging::kFillThreads);
-  const int64_t cap = 8LL * sm_count(current_device());
-  e = launch_pdl(dk::paging::fill_kernel, dim3(static_cast<unsigned>(want < cap ? want : cap)),
-                 dim3(dk::paging::kFillThreads), 0, st, p);
+  const bool fill = rows || row_tiles || free_blocks;
+  // One CTA of 1024 threads writes up to 4096 rows in one pass in MEASALONE; a second launch of more CTAs.
+  const bool alone = fill && most <= static_cast<int64_t>(dk::paging::kScanThreads) * dk::paging::kRowVec;
+  const int64_t busy = std::max<int64_t>(n_seqs, alone ? ceil_div(most, dk::paging::kRowVec) : 0);
+  const dim3 threads(static_cast<unsigned>(
+      std::max<int64_t>(64, std::min<int64_t>(dk::paging::kScanThreads, 32 * ceil_div(busy, 32)))));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = alone ? launch_pdl(dk::paging::scan_kernel<true>, dim3(1), threads, 0, st, p)
+                        : launch_pdl(dk::paging::scan_kernel<false>, dim3(1), threads, 0, st, p);
+  if (e == cudaSuccess && fill && !alone) {
+    const int64_t run = dk::paging::kFillThreads * static_cast<int64_t>(rows ? dk::paging::kRowVec : 1);
+    const int64_t want = ceil_div(most, run), cap = 64LL * sm_count(current_device());
+    e = launch_pdl(dk::paging::fill_kernel, dim3(static_cast<unsigned>(std::min(want, cap))),
+                   dim3(dk::paging::kFillThreads), 0, st, p);
+  }
   if (e != cudaSuccess) return fail(DK_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
   return DK_OK;
 }

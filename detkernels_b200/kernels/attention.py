@@ -218,7 +218,10 @@ def attention_shared_prefix_reference(q, k_prefix, v_prefix, k, v, kv_lens, scal
 def _tma_strides(t, name):
     """Element strides of a 16-bit cache tensor as the kernels need them (unit along D, the others
     multiples of 8 elements, 16-byte aligned base); a dimension of one element takes any stride."""
-    st = list(t.stride())
+    st = t.stride()
+    if st[-1] == 1 and min(t.shape) > 1 and not any([s % 8 for s in st[:-1]]) and t.data_ptr() % 16 == 0:
+        return st
+    st = list(st)
     nat = 1
     for i in range(t.dim() - 1, -1, -1):
         if t.shape[i] <= 1:
@@ -293,7 +296,7 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
     if scale is None:
         scale = 1.0 / (D ** 0.5)
     if out is None:
-        out = torch.empty((R, H, D), dtype=q.dtype, device=q.device)
+        out = q.new_empty((R, H, D))
     assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and out.stride(2) == 1
     if row_tiles is not None:
         assert row_tiles.dtype == torch.int32 and row_tiles.device == q.device and row_tiles.is_contiguous()
@@ -302,23 +305,23 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
         return out
     if q.data_ptr() % 16 or q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8:
         q = q.clone(memory_format=torch.contiguous_format)
-    with torch.cuda.device(q.device):
+    with _lib.on_device(q.device):
         if P == 0:
             return attention_decode(q, k_cache, v_cache, kv_lens, scale=scale, row_tiles=row_tiles,
                                     max_kv_len=max_kv_len, out=out, block_table=block_table)
         ps, vps = _tma_strides(k_prefix, "k_prefix"), _tma_strides(v_prefix, "v_prefix")
-        assert ps == vps, "k and v prefixes must share strides"
+        assert tuple(ps) == tuple(vps), "k and v prefixes must share strides"
         cs = [0, 0, 0, 1]
         n_tiles = R if row_tiles is None else row_tiles.shape[0]
         if max_kv_len:
             cs, cvs = _tma_strides(k_cache, "k_cache"), _tma_strides(v_cache, "v_cache")
-            assert cs == cvs, "k and v caches must share strides"
+            assert tuple(cs) == tuple(cvs), "k and v caches must share strides"
             if uniform:
                 kv_lens = torch.full((R,), kv_lens, dtype=torch.int32, device=q.device)
         lib = _lib.load()
         nbytes = lib.dk_attention_shared_prefix_workspace_size(R, n_tiles, H, Hkv, D, P, max_kv_len)
         if workspace is None:
-            workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+            workspace = q.new_empty(max(nbytes, 16), dtype=torch.uint8)
         rc = lib.dk_attention_shared_prefix(
             q.data_ptr(), q.stride(0), q.stride(1), k_prefix.data_ptr(), v_prefix.data_ptr(),
             ps[0] if prefix_blocks is not None else 0, ps[-3], ps[-2], P,

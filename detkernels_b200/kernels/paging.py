@@ -90,12 +90,12 @@ def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=No
     def take(field, shape, dtype):
         t = getattr(out, field) if out is not None else None
         if t is None:
-            return torch.empty(shape, dtype=dtype, device=dev)
+            return kv_lens.new_empty(shape, dtype=dtype)
         assert t.dtype == dtype and t.device == dev and tuple(t.shape) == tuple(shape) and t.is_contiguous(), \
             "paged_plan: out.%s does not fit" % field
         return t
 
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         kv_lens, new_lens = kv_lens.contiguous(), new_lens.contiguous()
         cu = take("cu_rows", (B + 1,), torch.int32)
         cur = take("cursor", (1,), torch.int32) if cursor is not None else None
@@ -114,7 +114,7 @@ def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=No
                 cur.copy_(cursor.view(1))
             return plan
         lib = _lib.load()
-        ws = torch.empty(lib.dk_paged_plan_workspace_size(B), dtype=torch.uint8, device=dev)
+        ws = kv_lens.new_empty(-(-lib.dk_paged_plan_workspace_size(B) // 4))
 
         def ptr(t):
             # an output of no entries is still asked for: its pointer is never followed
@@ -125,7 +125,7 @@ def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=No
             kv_lens.data_ptr(), new_lens.data_ptr(), B, int(page_size),
             ptr(free_blocks), 0 if free_blocks is None else free_blocks.numel(), ptr(cursor), ptr(cur), cu.data_ptr(),
             ptr(row_seq), ptr(row_pos), ptr(slots), ptr(q_lens), n_rows or 0, ptr(tiles), int(rows_per_tile),
-            n_tiles or 0, ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev))
+            n_tiles or 0, ws.data_ptr(), 4 * ws.numel(), _lib.stream_ptr(dev))
     _lib.check(rc, "paged_plan")
     _lib.count_launch(2)
     return plan

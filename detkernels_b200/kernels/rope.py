@@ -111,11 +111,12 @@ def qk_norm_rope(q, k, positions, q_weight, k_weight, table, eps: float = 1e-6, 
         return t if t is None or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
     def st(t):
-        return (0, 0) if t is None else (t.stride(0), t.stride(1))
+        return (0, 0) if t is None else t.stride()[:2]
 
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         q2, k2, v2 = unit(q), unit(k), unit(v)
-        qw, kw = q_weight.reshape(-1).contiguous(), k_weight.reshape(-1).contiguous()
+        qw = q_weight if q_weight.is_contiguous() else q_weight.reshape(-1).contiguous()
+        kw = k_weight if k_weight.is_contiguous() else k_weight.reshape(-1).contiguous()
         pos = positions.contiguous()
         slots = slots.contiguous() if slots is not None else None
         rc = _lib.load().dk_qk_norm_rope(
