@@ -30,6 +30,27 @@ enum : int {
   kDetRows = 0x602,   // more rows or tiles than the outputs hold
 };
 
+// Division of any 32-bit n by a number that the host knows, after Granlund and Montgomery ("Division by
+// invariant integers using multiplication"): with l = ceil(log2 d) and m = floor(2^32 (2^l - d) / d) + 1,
+// n / d = (t + ((n - t) >> 1)) >> (l - 1), t the high half of m n; d = 1 is n itself.
+struct Divisor {
+  uint32_t d, m, sh1, sh2;
+};
+inline Divisor divisor(uint32_t d) {
+  uint32_t l = 0;
+  while ((1ull << l) < d) ++l;
+  const uint64_t m = ((((1ull << l) - d) << 32) / d) + 1;
+  return Divisor{d, static_cast<uint32_t>(m), l < 1 ? l : 1, l > 1 ? l - 1 : 0};
+}
+__device__ __forceinline__ uint32_t div_by(uint32_t n, const Divisor& v) {
+  const uint32_t t = __umulhi(v.m, n);
+  return (t + ((n - t) >> v.sh1)) >> v.sh2;
+}
+__device__ __forceinline__ uint32_t ceil_div32(uint32_t a, const Divisor& v) {
+  const uint32_t q = div_by(a, v);
+  return q + (a != q * v.d);
+}
+
 struct Params {
   int32_t* table;
   int64_t table_stride;
@@ -37,7 +58,7 @@ struct Params {
   const int32_t* kv;
   const int32_t* nw;
   int32_t n_seqs;
-  int32_t page;
+  Divisor page;
   const int32_t* free_list;  // null: the table does not grow
   int64_t n_free;
   const int32_t* cursor_in;
@@ -49,17 +70,13 @@ struct Params {
   int32_t* q_lens;
   int64_t n_rows;
   int32_t* tiles;           // null: no tiles
-  int32_t rpt;
+  int32_t tiled;            // tiles of rpt.d rows are asked for
+  Divisor rpt;
   int64_t n_tiles;
   int vec;                  // the row outputs take 16-byte stores
   // scratch: [0] 1 when the plan stands, [1] cursor, then cu_blk [n_seqs + 1], cu_tile [n_seqs + 1]
   int32_t* ws;
 };
-
-__device__ __forceinline__ uint32_t ceil_div32(uint32_t a, uint32_t b) {
-  const uint32_t q = a / b;
-  return q + (a != q * b);
-}
 
 struct Sum3 {
   int64_t r, k, t;
@@ -111,7 +128,7 @@ __device__ void fill_rows(const Params& p, int64_t cursor, int cta, int ctas) {
   const int64_t n = cu[p.n_seqs];
   const int64_t run = static_cast<int64_t>(blockDim.x) * kRowVec;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t page = p.page, rpt = p.rpt;
+  const uint32_t page = p.page.d;
   for (int64_t r0 = cta * run; r0 < n; r0 += ctas * run) {
     if (warp < 2) {
       const int64_t x = warp == 0 ? r0 : (r0 + run < n ? r0 + run : n) - 1;
@@ -140,9 +157,9 @@ __device__ void fill_rows(const Params& p, int64_t cursor, int cta, int ctas) {
             begin = cu[b];
             end = cu[b + 1];
             kv = p.kv[b];
-            have = ceil_div32(kv, page);
+            have = ceil_div32(kv, p.page);
             const uint32_t at = static_cast<uint32_t>(kv + (first + i - begin));
-            pg = at / page;
+            pg = div_by(at, p.page);
             off = at - pg * page;
             fresh = true;
           } else if (++off == page) {
@@ -166,11 +183,11 @@ __device__ void fill_rows(const Params& p, int64_t cursor, int cta, int ctas) {
           slot[i] = blk * page + off;
           if (p.tiles) {
             const uint32_t in = first + i - begin;
-            const uint32_t tile = in / rpt;
-            if (tile * rpt == in) {
+            const uint32_t tile = div_by(in, p.rpt);
+            if (tile * p.rpt.d == in) {
               int32_t* t = p.tiles + 3 * (static_cast<int64_t>(cu_tile[b]) + tile);
               t[0] = first + i;
-              t[1] = min(p.rpt, end - (first + i));
+              t[1] = min(static_cast<int>(p.rpt.d), end - (first + i));
               t[2] = b;
             }
           }
@@ -213,9 +230,9 @@ __device__ void fill_without_rows(const Params& p, int64_t cursor, int64_t tid, 
     const int64_t n = cu_tile[p.n_seqs];
     for (int64_t t = tid; t < n; t += step) {
       const int b = find_seq(cu_tile, 0, p.n_seqs, static_cast<int32_t>(t));
-      const int32_t at = static_cast<int32_t>(t - cu_tile[b]) * p.rpt;
+      const int32_t at = static_cast<int32_t>(t - cu_tile[b]) * static_cast<int32_t>(p.rpt.d);
       p.tiles[3 * t + 0] = p.cu_rows[b] + at;
-      p.tiles[3 * t + 1] = min(p.rpt, p.nw[b] - at);
+      p.tiles[3 * t + 1] = min(static_cast<int32_t>(p.rpt.d), p.nw[b] - at);
       p.tiles[3 * t + 2] = b;
     }
   }
@@ -261,7 +278,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(const Params p) {
           nw[i] = 0;
         } else {
           blk[i] = need - have;
-          if (p.rpt > 0) til[i] = ceil_div32(nw[i], p.rpt);
+          if (p.tiled) til[i] = ceil_div32(nw[i], p.rpt);
         }
         v.r += nw[i];
         v.k += blk[i];

@@ -242,7 +242,7 @@ int dk_paged_plan(int32_t* block_table, int64_t block_table_stride, int32_t bloc
   p.kv = kv_lens;
   p.nw = new_lens;
   p.n_seqs = n_seqs;
-  p.page = page_size;
+  p.page = dk::paging::divisor(page_size);
   p.free_list = free_blocks;
   p.n_free = n_free;
   p.cursor_in = cursor;
@@ -254,7 +254,8 @@ int dk_paged_plan(int32_t* block_table, int64_t block_table_stride, int32_t bloc
   p.q_lens = q_lens;
   p.n_rows = n_rows;
   p.tiles = row_tiles;
-  p.rpt = row_tiles ? rows_per_tile : 0;
+  p.tiled = row_tiles != nullptr;
+  p.rpt = dk::paging::divisor(row_tiles ? rows_per_tile : 1);
   p.n_tiles = n_tiles;
   p.ws = static_cast<int32_t*>(workspace);
   p.vec = aligned16(row_seq) && aligned16(row_pos) && aligned16(slots) && aligned16(q_lens);
