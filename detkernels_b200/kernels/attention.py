@@ -250,6 +250,8 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
     ``dk_attention_shared_prefix_workspace_size`` bytes (a new one if not given; its contents do not
     matter, and calls that may overlap need separate ones).
 
+    A row that row_tiles leaves out keeps what ``out`` holds (rows of a padded batch); with max_kv_len = 0
+    the tiles are not read and every row is written.
     A row's bits depend on its q, the prefix, its own tokens and nothing else of the batch."""
     import torch
 
@@ -332,5 +334,5 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
             row_tiles.data_ptr() if row_tiles is not None else None, n_tiles, R, H, Hkv, D, max_kv_len, float(scale),
             _lib.dtype_code(q.dtype), workspace.data_ptr(), workspace.numel(), _lib.stream_ptr(q.device))
     _lib.check(rc, "attention_shared_prefix")
-    _lib.count_launch(3 if max_kv_len else 2)
+    _lib.count_launch(2)   # at least: rows split over several warps take a third
     return out

@@ -200,6 +200,36 @@ def test_prefill_rows_of_ragged_sequences(dev, H, Hkv, D, page):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv,D,n_seq", [(4, 2, 64, 3), (4, 2, 64, 700), (16, 1, 128, 5), (2, 2, 32, 40)])
+def test_rows_that_no_tile_covers_are_left(dev, H, Hkv, D, n_seq):
+    """A batch padded behind its last sequence, and a gap in its middle: those rows keep what out held, whether
+    one warp owns a row (many tiles) or several do; the covered rows' bits are those of a batch without them."""
+    import torch
+    rng = np.random.default_rng(n_seq)
+    lens = [int(x) for x in rng.integers(1, 6, size=n_seq)]
+    q0, kp, vp, own, kw = _make(dev, torch.bfloat16, n_seq, H, Hkv, D, 300, lens, seed=4)
+    gap, pad = 3, 9
+    first = np.cumsum([0] + lens)[:-1] + gap * (np.arange(n_seq) >= n_seq // 2)
+    rows = int(first[-1] + lens[-1] + pad)
+    tiles = np.array([(f, n, s) for s, (f, n) in enumerate(zip(first, lens)) if n * (H // Hkv) <= 16]
+                     + [(f + i, 1, s) for s, (f, n) in enumerate(zip(first, lens)) if n * (H // Hkv) > 16
+                        for i in range(n)], np.int32)
+    rng.shuffle(tiles)
+    q = torch.randn(rows, H, D, device=dev, generator=torch.Generator(device=dev).manual_seed(8)).to(torch.bfloat16)
+    q_lens = np.zeros(rows, np.int32)
+    for f, n in zip(first, lens):
+        q_lens[f:f + n] = np.arange(1, n + 1)
+    covered = torch.from_numpy(q_lens > 0).to(dev)
+    q_lens[q_lens == 0] = 5   # a length of a row that is not there
+    out = torch.full_like(q, 7.0)
+    ln, tl = torch.from_numpy(q_lens).to(dev), torch.from_numpy(tiles).to(dev)
+    _call(q, kw, ln, row_tiles=tl, out=out)
+    assert (out[~covered] == 7.0).all() and int((~covered).sum()) == gap + pad
+    tight = torch.from_numpy(_tiles(lens, 16 // (H // Hkv))).to(dev)
+    assert torch.equal(out[covered], _call(q[covered], kw, ln[covered], row_tiles=tight))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,Hkv,D,P", [(8, 2, 64, 1500), (8, 8, 128, 700), (16, 2, 128, 5000), (4, 1, 32, 20000)])
 def test_a_row_does_not_depend_on_its_batch(dev, H, Hkv, D, P):
     """The same rows alone, in small batches and in one that takes whole groups a run: the same bits."""
@@ -247,7 +277,8 @@ def test_values_behind_a_rows_end_never_reach_it(dev, dt, D, page):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("R,H,Hkv,D,page", [(2, 4, 1, 64, 64), (3, 2, 2, 128, 0), (1, 16, 1, 128, 256), (700, 2, 1, 32, 0)])
+@pytest.mark.parametrize("R,H,Hkv,D,page", [(2, 4, 1, 64, 64), (3, 2, 2, 128, 0), (1, 16, 1, 128, 256), (700, 2, 1, 32, 0),
+                                               (700, 6, 3, 32, 0)])
 def test_long_own_sequences(dev, R, H, Hkv, D, page):
     """Own tokens over many splits, by one warp (many rows) or many (few rows): one definition, the same bits."""
     import torch
