@@ -25,7 +25,6 @@ namespace dk {
 namespace own {
 
 constexpr int kSplit = 64;
-constexpr int kStep = 16;
 constexpr int kRows = 16;
 
 enum : int {
@@ -99,9 +98,10 @@ struct Params {
 template <int D>
 struct Cfg {
   static constexpr int ROWB = D * 2;
-  static constexpr int TENSOR = kStep * ROWB;
+  static constexpr int STEP = D == 128 ? 16 : 32;   // tokens a step
+  static constexpr int TENSOR = STEP * ROWB;
   static constexpr int STAGE = 2 * TENSOR;
-  static constexpr int STAGES = D == 128 ? 3 : 4;
+  static constexpr int STAGES = D == 128 ? 3 : 2;
   static constexpr int RING = STAGES * STAGE;
   static constexpr int ROWF = D + 4;   // floats of a joined row in shared memory (conflict free either way)
   // the ring, then, for a warp that owns all splits, its 8 NB rows and their (m, l)
@@ -173,9 +173,10 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {   // an 8 x 8 matri
 
 // NB: column halves (8 query rows each).
 template <typename T, int D, int NB>
-__global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 14) : (D == 128 ? 12 : 16)) own_kernel(const Params p) {
+__global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 10) : (D == 128 ? 12 : 16)) own_kernel(const Params p) {
   using C = Cfg<D>;
   constexpr int KC = D / 16, CPR = D / 8;
+  constexpr int kStep = C::STEP, U = kStep / 16;
   constexpr int PER = kStep * CPR / 32;   // 16-byte chunks a lane copies of each tensor a step
   extern __shared__ __align__(128) uint8_t ring[];
   pdl_launch_dependents();
@@ -328,28 +329,35 @@ __global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 14) : (D == 128 
     issue(st + C::STAGES - 1);   // into the stage read in the previous step
     const uint32_t ka = ring_a + (st % C::STAGES) * C::STAGE, va = ka + C::TENSOR;
     const int t0 = t_begin + st * kStep;
-    float sc[NB][4];
+    float sc[U][NB][4];
 #pragma unroll
-    for (int h = 0; h < NB; ++h) sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.0f;
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
-    for (int kc = 0; kc < KC; ++kc) {
-      uint32_t a[4];
-      ldsm_x4(ka + chunk_off<D>(k_row, 2 * kc + k_c), a);
+      for (int h = 0; h < NB; ++h) sc[u][h][0] = sc[u][h][1] = sc[u][h][2] = sc[u][h][3] = 0.0f;
 #pragma unroll
-      for (int h = 0; h < NB; ++h) mma<T>(sc[h], a, qb[h][kc][0], qb[h][kc][1]);
+      for (int kc = 0; kc < KC; ++kc) {
+        uint32_t a[4];
+        ldsm_x4(ka + chunk_off<D>(16 * u + k_row, 2 * kc + k_c), a);
+#pragma unroll
+        for (int h = 0; h < NB; ++h) mma<T>(sc[u][h], a, qb[h][kc][0], qb[h][kc][1]);
+      }
     }
-    // scores: sc[h][0..1] token t0 + g, sc[h][2..3] token t0 + g + 8, columns 2 t4 and 2 t4 + 1
-    uint32_t pb[NB][2];
+    // scores: sc[u][h][0..1] token t0 + 16 u + g, sc[u][h][2..3] token t0 + 16 u + g + 8, columns 2 t4 and 2 t4 + 1
+    uint32_t pb[U][NB][2];
     bool same = true;
     float alpha[NB][2];
 #pragma unroll
     for (int h = 0; h < NB; ++h) {
-      float x[4];
+      float x[U][4];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        x[e] = (t0 + g < end[h][e]) ? __fmul_rn(sc[h][e], p.scale_log2) : -INFINITY;
-        x[2 + e] = (t0 + g + 8 < end[h][e]) ? __fmul_rn(sc[h][2 + e], p.scale_log2) : -INFINITY;
-        float mx = fmaxf(x[e], x[2 + e]);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          x[u][e] = (t0 + 16 * u + g < end[h][e]) ? __fmul_rn(sc[u][h][e], p.scale_log2) : -INFINITY;
+          x[u][2 + e] = (t0 + 16 * u + g + 8 < end[h][e]) ? __fmul_rn(sc[u][h][2 + e], p.scale_log2) : -INFINITY;
+          mx = fmaxf(mx, fmaxf(x[u][e], x[u][2 + e]));
+        }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -357,16 +365,23 @@ __global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 14) : (D == 128 
         const float ref = (mn == -INFINITY) ? 0.0f : mn;
         alpha[h][e] = exp2_hw(__fsub_rn(m_r[h][e], ref));
         same = same && alpha[h][e] == 1.0f;
-        x[e] = exp2_hw(__fsub_rn(x[e], ref));
-        x[2 + e] = exp2_hw(__fsub_rn(x[2 + e], ref));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          x[u][e] = exp2_hw(__fsub_rn(x[u][e], ref));
+          x[u][2 + e] = exp2_hw(__fsub_rn(x[u][2 + e], ref));
+        }
         m_r[h][e] = mn;
+        l_r[h][e] = __fmul_rn(l_r[h][e], alpha[h][e]);
       }
-      const uint32_t lo = pack2<T>(x[0], x[1]), hi = pack2<T>(x[2], x[3]);
-      const float2 a = unpack2<T>(lo), b = unpack2<T>(hi);
-      l_r[h][0] = __fmaf_rn(l_r[h][0], alpha[h][0], __fadd_rn(a.x, b.x));
-      l_r[h][1] = __fmaf_rn(l_r[h][1], alpha[h][1], __fadd_rn(a.y, b.y));
-      pb[h][0] = transpose8(lo);
-      pb[h][1] = transpose8(hi);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t lo = pack2<T>(x[u][0], x[u][1]), hi = pack2<T>(x[u][2], x[u][3]);
+        const float2 a = unpack2<T>(lo), b = unpack2<T>(hi);
+        l_r[h][0] = __fadd_rn(l_r[h][0], __fadd_rn(a.x, b.x));
+        l_r[h][1] = __fadd_rn(l_r[h][1], __fadd_rn(a.y, b.y));
+        pb[u][h][0] = transpose8(lo);
+        pb[u][h][1] = transpose8(hi);
+      }
     }
     if (!same) {   // a factor of exactly 1 changes nothing
 #pragma unroll
@@ -392,12 +407,14 @@ __global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 14) : (D == 128 
     }
     if (!alone) {
 #pragma unroll
-      for (int j = 0; j < KC; ++j) {
-        uint32_t a[4];
-        ldsm_x4_t(va + chunk_off<D>(v_row, 2 * j + v_c), a);
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int h = 0; h < NB; ++h) mma<T>(o[h][j], a, pb[h][0], pb[h][1]);
-      }
+        for (int j = 0; j < KC; ++j) {
+          uint32_t a[4];
+          ldsm_x4_t(va + chunk_off<D>(16 * u + v_row, 2 * j + v_c), a);
+#pragma unroll
+          for (int h = 0; h < NB; ++h) mma<T>(o[h][j], a, pb[u][h][0], pb[u][h][1]);
+        }
     } else {
       int left = lane < nr ? my_len : -1;
       for (int k = 0; k < nr; ++k) {
@@ -413,12 +430,14 @@ __global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 14) : (D == 128 
         __syncwarp();
 #pragma unroll
         for (int j = 0; j < KC; ++j) {
-          uint32_t a[4];
-          ldsm_x4_t(va + chunk_off<D>(v_row, 2 * j + v_c), a);
+          uint32_t a[U][4];
+#pragma unroll
+          for (int u = 0; u < U; ++u) ldsm_x4_t(va + chunk_off<D>(16 * u + v_row, 2 * j + v_c), a[u]);
 #pragma unroll
           for (int h = 0; h < NB; ++h) {
             float one[4] = {o[h][j][0], o[h][j][1], o[h][j][2], o[h][j][3]};
-            mma<T>(one, a, pb[h][0], pb[h][1]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) mma<T>(one, a[u], pb[u][h][0], pb[u][h][1]);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (col_row[h][e & 1] == row) o[h][j][e] = one[e];

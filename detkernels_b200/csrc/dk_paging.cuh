@@ -11,7 +11,7 @@
 // its four consecutive rows between those.  The row that opens a new page also writes the table entry,
 // and the row that opens a tile the tile, so that one search serves all outputs.  Bound by the 20
 // bytes stored per row when rows are many, by the latency of the two kernels' loads when they are few.
-// Inside a graph: 5 us for 7 sequences, 7 us for 256 prompts (62,794 rows), 23 us for 4099 prompts (2.1 M
+// Inside a graph: 5 us for 7 sequences, 7 us for 256 prompts (66,377 rows), 23 us for 4099 prompts (2.1 M
 // rows, floor 7 us), of which the scan takes 9 and the search and the look-ups 13; the stores add 2.
 #pragma once
 

@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
           }
           // The two tiles' warps of a scheduler take turns on its exponential unit: left alone they fall into
           // step, share it, and leave it idle together (4165 against 3800 cycles a
-          // block of both; 62,794 rows of 16 heads of 64 behind 256 tokens: 307 against 288 us).
+          // block of both; 6776 rows of 16 heads of 64 behind 4096 tokens: 307 against 288 us).
           if (it.tiles == 2) {
             if (!warp_wait(&turn[warp], tph, kDetTurn, abort_flag)) break;
             tph ^= 1u;

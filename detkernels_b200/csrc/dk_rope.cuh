@@ -182,7 +182,7 @@ __device__ __forceinline__ uint4 pack<__half>(const float* x) {
 // Warps walk units (a row, or part of one when rows are few) grid-stride, the next unit's position and
 // slot in flight while one is rotated.  The weights stay in shared memory as f32 and the angles are read
 // back from the cache a batch at a time, as 16-byte vectors: the loop is bound by the instructions it
-// issues before the bytes it moves, so that the 62,794-row prefill of 32 heads of 64 (floor 86 us) took
+// issues before the bytes it moves, so that the 66,377-row prefill of 32 vectors of 64 a row (floor 86 us) took
 // 161 us with both in registers through a type switch, 123 us with four vectors a lane in flight and
 // the spills of that, and takes 113 us with two.  One resident set of 3 CTAs an SM walks all units;
 // one CTA per 8 units took 15 % more.
