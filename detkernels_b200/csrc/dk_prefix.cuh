@@ -589,6 +589,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
           // The two tiles' warps of a scheduler take turns on its exponential unit: left alone they fall into
           // step, share it, and leave it idle together (4165 against 3800 cycles a
           // block of both; 6776 rows of 16 heads of 64 behind 4096 tokens: 307 against 288 us).
+          // the last block's P.V has read its weights (long since); no branch below, so that the chunks overlap
+          if (!pv_done()) break;
           if (it.tiles == 2) {
             if (!warp_wait(&turn[warp], tph, kDetTurn, abort_flag)) break;
             tph ^= 1u;
@@ -607,8 +609,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
               sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
               pk[i >> 1] = pack2<T>(e.x, e.y);
             }
-            // the last block's P.V has read its weights (long since)
-            if (c == 0 && !pv_done()) break;
             tmem_st_x16(p_t + c * 16, pk);
           }
           if (it.tiles == 2 && lane == 0) mbar_arrive(&turn[warp ^ 4]);
