@@ -586,11 +586,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
             }
             l = __fmul_rn(l, alpha);
           }
-          // The two tiles' warps of a scheduler take turns on its exponential unit: left alone they fall into
-          // step, share it, and leave it idle together (4165 against 3800 cycles a
-          // block of both; 6776 rows of 16 heads of 64 behind 4096 tokens: 307 against 288 us).
-          // the last block's P.V has read its weights (long since); no branch below, so that the chunks overlap
+          // the last block's P.V has read its weights (long since); no wait below, so that the chunks overlap
           if (!pv_done()) break;
+          // The two tiles' warps of a scheduler take turns on its exponential unit, a warp's first half beside the
+          // other's second: left alone they fall into step, share it, and leave it idle together (6776 rows of 16
+          // heads of 64 behind 4096 tokens: 267 us; taken whole, 240 us; so, 232 us).
           if (it.tiles == 2) {
             if (!warp_wait(&turn[warp], tph, kDetTurn, abort_flag)) break;
             tph ^= 1u;
@@ -601,6 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
 #pragma unroll
           for (int c = 0; c < NR; ++c) {
             uint32_t pk[16];
+            if (c == NR / 2 && it.tiles == 2 && lane == 0) mbar_arrive(&turn[warp ^ 4]);
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               float2 e = fma2(make_float2(s[c][i], s[c][i + 1]), c2, n2);
@@ -611,7 +612,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
             }
             tmem_st_x16(p_t + c * 16, pk);
           }
-          if (it.tiles == 2 && lane == 0) mbar_arrive(&turn[warp ^ 4]);
           tmem_st_wait();
           const float2 ps = add2(sum[0], sum[1]);
           l = __fadd_rn(l, __fadd_rn(ps.x, ps.y));
