@@ -252,10 +252,9 @@ def dtype_code(dtype) -> int:
 def stream_ptr(device=None) -> int:
     """The current stream of the device (the current one's by default) as a raw handle."""
     import torch
-    index = device if isinstance(device, int) else getattr(device, "index", None)
-    if index is None:
-        return torch.cuda.current_stream(device).cuda_stream
-    return torch._C._cuda_getCurrentRawStream(index)
+    if isinstance(device, torch.device) and device.index is not None and torch.cuda.is_initialized():
+        return torch._C._cuda_getCurrentRawStream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 _no_guard = contextlib.nullcontext()

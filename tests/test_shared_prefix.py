@@ -460,3 +460,87 @@ def test_a_decode_step_of_plan_norm_and_attention(dev, D, page):
             at += m
         _tol_check(out[some], qr[some], kp, vp, rows_k, rows_v, D ** -0.5)
     assert math.isfinite(float(out.float().sum()))
+
+
+def _step_state(dev, B, H, Hkv, D, P, page, seed):
+    import torch
+
+    from detkernels_b200.kernels.rope import rope_table
+    g = torch.Generator(device=dev).manual_seed(seed)
+
+    def randn(*s):
+        return torch.randn(*s, device=dev, generator=g).to(torch.bfloat16)
+    n_pre = -(-P // page)
+    st = dict(kc=randn(n_pre + 4 * B, Hkv, page, D), vc=randn(n_pre + 4 * B, Hkv, page, D), qkv=randn(B, (H + 2 * Hkv) * D),
+              qw=randn(D), kw=randn(D), rope=rope_table(2048, D, device=dev), kv=torch.full((B,), 60, dtype=torch.int32, device=dev),
+              nw=torch.ones(B, dtype=torch.int32, device=dev), cursor=torch.full((1,), B, dtype=torch.int32, device=dev))
+    order = torch.randperm(n_pre + 4 * B, device=dev, generator=g).to(torch.int32)
+    st["pre"], st["free"] = order[:n_pre].contiguous(), order[n_pre:].contiguous()
+    st["table"] = torch.zeros(B, 4, dtype=torch.int32, device=dev)
+    st["table"][:, 0] = st["free"][:B]     # 60 tokens each
+    return st
+
+
+def _step(st, H, Hkv, D, P, page, out=None):
+    """One decode step in place: plan, norm into the cache, attention, lengths."""
+    from detkernels_b200.kernels.attention import attention_shared_prefix
+    from detkernels_b200.kernels.paging import paged_plan
+    from detkernels_b200.kernels.rope import qk_norm_rope
+    B = st["qkv"].shape[0]
+    q, k, v = (x.view(B, -1, D) for x in st["qkv"].split([H * D, Hkv * D, Hkv * D], 1))
+    plan = paged_plan(st["table"], st["kv"], st["nw"], page, free_blocks=st["free"], cursor=st["cursor"], n_rows=B, out=out)
+    if plan.cursor is not st["cursor"]:
+        st["cursor"].copy_(plan.cursor)
+    qr, _ = qk_norm_rope(q, k, plan.row_pos, st["qw"], st["kw"], st["rope"], v=v, k_cache=st["kc"], v_cache=st["vc"],
+                         slots=plan.slots)
+    o = attention_shared_prefix(qr, st["kc"], st["vc"], st["kc"], st["vc"], plan.q_lens, prefix_len=P,
+                                prefix_blocks=st["pre"], block_table=st["table"])
+    st["kv"] += st["nw"]
+    return o, plan
+
+
+@pytest.mark.gpu
+def test_a_captured_step_replays_as_eager_steps(dev):
+    """A whole step captured once, its plan in the tensors of an earlier call, replayed over a page's end."""
+    import torch
+
+    from detkernels_b200 import _lib
+    dims = (8, 4, 64, 130, 64)
+    a, b = (_step_state(dev, 6, *dims, seed=5) for _ in range(2))
+    o, plan = _step(a, *dims)
+    plan = plan._replace(cursor=a["cursor"])
+    want, _ = _step(b, *dims)
+    assert torch.equal(o, want)
+    g = torch.cuda.CUDAGraph()
+    keep = {k: v.clone() for k, v in a.items()}
+    with _lib.graph_capture(g):
+        o, _ = _step(a, *dims, out=plan)
+    for k, v in keep.items():
+        assert torch.equal(a[k], v), k            # a capture runs nothing
+    for _ in range(9):
+        g.replay()
+        want, _ = _step(b, *dims)
+        assert torch.equal(o, want)
+        for k in ("table", "cursor", "kv", "kc", "vc"):
+            assert torch.equal(a[k], b[k]), k
+    assert int(a["cursor"]) == 12 and int(a["kv"][0]) == 70
+
+
+@pytest.mark.gpu
+def test_steps_on_two_streams_at_once(dev):
+    """Two servers' steps side by side on two streams, against the same steps one after the other."""
+    import torch
+    dims = [(8, 4, 64, 130, 64), (16, 2, 128, 1500, 128)]
+    make = lambda: [_step_state(dev, n, *d, seed=s) for s, (n, d) in enumerate(zip((6, 90), dims))]
+    alone, both = make(), make()
+    want = [[_step(st, *d)[0] for _ in range(20)] for st, d in zip(alone, dims)]
+    torch.cuda.synchronize(dev)
+    streams = [torch.cuda.Stream(device=dev) for _ in dims]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(_step(both[i], *dims[i])[0])
+    torch.cuda.synchronize(dev)
+    for w, g in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(w, g))
