@@ -219,17 +219,24 @@ def _tma_strides(t, name):
     """Element strides of a 16-bit cache tensor as the kernels need them (unit along D, the others
     multiples of 8 elements, 16-byte aligned base); a dimension of one element takes any stride."""
     st = t.stride()
-    if st[-1] == 1 and min(t.shape) > 1 and not any([s % 8 for s in st[:-1]]) and t.data_ptr() % 16 == 0:
-        return st
-    st = list(st)
-    nat = 1
-    for i in range(t.dim() - 1, -1, -1):
-        if t.shape[i] <= 1:
-            st[i] = nat
-        nat = max(nat, st[i] * max(1, t.shape[i]))
-    if st[-1] != 1 or any(s % 8 for s in st[:-1]) or t.data_ptr() % 16:
+    if min(t.shape) <= 1:
+        st, nat = list(st), 1
+        for i in range(t.dim() - 1, -1, -1):
+            if t.shape[i] <= 1:
+                st[i] = nat
+            nat = max(nat, st[i] * max(1, t.shape[i]))
+        st = tuple(st)
+    if st[-1] != 1 or any([s % 8 for s in st[:-1]]) or t.data_ptr() % 16:
         raise ValueError("%s: unit stride along head_dim, strides that are multiples of 8 elements and a 16-byte "
                          "aligned start required" % name)
+    return st
+
+
+def _shared_strides(k, v, what):
+    """The strides of a pair of equal shape, which must share them."""
+    st = _tma_strides(k, "k_" + what)
+    if v.stride() != k.stride() or v.data_ptr() % 16:
+        assert _tma_strides(v, "v_" + what) == st, "k and v %s must share strides" % what
     return st
 
 
@@ -255,35 +262,37 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
     A row's bits depend on its q, the prefix, its own tokens and nothing else of the batch."""
     import torch
 
+    dev, dt = q.device, q.dtype
+    index = dev.index
     for t in (q, k_prefix, v_prefix, k_cache, v_cache):
-        assert t.is_cuda and t.device == q.device, "attention_shared_prefix requires CUDA tensors on one device"
-    R, H, D = q.shape
-    for t in (k_prefix, v_prefix, k_cache, v_cache):
-        if t.dtype != q.dtype:
+        assert t.is_cuda and t.get_device() == index, "attention_shared_prefix requires CUDA tensors on one device"
+        if t.dtype != dt:
             raise TypeError("attention_shared_prefix: q, the prefix and the caches must share a dtype")
-    assert v_prefix.shape == k_prefix.shape and v_cache.shape == k_cache.shape, "q/k/v shape mismatch"
-    n_seq, Hkv, cap, Dk = k_cache.shape
+    R, H, D = q_shape = q.shape
+    p_shape, c_shape = k_prefix.shape, k_cache.shape
+    assert v_prefix.shape == p_shape and v_cache.shape == c_shape, "q/k/v shape mismatch"
+    n_seq, Hkv, cap, Dk = c_shape
     assert Dk == D and H % Hkv == 0, "q/k/v shape mismatch"
     n_pool = page_p = 0
     if prefix_blocks is None:
-        assert k_prefix.dim() == 3 and k_prefix.shape[0] == Hkv and k_prefix.shape[2] == D, "prefix shape mismatch"
-        p_cap = k_prefix.shape[1]
+        assert len(p_shape) == 3 and p_shape[0] == Hkv and p_shape[2] == D, "prefix shape mismatch"
+        p_cap = p_shape[1]
     else:
-        assert prefix_blocks.dtype == torch.int32 and prefix_blocks.device == q.device and prefix_blocks.dim() == 1
+        assert prefix_blocks.dtype == torch.int32 and prefix_blocks.get_device() == index and prefix_blocks.dim() == 1
         assert prefix_blocks.numel() <= 1 or prefix_blocks.stride(0) == 1
-        assert k_prefix.dim() == 4 and k_prefix.shape[1] == Hkv and k_prefix.shape[3] == D, "prefix shape mismatch"
-        n_pool, page_p = k_prefix.shape[0], k_prefix.shape[2]
+        assert len(p_shape) == 4 and p_shape[1] == Hkv and p_shape[3] == D, "prefix shape mismatch"
+        n_pool, page_p = p_shape[0], p_shape[2]
         p_cap = prefix_blocks.numel() * page_p
     P = p_cap if prefix_len is None else int(prefix_len)
     if P < 0 or P > p_cap:
         raise ValueError("attention_shared_prefix: prefix_len %d outside [0, %d]" % (P, p_cap))
     uniform = isinstance(kv_lens, int)
     if not uniform:
-        assert kv_lens.dtype == torch.int32 and kv_lens.device == q.device and kv_lens.numel() == R
+        assert kv_lens.dtype == torch.int32 and kv_lens.get_device() == index and kv_lens.numel() == R
         kv_lens = kv_lens.contiguous()
     n_blocks = page = width = bt_stride = 0
     if block_table is not None:
-        assert block_table.dtype == torch.int32 and block_table.device == q.device and block_table.dim() == 2
+        assert block_table.dtype == torch.int32 and block_table.get_device() == index and block_table.dim() == 2
         assert block_table.shape[1] <= 1 or block_table.stride(1) == 1
         n_blocks, page = n_seq, cap
         n_seq, width = block_table.shape
@@ -298,26 +307,27 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
     if scale is None:
         scale = 1.0 / (D ** 0.5)
     if out is None:
-        out = q.new_empty((R, H, D))
-    assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and out.stride(2) == 1
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    o_st = out.stride()
+    assert out.shape == q_shape and out.dtype == dt and out.get_device() == index and o_st[2] == 1
     if row_tiles is not None:
-        assert row_tiles.dtype == torch.int32 and row_tiles.device == q.device and row_tiles.is_contiguous()
+        assert row_tiles.dtype == torch.int32 and row_tiles.get_device() == index and row_tiles.is_contiguous()
         assert row_tiles.dim() == 2 and row_tiles.shape[1] == 3
     if R == 0:
         return out
-    if q.data_ptr() % 16 or q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8:
+    q_st = q.stride()
+    if q.data_ptr() % 16 or q_st[2] != 1 or q_st[0] % 8 or q_st[1] % 8:
         q = q.clone(memory_format=torch.contiguous_format)
-    with _lib.on_device(q.device):
+        q_st = q.stride()
+    with _lib.on_device(dev):
         if P == 0:
             return attention_decode(q, k_cache, v_cache, kv_lens, scale=scale, row_tiles=row_tiles,
                                     max_kv_len=max_kv_len, out=out, block_table=block_table)
-        ps, vps = _tma_strides(k_prefix, "k_prefix"), _tma_strides(v_prefix, "v_prefix")
-        assert tuple(ps) == tuple(vps), "k and v prefixes must share strides"
+        ps = _shared_strides(k_prefix, v_prefix, "prefix")
         cs = [0, 0, 0, 1]
         n_tiles = R if row_tiles is None else row_tiles.shape[0]
         if max_kv_len:
-            cs, cvs = _tma_strides(k_cache, "k_cache"), _tma_strides(v_cache, "v_cache")
-            assert tuple(cs) == tuple(cvs), "k and v caches must share strides"
+            cs = _shared_strides(k_cache, v_cache, "cache")
             if uniform:
                 kv_lens = torch.full((R,), kv_lens, dtype=torch.int32, device=q.device)
         lib = _lib.load()
@@ -325,14 +335,14 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
         if workspace is None:
             workspace = q.new_empty(max(nbytes, 16), dtype=torch.uint8)
         rc = lib.dk_attention_shared_prefix(
-            q.data_ptr(), q.stride(0), q.stride(1), k_prefix.data_ptr(), v_prefix.data_ptr(),
+            q.data_ptr(), q_st[0], q_st[1], k_prefix.data_ptr(), v_prefix.data_ptr(),
             ps[0] if prefix_blocks is not None else 0, ps[-3], ps[-2], P,
             prefix_blocks.data_ptr() if prefix_blocks is not None else None, n_pool, page_p, k_cache.data_ptr(),
             v_cache.data_ptr(), cs[0], cs[1], cs[2], n_seq, cap,
             block_table.data_ptr() if block_table is not None else None, bt_stride, width, n_blocks, page,
-            out.data_ptr(), out.stride(0), out.stride(1), None if uniform and not max_kv_len else kv_lens.data_ptr(),
+            out.data_ptr(), o_st[0], o_st[1], None if uniform and not max_kv_len else kv_lens.data_ptr(),
             row_tiles.data_ptr() if row_tiles is not None else None, n_tiles, R, H, Hkv, D, max_kv_len, float(scale),
-            _lib.dtype_code(q.dtype), workspace.data_ptr(), workspace.numel(), _lib.stream_ptr(q.device))
+            _lib.dtype_code(dt), workspace.data_ptr(), workspace.numel(), _lib.stream_ptr(dev))
     _lib.check(rc, "attention_shared_prefix")
     _lib.count_launch(2)   # at least: rows split over several warps take a third
     return out

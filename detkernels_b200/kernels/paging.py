@@ -26,6 +26,9 @@ class PagedPlan(NamedTuple):
     row_tiles: Optional[object]    # int32 [n_tiles, 3]: (first row, rows, sequence)
 
 
+_NOTHING = PagedPlan(*[None] * len(PagedPlan._fields))
+
+
 def paged_plan_reference(block_table, kv_lens, new_lens, page_size, *, free_blocks=None, cursor=0, rows_per_tile=0):
     """Plain Python plan of one step on host sequences; block_table is a list of lists.  Returns the
     fields of PagedPlan as Python lists (block_table a grown copy)."""
@@ -66,47 +69,46 @@ def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=No
     outputs but cu_rows as they were."""
     import torch
 
-    dev = block_table.device
-    B = kv_lens.numel()
-    assert block_table.is_cuda and kv_lens.device == dev and new_lens.device == dev, \
+    dev, i32 = block_table.device, torch.int32
+    B, index = kv_lens.numel(), dev.index
+    assert block_table.is_cuda and kv_lens.get_device() == index and new_lens.get_device() == index, \
         "paged_plan requires CUDA tensors on one device"
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] >= B
-    assert block_table.shape[1] <= 1 or block_table.stride(1) == 1, "block_table: unit stride along a row"
-    for t in (kv_lens, new_lens):
-        assert t.dtype == torch.int32 and t.dim() == 1 and t.numel() == B, "lengths must be int32 [B]"
+    shape, stride = block_table.shape, block_table.stride()
+    assert block_table.dtype == i32 and len(shape) == 2 and shape[0] >= B
+    assert shape[1] <= 1 or stride[1] == 1, "block_table: unit stride along a row"
+    assert kv_lens.dtype == i32 and new_lens.dtype == i32 and kv_lens.dim() == 1 and new_lens.shape == (B,), \
+        "lengths must be int32 [B]"
     if page_size < 1:
         raise ValueError("paged_plan: page_size must be positive")
     if (free_blocks is None) != (cursor is None):
         raise ValueError("paged_plan: free_blocks and cursor go together")
     if free_blocks is not None:
-        assert free_blocks.dtype == torch.int32 and free_blocks.device == dev and free_blocks.is_contiguous()
-        assert cursor.dtype == torch.int32 and cursor.device == dev and cursor.numel() == 1
+        assert free_blocks.dtype == i32 and free_blocks.get_device() == index and free_blocks.is_contiguous()
+        assert cursor.dtype == i32 and cursor.get_device() == index and cursor.numel() == 1
     if rows_per_tile < 0 or (rows_per_tile > 0 and n_tiles is None) or (rows_per_tile == 0 and n_tiles):
         raise ValueError("paged_plan: rows_per_tile and n_tiles go together")
-    for n in (n_rows, n_tiles):
-        if n is not None and n < 0:
-            raise ValueError("paged_plan: n_rows and n_tiles must not be negative")
+    if (n_rows is not None and n_rows < 0) or (n_tiles is not None and n_tiles < 0):
+        raise ValueError("paged_plan: n_rows and n_tiles must not be negative")
 
-    def take(field, shape, dtype):
-        t = getattr(out, field) if out is not None else None
+    def take(t, *shape, dtype=i32):
+        """The tensor of an earlier plan, or a new one."""
         if t is None:
-            return kv_lens.new_empty(shape, dtype=dtype)
-        assert t.dtype == dtype and t.device == dev and tuple(t.shape) == tuple(shape) and t.is_contiguous(), \
-            "paged_plan: out.%s does not fit" % field
+            return kv_lens.new_empty(*shape) if dtype == i32 else kv_lens.new_empty(shape, dtype=dtype)
+        assert t.dtype == dtype and t.get_device() == index and t.shape == shape and t.is_contiguous(), \
+            "paged_plan: a tensor of out does not fit"
         return t
 
+    old = out if out is not None else _NOTHING
     with _lib.on_device(dev):
         kv_lens, new_lens = kv_lens.contiguous(), new_lens.contiguous()
-        cu = take("cu_rows", (B + 1,), torch.int32)
-        cur = take("cursor", (1,), torch.int32) if cursor is not None else None
+        cu = take(old.cu_rows, B + 1)
+        cur = take(old.cursor, 1) if cursor is not None else None
         row_seq = row_pos = slots = q_lens = tiles = None
         if n_rows is not None:
-            row_seq = take("row_seq", (n_rows,), torch.int32)
-            row_pos = take("row_pos", (n_rows,), torch.int32)
-            slots = take("slots", (n_rows,), torch.int64)
-            q_lens = take("q_lens", (n_rows,), torch.int32)
+            row_seq, row_pos, q_lens = take(old.row_seq, n_rows), take(old.row_pos, n_rows), take(old.q_lens, n_rows)
+            slots = take(old.slots, n_rows, dtype=torch.int64)
         if rows_per_tile > 0:
-            tiles = take("row_tiles", (n_tiles, 3), torch.int32)
+            tiles = take(old.row_tiles, n_tiles, 3)
         plan = PagedPlan(block_table, cur, cu, row_seq, row_pos, slots, q_lens, tiles)
         if B == 0:
             cu.zero_()
@@ -115,17 +117,17 @@ def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=No
             return plan
         lib = _lib.load()
         ws = kv_lens.new_empty(-(-lib.dk_paged_plan_workspace_size(B) // 4))
+        ws_ptr = ws.data_ptr()
 
         def ptr(t):
             # an output of no entries is still asked for: its pointer is never followed
-            return None if t is None else (t.data_ptr() or ws.data_ptr())
+            return None if t is None else (t.data_ptr() or ws_ptr)
 
         rc = lib.dk_paged_plan(
-            block_table.data_ptr(), max(block_table.stride(0), block_table.shape[1]), block_table.shape[1],
-            kv_lens.data_ptr(), new_lens.data_ptr(), B, int(page_size),
-            ptr(free_blocks), 0 if free_blocks is None else free_blocks.numel(), ptr(cursor), ptr(cur), cu.data_ptr(),
-            ptr(row_seq), ptr(row_pos), ptr(slots), ptr(q_lens), n_rows or 0, ptr(tiles), int(rows_per_tile),
-            n_tiles or 0, ws.data_ptr(), 4 * ws.numel(), _lib.stream_ptr(dev))
+            block_table.data_ptr(), max(stride[0], shape[1]), shape[1], kv_lens.data_ptr(), new_lens.data_ptr(), B,
+            int(page_size), ptr(free_blocks), 0 if free_blocks is None else free_blocks.numel(), ptr(cursor), ptr(cur),
+            cu.data_ptr(), ptr(row_seq), ptr(row_pos), ptr(slots), ptr(q_lens), n_rows or 0, ptr(tiles),
+            int(rows_per_tile), n_tiles or 0, ws_ptr, 4 * ws.numel(), _lib.stream_ptr(dev))
     _lib.check(rc, "paged_plan")
     _lib.count_launch(2)
     return plan

@@ -63,70 +63,80 @@ def qk_norm_rope(q, k, positions, q_weight, k_weight, table, eps: float = 1e-6, 
     Returns (q_out, k_out); k_out is None when the keys went to the cache only."""
     import torch
 
-    dev = q.device
+    dev, dt = q.device, q.dtype
     assert q.is_cuda, "qk_norm_rope requires CUDA tensors"
     T, H, D = q.shape
-    assert k.dim() == 3 and k.shape[0] == T and k.shape[2] == D, "q/k shape mismatch"
-    Hkv = k.shape[1]
-    if k.dtype != q.dtype or q_weight.dtype != k_weight.dtype:
+    kv_shape = k.shape
+    assert len(kv_shape) == 3 and kv_shape[0] == T and kv_shape[2] == D, "q/k shape mismatch"
+    Hkv = kv_shape[1]
+    if k.dtype != dt or q_weight.dtype != k_weight.dtype:
         raise TypeError("qk_norm_rope: q and k, and the two weights, must share a dtype")
     assert q_weight.numel() == D and k_weight.numel() == D, "qk_norm_rope: weights must have head_dim elements"
-    assert positions.dtype in (torch.int32, torch.int64) and positions.dim() == 1 and positions.numel() == T, \
+    assert positions.dtype in (torch.int32, torch.int64) and positions.shape == (T,), \
         "positions must be int32 or int64 [T]"
     assert table.dtype == torch.float32 and table.dim() == 2 and table.is_contiguous(), "table must be f32, contiguous"
     if D > MAX_HEAD_DIM:
         raise NotImplementedError("qk_norm_rope: head_dim %d > %d" % (D, MAX_HEAD_DIM))
-    rd = table.shape[1]
-    if rd < 2 or rd % 2 or rd > D or table.shape[0] < 1:
+    max_pos, rd = table.shape
+    if rd < 2 or rd % 2 or rd > D or max_pos < 1:
         raise ValueError("qk_norm_rope: a table of an even rotary_dim in [2, head_dim] required")
-    cached = [t is not None for t in (v, k_cache, v_cache, slots)]
-    if any(cached) != all(cached):
+    n_cache = (v is not None) + (k_cache is not None) + (v_cache is not None) + (slots is not None)
+    if n_cache not in (0, 4):
         raise ValueError("qk_norm_rope: v, k_cache, v_cache and slots go together")
     tensors = [k, positions, q_weight, k_weight, table]
-    cs, n_slabs, cap = (0, 0, 0), 0, 0
-    if all(cached):
+    cs, n_slabs, cap = (0, 0, 0, 1), 0, 0
+    if n_cache:
         tensors += [v, k_cache, v_cache, slots]
-        assert v.shape == k.shape and v.dtype == k.dtype, "k/v shape mismatch"
-        assert k_cache.dtype == q.dtype and v_cache.dtype == q.dtype and k_cache.shape == v_cache.shape
-        assert k_cache.dim() == 4 and k_cache.shape[1] == Hkv and k_cache.shape[3] == D, "cache shape mismatch"
-        assert k_cache.stride() == v_cache.stride() and (D <= 1 or k_cache.stride(3) == 1), \
+        assert v.shape == kv_shape and v.dtype == dt, "k/v shape mismatch"
+        c_shape, cs = k_cache.shape, k_cache.stride()
+        assert k_cache.dtype == dt and v_cache.dtype == dt and c_shape == v_cache.shape
+        assert len(c_shape) == 4 and c_shape[1] == Hkv and c_shape[3] == D, "cache shape mismatch"
+        assert cs == v_cache.stride() and (D <= 1 or cs[3] == 1), \
             "k and v caches must share strides, with a unit stride along head_dim"
-        assert slots.dtype == torch.int64 and slots.dim() == 1 and slots.numel() == T, "slots must be int64 [T]"
-        n_slabs, cap, cs = k_cache.shape[0], k_cache.shape[2], k_cache.stride()[:3]
+        assert slots.dtype == torch.int64 and slots.shape == (T,), "slots must be int64 [T]"
+        n_slabs, cap = c_shape[0], c_shape[2]
     elif k_out is None:
-        k_out = torch.empty((T, Hkv, D), dtype=k.dtype, device=dev)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     if q_out is None:
-        q_out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
-    assert q_out.shape == q.shape and q_out.dtype == q.dtype and (D <= 1 or q_out.stride(2) == 1)
-    tensors.append(q_out)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        assert q_out.shape == q.shape and q_out.dtype == dt
+        tensors.append(q_out)
+    qo_st, ko_st = q_out.stride(), (0, 0, 1)
     if k_out is not None:
-        assert k_out.shape == k.shape and k_out.dtype == k.dtype and (D <= 1 or k_out.stride(2) == 1)
+        assert k_out.shape == kv_shape and k_out.dtype == dt
         tensors.append(k_out)
+        ko_st = k_out.stride()
+    assert D <= 1 or (qo_st[2] == 1 and ko_st[2] == 1), "outputs must have a unit stride along head_dim"
+    index = dev.index
     for t in tensors:
-        assert t.device == dev, "qk_norm_rope: all tensors must be on q's device"
+        assert t.get_device() == index, "qk_norm_rope: all tensors must be on q's device"
     if T == 0:
         return q_out, k_out
 
     def unit(t):
-        return t if t is None or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
-
-    def st(t):
-        return (0, 0) if t is None else t.stride()[:2]
+        """t and its strides, with a unit stride along head_dim."""
+        st = t.stride()
+        if D <= 1 or st[2] == 1:
+            return t, st
+        t = t.contiguous()
+        return t, t.stride()
 
     with _lib.on_device(dev):
-        q2, k2, v2 = unit(q), unit(k), unit(v)
+        (q2, q_st), (k2, k_st) = unit(q), unit(k)
+        v2, v_st = unit(v) if n_cache else (None, (0, 0))
         qw = q_weight if q_weight.is_contiguous() else q_weight.reshape(-1).contiguous()
         kw = k_weight if k_weight.is_contiguous() else k_weight.reshape(-1).contiguous()
         pos = positions.contiguous()
-        slots = slots.contiguous() if slots is not None else None
+        slots = slots.contiguous() if n_cache else None
         rc = _lib.load().dk_qk_norm_rope(
-            q2.data_ptr(), *st(q2), k2.data_ptr(), *st(k2), v2.data_ptr() if v2 is not None else None, *st(v2),
-            q_out.data_ptr(), *st(q_out), k_out.data_ptr() if k_out is not None else None, *st(k_out),
-            k_cache.data_ptr() if k_cache is not None else None, v_cache.data_ptr() if v_cache is not None else None,
-            *cs, n_slabs, cap, slots.data_ptr() if slots is not None else None, pos.data_ptr(),
+            q2.data_ptr(), q_st[0], q_st[1], k2.data_ptr(), k_st[0], k_st[1], v2.data_ptr() if n_cache else None,
+            v_st[0], v_st[1], q_out.data_ptr(), qo_st[0], qo_st[1], k_out.data_ptr() if k_out is not None else None,
+            ko_st[0], ko_st[1], k_cache.data_ptr() if n_cache else None, v_cache.data_ptr() if n_cache else None,
+            cs[0], cs[1], cs[2], n_slabs, cap, slots.data_ptr() if n_cache else None, pos.data_ptr(),
             1 if pos.dtype == torch.int64 else 0, qw.data_ptr(), kw.data_ptr(), _lib.dtype_code(qw.dtype),
-            table.data_ptr(), table.shape[0], T, H, Hkv, D, rd, 1 if interleaved else 0, float(eps),
-            _lib.dtype_code(q.dtype), _lib.stream_ptr(dev))
+            table.data_ptr(), max_pos, T, H, Hkv, D, rd, 1 if interleaved else 0, float(eps),
+            _lib.dtype_code(dt), _lib.stream_ptr(dev))
     _lib.check(rc, "qk_norm_rope")
     _lib.count_launch()
     return q_out, k_out
