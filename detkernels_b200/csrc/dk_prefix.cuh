@@ -13,8 +13,8 @@
 //     by more than 8 (a factor 256, so the weights stay in range of either 16-bit type), weights
 //     2^(S c - m) rounded to the input type for P.V as the left operand of a second tcgen05.mma in
 //     TMEM, l summed in f32 from the unrounded weights in a fixed order.
-//   * The chunks' states are joined in order inside groups of kGroup chunks (head_dim <= 64 only),
-//     the groups' states in order, and the states of the row's own tokens last.
+//   * The chunks' states are joined in order inside groups of group_chunks(D) chunks, the groups' states
+//     in order, and the states of the row's own tokens last.
 // No step looks at another row, so a row's bits do not depend on the batch.
 //
 // Work: an item is (up to two tiles of 128 rows, KV head, run of tokens), one persistent CTA per SM.
@@ -23,8 +23,12 @@
 // weights and the accumulator apart, so that the next scores are formed as soon as these are in
 // registers and the softmax, which is bound by the exponential unit, does not wait for products: blocks of
 // 128 tokens for head_dim <= 64, of 64 for 128 (whose accumulators take half of TMEM).  A run is a whole
-// group, whose chunks are joined in shared memory, or, when that leaves SMs idle, one chunk, whose state
-// combine_kernel joins; both give the same bits.
+// group, whose chunks are joined on chip, or, when that leaves SMs idle, one chunk, whose state
+// combine_kernel joins; both give the same bits.  The joined accumulators of head_dim 128 need 128 KB: three
+// quarters of them lie where half of the ring would be, the rest in TMEM's last free columns (512 rows of 32
+// heads behind 8191 tokens: 101 us against 120 with every chunk's state through memory), so that form
+// is one of its own, WHOLE, and a chunk a run keeps the long ring (32 rows behind 32768 tokens: 52 us; 57
+// with the short one).
 #pragma once
 
 #include "dk_common.cuh"
@@ -66,11 +70,11 @@ enum : int {
 __host__ __device__ constexpr int block_tokens(int head_dim) { return head_dim <= 64 ? 128 : 64; }
 
 // Chunks a group.
-__host__ __device__ constexpr int group_chunks(int head_dim) { return head_dim <= 64 ? 8 : 1; }
+__host__ __device__ constexpr int group_chunks(int head_dim) { return head_dim <= 64 ? 8 : 4; }
 
 // Tokens a chunk: a function of the prefix length and head_dim alone.  Short chunks give a small
-// batch enough items to fill the SMs; every chunk of a 128-wide head costs each row a 512-byte state
-// through memory, so those are longer.
+// batch enough items to fill the SMs; every chunk of a 128-wide head that is a run of its own costs each row a
+// 512-byte state through memory, so those are longer.
 __host__ __device__ inline int64_t chunk_tokens(int64_t prefix_len, int head_dim) {
   if (prefix_len <= 2048) return 512;
   if (head_dim <= 64) return 1024 * ((prefix_len + 32767) / 32768);
@@ -104,7 +108,7 @@ struct Maps {
   CUtensorMap k, v;       // boxes of 64 elements x 64 tokens
 };
 
-template <int D>
+template <int D, bool WHOLE>
 struct Cfg {
   static constexpr int DP = D < 64 ? 64 : D;      // columns in shared memory and TMEM (D = 32: zero filled)
   static constexpr int NH = DP / 64;              // 64-element halves
@@ -112,15 +116,16 @@ struct Cfg {
   static constexpr int BOX = 64 * 128;            // bytes of a 64-token box of 64 elements
   static constexpr int HALF = BLK / 64 * BOX;     // a block's 64-element half
   static constexpr int STAGE = NH * HALF;         // a K or V block
-  static constexpr int STAGES = 8;
+  static constexpr bool GROUPED = D <= 64 || WHOLE;
+  static constexpr int STAGES = D == 128 && WHOLE ? 4 : 8;
   static constexpr int QHALF = kRows * 128;       // bytes of a query tile's 64-element half
   static constexpr int QTILE = NH * QHALF;
-  static constexpr bool GROUPED = group_chunks(D) > 1;
-  static constexpr int RUN = GROUPED ? 2 * kRows * D * 4 : 0;   // joined chunks of both tiles [tile][D / 4][row][4]
+  static constexpr int RC = D == 128 ? 96 : D;    // columns of the joined chunks in shared memory; the rest in TMEM
+  static constexpr int RUN = GROUPED ? 2 * kRows * RC * 4 : 0;   // both tiles [tile][RC / 4][row][4]
   static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * QTILE + RUN + 512;
   // TMEM columns: scores, weights (16-bit pairs) and accumulator of tile t at X_COL + t * width
-  static constexpr uint32_t S_COL = 0, P_COL = 2 * BLK, O_COL = 512 - 2 * DP;
-  static_assert(P_COL + BLK <= O_COL, "TMEM");
+  static constexpr uint32_t S_COL = 0, P_COL = 2 * BLK, R_COL = P_COL + BLK, O_COL = 512 - 2 * DP;
+  static_assert(R_COL + 2 * (D - RC) <= O_COL, "TMEM");
 };
 
 // True for one lane of a converged warp.
@@ -233,9 +238,9 @@ __device__ __forceinline__ Item item_at(const Params& p, uint32_t w) {
   return it;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool WHOLE>
 __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_constant__ Maps maps, const Params p) {
-  using C = Cfg<D>;
+  using C = Cfg<D, WHOLE>;
   constexpr int BLK = C::BLK;
   constexpr uint32_t FMT = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   extern __shared__ uint8_t smem_raw[];
@@ -452,6 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
     const int r = threadIdx.x & 127;            // row of the tile
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t o_t = tmem + lane_base + C::O_COL + t * C::DP;
+    const uint32_t r_t = tmem + lane_base + C::R_COL + t * (D - C::RC);
     const uint32_t s_t = tmem + lane_base + C::S_COL + t * BLK, p_t = tmem + lane_base + C::P_COL + t * (BLK / 2);
     uint32_t sph = 0;                           // s_full parity
     uint32_t tph = t ^ 1;                       // turn parity (tile 0 goes first)
@@ -647,12 +653,36 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
             if (last && valid_row)
               *reinterpret_cast<float2*>(p.st_ml + 2 * (it.run * p.st_rows + n)) = make_float2(run_m, run_l);
             float4* dst = reinterpret_cast<float4*>(p.st_o) + static_cast<int64_t>(it.run) * (D / 4) * p.st_rows + n;
-            float4* run = s_run + t * (D / 4) * kRows + r;   // this row's joined chunks
+            float4* run = s_run + t * (C::RC / 4) * kRows + r;   // this row's joined chunks
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               float o[32];
               tmem_ld_32x32b_x32(o_t + c * 32, o);
               tmem_ld_wait();
+              if (C::GROUPED && c * 32 >= C::RC) {   // columns joined in TMEM
+                if (!head) {
+                  float u[32];
+                  tmem_ld_32x32b_x32(r_t, u);
+                  tmem_ld_wait();
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) o[i] = join(u[i], wa, o[i], wb);
+                }
+                if (!last) {
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    uint32_t w16[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) w16[i] = __float_as_uint(o[16 * h + i]);
+                    tmem_st_x16(r_t + 16 * h, w16);
+                  }
+                  tmem_st_wait();
+                } else if (valid_row) {
+#pragma unroll
+                  for (int i = 0; i < 8; ++i)
+                    dst[i * p.st_rows] = make_float4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
+                }
+                continue;
+              }
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 float4 v = make_float4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);

@@ -87,11 +87,16 @@ int rope_launch(dk::rope::Params& p, cudaStream_t st) {
 struct PrefixPlan {
   int64_t rg;           // rows * G
   int chunk_blocks, n_chunks, run_blocks, n_runs, n_pairs, per_group;
+  bool whole;           // a run is a whole group of chunks
   int max_splits, spu, upt, own_states;   // own tokens: splits a row, splits a unit, units a (tile, head), states a row
 };
 
-// Schedule (the bits are the same for every choice).  Prefix: a whole group of chunks a run when that
-// gives most SMs an item, else a chunk a run, whose states then travel through memory.  Own tokens: all
+// Schedule (the bits are the same for every choice).  Prefix: a whole group of chunks a run, or a chunk a
+// run, whose states then travel through memory, which costs about two fifths of a chunk's time; the fewer
+// units of a chunk's time, counting the waves of CTAs that either takes.  (Bf16, groups against chunks: 512
+// rows of 32 heads of 128 on 4, 8191 tokens: 90 against 112 us; 800 rows of 24 on 8, 5000 tokens: 139 against
+// 128; 2000 rows of 32 heads of 64 on 8, 2048 tokens: 114 against 138; 160 rows of 32 on 16, 8192: 119 against
+// 48.)  Own tokens: all
 // splits of a (tile, KV head) by one warp, which then also joins the prefix's states and writes the output,
 // when there are 12 such warps an SM (512 rows of 4 KV heads, 1 to 127 tokens: 125 us against 144 split up);
 // else enough units for three waves, and combine_kernel.
@@ -107,7 +112,9 @@ PrefixPlan plan_prefix(int64_t n_rows, int64_t n_tiles, int64_t hkv, int64_t G, 
   pl.n_pairs = static_cast<int>(ceil_div(pl.rg, 2 * dk::prefix::kRows));
   const int gc = dk::prefix::group_chunks(static_cast<int>(head_dim));
   const int64_t groups = ceil_div(pl.n_chunks, gc);
-  const bool whole = gc == 1 || 4 * groups * pl.n_pairs * hkv >= 3LL * sms;
+  const int64_t heads = pl.n_pairs * hkv;
+  const bool whole = pl.whole = pl.n_chunks > 1 && 5 * ceil_div(groups * heads, sms) * std::min(gc, pl.n_chunks) <=
+                                                       7 * ceil_div(pl.n_chunks * heads, sms);
   pl.run_blocks = pl.chunk_blocks * (whole ? gc : 1);
   pl.n_runs = static_cast<int>(whole ? groups : pl.n_chunks);
   pl.per_group = whole ? 1 : gc;
@@ -132,11 +139,11 @@ size_t prefix_state_bytes(const PrefixPlan& pl, int64_t st_rows, int64_t D) {
   return state_o_bytes(pl, st_rows, D) + static_cast<size_t>(pl.n_runs + pl.own_states) * st_rows * 2 * sizeof(float);
 }
 
-template <typename T, int D>
-int prefix_launch(const dk::prefix::Maps& maps, const dk::prefix::Params& p, cudaStream_t st) {
-  using C = dk::prefix::Cfg<D>;
+template <typename T, int D, bool WHOLE>
+int prefix_launch_as(const dk::prefix::Maps& maps, const dk::prefix::Params& p, cudaStream_t st) {
+  using C = dk::prefix::Cfg<D, WHOLE>;
   static bool done[kMaxDevices] = {false};
-  auto fn = dk::prefix::prefix_kernel<T, D>;
+  auto fn = dk::prefix::prefix_kernel<T, D, WHOLE>;
   int rc = ensure_smem(fn, C::SMEM, done);
   if (rc) return rc;
   static int regs[kMaxDevices] = {0};
@@ -156,6 +163,12 @@ int prefix_launch(const dk::prefix::Maps& maps, const dk::prefix::Params& p, cud
                              C::SMEM, st, maps, p);
   if (e != cudaSuccess) return fail(DK_ERR_CUDA, "attention_shared_prefix: launch failed: %s", cudaGetErrorString(e));
   return DK_OK;
+}
+
+template <typename T, int D>
+int prefix_launch(const dk::prefix::Maps& maps, const dk::prefix::Params& p, bool whole, cudaStream_t st) {
+  // up to head_dim 64 one form does both
+  return D <= 64 || whole ? prefix_launch_as<T, D, true>(maps, p, st) : prefix_launch_as<T, D, D <= 64>(maps, p, st);
 }
 
 // Follows prefix_launch on the same stream and starts without waiting for it: prefix_kernel has itself
@@ -455,7 +468,7 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
                     : (head_dim == 32   ? FN<__half, 32>(__VA_ARGS__)                          \
                        : head_dim == 64 ? FN<__half, 64>(__VA_ARGS__)                          \
                                         : FN<__half, 128>(__VA_ARGS__)))
-  rc = DK_DISPATCH_16(prefix_launch, maps, p, st);
+  rc = DK_DISPATCH_16(prefix_launch, maps, p, pl.whole, st);
   if (rc) return rc;
   if (own) {
     dk::own::Params o{};

@@ -230,7 +230,8 @@ def test_rows_that_no_tile_covers_are_left(dev, H, Hkv, D, n_seq):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("H,Hkv,D,P", [(8, 2, 64, 1500), (8, 8, 128, 700), (16, 2, 128, 5000), (4, 1, 32, 20000)])
+@pytest.mark.parametrize("H,Hkv,D,P", [(8, 2, 64, 1500), (8, 8, 128, 700), (16, 2, 128, 5000), (24, 8, 128, 5000),
+                                       (4, 1, 32, 20000)])
 def test_a_row_does_not_depend_on_its_batch(dev, H, Hkv, D, P):
     """The same rows alone, in small batches and in one that takes whole groups a run: the same bits."""
     import torch
@@ -244,6 +245,8 @@ def test_a_row_does_not_depend_on_its_batch(dev, H, Hkv, D, P):
         assert torch.equal(_call(q[lo:hi], part, lens[lo:hi]), full[lo:hi])
     again = _call(q, kw, lens)
     assert torch.equal(again, full)
+    some = [0, 399, 799]
+    _tol_check(full[some], q[some], kp, vp, [own[i][0] for i in some], [own[i][1] for i in some], D ** -0.5)
 
 
 @pytest.mark.gpu
