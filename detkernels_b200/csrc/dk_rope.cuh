@@ -6,8 +6,8 @@
 //
 // with pairs (i, i + rd / 2), or (2i, 2i + 1) when interleaved, and cos/sin of the row's position
 // from an f32 table.  Everything stays in f32 until the one rounding of the store.  The sum of
-// squares of a vector has a fixed order (a lane's elements in order, then a butterfly), so a row's
-// bits do not depend on the other rows.
+// squares of a vector has a fixed order (a lane's even and odd elements in order, then a butterfly), so a
+// row's bits do not depend on the other rows.
 //
 // Memory bound: every vector is read and written once.  A group of lanes owns a vector in 16-byte
 // chunks, lane l holding chunks l, l + L, l + 2L, ... with L = rd / 2 in chunks, so both elements of
@@ -176,16 +176,42 @@ __device__ __forceinline__ uint4 pack<__half>(const float* x) {
   return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
+// Two f32 operations an instruction, each rounded by itself.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
 // Vector path.  NC: chunks a lane holds (chunk l + j L, j < NC).  Rotated chunks: 0 and 1 (pairs
 // between them) or, interleaved, those with index < rd / N (pairs inside a chunk).
 //
 // Warps walk units (a row, or part of one when rows are few) grid-stride, the next unit's position and
 // slot in flight while one is rotated.  The weights stay in shared memory as f32 and the angles are read
-// back from the cache a batch at a time, as 16-byte vectors: the loop is bound by the instructions it
-// issues before the bytes it moves, so that the 66,377-row prefill of 32 vectors of 64 a row (floor 86 us) took
+// back from the cache a batch at a time, as 16-byte vectors: the loop is bound by its loads'
+// latency at the registers it leaves, so that the 66,377-row prefill of 32 vectors of 64 a row (floor 86 us) took
 // 161 us with both in registers through a type switch, 123 us with four vectors a lane in flight and
 // the spills of that, and takes 113 us with two.  One resident set of 3 CTAs an SM walks all units;
-// one CTA per 8 units took 15 % more.
+// one CTA per 8 units took 15 % more.  Half the arithmetic's instructions (f32x2) left the prefill as it was and took
+// small batches from 4.0 to 3.2 us; fetching the next unit's vectors ahead cost more registers than it hid (142 us).
 template <typename T, int NC, bool INTER>
 __global__ void __launch_bounds__(kThreads, 3) vec_kernel(const Params p) {
   constexpr int N = Chunk<T>::N;
@@ -242,10 +268,11 @@ __global__ void __launch_bounds__(kThreads, 3) vec_kernel(const Params p) {
       }
       // this lane's angles: pairs of chunk 0 with chunk 1 share index i in [l N, l N + N); interleaved,
       // chunk j's pairs are i = (l + j L) N / 2 + [0, N / 2)  (re-read a batch from the cache: no registers held)
-      float co[NA], si[NA];
+      F2 co[NA / 2], si[NA / 2], ns[NA / 2];   // ns: -sin
       if (on) {
         const float* cs = p.table + now.pos * p.rd;
         if constexpr (INTER) {
+          // pair (a, b) -> (a, b) (cos, cos) + (b, a) (-sin, sin): both factors of two elements in one register pair
 #pragma unroll
           for (int j = 0; j < NC; ++j) {
             const int at = (l + j * p.lanes) * (N / 2);
@@ -254,10 +281,8 @@ __global__ void __launch_bounds__(kThreads, 3) vec_kernel(const Params p) {
             for (int i = 0; i < N / 2; i += 2) {
               const float2 a = rot ? __ldg(reinterpret_cast<const float2*>(cs + at + i)) : make_float2(1.0f, 1.0f);
               const float2 b = rot ? __ldg(reinterpret_cast<const float2*>(cs + half + at + i)) : make_float2(0.0f, 0.0f);
-              co[j * (N / 2) + i] = a.x;
-              co[j * (N / 2) + i + 1] = a.y;
-              si[j * (N / 2) + i] = b.x;
-              si[j * (N / 2) + i + 1] = b.y;
+              co[(j * (N / 2) + i) / 2] = f2(a.x, a.y);
+              si[(j * (N / 2) + i) / 2] = f2(b.x, b.y);
             }
           }
         } else {
@@ -265,8 +290,9 @@ __global__ void __launch_bounds__(kThreads, 3) vec_kernel(const Params p) {
           for (int i = 0; i < N; i += 4) {
             const float4 a = __ldg(reinterpret_cast<const float4*>(cs + l * N + i));
             const float4 b = __ldg(reinterpret_cast<const float4*>(cs + half + l * N + i));
-            co[i] = a.x, co[i + 1] = a.y, co[i + 2] = a.z, co[i + 3] = a.w;
-            si[i] = b.x, si[i + 1] = b.y, si[i + 2] = b.z, si[i + 3] = b.w;
+            co[i / 2] = f2(a.x, a.y), co[i / 2 + 1] = f2(a.z, a.w);
+            si[i / 2] = f2(b.x, b.y), si[i / 2 + 1] = f2(b.z, b.w);
+            ns[i / 2] = f2(-b.x, -b.y), ns[i / 2 + 1] = f2(-b.z, -b.w);
           }
         }
       }
@@ -275,50 +301,65 @@ __global__ void __launch_bounds__(kThreads, 3) vec_kernel(const Params p) {
         // every lane of the warp takes part in the shuffles
         const int i = i0 + gi + u * gpw;
         const bool live = on && i < end && i < p.H + p.Hkv;
-        float x[NC][N];
+        F2 x[NC][N / 2];
         float ss = 0.0f;
         if (live) {
+          F2 sum = f2(0.0f, 0.0f);
 #pragma unroll
           for (int j = 0; j < NC; ++j) {
-            unpack<T>(c[u][j], x[j]);
+            float f[N];
+            unpack<T>(c[u][j], f);
 #pragma unroll
-            for (int e = 0; e < N; ++e) ss = __fmaf_rn(x[j][e], x[j][e], ss);
+            for (int e = 0; e < N / 2; ++e) {
+              x[j][e] = f2(f[2 * e], f[2 * e + 1]);
+              sum = fma2(x[j][e], x[j][e], sum);
+            }
           }
+          const float2 parts = unpair(sum);
+          ss = __fadd_rn(parts.x, parts.y);
         }
         for (int d = gl >> 1; d > 0; d >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, d));
         if (live) {
           const float rs = rsqrtf(__fmaf_rn(ss, p.inv_d, p.eps));
+          const F2 rs2 = f2(rs, rs);
           const float* w = s_w[i >= p.H] + l * N;
 #pragma unroll
           for (int j = 0; j < NC; ++j)
 #pragma unroll
             for (int e = 0; e < N; e += 4) {
               const float4 f = *reinterpret_cast<const float4*>(w + j * cstep + e);
-              x[j][e] = __fmul_rn(__fmul_rn(x[j][e], rs), f.x);
-              x[j][e + 1] = __fmul_rn(__fmul_rn(x[j][e + 1], rs), f.y);
-              x[j][e + 2] = __fmul_rn(__fmul_rn(x[j][e + 2], rs), f.z);
-              x[j][e + 3] = __fmul_rn(__fmul_rn(x[j][e + 3], rs), f.w);
+              x[j][e / 2] = mul2(mul2(x[j][e / 2], rs2), f2(f.x, f.y));
+              x[j][e / 2 + 1] = mul2(mul2(x[j][e / 2 + 1], rs2), f2(f.z, f.w));
             }
           if constexpr (INTER) {
 #pragma unroll
             for (int j = 0; j < NC; ++j)
 #pragma unroll
               for (int e = 0; e < N / 2; ++e) {
-                const float a = x[j][2 * e], b = x[j][2 * e + 1];
-                const float cc = co[j * (N / 2) + e], sn = si[j * (N / 2) + e];
-                x[j][2 * e] = __fmaf_rn(a, cc, -__fmul_rn(b, sn));
-                x[j][2 * e + 1] = __fmaf_rn(a, sn, __fmul_rn(b, cc));
+                const float2 y = unpair(x[j][e]);
+                const float2 c2 = unpair(co[(j * (N / 2) + e) / 2]), s2 = unpair(si[(j * (N / 2) + e) / 2]);
+                const float cc = (e & 1) ? c2.y : c2.x, sn = (e & 1) ? s2.y : s2.x;
+                x[j][e] = fma2(x[j][e], f2(cc, cc), mul2(f2(y.y, y.x), f2(-sn, sn)));
               }
           } else {
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-              const float a = x[0][e], b = x[1][e];
-              x[0][e] = __fmaf_rn(a, co[e], -__fmul_rn(b, si[e]));
-              x[1][e] = __fmaf_rn(a, si[e], __fmul_rn(b, co[e]));
+            for (int e = 0; e < N / 2; ++e) {
+              const F2 a = x[0][e], b = x[1][e];
+              x[0][e] = fma2(a, co[e], mul2(b, ns[e]));
+              x[1][e] = fma2(a, si[e], mul2(b, co[e]));
             }
           }
 #pragma unroll
-          for (int j = 0; j < NC; ++j) c[u][j] = pack<T>(x[j]);
+          for (int j = 0; j < NC; ++j) {
+            float f[N];
+#pragma unroll
+            for (int e = 0; e < N / 2; ++e) {
+              const float2 y = unpair(x[j][e]);
+              f[2 * e] = y.x;
+              f[2 * e + 1] = y.y;
+            }
+            c[u][j] = pack<T>(f);
+          }
         }
         if (on && i < end) {
           const int h = i < p.H ? i : (i < p.H + p.Hkv ? i - p.H : i - p.H - p.Hkv);
