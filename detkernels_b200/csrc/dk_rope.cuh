@@ -11,7 +11,7 @@
 //
 // Memory bound: every vector is read and written once.  A group of lanes owns a vector in 16-byte
 // chunks, lane l holding chunks l, l + L, l + 2L, ... with L = rd / 2 in chunks, so both elements of
-// a pair sit in one lane; the row's cos/sin stay in registers over the vectors a group walks.
+// a pair sit in one lane.
 #pragma once
 
 #include "dk_common.cuh"
@@ -206,12 +206,12 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
 //
 // Warps walk units (a row, or part of one when rows are few) grid-stride, the next unit's position and
 // slot in flight while one is rotated.  The weights stay in shared memory as f32 and the angles are read
-// back from the cache a batch at a time, as 16-byte vectors: the loop is bound by its loads'
-// latency at the registers it leaves, so that the 66,377-row prefill of 32 vectors of 64 a row (floor 86 us) took
-// 161 us with both in registers through a type switch, 123 us with four vectors a lane in flight and
-// the spills of that, and takes 113 us with two.  One resident set of 3 CTAs an SM walks all units;
-// one CTA per 8 units took 15 % more.  Half the arithmetic's instructions (f32x2) left the prefill as it was and took
-// small batches from 4.0 to 3.2 us; fetching the next unit's vectors ahead cost more registers than it hid (142 us).
+// back from the cache a batch at a time, as 16-byte vectors.  Bound by the latency of its loads at the registers
+// they leave: the 66,377-row prefill of 32 vectors of 64 a row (floor 86 us) took 161 us with both in registers
+// through a type switch, 123 us with four vectors a lane in flight and the spills of that, and takes 113 us
+// (5.0 TB/s) with two.  One resident set of 3 CTAs an SM walks all units; one CTA per 8 units took 15 % more.
+// Half the arithmetic's instructions (f32x2) left the prefill as it was and took small batches from 4.0 to 3.2 us;
+// fetching the next unit's vectors ahead cost more registers than it hid (142 us).
 template <typename T, int NC, bool INTER>
 __global__ void __launch_bounds__(kThreads, 3) vec_kernel(const Params p) {
   constexpr int N = Chunk<T>::N;
