@@ -208,6 +208,16 @@ __device__ __forceinline__ uint4 times_zero(uint4 v) {
   return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
+// An arrival of the lanes with `yes`, without a branch that would part them from the warp.
+__device__ __forceinline__ void arrive_if(uint64_t* bar, bool yes) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(yes ? 1 : 0)
+      : "memory");
+}
+
 // x / G for x < 2^31, G <= 16 (the excess of the rounded-up reciprocal stays below 1 / G).
 __device__ __forceinline__ uint32_t div_g(uint32_t x, uint64_t magic) {
   return static_cast<uint32_t>((x * magic) >> 36);
@@ -607,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
 #pragma unroll
           for (int c = 0; c < NR; ++c) {
             uint32_t pk[16];
-            if (c == NR / 2 && it.tiles == 2 && lane == 0) mbar_arrive(&turn[warp ^ 4]);
+            if (c == NR / 2) arrive_if(&turn[warp ^ 4], it.tiles == 2 && lane == 0);
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               float2 e = fma2(make_float2(s[c][i], s[c][i + 1]), c2, n2);
