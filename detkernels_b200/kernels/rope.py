@@ -58,7 +58,7 @@ def qk_norm_rope(q, k, positions, q_weight, k_weight, table, eps: float = 1e-6, 
     and slots (int64 CUDA [T], slab * capacity + token, e.g. ``paged_plan(...).slots``), the key and the
     value of each row are stored at its slot; a negative slot stores nothing.  k_out is then only written
     if given.  A position outside the table or a slot outside the cache sets the device status, and that
-    row (or its K and V) is not written.
+    row (or its K and V) is not written.  Rows of one call must not share a slot.
 
     Returns (q_out, k_out); k_out is None when the keys went to the cache only."""
     import torch

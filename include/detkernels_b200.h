@@ -367,7 +367,7 @@ int dk_paged_plan(int32_t* block_table, int64_t block_table_stride, int32_t bloc
  * cache_capacity, head_dim] (slab = sequence or block), slots (device int64[n_rows]) and v, the rotated
  * key and the value of row r go to slab slots[r] / cache_capacity, token slots[r] % cache_capacity; a
  * negative slot stores nothing, one beyond the cache is recorded (DK_ERR_DEVICE_CHECK, detail 0x611) and
- * stores nothing.  k_out may be NULL with a cache.  A position outside the table is recorded (0x610) and
+ * stores nothing; rows must not share a slot.  k_out may be NULL with a cache.  A position outside the table is recorded (0x610) and
  * its row not written.  head_dim <= 512; any dtype of the three for q/k/v/caches, and for the weights
  * [head_dim].  16-byte aligned vectors take the vector path. */
 int dk_qk_norm_rope(const void* q, int64_t q_stride_row, int64_t q_stride_head, const void* k, int64_t k_stride_row,
