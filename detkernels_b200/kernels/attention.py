@@ -252,7 +252,8 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
     block pools [n_blocks, H_kv, page, D] (page a multiple of 64) whose block prefix_blocks[t // page]
     holds prefix token t.  prefix_len defaults to all of it; 0 is plain ``attention_decode``.
     k_cache, v_cache, kv_lens, block_table, max_kv_len: as in ``attention_decode`` (kv_lens and
-    max_kv_len count the rows' own tokens only).  bf16 or f16; head_dim 32, 64 or 128; at most 16 query
+    max_kv_len count the rows' own tokens only; the workspace of a small batch grows with max_kv_len, so
+    give it where the cache is much longer than the rows).  bf16 or f16; head_dim 32, 64 or 128; at most 16 query
     heads per KV head.  workspace: uint8 CUDA tensor of at least
     ``dk_attention_shared_prefix_workspace_size`` bytes (a new one if not given; its contents do not
     matter, and calls that may overlap need separate ones).
@@ -296,7 +297,8 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
         assert block_table.shape[1] <= 1 or block_table.stride(1) == 1
         n_blocks, page = n_seq, cap
         n_seq, width = block_table.shape
-        cap, bt_stride = width * page, max(block_table.stride(0), width)
+        # a single row has any stride; the rows of a larger table must not overlap (the C entry refuses them)
+        cap, bt_stride = width * page, block_table.stride(0) if n_seq > 1 else width
     if max_kv_len is None:
         max_kv_len = kv_lens if uniform else cap
     max_kv_len = int(max_kv_len)

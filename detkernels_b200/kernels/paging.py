@@ -124,7 +124,7 @@ def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=No
             return None if t is None else (t.data_ptr() or ws_ptr)
 
         rc = lib.dk_paged_plan(
-            block_table.data_ptr(), max(stride[0], shape[1]), shape[1], kv_lens.data_ptr(), new_lens.data_ptr(), B,
+            block_table.data_ptr(), stride[0] if shape[0] > 1 else shape[1], shape[1], kv_lens.data_ptr(), new_lens.data_ptr(), B,
             int(page_size), ptr(free_blocks), 0 if free_blocks is None else free_blocks.numel(), ptr(cursor), ptr(cur),
             cu.data_ptr(), ptr(row_seq), ptr(row_pos), ptr(slots), ptr(q_lens), n_rows or 0, ptr(tiles),
             int(rows_per_tile), n_tiles or 0, ws_ptr, 4 * ws.numel(), _lib.stream_ptr(dev))

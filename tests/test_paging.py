@@ -189,3 +189,25 @@ def test_equals_the_host_allocator(dev):
     paged_plan(table, _i32(np.zeros(40), dev), _i32(tokens, dev), 64, free_blocks=_i32(al.order, dev),
                cursor=_i32([0], dev))
     assert np.array_equal(table.cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+def test_rows_of_a_table_that_overlap_are_refused(dev):
+    """An expanded table has one row in memory: no call may take it for B."""
+    import torch
+
+    from detkernels_b200.kernels.attention import attention_shared_prefix
+    from detkernels_b200.kernels.paging import paged_plan
+    one = torch.zeros(1, 4, dtype=torch.int32, device=dev)
+    ln = torch.ones(3, dtype=torch.int32, device=dev)
+    with pytest.raises(ValueError):
+        paged_plan(one.expand(3, 4), ln, ln, 64, n_rows=3)
+    q = torch.zeros(3, 2, 64, device=dev, dtype=torch.bfloat16)
+    pool = torch.zeros(2, 2, 64, 64, device=dev, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        attention_shared_prefix(q, pool[0], pool[0], pool, pool, ln, block_table=one.expand(3, 4))
+    # one row of a wider table, and a single sequence, are fine with any stride
+    wide = torch.zeros(3, 8, dtype=torch.int32, device=dev)
+    plan = paged_plan(wide[:, :4], ln, ln, 64, n_rows=3)
+    assert plan.slots.tolist() == [1, 1, 1]
+    assert paged_plan(one, ln[:1], ln[:1], 64, n_rows=1).slots.tolist() == [1]
