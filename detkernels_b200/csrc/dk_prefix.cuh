@@ -76,7 +76,8 @@ __host__ __device__ constexpr int group_chunks(int head_dim) { return head_dim <
 // batch enough items to fill the SMs; every chunk of a 128-wide head that is a run of its own costs each row a
 // 512-byte state through memory, so those are longer.  Measured: 1500 to 2048 tokens in chunks of 512 and 1024, 4
 // rows of 8 heads of 64: 12 and 16 us, 64 rows of 16: 15 and 18, 1000 rows of 16: 51 and 45; 8191 tokens in chunks of
-// 512, 1024 and 2048, heads of 128, 4 rows: 21, 24 and 36 us, 128 rows: 47, 39 and 52.
+// 512, 1024 and 2048, heads of 128, 4 rows: 21, 24 and 36 us, 128 rows: 47, 39 and 52; 32768 tokens in 16, 24 and 36
+// chunks, 32 rows of 32 heads of 128 on 8: 51, 64 and 59 (128, 192 and 288 items for 148 SMs), on 4: 50, 46 and 47.
 __host__ __device__ inline int64_t chunk_tokens(int64_t prefix_len, int head_dim) {
   if (prefix_len <= 2048) return 512;
   if (head_dim <= 64) return 1024 * ((prefix_len + 32767) / 32768);
