@@ -478,10 +478,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
     uint32_t oseen = 0;                         // of them, those whose P.V this warp has waited for
     // All P.V so far are done.  Each warp takes every phase of o_full once and in order: a block's weights
     // go out only after the previous P.V has been seen, so the barrier is never two phases ahead, where its
-    // parity would say nothing.
+    // parity would say nothing.  The fence orders what the warp does to TMEM next (the weights it overwrites
+    // are the left operand that P.V has read) behind that completion.
     auto pv_done = [&]() {
       if (oseen == ocnt) return true;
       const bool ok = warp_wait(&o_full[t], oseen & 1, kDetOut, abort_flag);
+      tc_fence_after();
       oseen = ocnt;
       return ok;
     };
@@ -593,7 +595,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
           if (!first && __any_sync(0xffffffffu, alpha != 1.0f)) {
             // rescale the accumulator once the previous block's P.V is done
             if (!pv_done()) break;
-            tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < C::DP / 16; ++c) {
               uint32_t o[16];
@@ -650,7 +651,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
         if (in_chunk == 0 || last) {
           // the chunk's state joins the run's, which leaves with the last chunk
           if (!pv_done()) break;
-          tc_fence_after();
           if (warp_live) {
             const bool head = b < p.chunk_blocks;   // the run's first chunk
             float wa = 0.0f, wb = 1.0f;
