@@ -286,7 +286,8 @@ __device__ __forceinline__ int describe_item(const Params& p, int64_t w, Item& i
   it.nsplits = 0;
   it.s_begin = it.s_end = 0;
   const int rows_per_tile_max = kRows / p.G;
-  if (it.nr < 1 || it.nr > rows_per_tile_max || it.r0 < 0 || it.r0 + it.nr > p.n_rows || it.seq < 0 ||
+  // r0 against n_rows - nr: r0 + nr may leave 32 bits
+  if (it.nr < 1 || it.nr > rows_per_tile_max || it.r0 < 0 || it.r0 > p.n_rows - it.nr || it.seq < 0 ||
       it.seq >= p.kv_n_seq || it.nr * p.G > p.rows_cap)
     return 2;
   for (int i = 0; i < it.nr; ++i) {
