@@ -16,6 +16,7 @@
 #pragma once
 
 #include "dk_common.cuh"
+#include "dk_divide.cuh"
 
 namespace dk {
 namespace paging {
@@ -30,27 +31,6 @@ enum : int {
   kDetPool = 0x601,   // the free list is exhausted
   kDetRows = 0x602,   // more rows or tiles than the outputs hold
 };
-
-// Division of any 32-bit n by a number that the host knows, after Granlund and Montgomery ("Division by
-// invariant integers using multiplication"): with l = ceil(log2 d) and m = floor(2^32 (2^l - d) / d) + 1,
-// n / d = (t + ((n - t) >> 1)) >> (l - 1), t the high half of m n; d = 1 is n itself.
-struct Divisor {
-  uint32_t d, m, sh1, sh2;
-};
-inline Divisor divisor(uint32_t d) {
-  uint32_t l = 0;
-  while ((1ull << l) < d) ++l;
-  const uint64_t m = ((((1ull << l) - d) << 32) / d) + 1;
-  return Divisor{d, static_cast<uint32_t>(m), l < 1 ? l : 1, l > 1 ? l - 1 : 0};
-}
-__device__ __forceinline__ uint32_t div_by(uint32_t n, const Divisor& v) {
-  const uint32_t t = __umulhi(v.m, n);
-  return (t + ((n - t) >> v.sh1)) >> v.sh2;
-}
-__device__ __forceinline__ uint32_t ceil_div32(uint32_t a, const Divisor& v) {
-  const uint32_t q = div_by(a, v);
-  return q + (a != q * v.d);
-}
 
 struct Params {
   int32_t* table;

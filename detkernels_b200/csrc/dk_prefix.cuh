@@ -32,6 +32,7 @@
 #pragma once
 
 #include "dk_common.cuh"
+#include "dk_divide.cuh"
 #include "dk_own.cuh"
 
 namespace dk {
@@ -90,7 +91,7 @@ struct Params {
   int64_t q_sr, q_sh;
   int32_t hq, hkv, G;
   int32_t rg;             // rows * G
-  uint64_t g_magic;       // ceil(2^36 / G)
+  Divisor31 group;        // by G
   int32_t prefix_len;
   int32_t chunk_blocks;   // blocks a chunk
   int32_t run_blocks;     // blocks a run: a chunk or a group
@@ -219,11 +220,6 @@ __device__ __forceinline__ void arrive_if(uint64_t* bar, bool yes) {
       "@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(smem_u32(bar)),
       "r"(yes ? 1 : 0)
       : "memory");
-}
-
-// x / G for x < 2^31, G <= 16 (the excess of the rounded-up reciprocal stays below 1 / G).
-__device__ __forceinline__ uint32_t div_g(uint32_t x, uint64_t magic) {
-  return static_cast<uint32_t>((x * magic) >> 36);
 }
 
 // Bounded wait by a whole warp, with one answer for all of its lanes.
@@ -502,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
         const int e = i * 128 + tt, c = e % CPR;
         const uint32_t mrow = (it.pair * 2 + t) * kRows + e / CPR;
         const bool valid = mrow < static_cast<uint32_t>(p.rg) && c < D / 8;
-        const uint32_t row = valid ? div_g(mrow, p.g_magic) : 0, gh = valid ? mrow - row * p.G : 0;
+        const uint32_t row = valid ? div_by(mrow, p.group) : 0, gh = valid ? mrow - row * p.G : 0;
         own::cp_async16(smem_u32(q_at(i)), static_cast<const T*>(p.q) + row * p.q_sr + (it.kvh * p.G + gh) * p.q_sh +
                                                (valid ? c * 8 : 0), valid);
       }
@@ -743,7 +739,7 @@ struct CombineParams {
   int32_t n_tiles, n_rows, n_seq;
   int64_t st_rows, rg;      // hkv * rows * G, rows * G
   int G;
-  uint64_t g_magic;         // ceil(2^36 / G)
+  Divisor31 group;          // by G
   void* out;
   int64_t o_sr, o_sh;
 };
@@ -789,14 +785,14 @@ __global__ void __launch_bounds__(CombineCfg<D, Q>::WARPS * 32) combine_kernel(c
   int n_own = 0;
   if (live && p.kv_lens) {
     const uint32_t mrow = static_cast<uint32_t>(n) % rg;
-    n_own = min(max((p.kv_lens[div_g(mrow, p.g_magic)] + own::kSplit - 1) / own::kSplit, 0), p.own_max);
+    n_own = min(max((p.kv_lens[div_by(mrow, p.group)] + own::kSplit - 1) / own::kSplit, 0), p.own_max);
   }
   const int total = runs + n_own;
   fetch(0, 0, runs, total);
   if (p.tiles) {
     // a row that no tile covers has no own states and keeps what `out` holds
     __syncthreads();
-    const int row = live ? static_cast<int>(div_g(static_cast<uint32_t>(n) % rg, p.g_magic)) : -1;
+    const int row = live ? static_cast<int>(div_by(static_cast<uint32_t>(n) % rg, p.group)) : -1;
     const int low = __reduce_min_sync(0xffffffffu, live ? row : p.n_rows), high = __reduce_max_sync(0xffffffffu, row);
     bool covered = false;
     for (int t0 = warp * 32; t0 < p.n_tiles; t0 += C::WARPS * 32) {
@@ -874,7 +870,7 @@ __global__ void __launch_bounds__(CombineCfg<D, Q>::WARPS * 32) combine_kernel(c
   for (int k = warp; k < 32; k += C::WARPS) {
     const uint32_t nk = blockIdx.x * 32u + k;
     if (nk < p.st_rows && (s_covered >> k & 1u)) {
-      const uint32_t kh = nk / rg, mk = nk - kh * rg, rk = div_g(mk, p.g_magic);
+      const uint32_t kh = nk / rg, mk = nk - kh * rg, rk = div_by(mk, p.group);
       T* dst = out + rk * p.o_sr + (kh * p.G + mk - rk * p.G) * p.o_sh;
 #pragma unroll
       for (int d = 0; d < C::COLS; d += 32) dst[d] = s_out[k][lane + d];

@@ -259,7 +259,7 @@ int dk_paged_plan(int32_t* block_table, int64_t block_table_stride, int32_t bloc
   p.kv = kv_lens;
   p.nw = new_lens;
   p.n_seqs = n_seqs;
-  p.page = dk::paging::divisor(page_size);
+  p.page = dk::divisor(page_size);
   p.free_list = free_blocks;
   p.n_free = n_free;
   p.cursor_in = cursor;
@@ -272,7 +272,7 @@ int dk_paged_plan(int32_t* block_table, int64_t block_table_stride, int32_t bloc
   p.n_rows = n_rows;
   p.tiles = row_tiles;
   p.tiled = row_tiles != nullptr;
-  p.rpt = dk::paging::divisor(row_tiles ? rows_per_tile : 1);
+  p.rpt = dk::divisor(row_tiles ? rows_per_tile : 1);
   p.n_tiles = n_tiles;
   p.ws = static_cast<int32_t*>(workspace);
   p.vec = aligned16(row_seq) && aligned16(row_pos) && aligned16(slots) && aligned16(q_lens);
@@ -433,7 +433,7 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
   p.hq = n_q_heads;
   p.hkv = n_kv_heads;
   p.G = G;
-  p.g_magic = ((1ull << 36) + G - 1) / G;
+  p.group = dk::divisor31(G);
   p.rg = static_cast<int32_t>(pl.rg);
   p.prefix_len = prefix_len;
   p.chunk_blocks = pl.chunk_blocks;
@@ -535,7 +535,7 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
   c.st_rows = st_rows;
   c.rg = pl.rg;
   c.G = G;
-  c.g_magic = p.g_magic;
+  c.group = p.group;
   c.out = out;
   c.o_sr = out_stride_row;
   c.o_sh = out_stride_head;

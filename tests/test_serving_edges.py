@@ -35,3 +35,66 @@ def test_a_tile_outside_the_batch_is_reported_and_skipped(dev, prefix, tile):
     assert _lib.device_status(dev.index) == (_lib.DK_ERR_DEVICE_CHECK, 0x211)
     want = attention_shared_prefix(q, kp, vp, k, v, ln, prefix_len=prefix, row_tiles=_i32([(2, 2, 1)], dev))
     assert torch.equal(out[2:], want[2:]) and (out[:2] == 7.0).all()
+
+
+def test_divisions_are_exact_over_all_32_bits(tmp_path):
+    """The kernels' division by the heads a group, the page size and the tile rows, compiled for the host: around
+    multiples near every power of two (2^28 rows and up among them) and at the ends."""
+    import os
+    import subprocess
+    src = tmp_path / "divide.cpp"
+    src.write_text(r"""
+#include <initializer_list>
+#include <stdio.h>
+#include "dk_divide.cuh"
+int main() {
+  const uint32_t odd[] = {24, 64, 96, 127, 128, 1000, 4097, 65535, 65536, 65537, 1u << 28, (1u << 31) - 1, 1u << 31, 0xffffffffu};
+  unsigned long long bad = 0, n = 0;
+  for (uint32_t i = 1; i <= 16 + sizeof(odd) / sizeof(odd[0]); ++i) {
+    const uint32_t d = i <= 16 ? i : odd[i - 17];
+    const dk::Divisor v = dk::divisor(d);
+    const dk::Divisor31 w = dk::divisor31(d);
+    for (int e = 0; e < 32; ++e)
+      for (uint32_t k = 0; k < 64; ++k)
+        for (int s = -1; s <= 1; ++s) {
+          const uint32_t near = ((1u << e) / d + k) * d + s, at = (1u << e) + k + s, end = 0xffffffffu - k;
+          bad += dk::div_by(near, v) != near / d;
+          bad += dk::div_by(at, v) != at / d;
+          bad += dk::div_by(end, v) != end / d;
+          for (uint32_t x : {near & 0x7fffffffu, at & 0x7fffffffu, end & 0x7fffffffu}) bad += dk::div_by(x, w) != x / d;
+          bad += dk::ceil_div32(at, v) != at / d + (at % d != 0);
+          n += 7;
+        }
+  }
+  printf("%llu wrong of %llu\n", bad, n);
+  return bad != 0;
+}
+""")
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "detkernels_b200", "csrc")
+    exe = tmp_path / "divide"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-I", csrc, "-o", str(exe), str(src)], check=True)
+    res = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert res.returncode == 0, res.stdout
+
+
+@pytest.mark.gpu
+def test_more_than_2_to_28_rows(dev):
+    """One narrow head of 2^28 + 300 rows (17 GB of queries): each row is its own, bit for bit that of a small call."""
+    import torch
+
+    from detkernels_b200.kernels.attention import attention_shared_prefix
+    if torch.cuda.mem_get_info(dev)[0] < 100 << 30:
+        pytest.skip("needs 100 GB of free device memory")
+    R = 2 ** 28 + 300
+    g = torch.Generator(device=dev).manual_seed(3)
+    kp, vp = (torch.randn(1, 70, 32, device=dev, generator=g).to(torch.bfloat16) for _ in range(2))
+    some = torch.tensor([0, 1, 255, 2 ** 27, 2 ** 28 - 1, 2 ** 28, 2 ** 28 + 1, 2 ** 28 + 44, R - 1], device=dev)
+    q = torch.zeros(R, 1, 32, dtype=torch.bfloat16, device=dev)
+    q[some] = torch.randn(len(some), 1, 32, device=dev, generator=g).to(torch.bfloat16)
+    k = torch.zeros(1, 1, 64, 32, dtype=torch.bfloat16, device=dev)
+    out = attention_shared_prefix(q, kp, vp, k, k, 0)
+    assert torch.equal(out[some], attention_shared_prefix(q[some], kp, vp, k, k, 0))
+    flat = attention_shared_prefix(q[2:3], kp, vp, k, k, 0)
+    assert torch.equal(out[2], flat[0]) and torch.equal(out[2 ** 28 + 2], flat[0])
+    del q, out
+    torch.cuda.empty_cache()
