@@ -333,14 +333,18 @@ __global__ void __launch_bounds__(kThreads, 3) vec_kernel(const Params p) {
             }
           if constexpr (INTER) {
 #pragma unroll
-            for (int j = 0; j < NC; ++j)
+            for (int j = 0; j < NC; ++j) {
+              // a chunk that is not rotated keeps its values as they are: times (1, 0) a NaN would reach its neighbour
+              const bool rot = (l + j * p.lanes) * (N / 2) < half;
 #pragma unroll
               for (int e = 0; e < N / 2; ++e) {
                 const float2 y = unpair(x[j][e]);
                 const float2 c2 = unpair(co[(j * (N / 2) + e) / 2]), s2 = unpair(si[(j * (N / 2) + e) / 2]);
                 const float cc = (e & 1) ? c2.y : c2.x, sn = (e & 1) ? s2.y : s2.x;
-                x[j][e] = fma2(x[j][e], f2(cc, cc), mul2(f2(y.y, y.x), f2(-sn, sn)));
+                const F2 turned = fma2(x[j][e], f2(cc, cc), mul2(f2(y.y, y.x), f2(-sn, sn)));
+                if (rot) x[j][e] = turned;
               }
+            }
           } else {
 #pragma unroll
             for (int e = 0; e < N / 2; ++e) {

@@ -98,3 +98,33 @@ def test_more_than_2_to_28_rows(dev):
     assert torch.equal(out[2], flat[0]) and torch.equal(out[2 ** 28 + 2], flat[0])
     del q, out
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D,rd,inter", [(96, 48, True), (64, 32, True), (128, 128, True), (128, 64, False), (50, 20, True)])
+def test_an_infinite_element_reaches_only_its_own_pair(dev, dt, D, rd, inter):
+    """1 / root is 0 then: by the definition the element itself (and, if rotated, its partner) is NaN, everything else
+    a zero, which behind the rotated part has the sign of its element times its weight."""
+    import torch
+
+    from detkernels_b200.kernels.rope import qk_norm_rope, rope_table
+    t = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}[dt]
+    g = torch.Generator(device=dev).manual_seed(D)
+    T = D
+    q = torch.randn(T, 2, D, device=dev, generator=g).to(t)
+    k = torch.randn(T, 1, D, device=dev, generator=g).to(t)
+    q[torch.arange(T), 0, torch.arange(T)] = float("inf")      # row i: element i of head 0
+    w = torch.randn(D, device=dev, generator=g).to(t)
+    pos = torch.arange(1, T + 1, device=dev)
+    qo, _ = qk_norm_rope(q, k, pos, w, w, rope_table(T + 2, rd, device=dev), interleaved=inter)
+    want = torch.zeros(T, D, dtype=torch.bool, device=dev)
+    for i in range(T):
+        want[i, i] = True
+        if i < rd:
+            want[i, i ^ 1 if inter else (i + rd // 2) % rd] = True
+    assert torch.equal(torch.isnan(qo[:, 0]), want)
+    assert torch.isfinite(qo[:, 1]).all() and (qo[:, 0][~want] == 0).all()
+    rest = ~want[:, rd:]
+    sign = torch.signbit(q[:, 0, rd:]) ^ torch.signbit(w[rd:])
+    assert torch.equal(torch.signbit(qo[:, 0, rd:])[rest], sign[rest])
