@@ -734,7 +734,7 @@ struct CombineParams {
   const float* st_ml;       // [states][st_rows][2]
   int n_runs, per_group;
   const int32_t* kv_lens;   // null: no row has tokens of its own
-  int own_max;              // the most states a row's own tokens have
+  int own_max;              // the longest length a row may have
   const int32_t* tiles;     // the row tiles, null: every row is its own
   int32_t n_tiles, n_rows, n_seq;
   int64_t st_rows, rg;      // hkv * rows * G, rows * G
@@ -756,8 +756,8 @@ template <typename T, int D, int Q, int UN>
 __global__ void __launch_bounds__(CombineCfg<D, Q>::WARPS * 32) combine_kernel(const CombineParams p) {
   using C = CombineCfg<D, Q>;
   __shared__ __align__(16) T s_out[32][C::COLS + 2];
-  __shared__ uint32_t s_covered;   // which of the 32 state rows a tile covers
-  if (threadIdx.x == 0) s_covered = p.tiles ? 0u : 0xffffffffu;
+  __shared__ uint32_t s_covered;   // which of the 32 state rows are written
+  if (threadIdx.x == 0) s_covered = 0u;
   pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -782,15 +782,23 @@ __global__ void __launch_bounds__(CombineCfg<D, Q>::WARPS * 32) combine_kernel(c
   };
   const int runs = live ? p.n_runs : 0;
   fetch(0, 0, 0, runs);        // the prefix's states do not wait for the row's length
+  // A row of a tile with a length outside the cache has no own states (own_kernel has reported it and left the
+  // whole tile out) and keeps what `out` holds.
   int n_own = 0;
+  bool good = true;
   if (live && p.kv_lens) {
     const uint32_t mrow = static_cast<uint32_t>(n) % rg;
-    n_own = min(max((p.kv_lens[div_by(mrow, p.group)] + own::kSplit - 1) / own::kSplit, 0), p.own_max);
+    const int len = p.kv_lens[div_by(mrow, p.group)];
+    good = len >= 0 && len <= p.own_max;
+    n_own = good ? (len + own::kSplit - 1) / own::kSplit : 0;
   }
   const int total = runs + n_own;
   fetch(0, 0, runs, total);
-  if (p.tiles) {
-    // a row that no tile covers has no own states and keeps what `out` holds
+  if (!p.tiles) {
+    const uint32_t mine = __ballot_sync(0xffffffffu, good);
+    if (threadIdx.x == 0) s_covered = mine;
+  } else {
+    // so does a row that no tile covers
     __syncthreads();
     const int row = live ? static_cast<int>(div_by(static_cast<uint32_t>(n) % rg, p.group)) : -1;
     const int low = __reduce_min_sync(0xffffffffu, live ? row : p.n_rows), high = __reduce_max_sync(0xffffffffu, row);
@@ -809,6 +817,8 @@ __global__ void __launch_bounds__(CombineCfg<D, Q>::WARPS * 32) combine_kernel(c
         const int src = __ffs(hits) - 1;
         hits &= hits - 1;
         const int a = __shfl_sync(0xffffffffu, r0, src), c = __shfl_sync(0xffffffffu, nr, src);
+        const int len = lane < c ? p.kv_lens[a + lane] : 0;
+        if (__any_sync(0xffffffffu, len < 0 || len > p.own_max)) continue;
         covered |= row >= a && row < a + c;
       }
     }

@@ -477,6 +477,7 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
                                         : FN<__half, 128>(__VA_ARGS__)))
   rc = DK_DISPATCH_16(prefix_launch, maps, p, pl.whole, st);
   if (rc) return rc;
+  int32_t own_max = 0;
   if (own) {
     dk::own::Params o{};
     o.q = q;
@@ -516,6 +517,7 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
       o.n_runs = pl.n_runs;
       o.per_group = pl.per_group;
     }
+    own_max = o.capacity;
     rc = DK_DISPATCH_16(own_launch, o, st);
     if (rc || pl.upt == 1) return rc;
   }
@@ -525,7 +527,7 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
   c.n_runs = pl.n_runs;
   c.per_group = pl.per_group;
   c.kv_lens = own ? kv_lens : nullptr;
-  c.own_max = pl.own_states;
+  c.own_max = own_max;
   if (own && row_tiles) {
     c.tiles = row_tiles;
     c.n_tiles = n_tiles;

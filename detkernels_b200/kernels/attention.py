@@ -259,7 +259,8 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
     matter, and calls that may overlap need separate ones).
 
     A row that row_tiles leaves out keeps what ``out`` holds (rows of a padded batch); with max_kv_len = 0
-    the tiles are not read and every row is written.
+    the tiles are not read and every row is written.  A length outside [0, max_kv_len] or the cache, or a
+    malformed tile, sets the device status; the rows of that tile keep what ``out`` holds too.
     A row's bits depend on its q, the prefix, its own tokens and nothing else of the batch."""
     import torch
 

@@ -394,9 +394,9 @@ size_t dk_attention_shared_prefix_workspace_size(int32_t n_rows, int32_t n_tiles
  * dk_attention_batch_invariant, or with block_table as in dk_attention_paged_batch_invariant
  * (kv_stride_seq is then the block stride); max_kv_len = 0: no row has any, and k, v, kv_lens and
  * row_tiles are not read.  A length beyond max_kv_len or the cache (detail 0x210), a malformed tile (0x211)
- * or a block id outside the pool (0x212) is recorded as DK_ERR_DEVICE_CHECK.  Nothing beyond a row's own
- * length reaches it, whatever the cache holds there; a row that row_tiles is given without is left as it
- * was in out.  q must be 16-byte aligned with strides that are multiples of 8 elements.
+ * or a block id outside the pool (0x212) is recorded as DK_ERR_DEVICE_CHECK; the rows of a tile that is malformed
+ * or holds such a length are left as they were in out, and so is a row that no tile covers.  Nothing beyond a row's
+ * own length reaches it, whatever the cache holds there.  q must be 16-byte aligned with strides that are multiples of 8 elements.
  * Batch invariant: a row's bits follow from its q, the prefix and its own tokens. */
 int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_stride_head, const void* k_prefix,
                                const void* v_prefix, int64_t prefix_stride_block, int64_t prefix_stride_head,

@@ -128,3 +128,36 @@ def test_an_infinite_element_reaches_only_its_own_pair(dev, dt, D, rd, inter):
     rest = ~want[:, rd:]
     sign = torch.signbit(q[:, 0, rd:]) ^ torch.signbit(w[rd:])
     assert torch.equal(torch.signbit(qo[:, 0, rd:])[rest], sign[rest])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("R", [24, 3000])
+@pytest.mark.parametrize("tiled", [False, True])
+@pytest.mark.parametrize("bad", [-1, 641, 2 ** 31 - 1])
+def test_rows_of_a_bad_length_are_left(dev, D, R, tiled, bad):
+    """Whether several warps share a row (few rows) or one owns it: a length outside the announced maximum is reported,
+    its row, or every row of its tile, keeps what out held, and all others are as in a call without it."""
+    import torch
+
+    from detkernels_b200 import _lib
+    from detkernels_b200.kernels.attention import attention_shared_prefix
+    per = 4 if tiled else 1                      # rows a sequence
+    q, kp, vp, k, v = _attn_inputs(dev, R, 4, 2, D, 200, 704, R // per, seed=R)
+    rng = np.random.default_rng(R)
+    lens = rng.integers(0, 641, size=R)
+    kw = dict(max_kv_len=640)
+    if tiled:
+        kw["row_tiles"] = _i32([(4 * s, 4, s) for s in range(R // 4)], dev)
+    want = attention_shared_prefix(q, kp, vp, k, v, _i32(lens, dev), **kw)
+    at = [0, 9, R - 1]
+    lens[at] = bad
+    left = np.zeros(R, bool)
+    for r in at:
+        left[r // per * per:r // per * per + per] = True
+    out = torch.full_like(q, 7.0)
+    torch.cuda.synchronize(dev)
+    attention_shared_prefix(q, kp, vp, k, v, _i32(lens, dev), out=out, **kw)
+    assert _lib.device_status(dev.index) == (_lib.DK_ERR_DEVICE_CHECK, 0x210)
+    left = torch.from_numpy(left).to(dev)
+    assert (out[left] == 7.0).all() and torch.equal(out[~left], want[~left])
