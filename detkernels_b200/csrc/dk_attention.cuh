@@ -285,6 +285,7 @@ __device__ __forceinline__ int describe_item(const Params& p, int64_t w, Item& i
   it.max_len = 0;
   it.nsplits = 0;
   it.s_begin = it.s_end = 0;
+  if (it.nr == 0) return 1;   // padding of a tile list
   const int rows_per_tile_max = kRows / p.G;
   // r0 against n_rows - nr: r0 + nr may leave 32 bits
   if (it.nr < 1 || it.nr > rows_per_tile_max || it.r0 < 0 || it.r0 > p.n_rows - it.nr || it.seq < 0 ||

@@ -195,6 +195,10 @@ __global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 10) : (D == 128 
     nr = p.tiles[3 * tile + 1];
     seq = p.tiles[3 * tile + 2];
   }
+  if (nr == 0) {   // padding of a tile list
+    pdl_wait();
+    return;
+  }
   if (!tile_fits(r0, nr, seq, p.G, 8 * NB, p.n_rows, p.n_seq)) {
     if (lane == 0 && unit == 0 && kvh == 0) report_error(DK_ERR_DEVICE_CHECK, kDetTile);
     pdl_wait();

@@ -73,7 +73,8 @@ def attention_decode(q, k_cache, v_cache, kv_lens, *, scale=None, row_tiles=None
 
     kv_lens: int32 CUDA tensor [R] (or an int for every row).  row_tiles:
     optional int32 CUDA tensor [T, 3] (first row, row count, sequence) grouping
-    consecutive rows of one sequence; without it row r reads sequence r.
+    consecutive rows of one sequence; without it row r reads sequence r.  A tile of 0 rows is skipped
+    (padding), and rows that no tile covers keep what ``out`` holds.
     max_kv_len: host-side bound on every kv_len (defaults to the capacity).
     block_table: optional int32 CUDA tensor [N_seq, blocks_per_seq] for a paged cache: k_cache /
     v_cache are then block pools [n_blocks, H_kv, page, D] (page a multiple of 64) and token t of

@@ -239,7 +239,8 @@ int dk_argmax_finish_parts(const unsigned long long* keys, int n_parts, int64_t 
  * Row r attends to tokens [0, kv_len_r) of KV sequence seq_r, q head h uses kv head
  * h / (n_q_heads / n_kv_heads).  kv_lens (device int32[n_rows]) may be NULL, then every row
  * uses uniform_kv_len.  row_tiles (device int32[3 * n_tiles]: first row, row count, seq) groups
- * consecutive rows that read the same KV sequence (at most 16 / group rows per tile); when NULL,
+ * consecutive rows that read the same KV sequence (at most 16 / group rows per tile; a tile of 0 rows is
+ * skipped, and rows that no tile covers are left as they were in out); when NULL,
  * row r is its own tile reading sequence r.  max_kv_len bounds every kv_len_r (sizes the grid).
  * head_dim in {32, 64, 128}; dtype DK_BF16 or DK_F16; scale multiplies q.k. */
 /* Scratch bytes for a call with n_tiles tiles (n_rows when row_tiles is NULL) of up to rows_per_tile rows

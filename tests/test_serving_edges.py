@@ -161,3 +161,26 @@ def test_rows_of_a_bad_length_are_left(dev, D, R, tiled, bad):
     assert _lib.device_status(dev.index) == (_lib.DK_ERR_DEVICE_CHECK, 0x210)
     left = torch.from_numpy(left).to(dev)
     assert (out[left] == 7.0).all() and torch.equal(out[~left], want[~left])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_seq", [3, 900])
+@pytest.mark.parametrize("prefix", [0, 100])
+def test_tiles_of_no_rows_are_padding(dev, n_seq, prefix):
+    """Tiles of 0 rows, whatever else they hold, between and behind the others: nothing is reported, the covered rows'
+    bits are those of a list without them and the rest of out stays."""
+    import torch
+
+    from detkernels_b200.kernels.attention import attention_shared_prefix
+    R = 4 * n_seq + 5
+    q, kp, vp, k, v = _attn_inputs(dev, R, 4, 2, 64, 100, 640, n_seq)
+    rng = np.random.default_rng(n_seq)
+    ln = _i32(rng.integers(0, 641, size=R), dev)
+    tiles = [(4 * s, 4, s) for s in range(n_seq)]
+    padded = [(0, 0, 0), (-1, 0, -5)] + [x for t in tiles for x in (t, (2 ** 31 - 1, 0, 2 ** 31 - 1))] + [(0, 0, 0)] * 7
+    outs = []
+    for t in (tiles, padded):
+        out = torch.full_like(q, 7.0)
+        attention_shared_prefix(q, kp, vp, k, v, ln, prefix_len=prefix, row_tiles=_i32(t, dev), out=out)
+        outs.append(out)
+    assert torch.equal(*outs) and (outs[1][4 * n_seq:] == 7.0).all() and not (outs[1][:4 * n_seq] == 7.0).all(-1).any()
