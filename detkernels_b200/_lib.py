@@ -94,6 +94,9 @@ SIGNATURES = {
     "dk_paged_plan": (_int, [_c_void_p, _i64, _i32, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i64, _c_void_p,
                              _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i32,
                              _i64, _c_void_p, _size, _c_void_p]),
+    "dk_paged_plan_padded": (_int, [_c_void_p, _i64, _i32, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i64,
+                                    _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64,
+                                    _c_void_p, _i32, _i64, _c_void_p, _size, _c_void_p]),
     "dk_qk_norm_rope": (_int, [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64,
                                _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64,
                                _c_void_p, _c_void_p, _int, _c_void_p, _c_void_p, _int, _c_void_p, _i64, _i64, _i32,

@@ -220,18 +220,13 @@ int combine_launch(const dk::prefix::CombineParams& p, cudaStream_t st) {
   return combine_launch_q<T, D, 4, 2>(p, st);
 }
 
-}  // namespace
-
-extern "C" {
-
-size_t dk_paged_plan_workspace_size(int64_t n_seqs) { return n_seqs > 0 ? plan_ws_bytes(n_seqs) : 0; }
-
-int dk_paged_plan(int32_t* block_table, int64_t block_table_stride, int32_t blocks_per_seq, const int32_t* kv_lens,
-                  const int32_t* new_lens, int32_t n_seqs, int32_t page_size, const int32_t* free_blocks,
-                  int64_t n_free, const int32_t* cursor, int32_t* cursor_out, int32_t* cu_rows, int32_t* row_seq,
-                  int32_t* row_pos, int64_t* slots, int32_t* q_lens, int64_t n_rows, int32_t* row_tiles,
-                  int32_t rows_per_tile, int64_t n_tiles, void* workspace, size_t workspace_bytes, void* stream) {
-  const char* what = "paged_plan";
+// The entry points of the page plan differ in what becomes of the entries past its totals.
+int paged_plan(const char* what, bool pad, int32_t* block_table, int64_t block_table_stride, int32_t blocks_per_seq,
+               const int32_t* kv_lens, const int32_t* new_lens, int32_t n_seqs, int32_t page_size,
+               const int32_t* free_blocks, int64_t n_free, const int32_t* cursor, int32_t* cursor_out,
+               int32_t* cu_rows, int32_t* row_seq, int32_t* row_pos, int64_t* slots, int32_t* q_lens, int64_t n_rows,
+               int32_t* row_tiles, int32_t rows_per_tile, int64_t n_tiles, void* workspace, size_t workspace_bytes,
+               void* stream) {
   if (n_seqs < 0 || page_size <= 0 || blocks_per_seq < 0 || n_rows < 0 || n_tiles < 0 || n_free < 0)
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: negative size or page_size < 1", what);
   if (n_seqs == 0) return DK_OK;
@@ -275,6 +270,7 @@ int dk_paged_plan(int32_t* block_table, int64_t block_table_stride, int32_t bloc
   p.rpt = dk::divisor(row_tiles ? rows_per_tile : 1);
   p.n_tiles = n_tiles;
   p.ws = static_cast<int32_t*>(workspace);
+  p.pad = pad;
   p.vec = aligned16(row_seq) && aligned16(row_pos) && aligned16(slots) && aligned16(q_lens);
   // at most so many outputs of each kind (the growth is known on the device only)
   int64_t most = rows ? n_rows : n_tiles;
@@ -302,6 +298,33 @@ int dk_paged_plan(int32_t* block_table, int64_t block_table_stride, int32_t bloc
   }
   if (e != cudaSuccess) return fail(DK_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
   return DK_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t dk_paged_plan_workspace_size(int64_t n_seqs) { return n_seqs > 0 ? plan_ws_bytes(n_seqs) : 0; }
+
+int dk_paged_plan(int32_t* block_table, int64_t block_table_stride, int32_t blocks_per_seq, const int32_t* kv_lens,
+                  const int32_t* new_lens, int32_t n_seqs, int32_t page_size, const int32_t* free_blocks,
+                  int64_t n_free, const int32_t* cursor, int32_t* cursor_out, int32_t* cu_rows, int32_t* row_seq,
+                  int32_t* row_pos, int64_t* slots, int32_t* q_lens, int64_t n_rows, int32_t* row_tiles,
+                  int32_t rows_per_tile, int64_t n_tiles, void* workspace, size_t workspace_bytes, void* stream) {
+  return paged_plan("paged_plan", false, block_table, block_table_stride, blocks_per_seq, kv_lens, new_lens, n_seqs,
+                    page_size, free_blocks, n_free, cursor, cursor_out, cu_rows, row_seq, row_pos, slots, q_lens,
+                    n_rows, row_tiles, rows_per_tile, n_tiles, workspace, workspace_bytes, stream);
+}
+
+int dk_paged_plan_padded(int32_t* block_table, int64_t block_table_stride, int32_t blocks_per_seq,
+                         const int32_t* kv_lens, const int32_t* new_lens, int32_t n_seqs, int32_t page_size,
+                         const int32_t* free_blocks, int64_t n_free, const int32_t* cursor, int32_t* cursor_out,
+                         int32_t* cu_rows, int32_t* row_seq, int32_t* row_pos, int64_t* slots, int32_t* q_lens,
+                         int64_t n_rows, int32_t* row_tiles, int32_t rows_per_tile, int64_t n_tiles, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  return paged_plan("paged_plan_padded", true, block_table, block_table_stride, blocks_per_seq, kv_lens, new_lens,
+                    n_seqs, page_size, free_blocks, n_free, cursor, cursor_out, cu_rows, row_seq, row_pos, slots,
+                    q_lens, n_rows, row_tiles, rows_per_tile, n_tiles, workspace, workspace_bytes, stream);
 }
 
 int dk_qk_norm_rope(const void* q, int64_t q_stride_row, int64_t q_stride_head, const void* k, int64_t k_stride_row,

@@ -51,7 +51,7 @@ def paged_plan_reference(block_table, kv_lens, new_lens, page_size, *, free_bloc
 
 def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=None, cursor=None,
                n_rows: Optional[int] = None, rows_per_tile: int = 0, n_tiles: Optional[int] = None,
-               out: Optional[PagedPlan] = None) -> PagedPlan:
+               out: Optional[PagedPlan] = None, pad: bool = False) -> PagedPlan:
     """Plan one step in which sequence b, holding kv_lens[b] tokens, gets new_lens[b] more.
 
     block_table: int32 CUDA [>= B, blocks_per_seq]; kv_lens, new_lens: int32 CUDA [B].
@@ -61,12 +61,17 @@ def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=No
     table past B, stay as they are.
     n_rows: how many new tokens there are (the sum of new_lens, or a bound on it): asks for row_seq,
     row_pos, slots and q_lens.  rows_per_tile and n_tiles (the sum of ceil(new_lens / rows_per_tile), or
-    a bound) ask for row_tiles.  Entries past the step's own total stay as they are (uninitialised in new tensors).
+    a bound) ask for row_tiles.
     out: a PagedPlan of an earlier call whose tensors take the results (its cursor may be ``cursor``).
+    pad: what lies past the step's own totals in the tensors of ``out`` becomes neutral: row_seq, row_pos
+    and q_lens 0, slots -1 (``qk_norm_rope`` stores nothing there), tiles of 0 rows (attention skips them).
+    A captured step that serves smaller ones needs it: without it those entries, an earlier step's slots and
+    tiles, stay as they are.  New tensors are always padded.
 
     A negative length, a sequence longer than its table row, an exhausted free list or more rows or tiles
     than announced sets the device status (``_lib.raise_on_device_error``) and leaves the table and all
-    outputs but cu_rows as they were."""
+    outputs but cu_rows as they were; where entries are padded all of them become neutral, so that the rest
+    of the step stores nothing."""
     import torch
 
     dev, i32 = block_table.device, torch.int32
@@ -90,30 +95,39 @@ def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=No
     if (n_rows is not None and n_rows < 0) or (n_tiles is not None and n_tiles < 0):
         raise ValueError("paged_plan: n_rows and n_tiles must not be negative")
 
-    def take(t, *shape, dtype=i32):
+    def take(t, *shape, dtype=i32, neutral=None):
         """The tensor of an earlier plan, or a new one."""
         if t is None:
-            return kv_lens.new_empty(*shape) if dtype == i32 else kv_lens.new_empty(shape, dtype=dtype)
+            t = kv_lens.new_empty(*shape) if dtype == i32 else kv_lens.new_empty(shape, dtype=dtype)
+            return t if neutral is None or padded else t.fill_(neutral)
         assert t.dtype == dtype and t.get_device() == index and t.shape == shape and t.is_contiguous(), \
             "paged_plan: a tensor of out does not fit"
         return t
 
     old = out if out is not None else _NOTHING
+    # the kernel pads all outputs or none; new tensors beside given ones that stay as they are get it beforehand
+    padded = pad or out is None or (old.row_seq is None and old.row_pos is None and old.slots is None
+                                    and old.q_lens is None and old.row_tiles is None)
     with _lib.on_device(dev):
         kv_lens, new_lens = kv_lens.contiguous(), new_lens.contiguous()
         cu = take(old.cu_rows, B + 1)
         cur = take(old.cursor, 1) if cursor is not None else None
         row_seq = row_pos = slots = q_lens = tiles = None
         if n_rows is not None:
-            row_seq, row_pos, q_lens = take(old.row_seq, n_rows), take(old.row_pos, n_rows), take(old.q_lens, n_rows)
-            slots = take(old.slots, n_rows, dtype=torch.int64)
+            row_seq, row_pos = take(old.row_seq, n_rows, neutral=0), take(old.row_pos, n_rows, neutral=0)
+            q_lens = take(old.q_lens, n_rows, neutral=0)
+            slots = take(old.slots, n_rows, dtype=torch.int64, neutral=-1)
         if rows_per_tile > 0:
-            tiles = take(old.row_tiles, n_tiles, 3)
+            tiles = take(old.row_tiles, n_tiles, 3, neutral=0)
         plan = PagedPlan(block_table, cur, cu, row_seq, row_pos, slots, q_lens, tiles)
         if B == 0:
             cu.zero_()
             if cur is not None and cur.data_ptr() != cursor.data_ptr():
                 cur.copy_(cursor.view(1))
+            if padded:
+                for t, neutral in ((row_seq, 0), (row_pos, 0), (slots, -1), (q_lens, 0), (tiles, 0)):
+                    if t is not None:
+                        t.fill_(neutral)
             return plan
         lib = _lib.load()
         ws = kv_lens.new_empty(-(-lib.dk_paged_plan_workspace_size(B) // 4))
@@ -123,7 +137,7 @@ def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=No
             # an output of no entries is still asked for: its pointer is never followed
             return None if t is None else (t.data_ptr() or ws_ptr)
 
-        rc = lib.dk_paged_plan(
+        rc = (lib.dk_paged_plan_padded if padded else lib.dk_paged_plan)(
             block_table.data_ptr(), stride[0] if shape[0] > 1 else shape[1], shape[1], kv_lens.data_ptr(), new_lens.data_ptr(), B,
             int(page_size), ptr(free_blocks), 0 if free_blocks is None else free_blocks.numel(), ptr(cursor), ptr(cur),
             cu.data_ptr(), ptr(row_seq), ptr(row_pos), ptr(slots), ptr(q_lens), n_rows or 0, ptr(tiles),

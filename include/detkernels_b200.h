@@ -352,12 +352,23 @@ size_t dk_paged_plan_workspace_size(int64_t n_seqs);
  *    of one sequence, the row_tiles of the attention entry points.  Tiles past the last stay as they are.
  * A negative length or a sequence beyond blocks_per_seq pages (detail 0x600), too few free blocks (0x601)
  * or more rows or tiles than the outputs hold (0x602) is recorded as DK_ERR_DEVICE_CHECK; then only cu_rows
- * and the workspace are written and *cursor_out = *cursor. */
+ * and the workspace are written and *cursor_out = *cursor.  The operators below take an earlier plan's slots and
+ * tiles for this step's: where the sizes are bounds, or a refused plan may go unseen, use dk_paged_plan_padded. */
 int dk_paged_plan(int32_t* block_table, int64_t block_table_stride, int32_t blocks_per_seq, const int32_t* kv_lens,
                   const int32_t* new_lens, int32_t n_seqs, int32_t page_size, const int32_t* free_blocks,
                   int64_t n_free, const int32_t* cursor, int32_t* cursor_out, int32_t* cu_rows, int32_t* row_seq,
                   int32_t* row_pos, int64_t* slots, int32_t* q_lens, int64_t n_rows, int32_t* row_tiles,
                   int32_t rows_per_tile, int64_t n_tiles, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same plan for outputs whose sizes are bounds (a captured step that serves smaller ones): the entries past its
+ * totals, and all of them when the plan is refused, become neutral for the operators below: row_seq, row_pos and
+ * q_lens 0, slots -1 (nothing is stored there), tiles of 0 rows (attention skips them).  n_seqs = 0 writes nothing. */
+int dk_paged_plan_padded(int32_t* block_table, int64_t block_table_stride, int32_t blocks_per_seq,
+                         const int32_t* kv_lens, const int32_t* new_lens, int32_t n_seqs, int32_t page_size,
+                         const int32_t* free_blocks, int64_t n_free, const int32_t* cursor, int32_t* cursor_out,
+                         int32_t* cu_rows, int32_t* row_seq, int32_t* row_pos, int64_t* slots, int32_t* q_lens,
+                         int64_t n_rows, int32_t* row_tiles, int32_t rows_per_tile, int64_t n_tiles, void* workspace,
+                         size_t workspace_bytes, void* stream);
 
 /* RMSNorm of every query and key head followed by the rotation of its first rotary_dim elements, f32
  * math, one rounding at the store.  q [n_rows, n_q_heads, head_dim], k and v [n_rows, n_kv_heads,

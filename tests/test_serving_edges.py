@@ -184,3 +184,138 @@ def test_tiles_of_no_rows_are_padding(dev, n_seq, prefix):
         attention_shared_prefix(q, kp, vp, k, v, ln, prefix_len=prefix, row_tiles=_i32(t, dev), out=out)
         outs.append(out)
     assert torch.equal(*outs) and (outs[1][4 * n_seq:] == 7.0).all() and not (outs[1][:4 * n_seq] == 7.0).all(-1).any()
+
+
+NEUTRAL = dict(row_seq=0, row_pos=0, slots=-1, q_lens=0, row_tiles=0)
+
+
+def _plan_outputs(dev, B, n_rows, n_tiles, fill):
+    """A plan whose tensors hold an earlier step's values."""
+    import torch
+
+    from detkernels_b200.kernels.paging import PagedPlan
+    full = lambda *s, d=torch.int32: torch.full(s, fill, dtype=d, device=dev)
+    return PagedPlan(None, None, None, full(n_rows), full(n_rows), full(n_rows, d=torch.int64), full(n_rows),
+                     full(n_tiles, 3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,new_hi,spare", [(1, 1, 3), (7, 5, 1), (40, 30, 700), (40, 300, 9), (2500, 40, 5), (64, 64, 70000)])
+def test_entries_behind_a_plan_are_neutral(dev, B, new_hi, spare):
+    """Bounds larger than the step, in one launch and in two: new tensors, and with pad those of an earlier step, hold
+    the plan and neutral entries behind it; rows alone and tiles alone too."""
+    import torch
+
+    from detkernels_b200.kernels.paging import paged_plan, paged_plan_reference
+    rng = np.random.default_rng(B + spare)
+    kv, new = rng.integers(0, 200, size=B), rng.integers(0, new_hi + 1, size=B)
+    width = int(-(-(kv + new).max() // 16))
+    table = rng.permutation(B * width).reshape(B, width)
+    want = paged_plan_reference(table.tolist(), kv.tolist(), new.tolist(), 16, rows_per_tile=4)
+    n, nt = len(want.row_seq), len(want.row_tiles)
+    args = (_i32(table, dev), _i32(kv, dev), _i32(new, dev), 16)
+    rows, tiles = dict(n_rows=n + spare), dict(rows_per_tile=4, n_tiles=nt + spare)
+    old = lambda: _plan_outputs(dev, B, n + spare, nt + spare, 12345)
+    mixed = old()._replace(slots=None, row_tiles=None)     # some tensors of an earlier step, which stay; the rest new
+    for kw, out, pad in (({**rows, **tiles}, None, False), ({**rows, **tiles}, old(), True), (rows, None, False),
+                         (rows, old(), True), (tiles, None, False), (tiles, old(), True), ({**rows, **tiles}, mixed, False)):
+        got = paged_plan(*args, **kw, out=out, pad=pad)
+        for name, m in (("row_seq", n), ("row_pos", n), ("slots", n), ("q_lens", n), ("row_tiles", nt)):
+            t, w = getattr(got, name), getattr(want, name)
+            if (name == "row_tiles" and "n_tiles" not in kw) or (name != "row_tiles" and "n_rows" not in kw):
+                assert t is None
+                continue
+            w = np.asarray(w, np.int64).reshape(m, *t.shape[1:])
+            assert np.array_equal(t[:m].cpu().numpy(), w), name
+            rest = 12345 if out is mixed and getattr(mixed, name) is not None else NEUTRAL[name]
+            assert t.shape[0] == m + spare and (t[m:] == rest).all(), name
+    none = paged_plan(_i32(np.zeros((2, 1)), dev), _i32([], dev), _i32([], dev), 16, n_rows=5, rows_per_tile=4, n_tiles=2)
+    assert all((getattr(none, k) == v).all() for k, v in NEUTRAL.items())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [2, 3000])
+@pytest.mark.parametrize("why", ["length", "pool", "rows"])
+def test_a_refused_plan_leaves_nothing_to_do(dev, B, why):
+    import torch
+
+    from detkernels_b200 import _lib
+    from detkernels_b200.kernels.paging import paged_plan
+    new = np.full(B, 3)
+    new[-1] = -1 if why == "length" else 3
+    n = 3 * B - (why == "rows")
+    free = _i32(np.arange(B - (why == "pool")), dev)
+    for out in (None, _plan_outputs(dev, B, n, B, 7)):
+        table = torch.full((B, 1), -9, dtype=torch.int32, device=dev)
+        got = paged_plan(table, _i32(np.zeros(B), dev), _i32(new, dev), 64, free_blocks=free, cursor=_i32([0], dev),
+                         n_rows=n, rows_per_tile=3, n_tiles=B, out=out, pad=True)
+        code = {"length": 0x600, "pool": 0x601, "rows": 0x602}[why]
+        assert _lib.device_status(dev.index) == (_lib.DK_ERR_DEVICE_CHECK, code)
+        assert (table == -9).all() and got.cursor.tolist() == [0]
+        for k, v in NEUTRAL.items():
+            assert (getattr(got, k) == v).all(), k
+
+
+@pytest.mark.gpu
+def test_a_step_captured_at_its_largest_serves_smaller_ones(dev):
+    """Plan, norm into the cache and attention captured once for 40 rows and 16 tiles, then replayed for ragged steps of
+    fewer, the last one refused: caches, tables and covered rows as in eager steps of the exact sizes, everything else
+    as it was."""
+    import torch
+
+    from detkernels_b200 import _lib
+    from detkernels_b200.kernels.attention import attention_shared_prefix
+    from detkernels_b200.kernels.paging import paged_plan
+    from detkernels_b200.kernels.rope import qk_norm_rope, rope_table
+    B, H, Hkv, D, P, page, rows, tiles = 6, 8, 2, 64, 130, 64, 40, 16
+    g = torch.Generator(device=dev).manual_seed(2)
+    randn = lambda *s: torch.randn(*s, device=dev, generator=g).to(torch.bfloat16)
+    rope, qw, kw = rope_table(1024, D, device=dev), randn(D), randn(D)
+    n_pre = -(-P // page)
+    kc0, vc0 = randn(n_pre + 14, Hkv, page, D), randn(n_pre + 14, Hkv, page, D)
+    order = torch.randperm(n_pre + 14, device=dev, generator=g).to(torch.int32)
+    pre, free = order[:n_pre].contiguous(), order[n_pre:].contiguous()
+
+    def state():
+        z = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)
+        return dict(kc=kc0.clone(), vc=vc0.clone(), table=z(B, 5), cursor=z(1), kv=z(B), nw=z(B),
+                    qkv=torch.zeros(rows, (H + 2 * Hkv) * D, dtype=torch.bfloat16, device=dev),
+                    out=torch.full((rows, H, D), 7.0, dtype=torch.bfloat16, device=dev))
+
+    def step(s, n_rows, n_tiles, plan=None, pad=False):
+        q, k, v = (x.view(n_rows, -1, D) for x in s["qkv"][:n_rows].split([H * D, Hkv * D, Hkv * D], 1))
+        plan = paged_plan(s["table"], s["kv"], s["nw"], page, free_blocks=free, cursor=s["cursor"], n_rows=n_rows,
+                          rows_per_tile=4, n_tiles=n_tiles, out=plan, pad=pad)
+        s["cursor"].copy_(plan.cursor)
+        q, _ = qk_norm_rope(q, k, plan.row_pos + P, qw, kw, rope, v=v, k_cache=s["kc"], v_cache=s["vc"], slots=plan.slots)
+        attention_shared_prefix(q, s["kc"], s["vc"], s["kc"], s["vc"], plan.q_lens, prefix_len=P, prefix_blocks=pre,
+                                block_table=s["table"], row_tiles=plan.row_tiles, out=s["out"][:n_rows], max_kv_len=320)
+        return plan
+
+    a, b = state(), state()
+    plan = step(a, rows, tiles)          # an empty step: loads the library and makes the plan's tensors
+    for k in ("kc", "vc", "table", "kv"):
+        assert torch.equal(a[k], b[k])
+    graph = torch.cuda.CUDAGraph()
+    with _lib.graph_capture(graph):
+        step(a, rows, tiles, plan=plan, pad=True)
+    for i, new in enumerate(([8, 8, 8, 8, 4, 4], [1, 0, 3, 1, 0, 9], [0] * 6, [1] * 6, [0, 0, 33, 1, 0, 0], [1, 1, 0, 0, 0, 1])):
+        a["nw"].copy_(_i32(new, dev))
+        a["qkv"].copy_(randn(*a["qkv"].shape))
+        a["out"].fill_(7.0)
+        for k in ("nw", "qkv", "out"):
+            b[k].copy_(a[k])
+        graph.replay()
+        n = sum(new)
+        if n:
+            step(b, n, sum(-(-x // 4) for x in new))
+        for k in ("kc", "vc", "table", "cursor", "out"):
+            assert torch.equal(a[k], b[k]), (i, k)
+        a["kv"] += a["nw"]
+        b["kv"] += b["nw"]
+    keep = {k: v.clone() for k, v in a.items()}
+    a["nw"].fill_(64)                    # more rows than the step was captured for
+    graph.replay()
+    assert _lib.device_status(dev.index) == (_lib.DK_ERR_DEVICE_CHECK, 0x602)
+    for k in ("kc", "vc", "table", "cursor", "out"):
+        assert torch.equal(a[k], keep[k]), k
