@@ -737,6 +737,7 @@ struct CombineParams {
   int own_max;              // the longest length a row may have
   const int32_t* tiles;     // the row tiles, null: every row is its own
   int32_t n_tiles, n_rows, n_seq;
+  int report;               // a malformed tile is reported here (own_kernel does where it runs)
   int64_t st_rows, rg;      // hkv * rows * G, rows * G
   int G;
   Divisor31 group;          // by G
@@ -810,14 +811,17 @@ __global__ void __launch_bounds__(CombineCfg<D, Q>::WARPS * 32) combine_kernel(c
         r0 = p.tiles[3 * static_cast<int64_t>(t)];
         nr = p.tiles[3 * static_cast<int64_t>(t) + 1];
         const int seq = p.tiles[3 * static_cast<int64_t>(t) + 2];
-        if (!own::tile_fits(r0, nr, seq, p.G, own::kRows, p.n_rows, p.n_seq)) nr = 0;
+        if (!own::tile_fits(r0, nr, seq, p.G, own::kRows, p.n_rows, p.n_seq)) {
+          if (p.report && nr != 0 && blockIdx.x == 0 && blockIdx.y == 0) report_error(DK_ERR_DEVICE_CHECK, own::kDetTile);
+          nr = 0;
+        }
       }
       uint32_t hits = __ballot_sync(0xffffffffu, nr > 0 && r0 <= high && r0 + nr > low);
       while (hits) {
         const int src = __ffs(hits) - 1;
         hits &= hits - 1;
         const int a = __shfl_sync(0xffffffffu, r0, src), c = __shfl_sync(0xffffffffu, nr, src);
-        const int len = lane < c ? p.kv_lens[a + lane] : 0;
+        const int len = p.kv_lens && lane < c ? p.kv_lens[a + lane] : 0;
         if (__any_sync(0xffffffffu, len < 0 || len > p.own_max)) continue;
         covered |= row >= a && row < a + c;
       }

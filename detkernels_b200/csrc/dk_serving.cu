@@ -551,10 +551,11 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
   c.per_group = pl.per_group;
   c.kv_lens = own ? kv_lens : nullptr;
   c.own_max = own_max;
-  if (own && row_tiles) {
+  if (row_tiles) {
     c.tiles = row_tiles;
     c.n_tiles = n_tiles;
-    c.n_seq = static_cast<int32_t>(kv_n_seq);
+    c.n_seq = static_cast<int32_t>(own ? kv_n_seq : kI32Max);   // without own tokens no sequence is read
+    c.report = !own;
   }
   c.n_rows = n_rows;
   c.st_rows = st_rows;

@@ -260,7 +260,7 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
     matter, and calls that may overlap need separate ones).
 
     A row that row_tiles leaves out keeps what ``out`` holds (rows of a padded batch); with max_kv_len = 0
-    the tiles are not read and every row is written.  A length outside [0, max_kv_len] or the cache, or a
+    no row has tokens of its own, and kv_lens are not read.  A length outside [0, max_kv_len] or the cache, or a
     malformed tile, sets the device status; the rows of that tile keep what ``out`` holds too.
     A row's bits depend on its q, the prefix, its own tokens and nothing else of the batch."""
     import torch
@@ -325,8 +325,8 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
         q_st = q.stride()
     with _lib.on_device(dev):
         if P == 0:
-            return attention_decode(q, k_cache, v_cache, kv_lens, scale=scale, row_tiles=row_tiles,
-                                    max_kv_len=max_kv_len, out=out, block_table=block_table)
+            return attention_decode(q, k_cache, v_cache, kv_lens if max_kv_len else 0, scale=scale,
+                                    row_tiles=row_tiles, max_kv_len=max_kv_len, out=out, block_table=block_table)
         ps = _shared_strides(k_prefix, v_prefix, "prefix")
         cs = [0, 0, 0, 1]
         n_tiles = R if row_tiles is None else row_tiles.shape[0]

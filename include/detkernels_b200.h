@@ -404,8 +404,8 @@ size_t dk_attention_shared_prefix_workspace_size(int32_t n_rows, int32_t n_tiles
  * outside the pool: DK_ERR_DEVICE_CHECK, detail 0x62a).  prefix_page is a multiple of 64.
  * The rows' own tokens: q, k, v, kv_lens, row_tiles, max_kv_len, scale as in
  * dk_attention_batch_invariant, or with block_table as in dk_attention_paged_batch_invariant
- * (kv_stride_seq is then the block stride); max_kv_len = 0: no row has any, and k, v, kv_lens and
- * row_tiles are not read.  A length beyond max_kv_len or the cache (detail 0x210), a malformed tile (0x211)
+ * (kv_stride_seq is then the block stride); max_kv_len = 0: no row has any, and k, v and kv_lens are not
+ * read.  A length beyond max_kv_len or the cache (detail 0x210), a malformed tile (0x211)
  * or a block id outside the pool (0x212) is recorded as DK_ERR_DEVICE_CHECK; the rows of a tile that is malformed
  * or holds such a length are left as they were in out, and so is a row that no tile covers.  Nothing beyond a row's
  * own length reaches it, whatever the cache holds there.  q must be 16-byte aligned with strides that are multiples of 8 elements.

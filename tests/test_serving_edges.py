@@ -319,3 +319,30 @@ def test_a_step_captured_at_its_largest_serves_smaller_ones(dev):
     assert _lib.device_status(dev.index) == (_lib.DK_ERR_DEVICE_CHECK, 0x602)
     for k in ("kc", "vc", "table", "cursor", "out"):
         assert torch.equal(a[k], keep[k]), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,n_tiles", [(9, 1), (700, 300)])
+@pytest.mark.parametrize("prefix", [0, 100])
+def test_rows_without_tokens_of_their_own_keep_to_the_tiles(dev, R, n_tiles, prefix):
+    """max_kv_len = 0: lengths are not read, rows that a tile covers are those of a call without tiles, the others stay,
+    and a malformed tile is reported."""
+    import torch
+
+    from detkernels_b200 import _lib
+    from detkernels_b200.kernels.attention import attention_shared_prefix
+    q, kp, vp, k, v = _attn_inputs(dev, R, 6, 2, 64, 100, 64, R)
+    ln = torch.full((R,), 5, dtype=torch.int32, device=dev)
+    kw = dict(prefix_len=prefix, max_kv_len=0)
+    want = attention_shared_prefix(q, kp, vp, k, v, ln, **kw)
+    assert prefix or (want == 0).all()
+    tiles = [(2 * i + 1, 1 + i % 2, i) for i in range(n_tiles)] + [(0, 0, 0)]
+    covered = np.zeros(R, bool)
+    for a, n, _ in tiles:
+        covered[a:a + n] = True
+    covered = torch.from_numpy(covered).to(dev)
+    for extra in ([], [(R, 1, 0)]):
+        out = torch.full_like(q, 7.0)
+        attention_shared_prefix(q, kp, vp, k, v, ln, row_tiles=_i32(tiles + extra, dev), out=out, **kw)
+        assert _lib.device_status(dev.index) == ((_lib.DK_ERR_DEVICE_CHECK, 0x211) if extra else (0, 0))
+        assert torch.equal(out[covered], want[covered]) and (out[~covered] == 7.0).all() and not covered.all()
