@@ -113,6 +113,9 @@ SIGNATURES = {
 # layout version of the structs mirrored here (DK_ABI_VERSION of include/detkernels_b200.h)
 ABI_VERSION = 3
 
+# the zeroed arrival counters at the start of a workspace (DK_WORKSPACE_COUNTER_BYTES)
+WORKSPACE_COUNTER_BYTES = 1 << 20
+
 DK_EPI_STORE = 0
 DK_EPI_RESIDUAL = 1
 DK_EPI_SILU = 2

@@ -256,8 +256,8 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
     max_kv_len count the rows' own tokens only; the workspace of a small batch grows with max_kv_len, so
     give it where the cache is much longer than the rows).  bf16 or f16; head_dim 32, 64 or 128; at most 16 query
     heads per KV head.  workspace: uint8 CUDA tensor of at least
-    ``dk_attention_shared_prefix_workspace_size`` bytes (a new one if not given; its contents do not
-    matter, and calls that may overlap need separate ones).
+    ``dk_attention_shared_prefix_workspace_size`` bytes (a new one if not given, and without a prefix; its
+    contents do not matter, and calls that may overlap need separate ones).
 
     A row that row_tiles leaves out keeps what ``out`` holds (rows of a padded batch); with max_kv_len = 0
     no row has tokens of its own, and kv_lens are not read.  A length outside [0, max_kv_len] or the cache, or a
@@ -325,7 +325,14 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
         q_st = q.stride()
     with _lib.on_device(dev):
         if P == 0:
-            return attention_decode(q, k_cache, v_cache, kv_lens if max_kv_len else 0, scale=scale,
+            # scratch of this call alone, its counters zeroed: the shared one of attention_decode would be raced for
+            # by two captured calls replayed at once
+            n_tiles, per = (R, 1) if row_tiles is None else (row_tiles.shape[0], 2)
+            nbytes = _lib.load().dk_attention_workspace_size(n_tiles, per, H, Hkv, D, max_kv_len)
+            ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+            if nbytes:
+                ws[:_lib.WORKSPACE_COUNTER_BYTES].zero_()
+            return attention_decode(q, k_cache, v_cache, kv_lens if max_kv_len else 0, scale=scale, workspace=ws,
                                     row_tiles=row_tiles, max_kv_len=max_kv_len, out=out, block_table=block_table)
         ps = _shared_strides(k_prefix, v_prefix, "prefix")
         cs = [0, 0, 0, 1]

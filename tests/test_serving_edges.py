@@ -346,3 +346,36 @@ def test_rows_without_tokens_of_their_own_keep_to_the_tiles(dev, R, n_tiles, pre
         attention_shared_prefix(q, kp, vp, k, v, ln, row_tiles=_i32(tiles + extra, dev), out=out, **kw)
         assert _lib.device_status(dev.index) == ((_lib.DK_ERR_DEVICE_CHECK, 0x211) if extra else (0, 0))
         assert torch.equal(out[covered], want[covered]) and (out[~covered] == 7.0).all() and not covered.all()
+
+
+@pytest.mark.gpu
+def test_calls_without_a_prefix_share_no_scratch(dev, monkeypatch):
+    """prefix_len = 0 with rows of several splits: the bits of attention_decode, from scratch of the call's own; two
+    captured calls replayed at once on two streams."""
+    import torch
+
+    from detkernels_b200 import _lib
+    from detkernels_b200.kernels.attention import attention_decode, attention_shared_prefix
+    cases = []
+    for R, seed in ((3, 1), (40, 2)):
+        q, kp, vp, k, v = _attn_inputs(dev, R, 8, 4, 64, 1, 2048, R, seed)
+        ln = _i32(np.random.default_rng(seed).integers(0, 2049, size=R), dev)
+        cases.append((q, kp, vp, k, v, ln, attention_decode(q, k, v, ln)))
+
+    def shared(nbytes, *_):
+        assert nbytes == 0, "a workspace that other calls use"
+    monkeypatch.setattr(_lib, "workspace", shared)
+    graphs = []
+    for q, kp, vp, k, v, ln, want in cases:
+        assert torch.equal(attention_shared_prefix(q, kp, vp, k, v, ln, prefix_len=0), want)
+        g = torch.cuda.CUDAGraph()
+        with _lib.graph_capture(g):
+            out = attention_shared_prefix(q, kp, vp, k, v, ln, prefix_len=0)
+        graphs.append((g, out, want, torch.cuda.Stream(device=dev)))
+    for _ in range(20):
+        for g, out, _, s in graphs:
+            with torch.cuda.stream(s):
+                out.zero_()
+                g.replay()
+        torch.cuda.synchronize(dev)
+        assert all(torch.equal(out, want) for _, out, want, _ in graphs)
