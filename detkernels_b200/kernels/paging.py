@@ -49,6 +49,16 @@ def paged_plan_reference(block_table, kv_lens, new_lens, page_size, *, free_bloc
     return PagedPlan(table, cursor, cu, seq, pos, slots, [t + 1 for t in pos], tiles)
 
 
+def _apart(lens, plan):
+    """lens, or a copy if a row or tile output lies over it (the kernels read lengths while they write rows)."""
+    begin = lens.data_ptr()
+    end = begin + 4 * lens.numel()
+    for t in plan[2:]:
+        if t is not None and t.data_ptr() < end and begin < t.data_ptr() + t.numel() * t.element_size():
+            return lens.clone()
+    return lens
+
+
 def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=None, cursor=None,
                n_rows: Optional[int] = None, rows_per_tile: int = 0, n_tiles: Optional[int] = None,
                out: Optional[PagedPlan] = None, pad: bool = False) -> PagedPlan:
@@ -62,7 +72,8 @@ def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=No
     n_rows: how many new tokens there are (the sum of new_lens, or a bound on it): asks for row_seq,
     row_pos, slots and q_lens.  rows_per_tile and n_tiles (the sum of ceil(new_lens / rows_per_tile), or
     a bound) ask for row_tiles.
-    out: a PagedPlan of an earlier call whose tensors take the results (its cursor may be ``cursor``).
+    out: a PagedPlan of an earlier call whose tensors take the results (its cursor may be ``cursor``, its
+    q_lens kv_lens: a decode step's lengths are the next one's).
     pad: what lies past the step's own totals in the tensors of ``out`` becomes neutral: row_seq, row_pos
     and q_lens 0, slots -1 (``qk_norm_rope`` stores nothing there), tiles of 0 rows (attention skips them).
     A captured step that serves smaller ones needs it: without it those entries, an earlier step's slots and
@@ -120,6 +131,8 @@ def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=No
         if rows_per_tile > 0:
             tiles = take(old.row_tiles, n_tiles, 3, neutral=0)
         plan = PagedPlan(block_table, cur, cu, row_seq, row_pos, slots, q_lens, tiles)
+        if out is not None:
+            kv_lens, new_lens = _apart(kv_lens, plan), _apart(new_lens, plan)
         if B == 0:
             cu.zero_()
             if cur is not None and cur.data_ptr() != cursor.data_ptr():

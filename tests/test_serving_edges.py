@@ -379,3 +379,26 @@ def test_calls_without_a_prefix_share_no_scratch(dev, monkeypatch):
                 g.replay()
         torch.cuda.synchronize(dev)
         assert all(torch.equal(out, want) for _, out, want, _ in graphs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [5, 900, 6000])
+def test_a_plan_over_its_own_lengths(dev, B):
+    """kv_lens and new_lens inside the outputs that the plan writes: the plan of copies of them."""
+    import torch
+
+    from detkernels_b200.kernels.paging import paged_plan
+    rng = np.random.default_rng(B)
+    kv, new = rng.integers(1, 60, size=B), rng.integers(0, 4, size=B)
+    table = _i32(rng.permutation(B * 64).reshape(B, 64), dev)
+    n, nt = int(new.sum()), int((-(-new // 2)).sum())
+    kw = dict(n_rows=n, rows_per_tile=2, n_tiles=nt)
+    want = paged_plan(table, _i32(kv, dev), _i32(new, dev), 1, **kw)
+    for lens, name, at in ((kv, "q_lens", n - B), (kv, "q_lens", 0), (new, "row_seq", n - B), (new, "row_tiles", 0), (kv, "cu_rows", 1)):
+        old = paged_plan(table, _i32(kv, dev), _i32(new, dev), 1, **kw)
+        over = getattr(old, name).view(-1)[at:at + B]
+        over.copy_(_i32(lens, dev))
+        a, b = (over, _i32(new, dev)) if lens is kv else (_i32(kv, dev), over)
+        got = paged_plan(table, a, b, 1, out=old, **kw)
+        for x, y in zip(got, want):
+            assert (x is None and y is None) or torch.equal(x, y), name
