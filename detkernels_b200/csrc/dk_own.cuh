@@ -80,7 +80,7 @@ struct Params {
   const int32_t* kv_lens;
   const int32_t* tiles;       // null: row r is a tile of sequence r
   int32_t n_tiles, n_rows, hq, hkv, G;
-  int32_t n_seq, capacity;
+  int32_t n_seq, capacity;    // capacity: the longest length a row may have, at most max_splits splits
   const int32_t* block_table; // null: contiguous
   int64_t bt_stride;
   int32_t page, n_blocks;
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 10) : (D == 128 
     return;
   }
   const int my_len = lane < nr ? p.kv_lens[r0 + lane] : 0;
-  const bool bad = my_len < 0 || my_len > p.capacity || my_len > p.max_splits * kSplit;
+  const bool bad = my_len < 0 || my_len > p.capacity;
   if (__any_sync(0xffffffffu, bad)) {
     if (lane == 0 && unit == 0 && kvh == 0) report_error(DK_ERR_DEVICE_CHECK, kDetLen);
     pdl_wait();
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(32, NB == 2 ? (D == 128 ? 9 : 10) : (D == 128 
   const int min_len = __reduce_min_sync(0xffffffffu, lane < nr ? my_len : max_len);
   const bool all = p.upt == 1;
   const int t_begin = unit * p.spu * kSplit;
-  const int t_end = min(max_len, t_begin + p.spu * kSplit);
+  const int t_end = t_begin + min(max_len - t_begin, p.spu * kSplit);   // (the sum of the two may leave 32 bits)
   if (t_begin >= t_end && !all) {
     pdl_wait();
     return;

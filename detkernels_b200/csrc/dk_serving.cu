@@ -432,8 +432,10 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
                     "block_table_stride >= blocks_per_seq", what);
       kv_capacity = static_cast<int64_t>(page_size) * blocks_per_seq;
     }
-    if (kv_capacity <= 0 || kv_n_seq <= 0 || kv_capacity > kI32Max || kv_n_seq > kI32Max)
+    // whole splits of the longest row stay inside 32 bits
+    if (kv_capacity <= 0 || kv_n_seq <= 0 || kv_capacity > kI32Max - (dk::own::kSplit - 1) || kv_n_seq > kI32Max)
       return fail(DK_ERR_INVALID_ARGUMENT, "%s: bad KV extents", what);
+    if (max_kv_len > kv_capacity) max_kv_len = static_cast<int32_t>(kv_capacity);
     if (!row_tiles && kv_n_seq < n_rows) return fail(DK_ERR_INVALID_ARGUMENT, "%s: fewer KV sequences than rows", what);
   }
   if (!row_tiles) n_tiles = n_rows;
@@ -519,7 +521,7 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
     o.hkv = n_kv_heads;
     o.G = G;
     o.n_seq = static_cast<int32_t>(kv_n_seq);
-    o.capacity = static_cast<int32_t>(kv_capacity < max_kv_len ? kv_capacity : max_kv_len);
+    o.capacity = max_kv_len;
     o.block_table = block_table;
     o.bt_stride = block_table_stride;
     o.page = block_table ? page_size : 0;

@@ -24,6 +24,7 @@ from __future__ import annotations
 from detkernels_b200 import _lib
 
 KV_SPLIT = _lib.ATTN_KV_SPLIT
+_I32_MAX = 2 ** 31 - 1
 
 
 def attention_reference(q, k, v, scale: float | None = None, *, kv_lens=None):
@@ -287,8 +288,8 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
         n_pool, page_p = p_shape[0], p_shape[2]
         p_cap = prefix_blocks.numel() * page_p
     P = p_cap if prefix_len is None else int(prefix_len)
-    if P < 0 or P > p_cap:
-        raise ValueError("attention_shared_prefix: prefix_len %d outside [0, %d]" % (P, p_cap))
+    if P < 0 or P > min(p_cap, _I32_MAX):
+        raise ValueError("attention_shared_prefix: prefix_len %d outside [0, %d]" % (P, min(p_cap, _I32_MAX)))
     uniform = isinstance(kv_lens, int)
     if not uniform:
         assert kv_lens.dtype == torch.int32 and kv_lens.get_device() == index and kv_lens.numel() == R
@@ -306,6 +307,9 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
     max_kv_len = int(max_kv_len)
     if max_kv_len < 0 or (max_kv_len and not cap):
         raise ValueError("attention_shared_prefix: max_kv_len %d outside the cache" % max_kv_len)
+    max_kv_len = min(max_kv_len, cap)   # a bound beyond the cache bounds nothing, but sizes the work
+    if max_kv_len > _I32_MAX:
+        raise ValueError("attention_shared_prefix: max_kv_len %d exceeds 2^31 - 1" % max_kv_len)
     if uniform and not 0 <= kv_lens <= max_kv_len:
         raise ValueError("attention_shared_prefix: kv_lens %d outside [0, %d]" % (kv_lens, max_kv_len))
     if scale is None:

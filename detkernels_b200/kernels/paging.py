@@ -94,8 +94,8 @@ def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=No
     assert shape[1] <= 1 or stride[1] == 1, "block_table: unit stride along a row"
     assert kv_lens.dtype == i32 and new_lens.dtype == i32 and kv_lens.dim() == 1 and new_lens.shape == (B,), \
         "lengths must be int32 [B]"
-    if page_size < 1:
-        raise ValueError("paged_plan: page_size must be positive")
+    if not 1 <= page_size < 2 ** 31:
+        raise ValueError("paged_plan: page_size must be positive and below 2^31")
     if (free_blocks is None) != (cursor is None):
         raise ValueError("paged_plan: free_blocks and cursor go together")
     if free_blocks is not None:
@@ -103,6 +103,7 @@ def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=No
         assert cursor.dtype == i32 and cursor.get_device() == index and cursor.numel() == 1
     if rows_per_tile < 0 or (rows_per_tile > 0 and n_tiles is None) or (rows_per_tile == 0 and n_tiles):
         raise ValueError("paged_plan: rows_per_tile and n_tiles go together")
+    rows_per_tile = min(rows_per_tile, 2 ** 31 - 1)   # no sequence has more rows
     if (n_rows is not None and n_rows < 0) or (n_tiles is not None and n_tiles < 0):
         raise ValueError("paged_plan: n_rows and n_tiles must not be negative")
 

@@ -402,3 +402,42 @@ def test_a_plan_over_its_own_lengths(dev, B):
         got = paged_plan(table, a, b, 1, out=old, **kw)
         for x, y in zip(got, want):
             assert (x is None and y is None) or torch.equal(x, y), name
+
+
+def test_the_longest_caches_on_the_host():
+    """Whole splits of 64 stay inside 32 bits: a capacity of 2^31 - 64 tokens gets as far as its workspace."""
+    from detkernels_b200 import _lib
+    lib = _lib.load()
+
+    def call(cap, max_len):
+        return lib.dk_attention_shared_prefix(16, 128, 64, 16, 16, 0, 640, 64, 10, None, 0, 0, 16, 16, 64, 64, 64, 3, cap,
+                                              None, 0, 0, 0, 0, 16, 128, 64, 16, None, 0, 3, 2, 2, 64, max_len, 0.1,
+                                              _lib.DK_BF16, 16, 0, None)
+    assert call(2 ** 31 - 64, 2 ** 31 - 1) == _lib.DK_ERR_WORKSPACE
+    assert call(2 ** 31 - 63, 100) == _lib.DK_ERR_INVALID_ARGUMENT and "KV extents" in _lib.last_error()
+
+
+@pytest.mark.gpu
+def test_sizes_that_leave_32_bits(dev):
+    """Refused, not cut to their low half; a maximum beyond the cache is the cache's."""
+    import torch
+
+    from detkernels_b200.kernels.attention import attention_shared_prefix
+    from detkernels_b200.kernels.paging import paged_plan
+    one, none = _i32([1], dev), _i32([0], dev)
+    table = _i32([[0]], dev)
+    with pytest.raises(ValueError):
+        paged_plan(table, none, one, 2 ** 32 + 64, n_rows=1)
+    got = paged_plan(table, none, one, 64, n_rows=1, rows_per_tile=2 ** 32 + 1, n_tiles=1)
+    assert got.row_tiles.tolist() == [[0, 1, 0]]
+    q, kp, vp, k, v = _attn_inputs(dev, 3, 2, 1, 32, 10, 64, 3)
+    ln = _i32([5, 0, 64], dev)
+    want = attention_shared_prefix(q, kp, vp, k, v, ln)
+    for most in (65, 2 ** 31 - 1, 2 ** 32, 2 ** 40 + 1):
+        assert torch.equal(attention_shared_prefix(q, kp, vp, k, v, ln, max_kv_len=most), want)
+    pool = torch.zeros(1, 1, 4096, 32, dtype=q.dtype, device=dev)
+    wide = torch.zeros(3, 2 ** 20, dtype=torch.int32, device=dev)      # 2^32 tokens a row
+    with pytest.raises(ValueError):
+        attention_shared_prefix(q, kp, vp, pool, pool, ln, block_table=wide)
+    with pytest.raises(ValueError):
+        attention_shared_prefix(q, pool, pool, k, v, ln, prefix_blocks=wide[0].repeat(2)[:2 ** 20 + 1])
