@@ -321,6 +321,9 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
     if row_tiles is not None:
         assert row_tiles.dtype == torch.int32 and row_tiles.get_device() == index and row_tiles.is_contiguous()
         assert row_tiles.dim() == 2 and row_tiles.shape[1] == 3
+    if workspace is not None:
+        assert workspace.dtype == torch.uint8 and workspace.get_device() == index and workspace.is_contiguous(), \
+            "workspace must be a contiguous uint8 CUDA tensor on q's device"
     if R == 0:
         return out
     q_st = q.stride()

@@ -441,3 +441,23 @@ def test_sizes_that_leave_32_bits(dev):
         attention_shared_prefix(q, kp, vp, pool, pool, ln, block_table=wide)
     with pytest.raises(ValueError):
         attention_shared_prefix(q, pool, pool, k, v, ln, prefix_blocks=wide[0].repeat(2)[:2 ** 20 + 1])
+
+
+@pytest.mark.gpu
+def test_a_workspace_of_the_callers(dev):
+    """Its contents do not matter, too small a one is refused, and so is anything that is not bytes on the device."""
+    import torch
+
+    from detkernels_b200 import _lib
+    from detkernels_b200.kernels.attention import attention_shared_prefix
+    q, kp, vp, k, v = _attn_inputs(dev, 3, 4, 2, 64, 700, 640, 3)
+    ln = _i32([5, 0, 640], dev)
+    want = attention_shared_prefix(q, kp, vp, k, v, ln)
+    n = _lib.load().dk_attention_shared_prefix_workspace_size(3, 3, 4, 2, 64, 700, 640)
+    ws = torch.full((n,), 255, dtype=torch.uint8, device=dev)
+    assert torch.equal(attention_shared_prefix(q, kp, vp, k, v, ln, workspace=ws), want)
+    with pytest.raises(_lib.DetKernelsError):
+        attention_shared_prefix(q, kp, vp, k, v, ln, workspace=ws[:n - 16])
+    for bad in (ws.cpu(), ws[:n // 4 * 4].view(torch.int32), ws[::2]):
+        with pytest.raises(AssertionError):
+            attention_shared_prefix(q, kp, vp, k, v, ln, workspace=bad)
