@@ -461,3 +461,12 @@ def test_a_workspace_of_the_callers(dev):
     for bad in (ws.cpu(), ws[:n // 4 * 4].view(torch.int32), ws[::2]):
         with pytest.raises(AssertionError):
             attention_shared_prefix(q, kp, vp, k, v, ln, workspace=bad)
+
+
+@pytest.mark.gpu
+def test_a_small_plan_counts_the_one_launch_it_takes(dev):
+    from detkernels_b200 import _lib
+    from detkernels_b200.kernels.paging import paged_plan
+    n0 = _lib.launch_count()
+    paged_plan(_i32([[0]], dev), _i32([0], dev), _i32([1], dev), 64, n_rows=1)
+    assert _lib.launch_count() - n0 == 1
