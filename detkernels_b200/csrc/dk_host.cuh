@@ -38,7 +38,11 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // Launch with programmatic stream serialization: the kernel may begin (and run
 // its preamble) while the previous kernel on the stream finishes; every kernel
 // of this library waits for its predecessor (griddepcontrol.wait) before it
-// touches global memory.
+// touches global memory that the predecessor may write.  One reads other memory
+// first: own::own_kernel its lengths, tiles, queries, keys and values, which is
+// safe behind prefix_kernel alone, whose CTAs let it begin only once they have
+// themselves waited for whatever wrote those.  Every kernel waits before it ends,
+// so that a kernel's end always means the end of all before it.
 template <typename... KArgs, typename... Args>
 cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                        Args&&... args) {

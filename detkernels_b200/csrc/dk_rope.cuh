@@ -6,8 +6,8 @@
 //
 // with pairs (i, i + rd / 2), or (2i, 2i + 1) when interleaved, and cos/sin of the row's position
 // from an f32 table.  Everything stays in f32 until the one rounding of the store.  The sum of
-// squares of a vector has a fixed order (a lane's even and odd elements in order, then a butterfly), so a
-// row's bits do not depend on the other rows.
+// squares of a vector has a fixed order (a lane's elements in order, on the vector path even and odd ones apart, then
+// a butterfly), so a row's bits depend on the path, which the call's layout decides, and not on the other rows.
 //
 // Memory bound: every vector is read and written once.  A group of lanes owns a vector in 16-byte
 // chunks, lane l holding chunks l, l + L, l + 2L, ... with L = rd / 2 in chunks, so both elements of

@@ -4,7 +4,8 @@ Stands beside ``rmsnorm.py`` (the whole-row norm): every query and key head is
 normalised over its own head_dim, its first rotary_dim elements are rotated by
 the row's position, and, with a KV cache, the key and the value go straight to
 their slot.  f32 math with one rounding at the store; a row's bits depend on
-that row alone.  No counterpart in the reference (its decoder has neither,
+that row alone, and on which of two kernels the call's layout takes (their sums
+of squares differ in order).  No counterpart in the reference (its decoder has neither,
 tiny_model.py:99-140).
 """
 from __future__ import annotations
@@ -59,6 +60,11 @@ def qk_norm_rope(q, k, positions, q_weight, k_weight, table, eps: float = 1e-6, 
     value of each row are stored at its slot; a negative slot stores nothing.  k_out is then only written
     if given.  A position outside the table or a slot outside the cache sets the device status, and that
     row (or its K and V) is not written.  Rows of one call must not share a slot.
+
+    Two kernels, either batch invariant: vectors of 16 bytes where every tensor's rows and heads start on 16
+    bytes and the rotated half is a half or a quarter of the head in whole vectors (neighbouring pairs: any
+    rotary_dim of whole vectors); elements otherwise, for all of the call, also where only one tensor is
+    laid out so, and for some f32 heads beyond 256 elements.  Their results may differ in the last bit.
 
     Returns (q_out, k_out); k_out is None when the keys went to the cache only."""
     import torch

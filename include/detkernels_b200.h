@@ -381,7 +381,9 @@ int dk_paged_plan_padded(int32_t* block_table, int64_t block_table_stride, int32
  * negative slot stores nothing, one beyond the cache is recorded (DK_ERR_DEVICE_CHECK, detail 0x611) and
  * stores nothing; rows must not share a slot.  k_out may be NULL with a cache.  A position outside the table is recorded (0x610) and
  * its row not written.  head_dim <= 512; any dtype of the three for q/k/v/caches, and for the weights
- * [head_dim].  16-byte aligned vectors take the vector path. */
+ * [head_dim].  Calls whose every tensor has rows and heads on 16 bytes, and whose rotated half is a half or a quarter
+ * of the head in whole 16-byte vectors (neighbouring pairs: any rotary_dim of whole vectors, an even number of
+ * vectors a head), take the vector path; it and the other are each batch invariant, but sum squares in another order. */
 int dk_qk_norm_rope(const void* q, int64_t q_stride_row, int64_t q_stride_head, const void* k, int64_t k_stride_row,
                     int64_t k_stride_head, const void* v, int64_t v_stride_row, int64_t v_stride_head, void* q_out,
                     int64_t q_out_stride_row, int64_t q_out_stride_head, void* k_out, int64_t k_out_stride_row,
