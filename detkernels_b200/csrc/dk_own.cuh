@@ -2,7 +2,8 @@
 //
 // Fixed reduction structure: the row's tokens [0, len) in splits of kSplit = 64; inside a split
 // steps of 32 tokens (16 for head_dim 128) in order with an online softmax (m, l, O), scores from
-// mma.m16n8k16 (f32 accumulation), weights rounded to the input type for P.V and summed as rounded;
+// mma.m16n8k16 (f32 accumulation), weights rounded to the input type for P.V (the MMA takes 16-bit operands)
+// and summed as rounded, so that those of a row of few tokens still add up to one;
 // split states joined in order.  Nothing depends on the batch, the tile a row sits in or the schedule.
 //
 // Work: a unit is (row tile of at most 16 query rows of one sequence, KV head, run of splits), one

@@ -11,8 +11,9 @@
 //   * Inside a chunk, blocks of block_tokens(D) tokens in order: S from tcgen05.mma (f32 accumulation over D in
 //     16-deep steps), a reference maximum m that is raised only when a block's maximum exceeds it
 //     by more than 8 (a factor 256, so the weights stay in range of either 16-bit type), weights
-//     2^(S c - m) rounded to the input type for P.V as the left operand of a second tcgen05.mma in
-//     TMEM, l summed in f32 from the unrounded weights in a fixed order.
+//     2^(S c - m) rounded to the input type for P.V (the MMA takes 16-bit operands) as the left operand of a
+//     second tcgen05.mma in TMEM, l summed in f32 in a fixed order from the weights before that rounding, which
+//     keeps the sums beside the exponentials; over a block's many tokens the roundings average out.
 //   * The chunks' states are joined in order inside groups of group_chunks(D) chunks, the groups' states
 //     in order, and the states of the row's own tokens last.
 // No step looks at another row, so a row's bits do not depend on the batch.
@@ -21,7 +22,8 @@
 // One warp streams K and V blocks with TMA, one warp a tile issues its MMAs, and a warpgroup a tile does
 // the softmax, a row a thread.  The tiles share K and V.  TMEM holds, for either tile, the scores, the
 // weights and the accumulator apart, so that the next scores are formed as soon as these are in
-// registers and the softmax, which is bound by the exponential unit, does not wait for products: blocks of
+// registers and the softmax, whose chain of a block (load, maximum, exponentials) bounds the kernel, does not wait
+// for products (exponential unit 50 to 66 % busy, tensor pipe 49 to 32 %): blocks of
 // 128 tokens for head_dim <= 64, of 64 for 128 (whose accumulators take half of TMEM).  A run is a whole
 // group, whose chunks are joined on chip, or, when that leaves SMs idle, one chunk, whose state
 // combine_kernel joins; both give the same bits.  The joined accumulators of head_dim 128 need 128 KB: three
