@@ -77,7 +77,8 @@ def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=No
     pad: what lies past the step's own totals in the tensors of ``out`` becomes neutral: row_seq, row_pos
     and q_lens 0, slots -1 (``qk_norm_rope`` stores nothing there), tiles of 0 rows (attention skips them).
     A captured step that serves smaller ones needs it: without it those entries, an earlier step's slots and
-    tiles, stay as they are.  New tensors are always padded.
+    tiles, stay as they are.  New tensors are always padded.  (The matmul's fused store of K and V goes by
+    row_seq and row_pos and has no neutral rows: give it exact sizes.)
 
     A negative length, a sequence longer than its table row, an exhausted free list or more rows or tiles
     than announced sets the device status (``_lib.raise_on_device_error``) and leaves the table and all

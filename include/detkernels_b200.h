@@ -362,7 +362,8 @@ int dk_paged_plan(int32_t* block_table, int64_t block_table_stride, int32_t bloc
 
 /* The same plan for outputs whose sizes are bounds (a captured step that serves smaller ones): the entries past its
  * totals, and all of them when the plan is refused, become neutral for the operators below: row_seq, row_pos and
- * q_lens 0, slots -1 (nothing is stored there), tiles of 0 rows (attention skips them).  n_seqs = 0 writes nothing. */
+ * q_lens 0, slots -1 (nothing is stored there), tiles of 0 rows (attention skips them).  dk_matmul_epilogue's store into
+ * the cache goes by row_seq and row_pos and knows no such rows: it needs exact sizes.  n_seqs = 0 writes nothing. */
 int dk_paged_plan_padded(int32_t* block_table, int64_t block_table_stride, int32_t blocks_per_seq,
                          const int32_t* kv_lens, const int32_t* new_lens, int32_t n_seqs, int32_t page_size,
                          const int32_t* free_blocks, int64_t n_free, const int32_t* cursor, int32_t* cursor_out,
@@ -407,10 +408,11 @@ size_t dk_attention_shared_prefix_workspace_size(int32_t n_rows, int32_t n_tiles
  * The rows' own tokens: q, k, v, kv_lens, row_tiles, max_kv_len, scale as in
  * dk_attention_batch_invariant, or with block_table as in dk_attention_paged_batch_invariant
  * (kv_stride_seq is then the block stride); max_kv_len = 0: no row has any, and k, v and kv_lens are not
- * read.  A length beyond max_kv_len or the cache (detail 0x210), a malformed tile (0x211)
- * or a block id outside the pool (0x212) is recorded as DK_ERR_DEVICE_CHECK; the rows of a tile that is malformed
- * or holds such a length are left as they were in out, and so is a row that no tile covers.  Nothing beyond a row's
- * own length reaches it, whatever the cache holds there.  q must be 16-byte aligned with strides that are multiples of 8 elements.
+ * read.  A length beyond max_kv_len or the cache (detail 0x210), a malformed tile (0x211) or a block id outside
+ * the pool (0x212) is recorded as DK_ERR_DEVICE_CHECK; the rows of a tile that is malformed or holds such a
+ * length are left as they were in out, and so is a row that no tile covers.  Nothing beyond a row's own length
+ * reaches it, whatever the cache holds there.  q must be 16-byte aligned with strides that are multiples
+ * of 8 elements.
  * Batch invariant: a row's bits follow from its q, the prefix and its own tokens. */
 int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_stride_head, const void* k_prefix,
                                const void* v_prefix, int64_t prefix_stride_block, int64_t prefix_stride_head,

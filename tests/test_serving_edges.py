@@ -470,3 +470,47 @@ def test_a_small_plan_counts_the_one_launch_it_takes(dev):
     n0 = _lib.launch_count()
     paged_plan(_i32([[0]], dev), _i32([0], dev), _i32([1], dev), 64, n_rows=1)
     assert _lib.launch_count() - n0 == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("paged", [True, False])
+def test_caches_beyond_32_bit_offsets(dev, paged):
+    """Slots, pages, prefix blocks and whole sequences whose element offsets pass 2^32: the norm's stores, the own tokens'
+    and the prefix's reads are those of a small cache with the same contents."""
+    import torch
+
+    from detkernels_b200.kernels.attention import attention_shared_prefix
+    from detkernels_b200.kernels.rope import qk_norm_rope, rope_table
+    if torch.cuda.mem_get_info(dev)[0] < 40 << 30:
+        pytest.skip("needs 40 GB of free device memory")
+    H, Hkv, D, page = 8, 4, 128, 64
+    T = 3
+    n = 2 ** 32 // (Hkv * page * D) + 9
+    small = 12
+    g = torch.Generator(device=dev).manual_seed(1)
+    randn = lambda *s: torch.randn(*s, device=dev, generator=g).to(torch.bfloat16)
+    ks, vs = randn(small, Hkv, page, D), randn(small, Hkv, page, D)
+    kb, vb = (torch.empty(n, Hkv, page, D, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    far = torch.tensor([n - 1 - i * (n // 13) for i in range(small)], device=dev)   # where block i of the small one lies
+    kb[far], vb[far] = ks, vs
+    qkv = randn(T, (H + 2 * Hkv) * D)
+    q, k, v = (x.view(T, -1, D) for x in qkv.split([H * D, Hkv * D, Hkv * D], 1))
+    w, table, pos = randn(D), rope_table(300, D, device=dev), torch.arange(200, 200 + T, device=dev)
+    own = torch.tensor([0, 1, 2], device=dev)            # a block a row, its last token new
+    outs = []
+    for kc, vc, where in ((ks, vs, torch.arange(small, device=dev)), (kb, vb, far)):
+        slots = where[own] * page + page - 1
+        qr, _ = qk_norm_rope(q, k, pos, w, w, table, v=v, k_cache=kc, v_cache=vc, slots=slots)
+        ln = torch.full((T,), page, dtype=torch.int32, device=dev)
+        i32 = lambda x: x.to(torch.int32)
+        if paged:
+            outs.append(attention_shared_prefix(qr, kc, vc, kc, vc, ln, prefix_len=page * 9 - 5, prefix_blocks=i32(where[3:]),
+                                                block_table=i32(where[own][:, None])))
+        else:
+            kp, vp = (x.permute(1, 0, 2, 3)[:, where[3:]].reshape(Hkv, -1, D) for x in (kc, vc))
+            tiles = torch.stack([own, torch.ones_like(own), where[own]], 1).to(torch.int32)
+            outs.append(attention_shared_prefix(qr, kp, vp, kc, vc, ln, row_tiles=tiles))
+    assert torch.equal(kb[far], ks) and torch.equal(vb[far], vs)
+    assert torch.equal(*outs) and torch.isfinite(outs[0].float()).all()
+    del kb, vb
+    torch.cuda.empty_cache()
