@@ -285,12 +285,11 @@ __device__ __forceinline__ int describe_item(const Params& p, int64_t w, Item& i
   it.max_len = 0;
   it.nsplits = 0;
   it.s_begin = it.s_end = 0;
-  if (it.nr == 0) return 1;   // padding of a tile list
   const int rows_per_tile_max = kRows / p.G;
   // r0 against n_rows - nr: r0 + nr may leave 32 bits
   if (it.nr < 1 || it.nr > rows_per_tile_max || it.r0 < 0 || it.r0 > p.n_rows - it.nr || it.seq < 0 ||
       it.seq >= p.kv_n_seq || it.nr * p.G > p.rows_cap)
-    return 2;
+    return it.nr == 0 ? 1 : 2;   // (a tile of 0 rows is padding of a tile list)
   for (int i = 0; i < it.nr; ++i) {
     const int L = p.kv_lens ? p.kv_lens[it.r0 + i] : p.uniform_len;
     if (L < 0 || L > p.kv_capacity || L > p.max_splits * kSplit) return 3;
