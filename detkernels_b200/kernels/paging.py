@@ -160,3 +160,201 @@ def paged_plan(block_table, kv_lens, new_lens, page_size: int, *, free_blocks=No
     _lib.check(rc, "paged_plan")
     _lib.count_launch()   # at least: large steps take a second
     return plan
+
+
+class PagedCompact(NamedTuple):
+    lens: object                 # int32 [B]: tokens each sequence holds now
+    cursor: Optional[object]     # int32 [1]: free blocks handed out, without those that came back
+
+
+def paged_fork_reference(block_table, kv_lens, src, dst, page_size, *, free_blocks, cursor=0, shares=None):
+    """Plain Python form on host sequences (block_table a list of lists).  Returns (table, kv_lens, cursor, shares,
+    copies), copied lists, copies the (source block, new block, tokens) to copy in every pool."""
+    table, kv = [list(r) for r in block_table], list(kv_lens)
+    shares = None if shares is None else list(shares)
+    copies = []
+    for s, d in zip(src, dst):
+        for j in range(-(-kv[s] // page_size)):
+            if shares is not None and (j + 1) * page_size <= kv[s]:
+                table[d][j] = table[s][j]
+                shares[table[s][j]] += 1
+            else:
+                table[d][j] = free_blocks[cursor]
+                cursor += 1
+                copies.append((table[s][j], table[d][j], min(page_size, kv[s] - j * page_size)))
+        kv[d] = kv[s]
+    return table, kv, cursor, shares, copies
+
+
+def paged_compact_reference(block_table, kv_lens, new_lens, n_keep, page_size, *, keep=None, free_blocks=None, cursor=0,
+                            shares=None):
+    """Plain Python form on host sequences.  Returns (lens, cursor, free_blocks, shares, moves), copied lists, moves the
+    (block, token, new block, new token) of the tokens to move in every pool, to be done in order."""
+    free = None if free_blocks is None else list(free_blocks)
+    shares = None if shares is None else list(shares)
+    lens, moves, given = [], [], []
+    for b, (kv, new, nk) in enumerate(zip(kv_lens, new_lens, n_keep)):
+        for j in range(nk):
+            s, d = kv + (j if keep is None else keep[b][j]), kv + j
+            if s != d:
+                moves.append((block_table[b][s // page_size], s % page_size, block_table[b][d // page_size], d % page_size))
+        given += [block_table[b][j] for j in range(-(-(kv + nk) // page_size), -(-(kv + new) // page_size))]
+        lens.append(kv + nk)
+    if free is not None:
+        if shares is not None:
+            for x in given:
+                shares[x] -= 1
+            # a page without a holder goes back where the last one gave it up
+            given = [x for i, x in enumerate(given) if shares[x] < 0 and x not in given[i + 1:]]
+            for x in given:
+                shares[x] = 0
+        cursor -= len(given)
+        free[cursor:cursor + len(given)] = given
+    return lens, cursor, free, shares, moves
+
+
+def _check_pools(pools, dev, page_size, what):
+    """(pointer array, number, element strides by block, head and token, blocks, heads, head_dim, element size)."""
+    import ctypes
+    pools = list(pools)
+    if not pools:
+        return None, 0, (0, 0, 0), 0, 0, 0, 1
+    first = pools[0]
+    shape, stride, dtype = first.shape, first.stride(), first.dtype
+    for t in pools:
+        assert t.is_cuda and t.get_device() == dev.index, "%s requires CUDA tensors on one device" % what
+        if t.shape != shape or t.stride() != stride or t.dtype != dtype:
+            raise ValueError("%s: the pools must share shape, strides and dtype" % what)
+    assert len(shape) == 4 and shape[2] == page_size, "%s: pools must be [n_blocks, heads, page_size, head_dim]" % what
+    if shape[3] > 1 and stride[3] != 1:
+        raise ValueError("%s: unit stride along head_dim required" % what)
+    at = [t.data_ptr() for t in pools]
+    if len(set(at)) != len(at):
+        raise ValueError("%s: a pool is named twice" % what)
+    ptrs = (ctypes.c_void_p * len(pools))(*at)
+    return ptrs, len(pools), stride[:3], shape[0], shape[1], shape[3], first.element_size()
+
+
+def _check_books(block_table, kv_lens, page_size, free_blocks, cursor, shares, n_blocks, what):
+    """The table, the free list and the holders: (table stride, blocks that ids may name)."""
+    import torch
+    dev, i32 = block_table.device, torch.int32
+    assert block_table.is_cuda and kv_lens.get_device() == dev.index, "%s requires CUDA tensors on one device" % what
+    assert block_table.dtype == i32 and block_table.dim() == 2
+    assert block_table.shape[1] <= 1 or block_table.stride(1) == 1, "block_table: unit stride along a row"
+    assert kv_lens.dtype == i32 and kv_lens.dim() == 1, "%s: lengths must be int32 vectors" % what
+    if not 1 <= page_size < 2 ** 31:
+        raise ValueError("%s: page_size must be positive and below 2^31" % what)
+    if (free_blocks is None) != (cursor is None):
+        raise ValueError("%s: free_blocks and cursor go together" % what)
+    if free_blocks is not None:
+        assert free_blocks.dtype == i32 and free_blocks.get_device() == dev.index and free_blocks.is_contiguous()
+        assert free_blocks.dim() == 1 and cursor.dtype == i32 and cursor.get_device() == dev.index and cursor.numel() == 1
+    if shares is not None:
+        assert shares.dtype == i32 and shares.get_device() == dev.index and shares.is_contiguous() and shares.dim() == 1
+        if n_blocks and shares.numel() < n_blocks:
+            raise ValueError("%s: shares must have an entry a block" % what)
+        n_blocks = n_blocks or shares.numel()
+    return block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1], n_blocks or 2 ** 31 - 1
+
+
+def paged_fork(block_table, kv_lens, src, dst, page_size: int, *, free_blocks, cursor, pools=(), shares=None):
+    """Sequence dst[i] becomes a copy of sequence src[i]: several samples of one prompt, or the beams of a search.
+
+    block_table (int32 CUDA [n, blocks_per_seq]) and kv_lens (int32 CUDA [n], the tokens each row holds) are updated in
+    place; src, dst: int32 CUDA [F].  A source may be named several times, a destination once and not as a source; the
+    blocks that a destination held are not given back (``paged_compact`` does that).
+    shares (int32 CUDA [n_blocks]): how many further sequences hold a block beyond the first.  With it whole pages are
+    shared (shares[block] += 1), and only the last, open page gets a block of its own; without it every page does.  New
+    blocks are the next of free_blocks from cursor on (as for ``paged_plan``), in the order of the forks; returns the
+    new cursor (int32 CUDA [1]).
+    pools: the K and V pools of all layers ([n_blocks, heads, page_size, head_dim], any dtype, same strides), in which
+    the tokens of the new blocks are copied; what lies behind a sequence's last token is left as it was.
+
+    Rows outside the table or misnamed, a length outside its row, a block id outside the pools or too few free blocks set
+    the device status (``_lib.raise_on_device_error``), and nothing changes."""
+    import torch
+
+    what = "paged_fork"
+    dev = block_table.device
+    ptrs, n_pools, st, n_blocks, heads, dim, size = _check_pools(pools, dev, page_size, what)
+    if free_blocks is None or cursor is None:
+        raise ValueError("paged_fork: free_blocks and cursor are needed")
+    stride, n_blocks = _check_books(block_table, kv_lens, page_size, free_blocks, cursor, shares, n_blocks, what)
+    assert kv_lens.shape == (block_table.shape[0],) and kv_lens.is_contiguous(), "paged_fork: one length a table row"
+    assert src.dtype == torch.int32 and dst.dtype == torch.int32 and src.shape == dst.shape and src.dim() == 1
+    assert src.get_device() == dev.index and dst.get_device() == dev.index, "paged_fork requires CUDA tensors on one device"
+    with _lib.on_device(dev):
+        src, dst = src.contiguous(), dst.contiguous()
+        if src.numel() == 0 or block_table.shape[0] == 0:
+            if src.numel():
+                raise ValueError("paged_fork: the table has no rows")
+            return cursor.clone()
+        out = torch.empty_like(cursor)
+        lib = _lib.load()
+        ws = src.new_empty(-(-lib.dk_paged_fork_workspace_size(block_table.shape[0]) // 4))
+        rc = lib.dk_paged_fork(
+            block_table.data_ptr(), stride, block_table.shape[0], block_table.shape[1], kv_lens.data_ptr(), src.data_ptr(),
+            dst.data_ptr(), src.numel(), int(page_size), free_blocks.data_ptr() or ws.data_ptr(), free_blocks.numel(),
+            cursor.data_ptr(), out.data_ptr(), None if shares is None else shares.data_ptr(), n_blocks, ptrs, n_pools,
+            *st, heads, dim, size, ws.data_ptr(), 4 * ws.numel(), _lib.stream_ptr(dev))
+    _lib.check(rc, what)
+    _lib.count_launch(2 if n_pools else 1)
+    return out
+
+
+def paged_compact(block_table, kv_lens, new_lens, n_keep, page_size: int, *, keep=None, pools=(), free_blocks=None,
+                  cursor=None, shares=None) -> PagedCompact:
+    """Keep some of each sequence's last tokens, and give the pages back that then hold nothing.
+
+    Sequence b (row b of block_table, int32 CUDA [>= B, blocks_per_seq]) holds kv_lens[b] tokens and new_lens[b] behind
+    them, of which n_keep[b] stay (all int32 CUDA [B]): those at kv_lens[b] + keep[b, j], ascending (keep: int32 CUDA
+    [B, K], K at least the largest n_keep; what lies behind a row's n_keep is not read), or the first ones without
+    ``keep``.  They are moved to kv_lens[b] + j in all ``pools`` (as in ``paged_fork``): the accepted path of a tree
+    (``drafts.tree_accept``), or a cache thinned out.  kv_lens = 0 and n_keep = 0 free a sequence.
+    free_blocks (updated in place) and cursor: the pages behind a sequence's tokens go back before the cursor, in the order
+    of sequences and pages, and the new cursor, from which ``paged_plan`` and ``paged_fork`` take them again, is returned.  With shares (as in ``paged_fork``) a page with further holders loses one instead, and
+    one given up by all its holders goes back once.  Table entries stay as they are.  Tokens must not be moved inside a
+    page that another sequence shares; ``paged_fork`` leaves each sequence its open page to itself.
+
+    A negative length, more kept than held, a sequence beyond its table row, a ``keep`` that does not ascend inside the
+    new tokens, a block id outside the pools, more pages than were handed out or a page given up by more sequences than
+    hold it set the device status; then lens are kv_lens, the cursor stays, and nothing changes."""
+    import torch
+
+    what = "paged_compact"
+    dev = block_table.device
+    ptrs, n_pools, st, n_blocks, heads, dim, size = _check_pools(pools, dev, page_size, what)
+    stride, n_blocks = _check_books(block_table, kv_lens, page_size, free_blocks, cursor, shares, n_blocks, what)
+    if shares is not None and free_blocks is None:
+        raise ValueError("paged_compact: shares need a free list")
+    B = kv_lens.numel()
+    assert block_table.shape[0] >= B and new_lens.shape == (B,) and n_keep.shape == (B,), "paged_compact: [B] lengths"
+    for t in (new_lens, n_keep):
+        assert t.dtype == torch.int32 and t.get_device() == dev.index, "paged_compact: lengths must be int32 on one device"
+    if keep is not None:
+        assert keep.dtype == torch.int32 and keep.get_device() == dev.index and keep.dim() == 2 and keep.shape[0] == B
+        if keep.shape[1] > 1 and keep.stride(1) != 1:
+            keep = keep.contiguous()
+    with _lib.on_device(dev):
+        kv_lens, new_lens, n_keep = kv_lens.contiguous(), new_lens.contiguous(), n_keep.contiguous()
+        lens = torch.empty_like(kv_lens)
+        out = None if cursor is None else torch.empty_like(cursor)
+        if B == 0:
+            return PagedCompact(lens, None if cursor is None else cursor.clone())
+        lib = _lib.load()
+        ws = kv_lens.new_empty(-(-lib.dk_paged_compact_workspace_size() // 4))
+
+        def ptr(t):
+            # without entries nothing is followed, but it was given
+            return None if t is None else (t.data_ptr() or ws.data_ptr())
+
+        rc = lib.dk_paged_compact(
+            block_table.data_ptr(), stride, block_table.shape[1], kv_lens.data_ptr(), new_lens.data_ptr(),
+            n_keep.data_ptr(), ptr(keep), 0 if keep is None else keep.stride(0), 0 if keep is None else keep.shape[1], B,
+            int(page_size), lens.data_ptr(), ptr(free_blocks), 0 if free_blocks is None else free_blocks.numel(),
+            ptr(cursor), ptr(out), ptr(shares), n_blocks, ptrs, n_pools, *st, heads, dim, size, ws.data_ptr(),
+            4 * ws.numel(), _lib.stream_ptr(dev))
+    _lib.check(rc, what)
+    _lib.count_launch(2 if n_pools and keep is not None else 1)
+    return PagedCompact(lens, out)

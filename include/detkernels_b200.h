@@ -426,6 +426,72 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
                                int32_t n_kv_heads, int32_t head_dim, int32_t max_kv_len, float scale, int dtype,
                                void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Drafted tokens: log probabilities, the accepted path of a tree, pages forked, compacted and freed ----
+ * No counterparts in the reference (its decoder takes one token a step, greedily, into a cache that only grows:
+ * kernels/tiny_model.py:119-157). */
+
+/* Log probabilities of rows of logits [n_rows, n_vocab] (any of the three dtypes, element stride stride_row, unit
+ * stride along the vocabulary; rows need no alignment but their elements').
+ *  - tokens (device int64[n_rows], may be NULL): logprobs[r] = log softmax(row r)[tokens[r]]; a token of -1 asks for
+ *    nothing and gives 0, any other outside the vocabulary is recorded (DK_ERR_DEVICE_CHECK, detail 0x650) and gives NaN.
+ *  - entropy (may be NULL): -sum p log p in nats (a logit of -infinity has p = 0 and adds nothing).
+ *  - top_k <= 32 alternatives: top_ids [n_rows, top_k] int64 and their log probabilities, the largest logit first,
+ *    equal ones by their index (NaN is above all, -0 equals 0).
+ * f32 arithmetic.  A row with a NaN, +infinity or nothing but -infinity has NaN log probabilities and entropy.
+ * Batch invariant: a row's bits follow from its logits alone. */
+int dk_token_logprobs(const void* logits, int64_t stride_row, int64_t n_rows, int32_t n_vocab, int dtype,
+                      const int64_t* tokens, float* logprobs, float* entropy, int32_t top_k, int64_t* top_ids,
+                      float* top_logprobs, void* stream);
+
+/* The accepted path of each sequence's tree of drafted tokens.  Sequence b's nodes are the rows [cu_rows[b],
+ * cu_rows[b + 1]) of parents (index of the parent among the sequence's nodes, smaller than the node's own; -1: none),
+ * tokens and picked (the model's token after the node).  From node 0 the path goes to the first child whose token is
+ * the pick after the current node, at most max_keep nodes.  keep [n_seqs, max_keep]: its nodes in ascending order, -1
+ * behind them; n_keep [n_seqs]; next_tokens [n_seqs]: the pick after its last node.  A sequence without nodes has
+ * n_keep 0 and next_tokens -1, and so has one whose offsets do not ascend inside [0, n_rows], which is recorded
+ * (DK_ERR_DEVICE_CHECK, detail 0x660). */
+int dk_tree_accept(const int32_t* parents, const int64_t* tokens, const int64_t* picked, const int32_t* cu_rows,
+                   int32_t n_seqs, int32_t n_rows, int32_t max_keep, int32_t* keep, int32_t* n_keep,
+                   int64_t* next_tokens, void* stream);
+
+/* The pools of the next two calls: n_pools device pointers (an array on the host) to tensors [n_blocks, n_heads, page_size,
+ * head_dim] of elements of element_size bytes (1, 2, 4 or 8), all with the same element strides by block, head and token and unit
+ * stride along head_dim.  shares (device int32[n_blocks]): how many further sequences hold a block beyond the first.
+ * The free list: free_blocks[0, *cursor) are handed out, as for dk_paged_plan; cursor_out may be cursor. */
+size_t dk_paged_fork_workspace_size(int32_t table_rows);   /* uninitialised memory will do */
+/* Row dst[i] of block_table [table_rows][blocks_per_seq] becomes a copy of row src[i], kv_lens[dst[i]] =
+ * kv_lens[src[i]].  With shares, whole pages are shared (shares[block] += 1) and the last, open page gets the next
+ * free block; without, every page does.  The tokens of new blocks are copied in all pools.  The blocks that row dst
+ * held are not given back, its entries past the copied ones stay.  A source may be named several times; a destination
+ * once, and not as a source.  Recorded as DK_ERR_DEVICE_CHECK: rows outside the table or so misnamed (detail 0x640), a
+ * length outside its row (0x641), a block id outside [0, n_blocks) (0x642), too few free blocks (0x643); then nothing
+ * changes but the workspace, and *cursor_out = *cursor. */
+int dk_paged_fork(int32_t* block_table, int64_t block_table_stride, int32_t table_rows, int32_t blocks_per_seq,
+                  int32_t* kv_lens, const int32_t* src, const int32_t* dst, int32_t n_forks, int32_t page_size,
+                  const int32_t* free_blocks, int64_t n_free, const int32_t* cursor, int32_t* cursor_out,
+                  int32_t* shares, int64_t n_blocks, void* const* pools, int32_t n_pools, int64_t pool_stride_block,
+                  int64_t pool_stride_head, int64_t pool_stride_tok, int32_t n_heads, int32_t head_dim,
+                  int32_t element_size, void* workspace, size_t workspace_bytes, void* stream);
+
+size_t dk_paged_compact_workspace_size(void);              /* uninitialised memory will do */
+/* Sequence b holds kv_lens[b] tokens and new_lens[b] behind them, of which n_keep[b] stay: those at kv_lens[b] +
+ * keep[b][j], ascending (keep [n_seqs][keep_width], row stride keep_stride; NULL: the first n_keep[b]).  They are moved to
+ * kv_lens[b] + j in all pools, lens_out[b] = kv_lens[b] + n_keep[b] (lens_out is none of the inputs), and with
+ * free_blocks the pages [ceil(lens_out / page), ceil((kv + new) / page)) are given up: a page with shares loses one, any
+ * other goes back, free_blocks[*cursor_out, *cursor) in the order of (sequence, page), a page given up by all its
+ * holders in this call at the last of them.  Table entries stay.  kv_lens = 0 and n_keep = 0 free a whole sequence.
+ * Tokens must not be moved inside a page that another sequence shares: the pages from kv_lens[b] / page_size on are the
+ * sequence's own, as dk_paged_fork leaves them.  Recorded as DK_ERR_DEVICE_CHECK: bad lengths (detail 0x644), a bad row of
+ * keep (0x645), a block id outside [0, n_blocks) (0x642), more pages than were handed out (0x643), a page given up
+ * by more sequences than hold it (0x646); then lens_out = kv_lens, *cursor_out = *cursor, and nothing else changes. */
+int dk_paged_compact(const int32_t* block_table, int64_t block_table_stride, int32_t blocks_per_seq,
+                     const int32_t* kv_lens, const int32_t* new_lens, const int32_t* n_keep, const int32_t* keep,
+                     int64_t keep_stride, int32_t keep_width, int32_t n_seqs, int32_t page_size, int32_t* lens_out,
+                     int32_t* free_blocks, int64_t n_free, const int32_t* cursor, int32_t* cursor_out, int32_t* shares,
+                     int64_t n_blocks, void* const* pools, int32_t n_pools, int64_t pool_stride_block,
+                     int64_t pool_stride_head, int64_t pool_stride_tok, int32_t n_heads, int32_t head_dim,
+                     int32_t element_size, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
