@@ -1,5 +1,5 @@
-// C ABI of the operators for drafted tokens (see include/detkernels_b200.h): log probabilities of given tokens, the
-// accepted path of a tree, and forking, compacting and freeing the pages of a cache.
+// C ABI of the operators around drafted tokens (see include/detkernels_b200.h): log probabilities of given tokens, the
+// accepted path of a tree, and forking, compacting and freeing the pages of a cache.  (dk_tree.cu: their attention.)
 #include <algorithm>
 
 #include "dk_accept.cuh"

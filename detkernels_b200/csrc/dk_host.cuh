@@ -151,9 +151,10 @@ static inline cudaError_t unit_status(int clear, int* code, int* detail) {
   return e;
 }
 
-// Status words of dk_serving.cu and dk_drafts.cu (same contract as unit_status).
+// Status words of dk_serving.cu, dk_drafts.cu and dk_tree.cu (same contract as unit_status).
 cudaError_t serving_status(int clear, int* code, int* detail);
 cudaError_t drafts_status(int clear, int* code, int* detail);
+cudaError_t tree_status(int clear, int* code, int* detail);
 
 }  // namespace host
 }  // namespace dk

@@ -3,7 +3,7 @@
 // The kernels live in the dk_*.cuh headers; this file holds argument validation,
 // schedule selection and the extern "C" entry points of everything but the page
 // plan, the head norm with rotation and the shared-prefix attention
-// (dk_serving.cu), and the operators for drafted tokens (dk_drafts.cu).  Nothing here allocates device memory: scratch
+// (dk_serving.cu), and the operators for drafted tokens (dk_drafts.cu, dk_tree.cu).  Nothing here allocates device memory: scratch
 // space comes from the caller's workspace.
 #include "dk_common.cuh"
 #include "dk_host.cuh"
@@ -657,17 +657,14 @@ int dk_device_status(int device, int clear, int* code, int* detail) {
   if (cudaSetDevice(device) != cudaSuccess) return fail(DK_ERR_INVALID_ARGUMENT, "dk_device_status: bad device");
   int c = 0, d = 0;
   cudaError_t e = cudaDeviceSynchronize();
-  int c2 = 0, d2 = 0;
   if (e == cudaSuccess) e = unit_status(clear, &c, &d);
-  if (e == cudaSuccess) e = serving_status(clear, &c2, &d2);
-  if (c == DK_OK) {
-    c = c2;
-    d = d2;
-  }
-  if (e == cudaSuccess) e = drafts_status(clear, &c2, &d2);
-  if (c == DK_OK) {
-    c = c2;
-    d = d2;
+  for (auto unit : {serving_status, drafts_status, tree_status}) {
+    int c2 = 0, d2 = 0;
+    if (e == cudaSuccess) e = unit(clear, &c2, &d2);
+    if (c == DK_OK) {
+      c = c2;
+      d = d2;
+    }
   }
   cudaSetDevice(prev);
   if (e != cudaSuccess) return fail(DK_ERR_CUDA, "dk_device_status: %s", cudaGetErrorString(e));

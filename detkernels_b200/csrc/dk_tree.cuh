@@ -1,0 +1,829 @@
+// Attention of drafted tokens: the rows of a sequence are the nodes of a tree (or any other set) of drafts whose keys
+// and values lie behind the sequence's kv cached tokens; a row sees all of those, and of the drafts the ones that its
+// mask names.
+//
+// The query heads of all of a sequence's rows on KV head h are the rows of one matrix Q [t G, D], so that the cache is
+// read once for the whole tree: S = Q K^T scale, out = softmax(S + mask) V.  Fixed reduction structure (the definition of
+// a row's bits): the sequence's tokens are cut into chunks whose size follows kv and head_dim only (prefix::chunk_tokens), a
+// chunk's softmax state (m, l, O) is formed block by block as in dk_prefix.cuh, and the chunks' states are joined in
+// order.  No step looks at another row: a chunk of which a row sees nothing joins with weight 0.
+//
+// Work: an item is (sequence, chunk, up to two tiles of 128 rows): two tiles of one KV head, which then share K and V, or,
+// where the rows fit one tile, the tiles of two KV heads, each with its own K and V.  Either way both softmax
+// warpgroups have work, and take turns on the exponential unit.  One persistent CTA an SM: a TMA warp, an MMA warp a
+// tile (scores, weights and accumulator apart in TMEM), a warpgroup a tile for the softmax, a row a thread, and a
+// warp that makes the values of draft blocks safe: 0 weights must meet neither what lies behind the sequence in its last
+// page nor a non-finite value of a draft that some rows do not see.  Those elements become 0 in shared memory, and rows
+// that do see them have them added back from the cache (which no ordinary call does).
+#pragma once
+
+#include "dk_common.cuh"
+#include "dk_divide.cuh"
+#include "dk_prefix.cuh"
+
+namespace dk {
+namespace tree {
+
+using own::exp2_hw;
+using own::join;
+using own::join4;
+using own::join_weights;
+using own::pack2;
+using prefix::add2;
+using prefix::fma2;
+using prefix::kRows;
+using prefix::kSoftWarps;
+using prefix::warp_wait;
+
+constexpr int kThreads = prefix::kThreads;   // softmax warps, then TMA, two for MMA, and the one that cleans values
+
+enum : int {
+  kDetEmpty = 0x670,
+  kDetFull = 0x671,
+  kDetScores = 0x672,
+  kDetProbs = 0x673,
+  kDetOut = 0x674,
+  kDetQ = 0x675,
+  kDetOutFree = 0x676,
+  kDetDrain = 0x677,
+  kDetDone = 0x678,
+  kDetScoresFree = 0x679,
+  kDetPage = 0x67a,   // a block id outside the pool
+  kDetTurn = 0x67b,
+  kDetRaw = 0x67c,
+  kDetLens = 0x67d,   // a negative length, rows that do not ascend or exceed their bound, or tokens beyond the cache
+};
+
+struct Params {
+  const void* q;
+  int64_t q_sr, q_sh;
+  int32_t hkv, G;
+  Divisor31 group;          // by G
+  int32_t n_seqs, n_rows, max_rows;
+  const int32_t* kv_lens;
+  const int32_t* cu_rows;
+  const uint64_t* mask;     // [n_rows][words]
+  int64_t mask_stride;
+  int32_t words;
+  int32_t capacity;         // tokens a sequence may have, drafts included
+  int32_t units;            // items a (sequence, chunk), at most
+  int32_t max_chunks;
+  const void* v;            // for what is added back
+  int64_t c_sn, c_sh, c_st;
+  const int32_t* table;     // null: contiguous
+  int64_t table_stride;
+  int32_t page, n_blocks;
+  float c;                  // |scale| * log2(e)
+  uint32_t flip;            // sign mask for q (0x80008000 when scale < 0)
+  int zero;                 // scale is 0
+  void* out;
+  int64_t o_sr, o_sh;
+  int o_vec;                // out takes 16-byte stores
+  float* st_o;              // [max_chunks][D / 4][st_rows][4]
+  float* st_ml;             // [max_chunks][st_rows][2]
+  int64_t st_rows;          // hkv * n_rows * G: state row kvh * n_rows * G + row * G + head in the group
+};
+
+template <int D>
+struct Cfg {
+  static constexpr int DP = D < 64 ? 64 : D;
+  static constexpr int NH = DP / 64;
+  static constexpr int BLK = prefix::block_tokens(D);
+  static constexpr int BOX = 64 * 128;
+  static constexpr int HALF = BLK / 64 * BOX;
+  static constexpr int STAGE = NH * HALF;         // 16 KB
+  static constexpr int STAGES = D == 128 ? 8 : 10;
+  static constexpr int QHALF = kRows * 128;
+  static constexpr int QTILE = NH * QHALF;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * QTILE + 512;
+  static constexpr uint32_t S_COL = 0, P_COL = 2 * BLK, O_COL = 512 - 2 * DP;
+  static_assert(P_COL + BLK <= O_COL, "TMEM");
+};
+
+// A sequence's extents; nothing (rows = 0) where they are bad.
+struct Seq {
+  int row0, rows, kv, total, chunk, n_chunks;
+};
+// WARP: called by a whole converged warp; what is loaded is then one value for it as the compiler sees it, too (the MMA
+// issuers' operands stay in uniform registers).
+template <int D, bool WARP>
+__device__ __forceinline__ Seq seq_at(const Params& p, int b, bool report) {
+  Seq s;
+  s.row0 = p.cu_rows[b];
+  int r1 = p.cu_rows[b + 1];
+  s.kv = p.kv_lens[b];
+  if (WARP) {
+    s.row0 = __shfl_sync(0xffffffffu, s.row0, 0);
+    r1 = __shfl_sync(0xffffffffu, r1, 0);
+    s.kv = __shfl_sync(0xffffffffu, s.kv, 0);
+  }
+  s.rows = r1 - s.row0;
+  const bool bad = s.row0 < 0 || r1 < s.row0 || r1 > p.n_rows || s.rows > p.max_rows ||
+                   (s.rows > 0 && (s.kv < 0 || s.kv > p.capacity - s.rows));
+  if (bad && report) report_error(DK_ERR_DEVICE_CHECK, kDetLens);
+  if (bad || s.rows == 0) {
+    s.rows = s.total = s.n_chunks = s.kv = 0;
+    s.chunk = 1;
+    return s;
+  }
+  s.total = s.kv + s.rows;
+  s.chunk = static_cast<int>(prefix::chunk_tokens(s.kv, D));
+  s.n_chunks = (s.total + s.chunk - 1) / s.chunk;
+  return s;
+}
+
+struct Item {
+  Seq s;
+  int b, chunk;              // sequence; chunk of it
+  int kvh, m0;               // of tile 0
+  int tiles, streams;        // tiles with work; K/V streams (2: tile 1 is the next KV head)
+  int t_begin, tokens, n_blocks;   // n_blocks = 0: no work
+};
+template <int D, bool WARP>
+__device__ __forceinline__ Item item_at(const Params& p, uint32_t w, bool report) {
+  constexpr int BLK = Cfg<D>::BLK;
+  Item it;
+  const uint32_t r = w / static_cast<uint32_t>(p.units);
+  const int u = static_cast<int>(w - r * p.units);
+  it.chunk = static_cast<int>(r / static_cast<uint32_t>(p.n_seqs));
+  it.b = static_cast<int>(r - it.chunk * static_cast<uint32_t>(p.n_seqs));
+  it.s = seq_at<D, WARP>(p, it.b, report && u == 0 && it.chunk == 0);
+  it.n_blocks = 0;
+  if (it.chunk >= it.s.n_chunks) return it;
+  const int mg = it.s.rows * p.G, nt = (mg + kRows - 1) / kRows;
+  if (nt > 1) {
+    const int pairs = (nt + 1) >> 1;
+    it.kvh = u / pairs;
+    const int pair = u - it.kvh * pairs;
+    it.m0 = pair * 2 * kRows;
+    it.tiles = it.m0 + kRows < mg ? 2 : 1;
+    it.streams = 1;
+  } else {
+    it.kvh = 2 * u;
+    it.m0 = 0;
+    it.tiles = it.streams = it.kvh + 1 < p.hkv ? 2 : 1;
+  }
+  if (it.kvh >= p.hkv) return it;
+  it.t_begin = it.chunk * it.s.chunk;
+  it.tokens = min(it.s.total - it.t_begin, it.s.chunk);
+  it.n_blocks = (it.tokens + BLK - 1) / BLK;
+  return it;
+}
+
+// A whole warp's wait for fill f of a ring of N stages, whose barriers complete once a lap.  A parity tells a lap only from
+// its neighbours, so whoever waits must know that fill f - N has landed: the number of stages is even, as is that of an
+// item's fills, so fill f - N was this tile's own, or shared, and either way its issuer has waited for it (a tile without
+// work in a shared item waits all the same).  Nor can the barrier be ahead: f is not released before this tile has met it.
+template <int N>
+__device__ __forceinline__ bool wait_fill(uint64_t* full, uint32_t f, bool& abort_flag) {
+  static_assert(N % 2 == 0, "stages");
+  return warp_wait(&full[f % N], (f / N) & 1, kDetFull, abort_flag);
+}
+
+// Which of the 64 tokens from p0 on a row sees.
+__device__ __forceinline__ uint64_t sees64(const Params& p, const Seq& s, const uint64_t* row, int p0) {
+  if (p0 >= s.total) return 0;
+  const int off = p0 - s.kv;
+  uint64_t bits;
+  if (off <= -64) {
+    bits = ~0ull;
+  } else if (off < 0) {
+    bits = (row[0] << -off) | ((1ull << -off) - 1);
+  } else {
+    const int w = off >> 6, sh = off & 63;
+    bits = w < p.words ? row[w] >> sh : 0;
+    if (sh && w + 1 < p.words) bits |= row[w + 1] << (64 - sh);
+  }
+  const int left = s.total - p0;
+  return left < 64 ? bits & ((1ull << left) - 1) : bits;
+}
+// A row that sees nothing at all (asked only where the weights sum up to 0).
+__device__ __forceinline__ bool sees_nothing(const Params& p, const Seq& s, const uint64_t* row) {
+  if (s.kv > 0) return false;
+#pragma unroll 1
+  for (int p0 = 0; p0 < s.total; p0 += 64)
+    if (sees64(p, s, row, p0)) return false;
+  return true;
+}
+
+__device__ __forceinline__ bool wild16(uint32_t u, uint32_t expo) {
+  return (u & expo) == expo || ((u >> 16) & expo) == expo;
+}
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t expo_bits() {
+  return std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+}
+// The word without its non-finite halves.
+__device__ __forceinline__ uint32_t tamed(uint32_t u, uint32_t expo) {
+  if ((u & expo) == expo) u &= 0xffff0000u;
+  if (((u >> 16) & expo) == expo) u &= 0xffffu;
+  return u;
+}
+
+// The non-finite values of the drafts of this chunk that the row sees, added to 32 columns of its accumulator.  (Inlined, as
+// all of the kernel is: with a function call in it the two register budgets of its warps would not hold.)
+template <typename T>
+__device__ __forceinline__ void add_back(const Params& p, const Seq& s, const uint64_t* row, int b, int kvh, int begin, int end,
+                                         int col, float (&o)[32]) {
+#pragma unroll 1
+  for (int t = max(begin, s.kv); t < end; ++t) {
+    if (!(sees64(p, s, row, t) & 1)) continue;
+    int64_t at = b;
+    int tok = t;
+    if (p.table) {
+      const int pg = t / p.page;
+      at = p.table[b * p.table_stride + pg];
+      if (at < 0 || at >= p.n_blocks) at = 0;
+      tok -= pg * p.page;
+    }
+    const T* v = static_cast<const T*>(p.v) + at * p.c_sn + kvh * p.c_sh + tok * p.c_st + col;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float x = to_f32<T>(v[i]);
+      if (!(fabsf(x) < INFINITY)) o[i] += x;
+    }
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ prefix::Maps maps,
+                                                              const __grid_constant__ Params p) {
+  using C = Cfg<D>;
+  constexpr int BLK = C::BLK;
+  constexpr uint32_t FMT = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = base;
+  uint8_t* s_q = ring + C::STAGES * C::STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_q + 2 * C::QTILE);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* raw = empty + C::STAGES;      // values landed that are still to be cleaned
+  uint64_t* s_full = raw + C::STAGES;     // [2] by tile: scores formed
+  uint64_t* s_free = s_full + 2;          // [2] by tile: scores in registers
+  uint64_t* p_ready = s_free + 2;         // [2] by tile: weights in TMEM
+  uint64_t* o_full = p_ready + 2;         // [2] by tile: P.V of a block done
+  uint64_t* o_free = o_full + 2;          // [2] by tile: the accumulator has been read
+  uint64_t* q_ready = o_free + 2;         // [2] by tile
+  uint64_t* turn = q_ready + 2;           // [8] by softmax warp: the exponential unit is its
+  uint64_t* done = turn + kSoftWarps;     // [2]
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(done + 2);
+  uint32_t* s_wild = s_tmem + 1;          // by stage: its values had non-finite elements
+  static_assert((3 * C::STAGES + 12 + kSoftWarps + 2) * 8 + 4 + 4 * C::STAGES <= 512, "barriers");
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 2);   // both MMA issuers, or the one whose stage it is twice
+      mbar_init(&raw[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&s_free[t], 128);
+      mbar_init(&p_ready[t], 128);
+      mbar_init(&o_full[t], 1);
+      mbar_init(&o_free[t], 128);
+      mbar_init(&q_ready[t], 128);
+    }
+    for (int i = 0; i < kSoftWarps; ++i) mbar_init(&turn[i], 1);
+    mbar_init(&done[0], 1);
+    mbar_init(&done[1], 1);
+    fence_mbar_init();
+  }
+  if (warp == kSoftWarps && lane == 0) {
+    tma_prefetch_desc(&maps.k);
+    tma_prefetch_desc(&maps.v);
+  }
+  if (warp == kSoftWarps + 1) {
+    tmem_alloc(s_tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+
+  const uint32_t n_items = static_cast<uint32_t>(p.units) * p.n_seqs * p.max_chunks;   // < 2^31 (the host checks)
+  bool abort_flag = false;
+  // Stages of an item's block b: K of stream i in fill f0 + 2 streams b + i, V behind the K's of the block.
+  // A block that holds drafts has its values cleaned.
+  auto has_drafts = [](const Item& it, int b) { return it.t_begin + (b + 1) * BLK > it.s.kv; };
+
+  if (warp >= kSoftWarps) {
+    prefix::reg_dec<prefix::kIoRegs>();
+    if (warp == kSoftWarps && lane == 0) {
+      // ---------------- TMA producer ----------------
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t fills = 0;
+      for (uint32_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
+        const Item it = item_at<D, false>(p, w, true);
+        for (int b = 0; b < it.n_blocks && !abort_flag; ++b) {
+          int tok[BLK / 64], slab[BLK / 64], boxes = 0;   // 64-token boxes that hold a token
+#pragma unroll
+          for (int h = 0; h < BLK / 64; ++h) {
+            tok[h] = it.t_begin + b * BLK + 64 * h;
+            slab[h] = it.b;
+            if (b * BLK + 64 * h >= it.tokens) continue;
+            boxes = h + 1;
+            if (p.table) {   // a page holds whole boxes
+              const int pg = tok[h] / p.page;
+              tok[h] -= pg * p.page;
+              slab[h] = p.table[it.b * p.table_stride + pg];
+              if (slab[h] < 0 || slab[h] >= p.n_blocks) {
+                report_error(DK_ERR_DEVICE_CHECK, kDetPage);
+                slab[h] = 0;
+              }
+            }
+          }
+          const bool clean = has_drafts(it, b);
+          for (int e = 0; e < 2 * it.streams; ++e) {
+            const bool val = e >= it.streams;
+            const int kvh = it.kvh + (val ? e - it.streams : e);
+            if (!mbar_wait(&empty[stage], phase ^ 1u, kDetEmpty, abort_flag)) break;
+            uint8_t* st = ring + stage * C::STAGE;
+            uint64_t* bar = val && clean ? &raw[stage] : &full[stage];
+            mbar_arrive_expect_tx(bar, boxes * C::NH * C::BOX);
+#pragma unroll
+            for (int h = 0; h < BLK / 64; ++h)
+#pragma unroll
+              for (int n = 0; n < C::NH; ++n)
+                if (h < boxes)
+                  tma_load_4d(st + n * C::HALF + h * C::BOX, val ? &maps.v : &maps.k, bar, n * 64, tok[h], kvh, slab[h]);
+            ++fills;
+            if (++stage == C::STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+        }
+      }
+      // every copy has landed before the CTA may end (a cleaned stage's barrier completes behind its copies)
+      bool drain = false;
+      for (uint32_t f = (fills > C::STAGES ? fills - C::STAGES : 0); f < fills; ++f)
+        mbar_wait(&full[f % C::STAGES], static_cast<uint32_t>((f / C::STAGES) & 1), kDetDrain, drain);
+    } else if (warp == kSoftWarps + 1 || warp == kSoftWarps + 2) {
+      // ---------------- MMA issuers, one a tile ----------------
+      const int t = warp - (kSoftWarps + 1);
+      constexpr uint32_t idesc_s = umma_idesc_f16(FMT, 0, 0, kRows, BLK);
+      constexpr uint32_t idesc_o = umma_idesc_f16(FMT, 0, 1, kRows, C::DP);
+      const uint64_t k_desc = umma_sdesc(smem_u32(ring), 16, 1024, 2);
+      const uint64_t v_desc = umma_sdesc(smem_u32(ring), C::HALF, 1024, 2);
+      const uint64_t q_desc = umma_sdesc(smem_u32(s_q) + t * C::QTILE, 16, 1024, 2);
+      const uint32_t s_col = tmem + C::S_COL + t * BLK, p_col = tmem + C::P_COL + t * (BLK / 2);
+      const uint32_t o_col = tmem + C::O_COL + t * C::DP;
+      const bool leader = prefix::elect_one();
+      uint32_t fill = 0;
+      uint32_t qph = 0, sph = 0, pph = 0;    // q_ready, s_free, p_ready parities
+      uint32_t oph = 1;                      // o_free parity (the first wait passes)
+      bool mine = false;                     // the item's tiles have stages of their own
+      auto landed = [&](uint32_t f) { return wait_fill<C::STAGES>(full, f, abort_flag); };
+      auto release = [&](uint32_t f) {
+        tc_commit(&empty[f % C::STAGES]);
+        if (mine) tc_commit(&empty[f % C::STAGES]);
+      };
+      auto issue_qk = [&](uint32_t f) {      // scores from the K block of fill f
+        if (leader) {
+          const uint64_t kd = k_desc + static_cast<uint64_t>((f % C::STAGES) * (C::STAGE / 16));
+#pragma unroll
+          for (int j = 0; j < C::DP / 16; ++j)
+            tc_mma_f16(s_col, q_desc + static_cast<uint64_t>(((j >> 2) * C::QHALF + (j & 3) * 32) / 16),
+                       kd + static_cast<uint64_t>(((j >> 2) * C::HALF + (j & 3) * 32) / 16), idesc_s, j > 0 ? 1u : 0u);
+          tc_commit(&s_full[t]);
+          release(f);
+        }
+        __syncwarp();
+      };
+      for (uint32_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
+        const Item it = item_at<D, true>(p, w, false);
+        const int nb = it.n_blocks;
+        if (nb == 0) continue;
+        const uint32_t per = 2 * it.streams;
+        const uint32_t f0 = fill + (it.streams == 2 ? t : 0);   // K of block b: f0 + per b; V: streams further
+        fill += per * nb;
+        mine = it.streams == 2;
+        if (t >= it.tiles) {
+          // not this tile's item: its stages still need this warp's release, in order
+          for (uint32_t f = f0; f != fill; ++f) {
+            if (!landed(f)) break;
+            if (leader) mbar_arrive(&empty[f % C::STAGES]);
+          }
+          continue;
+        }
+        if (!warp_wait(&q_ready[t], qph, kDetQ, abort_flag)) break;
+        qph ^= 1u;
+        if (!landed(f0)) break;
+        tc_fence_after();
+        issue_qk(f0);
+        for (int b = 0; b < nb; ++b) {
+          const bool more = b + 1 < nb;
+          const uint32_t fv = f0 + per * b + it.streams, fk = f0 + per * (b + 1);
+          // the next scores, as soon as these are in registers (the last block's release is for the next item)
+          if (more && !landed(fk)) break;
+          if (!warp_wait(&s_free[t], sph, kDetScoresFree, abort_flag)) break;
+          sph ^= 1u;
+          tc_fence_after();
+          if (more) issue_qk(fk);
+          if (!landed(fv)) break;
+          const int valid = min(BLK, it.tokens - b * BLK);
+          const int steps = (valid + 15) >> 4;   // 16-token steps of P.V that hold a token
+          if (b == 0) {
+            if (!warp_wait(&o_free[t], oph, kDetOutFree, abort_flag)) break;
+            oph ^= 1u;
+          }
+          if (!warp_wait(&p_ready[t], pph, kDetProbs, abort_flag)) break;
+          pph ^= 1u;
+          tc_fence_after();
+          if (leader) {
+            const uint64_t vd = v_desc + static_cast<uint64_t>((fv % C::STAGES) * (C::STAGE / 16));
+#pragma unroll
+            for (int j = 0; j < BLK / 16; ++j)
+              if (j < steps)
+                prefix::mma_ts(o_col, p_col + j * 8, vd + static_cast<uint64_t>(j * (2048 / 16)), idesc_o,
+                               (b == 0 && j == 0) ? 0u : 1u);
+            tc_commit(&o_full[t]);
+            release(fv);
+          }
+          __syncwarp();
+        }
+      }
+      // all issued MMAs are complete before TMEM is freed
+      if (leader) tc_commit(&done[t]);
+      __syncwarp();
+      bool fin = false;
+      warp_wait(&done[t], 0, kDetDone, fin);
+    } else if (warp == kSoftWarps + 3) {
+      // ---------------- values of draft blocks ----------------
+      constexpr uint32_t expo = expo_bits<T>();
+      uint32_t fill = 0;
+      uint32_t seen = 0;                     // raw parities, a bit a stage
+      for (uint32_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
+        const Item it = item_at<D, true>(p, w, false);
+        if (it.n_blocks == 0) continue;
+        const uint32_t per = 2 * it.streams, f0 = fill;
+        fill += per * it.n_blocks;
+        const int first = max(0, (it.s.kv - it.t_begin) / BLK);   // the first block with drafts, if any
+        for (int b = first; b < it.n_blocks && !abort_flag; ++b) {
+          if (!has_drafts(it, b)) continue;
+          for (int i = 0; i < it.streams; ++i) {
+            const uint32_t f = f0 + per * b + it.streams + i, stage = f % C::STAGES;
+            if (!warp_wait(&raw[stage], (seen >> stage) & 1u, kDetRaw, abort_flag)) break;
+            seen ^= 1u << stage;
+            uint8_t* vb = ring + stage * C::STAGE;
+            const int begin = max(0, it.s.kv - it.t_begin - b * BLK);    // rows of the block
+            const int valid = min(BLK, it.tokens - b * BLK), end = (valid + 15) & ~15;
+            bool wild = false;
+            for (int e = lane; e < (end - begin) * C::NH * 8; e += 32) {
+              const int r = begin + e / (C::NH * 8), c = e % (C::NH * 8);
+              uint4* at = reinterpret_cast<uint4*>(vb + (c >> 3) * C::HALF + r * 128 + (c & 7) * 16);
+              if (r >= valid) {
+                *at = make_uint4(0, 0, 0, 0);
+                continue;
+              }
+              const uint4 v = *at;
+              if (wild16(v.x, expo) || wild16(v.y, expo) || wild16(v.z, expo) || wild16(v.w, expo)) {
+                wild = true;
+                *at = make_uint4(tamed(v.x, expo), tamed(v.y, expo), tamed(v.z, expo), tamed(v.w, expo));
+              }
+            }
+            wild = __any_sync(0xffffffffu, wild);
+            if (lane == 0) s_wild[stage] = wild ? 1u : 0u;
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[stage]);
+          }
+        }
+      }
+    }
+  } else {
+    // ---------------- softmax: one row a thread ----------------
+    prefix::reg_inc<prefix::kSoftRegs>();
+    const int t = warp >> 2;                    // tile of the item
+    const int r = threadIdx.x & 127;            // row of the tile
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t o_t = tmem + lane_base + C::O_COL + t * C::DP;
+    const uint32_t s_t = tmem + lane_base + C::S_COL + t * BLK, p_t = tmem + lane_base + C::P_COL + t * (BLK / 2);
+    uint32_t sph = 0;                           // s_full parity
+    uint32_t tph = t ^ 1;                       // turn parity (tile 0 goes first)
+    uint32_t ocnt = 0;                          // blocks of this tile whose weights are handed over
+    uint32_t oseen = 0;                         // of them, those whose P.V this warp has waited for
+    uint32_t fill = 0;
+    // All P.V so far are done; each warp takes every phase of o_full once and in order (see dk_prefix.cuh).
+    auto pv_done = [&]() {
+      if (oseen == ocnt) return true;
+      const bool ok = warp_wait(&o_full[t], oseen & 1, kDetOut, abort_flag);
+      tc_fence_after();
+      oseen = ocnt;
+      return ok;
+    };
+    // The tile's query rows into the swizzled K-major operand tile, asynchronously ...
+    constexpr int CPR = C::DP / 8;              // 16-byte chunks a row
+    constexpr int QN = kRows * CPR / 128;       // chunks a thread
+    auto q_at = [&](int i) {
+      const int e = i * 128 + r, row = e / CPR, c = e % CPR;
+      return s_q + t * C::QTILE + (c >> 3) * C::QHALF + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+    };
+    auto fetch_q = [&](const Item& it) {
+      const int kvh = it.kvh + (it.streams == 2 ? t : 0), m0 = it.m0 + (it.streams == 1 ? t * kRows : 0);
+#pragma unroll 4
+      for (int i = 0; i < QN; ++i) {
+        const int e = i * 128 + r, c = e % CPR;
+        const uint32_t mrow = m0 + e / CPR;
+        const bool valid = mrow < static_cast<uint32_t>(it.s.rows * p.G) && c < D / 8;
+        const uint32_t row = valid ? div_by(mrow, p.group) : 0, gh = valid ? mrow - row * p.G : 0;
+        own::cp_async16(smem_u32(q_at(i)),
+                        static_cast<const T*>(p.q) + (valid ? (it.s.row0 + row) * p.q_sr + (kvh * p.G + gh) * p.q_sh + c * 8 : 0),
+                        valid);
+      }
+    };
+    // ... and, once there, handed to the tensor cores.
+    auto q_here = [&]() {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if (p.flip | p.zero) {
+#pragma unroll 1
+        for (int i = 0; i < QN; ++i) {
+          uint4* at = reinterpret_cast<uint4*>(q_at(i));
+          uint4 v = *at;
+          v.x ^= p.flip;
+          v.y ^= p.flip;
+          v.z ^= p.flip;
+          v.w ^= p.flip;
+          *at = p.zero ? prefix::times_zero<T>(v) : v;
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&q_ready[t]);
+    };
+    bool q_loaded = false;
+    for (uint32_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
+      const Item it = item_at<D, true>(p, w, false);
+      if (it.n_blocks == 0) continue;
+      const uint32_t per = 2 * it.streams;
+      const uint32_t fv0 = fill + it.streams + (it.streams == 2 ? t : 0);   // V of block b: fv0 + per b
+      fill += per * it.n_blocks;
+      if (t >= it.tiles) continue;
+      const int kvh = it.kvh + (it.streams == 2 ? t : 0), m0 = it.m0 + (it.streams == 1 ? t * kRows : 0);
+      const int mg = it.s.rows * p.G, mrow = m0 + r;
+      const bool valid_row = mrow < mg;
+      const bool warp_live = m0 + (warp & 3) * 32 < mg;
+      const int row = it.s.row0 + (valid_row ? static_cast<int>(div_by(static_cast<uint32_t>(mrow), p.group)) : 0);
+      const uint64_t* mask = p.mask + row * p.mask_stride;
+      if (!q_loaded) {   // the CTA's first item with this tile; later ones are fetched ahead
+        fetch_q(it);
+        q_here();
+      }
+      q_loaded = false;
+      float m = -INFINITY, l = 0.0f;
+      bool wild = false;
+      for (int b = 0; b < it.n_blocks; ++b) {
+        const bool first = b == 0, last = b + 1 == it.n_blocks;
+        const bool drafts = has_drafts(it, b);
+        uint64_t sees[BLK / 64];
+        if (drafts) {
+#pragma unroll
+          for (int h = 0; h < BLK / 64; ++h)
+            sees[h] = valid_row ? sees64(p, it.s, mask, it.t_begin + b * BLK + 64 * h) : 0;
+        }
+        if (!warp_wait(&s_full[t], sph, kDetScores, abort_flag)) break;
+        sph ^= 1u;
+        tc_fence_after();
+        if (last) {   // all scores of this item are formed: q's place is free for the next one with this tile
+          for (uint32_t wn = w + gridDim.x; wn < n_items && !q_loaded; wn += gridDim.x) {
+            const Item next = item_at<D, true>(p, wn, false);
+            if (next.n_blocks > 0 && t < next.tiles) {
+              fetch_q(next);
+              q_loaded = true;
+            }
+          }
+        }
+        __syncwarp();
+        if (warp_live) {
+          constexpr int NR = BLK / 32;
+          float s[NR][32];
+#pragma unroll
+          for (int c = 0; c < NR; ++c) tmem_ld_32x32b_x32(s_t + c * 32, s[c]);
+          tmem_ld_wait();
+          tc_fence_before();
+          mbar_arrive(&s_free[t]);
+          if (drafts) {
+#pragma unroll
+            for (int c = 0; c < NR; ++c) {
+              const uint32_t bits = static_cast<uint32_t>(sees[c >> 1] >> (32 * (c & 1)));
+#pragma unroll
+              for (int i = 0; i < 32; ++i) s[c][i] = (bits >> i & 1u) ? s[c][i] : -INFINITY;
+            }
+          }
+          float mx = -INFINITY;
+          {
+            float part[2 * NR];
+#pragma unroll
+            for (int c = 0; c < 2 * NR; ++c) {
+              const float* v = &s[c >> 1][(c & 1) * 16];
+              part[c] = fmaxf(v[0], v[1]);
+#pragma unroll
+              for (int i = 2; i < 16; i += 2) part[c] = fmaxf(part[c], fmaxf(v[i], v[i + 1]));
+            }
+#pragma unroll
+            for (int c = 0; c < 2 * NR; ++c) mx = fmaxf(mx, part[c]);
+          }
+          mx = __fmul_rn(mx, p.c);
+          float alpha = 1.0f;
+          if (first) {
+            m = mx;
+            l = 0.0f;
+          } else if (mx > m + prefix::kLazy) {   // m = -inf: any finite maximum is above it
+            alpha = exp2_hw(__fsub_rn(m, mx));
+            m = mx;
+          }
+          if (!first && __any_sync(0xffffffffu, alpha != 1.0f)) {
+            // rescale the accumulator once the previous block's P.V is done
+            if (!pv_done()) break;
+#pragma unroll 1
+            for (int c = 0; c < C::DP / 16; ++c) {
+              uint32_t o[16];
+              prefix::tmem_ld_x16(o_t + c * 16, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__fmul_rn(__uint_as_float(o[i]), alpha));
+              prefix::tmem_st_x16(o_t + c * 16, o);
+            }
+            l = __fmul_rn(l, alpha);
+          }
+          // the last block's P.V has read its weights (long since)
+          if (!pv_done()) break;
+          // the two tiles' warps of a scheduler take turns on its exponential unit (see dk_prefix.cuh)
+          if (it.tiles == 2) {
+            if (!warp_wait(&turn[warp], tph, kDetTurn, abort_flag)) break;
+            tph ^= 1u;
+          }
+          const float neg = (m == -INFINITY) ? 0.0f : -m;
+          const float2 c2 = make_float2(p.c, p.c), n2 = make_float2(neg, neg);
+          float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+          for (int c = 0; c < NR; ++c) {
+            uint32_t pk[16];
+            if (c == NR / 2) prefix::arrive_if(&turn[warp ^ 4], it.tiles == 2 && lane == 0);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float2 e = fma2(make_float2(s[c][i], s[c][i + 1]), c2, n2);
+              e.x = exp2_hw(e.x);
+              e.y = exp2_hw(e.y);
+              sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
+              pk[i >> 1] = pack2<T>(e.x, e.y);
+            }
+            prefix::tmem_st_x16(p_t + c * 16, pk);
+          }
+          tmem_st_wait();
+          const float2 ps = add2(sum[0], sum[1]);
+          l = __fadd_rn(l, __fadd_rn(ps.x, ps.y));
+        } else {
+          mbar_arrive(&s_free[t]);
+          if (it.tiles == 2) {
+            if (!warp_wait(&turn[warp], tph, kDetTurn, abort_flag)) break;
+            tph ^= 1u;
+            if (lane == 0) mbar_arrive(&turn[warp ^ 4]);
+          }
+          if (!pv_done()) break;
+        }
+        if (drafts) {   // (its values stay until this tile's weights have met them)
+          const uint32_t f = fv0 + per * b;
+          if (!wait_fill<C::STAGES>(full, f, abort_flag)) break;
+          wild |= s_wild[f % C::STAGES] != 0;
+        }
+        tc_fence_before();
+        mbar_arrive(&p_ready[t]);
+        ++ocnt;
+        if (q_loaded) q_here();
+        if (last) {
+          if (!pv_done()) break;
+          if (warp_live) {
+            const int64_t n = kvh * static_cast<int64_t>(p.n_rows) * p.G + it.s.row0 * static_cast<int64_t>(p.G) + mrow;   // state row
+            const bool whole = it.s.n_chunks == 1;   // the output, at once
+            float4* dst = reinterpret_cast<float4*>(p.st_o) + static_cast<int64_t>(it.chunk) * (D / 4) * p.st_rows + n;
+            T* out = static_cast<T*>(p.out) + row * p.o_sr + (kvh * p.G + mrow - (row - it.s.row0) * p.G) * p.o_sh;
+            const bool empty = whole && valid_row && l == 0.0f && sees_nothing(p, it.s, mask);
+            if (!whole && valid_row)
+              *reinterpret_cast<float2*>(p.st_ml + 2 * (it.chunk * p.st_rows + n)) = make_float2(m, l);
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float o[32];
+              __syncwarp();   // rows part in what they store, the load is the whole warp's
+              tmem_ld_32x32b_x32(o_t + c * 32, o);
+              tmem_ld_wait();
+              if (wild && valid_row)
+                add_back<T>(p, it.s, mask, it.b, kvh, it.t_begin, it.t_begin + it.tokens, c * 32, o);
+              if (valid_row && !whole) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  dst[i * p.st_rows] = make_float4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
+                dst += 8 * p.st_rows;
+              } else if (valid_row) {
+                uint32_t u[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                  u[i] = empty ? 0u : pack2<T>(__fdiv_rn(o[2 * i], l), __fdiv_rn(o[2 * i + 1], l));
+                if (p.o_vec) {
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<uint4*>(out + c * 32 + i * 8) = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) {
+                    out[c * 32 + 2 * i] = *reinterpret_cast<const T*>(&u[i]);
+                    out[c * 32 + 2 * i + 1] = *(reinterpret_cast<const T*>(&u[i]) + 1);
+                  }
+                }
+              }
+            }
+          }
+          __syncwarp();
+          tc_fence_before();
+          mbar_arrive(&o_free[t]);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kSoftWarps + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// out = O / l of a row's chunks, joined in order.  A CTA takes 32 state rows of a (sequence, KV head), a lane each; its
+// warps take column quads (one coalesced load a state), and the outputs leave through shared memory.
+constexpr int kJoinThreads = 256;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p, int row_tiles) {
+  constexpr int WARPS = kJoinThreads / 32, Q = D / 4 / WARPS, UN = Q >= 4 ? 2 : 4;   // quads a warp; states in flight
+  __shared__ __align__(16) T s_out[32][D + 2];
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t tile = blockIdx.x % row_tiles, rest = blockIdx.x / row_tiles;
+  const int kvh = static_cast<int>(rest % p.hkv), b = static_cast<int>(rest / p.hkv);
+  const Seq s = seq_at<D, true>(p, b, false);
+  const int m0 = static_cast<int>(tile) * 32, mg = s.rows * p.G;
+  if (s.n_chunks <= 1 || m0 >= mg) return;
+  const bool live = m0 + lane < mg;
+  const int64_t n = kvh * static_cast<int64_t>(p.n_rows) * p.G + s.row0 * static_cast<int64_t>(p.G) + m0 + (live ? lane : 0);
+  const float4* src = reinterpret_cast<const float4*>(p.st_o) + static_cast<int64_t>(warp) * Q * p.st_rows + n;
+  const float2* mls = reinterpret_cast<const float2*>(p.st_ml) + n;
+  const int64_t state = p.st_rows * (D / 4);
+  float tm = -INFINITY, tl = 0.0f;
+  float4 to[Q];
+#pragma unroll
+  for (int i = 0; i < Q; ++i) to[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int c0 = 0; c0 < s.n_chunks; c0 += UN) {
+    float2 ml[UN];
+    float4 o[UN][Q];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      if (c0 + u < s.n_chunks) {
+        ml[u] = __ldcg(mls + (c0 + u) * p.st_rows);
+#pragma unroll
+        for (int i = 0; i < Q; ++i) o[u][i] = __ldcg(src + (c0 + u) * state + i * p.st_rows);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      if (c0 + u < s.n_chunks) {
+        const bool head = c0 + u == 0;
+        float a = 0.0f, w = 1.0f;
+        if (head) {
+          tm = ml[u].x;
+          tl = ml[u].y;
+        } else {
+          tm = join_weights(tm, ml[u].x, a, w);
+          tl = join(tl, a, ml[u].y, w);
+        }
+#pragma unroll
+        for (int i = 0; i < Q; ++i) to[i] = head ? o[u][i] : join4(to[i], a, o[u][i], w);
+      }
+    }
+  }
+  const int row = s.row0 + (live ? static_cast<int>(div_by(static_cast<uint32_t>(m0 + lane), p.group)) : 0);
+  const bool empty = live && tl == 0.0f && sees_nothing(p, s, p.mask + row * p.mask_stride);
+#pragma unroll
+  for (int i = 0; i < Q; ++i) {
+    T* d = &s_out[lane][(warp * Q + i) * 4];
+    *reinterpret_cast<uint32_t*>(d) = empty ? 0u : pack2<T>(__fdiv_rn(to[i].x, tl), __fdiv_rn(to[i].y, tl));
+    *reinterpret_cast<uint32_t*>(d + 2) = empty ? 0u : pack2<T>(__fdiv_rn(to[i].z, tl), __fdiv_rn(to[i].w, tl));
+  }
+  __syncthreads();
+  for (int k = warp; k < 32 && m0 + k < mg; k += WARPS) {
+    const int mk = m0 + k, rk = static_cast<int>(div_by(static_cast<uint32_t>(mk), p.group));
+    T* dst = static_cast<T*>(p.out) + (s.row0 + rk) * p.o_sr + (kvh * p.G + mk - rk * p.G) * p.o_sh;
+#pragma unroll
+    for (int d = 0; d < D; d += 32) dst[d + lane] = s_out[k][d + lane];
+  }
+}
+
+}  // namespace tree
+}  // namespace dk

@@ -16,6 +16,9 @@ Drop-in for the reference's ``kernels/attention.py``:
   attention of rows that share a prefix, whose part is computed once for the
   whole batch on the tensor cores; ``attention_shared_prefix_reference`` is its
   plain form.
+* ``attention_tree`` (no counterpart either): the rows of a sequence are drafted
+  tokens, a tree of them or any other set given by masks, behind its cached tokens;
+  ``attention_tree_reference`` is its plain form.
 
 Shapes: q [B, H, D]; k, v [B, H_kv, S, D]; out like q.
 """
@@ -363,4 +366,116 @@ def attention_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, kv_lens, *,
             _lib.dtype_code(dt), workspace.data_ptr(), workspace.numel(), _lib.stream_ptr(dev))
     _lib.check(rc, "attention_shared_prefix")
     _lib.count_launch(2)   # at least: rows split over several warps take a third
+    return out
+
+
+def attention_tree_reference(q, k, v, kv_lens, cu_rows, tree_mask, scale: float | None = None):
+    """Plain PyTorch attention of drafted tokens, f32.
+
+    q: (R, H, D); k, v: (B, H_kv, S, D); rows cu_rows[b] to cu_rows[b + 1] are sequence b's drafts, whose keys and values
+    lie behind its first kv_lens[b] tokens; tree_mask: int64 (R, W), bit j of a row's words: it sees draft j.  A row that
+    sees nothing is zero, and so are rows behind the last sequence."""
+    import torch
+
+    out = torch.zeros_like(q)
+    scale = 1.0 / (q.shape[-1] ** 0.5) if scale is None else scale
+    G = q.shape[1] // k.shape[1]
+    for b in range(len(cu_rows) - 1):
+        r0, n, t = int(cu_rows[b]), int(kv_lens[b]), int(cu_rows[b + 1]) - int(cu_rows[b])
+        for i in range(t):
+            sees = list(range(n)) + [n + j for j in range(min(t, 64 * tree_mask.shape[1]))
+                                     if int(tree_mask[r0 + i, j // 64]) >> (j % 64) & 1]
+            if sees:
+                ks, vs = (x[b][:, sees].float().repeat_interleave(G, 0) for x in (k, v))
+                p = torch.softmax((ks * q[r0 + i].float()[:, None]).sum(-1) * scale, -1)
+                out[r0 + i] = (p[..., None] * vs).sum(1).to(q.dtype)
+    return out
+
+
+def attention_tree(q, k_cache, v_cache, kv_lens, cu_rows, tree_mask, *, block_table=None, max_kv_len=None, max_rows=None,
+                   scale=None, out=None, workspace=None):
+    """Batch-invariant attention of drafted tokens over a cache that holds them.
+
+    q [R, H, D]; rows cu_rows[b] to cu_rows[b + 1] (int32 CUDA [B + 1]) are the drafts of sequence b, which holds kv_lens[b]
+    tokens (int32 CUDA [B]) and the drafts' keys and values behind them (``paged_plan`` gives their slots, and cu_rows).
+    A row attends to all of the kv_lens[b] tokens and to the drafts that its mask names: bit j of tree_mask[row]
+    (int64 CUDA [R, W], 64 drafts a word) stands for draft j of its sequence; ``drafts.tree_mask`` makes it from a tree.
+    Bits from the sequence's row count on are ignored, drafts past the words are not seen, and a row that sees nothing is 0.
+
+    k_cache, v_cache: [>= B, H_kv, S, D], or with ``block_table`` (int32 CUDA [>= B, blocks]) block pools [n_blocks, H_kv,
+    page, D], page a multiple of 64.  bf16 or f16; head_dim 32, 64 or 128; at most 128 query heads per KV head.
+    max_rows: a bound on a sequence's rows (64 W if not given); max_kv_len: one on its tokens, drafts included (the cache's
+    capacity if not given).  They size the work and the workspace: uint8 CUDA of at least
+    ``dk_attention_tree_workspace_size`` bytes (a new one if not given; its contents do not matter, and calls that may
+    overlap need separate ones).
+
+    Rows behind the last sequence keep what ``out`` holds.  Offsets that do not ascend inside the rows, more than max_rows
+    rows a sequence, a negative length or more than max_kv_len tokens set the device status; that sequence's rows keep what
+    ``out`` holds too.  A row's bits depend on its q and the tokens that it sees, and nothing else of the batch."""
+    import torch
+
+    dev, dt = q.device, q.dtype
+    index = dev.index
+    for t in (q, k_cache, v_cache):
+        assert t.is_cuda and t.get_device() == index, "attention_tree requires CUDA tensors on one device"
+        if t.dtype != dt:
+            raise TypeError("attention_tree: q and the caches must share a dtype")
+    R, H, D = q_shape = q.shape
+    c_shape = k_cache.shape
+    assert v_cache.shape == c_shape, "q/k/v shape mismatch"
+    n_seq, Hkv, cap, Dk = c_shape
+    assert Dk == D and H % Hkv == 0, "q/k/v shape mismatch"
+    assert kv_lens.dtype == torch.int32 and kv_lens.get_device() == index and kv_lens.dim() == 1
+    B = kv_lens.numel()
+    assert cu_rows.dtype == torch.int32 and cu_rows.get_device() == index and cu_rows.shape == (B + 1,)
+    assert tree_mask.dtype == torch.int64 and tree_mask.get_device() == index and tree_mask.dim() == 2
+    W = tree_mask.shape[1]
+    assert tree_mask.shape[0] == R and W >= 1, "attention_tree: one mask a row"
+    n_blocks = page = width = bt_stride = 0
+    if block_table is not None:
+        assert block_table.dtype == torch.int32 and block_table.get_device() == index and block_table.dim() == 2
+        assert block_table.shape[1] <= 1 or block_table.stride(1) == 1
+        n_blocks, page = n_seq, cap
+        n_seq, width = block_table.shape
+        cap, bt_stride = width * page, block_table.stride(0) if n_seq > 1 else width
+    assert n_seq >= B, "attention_tree: fewer KV sequences than lengths"
+    max_kv_len = min(cap, _I32_MAX) if max_kv_len is None else int(max_kv_len)
+    max_rows = 64 * W if max_rows is None else int(max_rows)
+    if max_rows < 0 or max_kv_len < 0:
+        raise ValueError("attention_tree: max_rows and max_kv_len must not be negative")
+    max_kv_len = min(max_kv_len, cap, _I32_MAX)   # bounds beyond the cache or the batch bound nothing, but size the work
+    max_rows = min(max_rows, R, max_kv_len)
+    if scale is None:
+        scale = 1.0 / (D ** 0.5)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    o_st = out.stride()
+    assert out.shape == q_shape and out.dtype == dt and out.get_device() == index and o_st[2] == 1
+    if workspace is not None:
+        assert workspace.dtype == torch.uint8 and workspace.get_device() == index and workspace.is_contiguous(), \
+            "workspace must be a contiguous uint8 CUDA tensor on q's device"
+    if R == 0 or B == 0:
+        return out
+    with _lib.on_device(dev):
+        kv_lens, cu_rows = kv_lens.contiguous(), cu_rows.contiguous()
+        if W > 1 and tree_mask.stride(1) != 1:
+            tree_mask = tree_mask.contiguous()
+        q_st = q.stride()
+        if q.data_ptr() % 16 or q_st[2] != 1 or q_st[0] % 8 or q_st[1] % 8:
+            q = q.clone(memory_format=torch.contiguous_format)
+            q_st = q.stride()
+        cs = _shared_strides(k_cache, v_cache, "cache")
+        lib = _lib.load()
+        nbytes = lib.dk_attention_tree_workspace_size(R, max_rows, H, D, max_kv_len)
+        if workspace is None and nbytes:
+            workspace = q.new_empty(nbytes, dtype=torch.uint8)
+        rc = lib.dk_attention_tree(
+            q.data_ptr(), q_st[0], q_st[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], n_seq, cap,
+            block_table.data_ptr() if block_table is not None else None, bt_stride, width, n_blocks, page, out.data_ptr(),
+            o_st[0], o_st[1], kv_lens.data_ptr(), cu_rows.data_ptr(), tree_mask.data_ptr(), tree_mask.stride(0), W, B, R,
+            max_rows, H, Hkv, D, max_kv_len, float(scale), _lib.dtype_code(dt),
+            workspace.data_ptr() if workspace is not None else None, workspace.numel() if workspace is not None else 0,
+            _lib.stream_ptr(dev))
+    _lib.check(rc, "attention_tree")
+    _lib.count_launch(2 if nbytes else 1)
     return out

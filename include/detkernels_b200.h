@@ -426,9 +426,34 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
                                int32_t n_kv_heads, int32_t head_dim, int32_t max_kv_len, float scale, int dtype,
                                void* workspace, size_t workspace_bytes, void* stream);
 
-/* ---- Drafted tokens: log probabilities, the accepted path of a tree, pages forked, compacted and freed ----
+/* ---- Drafted tokens: their attention, log probabilities, the accepted path of a tree, pages forked, compacted and freed ----
  * No counterparts in the reference (its decoder takes one token a step, greedily, into a cache that only grows:
  * kernels/tiny_model.py:119-157). */
+
+/* Workspace bytes of dk_attention_tree (uninitialised memory will do; 0: none is needed).  max_rows and max_kv_len bound
+ * the rows and the tokens (drafts included) of a sequence. */
+size_t dk_attention_tree_workspace_size(int32_t n_rows, int32_t max_rows, int32_t n_q_heads, int32_t head_dim,
+                                        int32_t max_kv_len);
+/* Attention of drafted tokens over a cache that holds them: sequence b has kv_lens[b] tokens and, behind them, its
+ * drafts, whose queries are the rows [cu_rows[b], cu_rows[b + 1]) of q [n_rows, n_q_heads, head_dim] (cu_rows: device
+ * int32[n_seqs + 1]).  Row cu_rows[b] + i attends to tokens [0, kv_lens[b]) and to token kv_lens[b] + j where bit j of its
+ * mask is set (mask: device int64[n_rows][mask_words], 64 drafts a word from the lowest bit, row stride mask_stride;
+ * bits from the sequence's row count on are ignored, drafts past the words are not seen).  A row that sees nothing is 0.
+ * The caches k, v are [kv_n_seq, n_kv_heads, kv_capacity, head_dim], or with block_table block pools as in
+ * dk_attention_paged_batch_invariant; strides, scale, head_dim and dtypes as there, at most 128 query heads a KV head.
+ * Rows behind cu_rows[n_seqs] are left as they were in out.  Offsets that do not ascend inside the rows, more than
+ * max_rows rows a sequence, a negative length or more than max_kv_len tokens (detail 0x67d: the sequence's rows are left
+ * as they were) and a block id outside the pool (0x67a: read as block 0) are recorded as DK_ERR_DEVICE_CHECK.  Nothing
+ * that a row does not see reaches it, whatever the cache holds there.
+ * Batch invariant: a row's bits follow from its q and the tokens that it sees at their positions. */
+int dk_attention_tree(const void* q, int64_t q_stride_row, int64_t q_stride_head, const void* k, const void* v,
+                      int64_t kv_stride_seq, int64_t kv_stride_head, int64_t kv_stride_tok, int64_t kv_n_seq,
+                      int64_t kv_capacity, const int32_t* block_table, int64_t block_table_stride,
+                      int32_t blocks_per_seq, int64_t n_blocks, int32_t page_size, void* out, int64_t out_stride_row,
+                      int64_t out_stride_head, const int32_t* kv_lens, const int32_t* cu_rows, const int64_t* mask,
+                      int64_t mask_stride, int32_t mask_words, int32_t n_seqs, int32_t n_rows, int32_t max_rows,
+                      int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_kv_len, float scale,
+                      int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Log probabilities of rows of logits [n_rows, n_vocab] (any of the three dtypes, element stride stride_row, unit
  * stride along the vocabulary; rows need no alignment but their elements').
