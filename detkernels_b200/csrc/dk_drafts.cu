@@ -21,11 +21,26 @@ namespace {
 constexpr int64_t kI32Max = 0x7fffffffLL;
 
 // ============================ log probabilities ============================
-template <typename T, bool TOPK>
-int logprobs_launch(const dk::logprobs::Params& p, int64_t n_rows, cudaStream_t st) {
+template <typename T, bool TOPK, bool ALIGNED>
+int logprobs_launch(dk::logprobs::Params p, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(n_rows * p.parts));
+  auto fn = dk::logprobs::logprobs_kernel<T, TOPK, ALIGNED>;
+  // the CTAs that fit at once, each walking rows
+  using C = dk::logprobs::Cfg<T, TOPK>;
+  static bool done[kMaxDevices] = {false};
+  constexpr int kShared = 226 * 1024;   // an SM's, without what the system takes of it for a few CTAs
+  int rc = ensure_smem(fn, C::STAGES * C::STAGE + C::STATES, done);
+  if (rc) return rc;
+  const int sms = sm_count(current_device());
+  const int64_t ctas = std::min<int64_t>(p.split ? p.n_rows * p.parts : p.n_rows, static_cast<int64_t>(C::CTAS) * sms);
+  // A ring as deep as the CTAs of an SM leave room for: at four, two stages (of 2 and 3 no difference: 99 and 100 us for 4096
+  // rows of 50,001 bf16 logits; the other CTAs' passes are in flight too); one alone needs more to cover a copy's latency.
+  const int share = kShared / static_cast<int>(ceil_div(ctas, sms)) - C::STATIC - 1024 - (p.split ? C::STATES : 0);
+  p.stages = std::max(2, std::min<int>(C::STAGES, share / C::STAGE));
+  const int64_t resident = static_cast<int64_t>(C::CTAS) * sms;
+  cfg.gridDim = dim3(static_cast<unsigned>(p.split ? p.n_rows * p.parts : std::min(p.n_rows, resident)));
   cfg.blockDim = dim3(dk::logprobs::kThreads);
+  cfg.dynamicSmemBytes = p.stages * C::STAGE + (p.split ? C::STATES : 0);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -35,15 +50,17 @@ int logprobs_launch(const dk::logprobs::Params& p, int64_t n_rows, cudaStream_t 
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = p.parts > 1 ? 2 : 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, dk::logprobs::logprobs_kernel<T, TOPK>, p);
+  cfg.numAttrs = p.split ? 2 : 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, fn, p);
   if (e != cudaSuccess) return fail(DK_ERR_CUDA, "token_logprobs: launch failed: %s", cudaGetErrorString(e));
   return DK_OK;
 }
 
 template <typename T>
-int logprobs_for(const dk::logprobs::Params& p, int64_t n_rows, cudaStream_t st) {
-  return p.k > 0 ? logprobs_launch<T, true>(p, n_rows, st) : logprobs_launch<T, false>(p, n_rows, st);
+int logprobs_for(const dk::logprobs::Params& p, cudaStream_t st) {
+  const bool aligned = aligned16(p.x) && (p.n_rows == 1 || p.stride * sizeof(T) % 16 == 0);
+  if (p.k > 0) return aligned ? logprobs_launch<T, true, true>(p, st) : logprobs_launch<T, true, false>(p, st);
+  return aligned ? logprobs_launch<T, false, true>(p, st) : logprobs_launch<T, false, false>(p, st);
 }
 
 // ============================ pages ============================
@@ -157,23 +174,27 @@ int dk_token_logprobs(const void* logits, int64_t stride_row, int64_t n_rows, in
   p.x = logits;
   p.stride = stride_row;
   p.n_vocab = n_vocab;
-  p.parts = static_cast<int32_t>(std::min<int64_t>(dk::logprobs::kMaxParts, ceil_div(n_vocab, dk::logprobs::kPart)));
-  // parts of equal size in whole vectors; beyond kMaxParts full ones each CTA takes several
-  p.part = n_vocab > dk::logprobs::kMaxParts * dk::logprobs::kPart
-               ? dk::logprobs::kPart
-               : static_cast<int32_t>(ceil_div(ceil_div(n_vocab, p.parts), dk::logprobs::kVec) * dk::logprobs::kVec);
+  p.n_rows = n_rows;
+  // parts of whole passes, of one while a cluster holds the row
+  const int64_t pass = dtype == DK_F32 ? dk::logprobs::Cfg<float, false>::PASS : dk::logprobs::Cfg<__half, false>::PASS;
+  p.part = static_cast<int32_t>(ceil_div(ceil_div(n_vocab, pass), dk::logprobs::kMaxParts) * pass);
+  p.parts = static_cast<int32_t>(ceil_div(n_vocab, p.part));
+  // Rows that leave half of the SMs idle are split over the CTAs of a cluster (with 20 alternatives: 64 rows of 32,000 bf16
+  // logits 11 us split, 17 not; 290 rows 30 and 19; 64 of 185,668 36 and 60, 290 rows 119 and 70).
+  p.split = p.parts > 1 && 2 * n_rows <= sm_count(current_device());
   p.k = top_k;
   p.tokens = tokens;
   p.lp = logprobs;
   p.entropy = entropy;
   p.top_ids = top_ids;
   p.top_lp = top_logprobs;
-  if (n_rows * p.parts > kI32Max || n_vocab > kI32Max - dk::logprobs::kMaxParts * dk::logprobs::kPart)
+  // parts that start inside the row end inside 32 bits
+  if (n_rows > kI32Max || n_vocab > kI32Max / 2)
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: too many rows or logits", what);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == DK_F32) return logprobs_for<float>(p, n_rows, st);
-  if (dtype == DK_F16) return logprobs_for<__half>(p, n_rows, st);
-  return logprobs_for<__nv_bfloat16>(p, n_rows, st);
+  if (dtype == DK_F32) return logprobs_for<float>(p, st);
+  if (dtype == DK_F16) return logprobs_for<__half>(p, st);
+  return logprobs_for<__nv_bfloat16>(p, st);
 }
 
 int dk_tree_accept(const int32_t* parents, const int64_t* tokens, const int64_t* picked, const int32_t* cu_rows,

@@ -5,13 +5,18 @@
 // f = 2^g.  The difference is taken before the product, so that logits of any size (a type's lowest value among
 // them) keep their distances.  One pass over the row, bound by its bytes.
 //
-// A row is cut into parts by the vocabulary's size alone, one CTA a part and the CTAs of a row a cluster: they join
-// in the first one's shared memory, in order, so that there is neither scratch nor a second launch, and a row's bits
-// follow from the row.  A thread holds up to 64 logits in registers (eights, 256 threads apart) against its own maximum.
-// The alternatives are chosen from the same registers.  A bound below the k-th largest logit is had from the
-// threads' maxima: in each of w warps the ceil(k / w)-th largest is at most it, and so is the least of these.  What
-// lies above the bound (about twice k of 16384) is collected and ranked by counting; ties at the bound are taken in
-// the order of their indices.  Where the bound is poor (logits in order), the k-th largest maximum itself is sought.
+// A row is cut into passes of 16 KB, and the passes of long rows into eight parts, by the vocabulary's size alone.  In a
+// pass a thread takes four 16-byte vectors, 256 threads apart, against its own maximum; it joins its passes, then
+// its parts, in order, and the threads are joined last.  So few rows may give each part a CTA of its own (a cluster,
+// whose first CTA gathers the threads' states in its shared memory), and many rows a CTA each, which goes through all parts:
+// the same bits, with neither scratch nor a second launch.  Passes come into a ring in shared memory by bulk copies, which
+// keep more of them in flight than registers would, and at any alignment of a row: the copy takes the whole 16-byte words around
+// it, and a thread shifts its vectors into place.
+// The alternatives are chosen from the same stage.  A bound below the k-th largest logit of the first pass is had
+// from the threads' maxima: in each of w warps the ceil(k / w)-th largest is at most it, and so is the least of
+// these.  What lies above the bound (about twice k) is collected and ranked by counting; ties at the bound are taken
+// in the order of their indices.  From then on the k-th largest so far is the bound.  Where a bound is poor (logits
+// in order), the k-th largest of the pass's maxima is sought.
 #pragma once
 
 #include "dk_common.cuh"
@@ -21,22 +26,26 @@ namespace logprobs {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kVec = 8;                         // consecutive logits of a thread
-constexpr int kIters = 8;                       // such vectors a thread holds
-constexpr int kPart = kThreads * kVec * kIters; // logits a CTA holds
-constexpr int kMaxParts = 8;                    // CTAs a row: a portable cluster
+constexpr int kIters = 4;                       // 16-byte vectors of a pass that a thread takes
+constexpr int kMaxParts = 8;                    // a portable cluster
 constexpr int kMaxK = 32;
-constexpr int kCandidates = 2048;               // above the k-th largest maximum lie at most (k - 1) * 64 logits
+constexpr int kCandidates = 1160;               // above the k-th largest maximum lie at most (k - 1) * 32 logits
 constexpr int kPoor = 256;                      // a bound with more above it is worth improving
+constexpr int kMany = 128;                      // candidates worth ranking before the row's end
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-static_assert((kMaxK - 1) * kVec * kIters + kMaxK <= kCandidates, "candidates");
+static_assert((kMaxK - 1) * 32 + kMany + kMaxK < kCandidates, "candidates");
 
-enum : int { kDetToken = 0x650 };               // a token outside the vocabulary (and not -1)
+enum : int {
+  kDetToken = 0x650,   // a token outside the vocabulary (and not -1)
+  kDetFull = 0x651,
+};
 
 struct Params {
   const void* x;
-  int64_t stride;
-  int32_t n_vocab, parts, part;     // CTAs a row, logits a part (whole vectors)
+  int64_t stride, n_rows;
+  int32_t n_vocab, parts, part;     // parts a row, logits a part (whole passes)
+  int32_t split;                    // a CTA a part, else a row
+  int32_t stages;                   // of the ring
   int32_t k;
   const int64_t* tokens;            // null: none asked for
   float* lp;
@@ -66,17 +75,16 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// Eight logits as they lie in memory.
+// A vector of logits as it lies in memory.
 template <typename T>
 struct Raw {
-  static constexpr int W = kVec * sizeof(T) / 4;
-  uint32_t w[W];
+  static constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  uint32_t w[4];   // kNone: nothing but -infinity
   __device__ __forceinline__ float2 pair(int i) const;   // logits 2 i and 2 i + 1
   __device__ __forceinline__ float at(int i) const {
     const float2 p = pair(i >> 1);
     return i & 1 ? p.y : p.x;
   }
-  __device__ __forceinline__ float max() const;
 };
 template <>
 __device__ __forceinline__ float2 Raw<float>::pair(int i) const {
@@ -90,92 +98,80 @@ template <>
 __device__ __forceinline__ float2 Raw<__half>::pair(int i) const {
   return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
 }
+// The larger ones of two words' logits, and the largest of a word's.
+template <typename T>
+__device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b);
 template <>
-__device__ __forceinline__ float Raw<float>::max() const {
-  float m = max_nan(__uint_as_float(w[0]), __uint_as_float(w[1]));
-#pragma unroll
-  for (int i = 2; i < 8; ++i) m = max_nan(m, __uint_as_float(w[i]));
-  return m;
+__device__ __forceinline__ uint32_t max_word<float>(uint32_t a, uint32_t b) {
+  return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
 }
 template <>
-__device__ __forceinline__ float Raw<__nv_bfloat16>::max() const {
-  uint32_t m = w[0];
-#pragma unroll
-  for (int i = 1; i < 4; ++i) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i]));
-  return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+__device__ __forceinline__ uint32_t max_word<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+  return a;
 }
 template <>
-__device__ __forceinline__ float Raw<__half>::max() const {
-  uint32_t m = w[0];
-#pragma unroll
-  for (int i = 1; i < 4; ++i) asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i]));
-  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&m));
+__device__ __forceinline__ uint32_t max_word<__half>(uint32_t a, uint32_t b) {
+  asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+  return a;
+}
+template <typename T>
+__device__ __forceinline__ float max_of(uint32_t a);
+template <>
+__device__ __forceinline__ float max_of<float>(uint32_t a) { return __uint_as_float(a); }
+template <>
+__device__ __forceinline__ float max_of<__nv_bfloat16>(uint32_t a) {
+  return max_nan(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float max_of<__half>(uint32_t a) {
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&a));
   return max_nan(v.x, v.y);
 }
-template <typename T>
-__device__ __forceinline__ uint32_t nothing();   // a word of logits that are -infinity
-template <>
-__device__ __forceinline__ uint32_t nothing<float>() { return 0xff800000u; }
-template <>
-__device__ __forceinline__ uint32_t nothing<__nv_bfloat16>() { return 0xff80ff80u; }
-template <>
-__device__ __forceinline__ uint32_t nothing<__half>() { return 0xfc00fc00u; }
 
-// The vector of logits [i, i + 8) of a row of n; what lies past n is -infinity.  A row that does not start on 16
-// bytes is read in whole 16-byte words around the vector (each holds some of its logits), shifted into place.
-template <typename T>
-__device__ __forceinline__ void load(Raw<T>& r, const T* row, int i, int n, uint32_t shift) {
-  constexpr int W = Raw<T>::W;
-  if (i + kVec <= n) {
-    const uint8_t* a = reinterpret_cast<const uint8_t*>(row + i) - shift;
-    if (shift == 0) {
+// A vector from the 16-byte word in which it starts and the next one; Q: whole 32-bit words, bits: and bits behind its start.
+template <typename T, int Q>
+__device__ __forceinline__ Raw<T> shifted(const uint4& a, const uint4& b, uint32_t bits) {
+  const uint32_t t[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  Raw<T> r;
 #pragma unroll
-      for (int h = 0; h < W / 4; ++h) {
-        const uint4 v = __ldcs(reinterpret_cast<const uint4*>(a) + h);
-        r.w[4 * h] = v.x;
-        r.w[4 * h + 1] = v.y;
-        r.w[4 * h + 2] = v.z;
-        r.w[4 * h + 3] = v.w;
-      }
-      return;
+  for (int j = 0; j < 4; ++j) r.w[j] = __funnelshift_r(t[Q + j], t[(Q + j + 1) & 7], bits);
+  return r;
+}
+// Vectors v, v + kThreads, ... of a stage whose row starts `shift` bytes behind a 16-byte word (the same for the whole row).
+template <typename T, bool ALIGNED, int N>
+__device__ __forceinline__ void vectors_at(Raw<T> (&r)[N], const uint8_t* stage, int v, uint32_t shift) {
+  const uint4* at = reinterpret_cast<const uint4*>(stage) + v;
+  auto all = [&](auto q) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = shifted<T, q>(at[i * kThreads], at[i * kThreads + 1], (shift & 3) * 8);
+  };
+  if (ALIGNED || shift == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint4 a = at[i * kThreads];
+      r[i] = Raw<T>{{a.x, a.y, a.z, a.w}};
     }
-    uint32_t t[W + 4];
-#pragma unroll
-    for (int h = 0; h <= W / 4; ++h) {
-      const uint4 v = *(reinterpret_cast<const uint4*>(a) + h);
-      t[4 * h] = v.x;
-      t[4 * h + 1] = v.y;
-      t[4 * h + 2] = v.z;
-      t[4 * h + 3] = v.w;
+  } else {
+    switch (shift >> 2) {
+      case 0: all(std::integral_constant<int, 0>()); break;
+      case 1: all(std::integral_constant<int, 1>()); break;
+      case 2: all(std::integral_constant<int, 2>()); break;
+      default: all(std::integral_constant<int, 3>()); break;
     }
-    if (shift & 8) {
-#pragma unroll
-      for (int j = 0; j < W + 2; ++j) t[j] = t[j + 2];
-    }
-    if (shift & 4) {
-#pragma unroll
-      for (int j = 0; j < W + 1; ++j) t[j] = t[j + 1];
-    }
-#pragma unroll
-    for (int j = 0; j < W; ++j) r.w[j] = __funnelshift_r(t[j], t[j + 1], (shift & 3) * 8);
-    return;
   }
+}
+// Of the vector's logits only the first n are the row's, the others become -infinity.
+template <typename T>
+__device__ __forceinline__ void cut(Raw<T>& r, int n) {
+  constexpr uint32_t none = Raw<T>::kNone;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int j = 0; j < W; ++j) r.w[j] = nothing<T>();
-  if (i < n) {
-    constexpr int PER = 4 / sizeof(T);
+    for (int e = 0; e < 4; ++e) r.w[e] = e < n ? r.w[e] : none;
+  } else {
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      if (i + e < n) {
-        uint32_t u;
-        if constexpr (sizeof(T) == 4) {
-          r.w[e] = *reinterpret_cast<const uint32_t*>(row + i + e);
-        } else {
-          u = *reinterpret_cast<const uint16_t*>(row + i + e);
-          r.w[e / PER] = e & 1 ? (r.w[e / PER] & 0xffffu) | u << 16 : (r.w[e / PER] & 0xffff0000u) | u;
-        }
-      }
-    }
+    for (int e = 0; e < 4; ++e)
+      r.w[e] = 2 * e + 1 < n ? r.w[e] : 2 * e < n ? (r.w[e] & 0xffffu) | (none & 0xffff0000u) : none;
   }
 }
 
@@ -234,13 +230,24 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, unsigned long long v) 
 }
 
 struct Shared {
-  float red[3 * kWarps];
+  float top[2][kWarps], sum[2][2 * kWarps];   // by row parity: the threads' maxima and sums, by warp
   uint32_t bound[kWarps];
   int scan[kWarps];
   int n_found;
-  State state[kMaxParts];
-  unsigned long long best[kMaxParts][kMaxK];   // the parts' alternatives, in the first CTA
+  __align__(16) unsigned long long best[kMaxParts * kMaxK + 1];   // the parts' alternatives (k of each), in the first CTA of a split row
   unsigned long long sorted[kMaxK];
+};
+
+// A pass, its stage of the ring, and CTAs an SM.
+template <typename T, bool TOPK>
+struct Cfg {
+  static constexpr int VEC = 16 / sizeof(T), ITERS = kIters;   // logits a vector, vectors a thread
+  static constexpr int PASS = kThreads * ITERS * VEC;          // logits a CTA holds
+  static constexpr int STAGE = PASS * sizeof(T) + 128;         // the words around a pass
+  static constexpr int STAGES = 8;                             // at most
+  static constexpr int CTAS = 4;
+  static constexpr int STATES = 3 * kMaxParts * kThreads * 4;  // behind the ring of a split row: its parts' threads' states
+  static constexpr int STATIC = sizeof(Shared) + (TOPK ? kCandidates * 8 : 8) + STAGES * 8 + 128;
 };
 
 // The places of `mine` ties in the order of the threads, and their total.
@@ -265,213 +272,364 @@ __device__ __forceinline__ int block_scan(int mine, int* warps, int& total) {
   return before + v - mine;
 }
 
-template <typename T, bool TOPK>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? (TOPK ? 3 : 4) : 2) logprobs_kernel(const Params p) {
+// How many of n keys (and what makes their number even, which is 0) are larger.
+__device__ __forceinline__ int count_above(const unsigned long long* keys, int n, unsigned long long key) {
+  int above = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; j += 2) {
+    const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(keys + j);
+    above += (two.x > key) + (two.y > key);
+  }
+  return above;
+}
+
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float r;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+template <typename T, bool TOPK, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(const Params p) {
+  using C = Cfg<T, TOPK>;
+  constexpr int VEC = C::VEC, ITERS = C::ITERS, kPass = C::PASS;
+  extern __shared__ __align__(128) uint8_t ring[];
   __shared__ Shared sh;
-  __shared__ unsigned long long found[TOPK ? kCandidates : 1];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = blockIdx.x / p.parts;
-  const int part = blockIdx.x - static_cast<int>(row) * p.parts;
-  if (p.parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA has begun
+  __shared__ __align__(16) unsigned long long found[TOPK ? kCandidates : 1];
+  __shared__ __align__(8) uint64_t full[C::STAGES];
+  float(*threads)[kMaxParts][kThreads] = reinterpret_cast<float(*)[kMaxParts][kThreads]>(ring + p.stages * C::STAGE);
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
+  if (p.split) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA has begun
+  if (tid == 0) {
+    for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
   pdl_wait();
-  if (threadIdx.x == 0) pdl_launch_dependents();
-  const T* x = static_cast<const T*>(p.x) + row * p.stride;
-  const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x) & 15u);
-  State st{-INFINITY, 0.0f, 0.0f};
-  int held = 0;   // alternatives of earlier slabs, at the front of `found`
-  // a part is one slab, but for vocabularies beyond kMaxParts of them
-  for (int slab = part * p.part; slab < p.n_vocab; slab += p.parts * p.part) {
-    const int end = min(p.n_vocab, slab + p.part);
-    Raw<T> r[kIters];
-#pragma unroll
-    for (int i = 0; i < kIters; ++i) load<T>(r[i], x, slab + (i * kThreads + threadIdx.x) * kVec, end, shift);
-    float m = r[0].max();
-#pragma unroll
-    for (int i = 1; i < kIters; ++i) m = max_nan(m, r[i].max());
-    const float ref = m == -INFINITY ? 0.0f : m;
-    const float2 off = make_float2(-ref, -ref), unit = make_float2(kLog2e, kLog2e);
-    float2 s2 = make_float2(0.0f, 0.0f), t2 = make_float2(0.0f, 0.0f);
-#pragma unroll
-    for (int i = 0; i < kIters; ++i) {
-#pragma unroll
-      for (int e = 0; e < kVec / 2; ++e) {
-        float2 y = mul2(add2(r[i].pair(e), off), unit);
-        // an excluded logit (-infinity) has weight 0 and must not meet its infinite distance
-        y.x = max_nan(y.x, -200.0f);
-        y.y = max_nan(y.y, -200.0f);
-        const float2 w = make_float2(ex2(y.x), ex2(y.y));
-        s2 = add2(s2, w);
-        t2 = fma2(y, w, t2);
-      }
+  if (tid == 0) pdl_launch_dependents();
+  // the passes that this CTA goes through
+  const int64_t row_step = p.split ? p.n_rows : gridDim.x;
+  const int64_t row0 = p.split ? blockIdx.x / p.parts : blockIdx.x;
+  const int first_part = p.split ? static_cast<int>(blockIdx.x - row0 * p.parts) : 0;
+  const int end_part = p.split ? first_part + 1 : p.parts;
+  struct Pass {
+    int64_t row;
+    int part, begin, end;   // its first logit, and the part's end
+    bool last_of_part, last;
+  };
+  auto set = [&](Pass& a) {
+    a.end = min(p.n_vocab, (a.part + 1) * p.part);
+    a.last_of_part = a.begin + kPass >= a.end;
+    a.last = a.last_of_part && a.part + 1 == end_part;
+  };
+  auto step = [&](Pass& a) {
+    if (a.last) {
+      a.row += row_step;
+      a.part = first_part;
+      a.begin = a.part * p.part;
+    } else if (a.last_of_part) {
+      a.part += 1;
+      a.begin = a.part * p.part;
+    } else {
+      a.begin += kPass;
     }
-    st = joined(st, State{m, s2.x + s2.y, t2.x + t2.y});
-    if constexpr (TOPK) {
-      const int nvec = (end - slab + kVec - 1) / kVec;
-      const int base = slab + threadIdx.x * kVec;
-      // the bound
-      uint32_t mine = threadIdx.x < nvec ? key_of(m) : 0u;
-      const uint32_t own = mine;
-      const int full = min(kWarps, max(1, nvec / 32));   // warps with a logit in every lane
-      uint32_t low = 0;
-      for (int n = (p.k + full - 1) / full; n > 0; --n) {
-        low = __reduce_max_sync(0xffffffffu, mine);
-        const uint32_t who = __ballot_sync(0xffffffffu, mine == low);
-        if (lane == __ffs(who) - 1) mine = 0u;
+    set(a);
+  };
+  auto row_of = [&](int64_t r) { return static_cast<const T*>(p.x) + r * p.stride; };
+  auto shift_of = [&](const T* x) { return ALIGNED ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x) & 15u); };
+  Pass at{row0, first_part, first_part * p.part, 0, false, false};
+  set(at);
+  Pass ahead = at;
+  bool abort_flag = false;
+  auto issue = [&](int stage) {   // thread 0: the next pass that is not on its way, with the words around it
+    if (ahead.row < p.n_rows) {
+      const uint8_t* a = reinterpret_cast<const uint8_t*>(row_of(ahead.row) + ahead.begin);
+      const uint32_t before = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a) & 15u);
+      const uint32_t bytes = (before + min(kPass, ahead.end - ahead.begin) * static_cast<uint32_t>(sizeof(T)) + 15u) & ~15u;
+      mbar_arrive_expect_tx(&full[stage], bytes);
+      bulk_load_1d(ring + stage * C::STAGE, a - before, bytes, &full[stage]);
+      step(ahead);
+    }
+  };
+  if (tid == 0)
+    for (int s = 0; s < p.stages; ++s) issue(s);
+  State st{-INFINITY, 0.0f, 0.0f}, in_part{-INFINITY, 0.0f, 0.0f};
+  int held = 0;         // alternatives so far, at the front of `found`
+  int n = 0;            // and candidates behind them
+  uint32_t bound = 0;   // below the k-th largest logit; once there are k of them, the k-th itself
+  int flip = 0;         // row parity
+  float asked = 0.0f;   // thread 0: the logit of the row's token, fetched long before it is used
+  int stage = 0;
+  uint32_t phase = 0;
+  for (; at.row < p.n_rows; step(at)) {
+    const int64_t row = at.row;
+    const int part = at.part, begin = at.begin, end = at.end;
+    const T* x = row_of(row);
+    const uint32_t shift = shift_of(x);
+    const uint8_t* here = ring + stage * C::STAGE;
+    const bool new_part = begin == part * p.part, new_row = new_part && part == first_part;
+    if (new_row && tid == 0 && part == 0 && p.tokens) {
+      const int64_t tok = p.tokens[row];
+      if (tok >= 0 && tok < p.n_vocab) asked = to_f32<T>(x[tok]);
+    }
+    mbar_wait(&full[stage], phase, kDetFull, abort_flag);
+    // vectors of which some lane of this warp has a logit
+    const int left = end - begin, some_have = (left - warp * 32 * VEC + kThreads * VEC - 1) / (kThreads * VEC);
+    State now{-INFINITY, 0.0f, 0.0f};
+    auto sum_up = [&](auto whole) {   // a whole pass, or what there is of one
+      Raw<T> r[ITERS];
+      vectors_at<T, ALIGNED>(r, here, tid, shift);
+      uint32_t mw = Raw<T>::kNone;
+#pragma unroll
+      for (int i = 0; i < ITERS; ++i) {
+        if (!whole) {
+          if (i >= some_have) break;
+          cut(r[i], left - (i * kThreads + tid) * VEC);
+        }
+        mw = max_word<T>(mw, max_word<T>(max_word<T>(r[i].w[0], r[i].w[1]), max_word<T>(r[i].w[2], r[i].w[3])));
       }
-      if (lane == 0) sh.bound[warp] = low;
-      if (threadIdx.x == 0) sh.n_found = held;
-      __syncthreads();
-      uint32_t bound = sh.bound[0];
-      for (int w = 1; w < full; ++w) bound = min(bound, sh.bound[w]);
-      auto collect = [&]() {   // everything above the bound
-        if (own > bound) {
+      now.m = max_of<T>(mw);
+      const float ref = now.m == -INFINITY ? 0.0f : now.m;
+      const float2 off = make_float2(-ref, -ref), unit = make_float2(kLog2e, kLog2e);
+      auto sums = [&](auto far) {
+        float2 s2[2], t2[2];
+        s2[0] = s2[1] = t2[0] = t2[1] = make_float2(0.0f, 0.0f);
 #pragma unroll
-          for (int i = 0; i < kIters; ++i) {
-            if (key_of(r[i].max()) > bound) {
-              const int at = base + i * kThreads * kVec;
+        for (int i = 0; i < ITERS; ++i) {
+          if (!whole && i >= some_have) break;
 #pragma unroll
-              for (int e = 0; e < kVec; ++e) {
-                const uint32_t key = key_of(r[i].at(e));
-                if (key > bound && at + e < end) {
-                  const int f = atomicAdd(&sh.n_found, 1);
-                  if (f < kCandidates)
-                    found[f] = static_cast<unsigned long long>(key) << 32 | ~static_cast<uint32_t>(at + e);
-                }
-              }
-            }
+          for (int e = 0; e < VEC / 2; ++e) {
+            float2 y = mul2(add2(r[i].pair(e), off), unit);
+            if (far) y = make_float2(max_nan(y.x, -200.0f), max_nan(y.y, -200.0f));
+            const float2 w = make_float2(ex2(y.x), ex2(y.y));
+            s2[e & 1] = add2(s2[e & 1], w);
+            t2[e & 1] = fma2(y, w, t2[e & 1]);
           }
         }
-        __syncthreads();
+        s2[0] = add2(s2[0], s2[1]);
+        t2[0] = add2(t2[0], t2[1]);
+        now.s = s2[0].x + s2[0].y;
+        now.t = t2[0].x + t2[0].y;
       };
-      collect();
-      if (sh.n_found - held > kPoor) {
+      sums(std::false_type());
+      // An excluded logit (-infinity, or as far away) has weight 0 and must not meet its infinite distance: once more, with
+      // distances that end where weights have long been 0.
+      if (now.t != now.t) sums(std::true_type());
+    };
+    if (left >= kPass) {
+      sum_up(std::true_type());
+    } else if (some_have > 0) {
+      sum_up(std::false_type());
+    }
+    const float m = now.m;
+    in_part = new_part ? now : joined(in_part, now);
+    if (at.last_of_part) st = part == first_part ? in_part : joined(st, in_part);
+    if constexpr (TOPK) {
+      if (new_row) held = n = 0;
+      const int nvec = min(kThreads * ITERS, (end - begin + VEC - 1) / VEC);
+      const uint32_t own = tid < nvec ? key_of(m) : 0u;
+      if (held < p.k) {
+        // the bound from the threads' maxima
+        uint32_t mine = own;
+        const int warps = min(kWarps, max(1, nvec / 32));   // those with a logit in every lane
+        uint32_t low = 0;
+        for (int a = (p.k + warps - 1) / warps; a > 0; --a) {
+          low = __reduce_max_sync(0xffffffffu, mine);
+          const uint32_t who = __ballot_sync(0xffffffffu, mine == low);
+          if (lane == __ffs(who) - 1) mine = 0u;
+        }
+        if (lane == 0) sh.bound[warp] = low;
+        if (tid == 0) sh.n_found = held;
+        n = held;
+        __syncthreads();
+        bound = sh.bound[0];
+        for (int w = 1; w < warps; ++w) bound = min(bound, sh.bound[w]);
+      }
+      // everything above the bound; whether there is any.  A warp takes its threads with a larger maximum one after the
+      // other, a lane a logit.
+      auto collect = [&]() {
+        const bool mine = own > bound;
+        uint32_t who = __ballot_sync(0xffffffffu, mine);
+        const float most = value_of(bound);
+        const T* logits = reinterpret_cast<const T*>(here + shift);
+        const int off = lane < ITERS * VEC ? lane / VEC * (kThreads * VEC) + lane % VEC : left;
+        while (who) {   // four threads at a time: one place in the list is asked for all that they have
+          constexpr int Q = 4;
+          float v[Q];
+          int at[Q];
+          uint32_t hits[Q];
+#pragma unroll
+          for (int q = 0; q < Q; ++q) {
+            at[q] = who ? (warp * 32 + __ffs(who) - 1) * VEC + off : left;
+            who &= who - 1;
+            v[q] = at[q] < left ? to_f32<T>(logits[at[q]]) : -INFINITY;
+          }
+          int n_hits = 0;
+#pragma unroll
+          for (int q = 0; q < Q; ++q) {
+            // (the bound is a number where something lies above it; below it there is nothing but at first)
+            hits[q] = __ballot_sync(0xffffffffu, at[q] < left && (bound == 0 || !(v[q] <= most)));
+            n_hits += __popc(hits[q]);
+          }
+          int f = 0;
+          if (lane == 0) f = atomicAdd(&sh.n_found, n_hits);
+          f = __shfl_sync(0xffffffffu, f, 0);
+#pragma unroll
+          for (int q = 0; q < Q; ++q) {
+            const int to = f + __popc(hits[q] & ((1u << lane) - 1));
+            if ((hits[q] >> lane & 1u) && to < kCandidates)
+              found[to] = static_cast<unsigned long long>(key_of(v[q])) << 32 | ~static_cast<uint32_t>(begin + at[q]);
+            f += __popc(hits[q]);
+          }
+        }
+        return __syncthreads_or(mine);
+      };
+      const bool some = collect();
+      if (some && sh.n_found - n > kPoor) {
         // the k-th largest of the threads' maxima, bit by bit
         uint32_t best = 0;
         for (int b = 31; b >= 0; --b) {
-          const uint32_t at = best | 1u << b;
-          if (__syncthreads_count(own >= at) >= p.k) best = at;
+          const uint32_t to = best | 1u << b;
+          if (__syncthreads_count(own >= to) >= p.k) best = to;
         }
         if (best > bound) {
           bound = best;
-          if (threadIdx.x == 0) sh.n_found = held;
+          if (tid == 0) sh.n_found = n;
           __syncthreads();
           collect();
         }
       }
-      int n = sh.n_found;
-      const int want = min(p.k, end - slab);
-      if (n - held < want) {
+      if (some) n = sh.n_found;
+      if (held < p.k) {
         // ties at the bound, in the order of their indices
-        int need = want - (n - held);
-#pragma unroll
-        for (int i = 0; i < kIters; ++i) {
-          if (need > 0) {
+        int need = min(p.k - held, end - begin) - (n - held);
+        if (need > 0) {
+#pragma unroll 1
+          for (int i = 0; i < ITERS && need > 0; ++i) {
+            const int first = begin + (i * kThreads + tid) * VEC;
             int ties = 0;
-            const int at = base + i * kThreads * kVec;
+            Raw<T> vs[1];
+            vectors_at<T, ALIGNED>(vs, here, i * kThreads + tid, shift);
+            const Raw<T>& v = vs[0];
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) ties += key_of(r[i].at(e)) == bound && at + e < end;
+            for (int e = 0; e < VEC; ++e) ties += key_of(v.at(e)) == bound && first + e < end;
             int total;
             int f = block_scan(ties, sh.scan, total);
 #pragma unroll
-            for (int e = 0; e < kVec; ++e)
-              if (key_of(r[i].at(e)) == bound && at + e < end) {
-                if (f < need) found[n + f] = static_cast<unsigned long long>(bound) << 32 | ~static_cast<uint32_t>(at + e);
+            for (int e = 0; e < VEC; ++e)
+              if (key_of(v.at(e)) == bound && first + e < end) {
+                if (f < need) found[n + f] = static_cast<unsigned long long>(bound) << 32 | ~static_cast<uint32_t>(first + e);
                 ++f;
               }
             n += min(total, need);
             need -= total;
           }
+          __syncthreads();
+        }
+      }
+      if (held < p.k || n > min(kMany, 2 * p.k + 16) || at.last) {
+        // the k largest so far, by counting (keys are distinct)
+        if (tid == 0 && (n & 1)) found[n] = 0ull;   // below all keys
+        __syncthreads();
+        for (int i = tid; i < n; i += kThreads) {
+          const unsigned long long key = found[i];
+          const int above = count_above(found, n, key);
+          if (above < p.k) sh.sorted[above] = key;
         }
         __syncthreads();
+        held = min(p.k, n);
+        if (tid < held) found[tid] = sh.sorted[tid];
+        if (held == p.k) bound = static_cast<uint32_t>(sh.sorted[p.k - 1] >> 32);   // an equal logit behind it comes later
+        if (tid == 0) sh.n_found = held;
+        n = held;
+        __syncthreads();
+      } else if (some) {
+        __syncthreads();   // everyone knows the count, the next pass may add to it
       }
-      // the k largest of all, by counting (keys are distinct)
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const unsigned long long key = found[i];
-        int above = 0;
-        for (int j = 0; j < n; ++j) above += found[j] > key;
-        if (above < p.k) sh.sorted[above] = key;
-      }
-      __syncthreads();
-      held = min(p.k, n);
-      if (threadIdx.x < held) found[threadIdx.x] = sh.sorted[threadIdx.x];
-      __syncthreads();
-    }
-  }
-  // threads, then parts
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    State o;
-    o.m = __shfl_xor_sync(0xffffffffu, st.m, d);
-    o.s = __shfl_xor_sync(0xffffffffu, st.s, d);
-    o.t = __shfl_xor_sync(0xffffffffu, st.t, d);
-    st = lane & d ? joined(o, st) : joined(st, o);
-  }
-  if (lane == 0) {
-    sh.red[warp] = st.m;
-    sh.red[kWarps + warp] = st.s;
-    sh.red[2 * kWarps + warp] = st.t;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    st = State{sh.red[0], sh.red[kWarps], sh.red[2 * kWarps]};
-#pragma unroll
-    for (int i = 1; i < kWarps; ++i) st = joined(st, State{sh.red[i], sh.red[kWarps + i], sh.red[2 * kWarps + i]});
-  }
-  if (p.parts > 1) {
-    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");   // the first CTA of the row has begun
-    if (threadIdx.x == 0) {
-      const uint32_t at = map_to_first(smem_u32(&sh.state[part]));
-      st_cluster(at, st.m);
-      st_cluster(at + 4, st.s);
-      st_cluster(at + 8, st.t);
-    }
-    if (TOPK && threadIdx.x < p.k)
-      st_cluster(map_to_first(smem_u32(&sh.best[part][threadIdx.x])), threadIdx.x < held ? found[threadIdx.x] : 0ull);
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    if (part != 0) {
-      return;
-    }
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    st = sh.state[0];
-    for (int i = 1; i < p.parts; ++i) st = joined(st, sh.state[i]);
-  } else {
-    if (threadIdx.x == 0) sh.state[0] = st;
-    __syncthreads();
-    st = sh.state[0];
-  }
-  const float log_s = log2f(st.s);
-  auto log_p = [&](float v) { return fmaf(-kLn2, log_s, v - st.m); };
-  if (threadIdx.x == 0) {
-    if (p.tokens) {
-      const int64_t tok = p.tokens[row];
-      float lp = 0.0f;   // -1 asks for nothing
-      if (tok >= 0 && tok < p.n_vocab) {
-        lp = log_p(to_f32<T>(x[tok]));
-      } else if (tok != -1) {
-        report_error(DK_ERR_DEVICE_CHECK, kDetToken);
-        lp = __uint_as_float(0x7fffffffu);
-      }
-      p.lp[row] = lp;
-    }
-    if (p.entropy) p.entropy[row] = kLn2 * (log_s - st.t / st.s);
-  }
-  if constexpr (TOPK) {
-    auto give = [&](int at, unsigned long long key) {
-      p.top_ids[row * p.k + at] = static_cast<int64_t>(~static_cast<uint32_t>(key));
-      p.top_lp[row * p.k + at] = log_p(value_of(static_cast<uint32_t>(key >> 32)));
-    };
-    if (p.parts == 1) {
-      if (threadIdx.x < held) give(threadIdx.x, found[threadIdx.x]);
     } else {
-      const int n = p.parts * p.k;   // at most 256
-      if (threadIdx.x < n) {
-        const unsigned long long key = sh.best[threadIdx.x / p.k][threadIdx.x % p.k];
-        int above = 0;
-        for (int a = 0; a < p.parts; ++a)
-          for (int j = 0; j < p.k; ++j) above += sh.best[a][j] > key;
-        if (key != 0 && above < p.k) give(above, key);
+      __syncthreads();     // the stage has been read
+    }
+    if (tid == 0) issue(stage);
+    if (++stage == p.stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+    if (!at.last) continue;
+    if (p.split) {
+      asm volatile("barrier.cluster.wait.aligned;" ::: "memory");   // the first CTA of the row has begun
+      st_cluster(map_to_first(smem_u32(&threads[0][part][tid])), st.m);
+      st_cluster(map_to_first(smem_u32(&threads[1][part][tid])), st.s);
+      st_cluster(map_to_first(smem_u32(&threads[2][part][tid])), st.t);
+      if (TOPK && tid < p.k) st_cluster(map_to_first(smem_u32(&sh.best[part * p.k + tid])), tid < held ? found[tid] : 0ull);
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+      if (part != 0) return;   // a split row is all that its CTAs do
+      if (TOPK && tid == 0) sh.best[p.parts * p.k] = 0ull;   // read where the keys are odd in number
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+      for (int q = 0; q < p.parts; ++q) {
+        const State o{threads[0][q][tid], threads[1][q][tid], threads[2][q][tid]};
+        st = q == 0 ? o : joined(st, o);
       }
     }
+    // the threads against the row's maximum, then their sums: lanes, warps
+    float top = warp_max_nan(st.m);
+    if (lane == 0) sh.top[flip][warp] = top;
+    __syncthreads();
+    top = sh.top[flip][0];
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i) top = max_nan(top, sh.top[flip][i]);
+    const float g = st.m == -INFINITY ? 0.0f : (st.m - top) * kLog2e, f = ex2(g);
+    float s = f * st.s, t = f * fmaf(max_nan(g, -200.0f), st.s, st.t);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, d);
+      t += __shfl_xor_sync(0xffffffffu, t, d);
+    }
+    if (lane == 0) {
+      sh.sum[flip][warp] = s;
+      sh.sum[flip][kWarps + warp] = t;
+    }
+    __syncthreads();
+    if (warp == 0 || p.split) {
+      s = sh.sum[flip][0];
+      t = sh.sum[flip][kWarps];
+#pragma unroll
+      for (int i = 1; i < kWarps; ++i) {
+        s += sh.sum[flip][i];
+        t += sh.sum[flip][kWarps + i];
+      }
+      const float log_s = log2f(s);
+      auto log_p = [&](float v) { return fmaf(-kLn2, log_s, v - top); };
+      if (tid == 0 && p.entropy) p.entropy[row] = kLn2 * (log_s - t / s);
+      if (tid == 0 && p.tokens) {
+        const int64_t tok = p.tokens[row];
+        float lp = 0.0f;   // -1 asks for nothing
+        if (tok >= 0 && tok < p.n_vocab) {
+          lp = log_p(asked);
+        } else if (tok != -1) {
+          report_error(DK_ERR_DEVICE_CHECK, kDetToken);
+          lp = __uint_as_float(0x7fffffffu);
+        }
+        p.lp[row] = lp;
+      }
+      if constexpr (TOPK) {
+        auto give = [&](int to, unsigned long long key) {
+          p.top_ids[row * p.k + to] = static_cast<int64_t>(~static_cast<uint32_t>(key));
+          p.top_lp[row * p.k + to] = log_p(value_of(static_cast<uint32_t>(key >> 32)));
+        };
+        if (!p.split) {
+          if (lane < held) give(lane, sh.sorted[lane]);
+        } else {
+          const int all = p.parts * p.k;   // at most 256
+          if (tid < all) {
+            const unsigned long long key = sh.best[tid];
+            const int above = count_above(sh.best, all, key);
+            if (key != 0 && above < p.k) give(above, key);
+          }
+        }
+      }
+    }
+    if (TOPK) __syncthreads();   // `sorted` is free for the next row
+    flip ^= 1;
   }
 }
 
