@@ -179,9 +179,9 @@ int dk_token_logprobs(const void* logits, int64_t stride_row, int64_t n_rows, in
   const int64_t pass = dtype == DK_F32 ? dk::logprobs::Cfg<float, false>::PASS : dk::logprobs::Cfg<__half, false>::PASS;
   p.part = static_cast<int32_t>(ceil_div(ceil_div(n_vocab, pass), dk::logprobs::kMaxParts) * pass);
   p.parts = static_cast<int32_t>(ceil_div(n_vocab, p.part));
-  // Rows that leave half of the SMs idle are split over the CTAs of a cluster (with 20 alternatives: 64 rows of 32,000 bf16
-  // logits 11 us split, 17 not; 290 rows 30 and 19; 64 of 185,668 36 and 60, 290 rows 119 and 70).
-  p.split = p.parts > 1 && 2 * n_rows <= sm_count(current_device());
+  // Rows that leave SMs idle are split over the CTAs of a cluster (with 20 alternatives: 74 rows of 32,000 bf16
+  // logits 15 us either way, 290 rows 30 us split and 19 not; 74 of 185,668 38 and 52, 150 67 and 72, 290 119 and 70).
+  p.split = p.parts > 1 && n_rows <= sm_count(current_device());
   p.k = top_k;
   p.tokens = tokens;
   p.lp = logprobs;

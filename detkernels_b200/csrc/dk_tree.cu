@@ -39,7 +39,7 @@ size_t state_bytes(int64_t chunks, int64_t st_rows, int64_t D) {
 }
 
 template <typename T, int D>
-int tree_launch(const dk::prefix::Maps& maps, const dk::tree::Params& p, cudaStream_t st) {
+int tree_launch(const dk::tree::Maps& maps, dk::tree::Params p, cudaStream_t st) {
   using C = dk::tree::Cfg<D>;
   static bool done[kMaxDevices] = {false};
   auto fn = dk::tree::tree_kernel<T, D>;
@@ -56,7 +56,9 @@ int tree_launch(const dk::prefix::Maps& maps, const dk::tree::Params& p, cudaStr
                   dk::prefix::kLaunchRegs);
     if (dev >= 0 && dev < kMaxDevices) regs[dev] = a.numRegs;
   }
+  // As many CTAs as SMs share the items, or, where even their bound is not more than that, each takes one at once.
   const int64_t items = static_cast<int64_t>(p.units) * p.n_seqs * p.max_chunks;
+  p.spread = items <= sm_count(dev);
   cudaError_t e = launch_pdl(fn, dim3(static_cast<unsigned>(std::min<int64_t>(items, sm_count(dev)))),
                              dim3(dk::tree::kThreads), C::SMEM, st, maps, p);
   if (e == cudaSuccess && p.max_chunks > 1) {
@@ -69,7 +71,7 @@ int tree_launch(const dk::prefix::Maps& maps, const dk::tree::Params& p, cudaStr
 }
 
 template <typename T>
-int tree_for(int D, const dk::prefix::Maps& maps, const dk::tree::Params& p, cudaStream_t st) {
+int tree_for(int D, const dk::tree::Maps& maps, const dk::tree::Params& p, cudaStream_t st) {
   return D == 32 ? tree_launch<T, 32>(maps, p, st) : D == 64 ? tree_launch<T, 64>(maps, p, st) : tree_launch<T, 128>(maps, p, st);
 }
 
@@ -125,7 +127,8 @@ int dk_attention_tree(const void* q, int64_t q_stride_row, int64_t q_stride_head
   max_rows = std::min(std::min(max_rows, n_rows), max_kv_len);
   const int64_t chunks = max_chunks(max_kv_len, max_rows, head_dim);
   const int64_t st_rows = static_cast<int64_t>(n_rows) * n_q_heads;
-  const int64_t tiles = ceil_div(static_cast<int64_t>(max_rows) * G, dk::tree::kRows);
+  const int rpt = dk::tree::kRows / G;
+  const int64_t tiles = ceil_div(max_rows, rpt);
   // items a (sequence, chunk): pairs of tiles, or pairs of heads where the rows fit one tile
   const int64_t units = tiles > 1 ? n_kv_heads * ceil_div(tiles, 2) : ceil_div(n_kv_heads, 2);
   if (st_rows > kI32Max - 512 || static_cast<int64_t>(max_rows) * G > kI32Max - 512 ||
@@ -137,11 +140,9 @@ int dk_attention_tree(const void* q, int64_t q_stride_row, int64_t q_stride_head
     return fail(DK_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
 
   dk::tree::Params p{};
-  p.q = q;
-  p.q_sr = q_stride_row;
-  p.q_sh = q_stride_head;
   p.hkv = n_kv_heads;
   p.G = G;
+  p.rpt = rpt;
   p.group = dk::divisor31(G);
   p.n_seqs = n_seqs;
   p.n_rows = n_rows;
@@ -174,15 +175,18 @@ int dk_attention_tree(const void* q, int64_t q_stride_row, int64_t q_stride_head
   p.st_ml = need ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + state_o_bytes(chunks, st_rows, head_dim))
                  : nullptr;
 
-  // K/V maps: (d, token, kv head, sequence or block)
-  dk::prefix::Maps maps;
+  dk::tree::Maps maps;
   const uint64_t dims[4] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(block_table ? page_size : kv_capacity),
                             static_cast<uint64_t>(n_kv_heads), static_cast<uint64_t>(block_table ? n_blocks : kv_n_seq)};
   const uint64_t strides[3] = {static_cast<uint64_t>(kv_stride_tok) * 2, static_cast<uint64_t>(kv_stride_head) * 2,
                                static_cast<uint64_t>(kv_stride_seq) * 2};
   const uint32_t box[4] = {64, 64, 1, 1};
   const CUtensorMapDataType dt = (dtype == DK_BF16) ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  int rc = encode_map(&maps.k, dt, 4, k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, what);
+  const uint64_t q_dims[3] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(n_q_heads), static_cast<uint64_t>(n_rows)};
+  const uint64_t q_strides[2] = {static_cast<uint64_t>(q_stride_head) * 2, static_cast<uint64_t>(q_stride_row) * 2};
+  const uint32_t q_box[3] = {64, static_cast<uint32_t>(G), static_cast<uint32_t>(rpt)};
+  int rc = encode_map(&maps.q, dt, 3, q, q_dims, q_strides, q_box, CU_TENSOR_MAP_SWIZZLE_128B, what);
+  if (!rc) rc = encode_map(&maps.k, dt, 4, k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, what);
   if (!rc) rc = encode_map(&maps.v, dt, 4, v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, what);
   if (rc) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

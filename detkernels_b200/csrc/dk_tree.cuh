@@ -8,11 +8,13 @@
 // chunk's softmax state (m, l, O) is formed block by block as in dk_prefix.cuh, and the chunks' states are joined in
 // order.  No step looks at another row: a chunk of which a row sees nothing joins with weight 0.
 //
-// Work: an item is (sequence, chunk, up to two tiles of 128 rows): two tiles of one KV head, which then share K and V, or,
-// where the rows fit one tile, the tiles of two KV heads, each with its own K and V.  Either way both softmax
-// warpgroups have work, and take turns on the exponential unit.  One persistent CTA an SM: a TMA warp, an MMA warp a
-// tile (scores, weights and accumulator apart in TMEM), a warpgroup a tile for the softmax, a row a thread, and a
-// warp that makes the values of draft blocks safe: 0 weights must meet neither what lies behind the sequence in its last
+// Work: an item is (sequence, up to two tiles of at most 128 rows, chunk): two tiles of one KV head, which then share K
+// and V, or, where the rows fit one tile, the tiles of two KV heads, each with its own K and V.  Either way both softmax
+// warpgroups have work, and take turns on the exponential unit.  One persistent CTA an SM takes a run of items in the order
+// (sequence, tiles, chunk), so that a run's chunks share their queries; the runs are cut at equal shares of the tokens'
+// and the items' cost, which every CTA finds for itself from the lengths.  A TMA warp, an MMA warp a tile (scores,
+// weights and accumulator apart in TMEM), a warpgroup a tile for the softmax, a row a thread, and a warp that fetches the
+// queries and makes the values of draft blocks safe: 0 weights must meet neither what lies behind the sequence in its last
 // page nor a non-finite value of a draft that some rows do not see.  Those elements become 0 in shared memory, and rows
 // that do see them have them added back from the cache (which no ordinary call does).
 #pragma once
@@ -35,7 +37,7 @@ using prefix::kRows;
 using prefix::kSoftWarps;
 using prefix::warp_wait;
 
-constexpr int kThreads = prefix::kThreads;   // softmax warps, then TMA, two for MMA, and the one that cleans values
+constexpr int kThreads = prefix::kThreads;   // softmax warps, then TMA, two for MMA, and one for queries and draft values
 
 enum : int {
   kDetEmpty = 0x670,
@@ -45,6 +47,7 @@ enum : int {
   kDetOut = 0x674,
   kDetQ = 0x675,
   kDetOutFree = 0x676,
+  kDetQFree = 0x66f,
   kDetDrain = 0x677,
   kDetDone = 0x678,
   kDetScoresFree = 0x679,
@@ -54,10 +57,14 @@ enum : int {
   kDetLens = 0x67d,   // a negative length, rows that do not ascend or exceed their bound, or tokens beyond the cache
 };
 
+struct Maps {
+  CUtensorMap q;            // (d, head, row): boxes of 64 elements of a tile's heads and rows
+  CUtensorMap k, v;         // (d, token, KV head, sequence or block): boxes of 64 elements x 64 tokens
+};
+
 struct Params {
-  const void* q;
-  int64_t q_sr, q_sh;
   int32_t hkv, G;
+  int32_t rpt;              // rows a tile: its query rows are rpt G
   Divisor31 group;          // by G
   int32_t n_seqs, n_rows, max_rows;
   const int32_t* kv_lens;
@@ -68,6 +75,7 @@ struct Params {
   int32_t capacity;         // tokens a sequence may have, drafts included
   int32_t units;            // items a (sequence, chunk), at most
   int32_t max_chunks;
+  int32_t spread;           // an item a CTA: CTA c takes item c of (chunk, sequence, unit)
   const void* v;            // for what is added back
   int64_t c_sn, c_sh, c_st;
   const int32_t* table;     // null: contiguous
@@ -132,42 +140,170 @@ __device__ __forceinline__ Seq seq_at(const Params& p, int b, bool report) {
   return s;
 }
 
-struct Item {
-  Seq s;
-  int b, chunk;              // sequence; chunk of it
-  int kvh, m0;               // of tile 0
-  int tiles, streams;        // tiles with work; K/V streams (2: tile 1 is the next KV head)
-  int t_begin, tokens, n_blocks;   // n_blocks = 0: no work
+// The items of a sequence: units (pairs of tiles, or of heads) and the cost of one's chunks, in blocks.
+struct Cost {
+  int units, pairs;      // pairs of tiles a KV head; 0: pairs of heads
+  int chunk, unit;       // cost of a whole chunk, of a unit
 };
-template <int D, bool WARP>
-__device__ __forceinline__ Item item_at(const Params& p, uint32_t w, bool report) {
+// What an item costs beside its blocks (states out, the first scores), in blocks.
+template <int D>
+constexpr int kItemCost = D == 128 ? 2 : 1;
+
+template <int D>
+__device__ __forceinline__ Cost cost_of(const Params& p, const Seq& s) {
   constexpr int BLK = Cfg<D>::BLK;
-  Item it;
-  const uint32_t r = w / static_cast<uint32_t>(p.units);
-  const int u = static_cast<int>(w - r * p.units);
-  it.chunk = static_cast<int>(r / static_cast<uint32_t>(p.n_seqs));
-  it.b = static_cast<int>(r - it.chunk * static_cast<uint32_t>(p.n_seqs));
-  it.s = seq_at<D, WARP>(p, it.b, report && u == 0 && it.chunk == 0);
-  it.n_blocks = 0;
-  if (it.chunk >= it.s.n_chunks) return it;
-  const int mg = it.s.rows * p.G, nt = (mg + kRows - 1) / kRows;
-  if (nt > 1) {
-    const int pairs = (nt + 1) >> 1;
-    it.kvh = u / pairs;
-    const int pair = u - it.kvh * pairs;
-    it.m0 = pair * 2 * kRows;
-    it.tiles = it.m0 + kRows < mg ? 2 : 1;
-    it.streams = 1;
-  } else {
-    it.kvh = 2 * u;
-    it.m0 = 0;
-    it.tiles = it.streams = it.kvh + 1 < p.hkv ? 2 : 1;
+  Cost c;
+  const int nt = (s.rows + p.rpt - 1) / p.rpt;
+  c.pairs = nt > 1 ? (nt + 1) >> 1 : 0;
+  c.units = nt > 1 ? p.hkv * c.pairs : nt == 1 ? (p.hkv + 1) >> 1 : 0;
+  c.chunk = s.chunk / BLK + kItemCost<D>;
+  c.unit = (s.total + BLK - 1) / BLK + s.n_chunks * kItemCost<D>;
+  return c;
+}
+
+// A CTA's walk over its items.
+template <int D, bool WARP>
+struct Walk {
+  static constexpr int BLK = Cfg<D>::BLK;
+  Seq s;
+  Cost c;
+  int b, u, chunk;           // the item
+  int64_t left;              // cost up to the end of the run
+  // of the item
+  int kvh, tile0;            // of tile 0
+  int tiles, streams;        // tiles with work; K/V streams (2: tile 1 is the next KV head)
+  int t_begin, tokens, n_blocks;
+
+  __device__ __forceinline__ void load(const Params& p, bool report) {
+    s = seq_at<D, WARP>(p, b, report);
+    c = cost_of<D>(p, s);
   }
-  if (it.kvh >= p.hkv) return it;
-  it.t_begin = it.chunk * it.s.chunk;
-  it.tokens = min(it.s.total - it.t_begin, it.s.chunk);
-  it.n_blocks = (it.tokens + BLK - 1) / BLK;
-  return it;
+  // begin: (sequence, unit, chunk) of the first item and the run's cost
+  __device__ __forceinline__ Walk(const Params& p, const int (&begin)[3], int64_t cost, bool report) {
+    b = begin[0];
+    u = begin[1];
+    chunk = begin[2];
+    left = cost;
+    if (left > 0) {
+      load(p, report);
+      settle(p, report);
+    }
+  }
+  __device__ __forceinline__ bool more() const { return left > 0; }
+  // From a position that may lie behind its unit or sequence to the item there.
+  __device__ __forceinline__ void settle(const Params& p, bool report) {
+    if (chunk >= s.n_chunks) {
+      chunk = 0;
+      ++u;
+    }
+    while (u >= c.units) {
+      u = 0;
+      if (++b >= p.n_seqs) {
+        left = 0;
+        return;
+      }
+      load(p, report);
+    }
+    if (c.pairs) {
+      kvh = u / c.pairs;
+      tile0 = (u - kvh * c.pairs) * 2;
+      tiles = (tile0 + 1) * p.rpt < s.rows ? 2 : 1;
+      streams = 1;
+    } else {
+      kvh = 2 * u;
+      tile0 = 0;
+      tiles = streams = kvh + 1 < p.hkv ? 2 : 1;
+    }
+    t_begin = chunk * s.chunk;
+    tokens = min(s.total - t_begin, s.chunk);
+    n_blocks = (tokens + BLK - 1) / BLK;
+  }
+  // Whether the next item, if there is one, has other queries.
+  __device__ __forceinline__ bool last_of_unit() const { return chunk + 1 == s.n_chunks || left <= n_blocks + kItemCost<D>; }
+  __device__ __forceinline__ void next(const Params& p, bool report) {
+    left -= n_blocks + kItemCost<D>;
+    if (left <= 0) return;
+    ++chunk;
+    settle(p, report);
+  }
+  // a block that holds drafts
+  __device__ __forceinline__ bool drafts(int block) const { return t_begin + (block + 1) * BLK > s.kv; }
+  __device__ __forceinline__ int head(int t) const { return kvh + (streams == 2 ? t : 0); }
+  __device__ __forceinline__ int first_row(const Params& p, int t) const { return (tile0 + (streams == 1 ? t : 0)) * p.rpt; }
+};
+
+// The CTA's run: shared memory for its first item and cost, and the block's scan.
+struct Run {
+  int begin[3];
+  long long cost;
+  long long warps[kThreads / 32];
+};
+template <int D>
+__device__ __forceinline__ void find_run(const Params& p, Run& run) {
+  if (threadIdx.x == 0) run.cost = 0;
+  if (p.spread) {
+    const uint32_t w = blockIdx.x, r = w / static_cast<uint32_t>(p.units);
+    if (threadIdx.x == 0) {
+      run.begin[1] = static_cast<int>(w - r * p.units);
+      run.begin[2] = static_cast<int>(r / static_cast<uint32_t>(p.n_seqs));
+      run.begin[0] = static_cast<int>(r - run.begin[2] * static_cast<uint32_t>(p.n_seqs));
+      const Seq s = seq_at<D, false>(p, run.begin[0], run.begin[1] == 0 && run.begin[2] == 0);
+      if (run.begin[2] < s.n_chunks && run.begin[1] < cost_of<D>(p, s).units) run.cost = 1;
+    }
+    __syncthreads();
+    return;
+  }
+  // every thread the cost of some sequences, then its place among all
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = (p.n_seqs + kThreads - 1) / kThreads;
+  const int b0 = min(static_cast<int64_t>(p.n_seqs), static_cast<int64_t>(threadIdx.x) * per), b1 = min(p.n_seqs, b0 + per);
+  auto seq_cost = [&](int b, Seq& s, Cost& c) {
+    s = seq_at<D, false>(p, b, blockIdx.x == 0);
+    c = cost_of<D>(p, s);
+    return static_cast<long long>(c.units) * c.unit;
+  };
+  long long mine = 0;
+  Seq s;
+  Cost c;
+  for (int b = b0; b < b1; ++b) mine += seq_cost(b, s, c);
+  long long at = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, at, d);
+    if (lane >= d) at += o;
+  }
+  if (lane == 31) run.warps[warp] = at;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int i = 0; i < kThreads / 32; ++i) {
+    if (i < warp) at += run.warps[i];
+    total += run.warps[i];
+  }
+  at -= mine;
+  // items that begin in [lo, hi)
+  const long long lo = total * blockIdx.x / gridDim.x, hi = total * (blockIdx.x + 1) / gridDim.x;
+  if (lo < hi && lo >= at && lo < at + mine) {
+    for (int b = b0; b < b1; ++b) {
+      const long long all = seq_cost(b, s, c);
+      if (lo >= at + all) {
+        at += all;
+        continue;
+      }
+      long long r = lo - at;
+      int u = static_cast<int>(r / c.unit);
+      r -= static_cast<long long>(u) * c.unit;
+      int chunk = min(static_cast<int>((r + c.chunk - 1) / c.chunk), s.n_chunks);   // n_chunks: the next unit's first
+      const long long start = at + static_cast<long long>(u) * c.unit +
+                              (chunk < s.n_chunks ? static_cast<long long>(chunk) * c.chunk : c.unit);
+      run.begin[0] = b;
+      run.begin[1] = u;
+      run.begin[2] = chunk;
+      run.cost = hi - start;   // none where the first item at or behind lo lies behind hi
+      break;
+    }
+  }
+  __syncthreads();
 }
 
 // A whole warp's wait for fill f of a ring of N stages, whose barriers complete once a lap.  A parity tells a lap only from
@@ -180,18 +316,18 @@ __device__ __forceinline__ bool wait_fill(uint64_t* full, uint32_t f, bool& abor
   return warp_wait(&full[f % N], (f / N) & 1, kDetFull, abort_flag);
 }
 
-// Which of the 64 tokens from p0 on a row sees.
-__device__ __forceinline__ uint64_t sees64(const Params& p, const Seq& s, const uint64_t* row, int p0) {
+// Which of the 64 tokens from p0 on a row sees (word: the first of its mask).
+__device__ __forceinline__ uint64_t sees64(const Params& p, const Seq& s, const uint64_t* row, uint64_t word, int p0) {
   if (p0 >= s.total) return 0;
   const int off = p0 - s.kv;
   uint64_t bits;
   if (off <= -64) {
     bits = ~0ull;
   } else if (off < 0) {
-    bits = (row[0] << -off) | ((1ull << -off) - 1);
+    bits = (word << -off) | ((1ull << -off) - 1);
   } else {
     const int w = off >> 6, sh = off & 63;
-    bits = w < p.words ? row[w] >> sh : 0;
+    bits = w == 0 ? word >> sh : w < p.words ? row[w] >> sh : 0;
     if (sh && w + 1 < p.words) bits |= row[w + 1] << (64 - sh);
   }
   const int left = s.total - p0;
@@ -202,7 +338,7 @@ __device__ __forceinline__ bool sees_nothing(const Params& p, const Seq& s, cons
   if (s.kv > 0) return false;
 #pragma unroll 1
   for (int p0 = 0; p0 < s.total; p0 += 64)
-    if (sees64(p, s, row, p0)) return false;
+    if (sees64(p, s, row, row[0], p0)) return false;
   return true;
 }
 
@@ -227,7 +363,7 @@ __device__ __forceinline__ void add_back(const Params& p, const Seq& s, const ui
                                          int col, float (&o)[32]) {
 #pragma unroll 1
   for (int t = max(begin, s.kv); t < end; ++t) {
-    if (!(sees64(p, s, row, t) & 1)) continue;
+    if (!(sees64(p, s, row, row[0], t) & 1)) continue;
     int64_t at = b;
     int tok = t;
     if (p.table) {
@@ -245,9 +381,17 @@ __device__ __forceinline__ void add_back(const Params& p, const Seq& s, const ui
   }
 }
 
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ prefix::Maps maps,
-                                                              const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ Maps maps,
+                                                           const __grid_constant__ Params p) {
   using C = Cfg<D>;
   constexpr int BLK = C::BLK;
   constexpr uint32_t FMT = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
@@ -263,12 +407,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   uint64_t* p_ready = s_free + 2;         // [2] by tile: weights in TMEM
   uint64_t* o_full = p_ready + 2;         // [2] by tile: P.V of a block done
   uint64_t* o_free = o_full + 2;          // [2] by tile: the accumulator has been read
-  uint64_t* q_ready = o_free + 2;         // [2] by tile
-  uint64_t* turn = q_ready + 2;           // [8] by softmax warp: the exponential unit is its
+  uint64_t* q_full = o_free + 2;          // [2] by tile: queries landed
+  uint64_t* q_ready = q_full + 2;         // [2] by tile: and their sign is right
+  uint64_t* q_free = q_ready + 2;         // [2] by tile: all scores of them are formed
+  uint64_t* turn = q_free + 2;            // [8] by softmax warp: the exponential unit is its
   uint64_t* done = turn + kSoftWarps;     // [2]
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(done + 2);
   uint32_t* s_wild = s_tmem + 1;          // by stage: its values had non-finite elements
-  static_assert((3 * C::STAGES + 12 + kSoftWarps + 2) * 8 + 4 + 4 * C::STAGES <= 512, "barriers");
+  static_assert((3 * C::STAGES + 16 + kSoftWarps + 2) * 8 + 4 + 4 * C::STAGES <= 512, "barriers");
+  __shared__ Run run;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
@@ -284,7 +431,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       mbar_init(&p_ready[t], 128);
       mbar_init(&o_full[t], 1);
       mbar_init(&o_free[t], 128);
-      mbar_init(&q_ready[t], 128);
+      mbar_init(&q_full[t], 1);
+      mbar_init(&q_ready[t], 1);
+      mbar_init(&q_free[t], 1);
     }
     for (int i = 0; i < kSoftWarps; ++i) mbar_init(&turn[i], 1);
     mbar_init(&done[0], 1);
@@ -292,6 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     fence_mbar_init();
   }
   if (warp == kSoftWarps && lane == 0) {
+    tma_prefetch_desc(&maps.q);
     tma_prefetch_desc(&maps.k);
     tma_prefetch_desc(&maps.v);
   }
@@ -305,13 +455,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   const uint32_t tmem = *s_tmem;
   pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
+  find_run<D>(p, run);
 
-  const uint32_t n_items = static_cast<uint32_t>(p.units) * p.n_seqs * p.max_chunks;   // < 2^31 (the host checks)
   bool abort_flag = false;
   // Stages of an item's block b: K of stream i in fill f0 + 2 streams b + i, V behind the K's of the block.
   // A block that holds drafts has its values cleaned.
-  auto has_drafts = [](const Item& it, int b) { return it.t_begin + (b + 1) * BLK > it.s.kv; };
-
   if (warp >= kSoftWarps) {
     prefix::reg_dec<prefix::kIoRegs>();
     if (warp == kSoftWarps && lane == 0) {
@@ -319,8 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       int stage = 0;
       uint32_t phase = 0;
       uint32_t fills = 0;
-      for (uint32_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
-        const Item it = item_at<D, false>(p, w, true);
+      for (Walk<D, false> it(p, run.begin, run.cost, false); it.more() && !abort_flag; it.next(p, false)) {
         for (int b = 0; b < it.n_blocks && !abort_flag; ++b) {
           int tok[BLK / 64], slab[BLK / 64], boxes = 0;   // 64-token boxes that hold a token
 #pragma unroll
@@ -339,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
               }
             }
           }
-          const bool clean = has_drafts(it, b);
+          const bool clean = it.drafts(b);
           for (int e = 0; e < 2 * it.streams; ++e) {
             const bool val = e >= it.streams;
             const int kvh = it.kvh + (val ? e - it.streams : e);
@@ -376,16 +523,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       const uint32_t s_col = tmem + C::S_COL + t * BLK, p_col = tmem + C::P_COL + t * (BLK / 2);
       const uint32_t o_col = tmem + C::O_COL + t * C::DP;
       const bool leader = prefix::elect_one();
+      uint64_t* const q_bar = (p.flip | p.zero) ? &q_ready[t] : &q_full[t];
       uint32_t fill = 0;
-      uint32_t qph = 0, sph = 0, pph = 0;    // q_ready, s_free, p_ready parities
+      uint32_t qph = 0, sph = 0, pph = 0;    // q_bar, s_free, p_ready parities
       uint32_t oph = 1;                      // o_free parity (the first wait passes)
       bool mine = false;                     // the item's tiles have stages of their own
+      bool fresh = true;                     // the unit's queries are still to be waited for
       auto landed = [&](uint32_t f) { return wait_fill<C::STAGES>(full, f, abort_flag); };
       auto release = [&](uint32_t f) {
         tc_commit(&empty[f % C::STAGES]);
         if (mine) tc_commit(&empty[f % C::STAGES]);
       };
-      auto issue_qk = [&](uint32_t f) {      // scores from the K block of fill f
+      auto issue_qk = [&](uint32_t f, bool last_q) {      // scores from the K block of fill f
         if (leader) {
           const uint64_t kd = k_desc + static_cast<uint64_t>((f % C::STAGES) * (C::STAGE / 16));
 #pragma unroll
@@ -394,13 +543,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
                        kd + static_cast<uint64_t>(((j >> 2) * C::HALF + (j & 3) * 32) / 16), idesc_s, j > 0 ? 1u : 0u);
           tc_commit(&s_full[t]);
           release(f);
+          if (last_q) tc_commit(&q_free[t]);
         }
         __syncwarp();
       };
-      for (uint32_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
-        const Item it = item_at<D, true>(p, w, false);
+      for (Walk<D, true> it(p, run.begin, run.cost, false); it.more() && !abort_flag; it.next(p, false)) {
         const int nb = it.n_blocks;
-        if (nb == 0) continue;
         const uint32_t per = 2 * it.streams;
         const uint32_t f0 = fill + (it.streams == 2 ? t : 0);   // K of block b: f0 + per b; V: streams further
         fill += per * nb;
@@ -413,11 +561,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           }
           continue;
         }
-        if (!warp_wait(&q_ready[t], qph, kDetQ, abort_flag)) break;
-        qph ^= 1u;
+        const bool last_chunk = it.last_of_unit();
+        if (fresh) {
+          if (!warp_wait(q_bar, qph, kDetQ, abort_flag)) break;
+          qph ^= 1u;
+        }
+        fresh = last_chunk;
         if (!landed(f0)) break;
         tc_fence_after();
-        issue_qk(f0);
+        issue_qk(f0, last_chunk && nb == 1);
         for (int b = 0; b < nb; ++b) {
           const bool more = b + 1 < nb;
           const uint32_t fv = f0 + per * b + it.streams, fk = f0 + per * (b + 1);
@@ -426,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           if (!warp_wait(&s_free[t], sph, kDetScoresFree, abort_flag)) break;
           sph ^= 1u;
           tc_fence_after();
-          if (more) issue_qk(fk);
+          if (more) issue_qk(fk, last_chunk && b + 2 == nb);
           if (!landed(fv)) break;
           const int valid = min(BLK, it.tokens - b * BLK);
           const int steps = (valid + 15) >> 4;   // 16-token steps of P.V that hold a token
@@ -456,18 +608,50 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       bool fin = false;
       warp_wait(&done[t], 0, kDetDone, fin);
     } else if (warp == kSoftWarps + 3) {
-      // ---------------- values of draft blocks ----------------
+      // ---------------- queries of a unit, values of draft blocks ----------------
       constexpr uint32_t expo = expo_bits<T>();
       uint32_t fill = 0;
       uint32_t seen = 0;                     // raw parities, a bit a stage
-      for (uint32_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
-        const Item it = item_at<D, true>(p, w, false);
-        if (it.n_blocks == 0) continue;
+      uint32_t fph[2] = {1, 1}, qph[2] = {0, 0};   // q_free (the first wait passes) and q_full parities
+      bool fresh = true;
+      for (Walk<D, true> it(p, run.begin, run.cost, false); it.more() && !abort_flag; it.next(p, false)) {
+        if (fresh) {
+          for (int t = 0; t < it.tiles && !abort_flag; ++t) {
+            if (!warp_wait(&q_free[t], fph[t], kDetQFree, abort_flag)) break;
+            fph[t] ^= 1u;
+            uint8_t* at = s_q + t * C::QTILE;
+            const int bytes = p.rpt * p.G * 128;   // of a 64-element half; rows behind the tensor's are zero
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&q_full[t], C::NH * bytes);
+              for (int n = 0; n < C::NH; ++n)
+                tma_load_3d(at + n * C::QHALF, &maps.q, &q_full[t], n * 64, it.head(t) * p.G, it.s.row0 + it.first_row(p, t));
+            }
+            __syncwarp();
+            if (p.flip | p.zero) {
+              if (!warp_wait(&q_full[t], qph[t], kDetQ, abort_flag)) break;
+              qph[t] ^= 1u;
+              for (int e = lane; e < C::NH * bytes / 16; e += 32) {
+                const int n = e / (bytes / 16);
+                uint4* v = reinterpret_cast<uint4*>(at + n * C::QHALF) + (e - n * (bytes / 16));
+                uint4 x = *v;
+                x.x ^= p.flip;
+                x.y ^= p.flip;
+                x.z ^= p.flip;
+                x.w ^= p.flip;
+                *v = p.zero ? prefix::times_zero<T>(x) : x;
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&q_ready[t]);
+            }
+          }
+        }
+        fresh = it.last_of_unit();
         const uint32_t per = 2 * it.streams, f0 = fill;
         fill += per * it.n_blocks;
         const int first = max(0, (it.s.kv - it.t_begin) / BLK);   // the first block with drafts, if any
         for (int b = first; b < it.n_blocks && !abort_flag; ++b) {
-          if (!has_drafts(it, b)) continue;
+          if (!it.drafts(b)) continue;
           for (int i = 0; i < it.streams; ++i) {
             const uint32_t f = f0 + per * b + it.streams + i, stage = f % C::STAGES;
             if (!warp_wait(&raw[stage], (seen >> stage) & 1u, kDetRaw, abort_flag)) break;
@@ -511,6 +695,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     uint32_t ocnt = 0;                          // blocks of this tile whose weights are handed over
     uint32_t oseen = 0;                         // of them, those whose P.V this warp has waited for
     uint32_t fill = 0;
+    const int i_r = static_cast<int>(div_by(static_cast<uint32_t>(r), p.group)), g_r = r - i_r * p.G;   // draft and head of it
     // All P.V so far are done; each warp takes every phase of o_full once and in order (see dk_prefix.cuh).
     auto pv_done = [&]() {
       if (oseen == ocnt) return true;
@@ -519,87 +704,25 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       oseen = ocnt;
       return ok;
     };
-    // The tile's query rows into the swizzled K-major operand tile, asynchronously ...
-    constexpr int CPR = C::DP / 8;              // 16-byte chunks a row
-    constexpr int QN = kRows * CPR / 128;       // chunks a thread
-    auto q_at = [&](int i) {
-      const int e = i * 128 + r, row = e / CPR, c = e % CPR;
-      return s_q + t * C::QTILE + (c >> 3) * C::QHALF + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-    };
-    auto fetch_q = [&](const Item& it) {
-      const int kvh = it.kvh + (it.streams == 2 ? t : 0), m0 = it.m0 + (it.streams == 1 ? t * kRows : 0);
-#pragma unroll 4
-      for (int i = 0; i < QN; ++i) {
-        const int e = i * 128 + r, c = e % CPR;
-        const uint32_t mrow = m0 + e / CPR;
-        const bool valid = mrow < static_cast<uint32_t>(it.s.rows * p.G) && c < D / 8;
-        const uint32_t row = valid ? div_by(mrow, p.group) : 0, gh = valid ? mrow - row * p.G : 0;
-        own::cp_async16(smem_u32(q_at(i)),
-                        static_cast<const T*>(p.q) + (valid ? (it.s.row0 + row) * p.q_sr + (kvh * p.G + gh) * p.q_sh + c * 8 : 0),
-                        valid);
-      }
-    };
-    // ... and, once there, handed to the tensor cores.
-    auto q_here = [&]() {
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      if (p.flip | p.zero) {
-#pragma unroll 1
-        for (int i = 0; i < QN; ++i) {
-          uint4* at = reinterpret_cast<uint4*>(q_at(i));
-          uint4 v = *at;
-          v.x ^= p.flip;
-          v.y ^= p.flip;
-          v.z ^= p.flip;
-          v.w ^= p.flip;
-          *at = p.zero ? prefix::times_zero<T>(v) : v;
-        }
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&q_ready[t]);
-    };
-    bool q_loaded = false;
-    for (uint32_t w = blockIdx.x; w < n_items && !abort_flag; w += gridDim.x) {
-      const Item it = item_at<D, true>(p, w, false);
-      if (it.n_blocks == 0) continue;
+    for (Walk<D, true> it(p, run.begin, run.cost, false); it.more() && !abort_flag; it.next(p, false)) {
       const uint32_t per = 2 * it.streams;
       const uint32_t fv0 = fill + it.streams + (it.streams == 2 ? t : 0);   // V of block b: fv0 + per b
       fill += per * it.n_blocks;
       if (t >= it.tiles) continue;
-      const int kvh = it.kvh + (it.streams == 2 ? t : 0), m0 = it.m0 + (it.streams == 1 ? t * kRows : 0);
-      const int mg = it.s.rows * p.G, mrow = m0 + r;
-      const bool valid_row = mrow < mg;
-      const bool warp_live = m0 + (warp & 3) * 32 < mg;
-      const int row = it.s.row0 + (valid_row ? static_cast<int>(div_by(static_cast<uint32_t>(mrow), p.group)) : 0);
+      const int kvh = it.head(t), i0 = it.first_row(p, t), here = min(p.rpt, it.s.rows - i0);   // drafts of the tile
+      const bool valid_row = i_r < here;
+      const bool warp_live = (warp & 3) * 32 < here * p.G;
+      const int row = it.s.row0 + i0 + (valid_row ? i_r : 0);
       const uint64_t* mask = p.mask + row * p.mask_stride;
-      if (!q_loaded) {   // the CTA's first item with this tile; later ones are fetched ahead
-        fetch_q(it);
-        q_here();
-      }
-      q_loaded = false;
+      const uint64_t word = it.drafts(it.n_blocks - 1) ? mask[0] : 0;   // on its way long before it is asked for
       float m = -INFINITY, l = 0.0f;
       bool wild = false;
       for (int b = 0; b < it.n_blocks; ++b) {
         const bool first = b == 0, last = b + 1 == it.n_blocks;
-        const bool drafts = has_drafts(it, b);
-        uint64_t sees[BLK / 64];
-        if (drafts) {
-#pragma unroll
-          for (int h = 0; h < BLK / 64; ++h)
-            sees[h] = valid_row ? sees64(p, it.s, mask, it.t_begin + b * BLK + 64 * h) : 0;
-        }
+        const bool drafts = it.drafts(b);
         if (!warp_wait(&s_full[t], sph, kDetScores, abort_flag)) break;
         sph ^= 1u;
         tc_fence_after();
-        if (last) {   // all scores of this item are formed: q's place is free for the next one with this tile
-          for (uint32_t wn = w + gridDim.x; wn < n_items && !q_loaded; wn += gridDim.x) {
-            const Item next = item_at<D, true>(p, wn, false);
-            if (next.n_blocks > 0 && t < next.tiles) {
-              fetch_q(next);
-              q_loaded = true;
-            }
-          }
-        }
-        __syncwarp();
         if (warp_live) {
           constexpr int NR = BLK / 32;
           float s[NR][32];
@@ -610,10 +733,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           mbar_arrive(&s_free[t]);
           if (drafts) {
 #pragma unroll
-            for (int c = 0; c < NR; ++c) {
-              const uint32_t bits = static_cast<uint32_t>(sees[c >> 1] >> (32 * (c & 1)));
+            for (int h = 0; h < NR / 2; ++h) {
+              const uint64_t sees = valid_row ? sees64(p, it.s, mask, word, it.t_begin + b * BLK + 64 * h) : 0;
 #pragma unroll
-              for (int i = 0; i < 32; ++i) s[c][i] = (bits >> i & 1u) ? s[c][i] : -INFINITY;
+              for (int i = 0; i < 64; ++i) s[2 * h + (i >> 5)][i & 31] = (sees >> i & 1u) ? s[2 * h + (i >> 5)][i & 31] : -INFINITY;
             }
           }
           float mx = -INFINITY;
@@ -662,6 +785,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           const float neg = (m == -INFINITY) ? 0.0f : -m;
           const float2 c2 = make_float2(p.c, p.c), n2 = make_float2(neg, neg);
           float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+          __syncwarp();
 #pragma unroll
           for (int c = 0; c < NR; ++c) {
             uint32_t pk[16];
@@ -696,14 +820,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         tc_fence_before();
         mbar_arrive(&p_ready[t]);
         ++ocnt;
-        if (q_loaded) q_here();
         if (last) {
           if (!pv_done()) break;
           if (warp_live) {
-            const int64_t n = kvh * static_cast<int64_t>(p.n_rows) * p.G + it.s.row0 * static_cast<int64_t>(p.G) + mrow;   // state row
+            // state row
+            const int64_t n = (kvh * static_cast<int64_t>(p.n_rows) + row) * p.G + g_r;
             const bool whole = it.s.n_chunks == 1;   // the output, at once
             float4* dst = reinterpret_cast<float4*>(p.st_o) + static_cast<int64_t>(it.chunk) * (D / 4) * p.st_rows + n;
-            T* out = static_cast<T*>(p.out) + row * p.o_sr + (kvh * p.G + mrow - (row - it.s.row0) * p.G) * p.o_sh;
+            T* out = static_cast<T*>(p.out) + row * p.o_sr + (kvh * p.G + g_r) * p.o_sh;
             const bool empty = whole && valid_row && l == 0.0f && sees_nothing(p, it.s, mask);
             if (!whole && valid_row)
               *reinterpret_cast<float2*>(p.st_ml + 2 * (it.chunk * p.st_rows + n)) = make_float2(m, l);
@@ -760,19 +884,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 constexpr int kJoinThreads = 256;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p, int row_tiles) {
+__global__ void __launch_bounds__(kJoinThreads, 3) join_kernel(const __grid_constant__ Params p, int row_tiles) {
   constexpr int WARPS = kJoinThreads / 32, Q = D / 4 / WARPS, UN = Q >= 4 ? 2 : 4;   // quads a warp; states in flight
   __shared__ __align__(16) T s_out[32][D + 2];
-  pdl_wait();
-  if (threadIdx.x == 0) pdl_launch_dependents();
+  // (lengths and offsets were there before tree_kernel, which has waited for them before it let this kernel begin)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t tile = blockIdx.x % row_tiles, rest = blockIdx.x / row_tiles;
   const int kvh = static_cast<int>(rest % p.hkv), b = static_cast<int>(rest / p.hkv);
   const Seq s = seq_at<D, true>(p, b, false);
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
   const int m0 = static_cast<int>(tile) * 32, mg = s.rows * p.G;
   if (s.n_chunks <= 1 || m0 >= mg) return;
   const bool live = m0 + lane < mg;
-  const int64_t n = kvh * static_cast<int64_t>(p.n_rows) * p.G + s.row0 * static_cast<int64_t>(p.G) + m0 + (live ? lane : 0);
+  const int64_t n = (kvh * static_cast<int64_t>(p.n_rows) + s.row0) * p.G + m0 + (live ? lane : 0);
   const float4* src = reinterpret_cast<const float4*>(p.st_o) + static_cast<int64_t>(warp) * Q * p.st_rows + n;
   const float2* mls = reinterpret_cast<const float2*>(p.st_ml) + n;
   const int64_t state = p.st_rows * (D / 4);
