@@ -22,9 +22,9 @@ int64_t max_chunks(int64_t max_kv_len, int64_t max_rows, int D) {
   int64_t most = 1;
   // a chunk's size is constant between these lengths of the cached part, or grows with it
   const int64_t last = D <= 64 ? 32768 : 16384;
-  for (int64_t kv : {int64_t{2048}, last, max_kv_len}) {
+  for (int64_t kv : {int64_t{4096}, last, max_kv_len}) {
     kv = std::min(kv, max_kv_len);
-    most = std::max(most, ceil_div(std::min(kv + max_rows, max_kv_len), dk::prefix::chunk_tokens(kv, D)));
+    most = std::max(most, ceil_div(std::min(kv + max_rows, max_kv_len), dk::tree::chunk_tokens(kv, D)));
   }
   // beyond `last` a chunk holds at least a 32nd (D <= 64) or 16th of the cached part
   if (max_kv_len > last) most = std::max(most, (D <= 64 ? 32 : 16) + ceil_div(max_rows, 1024) + 1);

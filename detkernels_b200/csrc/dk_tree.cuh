@@ -4,7 +4,7 @@
 //
 // The query heads of all of a sequence's rows on KV head h are the rows of one matrix Q [t G, D], so that the cache is
 // read once for the whole tree: S = Q K^T scale, out = softmax(S + mask) V.  Fixed reduction structure (the definition of
-// a row's bits): the sequence's tokens are cut into chunks whose size follows kv and head_dim only (prefix::chunk_tokens), a
+// a row's bits): the sequence's tokens are cut into chunks whose size follows kv and head_dim only (chunk_tokens), a
 // chunk's softmax state (m, l, O) is formed block by block as in dk_prefix.cuh, and the chunks' states are joined in
 // order.  No step looks at another row: a chunk of which a row sees nothing joins with weight 0.
 //
@@ -108,6 +108,14 @@ struct Cfg {
   static_assert(P_COL + BLK <= O_COL, "TMEM");
 };
 
+// Tokens a chunk: a function of the cached tokens and head_dim alone.
+__host__ __device__ inline int64_t chunk_tokens(int64_t kv, int head_dim) {
+  if (kv <= 4096) return 512;
+  if (head_dim <= 64) return 1024 * ((kv + 32767) / 32768);
+  if (kv <= 16384) return 1024;
+  return ((kv + 15) / 16 + 127) / 128 * 128;
+}
+
 // A sequence's extents; nothing (rows = 0) where they are bad.
 struct Seq {
   int row0, rows, kv, total, chunk, n_chunks;
@@ -135,7 +143,7 @@ __device__ __forceinline__ Seq seq_at(const Params& p, int b, bool report) {
     return s;
   }
   s.total = s.kv + s.rows;
-  s.chunk = static_cast<int>(prefix::chunk_tokens(s.kv, D));
+  s.chunk = static_cast<int>(chunk_tokens(s.kv, D));
   s.n_chunks = (s.total + s.chunk - 1) / s.chunk;
   return s;
 }
@@ -147,7 +155,7 @@ struct Cost {
 };
 // What an item costs beside its blocks (states out, the first scores), in blocks.
 template <int D>
-constexpr int kItemCost = D == 128 ? 2 : 1;
+constexpr int kItemCost = D == 128 ? 3 : 2;
 
 template <int D>
 __device__ __forceinline__ Cost cost_of(const Params& p, const Seq& s) {
@@ -829,6 +837,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             float4* dst = reinterpret_cast<float4*>(p.st_o) + static_cast<int64_t>(it.chunk) * (D / 4) * p.st_rows + n;
             T* out = static_cast<T*>(p.out) + row * p.o_sr + (kvh * p.G + g_r) * p.o_sh;
             const bool empty = whole && valid_row && l == 0.0f && sees_nothing(p, it.s, mask);
+            const float inv = __frcp_rn(l);   // one more rounding of 2^-24 an output, before the type's
             if (!whole && valid_row)
               *reinterpret_cast<float2*>(p.st_ml + 2 * (it.chunk * p.st_rows + n)) = make_float2(m, l);
 #pragma unroll 1
@@ -848,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
                 uint32_t u[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                  u[i] = empty ? 0u : pack2<T>(__fdiv_rn(o[2 * i], l), __fdiv_rn(o[2 * i + 1], l));
+                  u[i] = empty ? 0u : pack2<T>(__fmul_rn(o[2 * i], inv), __fmul_rn(o[2 * i + 1], inv));
                 if (p.o_vec) {
 #pragma unroll
                   for (int i = 0; i < 4; ++i)
@@ -935,11 +944,12 @@ __global__ void __launch_bounds__(kJoinThreads, 3) join_kernel(const __grid_cons
   }
   const int row = s.row0 + (live ? static_cast<int>(div_by(static_cast<uint32_t>(m0 + lane), p.group)) : 0);
   const bool empty = live && tl == 0.0f && sees_nothing(p, s, p.mask + row * p.mask_stride);
+  const float inv = __frcp_rn(tl);
 #pragma unroll
   for (int i = 0; i < Q; ++i) {
     T* d = &s_out[lane][(warp * Q + i) * 4];
-    *reinterpret_cast<uint32_t*>(d) = empty ? 0u : pack2<T>(__fdiv_rn(to[i].x, tl), __fdiv_rn(to[i].y, tl));
-    *reinterpret_cast<uint32_t*>(d + 2) = empty ? 0u : pack2<T>(__fdiv_rn(to[i].z, tl), __fdiv_rn(to[i].w, tl));
+    *reinterpret_cast<uint32_t*>(d) = empty ? 0u : pack2<T>(__fmul_rn(to[i].x, inv), __fmul_rn(to[i].y, inv));
+    *reinterpret_cast<uint32_t*>(d + 2) = empty ? 0u : pack2<T>(__fmul_rn(to[i].z, inv), __fmul_rn(to[i].w, inv));
   }
   __syncthreads();
   for (int k = warp; k < 32 && m0 + k < mg; k += WARPS) {

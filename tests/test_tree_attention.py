@@ -149,9 +149,9 @@ def test_entry_point_refuses_on_the_host():
     assert size(8, 8, 8, 64, 512) == 0 and size(8, 8, 8, 64, 700) >= 2 * 64 * 66 * 4
     # a chunk's number never exceeds what the workspace was sized for
     for D in (64, 128):
-        for kv in (0, 511, 2048, 2049, 9000, 16384, 16385, 20000, 32768, 32769, 70001, 1000003):
+        for kv in (0, 511, 2048, 2049, 4096, 4097, 9000, 16384, 16385, 20000, 32768, 32769, 70001, 1000003):
             for t in (1, 64, 700, 5000):
-                chunk = (512 if kv <= 2048 else 1024 * -(-kv // 32768) if D == 64 else 1024 if kv <= 16384 else
+                chunk = (512 if kv <= 4096 else 1024 * -(-kv // 32768) if D == 64 else 1024 if kv <= 16384 else
                          -(-(-(-kv // 16)) // 128) * 128)
                 n = -(-(kv + t) // chunk)
                 assert n == 1 or size(1, t, 1, D, kv + t) >= n * (D + 2) * 4, (D, kv, t)
