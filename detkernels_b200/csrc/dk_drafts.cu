@@ -86,9 +86,13 @@ int check_pools(const Pools& c, const char* what) {
 }
 
 template <typename V>
-cudaError_t move_launch(const dk::pages::MoveParams& p, int64_t grid, cudaStream_t st) {
-  return launch_pdl(dk::pages::move_kernel<V, 8>, dim3(static_cast<unsigned>(grid)), dim3(dk::pages::kMoveThreads), 0,
-                    st, p);
+cudaError_t move_launch(const dk::pages::MoveParams& p, int64_t grid, bool after_another, cudaStream_t st) {
+  const dim3 g(static_cast<unsigned>(grid)), t(dk::pages::kMoveThreads);
+  if (p.src) return launch_pdl(dk::pages::move_kernel<V, 8, true>, g, t, 0, st, p);
+  if (!after_another) return launch_pdl(dk::pages::move_kernel<V, 8, false>, g, t, 0, st, p);
+  // the kernel before this one is another part of the pools' move, not release_kernel: it is waited for in whole
+  dk::pages::move_kernel<V, 8, false><<<g, t, 0, st>>>(p);
+  return cudaGetLastError();
 }
 
 // Moves the tokens of `n` sequences, at most `most` each, in every pool.
@@ -122,11 +126,11 @@ int move(dk::pages::MoveParams& p, const Pools& c, int64_t n, int64_t most, cons
                      : 1;
     const int64_t grid = units * p.splits;
     if (grid > kI32Max) return fail(DK_ERR_INVALID_ARGUMENT, "%s: too many sequences", what);
-    cudaError_t e = wide          ? move_launch<uint4>(p, grid, st)
-                    : c.size == 1 ? move_launch<uint8_t>(p, grid, st)
-                    : c.size == 2 ? move_launch<uint16_t>(p, grid, st)
-                    : c.size == 4 ? move_launch<uint32_t>(p, grid, st)
-                                  : move_launch<uint64_t>(p, grid, st);
+    cudaError_t e = wide          ? move_launch<uint4>(p, grid, first > 0, st)
+                    : c.size == 1 ? move_launch<uint8_t>(p, grid, first > 0, st)
+                    : c.size == 2 ? move_launch<uint16_t>(p, grid, first > 0, st)
+                    : c.size == 4 ? move_launch<uint32_t>(p, grid, first > 0, st)
+                                  : move_launch<uint64_t>(p, grid, first > 0, st);
     if (e != cudaSuccess) return fail(DK_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
   }
   return DK_OK;
@@ -147,7 +151,7 @@ int check_ws(const void* ws, size_t given, size_t need, const char* what) {
   return DK_OK;
 }
 
-size_t fork_ws_bytes(int64_t rows) { return static_cast<size_t>(dk::pages::kWsMark + rows) * sizeof(int32_t); }
+size_t fork_ws_bytes(int64_t rows) { return static_cast<size_t>(dk::pages::kWsMark + 2 * rows) * sizeof(int32_t); }
 size_t compact_ws_bytes() { return static_cast<size_t>(dk::pages::kWsMark) * sizeof(int32_t); }
 
 }  // namespace
@@ -264,6 +268,7 @@ int dk_paged_fork(int32_t* block_table, int64_t block_table_stride, int32_t tabl
   m.src = src;
   m.dst = dst;
   m.all = shares == nullptr;
+  m.width = blocks_per_seq;
   m.ws = p.ws;
   const int64_t most = shares ? page_size - 1 : static_cast<int64_t>(blocks_per_seq) * page_size;
   return move(m, c, n_forks, most, what, st);
@@ -290,8 +295,8 @@ int dk_paged_compact(const int32_t* block_table, int64_t block_table_stride, int
   if (shares && !free_blocks) return fail(DK_ERR_INVALID_ARGUMENT, "%s: shares need a free list", what);
   if (free_blocks && (!cursor || !cursor_out))
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: a free list needs its cursor", what);
-  if (shares && static_cast<int64_t>(n_seqs) * blocks_per_seq > kI32Max - 2)
-    return fail(DK_ERR_INVALID_ARGUMENT, "%s: more than 2^31 table entries with shares", what);
+  if (shares && static_cast<int64_t>(n_seqs) * blocks_per_seq >= 1LL << 30)
+    return fail(DK_ERR_INVALID_ARGUMENT, "%s: 2^30 table entries or more with shares", what);
   if (n_seqs == 0) return DK_OK;
   if (!kv_lens || !new_lens || !n_keep || !lens_out || lens_out == kv_lens || lens_out == new_lens || lens_out == n_keep)
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: null pointer, or lens_out is one of the inputs", what);
@@ -329,6 +334,8 @@ int dk_paged_compact(const int32_t* block_table, int64_t block_table_stride, int
   m.n_keep = n_keep;
   m.keep = keep;
   m.keep_stride = keep_stride;
+  m.keep_width = keep_width;
+  m.width = blocks_per_seq;
   m.ws = p.ws;
   return move(m, c, n_seqs, keep_width, what, st);
 }

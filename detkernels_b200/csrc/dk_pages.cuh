@@ -11,8 +11,9 @@
 //
 // Either is one kernel that checks everything, and only then changes the tables (fork_kernel, release_kernel), and
 // one that moves tokens in all layers' pools (move_kernel).  The first is bound by the latency of a few dependent
-// look-ups and barriers: one cluster of eight CTAs, whose barrier needs no memory that anybody has to clear, a warp
-// a run of consecutive sequences.  The second is bound by the bytes it copies.
+// look-ups and barriers: one cluster of eight CTAs, a warp a run of consecutive sequences, whose flags and counts go
+// into every CTA's shared memory, so that a barrier of the cluster is all that stands between two phases and no
+// scratch has to be cleared.  The second is bound by the bytes it copies.
 #pragma once
 
 #include "dk_common.cuh"
@@ -37,32 +38,48 @@ enum : int {
   kDetShares = 0x646,     // a page with fewer holders than give it back
 };
 
-// Scratch, int32: [0] the plan stands, [1 .. 8] a flag a CTA, [16 ..] a count a warp, then a mark a table row (fork).
-constexpr int kWsOk = 0, kWsBad = 1, kWsCount = 16, kWsMark = kWsCount + kPlanWarps;
+// Scratch, int32: [0] the plan stands, then two marks a table row (fork).
+constexpr int kWsOk = 0, kWsMark = 16;
 
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+// What the CTAs of the cluster tell one another: by round, whether a CTA has found something wrong; a count a warp.
+struct Told {
+  int bad[4][kPlanCtas];
+  int count[2][kPlanWarps];
+};
+
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
-
-// A barrier of the cluster that says whether any thread had `bad`; `round` alternates between calls that follow one
-// another (a CTA may still read one round's flags while another writes the next's).
-__device__ __forceinline__ bool cluster_any(bool bad, int32_t* flags) {
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync() {
+  cluster_arrive();
+  cluster_wait();
+}
+// Writes a word of CTA `rank`'s shared memory.
+__device__ __forceinline__ void tell(int* mine, int rank, int v) {
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(rank));
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+// A barrier of the cluster, with this warp's count for all (slot 0 or 1), that says whether any thread had `bad`.
+__device__ __forceinline__ bool cluster_any(Told& told, int round, bool bad, int slot, int count) {
+  const int lane = threadIdx.x & 31, w = blockIdx.x * (kPlanThreads / 32) + (threadIdx.x >> 5);
+  if (lane < kPlanCtas) tell(&told.count[slot][w], lane, count);
   const int mine = __syncthreads_or(bad);
-  if (threadIdx.x == 0) __stcg(flags + blockIdx.x, mine);
+  if (threadIdx.x < kPlanCtas) tell(&told.bad[round][blockIdx.x], threadIdx.x, mine);
   cluster_sync();
   int any = 0;
 #pragma unroll
-  for (int c = 0; c < kPlanCtas; ++c) any |= __ldcg(flags + c);
-  cluster_sync();   // everyone has read them
+  for (int c = 0; c < kPlanCtas; ++c) any |= told.bad[round][c];
   return any != 0;
 }
 
-// What the warps before this one counted, and what all did (after a cluster barrier).
-__device__ __forceinline__ void warp_prefix(const int32_t* count, int w, int lane, int64_t& before, int64_t& total) {
+// What the warps before this one counted, and what all did.
+__device__ __forceinline__ void warp_prefix(const int (&count)[kPlanWarps], int w, int lane, int64_t& before, int64_t& total) {
   int64_t b = 0, t = 0;
 #pragma unroll
   for (int i = 0; i < kPlanWarps / 32; ++i) {
-    const int64_t c = __ldcg(count + i * 32 + lane);
+    const int64_t c = count[i * 32 + lane];
     t += c;
     if (i * 32 + lane < w) b += c;
   }
@@ -94,16 +111,18 @@ struct ForkParams {
 };
 
 __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) fork_kernel(const ForkParams p) {
+  __shared__ Told told;
+  cluster_arrive();   // this CTA has begun
   pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int w = blockIdx.x * (kPlanThreads / 32) + (threadIdx.x >> 5);
   const int per = (p.n + kPlanWarps - 1) / kPlanWarps;
   const int i0 = min(static_cast<int64_t>(p.n), static_cast<int64_t>(w) * per), i1 = min(p.n, i0 + per);
-  int32_t* mark = p.ws + kWsMark;
-  const uint32_t page = p.page.d;
-  for (int64_t r = blockIdx.x * kPlanThreads + threadIdx.x; r < p.rows; r += kPlanCtas * kPlanThreads) mark[r] = 0;
-  cluster_sync();
+  // A row's marks: a fork that it is the source of, and one that it is the destination of.  They are never cleared: what
+  // a mark names is looked up.
+  int32_t *as_src = p.ws + kWsMark, *as_dst = as_src + p.rows;
+  const int64_t cursor = *p.cursor_in;
   // rows and lengths; what the new pages are
   bool bad = false;
   int64_t need = 0;
@@ -114,11 +133,8 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
       bad = true;
       continue;
     }
-    atomicOr(&mark[s], 1);
-    if (atomicOr(&mark[d], 2) & 2) {
-      report_error(DK_ERR_DEVICE_CHECK, kDetForkRows);
-      bad = true;
-    }
+    __stcg(as_src + s, i);
+    __stcg(as_dst + d, i);
     const int n = p.kv[s];
     if (n < 0 || ceil_div32(n, p.page) > static_cast<uint32_t>(p.width)) {
       report_error(DK_ERR_DEVICE_CHECK, kDetForkLens);
@@ -126,26 +142,24 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
       continue;
     }
     const uint32_t whole = div_by(n, p.page);
-    need += (p.shares ? 0 : whole) + (n != static_cast<int>(whole * page));
+    need += (p.shares ? 0 : whole) + (n != static_cast<int>(whole * p.page.d));
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) need += __shfl_xor_sync(0xffffffffu, need, d);
-  // beyond 2^31 blocks no list holds them: the sum of the warps' counts stays inside 64 bits and is refused
-  if (lane == 0) __stcg(p.ws + kWsCount + w, static_cast<int32_t>(need < 0x7fffffff ? need : 0x7fffffff));
-  bad = cluster_any(bad, p.ws + kWsBad);
+  cluster_wait();     // all have begun
+  bad = cluster_any(told, 0, bad, 0, static_cast<int>(need < 0x7fffffff ? need : 0x7fffffff));
   int64_t at = 0, total = 0;
-  const int64_t cursor = *p.cursor_in;
   if (!bad) {
-    warp_prefix(p.ws + kWsCount, w, lane, at, total);
+    warp_prefix(told.count[0], w, lane, at, total);
     at += cursor;
     if (cursor < 0 || cursor + total > p.n_free) {
       if (w == 0 && lane == 0) report_error(DK_ERR_DEVICE_CHECK, kDetPool);
       bad = true;
     }
-    // no destination is a source, and all blocks are of the pool
+    // each destination is one fork's, and no source; all blocks are of the pool
     int64_t a = at;
     for (int i = i0; i < i1 && !bad; ++i) {
-      const int s = p.src[i], n = p.kv[s], np = ceil_div32(n, p.page), whole = div_by(n, p.page);
+      const int s = p.src[i], d = p.dst[i], n = p.kv[s], np = ceil_div32(n, p.page), whole = div_by(n, p.page);
       const int kept = p.shares ? whole : 0;
       bool wrong = false;
       for (int j = lane; j < np; j += 32) {
@@ -154,7 +168,8 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
         wrong |= x < 0 || x >= p.n_blocks || y < 0 || y >= p.n_blocks;
       }
       if (wrong) report_error(DK_ERR_DEVICE_CHECK, kDetBlock);
-      if (__ldcg(mark + p.dst[i]) & 1) {
+      const int named = __ldcg(as_src + d);
+      if (__ldcg(as_dst + d) != i || (named >= 0 && named < p.n && p.src[named] == d)) {
         if (lane == 0) report_error(DK_ERR_DEVICE_CHECK, kDetForkRows);
         wrong = true;
       }
@@ -162,7 +177,7 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
       a += np - kept;
     }
   }
-  bad = cluster_any(bad, p.ws + kWsBad);
+  bad = cluster_any(told, 1, bad, 1, 0);
   if (w == 0 && lane == 0) {
     p.ws[kWsOk] = bad ? 0 : 1;
     *p.cursor_out = static_cast<int32_t>(bad ? cursor : cursor + total);
@@ -208,31 +223,35 @@ struct ReleaseParams {
   int32_t* ws;
 };
 
+// Entries of a row of `keep` that a warp checks at a time: a few long rows are shared by many warps.
+constexpr int kKeepRun = 512;
+
 __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) release_kernel(const ReleaseParams p) {
+  __shared__ Told told;
+  cluster_arrive();   // this CTA has begun
   pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int w = blockIdx.x * (kPlanThreads / 32) + (threadIdx.x >> 5);
   const int per = (p.n + kPlanWarps - 1) / kPlanWarps;
   const int b0 = min(static_cast<int64_t>(p.n), static_cast<int64_t>(w) * per), b1 = min(p.n, b0 + per);
-  int32_t* flags = p.ws + kWsBad;
   const bool back = p.free_list != nullptr;
+  const int64_t cursor = back ? *p.cursor_in : 0;
   bool bad = false;
   int64_t given = 0;   // pages of this warp's sequences that come back
   auto first_page = [&](int b) { return static_cast<int>(ceil_div32(p.kv[b] + p.n_keep[b], p.page)); };
   auto last_page = [&](int b) { return static_cast<int>(ceil_div32(p.kv[b] + p.nw[b], p.page)); };
-  for (int b = b0; b < b1; ++b) {
-    const int64_t kv = p.kv[b], nw = p.nw[b], nk = p.n_keep[b];
-    if (kv < 0 || nw < 0 || nk < 0 || nk > nw || kv + nw > 0x7fffffff || (p.keep && nk > p.keep_width) ||
-        ceil_div32(static_cast<uint32_t>(kv + nw), p.page) > static_cast<uint32_t>(p.width)) {
-      if (lane == 0) report_error(DK_ERR_DEVICE_CHECK, kDetLens);
-      bad = true;
-      continue;
-    }
-    if (p.keep) {
+  if (p.keep) {
+    const int runs = (p.keep_width + kKeepRun - 1) / kKeepRun;
+    for (int64_t e = w; e < static_cast<int64_t>(p.n) * runs; e += kPlanWarps) {
+      const int b = static_cast<int>(e / runs);
+      const int64_t j0 = (e - static_cast<int64_t>(b) * runs) * kKeepRun;
+      const int nw = p.nw[b], nk = p.n_keep[b];
+      if (nk > nw || nk > p.keep_width) continue;   // refused below
       const int32_t* row = p.keep + b * p.keep_stride;
+      const int64_t j1 = j0 + kKeepRun < nk ? j0 + kKeepRun : nk;
       bool wrong = false;
-      for (int64_t j = lane; j < nk; j += 32) {
+      for (int64_t j = j0 + lane; j < j1; j += 32) {
         const int k = row[j];
         wrong |= k < 0 || k >= nw || (j > 0 && row[j - 1] >= k);
       }
@@ -240,6 +259,15 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
         report_error(DK_ERR_DEVICE_CHECK, kDetKeep);
         bad = true;
       }
+    }
+  }
+  for (int b = b0; b < b1; ++b) {
+    const int64_t kv = p.kv[b], nw = p.nw[b], nk = p.n_keep[b];
+    if (kv < 0 || nw < 0 || nk < 0 || nk > nw || kv + nw > 0x7fffffff || (p.keep && nk > p.keep_width) ||
+        ceil_div32(static_cast<uint32_t>(kv + nw), p.page) > static_cast<uint32_t>(p.width)) {
+      if (lane == 0) report_error(DK_ERR_DEVICE_CHECK, kDetLens);
+      bad = true;
+      continue;
     }
     if (back) {
       const int lo = first_page(b), hi = last_page(b);
@@ -255,10 +283,9 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
       given += max(0, hi - lo);
     }
   }
-  const int64_t cursor = back ? *p.cursor_in : 0;
+  cluster_wait();     // all have begun
   // Without shares every page comes back, and that is known here already.
-  if (lane == 0) __stcg(p.ws + kWsCount + w, static_cast<int32_t>(given < 0x7fffffff ? given : 0x7fffffff));
-  bad = cluster_any(bad, flags);
+  bad = cluster_any(told, 0, bad, 0, static_cast<int>(given < 0x7fffffff ? given : 0x7fffffff));
   auto each_page = [&](auto&& f) {   // (sequence, column, block) of the warp's pages, a lane each; all lanes call f
     for (int b = b0; b < b1; ++b) {
       const int lo = first_page(b), hi = last_page(b);
@@ -268,46 +295,45 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
       }
     }
   };
-  // The page's place in the order of all, as a negative number that no count of holders is.
-  auto code = [&](int b, int j) { return -2 - (b * p.width + j); };
+  // The page's place in the order of all, as a number below any that a count of holders falls to.
+  constexpr int kClaim = -(1 << 30);
+  auto code = [&](int b, int j) { return kClaim - (b * p.width + j); };
   int64_t at = 0, total = 0;
   if (back && !bad) {
     if (p.shares) {
       // one holder less a page ...
       each_page([&](int, int, int x) { if (x >= 0) atomicSub(&p.shares[x], 1); });
       cluster_sync();
+      // ... and where none is left, the last of those that gave it up hands it back
       bool over = false;
-      each_page([&](int, int, int x) { if (x >= 0) over |= __ldcg(p.shares + x) < -1; });
+      each_page([&](int b, int j, int x) {
+        if (x < 0) return;
+        const int v = __ldcg(p.shares + x);
+        if (v == -1 || v <= kClaim) atomicMin(&p.shares[x], code(b, j));
+        else if (v < -1) over = true;
+      });
       if (over) report_error(DK_ERR_DEVICE_CHECK, kDetShares);
-      bad = cluster_any(over, flags);
-      if (!bad) {
-        // ... and where none is left, the last of those that gave it up hands it back
-        each_page([&](int b, int j, int x) {
-          if (x >= 0 && __ldcg(p.shares + x) < 0) atomicMin(&p.shares[x], code(b, j));
-        });
-        cluster_sync();
-        given = 0;
-        each_page([&](int b, int j, int x) { given += x >= 0 && __ldcg(p.shares + x) == code(b, j); });
+      bad = cluster_any(told, 1, over, 1, 0);
+      given = 0;
+      each_page([&](int b, int j, int x) { given += x >= 0 && __ldcg(p.shares + x) == code(b, j); });
 #pragma unroll
-        for (int d = 16; d; d >>= 1) given += __shfl_xor_sync(0xffffffffu, given, d);
-        if (lane == 0) __stcg(p.ws + kWsCount + w, static_cast<int32_t>(given));
-        cluster_sync();
-      }
+      for (int d = 16; d; d >>= 1) given += __shfl_xor_sync(0xffffffffu, given, d);
+      cluster_any(told, 2, false, 0, static_cast<int>(given));
     }
     if (!bad) {
-      warp_prefix(p.ws + kWsCount, w, lane, at, total);
+      warp_prefix(told.count[0], w, lane, at, total);
       if (total > cursor || cursor > p.n_free) {
         if (w == 0 && lane == 0) report_error(DK_ERR_DEVICE_CHECK, kDetPool);
         bad = true;   // the same for every thread
-        if (p.shares) {   // the claims go, then the holders come back
-          each_page([&](int b, int j, int x) {
-            if (x >= 0 && __ldcg(p.shares + x) == code(b, j)) __stcg(p.shares + x, -1);
-          });
-          cluster_sync();
-        }
       }
     }
-    if (bad && p.shares) each_page([&](int, int, int x) { if (x >= 0) atomicAdd(&p.shares[x], 1); });
+    if (bad && p.shares) {   // the claims go, then the holders come back
+      each_page([&](int b, int j, int x) {
+        if (x >= 0 && __ldcg(p.shares + x) == code(b, j)) __stcg(p.shares + x, -1);
+      });
+      cluster_sync();
+      each_page([&](int, int, int x) { if (x >= 0) atomicAdd(&p.shares[x], 1); });
+    }
   }
   if (w == 0 && lane == 0) {
     p.ws[kWsOk] = bad ? 0 : 1;
@@ -346,6 +372,7 @@ struct MoveParams {
   const int32_t* n_keep;   // compact
   const int32_t* keep;
   int64_t keep_stride;
+  int32_t keep_width, width;   // width: entries of a table row
   int32_t cols_log;        // log2 of the columns a CTA takes at once; the other threads are token lanes
   int32_t col_groups, splits;
   const int32_t* ws;
@@ -355,18 +382,23 @@ struct MoveParams {
 // the tokens, (threads / columns) * U at a time: their places first, into shared memory, then all loads, then all
 // stores.  Compacting in place needs no more order than that: a token moves down or not at all, so what one step
 // writes lies below everything that a later step reads, and inside a step the barrier parts loads from stores.
-template <typename V, int U>
+// FORK: the destinations' rows are fork_kernel's, so nothing is read before it has ended.  A compaction reads its first
+// tokens while release_kernel still runs, which has itself waited for whatever wrote them, and changes none of what is
+// read here; it stores once that has said that all is well.
+template <typename V, int U, bool FORK>
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ MoveParams p) {
   __shared__ int64_t s_from[kMoveThreads * U], s_to[kMoveThreads * U];
-  pdl_wait();
-  if (threadIdx.x == 0) pdl_launch_dependents();
-  if (__ldcg(p.ws + kWsOk) == 0) return;
+  if (FORK) {
+    pdl_wait();
+    if (threadIdx.x == 0) pdl_launch_dependents();
+    if (__ldcg(p.ws + kWsOk) == 0) return;
+  }
   const uint32_t group = blockIdx.x % p.col_groups, rest = blockIdx.x / p.col_groups;
   const uint32_t split = rest % p.splits, i = rest / p.splits;
   const int cols = 1 << p.cols_log, lanes = kMoveThreads >> p.cols_log, step = lanes * U;
   const int32_t *row_from, *row_to, *keep = nullptr;
   int base, count;
-  if (p.src) {
+  if (FORK) {
     const int s = p.src[i], d = p.dst[i], n = p.kv[s];
     row_from = p.table + s * p.table_stride;
     row_to = p.table + d * p.table_stride;
@@ -377,6 +409,8 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
     base = p.kv[i];
     count = p.n_keep[i];
     keep = p.keep + i * p.keep_stride;
+    // (what release_kernel refuses is not looked up out of bounds either)
+    if (base < 0 || count < 0 || count > p.keep_width) base = count = 0;
   }
   // this CTA's share of the tokens, in whole steps (a compaction has one share)
   const int64_t per = ((count + static_cast<int64_t>(step) * p.splits - 1) / (static_cast<int64_t>(step) * p.splits)) * step;
@@ -388,20 +422,23 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
     const int v = col % p.vecs, hp = col / p.vecs, h = hp % p.heads, pool = hp / p.heads;
     at = static_cast<V*>(p.pool[pool]) + h * p.s_head + v;
   }
+  bool waited = FORK, lost = false;   // lost: a block that does not exist
   for (int64_t t0 = begin; t0 < end; t0 += step) {
     for (int e = threadIdx.x; e < step; e += kMoveThreads) {
       const int64_t j = t0 + e;
       int64_t from = -1, to = -1;
       if (j < end) {
-        const int tf = base + static_cast<int>(keep ? keep[j] : j), tt = base + static_cast<int>(j);
-        if (row_from != row_to || tf != tt) {
-          const uint32_t pf = div_by(tf, p.page), pt = div_by(tt, p.page);
-          const int bf = row_from[pf], bt = row_to[pt];
-          if (bf < 0 || bf >= p.n_blocks || bt < 0 || bt >= p.n_blocks) {
-            report_error(DK_ERR_DEVICE_CHECK, kDetBlock);
+        const int64_t tf = base + static_cast<int64_t>(FORK ? j : keep[j]), tt = base + j;
+        if (FORK || tf != tt) {
+          const uint32_t pf = div_by(static_cast<uint32_t>(tf), p.page), pt = div_by(static_cast<uint32_t>(tt), p.page);
+          const bool in = tf >= 0 && tf <= 0x7fffffff && tt <= 0x7fffffff && pf < static_cast<uint32_t>(p.width) &&
+                          pt < static_cast<uint32_t>(p.width);
+          const int bf = in ? row_from[pf] : -1, bt = in ? row_to[pt] : -1;
+          if (bf >= 0 && bf < p.n_blocks && bt >= 0 && bt < p.n_blocks) {
+            from = bf * p.s_block + (tf - static_cast<int64_t>(pf) * p.page.d) * p.s_tok;
+            to = bt * p.s_block + (tt - static_cast<int64_t>(pt) * p.page.d) * p.s_tok;
           } else {
-            from = bf * p.s_block + (tf - static_cast<int>(pf * p.page.d)) * p.s_tok;
-            to = bt * p.s_block + (tt - static_cast<int>(pt * p.page.d)) * p.s_tok;
+            lost = true;
           }
         }
       }
@@ -417,6 +454,13 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
         if (f >= 0) v[u] = at[f];
       }
     }
+    if (!waited) {
+      pdl_wait();
+      if (threadIdx.x == 0) pdl_launch_dependents();
+      if (__ldcg(p.ws + kWsOk) == 0) return;
+      waited = true;
+    }
+    if (lost) report_error(DK_ERR_DEVICE_CHECK, kDetBlock);
     __syncthreads();   // all of the step's tokens are read
     if (at) {
 #pragma unroll
@@ -427,6 +471,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
     }
     __syncthreads();   // the places are free for the next step
   }
+  if (!waited) pdl_wait();   // a kernel's end means the end of all before it
 }
 
 }  // namespace pages
