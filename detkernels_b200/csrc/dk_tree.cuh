@@ -11,8 +11,9 @@
 // Work: an item is (sequence, up to two tiles of at most 128 rows, chunk): two tiles of one KV head, which then share K
 // and V, or, where the rows fit one tile, the tiles of two KV heads, each with its own K and V.  Either way both softmax
 // warpgroups have work, and take turns on the exponential unit.  One persistent CTA an SM takes a run of items in the order
-// (sequence, tiles, chunk), so that a run's chunks share their queries; the runs are cut at equal shares of the tokens'
-// and the items' cost, which every CTA finds for itself from the lengths.  A TMA warp, an MMA warp a tile (scores,
+// (sequence, KV heads, chunk, tiles), so that one pair of tiles keeps its queries over a run's chunks, and several pairs find
+// a chunk's keys in L2; the runs are cut at equal shares of the tokens' and the items' cost, which every CTA finds for
+// itself from the lengths.  A TMA warp, an MMA warp a tile (scores,
 // weights and accumulator apart in TMEM), a warpgroup a tile for the softmax, a row a thread, and a warp that fetches the
 // queries and makes the values of draft blocks safe: 0 weights must meet neither what lies behind the sequence in its last
 // page nor a non-finite value of a draft that some rows do not see.  Those elements become 0 in shared memory, and rows
@@ -148,10 +149,13 @@ __device__ __forceinline__ Seq seq_at(const Params& p, int b, bool report) {
   return s;
 }
 
-// The items of a sequence: units (pairs of tiles, or of heads) and the cost of one's chunks, in blocks.
+// The items of a sequence: units (KV heads, or pairs of them where the rows fit a tile), of each its chunks, of each the
+// pairs of tiles, which so find the chunk's keys in L2; and their cost, in blocks.
 struct Cost {
-  int units, pairs;      // pairs of tiles a KV head; 0: pairs of heads
-  int chunk, unit;       // cost of a whole chunk, of a unit
+  int units, pairs;      // pairs: of tiles a KV head; 0: pairs of heads
+  int inner;             // items a (unit, chunk)
+  int chunk, last;       // cost of an item of a whole chunk, of the last one
+  int64_t unit;          // of a unit
 };
 // What an item costs beside its blocks (states out, the first scores), in blocks.
 template <int D>
@@ -163,9 +167,11 @@ __device__ __forceinline__ Cost cost_of(const Params& p, const Seq& s) {
   Cost c;
   const int nt = (s.rows + p.rpt - 1) / p.rpt;
   c.pairs = nt > 1 ? (nt + 1) >> 1 : 0;
-  c.units = nt > 1 ? p.hkv * c.pairs : nt == 1 ? (p.hkv + 1) >> 1 : 0;
+  c.units = nt > 1 ? p.hkv : nt == 1 ? (p.hkv + 1) >> 1 : 0;
+  c.inner = nt > 1 ? c.pairs : 1;
   c.chunk = s.chunk / BLK + kItemCost<D>;
-  c.unit = (s.total + BLK - 1) / BLK + s.n_chunks * kItemCost<D>;
+  c.last = (s.total - (s.n_chunks - 1) * s.chunk + BLK - 1) / BLK + kItemCost<D>;
+  c.unit = static_cast<int64_t>(c.inner) * (static_cast<int64_t>(max(s.n_chunks - 1, 0)) * c.chunk + c.last);
   return c;
 }
 
@@ -175,7 +181,7 @@ struct Walk {
   static constexpr int BLK = Cfg<D>::BLK;
   Seq s;
   Cost c;
-  int b, u, chunk;           // the item
+  int b, u, chunk, pair;     // the item
   int64_t left;              // cost up to the end of the run
   // of the item
   int kvh, tile0;            // of tile 0
@@ -186,11 +192,12 @@ struct Walk {
     s = seq_at<D, WARP>(p, b, report);
     c = cost_of<D>(p, s);
   }
-  // begin: (sequence, unit, chunk) of the first item and the run's cost
-  __device__ __forceinline__ Walk(const Params& p, const int (&begin)[3], int64_t cost, bool report) {
+  // begin: (sequence, unit, chunk, pair) of the first item and the run's cost
+  __device__ __forceinline__ Walk(const Params& p, const int (&begin)[4], int64_t cost, bool report) {
     b = begin[0];
     u = begin[1];
     chunk = begin[2];
+    pair = begin[3];
     left = cost;
     if (left > 0) {
       load(p, report);
@@ -198,8 +205,12 @@ struct Walk {
     }
   }
   __device__ __forceinline__ bool more() const { return left > 0; }
-  // From a position that may lie behind its unit or sequence to the item there.
+  // From a position that may lie behind its chunk, unit or sequence to the item there.
   __device__ __forceinline__ void settle(const Params& p, bool report) {
+    if (pair >= c.inner) {
+      pair = 0;
+      ++chunk;
+    }
     if (chunk >= s.n_chunks) {
       chunk = 0;
       ++u;
@@ -213,8 +224,8 @@ struct Walk {
       load(p, report);
     }
     if (c.pairs) {
-      kvh = u / c.pairs;
-      tile0 = (u - kvh * c.pairs) * 2;
+      kvh = u;
+      tile0 = pair * 2;
       tiles = (tile0 + 1) * p.rpt < s.rows ? 2 : 1;
       streams = 1;
     } else {
@@ -227,11 +238,15 @@ struct Walk {
     n_blocks = (tokens + BLK - 1) / BLK;
   }
   // Whether the next item, if there is one, has other queries.
-  __device__ __forceinline__ bool last_of_unit() const { return chunk + 1 == s.n_chunks || left <= n_blocks + kItemCost<D>; }
+  __device__ __forceinline__ bool other_queries_next() const {
+    return c.inner > 1 || chunk + 1 == s.n_chunks || left <= n_blocks + kItemCost<D>;
+  }
+  // No later item reads this one's keys.
+  __device__ __forceinline__ bool last_reader() const { return pair + 1 == c.inner; }
   __device__ __forceinline__ void next(const Params& p, bool report) {
     left -= n_blocks + kItemCost<D>;
     if (left <= 0) return;
-    ++chunk;
+    ++pair;
     settle(p, report);
   }
   // a block that holds drafts
@@ -242,7 +257,7 @@ struct Walk {
 
 // The CTA's run: shared memory for its first item and cost, and the block's scan.
 struct Run {
-  int begin[3];
+  int begin[4];
   long long cost;
   long long warps[kThreads / 32];
 };
@@ -252,11 +267,14 @@ __device__ __forceinline__ void find_run(const Params& p, Run& run) {
   if (p.spread) {
     const uint32_t w = blockIdx.x, r = w / static_cast<uint32_t>(p.units);
     if (threadIdx.x == 0) {
-      run.begin[1] = static_cast<int>(w - r * p.units);
+      const int u = static_cast<int>(w - r * p.units);
       run.begin[2] = static_cast<int>(r / static_cast<uint32_t>(p.n_seqs));
       run.begin[0] = static_cast<int>(r - run.begin[2] * static_cast<uint32_t>(p.n_seqs));
-      const Seq s = seq_at<D, false>(p, run.begin[0], run.begin[1] == 0 && run.begin[2] == 0);
-      if (run.begin[2] < s.n_chunks && run.begin[1] < cost_of<D>(p, s).units) run.cost = 1;
+      const Seq s = seq_at<D, false>(p, run.begin[0], u == 0 && run.begin[2] == 0);
+      const Cost c = cost_of<D>(p, s);
+      run.begin[1] = u / c.inner;
+      run.begin[3] = u - run.begin[1] * c.inner;
+      if (run.begin[2] < s.n_chunks && run.begin[1] < c.units) run.cost = 1;
     }
     __syncthreads();
     return;
@@ -299,15 +317,18 @@ __device__ __forceinline__ void find_run(const Params& p, Run& run) {
         continue;
       }
       long long r = lo - at;
-      int u = static_cast<int>(r / c.unit);
+      const int u = static_cast<int>(r / c.unit);
       r -= static_cast<long long>(u) * c.unit;
-      int chunk = min(static_cast<int>((r + c.chunk - 1) / c.chunk), s.n_chunks);   // n_chunks: the next unit's first
-      const long long start = at + static_cast<long long>(u) * c.unit +
-                              (chunk < s.n_chunks ? static_cast<long long>(chunk) * c.chunk : c.unit);
+      const long long step = static_cast<long long>(c.inner) * c.chunk;
+      const int chunk = min(static_cast<int>(r / step), s.n_chunks - 1), each = chunk + 1 < s.n_chunks ? c.chunk : c.last;
+      r -= chunk * step;
+      const int pair = static_cast<int>((r + each - 1) / each);   // inner: the next chunk's first
       run.begin[0] = b;
       run.begin[1] = u;
       run.begin[2] = chunk;
-      run.cost = hi - start;   // none where the first item at or behind lo lies behind hi
+      run.begin[3] = pair;
+      // none where the first item at or behind lo lies behind hi
+      run.cost = hi - (at + static_cast<long long>(u) * c.unit + chunk * step + static_cast<long long>(pair) * each);
       break;
     }
   }
@@ -389,6 +410,20 @@ __device__ __forceinline__ void add_back(const Params& p, const Seq& s, const ui
   }
 }
 
+// Keys and values that no other item reads leave L2 before the states, which are read again.
+__device__ __forceinline__ uint64_t evict_first() {
+  uint64_t policy;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  return policy;
+}
+__device__ __forceinline__ void tma_load_4d_once(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z,
+                                                 int w, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], "
+      "[%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "l"(policy)
+      : "memory");
+}
 __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
@@ -475,6 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       int stage = 0;
       uint32_t phase = 0;
       uint32_t fills = 0;
+      const uint64_t policy = evict_first();
       for (Walk<D, false> it(p, run.begin, run.cost, false); it.more() && !abort_flag; it.next(p, false)) {
         for (int b = 0; b < it.n_blocks && !abort_flag; ++b) {
           int tok[BLK / 64], slab[BLK / 64], boxes = 0;   // 64-token boxes that hold a token
@@ -494,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
               }
             }
           }
-          const bool clean = it.drafts(b);
+          const bool clean = it.drafts(b), once = it.last_reader();
           for (int e = 0; e < 2 * it.streams; ++e) {
             const bool val = e >= it.streams;
             const int kvh = it.kvh + (val ? e - it.streams : e);
@@ -506,8 +542,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             for (int h = 0; h < BLK / 64; ++h)
 #pragma unroll
               for (int n = 0; n < C::NH; ++n)
-                if (h < boxes)
-                  tma_load_4d(st + n * C::HALF + h * C::BOX, val ? &maps.v : &maps.k, bar, n * 64, tok[h], kvh, slab[h]);
+                if (h < boxes) {
+                  uint8_t* to = st + n * C::HALF + h * C::BOX;
+                  const CUtensorMap* from = val ? &maps.v : &maps.k;
+                  if (once) tma_load_4d_once(to, from, bar, n * 64, tok[h], kvh, slab[h], policy);
+                  else tma_load_4d(to, from, bar, n * 64, tok[h], kvh, slab[h]);
+                }
             ++fills;
             if (++stage == C::STAGES) {
               stage = 0;
@@ -569,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           }
           continue;
         }
-        const bool last_chunk = it.last_of_unit();
+        const bool last_chunk = it.other_queries_next();
         if (fresh) {
           if (!warp_wait(q_bar, qph, kDetQ, abort_flag)) break;
           qph ^= 1u;
@@ -654,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             }
           }
         }
-        fresh = it.last_of_unit();
+        fresh = it.other_queries_next();
         const uint32_t per = 2 * it.streams, f0 = fill;
         fill += per * it.n_blocks;
         const int first = max(0, (it.s.kv - it.t_begin) / BLK);   // the first block with drafts, if any

@@ -76,20 +76,20 @@ def tree_accept(parents, tokens, picked, cu_rows, *, max_keep: int) -> TreeAccep
     sequence keeps none; rows behind the last sequence are not read."""
     import torch
 
-    dev = parents.device
-    assert parents.is_cuda and all(t.get_device() == dev.index for t in (tokens, picked, cu_rows)), \
-        "tree_accept requires CUDA tensors on one device"
-    assert parents.dtype == torch.int32 and cu_rows.dtype == torch.int32, "parents and cu_rows must be int32"
-    assert tokens.dtype == torch.int64 and picked.dtype == torch.int64, "tokens and picked must be int64"
+    dev, i32, i64 = parents.device, torch.int32, torch.int64
+    index = dev.index
+    assert parents.is_cuda and tokens.get_device() == index and picked.get_device() == index \
+        and cu_rows.get_device() == index, "tree_accept requires CUDA tensors on one device"
+    assert parents.dtype == i32 and cu_rows.dtype == i32, "parents and cu_rows must be int32"
+    assert tokens.dtype == i64 and picked.dtype == i64, "tokens and picked must be int64"
     R, B = parents.numel(), cu_rows.numel() - 1
-    assert parents.shape == tokens.shape == picked.shape == (R,) and cu_rows.shape == (B + 1,) and B >= 0, \
+    assert parents.shape == tokens.shape == picked.shape == (R,) and cu_rows.dim() == 1 and B >= 0, \
         "tree_accept: one parent, token and pick a row, and B + 1 offsets"
     if max_keep < 1:
         raise ValueError("tree_accept: max_keep must be positive")
     with _lib.on_device(dev):
-        parents, tokens, picked, cu_rows = (t.contiguous() for t in (parents, tokens, picked, cu_rows))
-        r = TreeAccept(torch.empty((B, max_keep), dtype=torch.int32, device=dev),
-                       torch.empty(B, dtype=torch.int32, device=dev), torch.empty(B, dtype=torch.int64, device=dev))
+        parents, tokens, picked, cu_rows = parents.contiguous(), tokens.contiguous(), picked.contiguous(), cu_rows.contiguous()
+        r = TreeAccept(parents.new_empty(B, max_keep), parents.new_empty(B), tokens.new_empty(B))
         if B == 0:
             return r
         rc = _lib.load().dk_tree_accept(parents.data_ptr(), tokens.data_ptr(), picked.data_ptr(), cu_rows.data_ptr(), B, R,

@@ -65,23 +65,24 @@ def token_logprobs(logits, tokens=None, *, top_k: int = 0, entropy: bool = True)
         assert tokens.dtype == torch.int64 and tokens.get_device() == dev.index and tokens.shape == lead, \
             "token_logprobs: tokens must be int64 on the logits' device, one a row"
         tokens = tokens.contiguous()
-    x = logits.detach()
+    x = logits.detach() if logits.requires_grad else logits
     if V > 1 and x.stride(-1) != 1:
         x = x.contiguous()
     if x.dim() != 2:
         x = x.reshape(-1, V)   # a view where the leading strides allow it
     R = x.shape[0]
     f32 = torch.float32
-    lp = torch.empty(lead, dtype=f32, device=dev) if tokens is not None else None
-    ent = torch.empty(lead, dtype=f32, device=dev) if entropy else None
-    ids = torch.empty((*lead, top_k), dtype=torch.int64, device=dev) if top_k else None
-    top = torch.empty((*lead, top_k), dtype=f32, device=dev) if top_k else None
+    lp = x.new_empty(lead, dtype=f32) if tokens is not None else None
+    ent = x.new_empty(lead, dtype=f32) if entropy else None
+    ids = top = None
+    if top_k:
+        ids, top = x.new_empty((*lead, top_k), dtype=torch.int64), x.new_empty((*lead, top_k), dtype=f32)
     if R and not (lp is None and ent is None and ids is None):
-        def ptr(t):
-            return None if t is None else t.data_ptr()
         with _lib.on_device(dev):
-            rc = _lib.load().dk_token_logprobs(x.data_ptr(), x.stride(0), R, V, code, ptr(tokens), ptr(lp), ptr(ent),
-                                               top_k, ptr(ids), ptr(top), _lib.stream_ptr(dev))
+            rc = _lib.load().dk_token_logprobs(
+                x.data_ptr(), x.stride(0), R, V, code, None if lp is None else tokens.data_ptr(),
+                None if lp is None else lp.data_ptr(), None if ent is None else ent.data_ptr(), top_k,
+                None if ids is None else ids.data_ptr(), None if ids is None else top.data_ptr(), _lib.stream_ptr(dev))
         _lib.check(rc, "token_logprobs")
         _lib.count_launch()
     return TokenLogprobs(lp, ent, ids, top)

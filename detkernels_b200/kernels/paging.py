@@ -221,14 +221,15 @@ def _check_pools(pools, dev, page_size, what):
         return None, 0, (0, 0, 0), 0, 0, 0, 1
     first = pools[0]
     shape, stride, dtype = first.shape, first.stride(), first.dtype
+    index, at = dev.index, []
     for t in pools:
-        assert t.is_cuda and t.get_device() == dev.index, "%s requires CUDA tensors on one device" % what
+        assert t.get_device() == index, "%s requires CUDA tensors on one device" % what
         if t.shape != shape or t.stride() != stride or t.dtype != dtype:
             raise ValueError("%s: the pools must share shape, strides and dtype" % what)
+        at.append(t.data_ptr())
     assert len(shape) == 4 and shape[2] == page_size, "%s: pools must be [n_blocks, heads, page_size, head_dim]" % what
     if shape[3] > 1 and stride[3] != 1:
         raise ValueError("%s: unit stride along head_dim required" % what)
-    at = [t.data_ptr() for t in pools]
     if len(set(at)) != len(at):
         raise ValueError("%s: a pool is named twice" % what)
     ptrs = (ctypes.c_void_p * len(pools))(*at)
