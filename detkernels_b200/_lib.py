@@ -107,7 +107,7 @@ SIGNATURES = {
                                           _c_void_p, _i64, _i32, _i64, _i32, _c_void_p, _i64, _i64, _c_void_p,
                                           _c_void_p, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _int, _c_void_p, _size,
                                           _c_void_p]),
-    "dk_attention_tree_workspace_size": (_size, [_i32, _i32, _i32, _i32, _i32]),
+    "dk_attention_tree_workspace_size": (_size, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "dk_attention_tree": (_int, [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64, _c_void_p,
                                  _i64, _i32, _i64, _i32, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i64,
                                  _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _int, _c_void_p, _size,

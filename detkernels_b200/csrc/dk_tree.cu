@@ -37,6 +37,24 @@ size_t state_o_bytes(int64_t chunks, int64_t st_rows, int64_t D) {
 size_t state_bytes(int64_t chunks, int64_t st_rows, int64_t D) {
   return chunks <= 1 ? 0 : state_o_bytes(chunks, st_rows, D) + static_cast<size_t>(chunks) * st_rows * 2 * sizeof(float);
 }
+// What the sizes alone decide of a call.
+struct Schedule {
+  int64_t chunks, st_rows, units;
+  bool planned;          // more items, at most, than SMs: their order is planned
+  size_t states, need;   // bytes of the states, and of the workspace: the states, then the items' order
+};
+Schedule schedule(int64_t n_seqs, int64_t n_rows, int64_t max_rows, int64_t hq, int64_t hkv, int64_t D, int64_t max_kv_len) {
+  Schedule c{};
+  c.chunks = max_chunks(max_kv_len, max_rows, static_cast<int>(D));
+  c.st_rows = n_rows * hq;
+  const int64_t tiles = ceil_div(max_rows, dk::tree::kRows / (hq / hkv));
+  // items a (sequence, chunk): pairs of tiles, or pairs of heads where the rows fit one tile
+  c.units = tiles > 1 ? hkv * ceil_div(tiles, 2) : ceil_div(hkv, 2);
+  c.planned = c.units * n_seqs * c.chunks > sm_count(current_device());
+  c.states = (state_bytes(c.chunks, c.st_rows, D) + 15) / 16 * 16;
+  c.need = c.states + (c.planned ? static_cast<size_t>(dk::tree::plan_ints(n_seqs)) * sizeof(int32_t) : 0);
+  return c;
+}
 
 template <typename T, int D>
 int tree_launch(const dk::tree::Maps& maps, dk::tree::Params p, cudaStream_t st) {
@@ -58,8 +76,9 @@ int tree_launch(const dk::tree::Maps& maps, dk::tree::Params p, cudaStream_t st)
   }
   // As many CTAs as SMs share the items, or, where even their bound is not more than that, each takes one at once.
   const int64_t items = static_cast<int64_t>(p.units) * p.n_seqs * p.max_chunks;
-  p.spread = items <= sm_count(dev);
-  cudaError_t e = launch_pdl(fn, dim3(static_cast<unsigned>(std::min<int64_t>(items, sm_count(dev)))),
+  cudaError_t e = cudaSuccess;
+  if (p.plan) e = launch_pdl(dk::tree::plan_kernel<D>, dim3(1), dim3(dk::tree::kPlanThreads), 0, st, p);
+  if (e == cudaSuccess) e = launch_pdl(fn, dim3(static_cast<unsigned>(std::min<int64_t>(items, sm_count(dev)))),
                              dim3(dk::tree::kThreads), C::SMEM, st, maps, p);
   if (e == cudaSuccess && p.max_chunks > 1) {
     const int64_t row_tiles = ceil_div(static_cast<int64_t>(p.max_rows) * p.G, 32);
@@ -79,10 +98,13 @@ int tree_for(int D, const dk::tree::Maps& maps, const dk::tree::Params& p, cudaS
 
 extern "C" {
 
-size_t dk_attention_tree_workspace_size(int32_t n_rows, int32_t max_rows, int32_t n_q_heads, int32_t head_dim,
-                                        int32_t max_kv_len) {
-  if (n_rows <= 0 || max_rows <= 0 || n_q_heads <= 0 || head_dim <= 0 || max_kv_len <= 0) return 0;
-  return state_bytes(max_chunks(max_kv_len, max_rows, head_dim), static_cast<int64_t>(n_rows) * n_q_heads, head_dim);
+size_t dk_attention_tree_workspace_size(int32_t n_seqs, int32_t n_rows, int32_t max_rows, int32_t n_q_heads,
+                                        int32_t n_kv_heads, int32_t head_dim, int32_t max_kv_len) {
+  if (n_seqs <= 0 || n_rows <= 0 || max_rows <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads ||
+      n_q_heads / n_kv_heads > dk::tree::kRows || head_dim <= 0 || max_kv_len <= 0)
+    return 0;
+  max_rows = std::min(std::min(max_rows, n_rows), max_kv_len);
+  return schedule(n_seqs, n_rows, max_rows, n_q_heads, n_kv_heads, head_dim, max_kv_len).need;
 }
 
 int dk_attention_tree(const void* q, int64_t q_stride_row, int64_t q_stride_head, const void* k, const void* v,
@@ -125,19 +147,14 @@ int dk_attention_tree(const void* q, int64_t q_stride_row, int64_t q_stride_head
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: bad KV extents", what);
   max_kv_len = static_cast<int32_t>(std::min<int64_t>(max_kv_len, kv_capacity));
   max_rows = std::min(std::min(max_rows, n_rows), max_kv_len);
-  const int64_t chunks = max_chunks(max_kv_len, max_rows, head_dim);
-  const int64_t st_rows = static_cast<int64_t>(n_rows) * n_q_heads;
   const int rpt = dk::tree::kRows / G;
-  const int64_t tiles = ceil_div(max_rows, rpt);
-  // items a (sequence, chunk): pairs of tiles, or pairs of heads where the rows fit one tile
-  const int64_t units = tiles > 1 ? n_kv_heads * ceil_div(tiles, 2) : ceil_div(n_kv_heads, 2);
-  if (st_rows > kI32Max - 512 || static_cast<int64_t>(max_rows) * G > kI32Max - 512 ||
-      units * n_seqs * chunks > kI32Max - 2 * sm_count(current_device()) ||
+  const Schedule c = schedule(n_seqs, n_rows, max_rows, n_q_heads, n_kv_heads, head_dim, max_kv_len);
+  if (c.st_rows > kI32Max - 512 || static_cast<int64_t>(max_rows) * G > kI32Max - 512 ||
+      c.units * n_seqs > kI32Max / 8 || c.units * n_seqs * c.chunks > kI32Max - 2 * sm_count(current_device()) ||
       ceil_div(static_cast<int64_t>(max_rows) * G, 32) * n_kv_heads * n_seqs > kI32Max)
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: too many rows or sequences", what);
-  const size_t need = state_bytes(chunks, st_rows, head_dim);
-  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
-    return fail(DK_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
+  if (c.need && (!workspace || workspace_bytes < c.need || !aligned16(workspace)))
+    return fail(DK_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, c.need, workspace_bytes);
 
   dk::tree::Params p{};
   p.hkv = n_kv_heads;
@@ -153,8 +170,8 @@ int dk_attention_tree(const void* q, int64_t q_stride_row, int64_t q_stride_head
   p.mask_stride = mask_stride;
   p.words = mask_words;
   p.capacity = max_kv_len;
-  p.units = static_cast<int32_t>(units);
-  p.max_chunks = static_cast<int32_t>(chunks);
+  p.units = static_cast<int32_t>(c.units);
+  p.max_chunks = static_cast<int32_t>(c.chunks);
   p.v = v;
   p.c_sn = kv_stride_seq;
   p.c_sh = kv_stride_head;
@@ -170,10 +187,13 @@ int dk_attention_tree(const void* q, int64_t q_stride_row, int64_t q_stride_head
   p.o_sr = out_stride_row;
   p.o_sh = out_stride_head;
   p.o_vec = aligned16(out) && out_stride_row % 8 == 0 && out_stride_head % 8 == 0;
-  p.st_rows = st_rows;
-  p.st_o = need ? static_cast<float*>(workspace) : nullptr;
-  p.st_ml = need ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + state_o_bytes(chunks, st_rows, head_dim))
-                 : nullptr;
+  p.st_rows = c.st_rows;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (c.states) {
+    p.st_o = reinterpret_cast<float*>(ws);
+    p.st_ml = reinterpret_cast<float*>(ws + state_o_bytes(c.chunks, c.st_rows, head_dim));
+  }
+  if (c.planned) p.plan = reinterpret_cast<int32_t*>(ws + c.states);
 
   dk::tree::Maps maps;
   const uint64_t dims[4] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(block_table ? page_size : kv_capacity),

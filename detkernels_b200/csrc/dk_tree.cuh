@@ -10,14 +10,13 @@
 //
 // Work: an item is (sequence, up to two tiles of at most 128 rows, chunk): two tiles of one KV head, which then share K
 // and V, or, where the rows fit one tile, the tiles of two KV heads, each with its own K and V.  Either way both softmax
-// warpgroups have work, and take turns on the exponential unit.  One persistent CTA an SM takes a run of items in the order
-// (sequence, KV heads, chunk, tiles), so that one pair of tiles keeps its queries over a run's chunks, and several pairs find
-// a chunk's keys in L2; the runs are cut at equal shares of the tokens' and the items' cost, which every CTA finds for
-// itself from the lengths.  A TMA warp, an MMA warp a tile (scores,
-// weights and accumulator apart in TMEM), a warpgroup a tile for the softmax, a row a thread, and a warp that fetches the
-// queries and makes the values of draft blocks safe: 0 weights must meet neither what lies behind the sequence in its last
-// page nor a non-finite value of a draft that some rows do not see.  Those elements become 0 in shared memory, and rows
-// that do see them have them added back from the cache (which no ordinary call does).
+// warpgroups have work, and take turns on the exponential unit.  One persistent CTA an SM takes items in an order that
+// plan_kernel has made of the lengths, the most expensive first, so that the CTAs end together; several pairs of tiles of a
+// KV head come side by side, and find a chunk's keys in L2.  A TMA warp, an MMA warp a tile (scores, weights and accumulator apart in TMEM), a
+// warpgroup a tile for the softmax, a row a thread, and a warp that fetches the queries and makes the values of draft blocks
+// safe: 0 weights must meet neither what lies behind the sequence in its last page nor a non-finite value of a draft that
+// some rows do not see.  Those elements become 0 in shared memory, and rows that do see them have them added back from the
+// cache (which no ordinary call does).
 #pragma once
 
 #include "dk_common.cuh"
@@ -76,7 +75,7 @@ struct Params {
   int32_t capacity;         // tokens a sequence may have, drafts included
   int32_t units;            // items a (sequence, chunk), at most
   int32_t max_chunks;
-  int32_t spread;           // an item a CTA: CTA c takes item c of (chunk, sequence, unit)
+  int32_t* plan;            // the items' order; null: CTA c takes item c of (chunk, sequence, unit)
   const void* v;            // for what is added back
   int64_t c_sn, c_sh, c_st;
   const int32_t* table;     // null: contiguous
@@ -175,165 +174,197 @@ __device__ __forceinline__ Cost cost_of(const Params& p, const Seq& s) {
   return c;
 }
 
-// A CTA's walk over its items.
-template <int D, bool WARP>
+// The order of the items: by falling cost, in groups of a sequence's items of one cost (its whole chunks, its last ones),
+// dealt to the CTAs there and back.  So the CTAs' shares end within about the smallest items' cost of one another (64
+// requests, 148 CTAs: 239,000 cycles for the last CTA and 198,000 for the median one with runs of neighbouring items).  It
+// decides no bit.  Scratch, int32: [0] groups, [1] items, then by group its sequence (times 2, plus 1 for last chunks) and
+// its first item.
+__host__ __device__ inline int64_t plan_ints(int64_t n_seqs) { return 4 + 4 * n_seqs; }
+
+constexpr int kPlanThreads = 1024;
+template <int D>
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ Params p) {
+  __shared__ int bucket[kPlanThreads];   // by cost, the most expensive first: groups, then their places
+  __shared__ int warps[kPlanThreads / 32];
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
+  int32_t *group = p.plan + 4, *first = group + 2 * p.n_seqs;
+  auto scan = [&](int mine, int& total) {   // exclusive, block-wide
+    int v = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += o;
+    }
+    __syncthreads();
+    if (lane == 31) warps[warp] = v;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < kPlanThreads / 32; ++i) {
+      if (i < warp) before += warps[i];
+      total += warps[i];
+    }
+    return before + v - mine;
+  };
+  auto place = [](int cost) { return kPlanThreads - 1 - min(cost, kPlanThreads - 1); };
+  bucket[tid] = 0;
+  __syncthreads();
+  for (int b = tid; b < p.n_seqs; b += kPlanThreads) {
+    const Seq s = seq_at<D, false>(p, b, true);
+    if (s.n_chunks == 0) continue;
+    const Cost c = cost_of<D>(p, s);
+    if (s.n_chunks > 1) atomicAdd(&bucket[place(c.chunk)], 1);
+    atomicAdd(&bucket[place(c.last)], 1);
+  }
+  __syncthreads();
+  int groups;
+  const int at = scan(bucket[tid], groups);
+  __syncthreads();
+  bucket[tid] = at;
+  __syncthreads();
+  for (int b = tid; b < p.n_seqs; b += kPlanThreads) {
+    const Seq s = seq_at<D, false>(p, b, false);
+    if (s.n_chunks == 0) continue;
+    const Cost c = cost_of<D>(p, s);
+    const int each = c.units * c.inner;   // items a chunk
+    if (s.n_chunks > 1) {
+      const int g = atomicAdd(&bucket[place(c.chunk)], 1);
+      group[g] = 2 * b;
+      first[g] = each * (s.n_chunks - 1);
+    }
+    const int g = atomicAdd(&bucket[place(c.last)], 1);
+    group[g] = 2 * b + 1;
+    first[g] = each;
+  }
+  int items = 0;
+  for (int g0 = 0; g0 < groups; g0 += kPlanThreads) {
+    __syncthreads();
+    const int g = g0 + tid;
+    int total;
+    const int before = scan(g < groups ? first[g] : 0, total);
+    if (g < groups) first[g] = items + before;
+    items += total;
+  }
+  if (tid == 0) {
+    p.plan[0] = groups;
+    p.plan[1] = items;
+  }
+}
+
+// A CTA's walk over its items, by a whole warp: a lane looks one of the next 32 up.
+template <int D>
 struct Walk {
   static constexpr int BLK = Cfg<D>::BLK;
-  Seq s;
-  Cost c;
-  int b, u, chunk, pair;     // the item
-  int64_t left;              // cost up to the end of the run
+  // of the lane's item
+  int l_b, l_u, l_chunk, l_pair, l_row0, l_rows, l_kv;
+  int round, n_rounds;       // the item, and how many there are for this CTA
   // of the item
-  int kvh, tile0;            // of tile 0
+  Seq s;
+  int b, chunk, kvh;         // sequence, chunk, KV head of tile 0
+  int row0[2];               // first row of the sequence that is a tile's
   int tiles, streams;        // tiles with work; K/V streams (2: tile 1 is the next KV head)
   int t_begin, tokens, n_blocks;
+  bool last_reader;          // no later item reads this one's keys
 
-  __device__ __forceinline__ void load(const Params& p, bool report) {
-    s = seq_at<D, WARP>(p, b, report);
-    c = cost_of<D>(p, s);
-  }
-  // begin: (sequence, unit, chunk, pair) of the first item and the run's cost
-  __device__ __forceinline__ Walk(const Params& p, const int (&begin)[4], int64_t cost, bool report) {
-    b = begin[0];
-    u = begin[1];
-    chunk = begin[2];
-    pair = begin[3];
-    left = cost;
-    if (left > 0) {
-      load(p, report);
-      settle(p, report);
+  __device__ __forceinline__ explicit Walk(const Params& p) {
+    round = 0;
+    if (p.plan) {
+      const int items = p.plan[1], cta = static_cast<int>(blockIdx.x), n = static_cast<int>(gridDim.x);
+      n_rounds = __shfl_sync(0xffffffffu, items / n + (items / n % 2 ? cta >= n - items % n : cta < items % n), 0);
+    } else {
+      n_rounds = 1;   // an item a CTA, as far as there are any
+    }
+    if (n_rounds > 0) {
+      look_up(p);
+      settle(p);
     }
   }
-  __device__ __forceinline__ bool more() const { return left > 0; }
-  // From a position that may lie behind its chunk, unit or sequence to the item there.
-  __device__ __forceinline__ void settle(const Params& p, bool report) {
-    if (pair >= c.inner) {
-      pair = 0;
-      ++chunk;
-    }
-    if (chunk >= s.n_chunks) {
-      chunk = 0;
-      ++u;
-    }
-    while (u >= c.units) {
-      u = 0;
-      if (++b >= p.n_seqs) {
-        left = 0;
-        return;
+  __device__ __forceinline__ bool more() const { return round < n_rounds; }
+  __device__ __forceinline__ void next(const Params& p) {
+    if (++round >= n_rounds) return;
+    if ((round & 31) == 0) look_up(p);
+    settle(p);
+  }
+  __device__ __forceinline__ void look_up(const Params& p) {
+    const int lane = static_cast<int>(threadIdx.x & 31), n = static_cast<int>(gridDim.x);
+    l_b = l_u = l_chunk = l_pair = l_row0 = l_rows = l_kv = 0;
+    if (p.plan) {
+      const int k = round + lane, cta = static_cast<int>(blockIdx.x);
+      if (k < n_rounds) {
+        const int item = k * n + (k & 1 ? n - 1 - cta : cta);
+        const int32_t *group = p.plan + 4, *first = group + 2 * p.n_seqs;
+        int lo = 0, hi = p.plan[0];
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (first[mid] <= item) lo = mid; else hi = mid;
+        }
+        const int g = group[lo];
+        l_b = g >> 1;
+        const Seq q = seq_at<D, false>(p, l_b, false);
+        const Cost c = cost_of<D>(p, q);
+        int r = item - first[lo];
+        const int chunks = g & 1 ? 1 : q.n_chunks - 1;    // of the group: [unit][chunk][pair]
+        l_pair = r % c.inner;
+        r /= c.inner;
+        l_u = r / chunks;
+        l_chunk = g & 1 ? q.n_chunks - 1 : r - l_u * chunks;
+        l_row0 = q.row0;
+        l_rows = q.rows;
+        l_kv = q.kv;
       }
-      load(p, report);
+    } else {
+      // item (chunk, sequence, unit) of the CTA's number
+      const uint32_t w = blockIdx.x, r = w / static_cast<uint32_t>(p.units);
+      const int u = static_cast<int>(w - r * p.units);
+      l_chunk = static_cast<int>(r / static_cast<uint32_t>(p.n_seqs));
+      l_b = static_cast<int>(r - l_chunk * static_cast<uint32_t>(p.n_seqs));
+      const Seq q = seq_at<D, false>(p, l_b, lane == 0 && u == 0 && l_chunk == 0);
+      const Cost c = cost_of<D>(p, q);
+      l_u = c.inner ? u / c.inner : 0;
+      l_pair = u - l_u * c.inner;
+      l_row0 = q.row0;
+      l_rows = q.rows;
+      l_kv = q.kv;
+      const bool there = l_chunk < q.n_chunks && l_u < c.units;
+      if (!__shfl_sync(0xffffffffu, there, 0)) n_rounds = 0;
     }
-    if (c.pairs) {
+  }
+  __device__ __forceinline__ void settle(const Params& p) {
+    auto of = [&](int v) { return __shfl_sync(0xffffffffu, v, round & 31); };
+    b = of(l_b);
+    chunk = of(l_chunk);
+    const int u = of(l_u), pair = of(l_pair);
+    s.row0 = of(l_row0);
+    s.rows = of(l_rows);
+    s.kv = of(l_kv);
+    s.total = s.kv + s.rows;
+    s.chunk = static_cast<int>(chunk_tokens(s.kv, D));
+    s.n_chunks = (s.total + s.chunk - 1) / s.chunk;
+    const int nt = (s.rows + p.rpt - 1) / p.rpt;
+    if (nt > 1) {
       kvh = u;
-      tile0 = pair * 2;
-      tiles = (tile0 + 1) * p.rpt < s.rows ? 2 : 1;
+      row0[0] = pair * 2 * p.rpt;
+      row0[1] = row0[0] + p.rpt;
+      tiles = row0[1] < s.rows ? 2 : 1;
       streams = 1;
+      last_reader = row0[1] + p.rpt >= s.rows;
     } else {
       kvh = 2 * u;
-      tile0 = 0;
+      row0[0] = row0[1] = 0;
       tiles = streams = kvh + 1 < p.hkv ? 2 : 1;
+      last_reader = true;
     }
     t_begin = chunk * s.chunk;
     tokens = min(s.total - t_begin, s.chunk);
     n_blocks = (tokens + BLK - 1) / BLK;
   }
-  // Whether the next item, if there is one, has other queries.
-  __device__ __forceinline__ bool other_queries_next() const {
-    return c.inner > 1 || chunk + 1 == s.n_chunks || left <= n_blocks + kItemCost<D>;
-  }
-  // No later item reads this one's keys.
-  __device__ __forceinline__ bool last_reader() const { return pair + 1 == c.inner; }
-  __device__ __forceinline__ void next(const Params& p, bool report) {
-    left -= n_blocks + kItemCost<D>;
-    if (left <= 0) return;
-    ++pair;
-    settle(p, report);
-  }
   // a block that holds drafts
   __device__ __forceinline__ bool drafts(int block) const { return t_begin + (block + 1) * BLK > s.kv; }
   __device__ __forceinline__ int head(int t) const { return kvh + (streams == 2 ? t : 0); }
-  __device__ __forceinline__ int first_row(const Params& p, int t) const { return (tile0 + (streams == 1 ? t : 0)) * p.rpt; }
 };
-
-// The CTA's run: shared memory for its first item and cost, and the block's scan.
-struct Run {
-  int begin[4];
-  long long cost;
-  long long warps[kThreads / 32];
-};
-template <int D>
-__device__ __forceinline__ void find_run(const Params& p, Run& run) {
-  if (threadIdx.x == 0) run.cost = 0;
-  if (p.spread) {
-    const uint32_t w = blockIdx.x, r = w / static_cast<uint32_t>(p.units);
-    if (threadIdx.x == 0) {
-      const int u = static_cast<int>(w - r * p.units);
-      run.begin[2] = static_cast<int>(r / static_cast<uint32_t>(p.n_seqs));
-      run.begin[0] = static_cast<int>(r - run.begin[2] * static_cast<uint32_t>(p.n_seqs));
-      const Seq s = seq_at<D, false>(p, run.begin[0], u == 0 && run.begin[2] == 0);
-      const Cost c = cost_of<D>(p, s);
-      run.begin[1] = u / c.inner;
-      run.begin[3] = u - run.begin[1] * c.inner;
-      if (run.begin[2] < s.n_chunks && run.begin[1] < c.units) run.cost = 1;
-    }
-    __syncthreads();
-    return;
-  }
-  // every thread the cost of some sequences, then its place among all
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = (p.n_seqs + kThreads - 1) / kThreads;
-  const int b0 = min(static_cast<int64_t>(p.n_seqs), static_cast<int64_t>(threadIdx.x) * per), b1 = min(p.n_seqs, b0 + per);
-  auto seq_cost = [&](int b, Seq& s, Cost& c) {
-    s = seq_at<D, false>(p, b, blockIdx.x == 0);
-    c = cost_of<D>(p, s);
-    return static_cast<long long>(c.units) * c.unit;
-  };
-  long long mine = 0;
-  Seq s;
-  Cost c;
-  for (int b = b0; b < b1; ++b) mine += seq_cost(b, s, c);
-  long long at = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, at, d);
-    if (lane >= d) at += o;
-  }
-  if (lane == 31) run.warps[warp] = at;
-  __syncthreads();
-  long long total = 0;
-#pragma unroll
-  for (int i = 0; i < kThreads / 32; ++i) {
-    if (i < warp) at += run.warps[i];
-    total += run.warps[i];
-  }
-  at -= mine;
-  // items that begin in [lo, hi)
-  const long long lo = total * blockIdx.x / gridDim.x, hi = total * (blockIdx.x + 1) / gridDim.x;
-  if (lo < hi && lo >= at && lo < at + mine) {
-    for (int b = b0; b < b1; ++b) {
-      const long long all = seq_cost(b, s, c);
-      if (lo >= at + all) {
-        at += all;
-        continue;
-      }
-      long long r = lo - at;
-      const int u = static_cast<int>(r / c.unit);
-      r -= static_cast<long long>(u) * c.unit;
-      const long long step = static_cast<long long>(c.inner) * c.chunk;
-      const int chunk = min(static_cast<int>(r / step), s.n_chunks - 1), each = chunk + 1 < s.n_chunks ? c.chunk : c.last;
-      r -= chunk * step;
-      const int pair = static_cast<int>((r + each - 1) / each);   // inner: the next chunk's first
-      run.begin[0] = b;
-      run.begin[1] = u;
-      run.begin[2] = chunk;
-      run.begin[3] = pair;
-      // none where the first item at or behind lo lies behind hi
-      run.cost = hi - (at + static_cast<long long>(u) * c.unit + chunk * step + static_cast<long long>(pair) * each);
-      break;
-    }
-  }
-  __syncthreads();
-}
 
 // A whole warp's wait for fill f of a ring of N stages, whose barriers complete once a lap.  A parity tells a lap only from
 // its neighbours, so whoever waits must know that fill f - N has landed: the number of stages is even, as is that of an
@@ -458,7 +489,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(done + 2);
   uint32_t* s_wild = s_tmem + 1;          // by stage: its values had non-finite elements
   static_assert((3 * C::STAGES + 16 + kSoftWarps + 2) * 8 + 4 + 4 * C::STAGES <= 512, "barriers");
-  __shared__ Run run;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
@@ -498,20 +528,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   const uint32_t tmem = *s_tmem;
   pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
-  find_run<D>(p, run);
 
   bool abort_flag = false;
   // Stages of an item's block b: K of stream i in fill f0 + 2 streams b + i, V behind the K's of the block.
   // A block that holds drafts has its values cleaned.
   if (warp >= kSoftWarps) {
     prefix::reg_dec<prefix::kIoRegs>();
-    if (warp == kSoftWarps && lane == 0) {
+    if (warp == kSoftWarps) {
       // ---------------- TMA producer ----------------
       int stage = 0;
       uint32_t phase = 0;
       uint32_t fills = 0;
       const uint64_t policy = evict_first();
-      for (Walk<D, false> it(p, run.begin, run.cost, false); it.more() && !abort_flag; it.next(p, false)) {
+      for (Walk<D> it(p); it.more() && !abort_flag; it.next(p)) {
         for (int b = 0; b < it.n_blocks && !abort_flag; ++b) {
           int tok[BLK / 64], slab[BLK / 64], boxes = 0;   // 64-token boxes that hold a token
 #pragma unroll
@@ -525,29 +554,32 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
               tok[h] -= pg * p.page;
               slab[h] = p.table[it.b * p.table_stride + pg];
               if (slab[h] < 0 || slab[h] >= p.n_blocks) {
-                report_error(DK_ERR_DEVICE_CHECK, kDetPage);
+                if (lane == 0) report_error(DK_ERR_DEVICE_CHECK, kDetPage);
                 slab[h] = 0;
               }
             }
           }
-          const bool clean = it.drafts(b), once = it.last_reader();
+          const bool clean = it.drafts(b);
           for (int e = 0; e < 2 * it.streams; ++e) {
             const bool val = e >= it.streams;
             const int kvh = it.kvh + (val ? e - it.streams : e);
-            if (!mbar_wait(&empty[stage], phase ^ 1u, kDetEmpty, abort_flag)) break;
+            if (!warp_wait(&empty[stage], phase ^ 1u, kDetEmpty, abort_flag)) break;
             uint8_t* st = ring + stage * C::STAGE;
             uint64_t* bar = val && clean ? &raw[stage] : &full[stage];
-            mbar_arrive_expect_tx(bar, boxes * C::NH * C::BOX);
+            if (lane == 0) {
+              mbar_arrive_expect_tx(bar, boxes * C::NH * C::BOX);
 #pragma unroll
-            for (int h = 0; h < BLK / 64; ++h)
+              for (int h = 0; h < BLK / 64; ++h)
 #pragma unroll
-              for (int n = 0; n < C::NH; ++n)
-                if (h < boxes) {
-                  uint8_t* to = st + n * C::HALF + h * C::BOX;
-                  const CUtensorMap* from = val ? &maps.v : &maps.k;
-                  if (once) tma_load_4d_once(to, from, bar, n * 64, tok[h], kvh, slab[h], policy);
-                  else tma_load_4d(to, from, bar, n * 64, tok[h], kvh, slab[h]);
-                }
+                for (int n = 0; n < C::NH; ++n)
+                  if (h < boxes) {
+                    uint8_t* to = st + n * C::HALF + h * C::BOX;
+                    const CUtensorMap* from = val ? &maps.v : &maps.k;
+                    if (it.last_reader) tma_load_4d_once(to, from, bar, n * 64, tok[h], kvh, slab[h], policy);
+                    else tma_load_4d(to, from, bar, n * 64, tok[h], kvh, slab[h]);
+                  }
+            }
+            __syncwarp();
             ++fills;
             if (++stage == C::STAGES) {
               stage = 0;
@@ -559,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       // every copy has landed before the CTA may end (a cleaned stage's barrier completes behind its copies)
       bool drain = false;
       for (uint32_t f = (fills > C::STAGES ? fills - C::STAGES : 0); f < fills; ++f)
-        mbar_wait(&full[f % C::STAGES], static_cast<uint32_t>((f / C::STAGES) & 1), kDetDrain, drain);
+        warp_wait(&full[f % C::STAGES], static_cast<uint32_t>((f / C::STAGES) & 1), kDetDrain, drain);
     } else if (warp == kSoftWarps + 1 || warp == kSoftWarps + 2) {
       // ---------------- MMA issuers, one a tile ----------------
       const int t = warp - (kSoftWarps + 1);
@@ -576,7 +608,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       uint32_t qph = 0, sph = 0, pph = 0;    // q_bar, s_free, p_ready parities
       uint32_t oph = 1;                      // o_free parity (the first wait passes)
       bool mine = false;                     // the item's tiles have stages of their own
-      bool fresh = true;                     // the unit's queries are still to be waited for
       auto landed = [&](uint32_t f) { return wait_fill<C::STAGES>(full, f, abort_flag); };
       auto release = [&](uint32_t f) {
         tc_commit(&empty[f % C::STAGES]);
@@ -595,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
         }
         __syncwarp();
       };
-      for (Walk<D, true> it(p, run.begin, run.cost, false); it.more() && !abort_flag; it.next(p, false)) {
+      for (Walk<D> it(p); it.more() && !abort_flag; it.next(p)) {
         const int nb = it.n_blocks;
         const uint32_t per = 2 * it.streams;
         const uint32_t f0 = fill + (it.streams == 2 ? t : 0);   // K of block b: f0 + per b; V: streams further
@@ -609,15 +640,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           }
           continue;
         }
-        const bool last_chunk = it.other_queries_next();
-        if (fresh) {
-          if (!warp_wait(q_bar, qph, kDetQ, abort_flag)) break;
-          qph ^= 1u;
-        }
-        fresh = last_chunk;
+        if (!warp_wait(q_bar, qph, kDetQ, abort_flag)) break;
+        qph ^= 1u;
         if (!landed(f0)) break;
         tc_fence_after();
-        issue_qk(f0, last_chunk && nb == 1);
+        issue_qk(f0, nb == 1);
         for (int b = 0; b < nb; ++b) {
           const bool more = b + 1 < nb;
           const uint32_t fv = f0 + per * b + it.streams, fk = f0 + per * (b + 1);
@@ -626,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           if (!warp_wait(&s_free[t], sph, kDetScoresFree, abort_flag)) break;
           sph ^= 1u;
           tc_fence_after();
-          if (more) issue_qk(fk, last_chunk && b + 2 == nb);
+          if (more) issue_qk(fk, b + 2 == nb);
           if (!landed(fv)) break;
           const int valid = min(BLK, it.tokens - b * BLK);
           const int steps = (valid + 15) >> 4;   // 16-token steps of P.V that hold a token
@@ -656,45 +683,41 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       bool fin = false;
       warp_wait(&done[t], 0, kDetDone, fin);
     } else if (warp == kSoftWarps + 3) {
-      // ---------------- queries of a unit, values of draft blocks ----------------
+      // ---------------- an item's queries, values of draft blocks ----------------
       constexpr uint32_t expo = expo_bits<T>();
       uint32_t fill = 0;
       uint32_t seen = 0;                     // raw parities, a bit a stage
-      uint32_t fph[2] = {1, 1}, qph[2] = {0, 0};   // q_free (the first wait passes) and q_full parities
-      bool fresh = true;
-      for (Walk<D, true> it(p, run.begin, run.cost, false); it.more() && !abort_flag; it.next(p, false)) {
-        if (fresh) {
-          for (int t = 0; t < it.tiles && !abort_flag; ++t) {
-            if (!warp_wait(&q_free[t], fph[t], kDetQFree, abort_flag)) break;
-            fph[t] ^= 1u;
-            uint8_t* at = s_q + t * C::QTILE;
-            const int bytes = p.rpt * p.G * 128;   // of a 64-element half; rows behind the tensor's are zero
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&q_full[t], C::NH * bytes);
-              for (int n = 0; n < C::NH; ++n)
-                tma_load_3d(at + n * C::QHALF, &maps.q, &q_full[t], n * 64, it.head(t) * p.G, it.s.row0 + it.first_row(p, t));
+      uint32_t fph = 3u, qph = 0u;           // q_free (the first wait passes) and q_full parities, a bit a tile
+      for (Walk<D> it(p); it.more() && !abort_flag; it.next(p)) {
+        for (int t = 0; t < it.tiles && !abort_flag; ++t) {
+          if (!warp_wait(&q_free[t], (fph >> t) & 1u, kDetQFree, abort_flag)) break;
+          fph ^= 1u << t;
+          uint8_t* at = s_q + t * C::QTILE;
+          const int bytes = p.rpt * p.G * 128;   // of a 64-element half; rows behind the tensor's are zero
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&q_full[t], C::NH * bytes);
+            for (int n = 0; n < C::NH; ++n)
+              tma_load_3d(at + n * C::QHALF, &maps.q, &q_full[t], n * 64, it.head(t) * p.G, it.s.row0 + (t ? it.row0[1] : it.row0[0]));
+          }
+          __syncwarp();
+          if (p.flip | p.zero) {
+            if (!warp_wait(&q_full[t], (qph >> t) & 1u, kDetQ, abort_flag)) break;
+            qph ^= 1u << t;
+            for (int e = lane; e < C::NH * bytes / 16; e += 32) {
+              const int n = e / (bytes / 16);
+              uint4* v = reinterpret_cast<uint4*>(at + n * C::QHALF) + (e - n * (bytes / 16));
+              uint4 x = *v;
+              x.x ^= p.flip;
+              x.y ^= p.flip;
+              x.z ^= p.flip;
+              x.w ^= p.flip;
+              *v = p.zero ? prefix::times_zero<T>(x) : x;
             }
+            fence_proxy_async_smem();
             __syncwarp();
-            if (p.flip | p.zero) {
-              if (!warp_wait(&q_full[t], qph[t], kDetQ, abort_flag)) break;
-              qph[t] ^= 1u;
-              for (int e = lane; e < C::NH * bytes / 16; e += 32) {
-                const int n = e / (bytes / 16);
-                uint4* v = reinterpret_cast<uint4*>(at + n * C::QHALF) + (e - n * (bytes / 16));
-                uint4 x = *v;
-                x.x ^= p.flip;
-                x.y ^= p.flip;
-                x.z ^= p.flip;
-                x.w ^= p.flip;
-                *v = p.zero ? prefix::times_zero<T>(x) : x;
-              }
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&q_ready[t]);
-            }
+            if (lane == 0) mbar_arrive(&q_ready[t]);
           }
         }
-        fresh = it.other_queries_next();
         const uint32_t per = 2 * it.streams, f0 = fill;
         fill += per * it.n_blocks;
         const int first = max(0, (it.s.kv - it.t_begin) / BLK);   // the first block with drafts, if any
@@ -752,12 +775,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       oseen = ocnt;
       return ok;
     };
-    for (Walk<D, true> it(p, run.begin, run.cost, false); it.more() && !abort_flag; it.next(p, false)) {
+    for (Walk<D> it(p); it.more() && !abort_flag; it.next(p)) {
       const uint32_t per = 2 * it.streams;
       const uint32_t fv0 = fill + it.streams + (it.streams == 2 ? t : 0);   // V of block b: fv0 + per b
       fill += per * it.n_blocks;
       if (t >= it.tiles) continue;
-      const int kvh = it.head(t), i0 = it.first_row(p, t), here = min(p.rpt, it.s.rows - i0);   // drafts of the tile
+      const int kvh = it.head(t), i0 = t ? it.row0[1] : it.row0[0], here = min(p.rpt, it.s.rows - i0);   // drafts of the tile
       const bool valid_row = i_r < here;
       const bool warp_live = (warp & 3) * 32 < here * p.G;
       const int row = it.s.row0 + i0 + (valid_row ? i_r : 0);

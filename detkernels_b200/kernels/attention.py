@@ -466,7 +466,7 @@ def attention_tree(q, k_cache, v_cache, kv_lens, cu_rows, tree_mask, *, block_ta
             q_st = q.stride()
         cs = _shared_strides(k_cache, v_cache, "cache")
         lib = _lib.load()
-        nbytes = lib.dk_attention_tree_workspace_size(R, max_rows, H, D, max_kv_len)
+        nbytes = lib.dk_attention_tree_workspace_size(B, R, max_rows, H, Hkv, D, max_kv_len)
         if workspace is None and nbytes:
             workspace = q.new_empty(nbytes, dtype=torch.uint8)
         rc = lib.dk_attention_tree(

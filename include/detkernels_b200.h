@@ -432,8 +432,8 @@ int dk_attention_shared_prefix(const void* q, int64_t q_stride_row, int64_t q_st
 
 /* Workspace bytes of dk_attention_tree (uninitialised memory will do; 0: none is needed).  max_rows and max_kv_len bound
  * the rows and the tokens (drafts included) of a sequence. */
-size_t dk_attention_tree_workspace_size(int32_t n_rows, int32_t max_rows, int32_t n_q_heads, int32_t head_dim,
-                                        int32_t max_kv_len);
+size_t dk_attention_tree_workspace_size(int32_t n_seqs, int32_t n_rows, int32_t max_rows, int32_t n_q_heads,
+                                        int32_t n_kv_heads, int32_t head_dim, int32_t max_kv_len);
 /* Attention of drafted tokens over a cache that holds them: sequence b has kv_lens[b] tokens and, behind them, its
  * drafts, whose queries are the rows [cu_rows[b], cu_rows[b + 1]) of q [n_rows, n_q_heads, head_dim] (cu_rows: device
  * int32[n_seqs + 1]).  Row cu_rows[b] + i attends to tokens [0, kv_lens[b]) and to token kv_lens[b] + j where bit j of its

@@ -146,7 +146,8 @@ def test_entry_point_refuses_on_the_host():
     assert call(table=16, page=48) == bad and call(table=16, stride=3) == bad
     assert call(ws=100) == _lib.DK_ERR_WORKSPACE
     size = lib.dk_attention_tree_workspace_size
-    assert size(8, 8, 8, 64, 512) == 0 and size(8, 8, 8, 64, 700) >= 2 * 64 * 66 * 4
+    assert size(2, 8, 8, 8, 4, 64, 512) == 0 and size(2, 8, 8, 8, 4, 64, 700) >= 2 * 64 * 66 * 4
+    assert size(200, 200, 1, 8, 4, 64, 100) >= 4 * (4 + 4 * 200)      # more items than SMs: their order
     # a chunk's number never exceeds what the workspace was sized for
     for D in (64, 128):
         for kv in (0, 511, 2048, 2049, 4096, 4097, 9000, 16384, 16385, 20000, 32768, 32769, 70001, 1000003):
@@ -154,8 +155,8 @@ def test_entry_point_refuses_on_the_host():
                 chunk = (512 if kv <= 4096 else 1024 * -(-kv // 32768) if D == 64 else 1024 if kv <= 16384 else
                          -(-(-(-kv // 16)) // 128) * 128)
                 n = -(-(kv + t) // chunk)
-                assert n == 1 or size(1, t, 1, D, kv + t) >= n * (D + 2) * 4, (D, kv, t)
-                assert n == 1 or size(1, 2 * t, 1, D, 2 * (kv + t)) >= n * (D + 2) * 4, (D, kv, t)
+                assert n == 1 or size(1, t, t, 1, 1, D, kv + t) >= t * n * (D + 2) * 4, (D, kv, t)
+                assert n == 1 or size(1, 2 * t, 2 * t, 1, 1, D, 2 * (kv + t)) >= 2 * t * n * (D + 2) * 4, (D, kv, t)
 
 
 def test_wrapper_refuses_cpu_tensors():
