@@ -18,16 +18,15 @@ namespace {
 constexpr int64_t kI32Max = 0x7fffffffLL;
 
 // The most chunks that a sequence of at most max_kv_len tokens, max_rows of them drafts, is cut into.
-int64_t max_chunks(int64_t max_kv_len, int64_t max_rows, int D) {
+int64_t max_chunks(int64_t max_kv_len, int64_t max_rows) {
   int64_t most = 1;
-  // a chunk's size is constant between these lengths of the cached part, or grows with it
-  const int64_t last = D <= 64 ? 32768 : 16384;
-  for (int64_t kv : {int64_t{4096}, last, max_kv_len}) {
+  // a chunk's size is constant between these lengths of the cached part, and then grows with it
+  for (int64_t kv : {4096, 8192, 16384, 32768}) {
     kv = std::min(kv, max_kv_len);
-    most = std::max(most, ceil_div(std::min(kv + max_rows, max_kv_len), dk::tree::chunk_tokens(kv, D)));
+    most = std::max(most, ceil_div(std::min(kv + max_rows, max_kv_len), dk::tree::chunk_tokens(kv)));
   }
-  // beyond `last` a chunk holds at least a 32nd (D <= 64) or 16th of the cached part
-  if (max_kv_len > last) most = std::max(most, (D <= 64 ? 32 : 16) + ceil_div(max_rows, 1024) + 1);
+  // beyond, it holds at least a 16th of the cached part, and 2048 tokens
+  if (max_kv_len > 32768) most = std::max(most, 16 + ceil_div(max_rows, 2048) + 1);
   return most;
 }
 
@@ -45,7 +44,7 @@ struct Schedule {
 };
 Schedule schedule(int64_t n_seqs, int64_t n_rows, int64_t max_rows, int64_t hq, int64_t hkv, int64_t D, int64_t max_kv_len) {
   Schedule c{};
-  c.chunks = max_chunks(max_kv_len, max_rows, static_cast<int>(D));
+  c.chunks = max_chunks(max_kv_len, max_rows);
   c.st_rows = n_rows * hq;
   const int64_t tiles = ceil_div(max_rows, dk::tree::kRows / (hq / hkv));
   // items a (sequence, chunk): pairs of tiles, or pairs of heads where the rows fit one tile

@@ -144,15 +144,15 @@ def test_entry_point_refuses_on_the_host():
     assert call(words=0) == bad and call(max_rows=0) == bad and call(max_kv=0) == bad
     assert call(q=8) == bad and call(q_sr=511) == bad and call(mask=None) == bad and call(n_seq=1) == bad and call(cap=0) == bad
     assert call(table=16, page=48) == bad and call(table=16, stride=3) == bad
-    assert call(ws=100) == _lib.DK_ERR_WORKSPACE
+    assert call(max_kv=1000, ws=100) == _lib.DK_ERR_WORKSPACE
     size = lib.dk_attention_tree_workspace_size
-    assert size(2, 8, 8, 8, 4, 64, 512) == 0 and size(2, 8, 8, 8, 4, 64, 700) >= 2 * 64 * 66 * 4
+    assert size(2, 8, 8, 8, 4, 64, 768) == 0 and size(2, 8, 8, 8, 4, 64, 769) >= 2 * 64 * 66 * 4
     assert size(200, 200, 1, 8, 4, 64, 100) >= 4 * (4 + 4 * 200)      # more items than SMs: their order
     # a chunk's number never exceeds what the workspace was sized for
     for D in (64, 128):
-        for kv in (0, 511, 2048, 2049, 4096, 4097, 9000, 16384, 16385, 20000, 32768, 32769, 70001, 1000003):
+        for kv in (0, 511, 768, 2049, 4096, 4097, 8192, 8193, 9000, 16384, 16385, 20000, 32768, 32769, 70001, 1000003):
             for t in (1, 64, 700, 5000):
-                chunk = (512 if kv <= 4096 else 1024 * -(-kv // 32768) if D == 64 else 1024 if kv <= 16384 else
+                chunk = (768 if kv <= 4096 else 1024 if kv <= 8192 else 1536 if kv <= 16384 else 2048 if kv <= 32768 else
                          -(-(-(-kv // 16)) // 128) * 128)
                 n = -(-(kv + t) // chunk)
                 assert n == 1 or size(1, t, t, 1, 1, D, kv + t) >= t * n * (D + 2) * 4, (D, kv, t)
@@ -182,7 +182,7 @@ CASES = [
     ([10, 10], [0, 0], 4, 4, 64, 0, 1, "none"),                 # rows that see nothing
     ([10, 40], [0, 3], 4, 4, 128, 0, 1, "none"),
     ([600], [0], 2, 1, 64, 0, 10, "chain"),                     # a prompt
-    ([9, 9], [17000, 5000], 8, 4, 128, 64, 1, "tree"),          # chunks that grow with the length
+    ([9, 9, 9], [17000, 5000, 9000], 8, 4, 128, 64, 1, "tree"),   # chunks that grow with the length
     ([4], [40000], 2, 2, 64, 0, 1, "tree"),
     ([2], [50], 128, 1, 64, 0, 1, "tree"),                      # as many heads a KV head as a tile has rows
     ([16] * 40, [int(x) for x in np.arange(40) * 37], 4, 1, 64, 64, 1, "tree"),
@@ -295,7 +295,7 @@ def test_a_chain_is_decode_attention(dev):
     want = attention_decode(q, kc, vc, lens, block_table=kw["block_table"][seq].contiguous())
     assert (got.float() - want.float()).abs().max().item() <= 2.0 ** -6
     # a chain of one row a sequence, for every length around a block, a chunk and a page
-    for n in (1, 2, 63, 64, 65, 127, 128, 129, 511, 512, 513, 1023, 1024, 1025):
+    for n in (1, 2, 63, 64, 65, 127, 128, 129, 511, 512, 513, 767, 768, 769, 1535, 1536, 1537):
         args, kw, own = _case(dev, torch.float16, [1], [n - 1], 4, 2, 128, 64, seed=n)
         _check(attention_tree(*args, **kw), args, own, 128 ** -0.5, 128)
 
@@ -398,7 +398,7 @@ def test_wrapper_refuses_on_the_gpu(dev):
 
     from detkernels_b200 import _lib
     from detkernels_b200.kernels.attention import attention_tree
-    args, kw, own = _case(dev, torch.float16, [4, 6], [600, 77], 4, 2, 64, 64)
+    args, kw, own = _case(dev, torch.float16, [4, 6], [900, 77], 4, 2, 64, 64)
     q, kc, vc, kv, cu, mask = args
     with pytest.raises(TypeError):
         attention_tree(q.bfloat16(), kc, vc, kv, cu, mask, **kw)
