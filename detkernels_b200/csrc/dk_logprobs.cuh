@@ -16,7 +16,8 @@
 // from the threads' maxima: in each of w warps the ceil(k / w)-th largest is at most it, and so is the least of
 // these.  What lies above the bound (about twice k) is collected and ranked by counting; ties at the bound are taken
 // in the order of their indices.  From then on the k-th largest so far is the bound.  Where a bound is poor (logits
-// in order), the k-th largest of the pass's maxima is sought.
+// in order), the k-th largest of the pass's maxima is sought and takes its place; the pass then gives k alternatives by
+// itself, ties included.
 #pragma once
 
 #include "dk_common.cuh"
@@ -33,7 +34,7 @@ constexpr int kCandidates = 1160;               // above the k-th largest maximu
 constexpr int kPoor = 256;                      // a bound with more above it is worth improving
 constexpr int kMany = 128;                      // candidates worth ranking before the row's end
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-static_assert((kMaxK - 1) * 32 + kMany + kMaxK < kCandidates, "candidates");
+static_assert((kMaxK - 1) * 32 + 2 * kMaxK + 16 + kMaxK < kCandidates, "candidates");   // so many, those before, and ties
 
 enum : int {
   kDetToken = 0x650,   // a token outside the vocabulary (and not -1)
@@ -485,6 +486,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
         return __syncthreads_or(mine);
       };
       const bool some = collect();
+      bool fresh = held < p.k;   // the bound is of this pass's logits: at it, too, they may be alternatives
       if (some && sh.n_found - n > kPoor) {
         // the k-th largest of the threads' maxima, bit by bit
         uint32_t best = 0;
@@ -494,15 +496,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
         }
         if (best > bound) {
           bound = best;
+          fresh = true;
           if (tid == 0) sh.n_found = n;
           __syncthreads();
           collect();
         }
       }
+      const int before = n;
       if (some) n = sh.n_found;
-      if (held < p.k) {
-        // ties at the bound, in the order of their indices
-        int need = min(p.k - held, end - begin) - (n - held);
+      if (fresh) {
+        // ties at the bound, in the order of their indices, until the pass has given k
+        int need = min(p.k, end - begin) - (n - before);
         if (need > 0) {
 #pragma unroll 1
           for (int i = 0; i < ITERS && need > 0; ++i) {
@@ -527,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
           __syncthreads();
         }
       }
-      if (held < p.k || n > min(kMany, 2 * p.k + 16) || at.last) {
+      if (fresh || n > min(kMany, 2 * p.k + 16) || at.last) {
         // the k largest so far, by counting (keys are distinct)
         if (tid == 0 && (n & 1)) found[n] = 0ull;   // below all keys
         __syncthreads();
@@ -537,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
           if (above < p.k) sh.sorted[above] = key;
         }
         __syncthreads();
-        held = min(p.k, n);
+        held = min(p.k, n);   // (k of the first pass on, but for a row that has no more)
         if (tid < held) found[tid] = sh.sorted[tid];
         if (held == p.k) bound = static_cast<uint32_t>(sh.sorted[p.k - 1] >> 32);   // an equal logit behind it comes later
         if (tid == 0) sh.n_found = held;

@@ -186,6 +186,32 @@ def test_rows_that_go_wrong(dev, dt, kind, V):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("kind", ["crests", "plateau", "stairs"])
+@pytest.mark.parametrize("k", [1, 5, 32])
+def test_a_later_pass_is_far_above(dev, dt, kind, k):
+    """Many rows, a CTA each, whose later passes lie all above the alternatives so far: as many larger maxima as there are
+    alternatives and no more, equal ones, and ever larger ones."""
+    import torch
+
+    from detkernels_b200.kernels.logprobs import token_logprobs
+    V = 5 * 4096 + 100 if dt == "f32" else 5 * 8192 + 100
+    at = torch.arange(V, device=dev)
+    g = torch.Generator(device=dev).manual_seed(3)
+    x = torch.rand(200, V, device=dev, generator=g)
+    x[:, V // 2:] = 2.0
+    if kind == "crests":
+        x[:, V - 90 * 8::8] = 10.0 + (torch.arange(90, device=dev) * 37 % 90).float()
+    elif kind == "plateau":
+        x[:, V // 2 + 9::11] = 7.0
+    else:
+        x[:] = (at * 16 // V).float()
+    x = x.to(_dt(dt))
+    tok = torch.randint(0, V, (200,), device=dev, generator=g)
+    _check(x, tok, k, token_logprobs(x, tok, top_k=k))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("V", [37, 999, 20011, 140000])
 def test_a_row_is_itself_wherever_it_lies(dev, dt, V):
     """Bit for bit: alone, in a batch, at every alignment, behind a row stride, with more dimensions."""
