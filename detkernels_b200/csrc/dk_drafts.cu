@@ -71,7 +71,7 @@ struct Pools {
   int32_t heads, dim, size;
 };
 
-int check_pools(const Pools& c, const char* what) {
+int check_pools(const Pools& c, int64_t page, const char* what) {
   if (c.n < 0 || (c.n > 0 && !c.ptr)) return fail(DK_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   if (c.n_blocks <= 0 || c.n_blocks > kI32Max) return fail(DK_ERR_INVALID_ARGUMENT, "%s: bad number of blocks", what);
   if (c.n == 0) return DK_OK;
@@ -79,6 +79,8 @@ int check_pools(const Pools& c, const char* what) {
     return fail(DK_ERR_UNSUPPORTED, "%s: elements of %d bytes", what, c.size);
   if (c.heads <= 0 || c.dim <= 0 || static_cast<int64_t>(c.n) * c.heads * c.dim > kI32Max)
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: bad pool shape", what);
+  if ((c.n_blocks > 1 && c.s_block <= 0) || (c.heads > 1 && c.s_head <= 0) || (page > 1 && c.s_tok <= 0))
+    return fail(DK_ERR_INVALID_ARGUMENT, "%s: the pools' elements must each have a place of their own", what);
   for (int i = 0; i < c.n; ++i)
     if (!c.ptr[i] || reinterpret_cast<uintptr_t>(c.ptr[i]) % c.size)
       return fail(DK_ERR_INVALID_ARGUMENT, "%s: a pool's address is null or not that of an element", what);
@@ -95,8 +97,8 @@ cudaError_t move_launch(const dk::pages::MoveParams& p, int64_t grid, bool after
   return cudaGetLastError();
 }
 
-// Moves the tokens of `n` sequences, at most `most` each, in every pool.
-int move(dk::pages::MoveParams& p, const Pools& c, int64_t n, int64_t most, const char* what, cudaStream_t st) {
+// Moves the tokens of `n` sequences, at most `most` each, in every pool; or says beforehand whether it will.
+int move(dk::pages::MoveParams& p, const Pools& c, int64_t n, int64_t most, bool launch, const char* what, cudaStream_t st) {
   if (c.n == 0 || n == 0 || most <= 0) return DK_OK;
   bool wide = c.dim * static_cast<int64_t>(c.size) % 16 == 0 && c.s_block * c.size % 16 == 0 &&
               c.s_head * c.size % 16 == 0 && c.s_tok * c.size % 16 == 0;
@@ -126,6 +128,7 @@ int move(dk::pages::MoveParams& p, const Pools& c, int64_t n, int64_t most, cons
                      : 1;
     const int64_t grid = units * p.splits;
     if (grid > kI32Max) return fail(DK_ERR_INVALID_ARGUMENT, "%s: too many sequences", what);
+    if (!launch) continue;
     cudaError_t e = wide          ? move_launch<uint4>(p, grid, first > 0, st)
                     : c.size == 1 ? move_launch<uint8_t>(p, grid, first > 0, st)
                     : c.size == 2 ? move_launch<uint16_t>(p, grid, first > 0, st)
@@ -233,7 +236,7 @@ int dk_paged_fork(int32_t* block_table, int64_t block_table_stride, int32_t tabl
   if (n_forks > kI32Max - 4096) return fail(DK_ERR_INVALID_ARGUMENT, "%s: too many forks", what);
   const Pools c{pools, n_pools, pool_stride_block, pool_stride_head, pool_stride_tok, n_blocks, n_heads, head_dim,
                 element_size};
-  rc = check_pools(c, what);
+  rc = check_pools(c, page_size, what);
   if (rc) return rc;
   if (n_forks == 0) return DK_OK;
   if (!kv_lens || !src || !dst || !cursor || !cursor_out || (n_free > 0 && !free_blocks))
@@ -257,9 +260,6 @@ int dk_paged_fork(int32_t* block_table, int64_t block_table_stride, int32_t tabl
   p.shares = shares;
   p.n_blocks = n_blocks;
   p.ws = static_cast<int32_t*>(workspace);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_pdl(dk::pages::fork_kernel, dim3(dk::pages::kPlanCtas), dim3(dk::pages::kPlanThreads), 0, st, p);
-  if (e != cudaSuccess) return fail(DK_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
   dk::pages::MoveParams m{};
   m.table = block_table;
   m.table_stride = block_table_stride;
@@ -271,7 +271,12 @@ int dk_paged_fork(int32_t* block_table, int64_t block_table_stride, int32_t tabl
   m.width = blocks_per_seq;
   m.ws = p.ws;
   const int64_t most = shares ? page_size - 1 : static_cast<int64_t>(blocks_per_seq) * page_size;
-  return move(m, c, n_forks, most, what, st);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  rc = move(m, c, n_forks, most, false, what, st);
+  if (rc) return rc;
+  cudaError_t e = launch_pdl(dk::pages::fork_kernel, dim3(dk::pages::kPlanCtas), dim3(dk::pages::kPlanThreads), 0, st, p);
+  if (e != cudaSuccess) return fail(DK_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
+  return move(m, c, n_forks, most, true, what, st);
 }
 
 size_t dk_paged_compact_workspace_size(void) { return compact_ws_bytes(); }
@@ -290,7 +295,7 @@ int dk_paged_compact(const int32_t* block_table, int64_t block_table_stride, int
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: negative size, or too many sequences or free blocks", what);
   const Pools c{pools, n_pools, pool_stride_block, pool_stride_head, pool_stride_tok, n_blocks, n_heads, head_dim,
                 element_size};
-  rc = check_pools(c, what);
+  rc = check_pools(c, page_size, what);
   if (rc) return rc;
   if (shares && !free_blocks) return fail(DK_ERR_INVALID_ARGUMENT, "%s: shares need a free list", what);
   if (free_blocks && (!cursor || !cursor_out))
@@ -322,10 +327,6 @@ int dk_paged_compact(const int32_t* block_table, int64_t block_table_stride, int
   p.shares = shares;
   p.n_blocks = n_blocks;
   p.ws = static_cast<int32_t*>(workspace);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_pdl(dk::pages::release_kernel, dim3(dk::pages::kPlanCtas), dim3(dk::pages::kPlanThreads), 0, st, p);
-  if (e != cudaSuccess) return fail(DK_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
-  if (!keep) return DK_OK;   // the first tokens stay where they are
   dk::pages::MoveParams m{};
   m.table = block_table;
   m.table_stride = block_table_stride;
@@ -337,7 +338,13 @@ int dk_paged_compact(const int32_t* block_table, int64_t block_table_stride, int
   m.keep_width = keep_width;
   m.width = blocks_per_seq;
   m.ws = p.ws;
-  return move(m, c, n_seqs, keep_width, what, st);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t most = keep ? keep_width : 0;   // without `keep` the first tokens stay where they are
+  rc = move(m, c, n_seqs, most, false, what, st);
+  if (rc) return rc;
+  cudaError_t e = launch_pdl(dk::pages::release_kernel, dim3(dk::pages::kPlanCtas), dim3(dk::pages::kPlanThreads), 0, st, p);
+  if (e != cudaSuccess) return fail(DK_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
+  return move(m, c, n_seqs, most, true, what, st);
 }
 
 }  // extern "C"

@@ -443,6 +443,8 @@ def attention_tree(q, k_cache, v_cache, kv_lens, cu_rows, tree_mask, *, block_ta
     max_rows = 64 * W if max_rows is None else int(max_rows)
     if max_rows < 0 or max_kv_len < 0:
         raise ValueError("attention_tree: max_rows and max_kv_len must not be negative")
+    if max(R, B, width) > _I32_MAX:
+        raise ValueError("attention_tree: too many rows or sequences")
     max_kv_len = min(max_kv_len, cap, _I32_MAX)   # bounds beyond the cache or the batch bound nothing, but size the work
     max_rows = min(max_rows, R, max_kv_len)
     if scale is None:

@@ -18,13 +18,14 @@ class TreeAccept(NamedTuple):
     next_tokens: object   # int64 [B]: the pick after the path's last node, -1 without nodes
 
 
-def tree_mask(parents, cu_rows, words: int = 1):
+def tree_mask(parents, cu_rows, words: int = 1, max_rows=None):
     """The mask of ``attention_tree``: bit j of row i's words (int64 [R, words], 64 nodes a word) says that node j of the
     row's sequence is the row's node or one of its ancestors.
 
     parents: int32 [R], the parent's index among the sequence's nodes (smaller than the node's own), -1 for none;
-    cu_rows: int32 [B + 1], ascending.  Elementary torch operations, on any device, without a host round trip.  Nodes from
-    64 * words on have no bit, and rows behind the last sequence no bits at all."""
+    cu_rows: int32 [B + 1], ascending.  Elementary torch operations, on any device, without a host round trip, three for each
+    binary digit of max_rows, a bound on a sequence's nodes (all rows if not given).  Nodes from 64 * words on have no bit,
+    and rows behind the last sequence no bits at all."""
     import torch
 
     assert parents.dim() == 1 and cu_rows.dim() == 1 and words >= 1
@@ -40,7 +41,8 @@ def tree_mask(parents, cu_rows, words: int = 1):
     mask = torch.where(live[:, None] & (word[None, :] == (at >> 6)[:, None]), own[:, None], 0)
     parent = parents.long()
     up = torch.where(live & (parent >= 0) & (parent < at), start + parent, row)
-    for _ in range(max(1, (64 * words - 1).bit_length())):   # ancestors twice as far each time
+    deep = R if max_rows is None else min(R, int(max_rows))
+    for _ in range(max(deep - 1, 0).bit_length()):   # ancestors twice as far each time
         mask = mask | mask[up]
         up = up[up]
     return mask
@@ -85,8 +87,8 @@ def tree_accept(parents, tokens, picked, cu_rows, *, max_keep: int) -> TreeAccep
     R, B = parents.numel(), cu_rows.numel() - 1
     assert parents.shape == tokens.shape == picked.shape == (R,) and cu_rows.dim() == 1 and B >= 0, \
         "tree_accept: one parent, token and pick a row, and B + 1 offsets"
-    if max_keep < 1:
-        raise ValueError("tree_accept: max_keep must be positive")
+    if not 1 <= max_keep < 2 ** 31 or max(R, B) >= 2 ** 31:
+        raise ValueError("tree_accept: max_keep must be positive, and sizes below 2^31")
     with _lib.on_device(dev):
         parents, tokens, picked, cu_rows = parents.contiguous(), tokens.contiguous(), picked.contiguous(), cu_rows.contiguous()
         r = TreeAccept(parents.new_empty(B, max_keep), parents.new_empty(B), tokens.new_empty(B))

@@ -55,6 +55,8 @@ def token_logprobs(logits, tokens=None, *, top_k: int = 0, entropy: bool = True)
     if logits.dim() < 1 or shape[-1] < 1:
         raise ValueError("token_logprobs: logits must have at least one entry a row")
     V, lead = shape[-1], shape[:-1]
+    if V >= 2 ** 31:
+        raise ValueError("token_logprobs: %d logits a row" % V)
     top_k = int(top_k)
     if top_k < 0 or top_k > V:
         raise ValueError("token_logprobs: top_k %d outside [0, %d]" % (top_k, V))

@@ -246,6 +246,8 @@ def _check_books(block_table, kv_lens, page_size, free_blocks, cursor, shares, n
     assert kv_lens.dtype == i32 and kv_lens.dim() == 1, "%s: lengths must be int32 vectors" % what
     if not 1 <= page_size < 2 ** 31:
         raise ValueError("%s: page_size must be positive and below 2^31" % what)
+    if max(*block_table.shape, kv_lens.shape[0]) >= 2 ** 31:
+        raise ValueError("%s: a table of 2^31 rows or columns" % what)
     if (free_blocks is None) != (cursor is None):
         raise ValueError("%s: free_blocks and cursor go together" % what)
     if free_blocks is not None:
@@ -284,6 +286,8 @@ def paged_fork(block_table, kv_lens, src, dst, page_size: int, *, free_blocks, c
     stride, n_blocks = _check_books(block_table, kv_lens, page_size, free_blocks, cursor, shares, n_blocks, what)
     assert kv_lens.shape == (block_table.shape[0],) and kv_lens.is_contiguous(), "paged_fork: one length a table row"
     assert src.dtype == torch.int32 and dst.dtype == torch.int32 and src.shape == dst.shape and src.dim() == 1
+    if src.shape[0] >= 2 ** 31:
+        raise ValueError("paged_fork: 2^31 forks or more")
     assert src.get_device() == dev.index and dst.get_device() == dev.index, "paged_fork requires CUDA tensors on one device"
     with _lib.on_device(dev):
         src, dst = src.contiguous(), dst.contiguous()
@@ -314,9 +318,10 @@ def paged_compact(block_table, kv_lens, new_lens, n_keep, page_size: int, *, kee
     ``keep``.  They are moved to kv_lens[b] + j in all ``pools`` (as in ``paged_fork``): the accepted path of a tree
     (``drafts.tree_accept``), or a cache thinned out.  kv_lens = 0 and n_keep = 0 free a sequence.
     free_blocks (updated in place) and cursor: the pages behind a sequence's tokens go back before the cursor, in the order
-    of sequences and pages, and the new cursor, from which ``paged_plan`` and ``paged_fork`` take them again, is returned.  With shares (as in ``paged_fork``) a page with further holders loses one instead, and
-    one given up by all its holders goes back once.  Table entries stay as they are.  Tokens must not be moved inside a
-    page that another sequence shares; ``paged_fork`` leaves each sequence its open page to itself.
+    of sequences and pages, and the new cursor, from which ``paged_plan`` and ``paged_fork`` take them again, is returned.
+    With shares (as in ``paged_fork``) a page with further holders loses one instead, and one given up by all its holders
+    goes back once; without, a page must be one sequence's alone.  Table entries stay as they are.  Tokens must not be moved
+    inside a page that another sequence shares; ``paged_fork`` leaves each sequence its open page to itself.
 
     A negative length, more kept than held, a sequence beyond its table row, a ``keep`` that does not ascend inside the
     new tokens, a block id outside the pools, more pages than were handed out or a page given up by more sequences than
@@ -335,6 +340,8 @@ def paged_compact(block_table, kv_lens, new_lens, n_keep, page_size: int, *, kee
         assert t.dtype == torch.int32 and t.get_device() == dev.index, "paged_compact: lengths must be int32 on one device"
     if keep is not None:
         assert keep.dtype == torch.int32 and keep.get_device() == dev.index and keep.dim() == 2 and keep.shape[0] == B
+        if keep.shape[1] >= 2 ** 31:
+            raise ValueError("paged_compact: keep of 2^31 columns or more")
         if keep.shape[1] > 1 and keep.stride(1) != 1:
             keep = keep.contiguous()
     with _lib.on_device(dev):

@@ -480,8 +480,8 @@ int dk_tree_accept(const int32_t* parents, const int64_t* tokens, const int64_t*
                    int64_t* next_tokens, void* stream);
 
 /* The pools of the next two calls: n_pools device pointers (an array on the host) to tensors [n_blocks, n_heads, page_size,
- * head_dim] of elements of element_size bytes (1, 2, 4 or 8), all with the same element strides by block, head and token and unit
- * stride along head_dim.  shares (device int32[n_blocks]): how many further sequences hold a block beyond the first.
+ * head_dim] of elements of element_size bytes (1, 2, 4 or 8), all with the same element strides by block, head and token (positive,
+ * where there is more than one) and unit stride along head_dim; no two of them overlap.  shares (device int32[n_blocks]): how many further sequences hold a block beyond the first.
  * The free list: free_blocks[0, *cursor) are handed out, as for dk_paged_plan; cursor_out may be cursor. */
 size_t dk_paged_fork_workspace_size(int32_t table_rows);   /* uninitialised memory will do */
 /* Row dst[i] of block_table [table_rows][blocks_per_seq] becomes a copy of row src[i], kv_lens[dst[i]] =
@@ -504,7 +504,8 @@ size_t dk_paged_compact_workspace_size(void);              /* uninitialised memo
  * kv_lens[b] + j in all pools, lens_out[b] = kv_lens[b] + n_keep[b] (lens_out is none of the inputs), and with
  * free_blocks the pages [ceil(lens_out / page), ceil((kv + new) / page)) are given up: a page with shares loses one, any
  * other goes back, free_blocks[*cursor_out, *cursor) in the order of (sequence, page), a page given up by all its
- * holders in this call at the last of them.  Table entries stay.  kv_lens = 0 and n_keep = 0 free a whole sequence.
+ * holders in this call at the last of them.  Without shares a page is one sequence's alone; with them n_seqs *
+ * blocks_per_seq must be below 2^30.  Table entries stay.  kv_lens = 0 and n_keep = 0 free a whole sequence.
  * Tokens must not be moved inside a page that another sequence shares: the pages from kv_lens[b] / page_size on are the
  * sequence's own, as dk_paged_fork leaves them.  Recorded as DK_ERR_DEVICE_CHECK: bad lengths (detail 0x644), a bad row of
  * keep (0x645), a block id outside [0, n_blocks) (0x642), more pages than were handed out (0x643), a page given up

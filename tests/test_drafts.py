@@ -41,6 +41,11 @@ def test_tree_mask():
         mask = tree_mask(torch.from_numpy(parents), torch.from_numpy(cu), words)
         assert mask.dtype == torch.int64 and mask.shape == (len(parents), words)
         assert (_bits(mask) == _plain_mask(parents, cu, words)).all()
+    # nodes beyond the words have no bit, and their rows those of all their ancestors; a bound on the nodes changes nothing
+    parents, cu = _trees(rng, [7, 200, 31], reach=1), _cu([7, 200, 31])
+    for words, bound in ((1, None), (1, 200), (2, 1000), (4, 200)):
+        mask = tree_mask(torch.from_numpy(parents), torch.from_numpy(cu), words, max_rows=bound)
+        assert (_bits(mask) == _plain_mask(parents, cu, words)).all()
     # a chain is as deep as it is long; rows behind the last sequence have no bits
     chain = torch.arange(-1, 127, dtype=torch.int32)
     mask = tree_mask(torch.cat([chain, chain[:3]]), torch.tensor([0, 128], dtype=torch.int32), 2)

@@ -67,15 +67,18 @@ def test_entry_points_refuse_on_the_host():
     none = (ctypes.c_void_p * 1)(None)
 
     def fork(rows=4, width=4, stride=4, n=2, page=8, free=16, cursor=16, shares=None, n_blocks=9, pools=one, size=2,
-             dim=8, ws=1 << 16):
+             dim=8, ws=1 << 16, heads=1, st=(64, 64, 8)):
         return lib.dk_paged_fork(16, stride, rows, width, 16, 16, 16, n, page, free, 5, cursor, cursor, shares, n_blocks,
-                                 pools, 1, 64, 64, 8, 1, dim, size, 16, ws, None)
+                                 pools, 1, *st, heads, dim, size, 16, ws, None)
     bad = _lib.DK_ERR_INVALID_ARGUMENT
     assert fork(n=0) == _lib.DK_OK
     assert fork(n=-1) == bad and fork(page=0) == bad and fork(stride=3) == bad and fork(free=None) == bad
     assert fork(cursor=None) == bad and fork(n_blocks=0) == bad and fork(pools=None) == bad and fork(pools=none) == bad
     assert fork(width=1 << 20, stride=1 << 20, page=1 << 14) == bad
     assert fork(size=3) == _lib.DK_ERR_UNSUPPORTED and fork(dim=0) == bad
+    # elements of one place, and more tokens than a launch takes
+    assert fork(st=(0, 64, 8)) == bad and fork(st=(64, 0, 8), heads=2) == bad and fork(st=(64, 64, 0)) == bad
+    assert fork(n=1 << 28, heads=1 << 12) == bad
     assert fork(ws=lib.dk_paged_fork_workspace_size(4) - 1) == _lib.DK_ERR_WORKSPACE
 
     def compact(n=2, width=4, stride=4, page=8, out=32, free=16, cursor=16, shares=None, n_blocks=9, keep_width=3, ws=1 << 16):
@@ -335,6 +338,56 @@ def test_refused_compaction_changes_nothing(dev, what, shares):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 128, 300])
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_life_of_pages(dev, n, captured):
+    """Two forks of a prompt, one token of two drafts kept in each, all freed: in the pools of many layers."""
+    import torch
+
+    from detkernels_b200 import _lib
+    from detkernels_b200.kernels.paging import paged_compact, paged_fork
+    page = 4
+    pools = [torch.randn(9, 1, page, 8, device=dev, generator=torch.Generator(device=dev).manual_seed(i)) for i in range(n)]
+    start = [p.clone() for p in pools]
+    books = [_i32([[0, 1, 2], [0, 0, 0], [0, 0, 0]], dev), _i32([10, 0, 0], dev), _i32(np.zeros(9), dev),
+             _i32([0, 1, 2, 4, 5, 6, 7, 8], dev)]
+    table, kv, shares, free = books
+    was = [t.clone() for t in books]
+    cursor, src, dst = _i32([3], dev), _i32([0, 0], dev), _i32([1, 2], dev)
+    eight, two, one, none, nine = (_i32([x] * 3, dev) for x in (8, 2, 1, 0, 9))
+    keep = _i32([[1]] * 3, dev)
+
+    def step():
+        at = paged_fork(table, kv, src, dst, page, free_blocks=free, cursor=cursor, shares=shares, pools=pools)
+        a = paged_compact(table, eight, two, one, page, keep=keep, pools=pools, free_blocks=free, cursor=at, shares=shares)
+        held = shares.clone()
+        return a, held, paged_compact(table, none, nine, none, page, free_blocks=free, cursor=a.cursor, shares=shares)
+    if captured:
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream(dev)
+        with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+            a, held, b = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, s in zip(pools, start):
+            p.copy_(s)
+        for t, s in zip(books, was):
+            t.copy_(s)
+        graph.replay()
+    else:
+        a, held, b = step()
+    torch.cuda.synchronize()
+    _lib.raise_on_device_error(torch.cuda.current_device())
+    assert a.lens.tolist() == [9] * 3 and a.cursor.tolist() == [5] and kv.tolist() == [10] * 3
+    assert held.tolist() == [2, 2] + [0] * 7 and shares.tolist() == [0] * 9
+    assert table.tolist() == [[0, 1, 2], [0, 1, 4], [0, 1, 5]]
+    assert b.lens.tolist() == [0] * 3 and b.cursor.tolist() == [0] and free.tolist() == [2, 4, 0, 1, 5, 6, 7, 8]
+    for p, s in zip(pools, start):
+        for block in (2, 4, 5):      # token 9 is token 8 now
+            s[block, :, :2] = s[2, :, 1:2]
+        assert torch.equal(p, s)
+
+
+@pytest.mark.gpu
 def test_wrappers_refuse_on_the_gpu(dev):
     import torch
 
@@ -349,6 +402,8 @@ def test_wrappers_refuse_on_the_gpu(dev):
         paged_fork(t, i, i, i, 8, free_blocks=i, cursor=c, pools=[pool, torch.zeros(5, 1, 8, 8, device=dev)])
     with pytest.raises(ValueError):
         paged_fork(t, i, i, i, 8, free_blocks=i, cursor=c, pools=[pool], shares=i)
+    with pytest.raises(ValueError):
+        paged_fork(t, i, i, i, 8, free_blocks=i, cursor=c, pools=[pool[:1].expand(4, 1, 8, 8)])
     with pytest.raises(AssertionError):
         paged_fork(t, i, i, i, 16, free_blocks=i, cursor=c, pools=[pool])
     with pytest.raises(AssertionError):

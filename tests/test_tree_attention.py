@@ -354,6 +354,28 @@ def test_padded_rows_and_out(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kvs", [[100, 0, 200], [900, 2000, 5]])
+def test_broadcast_inputs(dev, kvs):
+    """Queries, caches and masks that take one place in memory for several rows, heads or sequences; out in q's place."""
+    import torch
+
+    from detkernels_b200.kernels.attention import attention_tree
+    args, kw, own = _case(dev, torch.bfloat16, [5, 5, 5], kvs, 8, 2, 64, fill=0.5)
+    q, kc, vc, kv, cu, mask = args
+
+    def same(q, kc, vc, mask):
+        want = attention_tree(q.contiguous(), kc.contiguous(), vc.contiguous(), kv, cu, mask.contiguous(), **kw)
+        assert torch.equal(attention_tree(q, kc, vc, kv, cu, mask, **kw), want)
+    same(q[:1].expand_as(q), kc, vc, mask)
+    same(q[:, :1].expand_as(q), kc, vc, mask)
+    same(q, kc[:1].expand_as(kc), vc[:1].expand_as(vc), mask)
+    same(q, kc[:, :1].expand_as(kc), vc[:, :1].expand_as(vc), mask)
+    same(q, kc, vc, mask[:1].expand_as(mask))
+    want, out = attention_tree(*args, **kw), q.clone()
+    assert attention_tree(out, kc, vc, kv, cu, mask, out=out, **kw) is out and torch.equal(out, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("what", ["cu_past", "cu_descends", "cu_negative", "rows", "kv_negative", "kv_long", "block"])
 def test_bad_extents_set_the_status(dev, what):
     import torch
