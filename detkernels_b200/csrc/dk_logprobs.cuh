@@ -80,7 +80,10 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 template <typename T>
 struct Raw {
   static constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-  uint32_t w[4];   // kNone: nothing but -infinity
+  // kNone: nothing but -infinity; kFar: logits of weight 0 beside any above kFloor
+  static constexpr uint32_t kFar = sizeof(T) == 4 ? 0xf149f2cau : std::is_same<T, __half>::value ? 0xfbfffbffu : 0xf14af14au;
+  static constexpr float kFloor = std::is_same<T, __half>::value ? -6e4f : -1e29f;
+  uint32_t w[4];
   __device__ __forceinline__ float2 pair(int i) const;   // logits 2 i and 2 i + 1
   __device__ __forceinline__ float at(int i) const {
     const float2 p = pair(i >> 1);
@@ -139,18 +142,23 @@ __device__ __forceinline__ Raw<T> shifted(const uint4& a, const uint4& b, uint32
   for (int j = 0; j < 4; ++j) r.w[j] = __funnelshift_r(t[Q + j], t[(Q + j + 1) & 7], bits);
   return r;
 }
-// Vectors v, v + kThreads, ... of a stage whose row starts `shift` bytes behind a 16-byte word (the same for the whole row).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// Vectors v, v + 32, ... of a warp's stage whose row starts `shift` bytes behind a 16-byte word (the same for the whole row).
 template <typename T, bool ALIGNED, int N>
 __device__ __forceinline__ void vectors_at(Raw<T> (&r)[N], const uint8_t* stage, int v, uint32_t shift) {
   const uint4* at = reinterpret_cast<const uint4*>(stage) + v;
   auto all = [&](auto q) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) r[i] = shifted<T, q>(at[i * kThreads], at[i * kThreads + 1], (shift & 3) * 8);
+    for (int i = 0; i < N; ++i) r[i] = shifted<T, q>(at[i * 32], at[i * 32 + 1], (shift & 3) * 8);
   };
   if (ALIGNED || shift == 0) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const uint4 a = at[i * kThreads];
+      const uint4 a = at[i * 32];
       r[i] = Raw<T>{{a.x, a.y, a.z, a.w}};
     }
   } else {
@@ -162,10 +170,9 @@ __device__ __forceinline__ void vectors_at(Raw<T> (&r)[N], const uint8_t* stage,
     }
   }
 }
-// Of the vector's logits only the first n are the row's, the others become -infinity.
+// Of the vector's logits only the first n are the row's, the others become `none`.
 template <typename T>
-__device__ __forceinline__ void cut(Raw<T>& r, int n) {
-  constexpr uint32_t none = Raw<T>::kNone;
+__device__ __forceinline__ void cut(Raw<T>& r, int n, uint32_t none = Raw<T>::kNone) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) r.w[e] = e < n ? r.w[e] : none;
@@ -231,7 +238,7 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, unsigned long long v) 
 }
 
 struct Shared {
-  float top[2][kWarps], sum[2][2 * kWarps];   // by row parity: the threads' maxima and sums, by warp
+  float top[2][kWarps], s[2][kWarps], t[2][kWarps];   // by row parity: the warps' states
   uint32_t bound[kWarps];
   int scan[kWarps];
   int n_found;
@@ -243,7 +250,8 @@ struct Shared {
 template <typename T, bool TOPK>
 struct Cfg {
   static constexpr int VEC = 16 / sizeof(T), ITERS = kIters;   // logits a vector, vectors a thread
-  static constexpr int PASS = kThreads * ITERS * VEC;          // logits a CTA holds
+  static constexpr int SEG = 32 * ITERS * VEC;                 // logits of a pass that are a warp's
+  static constexpr int PASS = kWarps * SEG;
   static constexpr int STAGE = PASS * sizeof(T) + 128;         // the words around a pass
   static constexpr int STAGES = 8;                             // at most
   static constexpr int CTAS = 4;
@@ -251,26 +259,17 @@ struct Cfg {
   static constexpr int STATIC = sizeof(Shared) + (TOPK ? kCandidates * 8 : 8) + STAGES * 8 + 128;
 };
 
-// The places of `mine` ties in the order of the threads, and their total.
-__device__ __forceinline__ int block_scan(int mine, int* warps, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// The sum of the lanes before this one, and of all.
+__device__ __forceinline__ int warp_scan(int mine, int& total) {
+  const int lane = threadIdx.x & 31;
   int v = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const int o = __shfl_up_sync(0xffffffffu, v, d);
     if (lane >= d) v += o;
   }
-  if (lane == 31) warps[warp] = v;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    if (i < warp) before += warps[i];
-    total += warps[i];
-  }
-  __syncthreads();
-  return before + v - mine;
+  total = __shfl_sync(0xffffffffu, v, 31);
+  return v - mine;
 }
 
 // How many of n keys (and what makes their number even, which is 0) are larger.
@@ -293,273 +292,288 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 template <typename T, bool TOPK, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(const Params p) {
   using C = Cfg<T, TOPK>;
-  constexpr int VEC = C::VEC, ITERS = C::ITERS, kPass = C::PASS;
+  constexpr int VEC = C::VEC, ITERS = C::ITERS, SEG = C::SEG, kPass = C::PASS;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ Shared sh;
   __shared__ __align__(16) unsigned long long found[TOPK ? kCandidates : 1];
   __shared__ __align__(8) uint64_t full[C::STAGES];
   float(*threads)[kMaxParts][kThreads] = reinterpret_cast<float(*)[kMaxParts][kThreads]>(ring + p.stages * C::STAGE);
-  const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   if (p.split) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA has begun
-  if (tid == 0) {
-    for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+  if (tid < C::STAGES) {
+    mbar_init(&full[tid], 1);
     fence_mbar_init();
   }
   __syncthreads();
   pdl_wait();
   if (tid == 0) pdl_launch_dependents();
-  // the passes that this CTA goes through
-  const int64_t row_step = p.split ? p.n_rows : gridDim.x;
-  const int64_t row0 = p.split ? blockIdx.x / p.parts : blockIdx.x;
+  // the passes that this CTA goes through: [j0, j0 + nj) of rows row0, row0 + row_step, ...
+  const uint32_t n_rows = static_cast<uint32_t>(p.n_rows), row_step = p.split ? n_rows : gridDim.x;
+  const uint32_t row0 = p.split ? blockIdx.x / static_cast<uint32_t>(p.parts) : blockIdx.x;
   const int first_part = p.split ? static_cast<int>(blockIdx.x - row0 * p.parts) : 0;
-  const int end_part = p.split ? first_part + 1 : p.parts;
-  struct Pass {
-    int64_t row;
-    int part, begin, end;   // its first logit, and the part's end
-    bool last_of_part, last;
-  };
-  auto set = [&](Pass& a) {
-    a.end = min(p.n_vocab, (a.part + 1) * p.part);
-    a.last_of_part = a.begin + kPass >= a.end;
-    a.last = a.last_of_part && a.part + 1 == end_part;
-  };
-  auto step = [&](Pass& a) {
-    if (a.last) {
-      a.row += row_step;
-      a.part = first_part;
-      a.begin = a.part * p.part;
-    } else if (a.last_of_part) {
-      a.part += 1;
-      a.begin = a.part * p.part;
-    } else {
-      a.begin += kPass;
-    }
-    set(a);
-  };
-  auto row_of = [&](int64_t r) { return static_cast<const T*>(p.x) + r * p.stride; };
-  auto shift_of = [&](const T* x) { return ALIGNED ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x) & 15u); };
-  Pass at{row0, first_part, first_part * p.part, 0, false, false};
-  set(at);
-  Pass ahead = at;
+  const int per = p.part / kPass, j0 = first_part * per, to_end = (p.n_vocab + kPass - 1) / kPass - j0;
+  const int nj = p.split ? min(to_end, per) : to_end;
+  constexpr int kSize = static_cast<int>(sizeof(T));
+  const int64_t row_bytes = static_cast<int64_t>(row_step) * p.stride * kSize;
+  const uint8_t* x_bytes = static_cast<const uint8_t*>(p.x) + row0 * p.stride * kSize;
   bool abort_flag = false;
-  auto issue = [&](int stage) {   // thread 0: the next pass that is not on its way, with the words around it
-    if (ahead.row < p.n_rows) {
-      const uint8_t* a = reinterpret_cast<const uint8_t*>(row_of(ahead.row) + ahead.begin);
-      const uint32_t before = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a) & 15u);
-      const uint32_t bytes = (before + min(kPass, ahead.end - ahead.begin) * static_cast<uint32_t>(sizeof(T)) + 15u) & ~15u;
+  const int from = j0 * kPass;                         // the CTA's first logit of a row
+  // The next pass that is not on its way (warp 0), with the words around it.
+  const uint8_t* ahead = x_bytes + static_cast<int64_t>(from) * kSize;
+  int ahead_left = p.n_vocab - from, ahead_n = nj;     // logits from there to the row's end; passes to go
+  uint32_t ahead_rows = row0 < n_rows ? (n_rows - row0 + row_step - 1) / row_step : 0;
+  auto issue = [&](int stage) {
+    if (ahead_rows == 0) return;
+    const uint32_t before = ALIGNED ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ahead) & 15u);
+    const uint32_t bytes = (before + static_cast<uint32_t>(min(kPass, ahead_left) * kSize) + 15u) & ~15u;
+    if (elect_one()) {
       mbar_arrive_expect_tx(&full[stage], bytes);
-      bulk_load_1d(ring + stage * C::STAGE, a - before, bytes, &full[stage]);
-      step(ahead);
+      bulk_load_1d(ring + stage * C::STAGE, ahead - before, bytes, &full[stage]);
+    }
+    __syncwarp();
+    ahead += kPass * kSize;
+    ahead_left -= kPass;
+    if (--ahead_n == 0) {
+      ahead_n = nj;
+      ahead_left += nj * kPass;
+      ahead += row_bytes - static_cast<int64_t>(nj) * (kPass * kSize);
+      --ahead_rows;
     }
   };
-  if (tid == 0)
+  if (warp == 0)
     for (int s = 0; s < p.stages; ++s) issue(s);
-  State st{-INFINITY, 0.0f, 0.0f}, in_part{-INFINITY, 0.0f, 0.0f};
   int held = 0;         // alternatives so far, at the front of `found`
   int n = 0;            // and candidates behind them
   uint32_t bound = 0;   // below the k-th largest logit; once there are k of them, the k-th itself
   int flip = 0;         // row parity
-  float asked = 0.0f;   // thread 0: the logit of the row's token, fetched long before it is used
   int stage = 0;
   uint32_t phase = 0;
-  for (; at.row < p.n_rows; step(at)) {
-    const int64_t row = at.row;
-    const int part = at.part, begin = at.begin, end = at.end;
-    const T* x = row_of(row);
-    const uint32_t shift = shift_of(x);
-    const uint8_t* here = ring + stage * C::STAGE;
-    const bool new_part = begin == part * p.part, new_row = new_part && part == first_part;
-    if (new_row && tid == 0 && part == 0 && p.tokens) {
+  for (uint32_t row = row0; row < n_rows; row += row_step, x_bytes += row_bytes) {
+    const uint32_t shift = ALIGNED ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x_bytes) & 15u);
+    float asked = 0.0f;   // thread 0: the logit of the row's token, fetched long before it is used
+    if (tid == 0 && first_part == 0 && p.tokens) {
       const int64_t tok = p.tokens[row];
-      if (tok >= 0 && tok < p.n_vocab) asked = to_f32<T>(x[tok]);
+      if (tok >= 0 && tok < p.n_vocab) asked = to_f32<T>(reinterpret_cast<const T*>(x_bytes)[tok]);
     }
-    mbar_wait(&full[stage], phase, kDetFull, abort_flag);
-    // vectors of which some lane of this warp has a logit
-    const int left = end - begin, some_have = (left - warp * 32 * VEC + kThreads * VEC - 1) / (kThreads * VEC);
-    State now{-INFINITY, 0.0f, 0.0f};
-    auto sum_up = [&](auto whole) {   // a whole pass, or what there is of one
-      Raw<T> r[ITERS];
-      vectors_at<T, ALIGNED>(r, here, tid, shift);
-      uint32_t mw = Raw<T>::kNone;
+    State st{-INFINITY, 0.0f, 0.0f}, in_part{-INFINITY, 0.0f, 0.0f};
+    int left = p.n_vocab - from - warp * SEG;   // logits from the warp's first of the pass on
+    int in = per;                      // passes to go in the part
+    if (TOPK) held = n = 0;
+    for (int j = 0; j < nj; ++j, left -= kPass) {
+      const uint8_t* here = ring + stage * C::STAGE + warp * (SEG * kSize);
+      mbar_wait(&full[stage], phase, kDetFull, abort_flag);
+      State now{-INFINITY, 0.0f, 0.0f};
+      if (left > 0) {
+        Raw<T> r[ITERS];
+        vectors_at<T, ALIGNED>(r, here, lane, shift);
+        if (left < SEG) {
 #pragma unroll
-      for (int i = 0; i < ITERS; ++i) {
-        if (!whole) {
-          if (i >= some_have) break;
-          cut(r[i], left - (i * kThreads + tid) * VEC);
+          for (int i = 0; i < ITERS; ++i) cut(r[i], left - (i * 32 + lane) * VEC);
         }
-        mw = max_word<T>(mw, max_word<T>(max_word<T>(r[i].w[0], r[i].w[1]), max_word<T>(r[i].w[2], r[i].w[3])));
-      }
-      now.m = max_of<T>(mw);
-      const float ref = now.m == -INFINITY ? 0.0f : now.m;
-      const float2 off = make_float2(-ref, -ref), unit = make_float2(kLog2e, kLog2e);
-      auto sums = [&](auto far) {
+        uint32_t mw = Raw<T>::kNone;
+#pragma unroll
+        for (int i = 0; i < ITERS; ++i)
+          mw = max_word<T>(mw, max_word<T>(max_word<T>(r[i].w[0], r[i].w[1]), max_word<T>(r[i].w[2], r[i].w[3])));
+        now.m = max_of<T>(mw);
+        const float ref = now.m == -INFINITY ? 0.0f : now.m, c = __fmul_rn(ref, kLog2e);
+        const float2 unit = make_float2(kLog2e, kLog2e);
         float2 s2[2], t2[2];
+        auto add = [&](float2 y, int e) {
+          const float2 w = make_float2(ex2(y.x), ex2(y.y));
+          s2[e & 1] = add2(s2[e & 1], w);
+          t2[e & 1] = fma2(y, w, t2[e & 1]);
+        };
+        auto sum_up = [&]() {
+          s2[0] = add2(s2[0], s2[1]);
+          t2[0] = add2(t2[0], t2[1]);
+          now.s = s2[0].x + s2[0].y;
+          now.t = t2[0].x + t2[0].y;
+        };
+        // (what is not the row's is -infinity no more, which would cost the second pass below)
+        if (left < SEG) {
+#pragma unroll
+          for (int i = 0; i < ITERS; ++i) cut(r[i], left - (i * 32 + lane) * VEC, Raw<T>::kFar);
+        }
+        // y = x log2 e - c, c = m log2 e rounded: one operation for two logits.  What c is off by is put right in the sums.
         s2[0] = s2[1] = t2[0] = t2[1] = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int i = 0; i < ITERS; ++i) {
-          if (!whole && i >= some_have) break;
+        for (int i = 0; i < ITERS; ++i)
 #pragma unroll
-          for (int e = 0; e < VEC / 2; ++e) {
-            float2 y = mul2(add2(r[i].pair(e), off), unit);
-            if (far) y = make_float2(max_nan(y.x, -200.0f), max_nan(y.y, -200.0f));
-            const float2 w = make_float2(ex2(y.x), ex2(y.y));
-            s2[e & 1] = add2(s2[e & 1], w);
-            t2[e & 1] = fma2(y, w, t2[e & 1]);
-          }
-        }
-        s2[0] = add2(s2[0], s2[1]);
-        t2[0] = add2(t2[0], t2[1]);
-        now.s = s2[0].x + s2[0].y;
-        now.t = t2[0].x + t2[0].y;
-      };
-      sums(std::false_type());
-      // An excluded logit (-infinity, or as far away) has weight 0 and must not meet its infinite distance: once more, with
-      // distances that end where weights have long been 0.
-      if (now.t != now.t) sums(std::true_type());
-    };
-    if (left >= kPass) {
-      sum_up(std::true_type());
-    } else if (some_have > 0) {
-      sum_up(std::false_type());
-    }
-    const float m = now.m;
-    in_part = new_part ? now : joined(in_part, now);
-    if (at.last_of_part) st = part == first_part ? in_part : joined(st, in_part);
-    if constexpr (TOPK) {
-      if (new_row) held = n = 0;
-      const int nvec = min(kThreads * ITERS, (end - begin + VEC - 1) / VEC);
-      const uint32_t own = tid < nvec ? key_of(m) : 0u;
-      if (held < p.k) {
-        // the bound from the threads' maxima
-        uint32_t mine = own;
-        const int warps = min(kWarps, max(1, nvec / 32));   // those with a logit in every lane
-        uint32_t low = 0;
-        for (int a = (p.k + warps - 1) / warps; a > 0; --a) {
-          low = __reduce_max_sync(0xffffffffu, mine);
-          const uint32_t who = __ballot_sync(0xffffffffu, mine == low);
-          if (lane == __ffs(who) - 1) mine = 0u;
-        }
-        if (lane == 0) sh.bound[warp] = low;
-        if (tid == 0) sh.n_found = held;
-        n = held;
-        __syncthreads();
-        bound = sh.bound[0];
-        for (int w = 1; w < warps; ++w) bound = min(bound, sh.bound[w]);
-      }
-      // everything above the bound; whether there is any.  A warp takes its threads with a larger maximum one after the
-      // other, a lane a logit.
-      auto collect = [&]() {
-        const bool mine = own > bound;
-        uint32_t who = __ballot_sync(0xffffffffu, mine);
-        const float most = value_of(bound);
-        const T* logits = reinterpret_cast<const T*>(here + shift);
-        const int off = lane < ITERS * VEC ? lane / VEC * (kThreads * VEC) + lane % VEC : left;
-        while (who) {   // four threads at a time: one place in the list is asked for all that they have
-          constexpr int Q = 4;
-          float v[Q];
-          int at[Q];
-          uint32_t hits[Q];
-#pragma unroll
-          for (int q = 0; q < Q; ++q) {
-            at[q] = who ? (warp * 32 + __ffs(who) - 1) * VEC + off : left;
-            who &= who - 1;
-            v[q] = at[q] < left ? to_f32<T>(logits[at[q]]) : -INFINITY;
-          }
-          int n_hits = 0;
-#pragma unroll
-          for (int q = 0; q < Q; ++q) {
-            // (the bound is a number where something lies above it; below it there is nothing but at first)
-            hits[q] = __ballot_sync(0xffffffffu, at[q] < left && (bound == 0 || !(v[q] <= most)));
-            n_hits += __popc(hits[q]);
-          }
-          int f = 0;
-          if (lane == 0) f = atomicAdd(&sh.n_found, n_hits);
-          f = __shfl_sync(0xffffffffu, f, 0);
-#pragma unroll
-          for (int q = 0; q < Q; ++q) {
-            const int to = f + __popc(hits[q] & ((1u << lane) - 1));
-            if ((hits[q] >> lane & 1u) && to < kCandidates)
-              found[to] = static_cast<unsigned long long>(key_of(v[q])) << 32 | ~static_cast<uint32_t>(begin + at[q]);
-            f += __popc(hits[q]);
-          }
-        }
-        return __syncthreads_or(mine);
-      };
-      const bool some = collect();
-      bool fresh = held < p.k;   // the bound is of this pass's logits: at it, too, they may be alternatives
-      if (some && sh.n_found - n > kPoor) {
-        // the k-th largest of the threads' maxima, bit by bit
-        uint32_t best = 0;
-        for (int b = 31; b >= 0; --b) {
-          const uint32_t to = best | 1u << b;
-          if (__syncthreads_count(own >= to) >= p.k) best = to;
-        }
-        if (best > bound) {
-          bound = best;
-          fresh = true;
-          if (tid == 0) sh.n_found = n;
-          __syncthreads();
-          collect();
-        }
-      }
-      const int before = n;
-      if (some) n = sh.n_found;
-      if (fresh) {
-        // ties at the bound, in the order of their indices, until the pass has given k
-        int need = min(p.k, end - begin) - (n - before);
-        if (need > 0) {
+          for (int e = 0; e < VEC / 2; ++e) add(fma2(r[i].pair(e), unit, make_float2(-c, -c)), e);
+        sum_up();
+        const float d = fmaf(-ref, kLog2e, c), f = ex2(d);   // (x - m) log2 e = y + d
+        now.t = f * fmaf(d, now.s, now.t);
+        now.s = f * now.s;
+        // An excluded logit (-infinity, or as far away) has weight 0 and must not meet its infinite distance, and a product may
+        // be beyond f32: once more, differences first, with distances that end where weights have long been 0.
+        if (!(fabsf(now.t) < INFINITY) || (left < SEG && now.m <= Raw<T>::kFloor && now.m != -INFINITY)) {
+          s2[0] = s2[1] = t2[0] = t2[1] = make_float2(0.0f, 0.0f);
 #pragma unroll 1
-          for (int i = 0; i < ITERS && need > 0; ++i) {
-            const int first = begin + (i * kThreads + tid) * VEC;
-            int ties = 0;
-            Raw<T> vs[1];
-            vectors_at<T, ALIGNED>(vs, here, i * kThreads + tid, shift);
-            const Raw<T>& v = vs[0];
+          for (int i = 0; i < ITERS; ++i) {
+            Raw<T> v[1];
+            vectors_at<T, ALIGNED>(v, here, i * 32 + lane, shift);
+            cut(v[0], left - (i * 32 + lane) * VEC);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) ties += key_of(v.at(e)) == bound && first + e < end;
-            int total;
-            int f = block_scan(ties, sh.scan, total);
+            for (int e = 0; e < VEC / 2; ++e) {
+              const float2 y = mul2(add2(v[0].pair(e), make_float2(-ref, -ref)), unit);
+              add(make_float2(max_nan(y.x, -200.0f), max_nan(y.y, -200.0f)), e);
+            }
+          }
+          sum_up();
+        }
+      }
+      const float m = now.m;
+      in_part = in == per ? now : joined(in_part, now);
+      if (--in == 0 || j + 1 == nj) {
+        st = j < per ? in_part : joined(st, in_part);
+        in = per;
+      }
+      if constexpr (TOPK) {
+        const int begin = (j0 + j) * kPass, end = min(p.n_vocab, begin + kPass);
+        const int nvec = (end - begin + VEC - 1) / VEC;
+        const uint32_t own = warp * (SEG / VEC) + lane < nvec ? key_of(m) : 0u;
+        if (held < p.k) {
+          // the bound from the threads' maxima
+          uint32_t mine = own;
+          const int warps = max(1, nvec / (SEG / VEC));   // whose threads all have as many logits
+          uint32_t low = 0;
+          for (int a = (p.k + warps - 1) / warps; a > 0; --a) {
+            low = __reduce_max_sync(0xffffffffu, mine);
+            const uint32_t who = __ballot_sync(0xffffffffu, mine == low);
+            if (lane == __ffs(who) - 1) mine = 0u;
+          }
+          if (lane == 0) sh.bound[warp] = low;
+          if (tid == 0) sh.n_found = held;
+          n = held;
+          __syncthreads();
+          bound = sh.bound[0];
+          for (int w = 1; w < warps; ++w) bound = min(bound, sh.bound[w]);
+        }
+        // Everything above `lim`; whether there is any.  A warp takes its threads with a larger maximum one after the other, a
+        // lane a logit.
+        auto collect = [&](uint32_t lim) {
+          const bool mine = own > lim;
+          uint32_t who = __ballot_sync(0xffffffffu, mine);
+          const T* logits = reinterpret_cast<const T*>(here + shift);
+          const int off = lane < ITERS * VEC ? lane / VEC * (32 * VEC) + lane % VEC : left;
+          while (who) {   // four threads at a time: one place in the list is asked for all that they have
+            constexpr int Q = 4;
+            uint32_t key[Q], hits[Q];
+            int at[Q];
+            int n_hits = 0;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e)
-              if (key_of(v.at(e)) == bound && first + e < end) {
-                if (f < need) found[n + f] = static_cast<unsigned long long>(bound) << 32 | ~static_cast<uint32_t>(first + e);
-                ++f;
+            for (int q = 0; q < Q; ++q) {
+              at[q] = who ? (__ffs(who) - 1) * VEC + off : left;
+              who &= who - 1;
+              key[q] = at[q] < left ? key_of(to_f32<T>(logits[at[q]])) : 0u;
+            }
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+              hits[q] = __ballot_sync(0xffffffffu, key[q] > lim);
+              n_hits += __popc(hits[q]);
+            }
+            int f = 0;
+            if (lane == 0) f = atomicAdd(&sh.n_found, n_hits);
+            f = __shfl_sync(0xffffffffu, f, 0);
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+              const int to = f + __popc(hits[q] & ((1u << lane) - 1));
+              if ((hits[q] >> lane & 1u) && to < kCandidates)
+                found[to] = static_cast<unsigned long long>(key[q]) << 32 | ~static_cast<uint32_t>(begin + warp * SEG + at[q]);
+              f += __popc(hits[q]);
+            }
+          }
+          return __syncthreads_or(mine);
+        };
+        // A bound from this pass's logits: at it, too, they may be alternatives.  (Every logit's key is above 0.)
+        bool fresh = held < p.k;
+        const bool some = collect(fresh && bound > 0 ? bound - 1 : bound);
+        bool ties = false;
+        if (some && sh.n_found - n > kPoor) {
+          // the k-th largest of the threads' maxima, bit by bit
+          uint32_t best = 0;
+          for (int b = 31; b >= 0; --b) {
+            const uint32_t to = best | 1u << b;
+            if (__syncthreads_count(own >= to) >= p.k) best = to;
+          }
+          if (fresh || best > bound) {
+            bound = max(bound, best);
+            fresh = ties = true;
+            if (tid == 0) sh.n_found = n;
+            __syncthreads();
+            collect(bound);
+          }
+        }
+        const int before = n;
+        if (some) n = sh.n_found;
+        if (ties) {
+          // those at the bound, in the order of their indices, until the pass has given k
+          const int need = min(p.k, end - begin) - (n - before);
+          if (need > 0) {
+            auto tie = [&](int i, int e) {   // the logit itself: a tie, or -1
+              const int at = (i * 32 + lane) * VEC + e;
+              return at < left && key_of(to_f32<T>(reinterpret_cast<const T*>(here + shift)[at])) == bound ? at : -1;
+            };
+            int mine = 0;
+#pragma unroll 1
+            for (int i = 0; i < ITERS; ++i)
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) mine += tie(i, e) >= 0;
+            const int all = __reduce_add_sync(0xffffffffu, mine);
+            if (lane == 0) sh.scan[warp] = all;
+            __syncthreads();
+            int total = 0, f = 0;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+              if (w < warp) f += sh.scan[w];
+              total += sh.scan[w];
+            }
+#pragma unroll 1
+            for (int i = 0; i < ITERS && f < need; ++i) {
+              int ties = 0, sum;
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) ties += tie(i, e) >= 0;
+              int g = f + warp_scan(ties, sum);
+              f += sum;
+              if (ties == 0) continue;
+#pragma unroll 1
+              for (int e = 0; e < VEC && g < need; ++e) {
+                const int at = tie(i, e);
+                if (at >= 0) found[n + g++] = static_cast<unsigned long long>(bound) << 32 | ~static_cast<uint32_t>(begin + warp * SEG + at);
               }
+            }
             n += min(total, need);
-            need -= total;
+          }
+        }
+        if (fresh || n > min(kMany, 2 * p.k + 16) || j + 1 == nj) {
+          // the k largest so far, by counting (keys are distinct)
+          if (tid == 0 && (n & 1)) found[n] = 0ull;   // below all keys
+          __syncthreads();
+          for (int i = tid; i < n; i += kThreads) {
+            const unsigned long long key = found[i];
+            const int above = count_above(found, n, key);
+            if (above < p.k) sh.sorted[above] = key;
           }
           __syncthreads();
+          held = min(p.k, n);   // (k of the first pass on, but for a row that has no more)
+          if (tid < held) found[tid] = sh.sorted[tid];
+          if (held == p.k) bound = static_cast<uint32_t>(sh.sorted[p.k - 1] >> 32);   // an equal logit behind it comes later
+          if (tid == 0) sh.n_found = held;
+          n = held;
+          __syncthreads();
+        } else if (some) {
+          __syncthreads();   // everyone knows the count, the next pass may add to it
         }
       }
-      if (fresh || n > min(kMany, 2 * p.k + 16) || at.last) {
-        // the k largest so far, by counting (keys are distinct)
-        if (tid == 0 && (n & 1)) found[n] = 0ull;   // below all keys
-        __syncthreads();
-        for (int i = tid; i < n; i += kThreads) {
-          const unsigned long long key = found[i];
-          const int above = count_above(found, n, key);
-          if (above < p.k) sh.sorted[above] = key;
-        }
-        __syncthreads();
-        held = min(p.k, n);   // (k of the first pass on, but for a row that has no more)
-        if (tid < held) found[tid] = sh.sorted[tid];
-        if (held == p.k) bound = static_cast<uint32_t>(sh.sorted[p.k - 1] >> 32);   // an equal logit behind it comes later
-        if (tid == 0) sh.n_found = held;
-        n = held;
-        __syncthreads();
-      } else if (some) {
-        __syncthreads();   // everyone knows the count, the next pass may add to it
+      if (!TOPK) __syncthreads();   // the stage has been read
+      if (warp == 0) issue(stage);
+      if (++stage == p.stages) {
+        stage = 0;
+        phase ^= 1u;
       }
-    } else {
-      __syncthreads();     // the stage has been read
     }
-    if (tid == 0) issue(stage);
-    if (++stage == p.stages) {
-      stage = 0;
-      phase ^= 1u;
-    }
-    if (!at.last) continue;
     if (p.split) {
+      const int part = first_part;
       asm volatile("barrier.cluster.wait.aligned;" ::: "memory");   // the first CTA of the row has begun
       st_cluster(map_to_first(smem_u32(&threads[0][part][tid])), st.m);
       st_cluster(map_to_first(smem_u32(&threads[1][part][tid])), st.s);
@@ -574,32 +588,32 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
         st = q == 0 ? o : joined(st, o);
       }
     }
-    // the threads against the row's maximum, then their sums: lanes, warps
-    float top = warp_max_nan(st.m);
-    if (lane == 0) sh.top[flip][warp] = top;
-    __syncthreads();
-    top = sh.top[flip][0];
-#pragma unroll
-    for (int i = 1; i < kWarps; ++i) top = max_nan(top, sh.top[flip][i]);
-    const float g = st.m == -INFINITY ? 0.0f : (st.m - top) * kLog2e, f = ex2(g);
-    float s = f * st.s, t = f * fmaf(max_nan(g, -200.0f), st.s, st.t);
+    // the lanes against their warp's maximum, then the warps against the row's
+    auto rebased = [](State a, float to) {
+      const float g = a.m == -INFINITY ? 0.0f : (a.m - to) * kLog2e, f = ex2(g);
+      return State{to, f * a.s, f * fmaf(max_nan(g, -200.0f), a.s, a.t)};
+    };
+    st = rebased(st, warp_max_nan(st.m));
 #pragma unroll
     for (int d = 16; d; d >>= 1) {
-      s += __shfl_xor_sync(0xffffffffu, s, d);
-      t += __shfl_xor_sync(0xffffffffu, t, d);
+      st.s += __shfl_xor_sync(0xffffffffu, st.s, d);
+      st.t += __shfl_xor_sync(0xffffffffu, st.t, d);
     }
     if (lane == 0) {
-      sh.sum[flip][warp] = s;
-      sh.sum[flip][kWarps + warp] = t;
+      sh.top[flip][warp] = st.m;
+      sh.s[flip][warp] = st.s;
+      sh.t[flip][warp] = st.t;
     }
     __syncthreads();
     if (warp == 0 || p.split) {
-      s = sh.sum[flip][0];
-      t = sh.sum[flip][kWarps];
+      float top = sh.top[flip][0], s = 0.0f, t = 0.0f;
 #pragma unroll
-      for (int i = 1; i < kWarps; ++i) {
-        s += sh.sum[flip][i];
-        t += sh.sum[flip][kWarps + i];
+      for (int i = 1; i < kWarps; ++i) top = max_nan(top, sh.top[flip][i]);
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) {
+        const State o = rebased(State{sh.top[flip][i], sh.s[flip][i], sh.t[flip][i]}, top);
+        s += o.s;
+        t += o.t;
       }
       const float log_s = log2f(s);
       auto log_p = [&](float v) { return fmaf(-kLn2, log_s, v - top); };
@@ -617,11 +631,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
       }
       if constexpr (TOPK) {
         auto give = [&](int to, unsigned long long key) {
-          p.top_ids[row * p.k + to] = static_cast<int64_t>(~static_cast<uint32_t>(key));
-          p.top_lp[row * p.k + to] = log_p(value_of(static_cast<uint32_t>(key >> 32)));
+          const int64_t at = static_cast<int64_t>(row) * p.k + to;
+          p.top_ids[at] = static_cast<int64_t>(~static_cast<uint32_t>(key));
+          p.top_lp[at] = log_p(value_of(static_cast<uint32_t>(key >> 32)));
         };
         if (!p.split) {
-          if (lane < held) give(lane, sh.sorted[lane]);
+          if (lane < held) give(lane, sh.sorted[lane]);   // (the next row's come behind more barriers)
         } else {
           const int all = p.parts * p.k;   // at most 256
           if (tid < all) {
@@ -632,7 +647,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
         }
       }
     }
-    if (TOPK) __syncthreads();   // `sorted` is free for the next row
     flip ^= 1;
   }
 }
