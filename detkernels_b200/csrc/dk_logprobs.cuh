@@ -241,8 +241,8 @@ struct Shared {
   float top[2][kWarps], s[2][kWarps], t[2][kWarps];   // by row parity: the warps' states
   uint32_t bound[kWarps];
   int scan[kWarps];
-  int n_found;
-  __align__(16) unsigned long long best[kMaxParts * kMaxK + 1];   // the parts' alternatives (k of each), in the first CTA of a split row
+  int n_found[3];   // by pass: what is being counted, what is read, what is 0
+  __align__(16) unsigned long long best[kMaxParts * kMaxK];   // the parts' alternatives (k of each), in the first CTA of a split row
   unsigned long long sorted[kMaxK];
 };
 
@@ -272,15 +272,15 @@ __device__ __forceinline__ int warp_scan(int mine, int& total) {
   return v - mine;
 }
 
-// How many of n keys (and what makes their number even, which is 0) are larger.
+// How many of n keys are larger.
 __device__ __forceinline__ int count_above(const unsigned long long* keys, int n, unsigned long long key) {
   int above = 0;
 #pragma unroll 4
-  for (int j = 0; j < n; j += 2) {
+  for (int j = 0; j + 1 < n; j += 2) {
     const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(keys + j);
     above += (two.x > key) + (two.y > key);
   }
-  return above;
+  return above + (n & 1 && keys[n - 1] > key);
 }
 
 __device__ __forceinline__ float warp_max_nan(float v) {
@@ -300,6 +300,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
   float(*threads)[kMaxParts][kThreads] = reinterpret_cast<float(*)[kMaxParts][kThreads]>(ring + p.stages * C::STAGE);
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   if (p.split) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA has begun
+  if (tid < 3) sh.n_found[tid] = 0;
   if (tid < C::STAGES) {
     mbar_init(&full[tid], 1);
     fence_mbar_init();
@@ -342,6 +343,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
   };
   if (warp == 0)
     for (int s = 0; s < p.stages; ++s) issue(s);
+  int slot = 0;         // of the count of found ones
   int held = 0;         // alternatives so far, at the front of `found`
   int n = 0;            // and candidates behind them
   uint32_t bound = 0;   // below the k-th largest logit; once there are k of them, the k-th itself
@@ -443,28 +445,31 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
             if (lane == __ffs(who) - 1) mine = 0u;
           }
           if (lane == 0) sh.bound[warp] = low;
-          if (tid == 0) sh.n_found = held;
-          n = held;
           __syncthreads();
           bound = sh.bound[0];
           for (int w = 1; w < warps; ++w) bound = min(bound, sh.bound[w]);
         }
-        // Everything above `lim`; whether there is any.  A warp takes its threads with a larger maximum one after the other, a
-        // lane a logit.
+        // Everything above `lim`, behind the n that there are; how many.  A warp takes its threads with a larger maximum some at
+        // a time, a lane a logit: one place in the list is asked for all that they have.
         auto collect = [&](uint32_t lim) {
-          const bool mine = own > lim;
-          uint32_t who = __ballot_sync(0xffffffffu, mine);
+          constexpr int OWN = ITERS * VEC, AT_ONCE = 32 / OWN, Q = 4 / AT_ONCE;   // a thread's logits, threads at once, times
+          uint32_t who = __ballot_sync(0xffffffffu, own > lim);
           const T* logits = reinterpret_cast<const T*>(here + shift);
-          const int off = lane < ITERS * VEC ? lane / VEC * (32 * VEC) + lane % VEC : left;
-          while (who) {   // four threads at a time: one place in the list is asked for all that they have
-            constexpr int Q = 4;
+          const int off = lane % OWN / VEC * (32 * VEC) + lane % VEC;
+          while (who) {
             uint32_t key[Q], hits[Q];
             int at[Q];
             int n_hits = 0;
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
-              at[q] = who ? (__ffs(who) - 1) * VEC + off : left;
+              int thread = who ? __ffs(who) - 1 : -1;
               who &= who - 1;
+              if (AT_ONCE == 2) {
+                const int other = who ? __ffs(who) - 1 : -1;
+                who &= who - 1;
+                if (lane >= OWN) thread = other;
+              }
+              at[q] = thread >= 0 ? thread * VEC + off : left;
               key[q] = at[q] < left ? key_of(to_f32<T>(logits[at[q]])) : 0u;
             }
 #pragma unroll
@@ -473,8 +478,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
               n_hits += __popc(hits[q]);
             }
             int f = 0;
-            if (lane == 0) f = atomicAdd(&sh.n_found, n_hits);
-            f = __shfl_sync(0xffffffffu, f, 0);
+            if (lane == 0) f = atomicAdd(&sh.n_found[slot], n_hits);
+            f = n + __shfl_sync(0xffffffffu, f, 0);
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
               const int to = f + __popc(hits[q] & ((1u << lane) - 1));
@@ -483,13 +488,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
               f += __popc(hits[q]);
             }
           }
-          return __syncthreads_or(mine);
+          __syncthreads();
+          return sh.n_found[slot];
         };
         // A bound from this pass's logits: at it, too, they may be alternatives.  (Every logit's key is above 0.)
         bool fresh = held < p.k;
-        const bool some = collect(fresh && bound > 0 ? bound - 1 : bound);
+        int got = collect(fresh && bound > 0 ? bound - 1 : bound);
         bool ties = false;
-        if (some && sh.n_found - n > kPoor) {
+        if (got > kPoor) {
           // the k-th largest of the threads' maxima, bit by bit
           uint32_t best = 0;
           for (int b = 31; b >= 0; --b) {
@@ -499,16 +505,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
           if (fresh || best > bound) {
             bound = max(bound, best);
             fresh = ties = true;
-            if (tid == 0) sh.n_found = n;
+            if (tid == 0) sh.n_found[slot] = 0;
             __syncthreads();
-            collect(bound);
+            got = collect(bound);
           }
         }
-        const int before = n;
-        if (some) n = sh.n_found;
+        n += got;
+        slot = slot == 2 ? 0 : slot + 1;
+        if (tid == 0) sh.n_found[slot == 2 ? 0 : slot + 1] = 0;   // read by all before this pass's barrier, counted in after the next
         if (ties) {
           // those at the bound, in the order of their indices, until the pass has given k
-          const int need = min(p.k, end - begin) - (n - before);
+          const int need = min(p.k, end - begin) - got;
           if (need > 0) {
             auto tie = [&](int i, int e) {   // the logit itself: a tie, or -1
               const int at = (i * 32 + lane) * VEC + e;
@@ -545,10 +552,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
             n += min(total, need);
           }
         }
-        if (fresh || n > min(kMany, 2 * p.k + 16) || j + 1 == nj) {
+        if (fresh || n > min(kMany, 2 * p.k + 16) || (j + 1 == nj && n > held)) {
           // the k largest so far, by counting (keys are distinct)
-          if (tid == 0 && (n & 1)) found[n] = 0ull;   // below all keys
-          __syncthreads();
+          if (ties) __syncthreads();
           for (int i = tid; i < n; i += kThreads) {
             const unsigned long long key = found[i];
             const int above = count_above(found, n, key);
@@ -558,11 +564,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
           held = min(p.k, n);   // (k of the first pass on, but for a row that has no more)
           if (tid < held) found[tid] = sh.sorted[tid];
           if (held == p.k) bound = static_cast<uint32_t>(sh.sorted[p.k - 1] >> 32);   // an equal logit behind it comes later
-          if (tid == 0) sh.n_found = held;
           n = held;
-          __syncthreads();
-        } else if (some) {
-          __syncthreads();   // everyone knows the count, the next pass may add to it
         }
       }
       if (!TOPK) __syncthreads();   // the stage has been read
@@ -578,10 +580,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
       st_cluster(map_to_first(smem_u32(&threads[0][part][tid])), st.m);
       st_cluster(map_to_first(smem_u32(&threads[1][part][tid])), st.s);
       st_cluster(map_to_first(smem_u32(&threads[2][part][tid])), st.t);
-      if (TOPK && tid < p.k) st_cluster(map_to_first(smem_u32(&sh.best[part * p.k + tid])), tid < held ? found[tid] : 0ull);
+      if (TOPK && tid < p.k) st_cluster(map_to_first(smem_u32(&sh.best[part * p.k + tid])), tid < held ? sh.sorted[tid] : 0ull);
       asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
       if (part != 0) return;   // a split row is all that its CTAs do
-      if (TOPK && tid == 0) sh.best[p.parts * p.k] = 0ull;   // read where the keys are odd in number
       asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
       for (int q = 0; q < p.parts; ++q) {
         const State o{threads[0][q][tid], threads[1][q][tid], threads[2][q][tid]};
