@@ -185,7 +185,7 @@ __device__ __forceinline__ Cost cost_of(const Params& p, const Seq& s) {
 // its first item.
 __host__ __device__ inline int64_t plan_ints(int64_t n_seqs) { return 4 + 4 * n_seqs; }
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 256;
 template <int D>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ Params p) {
   __shared__ int bucket[kPlanThreads];   // by cost, the most expensive first: groups, then their places
