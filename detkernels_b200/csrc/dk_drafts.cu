@@ -113,7 +113,7 @@ int move(dk::pages::MoveParams& p, const Pools& c, int64_t n, int64_t most, bool
   // Token lanes as the tokens ask for: a few of many columns at once, or many of a head's columns.
   constexpr int U = 8;
   int lanes_log = 0;
-  while (lanes_log < 4 && (static_cast<int64_t>(U) << lanes_log) < most) ++lanes_log;
+  while (lanes_log < dk::pages::kMaxLanesLog && (static_cast<int64_t>(U) << lanes_log) < most) ++lanes_log;
   p.cols_log = 8 - lanes_log;
   for (int first = 0; first < c.n; first += dk::pages::kMaxPools) {
     const int pools = std::min(c.n - first, dk::pages::kMaxPools);

@@ -26,6 +26,7 @@ constexpr int kPlanThreads = 1024;
 constexpr int kPlanCtas = 8;                 // one portable cluster
 constexpr int kPlanWarps = kPlanCtas * (kPlanThreads / 32);
 constexpr int kMoveThreads = 256;
+constexpr int kMaxLanesLog = 4;              // of them, token lanes: at most 16
 constexpr int kMaxPools = 128;               // pointers a launch takes
 
 enum : int {
@@ -387,7 +388,7 @@ struct MoveParams {
 // read here; it stores once that has said that all is well.
 template <typename V, int U, bool FORK>
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ MoveParams p) {
-  __shared__ int64_t s_from[kMoveThreads * U], s_to[kMoveThreads * U];
+  __shared__ int64_t s_from[U << kMaxLanesLog], s_to[U << kMaxLanesLog];
   if (FORK) {
     pdl_wait();
     if (threadIdx.x == 0) pdl_launch_dependents();
