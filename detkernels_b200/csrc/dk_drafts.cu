@@ -33,8 +33,8 @@ int logprobs_launch(dk::logprobs::Params p, cudaStream_t st) {
   if (rc) return rc;
   const int sms = sm_count(current_device());
   const int64_t ctas = std::min<int64_t>(p.split ? p.n_rows * p.parts : p.n_rows, static_cast<int64_t>(C::CTAS) * sms);
-  // A ring as deep as the CTAs of an SM leave room for: at four, two stages (of 2 and 3 no difference: 99 and 100 us for 4096
-  // rows of 50,001 bf16 logits; the other CTAs' passes are in flight too); one alone needs more to cover a copy's latency.
+  // A ring as deep as the CTAs of an SM leave room for: at four, three stages (of 2 and 3 no difference: 93 and 94 us for
+  // 4096 rows of 50,001 bf16 logits; the other CTAs' passes are in flight too); one alone needs more to cover a copy's latency.
   const int share = kShared / static_cast<int>(ceil_div(ctas, sms)) - C::STATIC - 1024 - (p.split ? C::STATES : 0);
   p.stages = std::max(2, std::min<int>(C::STAGES, share / C::STAGE));
   const int64_t resident = static_cast<int64_t>(C::CTAS) * sms;
@@ -186,9 +186,10 @@ int dk_token_logprobs(const void* logits, int64_t stride_row, int64_t n_rows, in
   const int64_t pass = dtype == DK_F32 ? dk::logprobs::Cfg<float, false>::PASS : dk::logprobs::Cfg<__half, false>::PASS;
   p.part = static_cast<int32_t>(ceil_div(ceil_div(n_vocab, pass), dk::logprobs::kMaxParts) * pass);
   p.parts = static_cast<int32_t>(ceil_div(n_vocab, p.part));
-  // Rows that leave SMs idle are split over the CTAs of a cluster (with 20 alternatives: 74 rows of 32,000 bf16
-  // logits 15 us either way, 290 rows 30 us split and 19 not; 74 of 185,668 38 and 52, 150 67 and 72, 290 119 and 70).
-  p.split = p.parts > 1 && n_rows <= sm_count(current_device());
+  // Rows that leave many SMs idle are split over the CTAs of a cluster.  With 20 alternatives, split and not: 8 rows of 32,000
+  // bf16 logits 8.0 and 13.8 us, 74 14.1 and 14.0, 148 16.4 and 14.9; of 185,668 74 rows 30 and 45, 148 51 and 46; of 50,001
+  // f32 74 rows 19 and 24, 148 28 and 25.
+  p.split = p.parts > 1 && 4 * n_rows <= 3 * sm_count(current_device());
   p.k = top_k;
   p.tokens = tokens;
   p.lp = logprobs;

@@ -6,18 +6,24 @@
 // them) keep their distances.  One pass over the row, bound by its bytes.
 //
 // A row is cut into passes of 16 KB, and the passes of long rows into eight parts, by the vocabulary's size alone.  In a
-// pass a thread takes four 16-byte vectors, 256 threads apart, against its own maximum; it joins its passes, then
-// its parts, in order, and the threads are joined last.  So few rows may give each part a CTA of its own (a cluster,
-// whose first CTA gathers the threads' states in its shared memory), and many rows a CTA each, which goes through all parts:
-// the same bits, with neither scratch nor a second launch.  Passes come into a ring in shared memory by bulk copies, which
-// keep more of them in flight than registers would, and at any alignment of a row: the copy takes the whole 16-byte words around
-// it, and a thread shifts its vectors into place.
-// The alternatives are chosen from the same stage.  A bound below the k-th largest logit of the first pass is had
-// from the threads' maxima: in each of w warps the ceil(k / w)-th largest is at most it, and so is the least of
-// these.  What lies above the bound (about twice k) is collected and ranked by counting; ties at the bound are taken
-// in the order of their indices.  From then on the k-th largest so far is the bound.  Where a bound is poor (logits
-// in order), the k-th largest of the pass's maxima is sought and takes its place; the pass then gives k alternatives by
-// itself, ties included.
+// pass a warp takes 2 KB side by side, a thread four 16-byte vectors of them, against its own maximum; it joins its passes,
+// then its parts, in order, and the lanes, then the warps, are joined last.  So few rows may give each part a CTA of its own
+// (a cluster, whose first CTA gathers the threads' states in its shared memory), and many rows a CTA each, which goes through
+// all parts: the same bits, with neither scratch nor a second launch.  Passes come into a ring in shared memory by bulk
+// copies, which keep more of them in flight than registers would, and at any alignment of a row: the copy takes the whole
+// 16-byte words around it, and a thread shifts its vectors into place.
+//
+// The alternatives are chosen from the same stage.  A bound below the k-th largest logit of the first pass is had from the
+// threads' maxima: in each of w warps the ceil(k / w)-th largest is at most it, and so is the least of these (of warps whose
+// threads all have their logits: a lane with fewer has a lower maximum, and 3 us were lost to a poor bound).  What reaches the
+// bound (about twice k) is collected and ranked by counting, equal ones by their indices.  From then on the k-th largest
+// so far is the bound, and only what lies above it is collected; a pass costs one barrier.  Where a bound is poor (logits in
+// order), the k-th largest of the pass's maxima is sought and takes its place; the pass then gives k alternatives by itself,
+// ties in the order of their indices.
+//
+// Measured, in a graph, logits out of L2: 4096 rows of 50,001 bf16 94 us (4.4 TB/s; the exponential unit is 56 % busy, the
+// issue slots 61 %: without exponentials 79 us, with a quarter of the sums 69); 1531 of 32,000 f32 with 5 alternatives
+// 55 us (3.6 TB/s, barriers), without any 38 (5.1); 8 of 32,000 bf16 with 20 alternatives 7.9 us (latency), without 3.8.
 #pragma once
 
 #include "dk_common.cuh"

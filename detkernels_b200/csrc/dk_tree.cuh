@@ -17,6 +17,13 @@
 // safe: 0 weights must meet neither what lies behind the sequence in its last page nor a non-finite value of a draft that
 // some rows do not see.  Those elements become 0 in shared memory, and rows that do see them have them added back from the
 // cache (which no ordinary call does).
+//
+// Measured, all kernels, in a graph: 64 requests of 8 to 32 drafts behind 200 to 4000 tokens, 32 heads of 128 on 8, bf16,
+// 131 us (4.4 TB/s of keys, values and queries; floor 89); 9 of 40 to 64 drafts behind 8000 to 20,000 tokens, 32 heads of
+// 128 on 4, f16, 168 us (750 TFLOP/s; floor 78 by its products); 4 of up to 6 behind up to 700, 8 heads of 64, 15 us.  Bound by a
+// block's chain from its scores to its weights (two tiles in turn: tensor pipe 47 % and exponential unit 45 % busy on the
+// long ones), the states of the chunks (out of the way in L2, then joined) and the last items.  In sustained runs the power
+// cap lowers the clocks: 148 and 196 us.
 #pragma once
 
 #include "dk_common.cuh"
@@ -180,9 +187,11 @@ __device__ __forceinline__ Cost cost_of(const Params& p, const Seq& s) {
 
 // The order of the items: by falling cost, in groups of a sequence's items of one cost (its whole chunks, its last ones),
 // dealt to the CTAs there and back.  So the CTAs' shares end within about the smallest items' cost of one another (64
-// requests, 148 CTAs: 239,000 cycles for the last CTA and 198,000 for the median one with runs of neighbouring items).  It
-// decides no bit.  Scratch, int32: [0] groups, [1] items, then by group its sequence (times 2, plus 1 for last chunks) and
-// its first item.
+// requests, 148 CTAs: 197,000 cycles for the last CTA and 185,000 on average; runs of neighbouring items had 239,000 for the
+// last and 198,000 for the median).  Items taken one by one as a CTA gets to them end no closer, and the walk through shared
+// memory that this needs made every warp slower (131 -> 146 us).  The order decides no bit.
+// One CTA, bound by its barriers and look-ups: 6.4 us alone for 64 requests (1024 threads: 8.4), of which about 2 are hidden.
+// Scratch, int32: [0] groups, [1] items, then by group its sequence (times 2, plus 1 for last chunks) and its first item.
 __host__ __device__ inline int64_t plan_ints(int64_t n_seqs) { return 4 + 4 * n_seqs; }
 
 constexpr int kPlanThreads = 256;
@@ -956,7 +965,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 }
 
 // out = O / l of a row's chunks, joined in order.  A CTA takes 32 state rows of a (sequence, KV head), a lane each; its
-// warps take column quads (one coalesced load a state), and the outputs leave through shared memory.
+// warps take column quads (one coalesced load a state), and the outputs leave through shared memory.  Bound by the states'
+// bytes and latency: alone, behind a flushed L2, 20 us for the 71 MB of the 64 requests (3.5 TB/s).
 constexpr int kJoinThreads = 256;
 
 template <typename T, int D>
