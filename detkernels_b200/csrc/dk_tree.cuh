@@ -12,9 +12,9 @@
 // and V, or, where the rows fit one tile, the tiles of two KV heads, each with its own K and V.  Either way both softmax
 // warpgroups have work, and take turns on the exponential unit.  One persistent CTA an SM takes items in an order that
 // plan_kernel has made of the lengths, the most expensive first, so that the CTAs end together; several pairs of tiles of a
-// KV head come side by side, and find a chunk's keys in L2.  A TMA warp, an MMA warp a tile (scores, weights and accumulator apart in TMEM), a
-// warpgroup a tile for the softmax, a row a thread, and a warp that fetches the queries and makes the values of draft blocks
-// safe: 0 weights must meet neither what lies behind the sequence in its last page nor a non-finite value of a draft that
+// KV head come side by side, and find a chunk's keys in L2.  A TMA warp, an MMA warp a tile (scores, weights and
+// accumulator apart in TMEM), a warpgroup a tile for the softmax, a row a thread, and a warp that fetches the queries and
+// makes the values of draft blocks safe: 0 weights must meet neither what lies behind the sequence in its last page nor a non-finite value of a draft that
 // some rows do not see.  Those elements become 0 in shared memory, and rows that do see them have them added back from the
 // cache (which no ordinary call does).
 //

@@ -480,8 +480,9 @@ int dk_tree_accept(const int32_t* parents, const int64_t* tokens, const int64_t*
                    int64_t* next_tokens, void* stream);
 
 /* The pools of the next two calls: n_pools device pointers (an array on the host) to tensors [n_blocks, n_heads, page_size,
- * head_dim] of elements of element_size bytes (1, 2, 4 or 8), all with the same element strides by block, head and token (positive,
- * where there is more than one) and unit stride along head_dim; no two of them overlap.  shares (device int32[n_blocks]): how many further sequences hold a block beyond the first.
+ * head_dim] of elements of element_size bytes (1, 2, 4 or 8), all with the same element strides by block, head and token
+ * (positive, where there is more than one) and unit stride along head_dim; no two of them overlap.  shares (device
+ * int32[n_blocks]): how many further sequences hold a block beyond the first.
  * The free list: free_blocks[0, *cursor) are handed out, as for dk_paged_plan; cursor_out may be cursor. */
 size_t dk_paged_fork_workspace_size(int32_t table_rows);   /* uninitialised memory will do */
 /* Row dst[i] of block_table [table_rows][blocks_per_seq] becomes a copy of row src[i], kv_lens[dst[i]] =

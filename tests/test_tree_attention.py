@@ -282,6 +282,33 @@ def test_many_items_a_cta(dev, D, Hkv, G):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D,long", [(128, 270000), (32, 9000)])
+def test_an_order_of_many_sequences(dev, D, long):
+    """More sequences than the order's threads, and a chunk that costs more than it tells apart."""
+    import torch
+
+    from detkernels_b200.kernels.attention import attention_tree
+    rng = np.random.default_rng(D)
+    B = 700
+    sizes = [int(x) for x in rng.choice([1, 4, 0, 70], size=B)]
+    kvs = [int(x) for x in rng.choice([0, 3, 64, 800, 1700], size=B)]
+    sizes[333], kvs[333] = 6, long
+    args, kw, own = _case(dev, torch.float16, sizes, kvs, 2, 1, D, 64, words=2, seed=D)
+    q, kc, vc, kv, cu, mask = args
+    want = attention_tree(*args, **kw)
+    assert torch.equal(attention_tree(*args, **kw), want)
+    ends = cu.tolist()
+    for b in list(range(0, B, 37)) + [333]:
+        r0, r1 = ends[b], ends[b + 1]
+        if r0 == r1:
+            continue
+        sub = (q[r0:r1], kc, vc, kv[b:b + 1], _i32([0, r1 - r0], dev), mask[r0:r1])
+        one = attention_tree(*sub, block_table=kw["block_table"][b:b + 1])
+        assert torch.equal(one, want[r0:r1]), b
+        _check(one, sub, own[b:b + 1], D ** -0.5, D)
+
+
+@pytest.mark.gpu
 def test_a_chain_is_decode_attention(dev):
     """Drafts that each see all before them are a causal continuation: the rows of attention_decode, up to rounding."""
     import torch
