@@ -17,7 +17,7 @@
 //
 // Measured, both kernels, in a graph: 28 forks of 7 prompts that share their pages, 16 heads of 64 in 8 pools, 14.6 us
 // (about 9 of them the first kernel); 24 copied whole, 1.2 GB, 199 us (6.1 TB/s); 256 accepted trees compacted, pages
-// shared, 17.8 us; 8 caches of up to 16,000 tokens halved, 1.5 GB, 286 us (5.3 TB/s: the CTAs of the longest cache end last).
+// shared, 17.8 us; 8 caches of up to 16,000 tokens halved, 1.5 GB, 276 us (5.5 TB/s, half of the 256-byte rows skipped).
 #pragma once
 
 #include "dk_common.cuh"
@@ -228,8 +228,8 @@ struct ReleaseParams {
   int32_t* ws;
 };
 
-// Entries of a row of `keep` that a warp checks at a time: a few long rows are shared by many warps.
-constexpr int kKeepRun = 512;
+// Entries of a row of `keep` that a warp checks at a time, all loaded at once: a few long rows are shared by many warps.
+constexpr int kKeepLoads = 8, kKeepRun = 32 * kKeepLoads;
 
 __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) release_kernel(const ReleaseParams p) {
   __shared__ Told told;
@@ -254,11 +254,16 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
       const int nw = p.nw[b], nk = p.n_keep[b];
       if (nk > nw || nk > p.keep_width) continue;   // refused below
       const int32_t* row = p.keep + b * p.keep_stride;
-      const int64_t j1 = j0 + kKeepRun < nk ? j0 + kKeepRun : nk;
+      int k[kKeepLoads];
+#pragma unroll
+      for (int i = 0; i < kKeepLoads; ++i) k[i] = j0 + 32 * i + lane < nk ? row[j0 + 32 * i + lane] : 0x7fffffff;
+      int last = lane == 31 && j0 > 0 && j0 < nk ? row[j0 - 1] : -1;   // lane 31: the entry before the next 32
       bool wrong = false;
-      for (int64_t j = j0 + lane; j < j1; j += 32) {
-        const int k = row[j];
-        wrong |= k < 0 || k >= nw || (j > 0 && row[j - 1] >= k);
+#pragma unroll
+      for (int i = 0; i < kKeepLoads; ++i) {
+        const int before = __shfl_sync(0xffffffffu, lane == 31 ? last : k[i], (lane + 31) & 31);
+        wrong |= j0 + 32 * i + lane < nk && (k[i] < 0 || k[i] >= nw || before >= k[i]);
+        last = k[i];
       }
       if (wrong) {
         report_error(DK_ERR_DEVICE_CHECK, kDetKeep);
@@ -390,8 +395,9 @@ struct MoveParams {
 // FORK: the destinations' rows are fork_kernel's, so nothing is read before it has ended.  A compaction reads its first
 // tokens while release_kernel still runs, which has itself waited for whatever wrote them, and changes none of what is
 // read here; it stores once that has said that all is well.
-// (Loads of the next step before the stores of this one: 279 us on the long caches, but 20 on the accepted trees; four CTAs
-// an SM instead of three, in 64 registers: 330 on the long ones.)
+// (Loads of the next step before the stores of this one: 279 against 286 us on the long caches, but 20 against 18 on the
+// accepted trees; four CTAs an SM instead of three, in 64 registers: 330 on the long ones; 32 token lanes instead of 16, or the
+// longest caches' CTAs first: 283 to 286.)
 template <typename V, int U, bool FORK>
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ MoveParams p) {
   __shared__ int64_t s_from[U << kMaxLanesLog], s_to[U << kMaxLanesLog];

@@ -338,6 +338,29 @@ def test_refused_compaction_changes_nothing(dev, what, shares):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("wrong", [None, 0, 1, 31, 32, 33, 255, 256, 257, 511, 512, 998])
+def test_long_rows_of_kept_tokens(dev, wrong):
+    """An entry that does not ascend is found wherever it stands, and only inside a row's n_keep."""
+    import torch
+
+    from detkernels_b200 import _lib
+    from detkernels_b200.kernels.paging import paged_compact
+    keep = np.sort(np.stack([np.random.default_rng(b).permutation(1500)[:1003] for b in range(3)]), axis=1)
+    n_keep = [1003, 999, 0]
+    keep[1, 999] = -5                      # behind the row's last
+    if wrong is not None:
+        keep[1, wrong] = keep[1, wrong - 1] if wrong else -1
+    table = _i32(np.arange(3 * 30).reshape(3, 30), dev)
+    got = paged_compact(table, _i32([5, 0, 9], dev), _i32([1500] * 3, dev), _i32(n_keep, dev), 64, keep=_i32(keep, dev),
+                        pools=[torch.zeros(90, 1, 64, 8, device=dev)])
+    code, det = _lib.device_status(dev.index)
+    if wrong is None:
+        assert code == _lib.DK_OK and got.lens.tolist() == [1008, 999, 9]
+    else:
+        assert (code, det) == (_lib.DK_ERR_DEVICE_CHECK, 0x645) and got.lens.tolist() == [5, 0, 9]
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 128, 300])
 @pytest.mark.parametrize("captured", [False, True])
 def test_a_life_of_pages(dev, n, captured):
