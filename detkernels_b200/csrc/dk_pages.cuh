@@ -30,7 +30,7 @@ constexpr int kPlanThreads = 1024;
 constexpr int kPlanCtas = 8;                 // one portable cluster
 constexpr int kPlanWarps = kPlanCtas * (kPlanThreads / 32);
 constexpr int kMoveThreads = 256;
-constexpr int kMaxLanesLog = 4;              // of them, token lanes: at most 16
+constexpr int kMaxLanesLog = 5;              // of them, token lanes: at most 32 (long caches: 16 279 us, 32 276)
 constexpr int kMaxPools = 128;               // pointers a launch takes
 
 enum : int {
@@ -383,6 +383,7 @@ struct MoveParams {
   const int32_t* keep;
   int64_t keep_stride;
   int32_t keep_width, width;   // width: entries of a table row
+  int32_t sorted;          // compact: so many sequences, the longest first; 0: any number in their order
   int32_t cols_log;        // log2 of the columns a CTA takes at once; the other threads are token lanes
   int32_t col_groups, splits;
   const int32_t* ws;
@@ -396,8 +397,7 @@ struct MoveParams {
 // tokens while release_kernel still runs, which has itself waited for whatever wrote them, and changes none of what is
 // read here; it stores once that has said that all is well.
 // (Loads of the next step before the stores of this one: 279 against 286 us on the long caches, but 20 against 18 on the
-// accepted trees; four CTAs an SM instead of three, in 64 registers: 330 on the long ones; 32 token lanes instead of 16, or the
-// longest caches' CTAs first: 283 to 286.)
+// accepted trees; four CTAs an SM instead of three, in 64 registers: 330 on the long ones.)
 template <typename V, int U, bool FORK>
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ MoveParams p) {
   __shared__ int64_t s_from[U << kMaxLanesLog], s_to[U << kMaxLanesLog];
@@ -407,7 +407,17 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
     if (__ldcg(p.ws + kWsOk) == 0) return;
   }
   const uint32_t group = blockIdx.x % p.col_groups, rest = blockIdx.x / p.col_groups;
-  const uint32_t split = rest % p.splits, i = rest / p.splits;
+  const uint32_t split = rest % p.splits;
+  uint32_t i = rest / p.splits;
+  if (!FORK && p.sorted > 0) {   // the sequence with that many longer ones, by a lane a sequence
+    const int lane = threadIdx.x & 31, mine = lane < p.sorted ? p.n_keep[lane] : 0;
+    int longer = 0;
+    for (int q = 0; q < p.sorted; ++q) {
+      const int other = __shfl_sync(0xffffffffu, mine, q);
+      longer += other > mine || (other == mine && q < lane);
+    }
+    i = __ffs(__ballot_sync(0xffffffffu, lane < p.sorted && longer == static_cast<int>(i))) - 1;
+  }
   const int cols = 1 << p.cols_log, lanes = kMoveThreads >> p.cols_log, step = lanes * U;
   const int32_t *row_from, *row_to, *keep = nullptr;
   int base, count;
