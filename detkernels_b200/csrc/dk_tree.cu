@@ -39,6 +39,7 @@ size_t state_bytes(int64_t chunks, int64_t st_rows, int64_t D) {
 // What the sizes alone decide of a call.
 struct Schedule {
   int64_t chunks, st_rows, units;
+  bool solo;             // an item a tile
   bool planned;          // more items, at most, than SMs: their order is planned
   size_t states, need;   // bytes of the states, and of the workspace: the states, then the items' order
 };
@@ -47,9 +48,14 @@ Schedule schedule(int64_t n_seqs, int64_t n_rows, int64_t max_rows, int64_t hq, 
   c.chunks = max_chunks(max_kv_len, max_rows);
   c.st_rows = n_rows * hq;
   const int64_t tiles = ceil_div(max_rows, dk::tree::kRows / (hq / hkv));
-  // items a (sequence, chunk): pairs of tiles, or pairs of heads where the rows fit one tile
-  c.units = tiles > 1 ? hkv * ceil_div(tiles, 2) : ceil_div(hkv, 2);
-  c.planned = c.units * n_seqs * c.chunks > sm_count(current_device());
+  // Items a (sequence, chunk): pairs of tiles, or pairs of heads where the rows fit one tile; and where single tiles are no
+  // more than the SMs, those, whose blocks take less time (4 requests of up to 700 tokens, 8 heads of 64: 12.3 and 14.9 us
+  // in a graph; 8 of up to 2776, 3 heads of 128: 17.2 and 21.9).  A few tokens leave nothing to gain by it, and on more than
+  // half of the SMs keep the next kernel from beginning beside them (22 requests of up to 18, 4 heads of 128: 8.5 and 6.6).
+  const int64_t single = hkv * tiles * n_seqs * c.chunks, sms = sm_count(current_device());
+  c.solo = single <= (max_kv_len > 256 ? sms : sms / 2);
+  c.units = c.solo ? hkv * tiles : tiles > 1 ? hkv * ceil_div(tiles, 2) : ceil_div(hkv, 2);
+  c.planned = c.units * n_seqs * c.chunks > sms;
   c.states = (state_bytes(c.chunks, c.st_rows, D) + 15) / 16 * 16;
   c.need = c.states + (c.planned ? static_cast<size_t>(dk::tree::plan_ints(n_seqs)) * sizeof(int32_t) : 0);
   return c;
@@ -170,6 +176,7 @@ int dk_attention_tree(const void* q, int64_t q_stride_row, int64_t q_stride_head
   p.words = mask_words;
   p.capacity = max_kv_len;
   p.units = static_cast<int32_t>(c.units);
+  p.solo = c.solo ? 1 : 0;
   p.max_chunks = static_cast<int32_t>(c.chunks);
   p.v = v;
   p.c_sn = kv_stride_seq;

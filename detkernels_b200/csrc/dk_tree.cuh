@@ -10,7 +10,7 @@
 //
 // Work: an item is (sequence, up to two tiles of at most 128 rows, chunk): two tiles of one KV head, which then share K
 // and V, or, where the rows fit one tile, the tiles of two KV heads, each with its own K and V.  Either way both softmax
-// warpgroups have work, and take turns on the exponential unit.  One persistent CTA an SM takes items in an order that
+// warpgroups have work, and take turns on the exponential unit (and where all single tiles find an SM, an item is one).  One persistent CTA an SM takes items in an order that
 // plan_kernel has made of the lengths, the most expensive first, so that the CTAs end together; several pairs of tiles of a
 // KV head come side by side, and find a chunk's keys in L2.  A TMA warp, an MMA warp a tile (scores, weights and
 // accumulator apart in TMEM), a warpgroup a tile for the softmax, a row a thread, and a warp that fetches the queries and
@@ -20,7 +20,7 @@
 //
 // Measured, all kernels, in a graph: 64 requests of 8 to 32 drafts behind 200 to 4000 tokens, 32 heads of 128 on 8, bf16,
 // 131 us (4.4 TB/s of keys, values and queries; floor 89); 9 of 40 to 64 drafts behind 8000 to 20,000 tokens, 32 heads of
-// 128 on 4, f16, 168 us (750 TFLOP/s; floor 78 by its products); 4 of up to 6 behind up to 700, 8 heads of 64, 15 us.  Bound by a
+// 128 on 4, f16, 168 us (750 TFLOP/s; floor 78 by its products); 4 of up to 6 behind up to 700, 8 heads of 64, 12 us.  Bound by a
 // block's chain from its scores to its weights (two tiles in turn: tensor pipe 47 % and exponential unit 45 % busy on the
 // long ones), the states of the chunks (out of the way in L2, then joined) and the last items.  In sustained runs the power
 // cap lowers the clocks: 148 and 196 us.
@@ -81,6 +81,7 @@ struct Params {
   int32_t words;
   int32_t capacity;         // tokens a sequence may have, drafts included
   int32_t units;            // items a (sequence, chunk), at most
+  int solo;                 // an item has one tile
   int32_t max_chunks;
   int32_t* plan;            // the items' order; null: CTA c takes item c of (chunk, sequence, unit)
   const void* v;            // for what is added back
@@ -162,7 +163,7 @@ __device__ __forceinline__ Seq seq_at(const Params& p, int b, bool report) {
 // The items of a sequence: units (KV heads, or pairs of them where the rows fit a tile), of each its chunks, of each the
 // pairs of tiles, which so find the chunk's keys in L2; and their cost, in blocks.
 struct Cost {
-  int units, pairs;      // pairs: of tiles a KV head; 0: pairs of heads
+  int units, pairs;      // pairs: of tiles a KV head (solo: its tiles); 0: pairs of heads (solo: heads)
   int inner;             // items a (unit, chunk)
   int chunk, last;       // cost of an item of a whole chunk, of the last one
   int64_t unit;          // of a unit
@@ -176,8 +177,8 @@ __device__ __forceinline__ Cost cost_of(const Params& p, const Seq& s) {
   constexpr int BLK = Cfg<D>::BLK;
   Cost c;
   const int nt = (s.rows + p.rpt - 1) / p.rpt;
-  c.pairs = nt > 1 ? (nt + 1) >> 1 : 0;
-  c.units = nt > 1 ? p.hkv : nt == 1 ? (p.hkv + 1) >> 1 : 0;
+  c.pairs = nt > 1 ? (p.solo ? nt : (nt + 1) >> 1) : 0;
+  c.units = nt > 1 || (nt == 1 && p.solo) ? p.hkv : nt == 1 ? (p.hkv + 1) >> 1 : 0;
   c.inner = nt > 1 ? c.pairs : 1;
   c.chunk = s.chunk / BLK + kItemCost<D>;
   c.last = (s.total - (s.n_chunks - 1) * s.chunk + BLK - 1) / BLK + kItemCost<D>;
@@ -359,15 +360,15 @@ struct Walk {
     const int nt = (s.rows + p.rpt - 1) / p.rpt;
     if (nt > 1) {
       kvh = u;
-      row0[0] = pair * 2 * p.rpt;
+      row0[0] = pair * (p.solo ? 1 : 2) * p.rpt;
       row0[1] = row0[0] + p.rpt;
-      tiles = row0[1] < s.rows ? 2 : 1;
+      tiles = !p.solo && row0[1] < s.rows ? 2 : 1;
       streams = 1;
-      last_reader = row0[1] + p.rpt >= s.rows;
+      last_reader = row0[0] + tiles * p.rpt >= s.rows;
     } else {
-      kvh = 2 * u;
+      kvh = p.solo ? u : 2 * u;
       row0[0] = row0[1] = 0;
-      tiles = streams = kvh + 1 < p.hkv ? 2 : 1;
+      tiles = streams = !p.solo && kvh + 1 < p.hkv ? 2 : 1;
       last_reader = true;
     }
     t_begin = chunk * s.chunk;
