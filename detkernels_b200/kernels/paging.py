@@ -1,14 +1,17 @@
-"""Page plan of a serving step, built on the GPU from the requests' lengths.
+"""Page plan of a serving step, built on the GPU from the requests' lengths; pages forked, compacted and freed.
 
 The device counterpart of ``tiny_model.BlockAllocator`` and of the host side of
 ``DecodeEngine.plan``: block-table growth from a free list, the slot of every
 new token in the paged cache, its sequence, position and attention length, and
 the attention kernels' row tiles, in one launch (small steps) or two, without a host round trip.
+``paged_fork`` and ``paged_compact`` keep the same table and free list for sequences that are copied,
+thinned out or ended.
 No counterpart in the reference (its cache is one tensor grown by
 ``torch.cat``, tiny_model.py:119-125).
 """
 from __future__ import annotations
 
+from array import array
 from typing import NamedTuple, Optional
 
 from detkernels_b200 import _lib
@@ -214,26 +217,24 @@ def paged_compact_reference(block_table, kv_lens, new_lens, n_keep, page_size, *
 
 
 def _check_pools(pools, dev, page_size, what):
-    """(pointer array, number, element strides by block, head and token, blocks, heads, head_dim, element size)."""
-    import ctypes
+    """(their addresses, number, element strides by block, head and token, blocks, heads, head_dim, element size)."""
     pools = list(pools)
     if not pools:
-        return None, 0, (0, 0, 0), 0, 0, 0, 1
+        return array("Q"), 0, (0, 0, 0), 0, 0, 0, 1
     first = pools[0]
     shape, stride, dtype = first.shape, first.stride(), first.dtype
-    index, at = dev.index, []
+    index = dev.index
     for t in pools:
         assert t.get_device() == index, "%s requires CUDA tensors on one device" % what
-        if t.shape != shape or t.stride() != stride or t.dtype != dtype:
+        if t.stride() != stride or t.shape != shape or t.dtype is not dtype:
             raise ValueError("%s: the pools must share shape, strides and dtype" % what)
-        at.append(t.data_ptr())
+    at = array("Q", [t.data_ptr() for t in pools])
     assert len(shape) == 4 and shape[2] == page_size, "%s: pools must be [n_blocks, heads, page_size, head_dim]" % what
     if shape[3] > 1 and stride[3] != 1:
         raise ValueError("%s: unit stride along head_dim required" % what)
     if len(set(at)) != len(at):
         raise ValueError("%s: a pool is named twice" % what)
-    ptrs = (ctypes.c_void_p * len(pools))(*at)
-    return ptrs, len(pools), stride[:3], shape[0], shape[1], shape[3], first.element_size()
+    return at, len(pools), stride[:3], shape[0], shape[1], shape[3], first.element_size()
 
 
 def _check_books(block_table, kv_lens, page_size, free_blocks, cursor, shares, n_blocks, what):
@@ -271,8 +272,8 @@ def paged_fork(block_table, kv_lens, src, dst, page_size: int, *, free_blocks, c
     shared (shares[block] += 1), and only the last, open page gets a block of its own; without it every page does.  New
     blocks are the next of free_blocks from cursor on (as for ``paged_plan``), in the order of the forks; returns the
     new cursor (int32 CUDA [1]).
-    pools: the K and V pools of all layers ([n_blocks, heads, page_size, head_dim], any dtype, same strides), in which
-    the tokens of the new blocks are copied; what lies behind a sequence's last token is left as it was.
+    pools: the K and V pools of all layers ([n_blocks, heads, page_size, head_dim], any dtype, same strides, none over
+    another), in which the tokens of the new blocks are copied; what lies behind a sequence's last token is left as it was.
 
     Rows outside the table or misnamed, a length outside its row, a block id outside the pools or too few free blocks set
     the device status (``_lib.raise_on_device_error``), and nothing changes."""
@@ -280,7 +281,7 @@ def paged_fork(block_table, kv_lens, src, dst, page_size: int, *, free_blocks, c
 
     what = "paged_fork"
     dev = block_table.device
-    ptrs, n_pools, st, n_blocks, heads, dim, size = _check_pools(pools, dev, page_size, what)
+    at, n_pools, st, n_blocks, heads, dim, size = _check_pools(pools, dev, page_size, what)
     if free_blocks is None or cursor is None:
         raise ValueError("paged_fork: free_blocks and cursor are needed")
     stride, n_blocks = _check_books(block_table, kv_lens, page_size, free_blocks, cursor, shares, n_blocks, what)
@@ -301,8 +302,8 @@ def paged_fork(block_table, kv_lens, src, dst, page_size: int, *, free_blocks, c
         rc = lib.dk_paged_fork(
             block_table.data_ptr(), stride, block_table.shape[0], block_table.shape[1], kv_lens.data_ptr(), src.data_ptr(),
             dst.data_ptr(), src.numel(), int(page_size), free_blocks.data_ptr() or ws.data_ptr(), free_blocks.numel(),
-            cursor.data_ptr(), out.data_ptr(), None if shares is None else shares.data_ptr(), n_blocks, ptrs, n_pools,
-            *st, heads, dim, size, ws.data_ptr(), 4 * ws.numel(), _lib.stream_ptr(dev))
+            cursor.data_ptr(), out.data_ptr(), None if shares is None else shares.data_ptr(), n_blocks, at.buffer_info()[0],
+            n_pools, *st, heads, dim, size, ws.data_ptr(), 4 * ws.numel(), _lib.stream_ptr(dev))
     _lib.check(rc, what)
     _lib.count_launch(2 if n_pools else 1)
     return out
@@ -330,7 +331,7 @@ def paged_compact(block_table, kv_lens, new_lens, n_keep, page_size: int, *, kee
 
     what = "paged_compact"
     dev = block_table.device
-    ptrs, n_pools, st, n_blocks, heads, dim, size = _check_pools(pools, dev, page_size, what)
+    at, n_pools, st, n_blocks, heads, dim, size = _check_pools(pools, dev, page_size, what)
     stride, n_blocks = _check_books(block_table, kv_lens, page_size, free_blocks, cursor, shares, n_blocks, what)
     if shares is not None and free_blocks is None:
         raise ValueError("paged_compact: shares need a free list")
@@ -361,8 +362,8 @@ def paged_compact(block_table, kv_lens, new_lens, n_keep, page_size: int, *, kee
             block_table.data_ptr(), stride, block_table.shape[1], kv_lens.data_ptr(), new_lens.data_ptr(),
             n_keep.data_ptr(), ptr(keep), 0 if keep is None else keep.stride(0), 0 if keep is None else keep.shape[1], B,
             int(page_size), lens.data_ptr(), ptr(free_blocks), 0 if free_blocks is None else free_blocks.numel(),
-            ptr(cursor), ptr(out), ptr(shares), n_blocks, ptrs, n_pools, *st, heads, dim, size, ws.data_ptr(),
-            4 * ws.numel(), _lib.stream_ptr(dev))
+            ptr(cursor), ptr(out), ptr(shares), n_blocks, at.buffer_info()[0], n_pools, *st, heads, dim, size,
+            ws.data_ptr(), 4 * ws.numel(), _lib.stream_ptr(dev))
     _lib.check(rc, what)
     _lib.count_launch(2 if n_pools and keep is not None else 1)
     return PagedCompact(lens, out)
