@@ -286,7 +286,7 @@ _no_guard = contextlib.nullcontext()
 def on_device(device):
     """``torch.cuda.device(device)`` for a tensor's device, which costs nothing when it is the current one."""
     import torch
-    return _no_guard if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _no_guard if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 _workspaces = {}
