@@ -409,7 +409,7 @@ def attention_tree(q, k_cache, v_cache, kv_lens, cu_rows, tree_mask, *, block_ta
     ``dk_attention_tree_workspace_size`` bytes (a new one if not given; its contents do not matter, and calls that may
     overlap need separate ones).
 
-    Rows behind the last sequence keep what ``out`` holds.  Offsets that do not ascend inside the rows, more than max_rows
+    Rows behind the last sequence keep what ``out`` (which may be q) holds.  Offsets that do not ascend inside the rows, more than max_rows
     rows a sequence, a negative length or more than max_kv_len tokens set the device status; that sequence's rows keep what
     ``out`` holds too.  A row's bits depend on its q and the tokens that it sees, and nothing else of the batch."""
     import torch

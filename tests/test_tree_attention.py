@@ -381,6 +381,41 @@ def test_padded_rows_and_out(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("page", [0, 64])
+@pytest.mark.parametrize("D,kvs", [(64, [100, 0, 200]), (128, [900, 2000, 5]), (32, [70, 1600, 300])])
+def test_layouts(dev, D, kvs, page):
+    """Queries inside a fused projection, caches by tokens, outputs inside a wider tensor, aligned and not, masks inside one."""
+    import torch
+
+    from detkernels_b200.kernels.attention import attention_tree
+    H, Hkv = 6, 2
+    args, kw, own = _case(dev, torch.float16, [5, 40, 2], kvs, H, Hkv, D, page, fill=0.5)
+    q, kc, vc, kv, cu, mask = args
+    want = attention_tree(*args, **kw)
+    R = q.shape[0]
+    for pad, off in ((2 * Hkv * D, 0), (24, 8), (5, 1)):
+        wide = torch.full((R, H * D + pad), 9.0, device=dev, dtype=q.dtype)
+        q2 = wide[:, off:off + H * D].view(R, H, D)
+        q2.copy_(q)
+        out_wide = torch.full((R, H * D + pad), 3.0, device=dev, dtype=q.dtype)
+        out = out_wide[:, off:off + H * D].view(R, H, D)
+        assert attention_tree(q2, kc, vc, kv, cu, mask, out=out, **kw) is out
+        assert torch.equal(out, want)
+        assert bool((out_wide[:, :off] == 3).all()) and bool((out_wide[:, off + H * D:] == 3).all())
+    k2, v2 = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in (kc, vc))
+    assert torch.equal(attention_tree(q, k2, v2, kv, cu, mask, **kw), want)
+    both = torch.stack([kc, vc], dim=2)     # K and V of a head side by side
+    assert torch.equal(attention_tree(q, both[:, :, 0], both[:, :, 1], kv, cu, mask, **kw), want)
+    m2 = torch.full((R, 3), -1, device=dev, dtype=torch.int64)
+    m2[:, 1:2] = mask
+    assert torch.equal(attention_tree(q, kc, vc, kv, cu, m2[:, 1:2], **kw), want)
+    if page:
+        t2 = torch.full((3, kw["block_table"].shape[1] + 5), -1, device=dev, dtype=torch.int32)
+        t2[:, 2:-3] = kw["block_table"]
+        assert torch.equal(attention_tree(q, kc, vc, kv, cu, mask, block_table=t2[:, 2:-3]), want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kvs", [[100, 0, 200], [900, 2000, 5]])
 def test_broadcast_inputs(dev, kvs):
     """Queries, caches and masks that take one place in memory for several rows, heads or sequences; out in q's place."""
