@@ -118,7 +118,7 @@ struct Cfg {
 
 // Tokens a chunk: a function of the cached tokens alone.  Short chunks give a small batch enough items to fill the SMs, but
 // each costs a row a state of D floats out and in again, about three blocks' time a tile.  Measured in chunks of 512, 768
-// and 1024: 64 requests of 200 to 4000 tokens 145, 131 and 125 us, 8 of one to two rows and up to 2776 tokens 18, 21 and 25;
+// and 1024: 64 requests of 200 to 4000 tokens 145, 131 and 126 us, 8 of one to two rows and up to 2776 tokens 17, 18 and 21;
 // of 1024, 1536 and 2048: 9 requests of 8000 to 20,000 tokens 191, 164 and 162 us, one of 6000 28, 37 and 45.
 __host__ __device__ inline int64_t chunk_tokens(int64_t kv) {
   if (kv <= 4096) return 768;
