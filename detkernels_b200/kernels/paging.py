@@ -256,7 +256,7 @@ def _check_books(block_table, kv_lens, page_size, free_blocks, cursor, shares, n
         assert free_blocks.dim() == 1 and cursor.dtype == i32 and cursor.get_device() == dev.index and cursor.numel() == 1
     if shares is not None:
         assert shares.dtype == i32 and shares.get_device() == dev.index and shares.is_contiguous() and shares.dim() == 1
-        if n_blocks and shares.numel() < n_blocks:
+        if shares.numel() < max(n_blocks, 1):   # (no entries bound no id: they would be looked up all the same)
             raise ValueError("%s: shares must have an entry a block" % what)
         n_blocks = n_blocks or shares.numel()
     return block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1], n_blocks or 2 ** 31 - 1

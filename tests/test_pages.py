@@ -444,3 +444,21 @@ def test_wrappers_refuse_on_the_gpu(dev):
     e = _i32([], dev)
     assert paged_compact(t, e, e, e, 8).lens.shape == (0,)
     assert paged_fork(t, i, e, e, 8, free_blocks=i, cursor=c).tolist() == [0]
+
+
+def test_shares_without_entries_are_refused():
+    """They would bound no block id, with pools or without.  (Tensors without memory, so that it runs anywhere.)"""
+    import torch
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from detkernels_b200.kernels.paging import paged_compact, paged_fork
+    with FakeTensorMode():
+        dev = torch.device("cuda", 0)
+        t, i, c = (torch.zeros(*s, dtype=torch.int32, device=dev) for s in ((2, 2), (2,), (1,)))
+        none = torch.zeros(0, dtype=torch.int32, device=dev)
+        with pytest.raises(ValueError, match="an entry a block"):
+            paged_fork(t, i, i, i, 8, free_blocks=i, cursor=c, shares=none)
+        with pytest.raises(ValueError, match="an entry a block"):
+            paged_compact(t, i, i, i, 8, free_blocks=i, cursor=c, shares=none)
+        with pytest.raises(ValueError, match="an entry a block"):
+            paged_compact(t, i, i, i, 8, keep=t, free_blocks=i, cursor=c, shares=none)
