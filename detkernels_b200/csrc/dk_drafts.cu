@@ -320,6 +320,7 @@ int dk_paged_compact(const int32_t* block_table, int64_t block_table_stride, int
   p.keep = keep;
   p.keep_stride = keep_stride;
   p.keep_width = keep_width;
+  p.moves = keep && n_pools > 0;
   p.n = n_seqs;
   p.page = dk::divisor(page_size);
   p.lens_out = lens_out;

@@ -216,6 +216,7 @@ struct ReleaseParams {
   const int32_t* keep;     // which, ascending; null: the first n_keep
   int64_t keep_stride;
   int32_t keep_width;
+  int moves;               // move_kernel follows: the blocks of the tokens that it moves are checked here
   int32_t n;
   Divisor page;
   int32_t* lens_out;
@@ -229,6 +230,8 @@ struct ReleaseParams {
 };
 
 // Entries of a row of `keep` that a warp checks at a time, all loaded at once: a few long rows are shared by many warps.
+// A token that moves has the blocks that it comes from and goes to looked up as well: nothing may be found wrong once
+// lengths, holders and the free list have changed.
 constexpr int kKeepLoads = 8, kKeepRun = 32 * kKeepLoads;
 
 __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) release_kernel(const ReleaseParams p) {
@@ -246,35 +249,46 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
   int64_t given = 0;   // pages of this warp's sequences that come back
   auto first_page = [&](int b) { return static_cast<int>(ceil_div32(p.kv[b] + p.n_keep[b], p.page)); };
   auto last_page = [&](int b) { return static_cast<int>(ceil_div32(p.kv[b] + p.nw[b], p.page)); };
+  auto bad_lens = [&](int64_t kv, int64_t nw, int64_t nk) {
+    return kv < 0 || nw < 0 || nk < 0 || nk > nw || kv + nw > 0x7fffffff || (p.keep && nk > p.keep_width) ||
+           ceil_div32(static_cast<uint32_t>(kv + nw), p.page) > static_cast<uint32_t>(p.width);
+  };
+  auto there = [&](int b, int tok) {   // the block of a token of the sequence is of the pool
+    const int x = p.table[b * p.table_stride + div_by(static_cast<uint32_t>(tok), p.page)];
+    return x >= 0 && x < p.n_blocks;
+  };
   if (p.keep) {
     const int runs = (p.keep_width + kKeepRun - 1) / kKeepRun;
     for (int64_t e = w; e < static_cast<int64_t>(p.n) * runs; e += kPlanWarps) {
       const int b = static_cast<int>(e / runs);
       const int64_t j0 = (e - static_cast<int64_t>(b) * runs) * kKeepRun;
-      const int nw = p.nw[b], nk = p.n_keep[b];
-      if (nk > nw || nk > p.keep_width) continue;   // refused below
+      const int kv = p.kv[b], nw = p.nw[b], nk = p.n_keep[b];
+      if (bad_lens(kv, nw, nk)) continue;   // refused below
       const int32_t* row = p.keep + b * p.keep_stride;
       int k[kKeepLoads];
 #pragma unroll
       for (int i = 0; i < kKeepLoads; ++i) k[i] = j0 + 32 * i + lane < nk ? row[j0 + 32 * i + lane] : 0x7fffffff;
       int last = lane == 31 && j0 > 0 && j0 < nk ? row[j0 - 1] : -1;   // lane 31: the entry before the next 32
-      bool wrong = false;
+      bool wrong = false, lost = false;
 #pragma unroll
       for (int i = 0; i < kKeepLoads; ++i) {
         const int before = __shfl_sync(0xffffffffu, lane == 31 ? last : k[i], (lane + 31) & 31);
-        wrong |= j0 + 32 * i + lane < nk && (k[i] < 0 || k[i] >= nw || before >= k[i]);
+        const int64_t j = j0 + 32 * i + lane;
+        if (j < nk) {
+          const bool in = k[i] >= 0 && k[i] < nw;
+          wrong |= !in || before >= k[i];
+          if (p.moves && in && k[i] != j) lost |= !there(b, kv + k[i]) || !there(b, kv + static_cast<int>(j));
+        }
         last = k[i];
       }
-      if (wrong) {
-        report_error(DK_ERR_DEVICE_CHECK, kDetKeep);
+      if (wrong || lost) {
+        report_error(DK_ERR_DEVICE_CHECK, wrong ? kDetKeep : kDetBlock);
         bad = true;
       }
     }
   }
   for (int b = b0; b < b1; ++b) {
-    const int64_t kv = p.kv[b], nw = p.nw[b], nk = p.n_keep[b];
-    if (kv < 0 || nw < 0 || nk < 0 || nk > nw || kv + nw > 0x7fffffff || (p.keep && nk > p.keep_width) ||
-        ceil_div32(static_cast<uint32_t>(kv + nw), p.page) > static_cast<uint32_t>(p.width)) {
+    if (bad_lens(p.kv[b], p.nw[b], p.n_keep[b])) {
       if (lane == 0) report_error(DK_ERR_DEVICE_CHECK, kDetLens);
       bad = true;
       continue;
@@ -432,7 +446,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
     base = p.kv[i];
     count = p.n_keep[i];
     keep = p.keep + i * p.keep_stride;
-    // (what release_kernel refuses is not looked up out of bounds either)
+    // (what release_kernel refuses is not looked up out of bounds either, here and below)
     if (base < 0 || count < 0 || count > p.keep_width) base = count = 0;
   }
   // this CTA's share of the tokens, in whole steps (a compaction has one share)
@@ -445,7 +459,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
     const int v = col % p.vecs, hp = col / p.vecs, h = hp % p.heads, pool = hp / p.heads;
     at = static_cast<V*>(p.pool[pool]) + h * p.s_head + v;
   }
-  bool waited = FORK, lost = false;   // lost: a block that does not exist
+  bool waited = FORK;
   for (int64_t t0 = begin; t0 < end; t0 += step) {
     for (int e = threadIdx.x; e < step; e += kMoveThreads) {
       const int64_t j = t0 + e;
@@ -460,8 +474,6 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
           if (bf >= 0 && bf < p.n_blocks && bt >= 0 && bt < p.n_blocks) {
             from = bf * p.s_block + (tf - static_cast<int64_t>(pf) * p.page.d) * p.s_tok;
             to = bt * p.s_block + (tt - static_cast<int64_t>(pt) * p.page.d) * p.s_tok;
-          } else {
-            lost = true;
           }
         }
       }
@@ -483,7 +495,6 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
       if (__ldcg(p.ws + kWsOk) == 0) return;
       waited = true;
     }
-    if (lost) report_error(DK_ERR_DEVICE_CHECK, kDetBlock);
     __syncthreads();   // all of the step's tokens are read
     if (at) {
 #pragma unroll

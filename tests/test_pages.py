@@ -462,3 +462,76 @@ def test_shares_without_entries_are_refused():
             paged_compact(t, i, i, i, 8, free_blocks=i, cursor=c, shares=none)
         with pytest.raises(ValueError, match="an entry a block"):
             paged_compact(t, i, i, i, 8, keep=t, free_blocks=i, cursor=c, shares=none)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("row,col", [(1, 1), (1, 2), (0, 0), (2, 2)])
+@pytest.mark.parametrize("bad", [-1, 12, 2 ** 31 - 1])
+@pytest.mark.parametrize("listed,shares", [(True, True), (True, False), (False, False)])
+def test_a_bad_block_under_kept_tokens_changes_nothing(dev, row, col, bad, listed, shares):
+    """Where moved tokens come from or go to, whether pages come back or not."""
+    import torch
+
+    from detkernels_b200 import _lib
+    from detkernels_b200.kernels.paging import paged_compact
+    page = 4
+    table = np.array([[3, 4, 5], [6, 7, 8], [9, 10, 11]])
+    table[row, col] = bad
+    kv, new, nk, keep = [2, 5, 0], [6, 6, 9], [2, 3, 2], [[1, 3, 0], [0, 4, 5], [2, 8, 0]]
+    pools = _pools(dev, 12, 2, page, 8, "float16", 2)
+    want = [p.clone() for p in pools]
+    free, cursor, s = _i32(np.arange(9), dev), _i32([9], dev), _i32(np.zeros(12), dev)
+    got = paged_compact(_i32(table, dev), _i32(kv, dev), _i32(new, dev), _i32(nk, dev), page, keep=_i32(keep, dev), pools=pools,
+                        free_blocks=free if listed else None, cursor=cursor if listed else None, shares=s if shares else None)
+    code, det = _lib.device_status(dev.index)
+    assert (code, det) == (_lib.DK_ERR_DEVICE_CHECK, 0x642), (code, hex(det))
+    assert got.lens.tolist() == kv and free.tolist() == list(range(9)) and not s.any()
+    assert got.cursor.tolist() == [9] if listed else got.cursor is None
+    for a, b in zip(pools, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_blocks_that_no_kept_token_needs_are_not_asked_for(dev):
+    """Without a free list: a page between kept tokens, the tokens that stay where they are, and a call that moves nothing."""
+    import torch
+
+    from detkernels_b200 import _lib
+    from detkernels_b200.kernels.paging import paged_compact
+    page = 4
+    table = np.array([[3, 4, 5], [-1, 7, 8], [9, -1, 11]])
+    kv, new, nk, keep = [2, 0, 0], [6, 10, 9], [2, 6, 2], [[1, 3, 0, 0, 0, 0], [0, 1, 2, 3, 5, 8], [2, 8, 0, 0, 0, 0]]
+    pools = _pools(dev, 12, 2, page, 8, "float16", 2)
+    want = [p.clone() for p in pools]
+    for p in want:
+        p[3, :, 2:] = torch.stack([p[3, :, 3], p[4, :, 1]], 1)
+        p[7, :, :2] = torch.stack([p[7, :, 1], p[8, :, 0]], 1)
+        p[9, :, :2] = torch.stack([p[9, :, 2], p[11, :, 0]], 1)
+    args = _i32(table, dev), _i32(kv, dev), _i32(new, dev), _i32(nk, dev), page
+    got = paged_compact(*args, keep=_i32(keep, dev), pools=pools)
+    assert _lib.device_status(dev.index)[0] == _lib.DK_OK and got.lens.tolist() == [4, 6, 2]
+    for a, b in zip(pools, want):
+        assert torch.equal(a, b)
+    assert paged_compact(_i32(table * 0 - 1, dev), *args[1:], keep=_i32(keep, dev)).lens.tolist() == [4, 6, 2]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("at", [0, 31, 250, 997])
+def test_a_bad_block_far_into_a_long_row(dev, at):
+    """Long rows are checked by many warps: entry `at` of 999 is the only one that needs the block."""
+    import torch
+
+    from detkernels_b200 import _lib
+    from detkernels_b200.kernels.paging import paged_compact
+    keep = np.arange(999) + 1
+    table = np.arange(2 * 1002).reshape(2, 1002)
+    table[1, 3 + at + 1] = -9           # pages of one token: entry at's source, entry at + 1's destination
+    pool = torch.randn(2004, 1, 1, 8, device=dev)
+    want = pool.clone()
+    free = _i32(np.arange(2004), dev)
+    got = paged_compact(_i32(table, dev), _i32([2, 3], dev), _i32([999, 999], dev), _i32([0, 998], dev), 1,
+                        keep=_i32(np.stack([keep, keep]), dev), pools=[pool], free_blocks=free, cursor=_i32([2003], dev))
+    code, det = _lib.device_status(dev.index)
+    assert (code, det) == (_lib.DK_ERR_DEVICE_CHECK, 0x642)
+    assert got.lens.tolist() == [2, 3] and got.cursor.tolist() == [2003] and free.tolist() == list(range(2004))
+    assert torch.equal(pool, want)
