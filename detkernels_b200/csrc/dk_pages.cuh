@@ -41,6 +41,7 @@ enum : int {
   kDetLens = 0x644,       // a negative length, more kept than held, or a sequence past its table row
   kDetKeep = 0x645,       // kept tokens that do not ascend inside the sequence
   kDetShares = 0x646,     // a page with fewer holders than give it back
+  kDetShared = 0x647,     // a token to move into a page that another sequence holds, too
 };
 
 // Scratch, int32: [0] the plan stands, then two marks a table row (fork).
@@ -231,7 +232,9 @@ struct ReleaseParams {
 
 // Entries of a row of `keep` that a warp checks at a time, all loaded at once: a few long rows are shared by many warps.
 // A token that moves has the blocks that it comes from and goes to looked up as well: nothing may be found wrong once
-// lengths, holders and the free list have changed.
+// lengths, holders and the free list have changed.  No token may go to a block with further holders, who would find it
+// among theirs; so none that is read is another sequence's to write, either.  (A holder that gives the block up in the
+// same call counts: it may read its own kept tokens there.)
 constexpr int kKeepLoads = 8, kKeepRun = 32 * kKeepLoads;
 
 __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) release_kernel(const ReleaseParams p) {
@@ -253,10 +256,8 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     return kv < 0 || nw < 0 || nk < 0 || nk > nw || kv + nw > 0x7fffffff || (p.keep && nk > p.keep_width) ||
            ceil_div32(static_cast<uint32_t>(kv + nw), p.page) > static_cast<uint32_t>(p.width);
   };
-  auto there = [&](int b, int tok) {   // the block of a token of the sequence is of the pool
-    const int x = p.table[b * p.table_stride + div_by(static_cast<uint32_t>(tok), p.page)];
-    return x >= 0 && x < p.n_blocks;
-  };
+  auto block_at = [&](int b, int tok) { return p.table[b * p.table_stride + div_by(static_cast<uint32_t>(tok), p.page)]; };
+  auto there = [&](int x) { return x >= 0 && x < p.n_blocks; };
   if (p.keep) {
     const int runs = (p.keep_width + kKeepRun - 1) / kKeepRun;
     for (int64_t e = w; e < static_cast<int64_t>(p.n) * runs; e += kPlanWarps) {
@@ -269,7 +270,7 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
 #pragma unroll
       for (int i = 0; i < kKeepLoads; ++i) k[i] = j0 + 32 * i + lane < nk ? row[j0 + 32 * i + lane] : 0x7fffffff;
       int last = lane == 31 && j0 > 0 && j0 < nk ? row[j0 - 1] : -1;   // lane 31: the entry before the next 32
-      bool wrong = false, lost = false;
+      bool wrong = false, lost = false, shared = false;
 #pragma unroll
       for (int i = 0; i < kKeepLoads; ++i) {
         const int before = __shfl_sync(0xffffffffu, lane == 31 ? last : k[i], (lane + 31) & 31);
@@ -277,12 +278,16 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
         if (j < nk) {
           const bool in = k[i] >= 0 && k[i] < nw;
           wrong |= !in || before >= k[i];
-          if (p.moves && in && k[i] != j) lost |= !there(b, kv + k[i]) || !there(b, kv + static_cast<int>(j));
+          if (p.moves && in && k[i] != j) {
+            const int to = block_at(b, kv + static_cast<int>(j));
+            lost |= !there(block_at(b, kv + k[i])) || !there(to);
+            shared |= p.shares && there(to) && p.shares[to] > 0;
+          }
         }
         last = k[i];
       }
-      if (wrong || lost) {
-        report_error(DK_ERR_DEVICE_CHECK, wrong ? kDetKeep : kDetBlock);
+      if (wrong || lost || shared) {
+        report_error(DK_ERR_DEVICE_CHECK, wrong ? kDetKeep : lost ? kDetBlock : kDetShared);
         bad = true;
       }
     }

@@ -321,12 +321,15 @@ def paged_compact(block_table, kv_lens, new_lens, n_keep, page_size: int, *, kee
     free_blocks (updated in place) and cursor: the pages behind a sequence's tokens go back before the cursor, in the order
     of sequences and pages, and the new cursor, from which ``paged_plan`` and ``paged_fork`` take them again, is returned.
     With shares (as in ``paged_fork``) a page with further holders loses one instead, and one given up by all its holders
-    goes back once; without, a page must be one sequence's alone.  Table entries stay as they are.  Tokens must not be moved
-    inside a page that another sequence shares; ``paged_fork`` leaves each sequence its open page to itself.
+    goes back once; without, a page must be one sequence's alone.  Table entries stay as they are.  Tokens are not moved
+    into a page that another sequence shares (free that one first, in a call before); ``paged_fork`` leaves each sequence its
+    open page to itself.  A sequence that a call leaves ending inside a shared page must not take new tokens there: its fork
+    may, which has a copy of that page.
 
     A negative length, more kept than held, a sequence beyond its table row, a ``keep`` that does not ascend inside the
-    new tokens, a block id outside the pools, more pages than were handed out or a page given up by more sequences than
-    hold it set the device status; then lens are kv_lens, the cursor stays, and nothing changes."""
+    new tokens, a block id outside the pools, more pages than were handed out, a page given up by more sequences than hold
+    it or a token to move into a shared page set the device status; then lens are kv_lens, the cursor stays, and nothing
+    changes."""
     import torch
 
     what = "paged_compact"

@@ -507,10 +507,13 @@ size_t dk_paged_compact_workspace_size(void);              /* uninitialised memo
  * other goes back, free_blocks[*cursor_out, *cursor) in the order of (sequence, page), a page given up by all its
  * holders in this call at the last of them.  Without shares a page is one sequence's alone; with them n_seqs *
  * blocks_per_seq must be below 2^30.  Table entries stay.  kv_lens = 0 and n_keep = 0 free a whole sequence.
- * Tokens must not be moved inside a page that another sequence shares: the pages from kv_lens[b] / page_size on are the
- * sequence's own, as dk_paged_fork leaves them.  Recorded as DK_ERR_DEVICE_CHECK: bad lengths (detail 0x644), a bad row of
- * keep (0x645), a block id outside [0, n_blocks) (0x642), more pages than were handed out (0x643), a page given up
- * by more sequences than hold it (0x646); then lens_out = kv_lens, *cursor_out = *cursor, and nothing else changes. */
+ * Tokens are not moved into a page that another sequence shares, were it to give the page up in the same call: from the
+ * first token that moves on, the pages are the sequence's own, as dk_paged_fork leaves the open one.  A sequence that then
+ * ends inside a shared page must not take new tokens there: dk_paged_fork gives its copy a page of its own.  Recorded as
+ * DK_ERR_DEVICE_CHECK: bad lengths (detail 0x644), a bad row of keep (0x645), a block id outside [0, n_blocks) among those
+ * that moved tokens or given-up pages name (0x642), more pages than were handed out (0x643), a page given up by more
+ * sequences than hold it (0x646), a token to move into a page that has shares (0x647); then lens_out = kv_lens, *cursor_out =
+ * *cursor, and nothing else changes. */
 int dk_paged_compact(const int32_t* block_table, int64_t block_table_stride, int32_t blocks_per_seq,
                      const int32_t* kv_lens, const int32_t* new_lens, const int32_t* n_keep, const int32_t* keep,
                      int64_t keep_stride, int32_t keep_width, int32_t n_seqs, int32_t page_size, int32_t* lens_out,

@@ -535,3 +535,67 @@ def test_a_bad_block_far_into_a_long_row(dev, at):
     assert (code, det) == (_lib.DK_ERR_DEVICE_CHECK, 0x642)
     assert got.lens.tolist() == [2, 3] and got.cursor.tolist() == [2003] and free.tolist() == list(range(2004))
     assert torch.equal(pool, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["thinned", "both", "given_up", "last_page"])
+def test_tokens_are_not_moved_into_a_shared_page(dev, what):
+    """Two sequences share the blocks 0 and 1 of four tokens: thinning one out would change the other's."""
+    import torch
+
+    from detkernels_b200 import _lib
+    from detkernels_b200.kernels.paging import paged_compact
+    page = 4
+    table, shares = np.array([[0, 1, 2], [0, 1, 3]]), [1, 1, 0, 0, 0]
+    kv, new, nk = [0, 0], [11, 10], [11, 5]
+    keep = [list(range(11)), [0, 2, 3, 5, 9] + [0] * 6]
+    if what == "both":              # in the same way: their moves would meet
+        nk[0], keep[0] = 5, keep[1]
+    elif what == "given_up":        # by the other one in the same call
+        nk[0] = 0
+    elif what == "last_page":       # only the last kept token's page is shared still
+        shares, nk[1], keep[1] = [0, 1, 0, 0, 0], 6, [0, 2, 3, 5, 8, 9] + [0] * 5
+    pools = _pools(dev, 5, 2, page, 8, "float16", 2)
+    want = [p.clone() for p in pools]
+    free, cursor, s = _i32([0, 1, 2, 3, 4], dev), _i32([4], dev), _i32(shares, dev)
+    got = paged_compact(_i32(table, dev), _i32(kv, dev), _i32(new, dev), _i32(nk, dev), page, keep=_i32(keep, dev), pools=pools,
+                        free_blocks=free, cursor=cursor, shares=s)
+    code, det = _lib.device_status(dev.index)
+    assert (code, det) == (_lib.DK_ERR_DEVICE_CHECK, 0x647), (code, hex(det))
+    assert got.lens.tolist() == kv and got.cursor.tolist() == [4] and free.tolist() == list(range(5)) and s.tolist() == shares
+    for a, b in zip(pools, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_shared_pages_before_the_first_moved_token(dev):
+    """They stay as they are, are read from and given up; once the other sequence is freed, tokens move in them, too."""
+    import torch
+
+    from detkernels_b200 import _lib
+    from detkernels_b200.kernels.paging import paged_compact
+    page = 4
+    pools = _pools(dev, 6, 2, page, 8, "float16", 2)
+    want = [p.clone() for p in pools]
+    free, s = _i32([0] * 6, dev), _i32([1, 0, 0, 1, 0, 0], dev)
+    t, kv = _i32([[0, 1, 3], [0, 2, 3]], dev), _i32([0, 0], dev)
+    # sequence 1 keeps its first five tokens and the two behind them in block 3, which it gives up
+    keep = _i32([list(range(12)), [0, 1, 2, 3, 4, 8, 10] + [0] * 5], dev)
+    a = paged_compact(t, kv, _i32([12, 12], dev), _i32([12, 7], dev), page, keep=keep, pools=pools, free_blocks=free,
+                      cursor=_i32([5], dev), shares=s)
+    assert _lib.device_status(dev.index)[0] == _lib.DK_OK
+    assert a.lens.tolist() == [12, 7] and a.cursor.tolist() == [5] and s.tolist() == [1, 0, 0, 0, 0, 0]
+    for p in want:
+        p[2, :, 1:3] = p[3, :, 0:3:2]
+    for x, y in zip(pools, want):
+        assert torch.equal(x, y)
+    b = paged_compact(t, kv, _i32([12, 0], dev), _i32([0, 0], dev), page, free_blocks=free, cursor=a.cursor, shares=s)
+    assert b.cursor.tolist() == [3] and free.tolist()[3:5] == [1, 3] and not s.any()
+    c = paged_compact(t, kv, _i32([0, 7], dev), _i32([0, 2], dev), page, keep=_i32([[0, 0], [1, 6]], dev), pools=pools,
+                      free_blocks=free, cursor=b.cursor, shares=s)
+    assert _lib.device_status(dev.index)[0] == _lib.DK_OK
+    assert c.lens.tolist() == [0, 2] and c.cursor.tolist() == [2] and free.tolist()[2:5] == [2, 1, 3]
+    for p in want:
+        p[0, :, 0], p[0, :, 1] = p[0, :, 1].clone(), p[2, :, 2]
+    for x, y in zip(pools, want):
+        assert torch.equal(x, y)
