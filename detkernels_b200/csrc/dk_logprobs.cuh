@@ -413,8 +413,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, TOPK>::CTAS) logprobs_kernel(
         now.t = f * fmaf(d, now.s, now.t);
         now.s = f * now.s;
         // An excluded logit (-infinity, or as far away) has weight 0 and must not meet its infinite distance, and a product may
-        // be beyond f32: once more, differences first, with distances that end where weights have long been 0.
-        if (!(fabsf(now.t) < INFINITY) || (left < SEG && now.m <= Raw<T>::kFloor && now.m != -INFINITY)) {
+        // be beyond f32: once more, differences first, with distances that end where weights have long been 0.  So, too, where
+        // c is off by much (logits from 7e8 on: c's last place is 128 there): from 126 on the maximum's own weight 2^-d would
+        // be 0, and the sums' roundings count d times in T.
+        if (!(fabsf(now.t) < INFINITY) || fabsf(d) > 32.0f || (left < SEG && now.m <= Raw<T>::kFloor && now.m != -INFINITY)) {
           s2[0] = s2[1] = t2[0] = t2[1] = make_float2(0.0f, 0.0f);
 #pragma unroll 1
           for (int i = 0; i < ITERS; ++i) {

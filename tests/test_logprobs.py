@@ -297,3 +297,32 @@ def test_the_pick_is_the_matmuls(dev):
     matmul_fused(a, w, epilogue="argmax", argmax_keys=keys, out=logits)
     tok = argmax_finish(keys, torch.empty(13, dtype=torch.int64, device=dev))
     assert torch.equal(token_logprobs(logits, top_k=1).top_ids[:, 0], tok)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("V", [40, 700, 40000])
+def test_maxima_of_any_size(dev, dt, sign, V):
+    """A row a maximum, from 2^20 on: neighbours of the type, so that every rounding of their products with log2 e occurs
+    (next to 1.5e9 that of a product is off by up to 128, which is a weight of 2^-128)."""
+    import torch
+
+    from detkernels_b200.kernels.logprobs import token_logprobs
+    first = [2.0 ** e for e in range(20, 40)] + [1.4885e9, 1.48853e9, 1.4886e9, 2.9e9]
+    at = torch.tensor(first, device=dev).to(_dt(dt))
+    ints = at.view(torch.int16 if dt == "bf16" else torch.int32)
+    m = torch.cat([(ints + i).view(_dt(dt)) for i in range(24)]).float() * sign
+    g = torch.Generator(device=dev).manual_seed(V)
+    # the maximum, its neighbours below, and logits far away
+    x = torch.where(m[:, None] > 0, 0.0, m[:, None] * 2).expand(-1, V).clone()
+    near = torch.rand(len(m), V, device=dev, generator=g) < 0.3
+    step = 2.0 ** (-8 if dt == "bf16" else -23)
+    below = m[:, None] * (1 - sign * step * torch.randint(0, 3, x.shape, device=dev, generator=g))
+    x = torch.where(near, below, x)
+    x[:, V // 3] = m
+    x = x.to(_dt(dt))
+    tok = torch.full((len(m),), V // 3, device=dev)
+    _check(x, tok, 5, token_logprobs(x, tok, top_k=5))
+    y = x[:, V // 3:V // 3 + 1].expand(-1, V).contiguous()      # nothing but the maximum
+    _check(y, tok, 5, token_logprobs(y, tok, top_k=5))
