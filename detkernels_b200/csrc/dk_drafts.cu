@@ -156,6 +156,14 @@ int check_ws(const void* ws, size_t given, size_t need, const char* what) {
   return DK_OK;
 }
 
+// A call of nothing leaves the cursor as it is, in its output too.
+int keep_cursor(const int32_t* cursor, int32_t* cursor_out, const char* what, cudaStream_t st) {
+  if (!cursor || !cursor_out || cursor == cursor_out) return DK_OK;
+  cudaError_t e = cudaMemcpyAsync(cursor_out, cursor, sizeof(int32_t), cudaMemcpyDeviceToDevice, st);
+  if (e != cudaSuccess) return fail(DK_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  return DK_OK;
+}
+
 size_t fork_ws_bytes(int64_t rows) { return static_cast<size_t>(dk::pages::kWsMark + 2 * rows) * sizeof(int32_t); }
 size_t compact_ws_bytes() { return static_cast<size_t>(dk::pages::kWsMark) * sizeof(int32_t); }
 
@@ -241,7 +249,7 @@ int dk_paged_fork(int32_t* block_table, int64_t block_table_stride, int32_t tabl
                 element_size};
   rc = check_pools(c, page_size, what);
   if (rc) return rc;
-  if (n_forks == 0) return DK_OK;
+  if (n_forks == 0) return keep_cursor(cursor, cursor_out, what, static_cast<cudaStream_t>(stream));
   if (!kv_lens || !src || !dst || !cursor || !cursor_out || (n_free > 0 && !free_blocks))
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   rc = check_ws(workspace, workspace_bytes, fork_ws_bytes(table_rows), what);
@@ -305,7 +313,7 @@ int dk_paged_compact(const int32_t* block_table, int64_t block_table_stride, int
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: a free list needs its cursor", what);
   if (shares && static_cast<int64_t>(n_seqs) * blocks_per_seq >= 1LL << 30)
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: 2^30 table entries or more with shares", what);
-  if (n_seqs == 0) return DK_OK;
+  if (n_seqs == 0) return free_blocks ? keep_cursor(cursor, cursor_out, what, static_cast<cudaStream_t>(stream)) : DK_OK;
   if (!kv_lens || !new_lens || !n_keep || !lens_out || lens_out == kv_lens || lens_out == new_lens || lens_out == n_keep)
     return fail(DK_ERR_INVALID_ARGUMENT, "%s: null pointer, or lens_out is one of the inputs", what);
   rc = check_ws(workspace, workspace_bytes, compact_ws_bytes(), what);

@@ -599,3 +599,24 @@ def test_shared_pages_before_the_first_moved_token(dev):
         p[0, :, 0], p[0, :, 1] = p[0, :, 1].clone(), p[2, :, 2]
     for x, y in zip(pools, want):
         assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_calls_of_nothing_hand_the_cursor_on(dev):
+    """Through the C entries, whose callers chain the cursors themselves."""
+    import torch
+
+    from detkernels_b200 import _lib
+    lib = _lib.load()
+    books, cursor, out = _i32(np.zeros(8), dev), _i32([5], dev), _i32([-1, -1], dev)
+    at, st = books.data_ptr(), _lib.stream_ptr(dev)
+    assert lib.dk_paged_fork(at, 2, 4, 2, at, None, None, 0, 8, at, 8, cursor.data_ptr(), out.data_ptr(), None, 9, None, 0,
+                             0, 0, 0, 0, 0, 2, None, 0, st) == _lib.DK_OK
+
+    def compact(free, to):
+        return lib.dk_paged_compact(at, 2, 2, None, None, None, None, 0, 0, 0, 8, None, free, 8, cursor.data_ptr(), to, None, 9,
+                                    None, 0, 0, 0, 0, 0, 0, 2, None, 0, st)
+    assert compact(at, out[1:].data_ptr()) == _lib.DK_OK and out.tolist() == [5, 5]
+    assert compact(at, cursor.data_ptr()) == _lib.DK_OK and cursor.tolist() == [5]
+    assert compact(None, None) == _lib.DK_OK      # without a free list there is no cursor
+    torch.cuda.synchronize(dev)
