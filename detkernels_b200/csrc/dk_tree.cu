@@ -74,9 +74,11 @@ int tree_launch(const dk::tree::Maps& maps, dk::tree::Params p, cudaStream_t st)
     cudaFuncAttributes a{};
     cudaError_t e = cudaFuncGetAttributes(&a, fn);
     if (e != cudaSuccess) return fail(DK_ERR_CUDA, "attention_tree: %s", cudaGetErrorString(e));
-    if (a.numRegs != dk::prefix::kLaunchRegs)   // the register split of the kernel is exact for this count
-      return fail(DK_ERR_UNSUPPORTED, "attention_tree: built with %d registers a thread, not %d", a.numRegs,
-                  dk::prefix::kLaunchRegs);
+    // The register split of the kernel is exact for this count, and for a kernel without calls or spills: a build that kept
+    // functions out of line had the same count, did not hold its warps to their shares, and failed at launch.
+    if (a.numRegs != dk::prefix::kLaunchRegs || a.localSizeBytes != 0)
+      return fail(DK_ERR_UNSUPPORTED, "attention_tree: built with %d registers a thread, not %d, and %d bytes of local memory",
+                  a.numRegs, dk::prefix::kLaunchRegs, static_cast<int>(a.localSizeBytes));
     if (dev >= 0 && dev < kMaxDevices) regs[dev] = a.numRegs;
   }
   // As many CTAs as SMs share the items, or, where even their bound is not more than that, each takes one at once.
