@@ -286,7 +286,9 @@ _no_guard = contextlib.nullcontext()
 def on_device(device):
     """``torch.cuda.device(device)`` for a tensor's device, which costs nothing when it is the current one."""
     import torch
-    return _no_guard if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+    # (asked for directly once CUDA is set up; before, the public function does that, or says why it cannot)
+    current = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else torch.cuda.current_device()
+    return _no_guard if current == device.index else torch.cuda.device(device)
 
 
 _workspaces = {}

@@ -93,3 +93,25 @@ def test_ops_refuse_cpu_tensors():
         matmul_batch_invariant(torch.randn(2, 8), torch.randn(8, 4))
     with pytest.raises(AssertionError):
         attention_batch_invariant(torch.randn(1, 2, 8), torch.randn(1, 2, 4, 8), torch.randn(1, 2, 4, 8))
+
+
+def test_the_current_device_is_asked_for_through_the_public_function_before_cuda_is_set_up(monkeypatch):
+    """``on_device`` of a process without CUDA, or forked from one with it, fails as torch says it."""
+    import torch
+
+    from detkernels_b200 import _lib
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: pytest.fail("CUDA is not set up"))
+    assert _lib.on_device(torch.device("cuda", 3)) is _lib._no_guard
+    assert isinstance(_lib.on_device(torch.device("cuda", 1)), torch.cuda.device)
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1)
+    assert _lib.on_device(torch.device("cuda", 1)) is _lib._no_guard
+
+    def no_cuda():
+        raise RuntimeError("Cannot re-initialize CUDA in forked subprocess")
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_device", no_cuda)
+    with pytest.raises(RuntimeError, match="forked"):
+        _lib.on_device(torch.device("cuda", 1))
