@@ -326,3 +326,33 @@ def test_maxima_of_any_size(dev, dt, sign, V):
     _check(x, tok, 5, token_logprobs(x, tok, top_k=5))
     y = x[:, V // 3:V // 3 + 1].expand(-1, V).contiguous()      # nothing but the maximum
     _check(y, tok, 5, token_logprobs(y, tok, top_k=5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("R", [3, 200])
+@pytest.mark.parametrize("passes", [(0,), (1,), (0, 1, 3), (2, 3)])
+def test_fewer_threads_than_alternatives_hold_the_largest(dev, dt, R, passes):
+    """All logits of 31 threads of a warp above all others, with 32 alternatives: the most that a bound from the threads'
+    maxima lets through, alone, behind alternatives of an earlier pass, and pass after pass ever larger ones.  Few rows
+    are split, many are not."""
+    import torch
+
+    from detkernels_b200.kernels.logprobs import token_logprobs
+    t = _dt(dt)
+    vec = 16 // torch.empty(0, dtype=t).element_size()   # logits a thread takes side by side; a warp 128 times as many a pass
+    span = 8 * 128 * vec                                 # a pass
+    V = 4 * span + 77
+    g = torch.Generator(device=dev).manual_seed(R)
+    x = torch.randn(R, V, device=dev, generator=g).to(t)
+    at = torch.arange(span, device=dev) // vec
+    bits = torch.int32 if dt == "f32" else torch.int16
+    for n, j in enumerate(passes):
+        for warp in (0, 5) if R == 3 else (5,):
+            hot = j * span + torch.nonzero((at // 128 == warp) & (at % 32 < 31))[:, 0]
+            # neighbours of the type from 8 (and then 2048) on, in any order: no two alike
+            base = torch.tensor(8.0 if n == 0 else 2048.0, device=dev).to(t).view(bits)
+            order = torch.randperm(len(hot), device=dev, generator=g)
+            x[:, hot] = (base + order.to(bits)).view(t) if n < 2 else x[:, hot] + 100
+    tok = torch.randint(0, V, (R,), device=dev, generator=g)
+    _check(x, tok, 32, token_logprobs(x, tok, top_k=32))
