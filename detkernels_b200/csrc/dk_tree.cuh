@@ -163,10 +163,9 @@ __device__ __forceinline__ Seq seq_at(const Params& p, int b, bool report) {
 // The items of a sequence: units (KV heads, or pairs of them where the rows fit a tile), of each its chunks, of each the
 // pairs of tiles, which so find the chunk's keys in L2; and their cost, in blocks.
 struct Cost {
-  int units, pairs;      // pairs: of tiles a KV head (solo: its tiles); 0: pairs of heads (solo: heads)
-  int inner;             // items a (unit, chunk)
+  int units;
+  int inner;             // items a (unit, chunk): pairs of tiles (solo: tiles), or one where the rows fit a tile
   int chunk, last;       // cost of an item of a whole chunk, of the last one
-  int64_t unit;          // of a unit
 };
 // What an item costs beside its blocks (states out, the first scores), in blocks.
 template <int D>
@@ -177,12 +176,10 @@ __device__ __forceinline__ Cost cost_of(const Params& p, const Seq& s) {
   constexpr int BLK = Cfg<D>::BLK;
   Cost c;
   const int nt = (s.rows + p.rpt - 1) / p.rpt;
-  c.pairs = nt > 1 ? (p.solo ? nt : (nt + 1) >> 1) : 0;
   c.units = nt > 1 || (nt == 1 && p.solo) ? p.hkv : nt == 1 ? (p.hkv + 1) >> 1 : 0;
-  c.inner = nt > 1 ? c.pairs : 1;
+  c.inner = nt <= 1 ? 1 : p.solo ? nt : (nt + 1) >> 1;
   c.chunk = s.chunk / BLK + kItemCost<D>;
   c.last = (s.total - (s.n_chunks - 1) * s.chunk + BLK - 1) / BLK + kItemCost<D>;
-  c.unit = static_cast<int64_t>(c.inner) * (static_cast<int64_t>(max(s.n_chunks - 1, 0)) * c.chunk + c.last);
   return c;
 }
 
@@ -337,7 +334,7 @@ struct Walk {
       l_b = static_cast<int>(r - l_chunk * static_cast<uint32_t>(p.n_seqs));
       const Seq q = seq_at<D, false>(p, l_b, lane == 0 && u == 0 && l_chunk == 0);
       const Cost c = cost_of<D>(p, q);
-      l_u = c.inner ? u / c.inner : 0;
+      l_u = u / c.inner;
       l_pair = u - l_u * c.inner;
       l_row0 = q.row0;
       l_rows = q.rows;
