@@ -7,7 +7,8 @@
 //   fork      row dst becomes a copy of row src: whole pages are shared (shares[x] += 1) and the open page gets a
 //             block of its own, or every page does when there are no shares; the tokens of new blocks are copied.
 //   compact   token kv + keep[j] becomes token kv + j, the rest behind kv is dropped; the pages that hold nothing any
-//             more lose a holder, and those without one go back to the list in (sequence, page) order.
+//             more lose a holder, and those without one go back to the list in (sequence, page) order.  No token goes
+//             to a page with further holders.
 //
 // Either is one kernel that checks everything, and only then changes the tables (fork_kernel, release_kernel), and
 // one that moves tokens in all layers' pools (move_kernel).  The first is bound by the latency of a few dependent
@@ -16,8 +17,9 @@
 // scratch has to be cleared.  The second is bound by the bytes it copies.
 //
 // Measured, both kernels, in a graph: 28 forks of 7 prompts that share their pages, 16 heads of 64 in 8 pools, 14.6 us
-// (about 9 of them the first kernel); 24 copied whole, 1.2 GB, 199 us (6.1 TB/s); 256 accepted trees compacted, pages
-// shared, 17.8 us; 8 caches of up to 16,000 tokens halved, 1.5 GB, 276 us (5.5 TB/s, half of the 256-byte rows skipped).
+// (about 9 of them the first kernel); 24 copied whole, 1.2 GB, 200 us (6.1 TB/s); 256 accepted trees compacted, pages
+// shared, 18.2 us (0.4 of them for the blocks and holders of moved tokens), 256 sequences freed 10.2; 8 caches of up
+// to 16,000 tokens halved, 1.5 GB, 277 us (5.5 TB/s, half of the 256-byte rows skipped).
 #pragma once
 
 #include "dk_common.cuh"
